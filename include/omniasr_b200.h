@@ -34,6 +34,7 @@ extern "C" {
 
 #define OMNIASR_BF16 0
 #define OMNIASR_F32 1
+#define OMNIASR_FP8 2 /* a paged cache's element type: e4m3 codes with one scale byte per vector */
 
 #define OMNIASR_OK 0
 #define OMNIASR_ERR_ARGUMENT 1    /* a shape, stride, pointer alignment or size is invalid */
@@ -255,6 +256,57 @@ size_t omniasr_noalloc_scratch_bytes(void);
  * (cudaMemsetAsync on the array itself; nothing is allocated). Needed only after a no-alloc call raised status
  * bit 2. No counterpart in the reference. */
 int omniasr_noalloc_reset(cudaStream_t stream);
+
+/* ---- Paged cache (no counterpart in the reference, whose caches are [rows, heads, len, dim] and whose heads are not
+ * grouped). K and V live in pages [pages, kv_heads, page, dim] (strides stride_page, stride_head, stride_pos in elements,
+ * shared by K and V, 16-byte aligned); a sequence's position j is offset j % page of the page its int32 table row names
+ * at j / page. cache_type is the dtype itself, or OMNIASR_FP8: each vector x (one position of one kv head) is held as
+ * e4m3 codes of x * 2^-e, e = the smallest integer with max|x| <= 448 * 2^e held to [-40, 40], and the byte e + 127 in
+ * k_scale / v_scale [pages, kv_heads, page] (contiguous; NULL for the other types). Infinities, NaN and values past
+ * 448 * 2^40 are held as NaN and do not count for the scale. heads must be a multiple of kv_heads; query head h reads kv
+ * head h / (heads / kv_heads). A page number outside the pool (or a length past the table) raises status bit 1, the
+ * row's result is then unspecified, and nothing outside the tensors is touched. */
+
+/* RoPE of q and k as omniasr_rope_kv() computes it, k and v written into the pages: qkv [n, (heads + 2 * kv_heads) *
+ * dim] (q | k | v), token n's k and v at slot slots[n] = page number * page + offset (negative: not written), rotated q
+ * to q_out [n, heads, dim]. Two tokens of one call must not share a slot. */
+int omniasr_paged_rope_kv(const void* qkv, int64_t qkv_stride, const float* cs, int64_t cs_positions, const int64_t* pos,
+                          const int64_t* slots, void* q_out, void* k_pages, void* v_pages, void* k_scale, void* v_scale,
+                          int64_t pages, int page, int64_t stride_page, int64_t stride_head, int64_t stride_pos, int n,
+                          int heads, int kv_heads, int dim, int dtype, int cache_type, int* status, cudaStream_t stream);
+
+/* Reads pages back: rows offsets[i] .. offsets[i + 1] - 1 of k_out / v_out [tokens, kv_heads, dim] (contiguous, dtype)
+ * get the first offsets[i + 1] - offsets[i] positions of table row i, for i < rows (offsets ascending, rows + 1 of
+ * them). Output rows outside every range are zeros. */
+int omniasr_paged_kv_read(const void* k_pages, const void* v_pages, const void* k_scale, const void* v_scale, int64_t pages,
+                          int page, int64_t stride_page, int64_t stride_head, int64_t stride_pos, const int32_t* table,
+                          int64_t table_stride, int table_width, int rows, const int64_t* offsets, int64_t tokens,
+                          void* k_out, void* v_out, int kv_heads, int dim, int dtype, int cache_type, int* status,
+                          cudaStream_t stream);
+
+/* Attention of each row's newest tokens over its pages: q [rows * tokens, heads, dim], query i of row b sees positions
+ * [0, lengths[b] + i) (as omniasr_draft_attention; tokens = 1: a decode step). out like q; a query that sees nothing
+ * gets zeros. rows <= 65535, tokens * heads <= 65535. The workspace (omniasr_paged_attention_workspace() bytes) starts
+ * with OMNIASR_ATTENTION_COUNTER_BYTES of counters under the rule of omniasr_attention_workspace(). */
+size_t omniasr_paged_attention_workspace(int dtype, int cache_type, int rows, int tokens, int heads, int kv_heads, int dim,
+                                         int page, int table_width);
+int omniasr_paged_attention(const void* q, const void* k_pages, const void* v_pages, const void* k_scale, const void* v_scale,
+                            int64_t pages, int page, int64_t stride_page, int64_t stride_head, int64_t stride_pos,
+                            const int32_t* table, int64_t table_stride, int table_width, const int64_t* lengths, void* out,
+                            int rows, int tokens, int heads, int kv_heads, int dim, float scale, int dtype, int cache_type,
+                            void* workspace, size_t workspace_bytes, int* status, cudaStream_t stream);
+
+/* Causal attention of packed sequences with grouped heads: sequence s has queries q_offsets[s] .. q_offsets[s + 1] - 1 of
+ * q [q_tokens, heads, dim] and keys k_offsets[s] .. k_offsets[s + 1] - 1 of k / v [k_tokens, kv_heads, dim] (token and
+ * head strides in elements); its last query sees its last key, so query i of lq sees i + 1 + lk - lq keys (none where
+ * that is not positive: zeros). out [q_tokens, heads, dim] contiguous; rows of no sequence are not written. Offsets are
+ * int64, ascending, on the device. The workspace begins with counters under the rule of omniasr_attention_workspace(). */
+#define OMNIASR_PACKED_WORKSPACE_BYTES 256
+int omniasr_packed_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k, int64_t k_stride_tok,
+                             int64_t k_stride_head, const void* v, int64_t v_stride_tok, int64_t v_stride_head, void* out,
+                             const int64_t* q_offsets, const int64_t* k_offsets, int64_t q_tokens, int64_t k_tokens, int seqs,
+                             int heads, int kv_heads, int dim, float scale, int dtype, void* workspace, size_t workspace_bytes,
+                             int* status, cudaStream_t stream);
 
 /* Self-test of the bounded device wait every kernel here uses (no counterpart in the reference): one kernel waits
  * on an mbarrier that nothing completes, gives up after limit_ns (0 < limit_ns <= 1e8), ORs the timeout bit (2)

@@ -1,0 +1,252 @@
+// Causal attention of packed sequences with grouped heads: entry, and the CUDA-core kernel for what the tensor-core
+// kernels (prefill.cu, prefill_wide.cu) do not take (fp32, head dims other than 128 and 512).
+//
+// Sequence s has queries q_offsets[s] .. q_offsets[s+1] - 1 and keys k_offsets[s] .. k_offsets[s+1] - 1; its last query
+// sees its last key (a chunk of a prompt attends to the keys before it), so query i sees i + 1 + lk - lq keys, none
+// where that is not positive. q [Tq, H, D], k and v [Tk, Hkv, D], head h reads kv head h / (H / Hkv).
+//
+// One CTA: BM queries of one head; K and V tiles of BN keys go through shared memory as fp32; S = Q K^T and O += P V
+// in registers (256 threads as 16 x 16: thread (y, x) holds rows y + 16 i and keys / dims x + 16 j, so a row's softmax
+// statistics are a shuffle over half a warp). FMA-bound; fp32 throughout, as an fp32 model needs.
+
+#include <math.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "attention.cuh"
+#include "common.cuh"
+#include "paged.cuh"
+
+namespace omni {
+namespace packed {
+
+constexpr int kThreads = 256;
+
+template <int D>
+struct Shape {
+  static constexpr int BM = D <= 128 ? 64 : 32;
+  static constexpr int BN = D <= 128 ? 64 : 32;
+  static constexpr int LD = D + 4;  // row stride in shared memory (floats): 16-byte aligned, rows on different banks
+  static constexpr int LP = BN + 4;
+  static constexpr int BYTES = (BM * LD + 2 * BN * LD + BM * LP) * 4;
+};
+
+// Tile `slot` of the packed queries -> sequence and first query: the sequences' tile counts, summed 32 at a time by one
+// warp. Returns the sequence, or -1 past the last tile.
+OMNI_DEV int find_tile(const int64_t* offsets, int seqs, int bm, int slot, int lane, int* tile) {
+  int before = 0;
+  for (int s0 = 0; s0 < seqs; s0 += 32) {
+    const int s = s0 + lane;
+    const int64_t n = s < seqs ? offsets[s + 1] - offsets[s] : 0;
+    const int mine = n > 0 ? (int)((n + bm - 1) / bm) : 0;
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, slot < before + incl);
+    if (hit) {
+      const int w = __ffs(hit) - 1;
+      *tile = slot - before - __shfl_sync(0xffffffffu, incl - mine, w);
+      return s0 + w;
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return -1;
+}
+
+template <typename T>
+OMNI_DEV void load4(const T* p, float* f);
+template <>
+OMNI_DEV void load4<float>(const float* p, float* f) {
+  const float4 v = __ldg(reinterpret_cast<const float4*>(p));
+  f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
+}
+template <>
+OMNI_DEV void load4<__nv_bfloat16>(const __nv_bfloat16* p, float* f) {
+  const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+  f[0] = __uint_as_float(v.x << 16), f[1] = __uint_as_float(v.x & 0xffff0000u);
+  f[2] = __uint_as_float(v.y << 16), f[3] = __uint_as_float(v.y & 0xffff0000u);
+}
+
+// `rows` rows of 4-element groups from global (row stride st) into shared memory; rows at or past `valid` are zeros.
+template <typename T, int D, int LD>
+OMNI_DEV void load_tile(float* dst, const T* src, int64_t st, int rows, int valid) {
+  for (int i = threadIdx.x; i < rows * (D / 4); i += kThreads) {
+    const int r = i / (D / 4), c = (i - r * (D / 4)) * 4;
+    float f[4] = {0.f, 0.f, 0.f, 0.f};
+    if (r < valid) load4(src + (int64_t)r * st + c, f);
+    *reinterpret_cast<float4*>(dst + r * LD + c) = make_float4(f[0], f[1], f[2], f[3]);
+  }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) packed_kernel(const PackedArgs a) {
+  using S = Shape<D>;
+  constexpr int BM = S::BM, BN = S::BN, LD = S::LD, LP = S::LP;
+  constexpr int MR = BM / 16, NR = BN / 16, DR = D / 16;
+  extern __shared__ __align__(16) float sm[];
+  float* qs = sm;
+  float* ks = qs + BM * LD;
+  float* vs = ks + BN * LD;
+  float* ps = vs + BN * LD;
+  __shared__ int s_seq, s_tile;
+  grid_launch_dependents();
+  grid_dependency_wait();
+  if (threadIdx.x < 32) {
+    int tile = 0;
+    const int seq = find_tile(a.q_offsets, a.seqs, BM, blockIdx.x, threadIdx.x, &tile);
+    if (threadIdx.x == 0) {
+      s_seq = seq;
+      s_tile = tile;
+    }
+  }
+  __syncthreads();
+  if (s_seq < 0) return;
+  const int h = blockIdx.y, kvh = h / (a.heads / a.kv_heads);
+  const int64_t qa = a.q_offsets[s_seq], qb = a.q_offsets[s_seq + 1];
+  const int64_t ka = a.k_offsets[s_seq], kb = a.k_offsets[s_seq + 1];
+  if (qa < 0 || qb > a.q_tokens || ka < 0 || kb > a.k_tokens || kb < ka) {
+    if (threadIdx.x == 0) raise_status(a.status, kStatusIndex);
+    return;
+  }
+  const int64_t q0 = qa + (int64_t)s_tile * BM;
+  const int rows = (int)min((int64_t)BM, qb - q0);
+  // Row r of the tile sees keys [0, lim0 + r) of the sequence.
+  const int64_t lim0 = (q0 - qa) + 1 + (kb - ka) - (qb - qa);
+  const int64_t keys = max((int64_t)0, lim0 + rows - 1);
+  const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
+  load_tile<T, D, LD>(qs, reinterpret_cast<const T*>(a.q) + q0 * a.q_st + (int64_t)h * a.q_sh, a.q_st, BM, rows);
+  const T* kg = reinterpret_cast<const T*>(a.k) + ka * a.k_st + (int64_t)kvh * a.k_sh;
+  const T* vg = reinterpret_cast<const T*>(a.v) + ka * a.v_st + (int64_t)kvh * a.v_sh;
+  const float qscale = a.scale * kLog2e;
+  float m[MR], l[MR], o[MR][DR];
+#pragma unroll
+  for (int i = 0; i < MR; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DR; ++d) o[i][d] = 0.f;
+  }
+  for (int64_t j0 = 0; j0 < keys; j0 += BN) {
+    const int valid = (int)min((int64_t)BN, keys - j0);
+    __syncthreads();  // the tile before is used up
+    load_tile<T, D, LD>(ks, kg + j0 * a.k_st, a.k_st, BN, valid);
+    load_tile<T, D, LD>(vs, vg + j0 * a.v_st, a.v_st, BN, valid);
+    __syncthreads();
+    float s[MR][NR];
+#pragma unroll
+    for (int i = 0; i < MR; ++i)
+#pragma unroll
+      for (int j = 0; j < NR; ++j) s[i][j] = 0.f;
+#pragma unroll 4
+    for (int d = 0; d < D; d += 4) {
+      float4 qv[MR], kv[NR];
+#pragma unroll
+      for (int i = 0; i < MR; ++i) qv[i] = *reinterpret_cast<const float4*>(qs + (y + 16 * i) * LD + d);
+#pragma unroll
+      for (int j = 0; j < NR; ++j) kv[j] = *reinterpret_cast<const float4*>(ks + (x + 16 * j) * LD + d);
+#pragma unroll
+      for (int i = 0; i < MR; ++i)
+#pragma unroll
+        for (int j = 0; j < NR; ++j)
+          s[i][j] = fmaf(qv[i].w, kv[j].w, fmaf(qv[i].z, kv[j].z, fmaf(qv[i].y, kv[j].y, fmaf(qv[i].x, kv[j].x, s[i][j]))));
+    }
+    const bool edge = j0 + BN > lim0;  // some row does not see all of the tile
+#pragma unroll
+    for (int i = 0; i < MR; ++i) {
+      const int64_t lim = lim0 + y + 16 * i - j0;
+      float top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < NR; ++j) {
+        s[i][j] = x + 16 * j < lim ? s[i][j] * qscale : -INFINITY;
+        top = fmaxf(top, s[i][j]);
+      }
+#pragma unroll
+      for (int w = 8; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+      const float mn = fmaxf(m[i], top);
+      const float base = mn == -INFINITY ? 0.f : mn;
+      const float f = ex2(m[i] - base);
+      m[i] = mn;
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < NR; ++j) {
+        const float p = ex2(s[i][j] - base);  // a NaN score gives NaN: the row is NaN, as the formula is
+        sum += p;
+        ps[(y + 16 * i) * LP + x + 16 * j] = p;
+      }
+      l[i] = fmaf(l[i], f, sum);
+#pragma unroll
+      for (int d = 0; d < DR; ++d) o[i][d] *= f;
+    }
+    __syncwarp();  // a row's probabilities are written and read by the same half-warp
+    auto values = [&](auto masked) {
+#pragma unroll 2
+      for (int k = 0; k < valid; ++k) {
+        float p[MR];
+#pragma unroll
+        for (int i = 0; i < MR; ++i) p[i] = ps[(y + 16 * i) * LP + k];
+#pragma unroll
+        for (int d = 0; d < DR; ++d) {
+          const float v = vs[k * LD + x + 16 * d];
+#pragma unroll
+          for (int i = 0; i < MR; ++i) {
+            // A key past the row's does not enter, whatever its value holds.
+            if (!decltype(masked)::value || j0 + k < lim0 + y + 16 * i) o[i][d] = fmaf(p[i], v, o[i][d]);
+          }
+        }
+      }
+    };
+    if (edge) values(std::true_type{});
+    else values(std::false_type{});
+  }
+#pragma unroll
+  for (int i = 0; i < MR; ++i) {
+#pragma unroll
+    for (int w = 8; w > 0; w >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], w);
+    const int r = y + 16 * i;
+    if (r < rows) {
+      const float inv = l[i] != 0.f ? 1.f / l[i] : 0.f;
+      T* dst = reinterpret_cast<T*>(a.out) + ((q0 + r) * a.heads + h) * D;
+#pragma unroll
+      for (int d = 0; d < DR; ++d) dst[x + 16 * d] = Elem<T>::from_float(o[i][d] * inv);
+    }
+  }
+}
+
+template <typename T, int D>
+cudaError_t launch_t(const PackedArgs& a, cudaStream_t s) {
+  using S = Shape<D>;
+  static bool configured = false;
+  if (!configured) {
+    cudaError_t e = cudaFuncSetAttribute(packed_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES);
+    if (e != cudaSuccess) return e;
+    configured = true;
+  }
+  // At most this many tiles: a sequence's last tile may be partly filled.
+  const int64_t tiles = a.q_tokens / S::BM + a.seqs;
+  return launch_dependent(packed_kernel<T, D>, dim3((unsigned)tiles, (unsigned)a.heads), dim3(kThreads), (size_t)S::BYTES, s, a);
+}
+
+template <typename T>
+cudaError_t launch_dim(const PackedArgs& a, cudaStream_t s) {
+  switch (a.dim) {
+    case 16: return launch_t<T, 16>(a, s);
+    case 32: return launch_t<T, 32>(a, s);
+    case 64: return launch_t<T, 64>(a, s);
+    case 128: return launch_t<T, 128>(a, s);
+    case 256: return launch_t<T, 256>(a, s);
+    case 512: return launch_t<T, 512>(a, s);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+}  // namespace packed
+
+cudaError_t launch_packed(int dtype, const PackedArgs& a, cudaStream_t stream) {
+  return dtype == kBF16 ? packed::launch_dim<__nv_bfloat16>(a, stream) : packed::launch_dim<float>(a, stream);
+}
+
+}  // namespace omni

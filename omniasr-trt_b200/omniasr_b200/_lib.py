@@ -12,7 +12,7 @@ from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent.parent / "lib" / "libomniasr_b200.so"
 
-BF16, F32 = 0, 1
+BF16, F32, FP8 = 0, 1, 2
 OK, ERR_ARGUMENT, ERR_UNSUPPORTED, ERR_WORKSPACE, ERR_CUDA, ERR_DEVICE = range(6)
 DECODE, DRAFT, BEAM = 0, 1, 2
 
@@ -55,6 +55,15 @@ SIGNATURES = {
     "omniasr_decode_gemm_rope": (_i, [_p, _i64, _i, _p, _i64, _i, _p, _i64, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64,
                                       _i64, _i64, _i, _i, _p, _sz, _p, _p]),
     "omniasr_accept": (_i, [_p, _p, _p, _i64, _i64, _p, _p, _p, _p, _p, _p, _i, _i, _i64, _i64, _p, _p]),
+    "omniasr_paged_rope_kv": (_i, [_p, _i64, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _i, _i64, _i64, _i64, _i, _i, _i,
+                                   _i, _i, _i, _p, _p]),
+    "omniasr_paged_kv_read": (_i, [_p, _p, _p, _p, _i64, _i, _i64, _i64, _i64, _p, _i64, _i, _i, _p, _i64, _p, _p, _i, _i,
+                                   _i, _i, _p, _p]),
+    "omniasr_paged_attention_workspace": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i, _i]),
+    "omniasr_paged_attention": (_i, [_p, _p, _p, _p, _p, _i64, _i, _i64, _i64, _i64, _p, _i64, _i, _p, _p, _i, _i, _i, _i,
+                                     _i, _f, _i, _i, _p, _sz, _p, _p]),
+    "omniasr_packed_attention": (_i, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _i64, _i, _i, _i,
+                                      _i, _f, _i, _p, _sz, _p, _p]),
     "omniasr_decode_gemm_workspace": (_sz, [_i, _i, _i, _i]),
     "omniasr_decode_gemm": (_i, [_p, _i64, _i, _p, _i64, _i, _i, _i, _p, _i64, _p, _i64, _p, _sz, _p, _p]),
 }

@@ -15,6 +15,12 @@ CUDA-graph capture run on these kernels unchanged:
 * :func:`reorder_gather` -- the beam reorder ``dst[r] = src[parent[r]]``, byte-exact (``llm.py:237-238``,
   ``beam.py:175-176``).
 
+Beside the reference's surface, a cache of pages for serving, with grouped heads and an optional 8-bit form:
+
+* :func:`paged_rope_kv` / :func:`paged_kv_read` -- RoPE and the append into pages, and pages read back as packed rows;
+* :func:`paged_attention` -- each sequence's newest token(s) over its pages;
+* :func:`packed_attention` -- causal attention of packed prompts (or chunks of them) of different lengths.
+
 Each call is a launch (or two) of hand-written CUDA through the C ABI of ``include/omniasr_b200.h`` on the
 current stream; outputs and the beam search's split workspace are allocated with ``torch.empty`` on the caller's
 device (from the graph pool during a capture); decode and draft calls reuse one zeroed workspace per stream, whose
@@ -489,6 +495,159 @@ def reorder_gather(src: torch.Tensor, parent: torch.Tensor, out: torch.Tensor | 
               out.stride(0) * out.element_size(), _ptr(parent), int(parent.dtype == torch.int64), rows, row_bytes,
               _ptr(status_word(src.device)), _stream(src.device))
     return out
+
+
+def _pages(k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None, v_scale: torch.Tensor | None, dtype: int,
+           name: str) -> tuple:
+    """A paged cache's arguments: (k, v, k_scale, v_scale, pages, page, strides), kv heads, head_dim and type code."""
+    if k.dim() != 4 or v.shape != k.shape or v.stride() != k.stride() or k.stride(3) != 1 or v.dtype != k.dtype:
+        raise ValueError(f"{name}: k and v pages must be [pages, kv_heads, page, D] views of one dtype with the same "
+                         "strides and unit stride in D")
+    pages, kv_heads, page, dim = k.shape
+    if k.dtype == torch.float8_e4m3fn:
+        code = _lib.FP8
+        for t in (k_scale, v_scale):
+            if t is None or t.dtype != torch.uint8 or t.shape != (pages, kv_heads, page) or not t.is_contiguous():
+                raise ValueError(f"{name}: float8_e4m3fn pages need contiguous uint8 scales [pages, kv_heads, page]")
+    else:
+        code = _DTYPES.get(k.dtype)
+        if code != dtype:
+            raise ValueError(f"{name}: pages of {k.dtype} (supported: the queries' dtype, float8_e4m3fn)")
+        if k_scale is not None or v_scale is not None:
+            raise ValueError(f"{name}: scales belong to float8_e4m3fn pages")
+    sp, sh, st, _ = k.stride()
+    return ((k.data_ptr(), v.data_ptr(), None if k_scale is None else k_scale.data_ptr(),
+             None if v_scale is None else v_scale.data_ptr()), (pages, page, sp, sh, st), kv_heads, dim, code)
+
+
+def _table(table: torch.Tensor, rows: int, name: str) -> tuple[int, int, int]:
+    if table.dtype != torch.int32 or table.dim() != 2 or table.size(0) < rows or (table.size(1) > 1 and table.stride(1) != 1):
+        raise ValueError(f"{name}: page_table must be int32 [rows, width] with unit inner stride")
+    return table.data_ptr(), table.stride(0), table.size(1)
+
+
+def paged_rope_kv(qkv: torch.Tensor, cs: torch.Tensor, pos: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                  slots: torch.Tensor, heads: int, kv_heads: int, k_scale: torch.Tensor | None = None,
+                  v_scale: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`rope_kv` into pages: ``qkv`` [N, (heads + 2 * kv_heads) * D] (q|k|v), ``cs`` [P, D/2, 2] fp32, ``pos`` [N];
+    token n's rotated k and its v go to slot ``slots[n]`` = page number * page size + offset (negative: not written) of
+    ``k_pages``/``v_pages`` [pages, kv_heads, page, D]; returns the rotated q [N, heads, D]. Pages hold qkv's dtype, or
+    float8_e4m3fn codes with one scale byte per vector in ``k_scale``/``v_scale`` (uint8 [pages, kv_heads, page]): the
+    vector x is held as codes of x * 2^-e and the byte e + 127, e the smallest integer with max|x| <= 448 * 2^e (within
+    [-40, 40])."""
+    dtype = _dtype(qkv, "paged_rope_kv")
+    ptrs, geo, kvh, dim, code = _pages(k_pages, v_pages, k_scale, v_scale, dtype, "paged_rope_kv")
+    n = qkv.size(0)
+    if kvh != kv_heads or qkv.dim() != 2 or qkv.size(1) != (heads + 2 * kv_heads) * dim or (n and qkv.stride(1) != 1):
+        raise ValueError("paged_rope_kv: qkv must be [N, (heads + 2 * kv_heads) * D] with unit inner stride")
+    if pos.numel() != n or slots.numel() != n:
+        raise ValueError("paged_rope_kv: pos and slots must hold one entry per token")
+    if cs.dim() != 3 or cs.size(1) != dim // 2 or cs.size(2) != 2:
+        raise ValueError("paged_rope_kv: cs must be [P, D / 2, 2]")
+    device = qkv.device
+    q = torch.empty(n, heads, dim, device=device, dtype=qkv.dtype)
+    if n == 0:
+        return q
+    cs = cs if cs.dtype == torch.float32 and cs.is_contiguous() else cs.float().contiguous()
+    pos, slots = _index(pos), _index(slots)
+    _lib.call("omniasr_paged_rope_kv", qkv.data_ptr(), qkv.stride(0), cs.data_ptr(), cs.size(0), pos.data_ptr(),
+              slots.data_ptr(), q.data_ptr(), *ptrs, *geo, n, heads, kv_heads, dim, dtype, code,
+              status_word(device).data_ptr(), _stream(device))
+    return q
+
+
+def paged_kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, offsets: torch.Tensor,
+                  tokens: int, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+                  dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Pages read back as packed rows: k and v [tokens, kv_heads, D], rows ``offsets[i]`` .. ``offsets[i + 1] - 1`` holding
+    the first positions of ``page_table`` row i (``offsets`` [rows + 1], ascending, ``tokens`` the last; output rows
+    outside them are zeros). 8-bit pages are read as ``dtype`` (default bfloat16), others as what they hold."""
+    if dtype is None:
+        dtype = torch.bfloat16 if k_pages.dtype == torch.float8_e4m3fn else k_pages.dtype
+    out_code = _DTYPES.get(dtype)
+    if out_code is None:
+        raise ValueError(f"paged_kv_read: dtype {dtype} (supported: bfloat16, float32)")
+    ptrs, geo, kvh, dim, code = _pages(k_pages, v_pages, k_scale, v_scale, out_code, "paged_kv_read")
+    rows = offsets.numel() - 1
+    if rows < 0:
+        raise ValueError("paged_kv_read: offsets must hold rows + 1 entries")
+    table = _table(page_table, rows, "paged_kv_read")
+    device = k_pages.device
+    k = torch.empty(tokens, kvh, dim, device=device, dtype=dtype)
+    v = torch.empty(tokens, kvh, dim, device=device, dtype=dtype)
+    if tokens == 0:
+        return k, v
+    offsets = _index(offsets)
+    _lib.call("omniasr_paged_kv_read", *ptrs, *geo, *table, rows, offsets.data_ptr(), tokens, k.data_ptr(), v.data_ptr(),
+              kvh, dim, out_code, code, status_word(device).data_ptr(), _stream(device))
+    return k, v
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                    lengths: torch.Tensor, scale: float, tokens: int = 1, k_scale: torch.Tensor | None = None,
+                    v_scale: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of each row's newest tokens over its pages: ``q`` [B * tokens, heads, D], row b's queries at rows
+    b * tokens ..; query i of row b sees positions [0, ``lengths[b]`` + i) of the pages that ``page_table`` [B, width]
+    (int32) names, head h those of kv head h // (heads / kv_heads). Pages as :func:`paged_rope_kv` writes them. Returns
+    q's shape and dtype; a query that sees nothing gets zeros."""
+    if q.dim() != 3 or not q.is_contiguous():
+        raise ValueError("paged_attention: q must be contiguous [B * tokens, heads, D]")
+    rows_q, heads, dim = q.shape
+    dtype = _dtype(q, "paged_attention")
+    ptrs, geo, kvh, pdim, code = _pages(k_pages, v_pages, k_scale, v_scale, dtype, "paged_attention")
+    if pdim != dim:
+        raise ValueError("paged_attention: q and the pages differ in head_dim")
+    if tokens < 1 or rows_q % tokens or lengths.numel() * tokens != rows_q:
+        raise ValueError(f"paged_attention: {rows_q} queries are not {lengths.numel()} rows of {tokens} tokens")
+    rows = rows_q // tokens
+    table = _table(page_table, rows, "paged_attention")
+    out = torch.empty_like(q)
+    if rows == 0:
+        return out
+    device = q.device
+    lengths = _index(lengths)
+    nbytes = _lib.load().omniasr_paged_attention_workspace(dtype, code, rows, tokens, heads, kvh, dim, geo[1], table[2])
+    ws = _attn_workspace(nbytes, device)
+    _lib.call("omniasr_paged_attention", q.data_ptr(), *ptrs, *geo, *table, lengths.data_ptr(), out.data_ptr(), rows, tokens,
+              heads, kvh, dim, scale, dtype, code, ws.data_ptr(), ws.numel(), status_word(device).data_ptr(), _stream(device))
+    return out
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor,
+                     k_offsets: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
+    """Causal attention of packed sequences: sequence s has queries ``q_offsets[s]`` .. ``q_offsets[s + 1] - 1`` of ``q``
+    [Tq, heads, D] and keys ``k_offsets[s]`` .. (default: the queries' offsets) of ``k``/``v`` [Tk, kv_heads, D]; its last
+    query sees its last key, so a chunk of a prompt attends to the keys before it. Any token and head strides with
+    16-byte alignment, unit stride in D; offsets ascending, on the device. Returns [Tq, heads, D] in q's dtype (a query
+    that sees no key gets zeros; rows of no sequence are not written)."""
+    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or q.size(2) != k.size(2):
+        raise ValueError("packed_attention: q [Tq, heads, D], k and v [Tk, kv_heads, D]")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("packed_attention: q, k and v must share a dtype")
+    tq, heads, dim = q.shape
+    tk, kv_heads, _ = k.shape
+    if (tq and q.stride(2) != 1) or (tk and (k.stride(2) != 1 or v.stride(2) != 1)):
+        raise ValueError("packed_attention: unit stride in D")
+    dtype = _dtype(q, "packed_attention")
+    if k_offsets is None:
+        k_offsets = q_offsets
+    seqs = q_offsets.numel() - 1
+    if seqs < 0 or k_offsets.numel() != seqs + 1:
+        raise ValueError("packed_attention: q_offsets and k_offsets must hold sequences + 1 entries")
+    out = torch.empty(tq, heads, dim, dtype=q.dtype, device=q.device)
+    if tq == 0:
+        return out
+    device = q.device
+    q_offsets, k_offsets = _index(q_offsets), _index(k_offsets)
+    ws = _attn_workspace(_PACKED_WS, device)
+    _lib.call("omniasr_packed_attention", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
+              v.data_ptr(), v.stride(0), v.stride(1), out.data_ptr(), q_offsets.data_ptr(), k_offsets.data_ptr(), tq, tk,
+              seqs, heads, kv_heads, dim, dim**-0.5 if scale is None else scale, dtype, ws.data_ptr(), ws.numel(),
+              status_word(device).data_ptr(), _stream(device))
+    return out
+
+
+_PACKED_WS = 256
 
 
 def splits_for(rows: int, heads: int, keys: int, block: int = 64, programs: int = 264) -> tuple[int, int]:
