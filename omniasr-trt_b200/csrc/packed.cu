@@ -246,6 +246,10 @@ cudaError_t launch_dim(const PackedArgs& a, cudaStream_t s) {
 }  // namespace packed
 
 cudaError_t launch_packed(int dtype, const PackedArgs& a, cudaStream_t stream) {
+  if (dtype == kBF16 && (a.dim == 128 || a.dim == 512) && a.heads / a.kv_heads <= 128 && a.k_tokens > 0) {
+    const cudaError_t e = a.dim == 128 ? launch_packed_tc(a, stream) : launch_packed_tc_wide(a, stream);
+    if (e != cudaErrorNotSupported) return e;
+  }
   return dtype == kBF16 ? packed::launch_dim<__nv_bfloat16>(a, stream) : packed::launch_dim<float>(a, stream);
 }
 

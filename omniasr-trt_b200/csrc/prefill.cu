@@ -33,10 +33,12 @@
 #include <memory>
 #include <mutex>
 #include <queue>
+#include <type_traits>
 #include <vector>
 
 #include "attention.cuh"
 #include "prefill.cuh"
+#include "paged.cuh"
 #include "prefill_common.cuh"
 #include "tc.cuh"
 #include "trace.cuh"
@@ -98,13 +100,18 @@ struct alignas(1024) Ctl {
   float lsum[NWG][BM];  // [warpgroup][row]: the unit's row sums for the epilogue
   uint32_t tmem_base;
   int abort_flag, issued_k, issued_v, issued_q;  // loads the producers issued
+  uint64_t u_full[kUnitRing], u_empty[kUnitRing];  // packed: the units claimed, for all roles
+  Unit unit[kUnitRing];
 };
 static_assert(sizeof(Ctl) + SMEM_BYTES <= 232448, "shared memory per block");
 static_assert(NSB * 128 + D <= TMEM_COLS, "S buffers and O in TMEM");
 
+// Src: Sched (dense rows) or PackedSrc (packed sequences with grouped heads).
+template <typename Src>
 __global__ void __launch_bounds__(THREADS, 1)
     prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
-                   const __grid_constant__ CUtensorMap vmap, const Params p, const __grid_constant__ Sched sched) {
+                   const __grid_constant__ CUtensorMap vmap, const Params p, const __grid_constant__ Src src) {
+  constexpr bool PACKED = std::is_same_v<Src, PackedSrc>;
   extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ Ctl ctl;
   uint64_t *k_full = ctl.k_full, *k_empty = ctl.k_empty, *v_full = ctl.v_full, *v_empty = ctl.v_empty;
@@ -119,7 +126,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int warp = tid >> 5;
   const int lane = tid & 31;
   const int units = p.batch * p.heads * p.qtiles;
-  if ((int)blockIdx.x >= units) return;
+  if (!PACKED && (int)blockIdx.x >= units) return;
   if (smem_addr(smem) & 1023u) {  // the swizzled tiles need a 1024-aligned ring
     if (tid == 0) raise_status(p.status, kStatusLayout);
     return;
@@ -148,6 +155,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     mbar_init(&l_full, SM_THREADS);
     mbar_init(&l_free, 128);
     mbar_init(&drain, 2);
+    if (PACKED) {
+      for (int j = 0; j < kUnitRing; ++j) {
+        mbar_init(&ctl.u_full[j], 1);
+        mbar_init(&ctl.u_empty[j], 3 + 4 * NWG + 4);  // V loads, S and P V issuers; softmax and epilogue warps
+      }
+    }
     mbar_fence_init();
     abort_flag = 0;
     issued_k = issued_v = issued_q = 0;
@@ -166,8 +179,85 @@ __global__ void __launch_bounds__(THREADS, 1)
     abort_flag = 1;
     return false;
   };
+  // The CTA's n-th unit; false past its last (or, packed, after an abort). put: this role (or warp) is done with it.
+  auto get = [&](int n, Unit& u) -> bool {
+    if constexpr (PACKED) {
+      if (!wait(&ctl.u_full[n % kUnitRing], (n / kUnitRing) & 1)) return false;
+      u = ctl.unit[n % kUnitRing];
+      return u.kt > 0;
+    } else {
+      const int i = cta_unit(src, units, n);
+      if (i < 0) return false;
+      unit_of(p, i, u.b, u.h, u.qt);
+      u.kt = u.qt + 1;
+      return true;
+    }
+  };
+  auto put = [&](int n) {
+    if constexpr (PACKED) mbar_arrive(&ctl.u_empty[n % kUnitRing]);
+  };
 
-  if (warp == W_LOADK || warp == W_LOADV) {
+  if (PACKED && warp == W_LOADK) {
+    // ------------------------------------------------------------------ packed: claims, query and K loads
+    if constexpr (PACKED) {
+      if (lane == 0) {
+        prefetch_tmap(&qmap);
+        prefetch_tmap(&kmap);
+      }
+      PackedWalk walk;
+      walk.init(src, lane, blockIdx.x == 0 ? p.status : nullptr);
+      int tile = 0;
+      long long next = blockIdx.x;
+      for (int n = 0;; ++n) {
+        const Unit u = walk.find(src, next, lane, blockIdx.x == 0 ? p.status : nullptr);
+        bool ok = true;
+        unsigned claim = 0;
+        if (lane == 0) {
+          const int us = n % kUnitRing;
+          ok = n < kUnitRing || wait(&ctl.u_empty[us], (n / kUnitRing - 1) & 1);
+          if (ok) {
+            ctl.unit[us] = u;
+            mbar_arrive(&ctl.u_full[us]);
+          }
+          if (ok && u.kt > 0) {
+            const int qslot = n % QS;
+            ok = n < QS || wait(&q_empty[qslot], (n / QS - 1) & 1);
+            if (ok) {
+              mbar_arrive_expect_tx(&q_full[qslot], (uint32_t)(src.group * src.pos) * 256u);
+              tma_load_4d(smem + Q_OFF + qslot * TILE, &qmap, 0, 0, u.h, u.q0, &q_full[qslot]);
+              tma_load_4d(smem + Q_OFF + qslot * TILE + BOX, &qmap, 64, 0, u.h, u.q0, &q_full[qslot]);
+              issued_q = n + 1;
+            }
+            for (int kt = 0; kt < u.kt && ok; ++kt, ++tile) {
+              // The next unit is claimed near the end of this one, so that no CTA holds units it starts late.
+              if (kt == max(0, u.kt - 3)) claim = atomicAdd(src.counters, 1u);
+              const int slot = tile % KS, use = tile / KS;
+              if (use >= 1 && !wait(&k_empty[slot], (use - 1) & 1)) {
+                ok = false;
+                break;
+              }
+              mbar_arrive_expect_tx(&k_full[slot], TILE);
+              tma_load_4d(smem + K_OFF + slot * TILE, &kmap, 0, u.k0 + kt * BN, u.h, 0, &k_full[slot]);
+              tma_load_4d(smem + K_OFF + slot * TILE + BOX, &kmap, 64, u.k0 + kt * BN, u.h, 0, &k_full[slot]);
+              issued_k = tile + 1;
+            }
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+        if (!ok || u.kt == 0 || abort_flag) break;
+        tile = __shfl_sync(0xffffffffu, tile, 0);
+        next = (long long)gridDim.x + __shfl_sync(0xffffffffu, claim, 0);
+      }
+      if (lane == 0) {
+        // The last CTA to stop claiming leaves the counters zero.
+        if (atomicAdd(src.counters + 1, 1u) == gridDim.x - 1) {
+          src.counters[0] = 0;
+          src.counters[1] = 0;
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == W_LOADK || warp == W_LOADV) {
     // ------------------------------------------------------------------ producers
     if (lane == 0) {
       const bool is_k = warp == W_LOADK;
@@ -178,19 +268,20 @@ __global__ void __launch_bounds__(THREADS, 1)
       uint64_t* full = is_k ? k_full : v_full;
       uint64_t* empty = is_k ? k_empty : v_empty;
       int tile = 0;
-      for (int n = 0, u; (u = cta_unit(sched, units, n)) >= 0 && !abort_flag; ++n) {
-        int b, h, qt;
-        unit_of(p, u, b, h, qt);
-        for (int kt = 0; kt <= qt && !abort_flag; ++kt, ++tile) {
+      Unit u;
+      for (int n = 0; get(n, u) && !abort_flag; ++n) {
+        const int row0 = PACKED ? u.k0 : 0, b = PACKED ? 0 : u.b;
+        for (int kt = 0; kt < u.kt && !abort_flag; ++kt, ++tile) {
           const int slot = tile % ns, use = tile / ns;
           if (use >= 1 && !wait(&empty[slot], (use - 1) & 1)) break;
           mbar_arrive_expect_tx(&full[slot], TILE);
-          tma_load_4d(ring + slot * TILE, map, 0, kt * BN, h, b, &full[slot]);
-          tma_load_4d(ring + slot * TILE + BOX, map, 64, kt * BN, h, b, &full[slot]);
+          tma_load_4d(ring + slot * TILE, map, 0, row0 + kt * BN, u.h, b, &full[slot]);
+          tma_load_4d(ring + slot * TILE + BOX, map, 64, row0 + kt * BN, u.h, b, &full[slot]);
           if (is_k) issued_k = tile + 1;
           else issued_v = tile + 1;
           OMNI_TRACE_AT(tile * 8 + (is_k ? 0 : 1));
         }
+        put(n);
       }
     }
     __syncwarp();
@@ -204,13 +295,12 @@ __global__ void __launch_bounds__(THREADS, 1)
       const uint64_t qdesc0 = smem_desc(smem_addr(smem + Q_OFF), 16, 1024, kLayoutSw128);
       int tile = 0, nunit = 0, sb = 0;
       bool ok = true;
-      for (int u; (u = cta_unit(sched, units, nunit)) >= 0 && ok && !abort_flag; ++nunit) {
-        int b, h, qt;
-        unit_of(p, u, b, h, qt);
+      Unit u;
+      for (; get(nunit, u) && ok && !abort_flag; ++nunit) {
         const int qslot = nunit % QS;
         if (!wait(&q_full[qslot], (nunit / QS) & 1)) break;
         const uint64_t qd = qdesc0 + (uint64_t)(qslot * (TILE >> 4));
-        for (int kt = 0; kt <= qt; ++kt, ++tile, sb = sb == NSB - 1 ? 0 : sb + 1) {
+        for (int kt = 0; kt < u.kt; ++kt, ++tile, sb = sb == NSB - 1 ? 0 : sb + 1) {
           const int slot = tile % KS;
           if (tile >= NSB && !wait(&pv_done[sb], ((tile - NSB) / NSB) & 1)) {
             ok = false;
@@ -230,9 +320,10 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           tc_commit(&s_full[sb]);
           tc_commit(&k_empty[slot]);
-          if (kt == qt) tc_commit(&q_empty[qslot]);  // the unit's last read of its query tile
+          if (kt == u.kt - 1) tc_commit(&q_empty[qslot]);  // the unit's last read of its query tile
           OMNI_TRACE_AT(tile * 8 + 2);
         }
+        put(nunit);
       }
     }
     __syncwarp();
@@ -244,10 +335,9 @@ __global__ void __launch_bounds__(THREADS, 1)
       const uint64_t vdesc0 = smem_desc(smem_addr(smem + V_OFF), BOX, 1024, kLayoutSw128);
       int tile = 0, nunit = 0;
       bool ok = true;
-      for (int u; (u = cta_unit(sched, units, nunit)) >= 0 && ok && !abort_flag; ++nunit) {
-        int b, h, qt;
-        unit_of(p, u, b, h, qt);
-        for (int kt = 0; kt <= qt; ++kt, ++tile) {
+      Unit u;
+      for (; get(nunit, u) && ok && !abort_flag; ++nunit) {
+        for (int kt = 0; kt < u.kt; ++kt, ++tile) {
           const int pb = tile % NSB, pu = tile / NSB;
           const int slot = tile % VS;
           if (kt == 0 && nunit >= 1 && !wait(&o_free, (nunit - 1) & 1)) {
@@ -278,6 +368,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           OMNI_TRACE_AT(tile * 8 + 3);
         }
         if (ok) tc_commit(&o_ready);
+        put(nunit);
       }
     }
     __syncwarp();
@@ -290,13 +381,21 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int row = tid & 127;  // query row within the tile = TMEM lane
     const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t col_o = tbase + lane_off + COL_O + x * DW;  // this warpgroup's head dims of O (rescale)
+    int row_pos = 0;  // packed: the row's position within the tile
+    if constexpr (PACKED) row_pos = row / src.group;
     int tile = 0, nunit = 0;
     bool quit = false;
-    for (int u; (u = cta_unit(sched, units, nunit)) >= 0 && !quit; ++nunit) {
-      int b, h, qt;
-      unit_of(p, u, b, h, qt);
+    for (; !quit; ++nunit) {
+      Unit u;
+      const bool more = get(nunit, u);
+      if constexpr (PACKED) {  // the claim's wait may have given up in some threads: decided by all of them
+        if (sync_or(1, SM_THREADS, abort_flag != 0)) break;
+      }
+      if (!more) break;
+      __syncwarp();
+      if (PACKED && lane == 0) put(nunit);
       float m = -INFINITY, l = 0.f;
-      for (int kt = 0; kt <= qt; ++kt, ++tile) {
+      for (int kt = 0; kt < u.kt; ++kt, ++tile) {
         const int sb = tile % NSB;
         if (row == 0 && x == 0 && tile < 300) OMNI_TRACE_AT(2400 + 1200 + tile);
         wait(&s_full[sb], (tile / NSB) & 1);
@@ -312,7 +411,14 @@ __global__ void __launch_bounds__(THREADS, 1)
         float v[KW];
 #pragma unroll
         for (int i = 0; i < KW; ++i) v[i] = __uint_as_float(raw[i]);
-        if (kt == qt) {  // the diagonal tile: keys past the query
+        if constexpr (PACKED) {
+          if ((kt + 1) * BN > u.lim0) {  // some row does not see all of the tile
+            const int lim = u.lim0 + row_pos - kt * BN - x * KW;  // keys of the warpgroup's half that the row sees
+#pragma unroll
+            for (int i = 0; i < KW; ++i)
+              if (i >= lim) v[i] = -INFINITY;
+          }
+        } else if (kt == u.kt - 1) {  // the diagonal tile: keys past the query
 #pragma unroll
           for (int i = 0; i < KW; ++i)
             if (x * KW + i > row) v[i] = -INFINITY;
@@ -348,11 +454,13 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         // Probabilities (bf16 pairs) over this warpgroup's keys, and the row sum; formed before any rescale of O, so
         // that the scores are dead by then (register pressure).
+        // Packed rows may have seen no key yet (or never see one): their probabilities are 2^(-inf - 0) = 0.
+        const float mref = PACKED && mnew == -INFINITY ? 0.f : mnew;
         uint32_t w[KW / 2];
         uint64_t ls2[4];  // row-sum partials, two per packed register
 #pragma unroll
         for (int j = 0; j < 4; ++j) ls2[j] = 0ull;
-        const uint64_t sc2 = f2_pack(p.qscale, p.qscale), nm2 = f2_pack(-mnew, -mnew);
+        const uint64_t sc2 = f2_pack(p.qscale, p.qscale), nm2 = f2_pack(-mref, -mref);
 #pragma unroll
         for (int i = 0; i < KW / 2; ++i) {
           // x = s * scale - max for a pair in one packed FMA; one pair in kPolyEvery exponentiated on the FMA pipe,
@@ -414,27 +522,33 @@ __global__ void __launch_bounds__(THREADS, 1)
     // One thread also loads the query tiles, two units ahead: unit n + 2's goes into unit n's slot once unit n's last
     // S has completed (q_empty, before its O is ready), so a unit's first S never waits for its queries.
     const bool q_loader = tid == W_EPI * 32;
-    auto load_q = [&](int n, int u) {
+    auto load_q = [&](int n, int i) {
       int b, h, qt;
-      unit_of(p, u, b, h, qt);
+      unit_of(p, i, b, h, qt);
       const int qslot = n % QS;
       mbar_arrive_expect_tx(&q_full[qslot], TILE);
       tma_load_4d(smem + Q_OFF + qslot * TILE, &qmap, 0, qt * BM, h, b, &q_full[qslot]);
       tma_load_4d(smem + Q_OFF + qslot * TILE + BOX, &qmap, 64, qt * BM, h, b, &q_full[qslot]);
       issued_q = n + 1;
     };
-    if (q_loader) {
-      prefetch_tmap(&qmap);
-      for (int n = 0, u; n < QS && (u = cta_unit(sched, units, n)) >= 0; ++n) load_q(n, u);
+    if constexpr (!PACKED) {
+      if (q_loader) {
+        prefetch_tmap(&qmap);
+        for (int n = 0, i; n < QS && (i = cta_unit(src, units, n)) >= 0; ++n) load_q(n, i);
+      }
     }
     int nunit = 0;
-    for (int u; (u = cta_unit(sched, units, nunit)) >= 0 && !abort_flag; ++nunit) {
-      int b, h, qt;
-      unit_of(p, u, b, h, qt);
-      const int ahead = q_loader ? cta_unit(sched, units, nunit + QS) : -1;
-      if (ahead >= 0) {
-        if (!wait(&q_empty[nunit % QS], (nunit / QS) & 1)) break;
-        load_q(nunit + QS, ahead);
+    Unit u;
+    for (; get(nunit, u) && !abort_flag; ++nunit) {
+      if constexpr (!PACKED) {
+        const int ahead = q_loader ? cta_unit(src, units, nunit + QS) : -1;
+        if (ahead >= 0) {
+          if (!wait(&q_empty[nunit % QS], (nunit / QS) & 1)) break;
+          load_q(nunit + QS, ahead);
+        }
+      } else {
+        __syncwarp();
+        if (lane == 0) put(nunit);
       }
       if (!wait(&o_ready, nunit & 1)) break;
       if (!wait(&l_full, nunit & 1)) break;
@@ -445,9 +559,23 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
       for (int y = 0; y < NWG; ++y) l += ctl.lsum[y][row];
       mbar_arrive(&l_free);
-      const float inv = l > 0.f ? 1.f / l : 0.f;
-      const int q = qt * BM + row;
-      __nv_bfloat16* dst = p.out + (int64_t)b * p.out_sb + (int64_t)q * p.out_sw + (int64_t)h * p.out_sh;
+      float inv = l > 0.f ? 1.f / l : 0.f;
+      const int q = u.qt * BM + row;
+      __nv_bfloat16* dst;
+      bool live;
+      int pos = 0, head = 0;
+      if constexpr (PACKED) {
+        pos = row / src.group;
+        head = u.h * src.group + row - pos * src.group;
+        live = pos < u.npos;
+        // A row that sees no key: zeros (its masked probabilities are not exactly zero: ex2_fma's smallest is 2^-126).
+        if (u.lim0 + pos <= 0) inv = 0.f;
+        dst = p.out + ((int64_t)(u.q0 + pos) * src.heads + head) * D;
+      } else {
+        dst = p.out + (int64_t)u.b * p.out_sb + (int64_t)q * p.out_sw + (int64_t)u.h * p.out_sh;
+        live = q < p.width;
+      }
+      float odd = 0.f;  // packed: turns NaN if a result of the row is not finite
       // O in two halves of 64 columns (two loads in flight per wait), released to the next unit's first P V once the
       // second half is in registers, before it is scaled and stored (measured: 183.0 us per config-4 call against
       // 186.5 us with four 32-column reads and the release after the last store).
@@ -461,7 +589,11 @@ __global__ void __launch_bounds__(THREADS, 1)
           tc_fence_before();
           mbar_arrive(&o_free);
         }
-        if (q < p.width) {
+        if (live) {
+          if constexpr (PACKED) {
+#pragma unroll
+            for (int i = 0; i < 64; ++i) odd = fmaf(__uint_as_float(r0[i]), 0.f, odd);
+          }
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             uint32_t w4[4];
@@ -472,6 +604,18 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
             *reinterpret_cast<uint4*>(dst + c * 64 + i * 8) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
           }
+        }
+      }
+      if constexpr (PACKED) {
+        const bool redo = live && !(odd == 0.f && l - l == 0.f);
+        __syncwarp();  // the rows' first results are written before they are written again
+        for (unsigned left = __ballot_sync(0xffffffffu, redo); left; left &= left - 1) {
+          const int w = __ffs(left) - 1;
+          const int wp = __shfl_sync(0xffffffffu, pos, w), wh = __shfl_sync(0xffffffffu, head, w);
+          const int64_t tok = u.q0 + wp;
+          exact_row<D>(src.q + tok * src.q_st + wh * src.q_sh, src.k + u.k0 * src.k_st + u.h * src.k_sh, src.k_st,
+                       src.v + u.k0 * src.v_st + u.h * src.v_sh, src.v_st, u.lim0 + wp, p.qscale,
+                       p.out + (tok * src.heads + wh) * D);
         }
       }
       if (row == 0) OMNI_TRACE_AT(1601 + nunit * 2);
@@ -501,8 +645,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   OMNI_TRACE_CTA(1);
 }
 
-bool make_map(CUtensorMap* map, const void* base, int64_t b, int64_t h, int64_t w, int64_t sb, int64_t sh,
-              int64_t sw) {
+bool encode_map(CUtensorMap* map, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
+                const cuuint32_t* box) {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
     void* ptr = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -512,13 +656,18 @@ bool make_map(CUtensorMap* map, const void* base, int64_t b, int64_t h, int64_t 
     return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
   }();
   if (!fn) return false;
-  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)w, (cuuint64_t)h, (cuuint64_t)b};
-  cuuint64_t strides[3] = {(cuuint64_t)sw * 2, (cuuint64_t)sh * 2, (cuuint64_t)sb * 2};
-  cuuint32_t box[4] = {64, 128, 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool make_map(CUtensorMap* map, const void* base, int64_t b, int64_t h, int64_t w, int64_t sb, int64_t sh,
+              int64_t sw) {
+  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)w, (cuuint64_t)h, (cuuint64_t)b};
+  cuuint64_t strides[3] = {(cuuint64_t)sw * 2, (cuuint64_t)sh * 2, (cuuint64_t)sb * 2};
+  cuuint32_t box[4] = {64, 128, 1, 1};
+  return encode_map(map, base, dims, strides, box);
 }
 
 }  // namespace prefill
@@ -595,7 +744,7 @@ cudaError_t launch_prefill(const PrefillArgs& a, cudaStream_t stream) {
     return cudaErrorInvalidValue;
   static bool configured = false;
   if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+    cudaError_t e = cudaFuncSetAttribute(prefill_kernel<Sched>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
     if (e != cudaSuccess) return e;
     configured = true;
   }
@@ -620,8 +769,68 @@ cudaError_t launch_prefill(const PrefillArgs& a, cudaStream_t stream) {
   if (grid > units) grid = units;
   if (grid <= 0) return cudaSuccess;
   const Sched* sched = prefill_schedule(p.batch, p.heads, p.qtiles, p.group, grid);
-  return launch_dependent(prefill_kernel, dim3(grid), dim3(THREADS), (size_t)SMEM_BYTES, stream, qm, km, vm, p,
+  return launch_dependent(prefill_kernel<Sched>, dim3(grid), dim3(THREADS), (size_t)SMEM_BYTES, stream, qm, km, vm, p,
                           sched ? *sched : prefill_round_robin());
+}
+
+bool packed_maps(const PackedArgs& a, int positions, CUtensorMap* q, CUtensorMap* k, CUtensorMap* v) {
+  using prefill::encode_map;
+  const int group = a.heads / a.kv_heads;
+  // An extent of one has a stride that nothing reads; PyTorch leaves any number there.
+  auto st = [](int64_t extent, int64_t stride) { return (cuuint64_t)(extent > 1 ? stride * 2 : 16); };
+  const cuuint64_t qd[4] = {(cuuint64_t)a.dim, (cuuint64_t)group, (cuuint64_t)a.kv_heads, (cuuint64_t)a.q_tokens};
+  const cuuint64_t qs[3] = {st(group, a.q_sh), st(a.kv_heads, group * a.q_sh), st(a.q_tokens, a.q_st)};
+  const cuuint32_t qb[4] = {64, (cuuint32_t)group, 1, (cuuint32_t)positions};
+  const cuuint64_t kd[4] = {(cuuint64_t)a.dim, (cuuint64_t)a.k_tokens, (cuuint64_t)a.kv_heads, 1};
+  const cuuint64_t ks[3] = {st(a.k_tokens, a.k_st), st(a.kv_heads, a.k_sh), 16};
+  const cuuint64_t vs[3] = {st(a.k_tokens, a.v_st), st(a.kv_heads, a.v_sh), 16};
+  const cuuint32_t kb[4] = {64, 128, 1, 1};
+  for (int i = 0; i < 3; ++i)
+    if (!qs[i] || !ks[i] || !vs[i]) return false;
+  return encode_map(q, a.q, qd, qs, qb) && encode_map(k, a.k, kd, ks, kb) && encode_map(v, a.v, kd, vs, kb);
+}
+
+pfx::PackedSrc packed_source(const PackedArgs& a, int positions) {
+  pfx::PackedSrc s;
+  s.q_offsets = a.q_offsets;
+  s.k_offsets = a.k_offsets;
+  s.q_tokens = a.q_tokens;
+  s.k_tokens = a.k_tokens;
+  s.seqs = a.seqs;
+  s.heads = a.heads;
+  s.kv_heads = a.kv_heads;
+  s.group = a.heads / a.kv_heads;
+  s.pos = positions;
+  s.counters = a.counters;
+  s.q = reinterpret_cast<const __nv_bfloat16*>(a.q);
+  s.k = reinterpret_cast<const __nv_bfloat16*>(a.k);
+  s.v = reinterpret_cast<const __nv_bfloat16*>(a.v);
+  s.q_st = a.q_st, s.q_sh = a.q_sh, s.k_st = a.k_st, s.k_sh = a.k_sh, s.v_st = a.v_st, s.v_sh = a.v_sh;
+  return s;
+}
+
+int packed_grid(const PackedArgs& a, int positions) {
+  const int64_t units = (a.q_tokens / positions + a.seqs) * a.kv_heads;  // at least as many as there are
+  return (int)std::min<int64_t>(device_sm_count(), units);
+}
+
+cudaError_t launch_packed_tc(const PackedArgs& a, cudaStream_t stream) {
+  using namespace prefill;
+  const int positions = BM / (a.heads / a.kv_heads);
+  CUtensorMap qm, km, vm;
+  if (!packed_maps(a, positions, &qm, &km, &vm)) return cudaErrorNotSupported;
+  static bool configured = false;
+  if (!configured) {
+    cudaError_t e = cudaFuncSetAttribute(prefill_kernel<PackedSrc>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+    if (e != cudaSuccess) return e;
+    configured = true;
+  }
+  Params p{};
+  p.qscale = a.scale * kLog2e;
+  p.out = reinterpret_cast<__nv_bfloat16*>(a.out);
+  p.status = a.status;
+  return launch_dependent(prefill_kernel<PackedSrc>, dim3(packed_grid(a, positions)), dim3(THREADS), (size_t)SMEM_BYTES, stream,
+                          qm, km, vm, p, packed_source(a, positions));
 }
 
 }  // namespace omni

@@ -167,6 +167,153 @@ OMNI_DEV int cta_unit(const Sched& s, int units, int n) {
   return k < (int)s.start[blockIdx.x + 1] ? (int)s.unit[k] : -1;
 }
 
+// ---- packed sequences with grouped heads -----------------------------------------------------------------------------
+// A unit's query tile holds `pos` consecutive positions of one kv head's G = heads / kv_heads query heads: tile row r is
+// position r / G, head kv * G + r % G, so that the G heads share every key tile and a short sequence fills more of the
+// 128 rows. Units are claimed by the CTAs as they become free (an atomic counter; the first by block index): sequences in
+// order, each in groups of 16 kv heads, a group's longest query tiles first. Claiming keeps the CTAs' end times together
+// whatever the lengths, which the device alone knows; the warp that loads K claims, and hands the units to the other
+// roles through a ring in shared memory.
+struct PackedSrc {
+  const int64_t* q_offsets;
+  const int64_t* k_offsets;
+  int64_t q_tokens, k_tokens;
+  int seqs, heads, kv_heads, group;  // group: query heads per kv head
+  int pos;                           // positions per query tile
+  unsigned* counters;                // [0] units claimed, [1] CTAs done: zero on entry and left zero
+  const __nv_bfloat16 *q, *k, *v;    // for rows that need the exact form
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;
+};
+
+struct Unit {
+  int b, h, qt;   // dense: row, head, query tile
+  int kt;         // key tiles (0: no more units)
+  int q0, npos;   // packed: first token of the tile, positions in it
+  int k0, lim0;   // first key token; keys the tile's first position sees (the next ones see one more each)
+};
+
+constexpr int kUnitRing = 4;
+constexpr int kUnitHeads = 16;  // kv heads per scheduling group (as prefill_group)
+
+// The claiming warp's place in the sequences: 32 of them at a time, one per lane.
+struct PackedWalk {
+  int s0;             // first sequence of the block in registers
+  long long before;   // units of the sequences before it
+  long long incl;     // units of the block's sequences up to this lane's
+  int tiles;          // this lane's sequence: query tiles, first query / key token, queries, keys
+  int q0, k0, lq, lk;
+
+  OMNI_DEV void load(const PackedSrc& p, int lane, int* status) {
+    const int s = s0 + lane;
+    tiles = 0;
+    if (s < p.seqs) {
+      const int64_t qa = p.q_offsets[s], qb = p.q_offsets[s + 1], ka = p.k_offsets[s], kb = p.k_offsets[s + 1];
+      if (qa < 0 || qb < qa || qb > p.q_tokens || ka < 0 || kb < ka || kb > p.k_tokens) {
+        raise_status(status, kStatusIndex);
+      } else {
+        q0 = (int)qa, lq = (int)(qb - qa), k0 = (int)ka, lk = (int)(kb - ka);
+        tiles = (lq + p.pos - 1) / p.pos;
+      }
+    }
+    long long c = (long long)tiles * p.kv_heads;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, c, o);
+      if (lane >= o) c += y;
+    }
+    incl = c;
+  }
+  OMNI_DEV void init(const PackedSrc& p, int lane, int* status) {
+    s0 = 0;
+    before = 0;
+    q0 = k0 = lq = lk = 0;
+    load(p, lane, status);
+  }
+  // Unit number `u` (ascending from call to call); kt = 0 past the last. All lanes call it and get the same answer.
+  OMNI_DEV Unit find(const PackedSrc& p, long long u, int lane, int* status) {
+    Unit r;
+    r.kt = 0;
+    for (;;) {
+      const unsigned hit = __ballot_sync(0xffffffffu, u < before + incl);
+      if (!hit) {
+        if (s0 + 32 >= p.seqs) return r;
+        before += __shfl_sync(0xffffffffu, incl, 31);
+        s0 += 32;
+        load(p, lane, status);
+        continue;
+      }
+      const int w = __ffs(hit) - 1;
+      const int nt = __shfl_sync(0xffffffffu, tiles, w);
+      int rem = (int)(u - before - (__shfl_sync(0xffffffffu, incl, w) - (long long)nt * p.kv_heads));
+      const int sq = __shfl_sync(0xffffffffu, q0, w), sk = __shfl_sync(0xffffffffu, k0, w);
+      const int nq = __shfl_sync(0xffffffffu, lq, w), nk = __shfl_sync(0xffffffffu, lk, w);
+      const int hg = rem / (kUnitHeads * nt);
+      rem -= hg * kUnitHeads * nt;
+      const int gs = min(kUnitHeads, p.kv_heads - hg * kUnitHeads);
+      const int qt = nt - 1 - rem / gs;
+      r.h = hg * kUnitHeads + rem % gs;
+      r.b = 0;
+      r.qt = qt;
+      r.q0 = sq + qt * p.pos;
+      r.npos = min(p.pos, nq - qt * p.pos);
+      r.k0 = sk;
+      r.lim0 = qt * p.pos + 1 + nk - nq;
+      const int seen = r.lim0 + r.npos - 1;
+      r.kt = seen > 128 ? (seen + 127) / 128 : 1;  // a tile that sees nothing still runs one (masked) key tile
+      return r;
+    }
+  }
+};
+
+// Attention of one query row over its first `lim` keys, by one warp, straight from the formula: for rows whose tensor-core
+// result is not finite, because 0 x NaN (or infinity) of a key the row does not see got into it, or because the row's own
+// keys are so. Keys past `lim` are not read. Rare, so it only has to be right.
+template <int D>
+__device__ __noinline__ void exact_row(const __nv_bfloat16* q, const __nv_bfloat16* k, int64_t k_st, const __nv_bfloat16* v,
+                                       int64_t v_st, int lim, float qscale, __nv_bfloat16* out) {
+  constexpr int N = D / 32;
+  const int lane = threadIdx.x & 31;
+  float qv[N], o[N], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    qv[i] = __bfloat162float(q[i * 32 + lane]);
+    o[i] = 0.f;
+  }
+  for (int j0 = 0; j0 < lim; j0 += 4) {  // four keys' loads in flight
+    __nv_bfloat16 kv[4][N], vv[4][N];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int64_t j = min(j0 + c, lim - 1);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        kv[c][i] = k[j * k_st + i * 32 + lane];
+        vv[c][i] = v[j * v_st + i * 32 + lane];
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      if (j0 + c >= lim) break;
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) s = fmaf(qv[i], __bfloat162float(kv[c][i]), s);
+#pragma unroll
+      for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+      s *= qscale;
+      const float mn = s > m ? s : m;
+      const float base = mn == -INFINITY ? 0.f : mn;
+      const float f = ex2(m - base), pr = ex2(s - base);
+      m = mn;
+      l = fmaf(l, f, pr);
+#pragma unroll
+      for (int i = 0; i < N; ++i) o[i] = fmaf(pr, __bfloat162float(vv[c][i]), o[i] * f);
+    }
+    if (l != l) break;  // a NaN score: the whole row is NaN
+  }
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) out[i * 32 + lane] = __float2bfloat16_rn(l != l ? l : o[i] * inv);
+}
+
 }  // namespace pfx
 
 // (row, head) pairs per scheduling group of the prefill kernels (prefill.cu).
@@ -176,5 +323,11 @@ int prefill_group(int bh_count);
 // shape is past what a schedule holds: then the kernels run round-robin (prefill_round_robin()).
 const pfx::Sched* prefill_schedule(int batch, int heads, int qtiles, int group, int grid);
 const pfx::Sched& prefill_round_robin();
+
+// The packed kernels' tensor maps (false where a stride has none), unit source and grid (prefill.cu).
+struct PackedArgs;
+bool packed_maps(const PackedArgs& a, int positions, CUtensorMap* q, CUtensorMap* k, CUtensorMap* v);
+pfx::PackedSrc packed_source(const PackedArgs& a, int positions);
+int packed_grid(const PackedArgs& a, int positions);
 
 }  // namespace omni

@@ -25,8 +25,11 @@
 #include <cudaTypedefs.h>
 #include <math.h>
 
+#include <type_traits>
+
 #include "attention.cuh"
 #include "prefill.cuh"
+#include "paged.cuh"
 #include "prefill_common.cuh"
 
 namespace omni {
@@ -78,13 +81,18 @@ struct alignas(1024) Ctl {
   float lsum[NWG][BM];
   uint32_t tmem_base;
   int abort_flag, issued_k, issued_v, issued_q;
+  uint64_t u_full[kUnitRing], u_empty[kUnitRing];  // packed: the units claimed, for all roles
+  Unit unit[kUnitRing];
 };
 static_assert(sizeof(Ctl) + SMEM_BYTES <= 232448, "shared memory per block");
 static_assert(NSB * 128 + DH <= TMEM_COLS, "S buffers and O in TMEM");
 
+// Src: Sched (dense rows) or PackedSrc (packed sequences with grouped heads).
+template <typename Src>
 __global__ void __launch_bounds__(THREADS, 1)
     prefill_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
-                        const __grid_constant__ CUtensorMap vmap, const Params p, const __grid_constant__ Sched sched) {
+                        const __grid_constant__ CUtensorMap vmap, const Params p, const __grid_constant__ Src src) {
+  constexpr bool PACKED = std::is_same_v<Src, PackedSrc>;
   extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ Ctl ctl;
   uint64_t *k_full = ctl.k_full, *k_empty = ctl.k_empty, *v_full = ctl.v_full, *v_empty = ctl.v_empty;
@@ -99,7 +107,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int warp = tid >> 5;
   const int lane = tid & 31;
   const int units = p.batch * p.heads * p.qtiles;
-  if ((int)blockIdx.x >= units) return;
+  if (!PACKED && (int)blockIdx.x >= units) return;
   if (smem_addr(smem) & 1023u) {
     if (tid == 0) raise_status(p.status, kStatusLayout);
     return;
@@ -127,6 +135,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     mbar_init(&l_full, SM_THREADS);
     mbar_init(&l_free, 128);
     mbar_init(&drain, 2);
+    if (PACKED) {
+      for (int j = 0; j < kUnitRing; ++j) {
+        mbar_init(&ctl.u_full[j], 1);
+        mbar_init(&ctl.u_empty[j], 3 + 4 * NWG + 4);  // V loads, S and P V issuers; softmax and epilogue warps
+      }
+    }
     mbar_fence_init();
     abort_flag = 0;
     issued_k = issued_v = issued_q = 0;
@@ -144,23 +158,101 @@ __global__ void __launch_bounds__(THREADS, 1)
   };
   auto decode = [&](int u, int& b, int& h, int& qt) { unit_of(p.batch, p.heads, p.qtiles, p.group, u, b, h, qt); };
 
-  if (warp == W_LOADK) {
+  // The CTA's n-th unit; false past its last (or, packed, after an abort). put: this role (or warp) is done with it.
+  auto get = [&](int n, Unit& u) -> bool {
+    if constexpr (PACKED) {
+      if (!wait(&ctl.u_full[n % kUnitRing], (n / kUnitRing) & 1)) return false;
+      u = ctl.unit[n % kUnitRing];
+      return u.kt > 0;
+    } else {
+      const int i = cta_unit(src, units, n);
+      if (i < 0) return false;
+      decode(i, u.b, u.h, u.qt);
+      u.kt = u.qt + 1;
+      return true;
+    }
+  };
+  auto put = [&](int n) {
+    if constexpr (PACKED) mbar_arrive(&ctl.u_empty[n % kUnitRing]);
+  };
+
+  if (PACKED && warp == W_LOADK) {
+    // ------------------------------------------------------------------ packed: claims, query and K loads
+    if constexpr (PACKED) {
+      if (lane == 0) {
+        prefetch_tmap(&qmap);
+        prefetch_tmap(&kmap);
+      }
+      PackedWalk walk;
+      walk.init(src, lane, blockIdx.x == 0 ? p.status : nullptr);
+      int kc = 0;
+      long long next = blockIdx.x;
+      for (int n = 0;; ++n) {
+        const Unit u = walk.find(src, next, lane, blockIdx.x == 0 ? p.status : nullptr);
+        bool ok = true;
+        unsigned claim = 0;
+        if (lane == 0) {
+          const int us = n % kUnitRing;
+          ok = n < kUnitRing || wait(&ctl.u_empty[us], (n / kUnitRing - 1) & 1);
+          if (ok) {
+            ctl.unit[us] = u;
+            mbar_arrive(&ctl.u_full[us]);
+          }
+          for (int pass = 0; pass < 2 && ok; ++pass)
+            for (int kt = 0; kt < u.kt && ok; ++kt) {
+              // The next unit is claimed with the last tile, so that no CTA holds units it starts late.
+              if (pass == 1 && kt == u.kt - 1) claim = atomicAdd(src.counters, 1u);
+              for (int c = 0; c < DC && ok; ++c, ++kc) {
+                if (pass == 0 && kt == 0) {
+                  ok = n < 1 || wait(&q_empty[c], (n - 1) & 1);
+                  if (!ok) break;
+                  mbar_arrive_expect_tx(&q_full[c], (uint32_t)(src.group * src.pos) * 256u);
+                  unsigned char* dst = smem + Q_OFF + c * CHUNK;
+                  tma_load_4d(dst, &qmap, c * 128, 0, u.h, u.q0, &q_full[c]);
+                  tma_load_4d(dst + BOX, &qmap, c * 128 + 64, 0, u.h, u.q0, &q_full[c]);
+                  issued_q = n * DC + c + 1;
+                }
+                const int slot = kc % KS, use = kc / KS;
+                ok = use < 1 || wait(&k_empty[slot], (use - 1) & 1);
+                if (!ok) break;
+                mbar_arrive_expect_tx(&k_full[slot], CHUNK);
+                unsigned char* dst = smem + K_OFF + slot * CHUNK;
+                tma_load_4d(dst, &kmap, c * 128, u.k0 + kt * BN, u.h, 0, &k_full[slot]);
+                tma_load_4d(dst + BOX, &kmap, c * 128 + 64, u.k0 + kt * BN, u.h, 0, &k_full[slot]);
+                issued_k = kc + 1;
+              }
+            }
+        }
+        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+        if (!ok || u.kt == 0 || abort_flag) break;
+        kc = __shfl_sync(0xffffffffu, kc, 0);
+        next = (long long)gridDim.x + __shfl_sync(0xffffffffu, claim, 0);
+      }
+      if (lane == 0) {
+        // The last CTA to stop claiming leaves the counters zero.
+        if (atomicAdd(src.counters + 1, 1u) == gridDim.x - 1) {
+          src.counters[0] = 0;
+          src.counters[1] = 0;
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == W_LOADK) {
     // ------------------------------------------------------------------ K: chunk c of key tile kt, both passes
     if (lane == 0) {
       prefetch_tmap(&kmap);
       int kc = 0;
-      for (int n = 0, u; (u = cta_unit(sched, units, n)) >= 0 && !abort_flag; ++n) {
-        int b, h, qt;
-        decode(u, b, h, qt);
+      Unit u;
+      for (int n = 0; get(n, u) && !abort_flag; ++n) {
         for (int pass = 0; pass < 2 && !abort_flag; ++pass)
-          for (int kt = 0; kt <= qt && !abort_flag; ++kt)
+          for (int kt = 0; kt < u.kt && !abort_flag; ++kt)
             for (int c = 0; c < DC && !abort_flag; ++c, ++kc) {
               const int slot = kc % KS, use = kc / KS;
               if (use >= 1 && !wait(&k_empty[slot], (use - 1) & 1)) break;
               mbar_arrive_expect_tx(&k_full[slot], CHUNK);
               unsigned char* dst = smem + K_OFF + slot * CHUNK;
-              tma_load_4d(dst, &kmap, c * 128, kt * BN, h, b, &k_full[slot]);
-              tma_load_4d(dst + BOX, &kmap, c * 128 + 64, kt * BN, h, b, &k_full[slot]);
+              tma_load_4d(dst, &kmap, c * 128, kt * BN, u.h, u.b, &k_full[slot]);
+              tma_load_4d(dst + BOX, &kmap, c * 128 + 64, kt * BN, u.h, u.b, &k_full[slot]);
               issued_k = kc + 1;
             }
       }
@@ -171,18 +263,19 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (lane == 0) {
       prefetch_tmap(&vmap);
       int vc = 0;
-      for (int n = 0, u; (u = cta_unit(sched, units, n)) >= 0 && !abort_flag; ++n) {
-        int b, h, qt;
-        decode(u, b, h, qt);
+      Unit u;
+      for (int n = 0; get(n, u) && !abort_flag; ++n) {
         for (int pass = 0; pass < 2 && !abort_flag; ++pass)
-          for (int kt = 0; kt <= qt && !abort_flag; ++kt)
+          for (int kt = 0; kt < u.kt && !abort_flag; ++kt)
             for (int sc = 0; sc < NSUB && !abort_flag; ++sc, ++vc) {
               const int slot = vc % VS, use = vc / VS;
               if (use >= 1 && !wait(&v_empty[slot], (use - 1) & 1)) break;
               mbar_arrive_expect_tx(&v_full[slot], BOX);
-              tma_load_4d(smem + V_OFF + slot * BOX, &vmap, pass * DH + sc * 64, kt * BN, h, b, &v_full[slot]);
+              tma_load_4d(smem + V_OFF + slot * BOX, &vmap, pass * DH + sc * 64, (PACKED ? u.k0 : 0) + kt * BN, u.h, u.b,
+                          &v_full[slot]);
               issued_v = vc + 1;
             }
+        put(n);
       }
     }
     __syncwarp();
@@ -193,11 +286,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       const uint64_t qdesc0 = smem_desc(smem_addr(smem + Q_OFF), 16, 1024, kLayoutSw128);
       int tile = 0, kc = 0;
       bool ok = true;
-      for (int n = 0, u; (u = cta_unit(sched, units, n)) >= 0 && ok && !abort_flag; ++n) {
-        int b, h, qt;
-        decode(u, b, h, qt);
+      Unit u;
+      for (int n = 0; get(n, u) && ok && !abort_flag; ++n) {
         for (int pass = 0; pass < 2 && ok; ++pass) {
-          for (int kt = 0; kt <= qt && ok; ++kt, ++tile) {
+          for (int kt = 0; kt < u.kt && ok; ++kt, ++tile) {
             const int sb = tile % NSB;
             if (tile >= NSB && !wait(&pv_done[sb], ((tile - NSB) / NSB) & 1)) {
               ok = false;
@@ -223,12 +315,13 @@ __global__ void __launch_bounds__(THREADS, 1)
                 mma_bf16_ss(dcol, qd + off, kd + off, IDESC_S, (c > 0 || kk > 0) ? 1u : 0u);
               }
               tc_commit(&k_empty[slot]);
-              if (pass == 1 && kt == qt) tc_commit(&q_empty[c]);  // the unit's last read of query chunk c
+              if (pass == 1 && kt == u.kt - 1) tc_commit(&q_empty[c]);  // the unit's last read of query chunk c
             }
             if (!ok) break;
             tc_commit(&s_full[sb]);
           }
         }
+        put(n);
       }
       if (!ok) abort_flag = 1;
     }
@@ -239,11 +332,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       const uint64_t vdesc0 = smem_desc(smem_addr(smem + V_OFF), BOX, 1024, kLayoutSw128);
       int tile = 0, vc = 0, item = 0;
       bool ok = true;
-      for (int n = 0, u; (u = cta_unit(sched, units, n)) >= 0 && ok && !abort_flag; ++n) {
-        int b, h, qt;
-        decode(u, b, h, qt);
+      Unit u;
+      for (int n = 0; get(n, u) && ok && !abort_flag; ++n) {
         for (int pass = 0; pass < 2 && ok; ++pass, ++item) {
-          for (int kt = 0; kt <= qt && ok; ++kt, ++tile) {
+          for (int kt = 0; kt < u.kt && ok; ++kt, ++tile) {
             const int pb = tile % NSB, pu = tile / NSB;
             if (kt == 0 && item >= 1 && !wait(&o_free, (item - 1) & 1)) {
               ok = false;
@@ -275,6 +367,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           if (ok) tc_commit(&o_ready);
         }
+        put(n);
       }
       if (!ok) abort_flag = 1;
     }
@@ -287,12 +380,20 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t col_o = tbase + lane_off + COL_O + x * DW;  // this warpgroup's head dims of O (rescale)
     int tile = 0, item = 0;
     bool quit = false;
-    for (int n = 0, u; (u = cta_unit(sched, units, n)) >= 0 && !quit; ++n) {
-      int b, h, qt;
-      decode(u, b, h, qt);
+    int row_pos = 0;  // packed: the row's position within the tile
+    if constexpr (PACKED) row_pos = row / src.group;
+    for (int n = 0; !quit; ++n) {
+      Unit u;
+      const bool more = get(n, u);
+      if constexpr (PACKED) {  // the claim's wait may have given up in some threads: decided by all of them
+        if (sync_or(1, SM_THREADS, abort_flag != 0)) break;
+      }
+      if (!more) break;
+      __syncwarp();
+      if (PACKED && lane == 0) put(n);
       for (int pass = 0; pass < 2 && !quit; ++pass, ++item) {
         float m = -INFINITY, l = 0.f;
-        for (int kt = 0; kt <= qt; ++kt, ++tile) {
+        for (int kt = 0; kt < u.kt; ++kt, ++tile) {
           const int sb = tile % NSB;
           wait(&s_full[sb], (tile / NSB) & 1);
           tc_fence_after();
@@ -305,7 +406,14 @@ __global__ void __launch_bounds__(THREADS, 1)
           float v[KW];
 #pragma unroll
           for (int i = 0; i < KW; ++i) v[i] = __uint_as_float(raw[i]);
-          if (kt == qt) {  // the diagonal tile: keys past the query
+          if constexpr (PACKED) {
+            if ((kt + 1) * BN > u.lim0) {  // some row does not see all of the tile
+              const int lim = u.lim0 + row_pos - kt * BN - x * KW;  // keys of the warpgroup's half that the row sees
+#pragma unroll
+              for (int i = 0; i < KW; ++i)
+                if (i >= lim) v[i] = -INFINITY;
+            }
+          } else if (kt == u.kt - 1) {  // the diagonal tile: keys past the query
 #pragma unroll
             for (int i = 0; i < KW; ++i)
               if (x * KW + i > row) v[i] = -INFINITY;
@@ -335,11 +443,12 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (t2 > m + kRescale) mnew = t2;
             slow = true;
           }
+          const float mref = PACKED && mnew == -INFINITY ? 0.f : mnew;  // a packed row may have seen no key
           uint32_t w[KW / 2];
           uint64_t ls2[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) ls2[j] = 0ull;
-          const uint64_t sc2 = f2_pack(p.qscale, p.qscale), nm2 = f2_pack(-mnew, -mnew);
+          const uint64_t sc2 = f2_pack(p.qscale, p.qscale), nm2 = f2_pack(-mref, -mref);
 #pragma unroll
           for (int i = 0; i < KW / 2; ++i) {
             float x0, x1;
@@ -391,9 +500,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int row = tid & 127;
     const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
     const bool q_loader = tid == W_EPI * 32;
-    auto load_q = [&](int n, int u) {  // unit u (the CTA's n-th) into the query chunks, each once it is free
+    auto load_q = [&](int n, int i) {  // unit i (the CTA's n-th) into the query chunks, each once it is free
       int b, h, qt;
-      decode(u, b, h, qt);
+      decode(i, b, h, qt);
       for (int c = 0; c < DC; ++c) {
         if (n >= 1 && !wait(&q_empty[c], (n - 1) & 1)) return;
         mbar_arrive_expect_tx(&q_full[c], CHUNK);
@@ -403,19 +512,38 @@ __global__ void __launch_bounds__(THREADS, 1)
         issued_q = n * DC + c + 1;  // chunk loads issued
       }
     };
-    if (q_loader) {
-      prefetch_tmap(&qmap);
-      const int u0 = cta_unit(sched, units, 0);
-      if (u0 >= 0) load_q(0, u0);
+    if constexpr (!PACKED) {
+      if (q_loader) {
+        prefetch_tmap(&qmap);
+        const int u0 = cta_unit(src, units, 0);
+        if (u0 >= 0) load_q(0, u0);
+      }
     }
     int item = 0;
-    for (int n = 0, u; (u = cta_unit(sched, units, n)) >= 0 && !abort_flag; ++n) {
-      int b, h, qt;
-      decode(u, b, h, qt);
+    Unit u;
+    for (int n = 0; get(n, u) && !abort_flag; ++n) {
+      int pos = 0, head = 0;
+      float odd = 0.f;  // packed: turns NaN if a result of the row is not finite
+      bool live;
+      __nv_bfloat16* row_out;
+      if constexpr (PACKED) {
+        __syncwarp();
+        if (lane == 0) put(n);
+        pos = row / src.group;
+        head = u.h * src.group + row - pos * src.group;
+        live = pos < u.npos;
+        row_out = p.out + ((int64_t)(u.q0 + pos) * src.heads + head) * D;
+      } else {
+        const int q = u.qt * BM + row;
+        live = q < p.width;
+        row_out = p.out + (int64_t)u.b * p.out_sb + (int64_t)q * p.out_sw + (int64_t)u.h * p.out_sh;
+      }
       for (int pass = 0; pass < 2 && !abort_flag; ++pass, ++item) {
-        if (pass == 1 && q_loader) {  // the next unit's queries, as the last S MMAs of this one free the chunks
-          const int un = cta_unit(sched, units, n + 1);
-          if (un >= 0) load_q(n + 1, un);
+        if constexpr (!PACKED) {
+          if (pass == 1 && q_loader) {  // the next unit's queries, as the last S MMAs of this one free the chunks
+            const int un = cta_unit(src, units, n + 1);
+            if (un >= 0) load_q(n + 1, un);
+          }
         }
         if (!wait(&o_ready, item & 1)) break;
         if (!wait(&l_full, item & 1)) break;
@@ -425,10 +553,9 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
         for (int y = 0; y < NWG; ++y) l += ctl.lsum[y][row];
         mbar_arrive(&l_free);
-        const float inv = l > 0.f ? 1.f / l : 0.f;
-        const int q = qt * BM + row;
-        __nv_bfloat16* dst =
-            p.out + (int64_t)b * p.out_sb + (int64_t)q * p.out_sw + (int64_t)h * p.out_sh + pass * DH;
+        // A packed row that sees no key: zeros (its masked probabilities are not exactly zero: ex2_fma's smallest is 2^-126).
+        const float inv = l > 0.f && !(PACKED && u.lim0 + pos <= 0) ? 1.f / l : 0.f;
+        __nv_bfloat16* dst = row_out + pass * DH;
 #pragma unroll 1
         for (int c = 0; c < DH / 64; ++c) {
           uint32_t r0[64];
@@ -439,7 +566,11 @@ __global__ void __launch_bounds__(THREADS, 1)
             tc_fence_before();
             mbar_arrive(&o_free);
           }
-          if (q < p.width) {
+          if (live) {
+            if constexpr (PACKED) {
+#pragma unroll
+              for (int i = 0; i < 64; ++i) odd = fmaf(__uint_as_float(r0[i]), 0.f, odd);
+            }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               uint32_t w4[4];
@@ -451,6 +582,19 @@ __global__ void __launch_bounds__(THREADS, 1)
               *reinterpret_cast<uint4*>(dst + c * 64 + i * 8) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
             }
           }
+        }
+        if constexpr (PACKED) odd = fmaf(l, 0.f, odd);
+      }
+      if constexpr (PACKED) {
+        const bool redo = live && odd != 0.f && !abort_flag;
+        __syncwarp();  // the rows' first results are written before they are written again
+        for (unsigned left = __ballot_sync(0xffffffffu, redo); left; left &= left - 1) {
+          const int w = __ffs(left) - 1;
+          const int wp = __shfl_sync(0xffffffffu, pos, w), wh = __shfl_sync(0xffffffffu, head, w);
+          const int64_t tok = u.q0 + wp;
+          exact_row<D>(src.q + tok * src.q_st + wh * src.q_sh, src.k + u.k0 * src.k_st + u.h * src.k_sh, src.k_st,
+                       src.v + u.k0 * src.v_st + u.h * src.v_sh, src.v_st, u.lim0 + wp, p.qscale,
+                       p.out + (tok * src.heads + wh) * D);
         }
       }
     }
@@ -509,7 +653,7 @@ cudaError_t launch_prefill_wide(const PrefillArgs& a, cudaStream_t stream) {
   static bool configured = false;
   if (!configured) {
     cudaError_t e =
-        cudaFuncSetAttribute(prefill_wide_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+        cudaFuncSetAttribute(prefill_wide_kernel<Sched>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
     if (e != cudaSuccess) return e;
     configured = true;
   }
@@ -530,8 +674,28 @@ cudaError_t launch_prefill_wide(const PrefillArgs& a, cudaStream_t stream) {
   if (grid > units) grid = units;
   if (grid <= 0) return cudaSuccess;
   const Sched* sched = prefill_schedule(p.batch, p.heads, p.qtiles, p.group, grid);
-  return launch_dependent(prefill_wide_kernel, dim3(grid), dim3(THREADS), (size_t)SMEM_BYTES, stream, qm, km, vm, p,
+  return launch_dependent(prefill_wide_kernel<Sched>, dim3(grid), dim3(THREADS), (size_t)SMEM_BYTES, stream, qm, km, vm, p,
                           sched ? *sched : prefill_round_robin());
+}
+
+cudaError_t launch_packed_tc_wide(const PackedArgs& a, cudaStream_t stream) {
+  using namespace prefillw;
+  const int positions = BM / (a.heads / a.kv_heads);
+  CUtensorMap qm, km, vm;
+  if (!packed_maps(a, positions, &qm, &km, &vm)) return cudaErrorNotSupported;
+  static bool configured = false;
+  if (!configured) {
+    cudaError_t e =
+        cudaFuncSetAttribute(prefill_wide_kernel<PackedSrc>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+    if (e != cudaSuccess) return e;
+    configured = true;
+  }
+  Params p{};
+  p.qscale = a.scale * kLog2e;
+  p.out = reinterpret_cast<__nv_bfloat16*>(a.out);
+  p.status = a.status;
+  return launch_dependent(prefill_wide_kernel<PackedSrc>, dim3(packed_grid(a, positions)), dim3(THREADS), (size_t)SMEM_BYTES,
+                          stream, qm, km, vm, p, packed_source(a, positions));
 }
 
 }  // namespace omni
