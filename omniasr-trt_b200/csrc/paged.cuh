@@ -66,8 +66,10 @@ struct PagedAttnArgs {
 size_t paged_attention_workspace(int dtype, int type, int rows, int tokens, int heads, int kv_heads, int dim, int page,
                                  int table_width);
 cudaError_t launch_paged_attention(int dtype, const PagedAttnArgs& a, cudaStream_t stream);
+// The tensor-core pass (paged_attention_tc.cu); cudaErrorNotSupported where the pages' strides have no tensor map or the
+// call has 2^31 key tiles and more.
 bool paged_tc_supported(int dtype, int type, int dim, int page);
-size_t paged_tc_workspace(int type, int dim);
+size_t paged_tc_workspace(int dim);
 cudaError_t launch_paged_attention_tc(const PagedAttnArgs& a, cudaStream_t stream);
 
 struct PackedArgs {

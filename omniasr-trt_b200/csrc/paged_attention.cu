@@ -311,10 +311,6 @@ cudaError_t launch_dim(const PagedAttnArgs& a, const Split& sp, cudaStream_t s) 
 
 }  // namespace paged
 
-bool paged_tc_supported(int, int, int, int) { return false; }
-size_t paged_tc_workspace(int, int) { return 0; }
-cudaError_t launch_paged_attention_tc(const PagedAttnArgs&, cudaStream_t) { return cudaErrorInvalidValue; }
-
 size_t paged_attention_workspace(int, int, int rows, int tokens, int heads, int kv_heads, int dim, int page,
                                  int table_width) {
   const paged::Split s = paged::plan(rows, tokens, heads, kv_heads, dim, page, table_width);

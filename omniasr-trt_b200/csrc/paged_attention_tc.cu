@@ -1,0 +1,1118 @@
+// Attention of each row's newest tokens over a paged KV cache on the 5th-generation tensor cores (tcgen05 + TMEM):
+// bf16 queries, bf16 or e4m3 pages, head_dim 128, 256 or 512, pages of 8 .. 64 positions (powers of two) or of a multiple
+// of 128.
+//
+// A unit is (row, kv head, chunk of at most 16 query columns): the row's T * G query vectors on that kv head share every
+// key. The keys of all units, in 128-key tiles, are cut evenly between the CTAs (one per SM), so that every SM streams
+// the same bytes whatever the lengths; a unit cut between CTAs leaves one partial result (maximum, sum, unnormalised
+// output) per CTA, and the CTA that finishes last joins them in the order of the keys. Per tile, keys and head dims lie in
+// the MMA's M, the query columns in its N:
+//   S^T [128 keys x N]  = K [128 x D] Q^T            accumulated over 128-dim chunks
+//   P^T = 2^(S^T scale log2e - m)                      one thread per key, m raised only when passed by 2^8
+//   O^T [D x N]        += V^T [D x 128 keys] P^T       accumulated in TMEM over the unit's tiles
+// K and V chunks stream through one ring of shared-memory slots in the order the MMAs use them (K of tile t + 1 before V of
+// tile t), filled by TMA page by page.
+//
+// e4m3 pages are fed to the tensor core as they are (kind::f8f6f4), at half the bytes of bf16; the query and the
+// probabilities become two e4m3 pieces each, in columns of their own: q = 2^e (q1 + q2 / 16), q1 = rn(q 2^-e), q2 =
+// rn(16 (q 2^-e - q1)), 4 + 4 significant bits, which hold a bf16 q exactly (down to 2^-22 of the vector's largest) and
+// a probability as well as bf16 does. The columns are there anyway: N is at least 16. A key's scale 2^ek multiplies its
+// scores; a value's scale 2^ev joins the probability as an exponent: w = 2^(x + ev - m), O = sum w v8, l = sum w 2^-ev,
+// with m the running maximum of x + ev, so that w stays in e4m3's range whatever the scales are. m is kept 2^4 below the
+// maximum, w up to 2^8: the pieces' smallest step is then 2^-17 of a typical largest weight.
+//
+// What bounds it: HBM. bytes = keys * kv_heads * D * 2 * element (+ 2 scale bytes a key).
+
+#include <cudaTypedefs.h>
+#include <math.h>
+
+#include <cuda_fp8.h>
+
+#include <algorithm>
+
+#include "attention.cuh"
+#include "paged.cuh"
+#include "tc.cuh"
+
+namespace omni {
+namespace pagedtc {
+
+constexpr int BN = 128;            // keys per tile (the MMA's M)
+constexpr int kMaxCols = 16;       // query columns per unit
+constexpr int kMaxRows = 1024;     // rows of one launch
+constexpr int kBox = BN * 128;     // 128 keys x 128 bytes
+constexpr int kScaleStages = 8;    // tiles of scale bytes in shared memory
+constexpr float kRaise = 8.f;      // log2: a weight may reach 2^8 before its column's maximum is raised
+constexpr float kHead8 = 4.f;      // e4m3: the maximum kept this far (log2) below the largest exponent seen
+constexpr float kBelow = 64.f;     // bf16: a unit starts from maximum 0 unless its scores lie 2^64 below
+
+template <bool FP8, int DIM, int NQT>
+struct Cfg {
+  static constexpr int DC = DIM / 128;                     // 128-dim chunks
+  static constexpr int SLOT = FP8 ? kBox : 2 * kBox;       // one chunk of a K or V tile
+  static constexpr int N = FP8 ? (2 * NQT < 16 ? 16 : 2 * NQT) : 16;  // MMA columns
+  static constexpr int QBOX = N * 128;                     // N rows x 128 bytes of the query
+  static constexpr int QB = DC * (FP8 ? 1 : 2) * QBOX;     // one query buffer
+  static constexpr int PB = BN * N * (FP8 ? 1 : 2);        // one P buffer
+  static constexpr int FIXED = 2 * QB + 2 * PB + 2 * kMaxRows * 4 + 64 + (FP8 ? kScaleStages * 2 * BN : 0);
+  static constexpr int FIT = (232448 - 2048 - 1024 - FIXED) / SLOT;
+  static constexpr int SLOTS = FIT > 12 ? 12 : FIT;
+  static constexpr int Q_OFF = SLOTS * SLOT;
+  static constexpr int P_OFF = Q_OFF + 2 * QB;
+  static constexpr int SC_OFF = P_OFF + 2 * PB;            // scale bytes [stage][K, V][128]
+  static constexpr int PRE_OFF = SC_OFF + (FP8 ? kScaleStages * 2 * BN : 0);  // int [rows + 1]: tiles before a row
+  static constexpr int LEN_OFF = PRE_OFF + (kMaxRows + 16) * 4;               // int [rows]
+  static constexpr int BYTES = LEN_OFF + kMaxRows * 4 + 1024;                 // + alignment slack
+  static constexpr uint32_t S_COLS = 2 * N;
+  static constexpr uint32_t COLS = S_COLS + 2 * DC * N;
+  static constexpr uint32_t TMEM = COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
+  static_assert(SLOTS >= DC, "a tile's V chunks are all resident when its stale rows are cleared");
+  static_assert(BYTES + 2048 <= 232448, "shared memory per block");
+};
+
+constexpr int kThreads = 384;
+constexpr int W_LOAD = 4, W_MMA = 5, W_Q = 6, W_SCALE = 7, W_EPI = 8;
+
+struct Params {
+  const __nv_bfloat16* q;
+  PageCache c;
+  const int32_t* table;
+  int64_t table_stride;
+  const int64_t* lengths;
+  __nv_bfloat16* out;
+  int rows, tokens, heads, group;  // group: query heads per kv head
+  int cols, chunk_cols, chunks;    // query columns per (row, kv head), per unit, units per (row, kv head)
+  int cap;                         // keys a row can have
+  int page_shift;                  // log2(page) for pages below 128, else -1
+  float qscale;
+  unsigned* counters;              // per CTA: partial results published of the unit that starts there and is cut
+  float* part_o;                   // [2 * CTA + place][column][DIM]; place 0: a unit begun in an earlier CTA, 1: in this one
+  float2* part_ml;                 // [2 * CTA + place][column]
+  int* status;
+};
+
+OMNI_DEV void mma_f8_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// kind::f8f6f4 instruction descriptor: e4m3 A and B (format 0), fp32 accumulator.
+constexpr uint32_t idesc_e4m3(int m, int n, int a_mn_major, int b_mn_major) {
+  return (1u << 4) | ((uint32_t)a_mn_major << 15) | ((uint32_t)b_mn_major << 16) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(m >> 4) << 24);
+}
+
+OMNI_DEV void tmem_st16(uint32_t taddr, const float* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16};" ::"r"(taddr),
+      "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3])),
+      "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])), "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7])),
+      "r"(__float_as_uint(v[8])), "r"(__float_as_uint(v[9])), "r"(__float_as_uint(v[10])), "r"(__float_as_uint(v[11])),
+      "r"(__float_as_uint(v[12])), "r"(__float_as_uint(v[13])), "r"(__float_as_uint(v[14])), "r"(__float_as_uint(v[15]))
+      : "memory");
+}
+
+OMNI_DEV bool sync_or(int id, int count, bool pred) {
+  uint32_t out;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, %2, %3, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(out)
+      : "r"((uint32_t)pred), "r"(id), "r"(count)
+      : "memory");
+  return out != 0;
+}
+
+// Column totals over a warp of NV values per lane; every lane gets every column's (maximum or sum).
+template <int NV, bool MAX>
+OMNI_DEV void warp_all(float (&v)[NV]) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const float y = __shfl_xor_sync(0xffffffffu, v[j], o);
+      v[j] = MAX ? fmaxf(v[j], y) : v[j] + y;
+    }
+}
+
+// A CTA's part of one unit: tiles [t0, t1) of the unit's nt.
+struct Seg {
+  int b, u;        // row; unit within the row (kv head * chunks + chunk)
+  int t0, t1, nt;
+  int first;       // first tile of the unit in the global numbering
+};
+
+struct Walk {
+  const int* pre;
+  int rows, per_row, pos, end, b;
+  OMNI_DEV void init(const int* pre_, int rows_, int per_row_, int c0, int c1) {
+    pre = pre_;
+    rows = rows_;
+    per_row = per_row_;
+    pos = c0;
+    end = c1;
+    int lo = 0, hi = rows - 1;  // the first row that ends past c0
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (pre[mid + 1] > c0) hi = mid;
+      else lo = mid + 1;
+    }
+    b = lo;
+  }
+  OMNI_DEV bool next(Seg& s) {
+    if (pos >= end) return false;
+    while (pre[b + 1] <= pos) ++b;  // rows without keys have no tiles
+    const int nt = (pre[b + 1] - pre[b]) / per_row;
+    const int r = pos - pre[b];
+    s.b = b;
+    s.nt = nt;
+    s.u = r / nt;
+    s.t0 = r - s.u * nt;
+    s.t1 = min(nt, s.t0 + (end - pos));
+    s.first = pos - s.t0;
+    pos += s.t1 - s.t0;
+    return true;
+  }
+};
+
+struct alignas(16) Ctl {
+  uint64_t full[12], empty[12];
+  uint64_t s_full[2], s_free[2], p_full[2], pv_done[2], q_full[2], q_empty[2], o_full[2], o_free[2], ml_full[2];
+  uint64_t sc_full[kScaleStages], sc_empty[kScaleStages];
+  uint64_t drain;
+  float red[4][kMaxCols];         // column maxima per softmax warp
+  float sum[2][4][kMaxCols];      // a finished segment's column sums per softmax warp
+  float top[2][kMaxCols];         // ... and maxima
+  float cq[4][kMaxCols];          // score factor per column (scale, log2e, the query's exponent)
+  int wsum[kThreads / 32];
+  uint32_t tmem_base;
+  int abort_flag, issued;         // chunks the producer has issued
+  int last;                       // epilogue: this CTA joins the unit
+  unsigned bad;                   // epilogue: columns to redo
+};
+static_assert(sizeof(Ctl) <= 2048, "control block");
+
+// The query row and the keys that column `col` of row b, kv head h sees.
+OMNI_DEV int64_t query_row(const Params& p, int b, int h, int col, int* t) {
+  *t = col / p.group;
+  return ((int64_t)b * p.tokens + *t) * p.heads + h * p.group + (col - *t * p.group);
+}
+
+// One column straight from the formula, by one warp: for a draft column whose tensor-core result is not finite, because a
+// later draft position that it does not see holds something that is not (0 x NaN), or its own keys do. Rare.
+template <bool FP8, int DIM>
+__device__ __noinline__ void exact_column(const __nv_bfloat16* q, const PageCache& c, const int32_t* table, int h, int lim,
+                                          float qscale, __nv_bfloat16* out) {
+  constexpr int NV = DIM / 32;
+  const int lane = threadIdx.x & 31;
+  float qv[NV], o[NV], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    qv[i] = __bfloat162float(q[i * 32 + lane]);
+    o[i] = 0.f;
+  }
+  auto value = [](const void* base, int64_t at) {
+    if (FP8) {
+      const __half_raw r = __nv_cvt_fp8_to_halfraw(reinterpret_cast<const uint8_t*>(base)[at], __NV_E4M3);
+      return __half2float(*reinterpret_cast<const __half*>(&r));
+    }
+    return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(base)[at]);
+  };
+  for (int j = 0; j < lim; ++j) {
+    const int pi = j / c.page, off = j - pi * c.page;
+    int64_t id = table[pi];
+    if (id < 0 || id >= c.pages) id = 0;
+    const int64_t at = id * c.s_page + (int64_t)h * c.s_head + (int64_t)off * c.s_pos;
+    float ks = 1.f, vs = 1.f;
+    if (FP8) {
+      const int64_t si = (id * c.kv_heads + h) * c.page + off;
+      ks = __uint_as_float((uint32_t)c.k_scale[si] << 23);
+      vs = __uint_as_float((uint32_t)c.v_scale[si] << 23);
+    }
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) s = fmaf(qv[i], value(c.k, at + i * 32 + lane), s);
+#pragma unroll
+    for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+    s *= qscale * ks;
+    const float mn = s > m ? s : m;
+    const float base = mn == -INFINITY ? 0.f : mn;
+    const float f = ex2(m - base), pr = ex2(s - base);
+    m = mn;
+    l = fmaf(l, f, pr);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) o[i] = fmaf(pr * vs, value(c.v, at + i * 32 + lane), o[i] * f);
+    if (l != l) break;  // a NaN score: the whole row is NaN
+  }
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) out[i * 32 + lane] = __float2bfloat16_rn(l != l ? l : o[i] * inv);
+}
+
+template <bool FP8, int DIM, int NQT>
+__global__ void __launch_bounds__(kThreads, 1)
+    paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ Params p) {
+  using C = Cfg<FP8, DIM, NQT>;
+  constexpr int DC = C::DC, N = C::N, SLOTS = C::SLOTS, SLOT = C::SLOT;
+  constexpr int NB = FP8 ? 1 : 2;  // 128-byte boxes per chunk
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ Ctl ctl;
+  int* pre = reinterpret_cast<int*>(smem + C::PRE_OFF);
+  int* len = reinterpret_cast<int*>(smem + C::LEN_OFF);
+  volatile int& abort_flag = ctl.abort_flag;
+  volatile int& issued = ctl.issued;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (tid == 0) {
+    for (int s = 0; s < SLOTS; ++s) {
+      mbar_init(&ctl.full[s], 1);
+      mbar_init(&ctl.empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&ctl.s_full[s], 1);
+      mbar_init(&ctl.s_free[s], 128);
+      mbar_init(&ctl.p_full[s], 128);
+      mbar_init(&ctl.pv_done[s], 1);
+      mbar_init(&ctl.q_full[s], 1);
+      mbar_init(&ctl.q_empty[s], 1);
+      mbar_init(&ctl.o_full[s], 1);
+      mbar_init(&ctl.o_free[s], 128);
+      mbar_init(&ctl.ml_full[s], 128);
+    }
+    for (int s = 0; s < kScaleStages; ++s) {
+      mbar_init(&ctl.sc_full[s], 1);
+      mbar_init(&ctl.sc_empty[s], 4);
+    }
+    mbar_init(&ctl.drain, 1);
+    mbar_fence_init();
+    abort_flag = 0;
+    issued = 0;
+    ctl.bad = 0;
+  }
+  if (warp == W_EPI) tmem_alloc(&ctl.tmem_base, C::TMEM);
+  if (warp == W_LOAD && lane == 0) {
+    prefetch_tmap(&kmap);
+    prefetch_tmap(&vmap);
+  }
+  grid_launch_dependents();
+  grid_dependency_wait();  // everything below may come from the kernel before
+
+  // Tiles before each row, and the rows' lengths, in shared memory (each thread sums consecutive rows, then a block scan).
+  const int per_row = p.c.kv_heads * p.chunks;
+  {
+    const int each = (p.rows + kThreads - 1) / kThreads;
+    int mine = 0;
+    for (int i = 0; i < each; ++i) {
+      const int b = tid * each + i;
+      if (b >= p.rows) break;
+      const int64_t raw = p.lengths[b], most = raw + p.tokens - 1;
+      if (blockIdx.x == 0 && (raw < 0 || most > p.cap)) raise_status(p.status, kStatusIndex);
+      // The keys of the row's last query; a length out of range is clamped (and was reported).
+      const int64_t lim = raw < -(int64_t)p.tokens ? -(int64_t)p.tokens : (raw > p.cap ? (int64_t)p.cap : raw);
+      len[b] = (int)lim;
+      const int64_t need = most < 0 ? 0 : (most > p.cap ? (int64_t)p.cap : most);
+      mine += (int)((need + BN - 1) / BN) * per_row;
+      pre[b + 1] = mine;
+    }
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    if (lane == 31) ctl.wsum[warp] = incl;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    int before = incl - mine;
+    for (int w = 0; w < warp; ++w) before += ctl.wsum[w];
+    for (int i = 0; i < each; ++i) {
+      const int b = tid * each + i;
+      if (b >= p.rows) break;
+      pre[b + 1] += before;
+    }
+    if (tid == 0) pre[0] = 0;
+    __syncthreads();
+  }
+  const int total = pre[p.rows];
+  const int per = max(1, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+  const int c0 = min(total, (int)blockIdx.x * per), c1 = min(total, c0 + per);
+  const int tiles = c1 - c0;
+  const uint32_t tbase = ctl.tmem_base;
+  auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+    if (mbar_wait_or(bar, parity, &abort_flag)) return true;
+    abort_flag = 1;
+    return false;
+  };
+  auto need_of = [&](int b) { return min(p.cap, len[b] + p.tokens - 1); };  // of a row that has tiles
+  // Ring position of tile i's first V chunk (K and V chunks in the MMAs' order: K0 K1 V0 K2 V1 .. V(n-1)).
+  auto v_chunk = [&](int i) { return DC * (i == tiles - 1 ? 2 * i + 1 : 2 * i + 2); };
+
+  if (warp == W_SCALE) {  // the rows without keys: zeros, by this warp of every CTA
+    for (int b = blockIdx.x; b < p.rows; b += gridDim.x) {
+      if (pre[b + 1] != pre[b]) continue;
+      uint4* o = reinterpret_cast<uint4*>(p.out + (int64_t)b * p.tokens * p.heads * DIM);
+      for (int i = lane; i < p.tokens * p.heads * (DIM / 8); i += 32) o[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
+
+  if (tiles <= 0) {
+    // nothing but giving the TMEM back
+  } else if (warp == W_LOAD) {
+    // ------------------------------------------------------------------ K and V, page by page
+    // Lane i holds the tile's i-th page (the only one, for pages of 128 positions and more), loaded a tile ahead.
+    const bool small = p.page_shift >= 0;
+    const int rows_box = small ? p.c.page : BN;
+    const int boxes = small ? BN >> p.page_shift : 1;
+    Walk w;
+    w.init(pre, p.rows, per_row, c0, c1);
+    Seg s{};
+    int t = 0, ntile = 0;  // the tile in hand
+    struct Tile {
+      int h, live, row, id;  // kv head, boxes with keys, first row within the page, this lane's page
+    };
+    auto fetch = [&](Tile& x) {  // the tile (s, t): its page numbers start to load
+      const int need = need_of(s.b);
+      const int left = need - t * BN;
+      x.h = s.u / p.chunks;
+      x.live = small ? min(boxes, (left + rows_box - 1) >> p.page_shift) : 1;
+      x.row = small ? 0 : (t * BN) % p.c.page;
+      const int pi = small ? ((t * BN) >> p.page_shift) + lane : (t * BN) / p.c.page;
+      x.id = lane < x.live ? __ldg(p.table + (int64_t)s.b * p.table_stride + pi) : 0;
+    };
+    auto step = [&]() {  // to the next tile; false past the last
+      if (++ntile >= tiles) return false;
+      if (++t >= s.t1) {
+        w.next(s);
+        t = s.t0;
+      }
+      return true;
+    };
+    int chunk = 0;
+    auto load = [&](const CUtensorMap* map, const Tile& x) -> bool {
+      for (int c = 0; c < DC; ++c, ++chunk) {
+        const int slot = chunk % SLOTS, use = chunk / SLOTS;
+        bool ok = true;
+        if (lane == 0) {
+          ok = use < 1 || wait(&ctl.empty[slot], (use - 1) & 1);
+          if (ok) mbar_arrive_expect_tx(&ctl.full[slot], (uint32_t)(x.live * rows_box * 128 * NB));
+        }
+        if (!__shfl_sync(0xffffffffu, ok ? 1 : 0, 0)) return false;
+        if (lane < x.live) {
+          unsigned char* dst = smem + slot * SLOT + lane * rows_box * 128;
+#pragma unroll
+          for (int x2 = 0; x2 < NB; ++x2)
+            tma_load_4d(dst + x2 * kBox, map, c * 128 + x2 * 64, x.row, x.h, x.id, &ctl.full[slot]);
+        }
+        __syncwarp();
+        if (lane == 0) issued = chunk + 1;
+      }
+      return true;
+    };
+    w.next(s);
+    t = s.t0;
+    Tile cur, nxt, prev;
+    fetch(cur);
+    prev = cur;
+    for (int i = 0; i < tiles; ++i) {
+      if (cur.id < 0 || cur.id >= (int)p.c.pages) {
+        raise_status(p.status, kStatusIndex);
+        cur.id = 0;
+      }
+      const bool more = step();
+      if (more) fetch(nxt);
+      if (!load(&kmap, cur)) break;
+      if (i > 0 && !load(&vmap, prev)) break;
+      prev = cur;
+      if (more) cur = nxt;
+      if (i == tiles - 1) load(&vmap, prev);
+    }
+    __syncwarp();
+  } else if (warp == W_MMA) {
+    // ------------------------------------------------------------------ S^T(i), then O^T += V(i-1)^T P(i-1)^T
+    if (lane == 0) {
+      constexpr uint32_t IS = FP8 ? idesc_e4m3(128, N, 0, 0) : idesc_bf16(128, N, 0, 0);
+      constexpr uint32_t IO = FP8 ? idesc_e4m3(128, N, 1, 1) : idesc_bf16(128, N, 1, 1);
+      const uint32_t ring = smem_addr(smem), qbase = smem_addr(smem + C::Q_OFF), pbase = smem_addr(smem + C::P_OFF);
+      Walk w;
+      w.init(pre, p.rows, per_row, c0, c1);
+      Seg s{};
+      int chunk = 0, i = 0, nseg = 0;
+      // The tile whose O^T is to issue: its segment's number, whether it is the segment's first / last tile.
+      int pi = -1, pseg = 0;
+      bool pfirst = false, plast = false, ok = true;
+      auto values = [&]() -> bool {
+        const int b = pi & 1;
+        if (pfirst && pseg >= 2 && !wait(&ctl.o_free[pseg & 1], (pseg / 2 - 1) & 1)) return false;
+        if (!wait(&ctl.p_full[b], (pi >> 1) & 1)) return false;
+        for (int c = 0; c < DC; ++c, ++chunk) {
+          const int slot = chunk % SLOTS;
+          if (!wait(&ctl.full[slot], (chunk / SLOTS) & 1)) return false;
+          tc_fence_after();
+          const uint32_t va = ring + slot * SLOT, pa = pbase + b * C::PB;
+          const uint32_t d = tbase + C::S_COLS + ((pseg & 1) * DC + c) * N;
+          if constexpr (FP8) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              mma_f8_ss(d, smem_desc(va + kk * 4096, kBox, 1024, kLayoutSw128), smem_desc(pa + kk * 512, 128, 2048, kLayoutNone),
+                        IO, (pfirst && kk == 0) ? 0u : 1u);
+          } else {
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk)
+              mma_bf16_ss(d, smem_desc(va + kk * 2048, kBox, 1024, kLayoutSw128), smem_desc(pa + kk * 256, 128, 2048, kLayoutNone),
+                          IO, (pfirst && kk == 0) ? 0u : 1u);
+          }
+          tc_commit(&ctl.empty[slot]);
+        }
+        tc_commit(&ctl.pv_done[b]);
+        if (plast) tc_commit(&ctl.o_full[pseg & 1]);
+        return true;
+      };
+      for (; ok && w.next(s); ++nseg) {
+        ok = wait(&ctl.q_full[nseg & 1], (nseg >> 1) & 1);
+        for (int t = s.t0; ok && t < s.t1; ++t, ++i) {
+          const int b = i & 1;
+          if (i >= 2) ok = wait(&ctl.s_free[b], ((i >> 1) - 1) & 1);
+          for (int c = 0; ok && c < DC; ++c, ++chunk) {
+            const int slot = chunk % SLOTS;
+            ok = wait(&ctl.full[slot], (chunk / SLOTS) & 1);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t ka = ring + slot * SLOT, qa = qbase + (nseg & 1) * C::QB + c * NB * C::QBOX;
+            const uint32_t d = tbase + b * N;
+            if constexpr (FP8) {
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)
+                mma_f8_ss(d, smem_desc(ka + kk * 32, 16, 1024, kLayoutSw128), smem_desc(qa + kk * 32, 16, 1024, kLayoutSw128),
+                          IS, (c > 0 || kk > 0) ? 1u : 0u);
+            } else {
+#pragma unroll
+              for (int kk = 0; kk < 8; ++kk)
+                mma_bf16_ss(d, smem_desc(ka + (kk >> 2) * kBox + (kk & 3) * 32, 16, 1024, kLayoutSw128),
+                            smem_desc(qa + (kk >> 2) * C::QBOX + (kk & 3) * 32, 16, 1024, kLayoutSw128), IS,
+                            (c > 0 || kk > 0) ? 1u : 0u);
+            }
+            tc_commit(&ctl.empty[slot]);
+          }
+          if (!ok) break;
+          tc_commit(&ctl.s_full[b]);
+          if (t == s.t1 - 1) tc_commit(&ctl.q_empty[nseg & 1]);
+          if (pi >= 0) ok = values();
+          pi = i;
+          pseg = nseg;
+          pfirst = t == s.t0;
+          plast = t == s.t1 - 1;
+        }
+      }
+      if (ok && pi >= 0) values();
+    }
+    __syncwarp();
+  } else if (warp == W_Q) {
+    // ------------------------------------------------------------------ a segment's queries, in the swizzled layout
+    Walk w;
+    w.init(pre, p.rows, per_row, c0, c1);
+    Seg s{};
+    for (int n = 0; w.next(s); ++n) {
+      bool ok = true;
+      if (lane == 0) ok = n < 2 || wait(&ctl.q_empty[n & 1], ((n >> 1) - 1) & 1);
+      if (!__shfl_sync(0xffffffffu, ok ? 1 : 0, 0)) break;
+      unsigned char* qb = smem + C::Q_OFF + (n & 1) * C::QB;
+      const int h = s.u / p.chunks, col0 = (s.u - h * p.chunks) * p.chunk_cols;
+      const int ncol = min(p.chunk_cols, p.cols - col0);
+      if constexpr (FP8) {
+        // Four dims per lane of each 128-dim chunk; one scale per vector.
+#pragma unroll 2
+        for (int j = 0; j < ncol; ++j) {
+          int tt;
+          const __nv_bfloat16* src = p.q + query_row(p, s.b, h, col0 + j, &tt) * DIM;
+          float x[DC][4];
+          uint32_t amax = 0u;
+#pragma unroll
+          for (int c = 0; c < DC; ++c) {
+            const uint2 r = __ldg(reinterpret_cast<const uint2*>(src + c * 128) + lane);
+            x[c][0] = __uint_as_float(r.x << 16), x[c][1] = __uint_as_float(r.x & 0xffff0000u);
+            x[c][2] = __uint_as_float(r.y << 16), x[c][3] = __uint_as_float(r.y & 0xffff0000u);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t bits = __float_as_uint(x[c][k]) & 0x7fffffffu;
+              amax = max(amax, bits < 0x7f800000u ? bits : 0u);
+            }
+          }
+          amax = __reduce_max_sync(0xffffffffu, amax);
+          int e = (int)(amax >> 23) - 127 - 7;  // the largest in [2^7, 2^8)
+          e = amax == 0u ? 0 : (e < -100 ? -100 : e);
+          const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+          for (int c = 0; c < DC; ++c) {
+            uint32_t hi = 0u, lo = 0u;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float y = x[c][k] * inv;
+              const uint32_t a = __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+              const __half_raw hr = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)a, __NV_E4M3);
+              const uint32_t r = __nv_cvt_float_to_fp8((y - __half2float(*reinterpret_cast<const __half*>(&hr))) * 16.f,
+                                                       __NV_SATFINITE, __NV_E4M3);
+              const bool fin = fabsf(y) <= 448.f;
+              hi |= (fin ? a : 0x7fu) << (8 * k);
+              lo |= (fin ? r : 0x7fu) << (8 * k);
+            }
+            const int r1 = j, r2 = NQT + j;
+            unsigned char* box = qb + c * C::QBOX;
+            *reinterpret_cast<uint32_t*>(box + r1 * 128 + (((lane >> 2) ^ (r1 & 7)) << 4) + (lane & 3) * 4) = hi;
+            *reinterpret_cast<uint32_t*>(box + r2 * 128 + (((lane >> 2) ^ (r2 & 7)) << 4) + (lane & 3) * 4) = lo;
+          }
+          if (lane == 0) ctl.cq[n & 3][j] = p.qscale * __uint_as_float((uint32_t)(e + 127) << 23);
+        }
+      } else {
+        constexpr int WPR = DIM / 8;  // 16-byte words per row
+        for (int i = lane; i < ncol * WPR; i += 32) {
+          const int j = i / WPR, k = i - j * WPR;
+          int tt;
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(p.q + query_row(p, s.b, h, col0 + j, &tt) * DIM) + k);
+          *reinterpret_cast<uint4*>(qb + (k >> 3) * C::QBOX + j * 128 + (((k & 7) ^ (j & 7)) << 4)) = v;
+        }
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl.q_full[n & 1]);
+    }
+    __syncwarp();
+  } else if (warp == W_SCALE) {
+    // ------------------------------------------------------------------ e4m3: scale bytes, four tiles at a time
+    if constexpr (FP8) {
+      Walk w;
+      w.init(pre, p.rows, per_row, c0, c1);
+      Seg s{};
+      w.next(s);
+      int t = s.t0;
+      for (int i0 = 0; i0 < tiles; i0 += 4) {
+        int64_t at[4];
+        int id[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          at[k] = -1;
+          id[k] = 0;
+          if (i0 + k >= tiles) continue;
+          const int key = t * BN + 4 * lane;  // this lane's four keys: within one page
+          if (key < need_of(s.b)) {
+            const int pi = p.page_shift >= 0 ? key >> p.page_shift : key / p.c.page;
+            id[k] = __ldg(p.table + (int64_t)s.b * p.table_stride + pi);
+            at[k] = (int64_t)(s.u / p.chunks) * p.c.page + (key - pi * p.c.page);
+          }
+          if (++t >= s.t1 && w.next(s)) t = s.t0;
+        }
+        uint32_t kk[4], vv[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          kk[k] = vv[k] = 0x7f7f7f7fu;
+          if (at[k] >= 0) {
+            if (id[k] < 0 || id[k] >= (int)p.c.pages) id[k] = 0;
+            const int64_t o = at[k] + (int64_t)id[k] * p.c.kv_heads * p.c.page;
+            kk[k] = __ldg(reinterpret_cast<const uint32_t*>(p.c.k_scale + o));
+            vv[k] = __ldg(reinterpret_cast<const uint32_t*>(p.c.v_scale + o));
+          }
+        }
+        bool ok = true;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int i = i0 + k;
+          if (i >= tiles || !ok) break;
+          const int st = i % kScaleStages;
+          if (lane == 0) ok = i < kScaleStages || wait(&ctl.sc_empty[st], (i / kScaleStages - 1) & 1);
+          ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+          if (!ok) break;
+          uint32_t* dst = reinterpret_cast<uint32_t*>(smem + C::SC_OFF + st * 2 * BN);
+          dst[lane] = kk[k];
+          dst[32 + lane] = vv[k];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl.sc_full[st]);
+        }
+        if (!ok) break;
+      }
+    }
+    __syncwarp();
+  } else if (warp < 4) {
+    // ------------------------------------------------------------------ softmax: thread = key of the tile
+    const uint32_t lane_off = (uint32_t)(32 * warp) << 16;
+    Walk w;
+    w.init(pre, p.rows, per_row, c0, c1);
+    Seg s{};
+    int i = 0;
+    bool quit = false;
+    for (int n = 0; !quit && w.next(s); ++n) {
+      const int need = need_of(s.b);
+      const int h = s.u / p.chunks, col0 = (s.u - h * p.chunks) * p.chunk_cols;
+      const int ncol = min(p.chunk_cols, p.cols - col0);
+      float m[NQT], l[NQT], cq[NQT];
+      int lim[NQT];
+      {
+        int tt = col0 / p.group, g = col0 - tt * p.group;
+#pragma unroll
+        for (int j = 0; j < NQT; ++j) {
+          lim[j] = j < ncol ? min(need, len[s.b] + tt) : 0;
+          if (++g == p.group) {
+            g = 0;
+            ++tt;
+          }
+          m[j] = 0.f;
+          l[j] = 0.f;
+          cq[j] = p.qscale;
+        }
+      }
+      for (int t = s.t0; t < s.t1; ++t, ++i) {
+        const int b = i & 1;
+        const bool first = t == s.t0;
+        const int key = t * BN + tid;
+        wait(&ctl.s_full[b], (i >> 1) & 1);
+        float ks = 1.f, ev = 0.f, iv = 1.f;
+        if constexpr (FP8) {
+          const int st = i % kScaleStages;
+          wait(&ctl.sc_full[st], (i / kScaleStages) & 1);
+          const unsigned char* sc = smem + C::SC_OFF + st * 2 * BN;
+          ks = __uint_as_float((uint32_t)sc[tid] << 23);
+          const int eb = sc[BN + tid];
+          ev = (float)(eb - 127);
+          iv = __uint_as_float((uint32_t)(254 - eb) << 23);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl.sc_empty[st]);
+          if (first) {
+#pragma unroll
+            for (int j = 0; j < NQT; ++j) cq[j] = ctl.cq[n & 3][j];
+          }
+        }
+        tc_fence_after();
+        __syncwarp();
+        float sv[N];
+#pragma unroll
+        for (int c = 0; c < N / 16; ++c) tmem_ld16(tbase + lane_off + b * N + c * 16, sv + c * 16);
+        tc_fence_before();
+        mbar_arrive(&ctl.s_free[b]);
+        float x[NQT];
+        bool over = FP8 && first;
+#pragma unroll
+        for (int j = 0; j < NQT; ++j) {
+          if constexpr (FP8) {
+            const float raw = fmaf(sv[NQT + j], 0.0625f, sv[j]);
+            x[j] = key < lim[j] ? fmaf(raw * ks, cq[j], ev) : -INFINITY;
+            if (!first) over |= x[j] > m[j] + kRaise;
+          } else {
+            x[j] = key < lim[j] ? sv[j] * p.qscale : -INFINITY;
+            over |= x[j] > m[j] + kRaise;
+            if (first) over |= x[j] > -INFINITY && x[j] < m[j] - kBelow;
+          }
+        }
+        const bool saw = abort_flag != 0;
+        if (sync_or(1, 128, over || saw)) {
+          float v[NQT];
+#pragma unroll
+          for (int j = 0; j < NQT; ++j) v[j] = x[j];
+          warp_all<NQT, true>(v);
+          if (lane == 0) {
+#pragma unroll
+            for (int j = 0; j < NQT; ++j) ctl.red[warp][j] = v[j];
+          }
+          if (sync_or(1, 128, saw)) {
+            quit = true;
+            break;
+          }
+          float scl[NQT];
+          bool any = false;
+#pragma unroll
+          for (int j = 0; j < NQT; ++j) {
+            const float top = fmaxf(fmaxf(ctl.red[0][j], ctl.red[1][j]), fmaxf(ctl.red[2][j], ctl.red[3][j]));
+            float mn = m[j];
+            if (top != -INFINITY) {
+              if (FP8) mn = first ? top - kHead8 : (top > m[j] + kRaise ? top - kHead8 : m[j]);
+              else mn = first ? top : fmaxf(m[j], top);
+            }
+            scl[j] = first ? 1.f : ex2(m[j] - mn);
+            any |= scl[j] != 1.f;
+            m[j] = mn;
+            l[j] *= scl[j];
+          }
+          if (any && !first) {  // the same in every thread: the maxima are
+            wait(&ctl.pv_done[b ^ 1], ((i - 1) >> 1) & 1);  // O holds every earlier tile of the unit
+            tc_fence_after();
+            __syncwarp();
+#pragma unroll 1
+            for (int c = 0; c < DC; ++c) {
+              const uint32_t o = tbase + lane_off + C::S_COLS + ((n & 1) * DC + c) * N;
+              float ov[N];
+#pragma unroll
+              for (int k = 0; k < N / 16; ++k) tmem_ld16(o + k * 16, ov + k * 16);
+#pragma unroll
+              for (int j = 0; j < NQT; ++j) {
+                ov[j] *= scl[j];
+                if (FP8) ov[NQT + j] *= scl[j];
+              }
+#pragma unroll
+              for (int k = 0; k < N / 16; ++k) tmem_st16(o + k * 16, ov + k * 16);
+            }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          }
+          named_sync(1, 128);  // the maxima are read before the next tile writes them
+        }
+        float pr[NQT];
+#pragma unroll
+        for (int j = 0; j < NQT; ++j) {
+          pr[j] = ex2(x[j] - m[j]);
+          l[j] = FP8 ? fmaf(pr[j], iv, l[j]) : l[j] + pr[j];
+        }
+        if (i >= 2) wait(&ctl.pv_done[b], ((i >> 1) - 1) & 1);  // P(i - 2) is used up
+        unsigned char* pb = smem + C::P_OFF + b * C::PB;
+        if constexpr (FP8) {
+          uint32_t hw[NQT >= 4 ? NQT / 4 : 1], lw[NQT >= 4 ? NQT / 4 : 1];
+#pragma unroll
+          for (int k = 0; k < (NQT >= 4 ? NQT / 4 : 1); ++k) hw[k] = lw[k] = 0u;
+#pragma unroll
+          for (int j = 0; j < NQT; j += 2) {
+            const float p0 = pr[j], p1 = j + 1 < NQT ? pr[j + 1 < NQT ? j + 1 : j] : 0.f;
+            const uint32_t a = __nv_cvt_float2_to_fp8x2(make_float2(p0, p1), __NV_SATFINITE, __NV_E4M3);
+            const __half2_raw hr = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)a, __NV_E4M3);
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hr));
+            const uint32_t r =
+                __nv_cvt_float2_to_fp8x2(make_float2((p0 - f.x) * 16.f, (p1 - f.y) * 16.f), __NV_SATFINITE, __NV_E4M3);
+            hw[j >> 2] |= a << (8 * (j & 3));
+            lw[j >> 2] |= r << (8 * (j & 3));
+          }
+          // Columns 0 .. NQT - 1 the first pieces, NQT .. 2 NQT - 1 the second, zeros after them.
+          uint4 w0, w1 = make_uint4(0u, 0u, 0u, 0u);
+          if constexpr (NQT == 16) {
+            w0 = make_uint4(hw[0], hw[1], hw[2], hw[3]);
+            w1 = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+          } else if constexpr (NQT == 8) {
+            w0 = make_uint4(hw[0], hw[1], lw[0], lw[1]);
+          } else if constexpr (NQT == 4) {
+            w0 = make_uint4(hw[0], lw[0], 0u, 0u);
+          } else if constexpr (NQT == 2) {
+            w0 = make_uint4((hw[0] & 0xffffu) | (lw[0] << 16), 0u, 0u, 0u);
+          } else {
+            w0 = make_uint4((hw[0] & 0xffu) | ((lw[0] & 0xffu) << 8), 0u, 0u, 0u);
+          }
+          *reinterpret_cast<uint4*>(pb + tid * 16) = w0;
+          if constexpr (N == 32) *reinterpret_cast<uint4*>(pb + 2048 + tid * 16) = w1;
+        } else {
+          uint32_t wv[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float lo = 2 * k < NQT ? pr[2 * k < NQT ? 2 * k : 0] : 0.f;
+            const float hi = 2 * k + 1 < NQT ? pr[2 * k + 1 < NQT ? 2 * k + 1 : 0] : 0.f;
+            const __nv_bfloat162 v2 = __floats2bfloat162_rn(lo, hi);
+            wv[k] = *reinterpret_cast<const uint32_t*>(&v2);
+          }
+          *reinterpret_cast<uint4*>(pb + tid * 16) = make_uint4(wv[0], wv[1], wv[2], wv[3]);
+          *reinterpret_cast<uint4*>(pb + 2048 + tid * 16) = make_uint4(wv[4], wv[5], wv[6], wv[7]);
+        }
+        if (t * BN + BN > need) {
+          // The row's last tile: V rows past its keys may hold anything, and 0 x NaN is NaN. Cleared once loaded (the
+          // producer has issued the chunk, so the slot's phase is the chunk's).
+          const int vc = v_chunk(i);
+          for (int c = 0; c < DC; ++c) {
+            const uint64_t t_start = global_ns();
+            while (issued <= vc + c) {
+              if (abort_flag) break;
+              if (global_ns() - t_start > kWaitLimitNs) {
+                abort_flag = 1;
+                break;
+              }
+            }
+            if (abort_flag) break;
+            wait(&ctl.full[(vc + c) % SLOTS], ((vc + c) / SLOTS) & 1);
+            if (key >= need) {
+              unsigned char* row = smem + ((vc + c) % SLOTS) * SLOT + tid * 128;
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+#pragma unroll
+                for (int x2 = 0; x2 < NB; ++x2) *reinterpret_cast<uint4*>(row + x2 * kBox + k * 16) = make_uint4(0u, 0u, 0u, 0u);
+              }
+            }
+          }
+        }
+        fence_async_smem();
+        tc_fence_before();
+        mbar_arrive(&ctl.p_full[b]);
+      }
+      if (quit) break;
+      // The segment's sums and maxima, once the epilogue has read those of two segments before.
+      if (n >= 2) wait(&ctl.o_free[n & 1], ((n >> 1) - 1) & 1);
+      warp_all<NQT, false>(l);
+      if (lane == 0) {
+#pragma unroll
+        for (int j = 0; j < NQT; ++j) ctl.sum[n & 1][warp][j] = l[j];
+      }
+      if (tid == 0) {
+#pragma unroll
+        for (int j = 0; j < NQT; ++j) ctl.top[n & 1][j] = m[j];
+      }
+      mbar_arrive(&ctl.ml_full[n & 1]);
+    }
+  } else {
+    // ------------------------------------------------------------------ epilogue: thread = head dim of each chunk
+    const int d = tid - W_EPI * 32;
+    const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
+    Walk w;
+    w.init(pre, p.rows, per_row, c0, c1);
+    Seg s{};
+    for (int n = 0; w.next(s); ++n) {
+      wait(&ctl.o_full[n & 1], (n >> 1) & 1);
+      wait(&ctl.ml_full[n & 1], (n >> 1) & 1);
+      if (sync_or(2, 128, abort_flag != 0)) break;  // all of these warps leave together
+      tc_fence_after();
+      const int h = s.u / p.chunks, col0 = (s.u - h * p.chunks) * p.chunk_cols;
+      const int ncol = min(p.chunk_cols, p.cols - col0);
+      float l[NQT], m[NQT];
+#pragma unroll
+      for (int j = 0; j < NQT; ++j) {
+        l[j] = (ctl.sum[n & 1][0][j] + ctl.sum[n & 1][1][j]) + (ctl.sum[n & 1][2][j] + ctl.sum[n & 1][3][j]);
+        m[j] = ctl.top[n & 1][j];
+      }
+      unsigned bad = 0;  // columns with a result that is not finite
+      auto store = [&](int c, const float (&o)[NQT], const float (&sum)[NQT]) {
+        int tt = col0 / p.group, g = col0 - tt * p.group;
+#pragma unroll
+        for (int j = 0; j < NQT; ++j) {
+          if (j < ncol) {
+            const int64_t row = ((int64_t)s.b * p.tokens + tt) * p.heads + h * p.group + g;
+            const float r = o[j] * (sum[j] != 0.f ? 1.f / sum[j] : 0.f);
+            if (!(fabsf(r) <= 3.3e38f)) bad |= 1u << j;
+            p.out[row * DIM + c * 128 + d] = __float2bfloat16_rn(r);
+          }
+          if (++g == p.group) {
+            g = 0;
+            ++tt;
+          }
+        }
+      };
+      const int f0 = s.first / per, f1 = (s.first + s.nt - 1) / per;  // the unit's first and last CTA
+      bool emit = f0 == f1;
+      const int64_t at = ((int64_t)2 * blockIdx.x + ((int)blockIdx.x == f0 ? 1 : 0)) * kMaxCols;
+#pragma unroll 1
+      for (int c = 0; c < DC; ++c) {
+        float v[N], o[NQT];
+#pragma unroll
+        for (int k = 0; k < N / 16; ++k) tmem_ld16(tbase + lane_off + C::S_COLS + ((n & 1) * DC + c) * N + k * 16, v + k * 16);
+        if (c == DC - 1) {
+          tc_fence_before();
+          mbar_arrive(&ctl.o_free[n & 1]);
+        }
+#pragma unroll
+        for (int j = 0; j < NQT; ++j) o[j] = FP8 ? fmaf(v[NQT + j], 0.0625f, v[j]) : v[j];
+        if (emit) {
+          store(c, o, l);
+        } else {
+#pragma unroll
+          for (int j = 0; j < NQT; ++j)
+            if (j < ncol) p.part_o[(at + j) * DIM + c * 128 + d] = o[j];
+        }
+      }
+      if (!emit) {
+        if (d == 0) {
+#pragma unroll
+          for (int j = 0; j < NQT; ++j)
+            if (j < ncol) p.part_ml[at + j] = make_float2(m[j], l[j]);
+        }
+        __threadfence();
+        named_sync(2, 128);  // every thread's part is out before the count
+        if (d == 0) {
+          const unsigned before = atomicAdd(p.counters + f0, 1u);
+          const bool last = before == (unsigned)(f1 - f0);
+          if (last) p.counters[f0] = 0;  // zero again for the next call
+          ctl.last = last;
+        }
+        named_sync(2, 128);
+        emit = ctl.last != 0;
+        if (emit) {
+          __threadfence();
+          // Joined in the order of the keys, whichever CTA came last.
+#pragma unroll 1
+          for (int c = 0; c < DC; ++c) {
+            float o[NQT];
+#pragma unroll
+            for (int j = 0; j < NQT; ++j) {
+              m[j] = -INFINITY;
+              l[j] = o[j] = 0.f;
+            }
+#pragma unroll 2
+            for (int f = f0; f <= f1; ++f) {
+              const int64_t src = ((int64_t)2 * f + (f == f0 ? 1 : 0)) * kMaxCols;
+              float2 e[NQT];
+              float v[NQT];
+#pragma unroll
+              for (int j = 0; j < NQT; ++j) {
+                e[j] = j < ncol ? __ldcg(p.part_ml + src + j) : make_float2(0.f, 0.f);
+                v[j] = j < ncol ? __ldcg(p.part_o + (src + j) * DIM + c * 128 + d) : 0.f;
+              }
+#pragma unroll
+              for (int j = 0; j < NQT; ++j) {
+                if (e[j].y != 0.f) {  // a part that saw no key takes no part
+                  const float mn = fmaxf(m[j], e[j].x);
+                  const float a = ex2(m[j] - mn), b = ex2(e[j].x - mn);
+                  l[j] = fmaf(l[j], a, e[j].y * b);
+                  m[j] = mn;
+                  o[j] = fmaf(o[j], a, v[j] * b);
+                }
+              }
+            }
+            store(c, o, l);
+          }
+        }
+      }
+      if (emit) {
+        if (p.tokens > 1) {  // a column may have met a key it does not see
+          if (sync_or(2, 128, bad != 0)) {
+            if (bad) atomicOr(&ctl.bad, bad);
+            named_sync(2, 128);
+            const unsigned all = *(volatile unsigned*)&ctl.bad;
+            for (int j = warp - W_EPI; j < ncol; j += 4) {
+              if (!(all >> j & 1)) continue;
+              int t2;
+              const int64_t row = query_row(p, s.b, h, col0 + j, &t2);
+              exact_column<FP8, DIM>(p.q + row * DIM, p.c, p.table + (int64_t)s.b * p.table_stride, h,
+                                     min(need_of(s.b), len[s.b] + t2), p.qscale, p.out + row * DIM);
+            }
+            named_sync(2, 128);
+            if (d == 0) ctl.bad = 0;
+            named_sync(2, 128);
+          }
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (abort_flag) {
+    if (tid == 0) raise_status(p.status, kStatusTimeout);
+    if (tid == W_MMA * 32) {
+      tc_commit(&ctl.drain);  // every MMA issued has completed once this arrives
+      mbar_wait(&ctl.drain, 0);
+    }
+    if (tid == W_LOAD * 32)  // the latest load of every slot lands before the shared memory goes away
+      for (int i = issued > SLOTS ? issued - SLOTS : 0; i < issued; ++i) mbar_wait(&ctl.full[i % SLOTS], (i / SLOTS) & 1);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == W_EPI) {
+    tc_fence_after();
+    tmem_dealloc(tbase, C::TMEM);
+  }
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      return (PFN_cuTensorMapEncodeTiled_v12000) nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+  }();
+  return fn;
+}
+
+bool page_map(CUtensorMap* map, const void* base, const PageCache& c) {
+  const auto fn = encode_fn();
+  if (!fn) return false;
+  const bool fp8 = c.type == kFp8;
+  const uint64_t es = fp8 ? 1 : 2;
+  // An extent of one has a stride that nothing reads.
+  auto st = [&](int64_t extent, int64_t stride) { return (cuuint64_t)(extent > 1 ? stride * es : 16); };
+  const cuuint64_t dims[4] = {(cuuint64_t)c.dim, (cuuint64_t)c.page, (cuuint64_t)c.kv_heads, (cuuint64_t)c.pages};
+  const cuuint64_t strides[3] = {st(c.page, c.s_pos), st(c.kv_heads, c.s_head), st(c.pages, c.s_page)};
+  const cuuint32_t box[4] = {(cuuint32_t)(fp8 ? 128 : 64), (cuuint32_t)(c.page < BN ? c.page : BN), 1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  if (!strides[0] || !strides[1] || !strides[2]) return false;
+  return fn(map, fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides,
+            box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool FP8, int DIM, int NQT>
+cudaError_t launch_t(const CUtensorMap& k, const CUtensorMap& v, const Params& p, int grid, cudaStream_t stream) {
+  using C = Cfg<FP8, DIM, NQT>;
+  static bool configured = false;
+  if (!configured) {
+    cudaError_t e = cudaFuncSetAttribute(paged_tc_kernel<FP8, DIM, NQT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES);
+    if (e != cudaSuccess) return e;
+    configured = true;
+  }
+  return launch_dependent(paged_tc_kernel<FP8, DIM, NQT>, dim3(grid), dim3(kThreads), (size_t)C::BYTES, stream, k, v, p);
+}
+
+template <bool FP8, int DIM>
+cudaError_t launch_cols(const CUtensorMap& k, const CUtensorMap& v, const Params& p, int grid, cudaStream_t s) {
+  if (p.chunk_cols <= 1) return launch_t<FP8, DIM, 1>(k, v, p, grid, s);
+  if (p.chunk_cols <= 2) return launch_t<FP8, DIM, 2>(k, v, p, grid, s);
+  if (p.chunk_cols <= 4) return launch_t<FP8, DIM, 4>(k, v, p, grid, s);
+  if (p.chunk_cols <= 8) return launch_t<FP8, DIM, 8>(k, v, p, grid, s);
+  return launch_t<FP8, DIM, 16>(k, v, p, grid, s);
+}
+
+template <bool FP8>
+cudaError_t launch_dim(const CUtensorMap& k, const CUtensorMap& v, const Params& p, int grid, cudaStream_t s) {
+  if (p.c.dim == 128) return launch_cols<FP8, 128>(k, v, p, grid, s);
+  if (p.c.dim == 256) return launch_cols<FP8, 256>(k, v, p, grid, s);
+  return launch_cols<FP8, 512>(k, v, p, grid, s);
+}
+
+}  // namespace pagedtc
+
+bool paged_tc_supported(int dtype, int type, int dim, int page) {
+  const bool pages = page >= 128 ? page % 128 == 0 : page >= 8 && (page & (page - 1)) == 0;
+  return dtype == kBF16 && (type == kBF16 || type == kFp8) && (dim == 128 || dim == 256 || dim == 512) && pages;
+}
+
+size_t paged_tc_workspace(int dim) {
+  return kCounterBytes + (size_t)2 * device_sm_count() * pagedtc::kMaxCols * (dim * sizeof(float) + sizeof(float2));
+}
+
+cudaError_t launch_paged_attention_tc(const PagedAttnArgs& a, cudaStream_t stream) {
+  using namespace pagedtc;
+  CUtensorMap km, vm;
+  if (!page_map(&km, a.c.k, a.c) || !page_map(&vm, a.c.v, a.c)) return cudaErrorNotSupported;
+  const int grid = device_sm_count();
+  Params p{};
+  p.c = a.c;
+  p.table_stride = a.table_stride;
+  p.tokens = a.tokens;
+  p.heads = a.heads;
+  p.group = a.heads / a.c.kv_heads;
+  p.cols = a.tokens * p.group;
+  p.chunks = (p.cols + kMaxCols - 1) / kMaxCols;
+  p.chunk_cols = (p.cols + p.chunks - 1) / p.chunks;
+  p.chunks = (p.cols + p.chunk_cols - 1) / p.chunk_cols;
+  p.cap = a.table_width * a.c.page;
+  p.page_shift = -1;
+  if (a.c.page < BN) {
+    p.page_shift = 3;
+    while ((1 << p.page_shift) < a.c.page) ++p.page_shift;
+  }
+  p.qscale = a.scale * kLog2e;
+  p.counters = reinterpret_cast<unsigned*>(a.workspace);
+  char* ws = reinterpret_cast<char*>(a.workspace) + kCounterBytes;
+  p.part_o = reinterpret_cast<float*>(ws);
+  p.part_ml = reinterpret_cast<float2*>(ws + (size_t)2 * grid * kMaxCols * a.c.dim * sizeof(float));
+  p.status = a.status;
+  // Rows per launch: what the shared-memory tables hold, and no more tiles than an int counts.
+  const int64_t row_tiles = ((int64_t)(p.cap + BN - 1) / BN) * p.c.kv_heads * p.chunks;
+  const int most = (int)std::min<int64_t>(kMaxRows, 0x7fffff00ll / std::max<int64_t>(1, row_tiles));
+  if (most < 1) return cudaErrorNotSupported;
+  for (int r0 = 0; r0 < a.rows; r0 += most) {
+    p.rows = std::min(most, a.rows - r0);
+    p.q = reinterpret_cast<const __nv_bfloat16*>(a.q) + (int64_t)r0 * a.tokens * a.heads * a.c.dim;
+    p.out = reinterpret_cast<__nv_bfloat16*>(a.out) + (int64_t)r0 * a.tokens * a.heads * a.c.dim;
+    p.table = a.table + (int64_t)r0 * a.table_stride;
+    p.lengths = a.lengths + r0;
+    const cudaError_t e = a.c.type == kFp8 ? launch_dim<true>(km, vm, p, grid, stream) : launch_dim<false>(km, vm, p, grid, stream);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
+}  // namespace omni

@@ -143,7 +143,7 @@ size_t omniasr_paged_attention_workspace(int dtype, int cache_type, int rows, in
   if (!omni::dim_supported(dtype, dim) || rows < 0 || tokens <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || page <= 0 ||
       table_width < 0)
     return 0;
-  if (omni::paged_tc_supported(dtype, cache_type, dim, page)) return omni::paged_tc_workspace(cache_type, dim);
+  if (omni::paged_tc_supported(dtype, cache_type, dim, page)) return omni::paged_tc_workspace(dim);
   return omni::paged_attention_workspace(dtype, cache_type, rows ? rows : 1, tokens, heads, kv_heads, dim, page, table_width);
 }
 
@@ -156,6 +156,8 @@ int omniasr_paged_attention(const void* q, const void* k_pages, const void* v_pa
   if (int e = check(name, dtype, cache_type, dim, heads, kv_heads)) return e;
   if (rows < 0 || rows > 65535 || tokens <= 0 || table_width < 0)
     return fail(OMNIASR_ERR_ARGUMENT, "%s: %d rows (at most 65535) of %d tokens", name, rows, tokens);
+  if ((int64_t)table_width * page > 0x7fffff00ll)
+    return fail(OMNIASR_ERR_ARGUMENT, "%s: %d pages of %d positions per row", name, table_width, page);
   if ((int64_t)tokens * heads > 65535)
     return fail(OMNIASR_ERR_ARGUMENT, "%s: %d tokens x %d heads per row (at most 65535)", name, tokens, heads);
   omni::PagedAttnArgs a;
@@ -179,7 +181,13 @@ int omniasr_paged_attention(const void* q, const void* k_pages, const void* v_pa
   a.scale = scale;
   a.workspace = workspace;
   a.status = status;
-  if (omni::paged_tc_supported(dtype, cache_type, dim, page)) return done(name, omni::launch_paged_attention_tc(a, stream));
+  if (omni::paged_tc_supported(dtype, cache_type, dim, page)) {
+    const cudaError_t e = omni::launch_paged_attention_tc(a, stream);
+    if (e == cudaErrorNotSupported)
+      return fail(OMNIASR_ERR_UNSUPPORTED, "%s: page strides (%lld, %lld, %lld), or rows of that many keys", name,
+                  (long long)stride_page, (long long)stride_head, (long long)stride_pos);
+    return done(name, e);
+  }
   return done(name, omni::launch_paged_attention(dtype, a, stream));
 }
 
