@@ -10,8 +10,10 @@
 //   S^T [128 keys x N]  = K [128 x D] Q^T            accumulated over 128-dim chunks
 //   P^T = 2^(S^T scale log2e - m)                      one thread per key, m raised only when passed by 2^8
 //   O^T [D x N]        += V^T [D x 128 keys] P^T       accumulated in TMEM over the unit's tiles
-// K and V chunks stream through one ring of shared-memory slots in the order the MMAs use them (K of tile t + 1 before V of
-// tile t), filled by TMA page by page.
+// K and V chunks stream through one ring of shared-memory slots in the order the MMAs use them (K of tile t + 2 before V of
+// tile t), filled by TMA page by page. Two groups of softmax warps take the tiles in turn, each with a maximum, sums and an
+// O of its own (the epilogue adds the two up), so that neither waits for the other: with one group, a tile of e4m3 keys took
+// 1.1 us to its softmax and 0.75 us to HBM.
 //
 // e4m3 pages are fed to the tensor core as they are (kind::f8f6f4), at half the bytes of bf16; the query and the
 // probabilities become two e4m3 pieces each, in columns of their own: q = 2^e (q1 + q2 / 16), q1 = rn(q 2^-e), q2 =
@@ -42,6 +44,7 @@ constexpr int kMaxCols = 16;       // query columns per unit
 constexpr int kMaxRows = 1024;     // rows of one launch
 constexpr int kBox = BN * 128;     // 128 keys x 128 bytes
 constexpr int kScaleStages = 8;    // tiles of scale bytes in shared memory
+constexpr int kCtlBytes = 3072;    // control block (below)
 constexpr float kRaise = 8.f;      // log2: a weight may reach 2^8 before its column's maximum is raised
 constexpr float kHead8 = 4.f;      // e4m3: the maximum kept this far (log2) below the largest exponent seen
 constexpr float kBelow = 64.f;     // bf16: a unit starts from maximum 0 unless its scores lie 2^64 below
@@ -55,7 +58,7 @@ struct Cfg {
   static constexpr int QB = DC * (FP8 ? 1 : 2) * QBOX;     // one query buffer
   static constexpr int PB = BN * N * (FP8 ? 1 : 2);        // one P buffer
   static constexpr int FIXED = 2 * QB + 2 * PB + 2 * kMaxRows * 4 + 64 + (FP8 ? kScaleStages * 2 * BN : 0);
-  static constexpr int FIT = (232448 - 2048 - 1024 - FIXED) / SLOT;
+  static constexpr int FIT = (232448 - kCtlBytes - 1024 - FIXED) / SLOT;
   static constexpr int SLOTS = FIT > 12 ? 12 : FIT;
   static constexpr int Q_OFF = SLOTS * SLOT;
   static constexpr int P_OFF = Q_OFF + 2 * QB;
@@ -63,15 +66,16 @@ struct Cfg {
   static constexpr int PRE_OFF = SC_OFF + (FP8 ? kScaleStages * 2 * BN : 0);  // int [rows + 1]: tiles before a row
   static constexpr int LEN_OFF = PRE_OFF + (kMaxRows + 16) * 4;               // int [rows]
   static constexpr int BYTES = LEN_OFF + kMaxRows * 4 + 1024;                 // + alignment slack
-  static constexpr uint32_t S_COLS = 2 * N;
-  static constexpr uint32_t COLS = S_COLS + 2 * DC * N;
+  static constexpr uint32_t S_COLS = 2 * N;                  // S^T of either softmax group
+  static constexpr int OB = S_COLS + 4 * DC * N <= 512 ? 2 : 1;  // O^T buffers (units in turn), per softmax group
+  static constexpr uint32_t COLS = S_COLS + 2 * OB * DC * N;
   static constexpr uint32_t TMEM = COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
   static_assert(SLOTS >= DC, "a tile's V chunks are all resident when its stale rows are cleared");
-  static_assert(BYTES + 2048 <= 232448, "shared memory per block");
+  static_assert(BYTES + kCtlBytes <= 232448, "shared memory per block");
 };
 
-constexpr int kThreads = 384;
-constexpr int W_LOAD = 4, W_MMA = 5, W_Q = 6, W_SCALE = 7, W_EPI = 8;
+constexpr int kThreads = 512;
+constexpr int W_LOAD = 4, W_MMA = 5, W_Q = 6, W_SCALE = 7, W_EPI = 8, W_SOFT1 = 12;  // softmax: warps 0-3 and 12-15
 
 struct Params {
   const __nv_bfloat16* q;
@@ -184,20 +188,21 @@ struct Walk {
 
 struct alignas(16) Ctl {
   uint64_t full[12], empty[12];
-  uint64_t s_full[2], s_free[2], p_full[2], pv_done[2], q_full[2], q_empty[2], o_full[2], o_free[2], ml_full[2];
+  uint64_t s_full[2], s_free[2], p_full[2], pv_done[2], q_full[2], q_empty[2], o_full[2], o_free[2], ml_full[2], ml_free[2];
   uint64_t sc_full[kScaleStages], sc_empty[kScaleStages];
   uint64_t drain;
-  float red[4][kMaxCols];         // column maxima per softmax warp
-  float sum[2][4][kMaxCols];      // a finished segment's column sums per softmax warp
-  float top[2][kMaxCols];         // ... and maxima
+  float red[2][4][kMaxCols];      // [softmax group][warp]: column maxima
+  float sum[2][2][4][kMaxCols];   // [segment parity][softmax group][warp]: a finished segment's column sums
+  float top[2][2][kMaxCols];      // ... and maxima
   float cq[4][kMaxCols];          // score factor per column (scale, log2e, the query's exponent)
   int wsum[kThreads / 32];
   uint32_t tmem_base;
-  int abort_flag, issued;         // chunks the producer has issued
+  int abort_flag;
+  int loads[12];                  // loads issued into each ring slot
   int last;                       // epilogue: this CTA joins the unit
   unsigned bad;                   // epilogue: columns to redo
 };
-static_assert(sizeof(Ctl) <= 2048, "control block");
+static_assert(sizeof(Ctl) <= kCtlBytes, "control block");
 
 // The query row and the keys that column `col` of row b, kv head h sees.
 OMNI_DEV int64_t query_row(const Params& p, int b, int h, int col, int* t) {
@@ -268,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   int* pre = reinterpret_cast<int*>(smem + C::PRE_OFF);
   int* len = reinterpret_cast<int*>(smem + C::LEN_OFF);
   volatile int& abort_flag = ctl.abort_flag;
-  volatile int& issued = ctl.issued;
+  volatile int* loads = ctl.loads;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
@@ -285,7 +290,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&ctl.q_empty[s], 1);
       mbar_init(&ctl.o_full[s], 1);
       mbar_init(&ctl.o_free[s], 128);
-      mbar_init(&ctl.ml_full[s], 128);
+      mbar_init(&ctl.ml_full[s], 256);
+      mbar_init(&ctl.ml_free[s], 128);
     }
     for (int s = 0; s < kScaleStages; ++s) {
       mbar_init(&ctl.sc_full[s], 1);
@@ -294,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&ctl.drain, 1);
     mbar_fence_init();
     abort_flag = 0;
-    issued = 0;
+    for (int s = 0; s < 12; ++s) loads[s] = 0;
     ctl.bad = 0;
   }
   if (warp == W_EPI) tmem_alloc(&ctl.tmem_base, C::TMEM);
@@ -352,9 +358,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     abort_flag = 1;
     return false;
   };
+  // Until `uses` loads into the slot have been issued: a wait on the slot's barriers, whose parity tells one phase from the
+  // next only, may then be made for that many uses.
+  auto wait_issued = [&](int slot, int uses) -> bool {
+    if (loads[slot] >= uses) return true;
+    const uint64_t t_start = global_ns();
+    while (loads[slot] < uses) {
+      if (abort_flag || global_ns() - t_start > kWaitLimitNs) {
+        abort_flag = 1;
+        return false;
+      }
+    }
+    return true;
+  };
   auto need_of = [&](int b) { return min(p.cap, len[b] + p.tokens - 1); };  // of a row that has tiles
-  // Ring position of tile i's first V chunk (K and V chunks in the MMAs' order: K0 K1 V0 K2 V1 .. V(n-1)).
-  auto v_chunk = [&](int i) { return DC * (i == tiles - 1 ? 2 * i + 1 : 2 * i + 2); };
+  // Ring positions of tile i's first K and V chunk, in the MMAs' order: K0 K1 K2 V0 K3 V1 .. K(n-1) V(n-3) V(n-2) V(n-1).
+  auto k_chunk = [&](int i) { return DC * (i < 2 ? i : 2 * i - 2); };
+  auto v_chunk = [&](int i) { return DC * min(2 * i + 3, tiles + i); };
 
   if (warp == W_SCALE) {  // the rows without keys: zeros, by this warp of every CTA
     for (int b = blockIdx.x; b < p.rows; b += gridDim.x) {
@@ -366,9 +386,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (tiles <= 0) {
     // nothing but giving the TMEM back
-  } else if (warp == W_LOAD) {
+  } else if (warp == W_LOAD || (!FP8 && warp == W_SCALE)) {
     // ------------------------------------------------------------------ K and V, page by page
-    // Lane i holds the tile's i-th page (the only one, for pages of 128 positions and more), loaded a tile ahead.
+    // Lane i holds the tile's i-th page (the only one, for pages of 128 positions and more), loaded a tile ahead. bf16: one
+    // warp loads K, one V (a box costs its warp about 50 ns to issue, which small pages would wait for); e4m3: one warp
+    // both, as the other loads the scale bytes and boxes are half as many.
+    const bool do_k = warp == W_LOAD, do_v = FP8 || warp == W_SCALE;
     const bool small = p.page_shift >= 0;
     const int rows_box = small ? p.c.page : BN;
     const int boxes = small ? BN >> p.page_shift : 1;
@@ -396,13 +419,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       return true;
     };
-    int chunk = 0;
-    auto load = [&](const CUtensorMap* map, const Tile& x) -> bool {
+    auto load = [&](const CUtensorMap* map, const Tile& x, int chunk) -> bool {
       for (int c = 0; c < DC; ++c, ++chunk) {
         const int slot = chunk % SLOTS, use = chunk / SLOTS;
         bool ok = true;
         if (lane == 0) {
-          ok = use < 1 || wait(&ctl.empty[slot], (use - 1) & 1);
+          // The slot's load before this one may be the other warp's.
+          ok = use < 1 || (wait_issued(slot, use) && wait(&ctl.empty[slot], (use - 1) & 1));
           if (ok) mbar_arrive_expect_tx(&ctl.full[slot], (uint32_t)(x.live * rows_box * 128 * NB));
         }
         if (!__shfl_sync(0xffffffffu, ok ? 1 : 0, 0)) return false;
@@ -413,31 +436,33 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma_load_4d(dst + x2 * kBox, map, c * 128 + x2 * 64, x.row, x.h, x.id, &ctl.full[slot]);
         }
         __syncwarp();
-        if (lane == 0) issued = chunk + 1;
+        if (lane == 0) loads[slot] = use + 1;
       }
       return true;
     };
     w.next(s);
     t = s.t0;
-    Tile cur, nxt, prev;
+    Tile cur, nxt, prev, prev2;
     fetch(cur);
-    prev = cur;
-    for (int i = 0; i < tiles; ++i) {
-      if (cur.id < 0 || cur.id >= (int)p.c.pages) {
-        raise_status(p.status, kStatusIndex);
-        cur.id = 0;
+    prev = prev2 = nxt = cur;
+    // V follows K by two tiles (the ring's order), also in a warp that loads V alone.
+    for (int i = 0; i < tiles + 2; ++i) {
+      if (i < tiles) {
+        if (cur.id < 0 || cur.id >= (int)p.c.pages) {
+          raise_status(p.status, kStatusIndex);
+          cur.id = 0;
+        }
+        if (step()) fetch(nxt);
+        if (do_k && !load(&kmap, cur, k_chunk(i))) break;
       }
-      const bool more = step();
-      if (more) fetch(nxt);
-      if (!load(&kmap, cur)) break;
-      if (i > 0 && !load(&vmap, prev)) break;
+      if (do_v && i >= 2 && !load(&vmap, prev2, v_chunk(i - 2))) break;
+      prev2 = prev;
       prev = cur;
-      if (more) cur = nxt;
-      if (i == tiles - 1) load(&vmap, prev);
+      cur = nxt;
     }
     __syncwarp();
   } else if (warp == W_MMA) {
-    // ------------------------------------------------------------------ S^T(i), then O^T += V(i-1)^T P(i-1)^T
+    // ------------------------------------------------------------------ S^T(i), then O^T += V(i-2)^T P(i-2)^T
     if (lane == 0) {
       constexpr uint32_t IS = FP8 ? idesc_e4m3(128, N, 0, 0) : idesc_bf16(128, N, 0, 0);
       constexpr uint32_t IO = FP8 ? idesc_e4m3(128, N, 1, 1) : idesc_bf16(128, N, 1, 1);
@@ -445,35 +470,40 @@ __global__ void __launch_bounds__(kThreads, 1)
       Walk w;
       w.init(pre, p.rows, per_row, c0, c1);
       Seg s{};
-      int chunk = 0, i = 0, nseg = 0;
-      // The tile whose O^T is to issue: its segment's number, whether it is the segment's first / last tile.
-      int pi = -1, pseg = 0;
-      bool pfirst = false, plast = false, ok = true;
-      auto values = [&]() -> bool {
-        const int b = pi & 1;
-        if (pfirst && pseg >= 2 && !wait(&ctl.o_free[pseg & 1], (pseg / 2 - 1) & 1)) return false;
-        if (!wait(&ctl.p_full[b], (pi >> 1) & 1)) return false;
+      int i = 0, nseg = 0;
+      bool ok = true;
+      // A tile whose O^T is to issue: its number and its segment's, its place among the segment's tiles.
+      struct Pending {
+        int i, seg;
+        bool first, fresh, last;  // the segment's first tile; the first of its softmax group; the last
+      } pend[2];
+      pend[0].i = pend[1].i = -1;
+      auto values = [&](const Pending& x) -> bool {
+        const int b = x.i & 1, ob = C::OB == 2 ? x.seg & 1 : 0;
+        if (x.first && x.seg >= C::OB && !wait(&ctl.o_free[ob], (x.seg / C::OB - 1) & 1)) return false;
+        if (!wait(&ctl.p_full[b], (x.i >> 1) & 1)) return false;
+        int chunk = v_chunk(x.i);
         for (int c = 0; c < DC; ++c, ++chunk) {
           const int slot = chunk % SLOTS;
           if (!wait(&ctl.full[slot], (chunk / SLOTS) & 1)) return false;
           tc_fence_after();
           const uint32_t va = ring + slot * SLOT, pa = pbase + b * C::PB;
-          const uint32_t d = tbase + C::S_COLS + ((pseg & 1) * DC + c) * N;
+          const uint32_t d = tbase + C::S_COLS + ((ob * 2 + b) * DC + c) * N;
           if constexpr (FP8) {
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
               mma_f8_ss(d, smem_desc(va + kk * 4096, kBox, 1024, kLayoutSw128), smem_desc(pa + kk * 512, 128, 2048, kLayoutNone),
-                        IO, (pfirst && kk == 0) ? 0u : 1u);
+                        IO, (x.fresh && kk == 0) ? 0u : 1u);
           } else {
 #pragma unroll
             for (int kk = 0; kk < 8; ++kk)
               mma_bf16_ss(d, smem_desc(va + kk * 2048, kBox, 1024, kLayoutSw128), smem_desc(pa + kk * 256, 128, 2048, kLayoutNone),
-                          IO, (pfirst && kk == 0) ? 0u : 1u);
+                          IO, (x.fresh && kk == 0) ? 0u : 1u);
           }
           tc_commit(&ctl.empty[slot]);
         }
         tc_commit(&ctl.pv_done[b]);
-        if (plast) tc_commit(&ctl.o_full[pseg & 1]);
+        if (x.last) tc_commit(&ctl.o_full[ob]);
         return true;
       };
       for (; ok && w.next(s); ++nseg) {
@@ -481,6 +511,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int t = s.t0; ok && t < s.t1; ++t, ++i) {
           const int b = i & 1;
           if (i >= 2) ok = wait(&ctl.s_free[b], ((i >> 1) - 1) & 1);
+          int chunk = k_chunk(i);
           for (int c = 0; ok && c < DC; ++c, ++chunk) {
             const int slot = chunk % SLOTS;
             ok = wait(&ctl.full[slot], (chunk / SLOTS) & 1);
@@ -505,14 +536,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) break;
           tc_commit(&ctl.s_full[b]);
           if (t == s.t1 - 1) tc_commit(&ctl.q_empty[nseg & 1]);
-          if (pi >= 0) ok = values();
-          pi = i;
-          pseg = nseg;
-          pfirst = t == s.t0;
-          plast = t == s.t1 - 1;
+          if (pend[0].i >= 0) ok = values(pend[0]);
+          pend[0] = pend[1];
+          pend[1] = {i, nseg, t == s.t0, t - s.t0 < 2, t == s.t1 - 1};
         }
       }
-      if (ok && pi >= 0) values();
+      if (ok && pend[0].i >= 0) ok = values(pend[0]);
+      if (ok && pend[1].i >= 0) values(pend[1]);
     }
     __syncwarp();
   } else if (warp == W_Q) {
@@ -639,54 +669,43 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     __syncwarp();
-  } else if (warp < 4) {
+  } else if (warp < 4 || warp >= W_SOFT1) {
     // ------------------------------------------------------------------ softmax: thread = key of the tile
-    const uint32_t lane_off = (uint32_t)(32 * warp) << 16;
+    // Group b takes the tiles of parity b, with its own S^T and P^T buffers.
+    const int b = warp >= W_SOFT1 ? 1 : 0, wq = warp & 3, key_in = tid & 127;
+    const int bar = b == 0 ? 1 : 3;
+    const uint32_t lane_off = (uint32_t)(32 * wq) << 16;
     Walk w;
     w.init(pre, p.rows, per_row, c0, c1);
     Seg s{};
-    int i = 0;
+    int seg0 = 0;  // the segment's first tile in this CTA's numbering
     bool quit = false;
     for (int n = 0; !quit && w.next(s); ++n) {
       const int need = need_of(s.b);
       const int h = s.u / p.chunks, col0 = (s.u - h * p.chunks) * p.chunk_cols;
       const int ncol = min(p.chunk_cols, p.cols - col0);
-      float m[NQT], l[NQT], cq[NQT];
-      int lim[NQT];
-      {
-        int tt = col0 / p.group, g = col0 - tt * p.group;
+      const int tok0 = col0 / p.group;         // the first column's token
+      const int lim0 = len[s.b] + tok0;        // the keys it sees; later tokens see more
+      const int ob = C::OB == 2 ? n & 1 : 0;
+      float m[NQT], l[NQT];
 #pragma unroll
-        for (int j = 0; j < NQT; ++j) {
-          lim[j] = j < ncol ? min(need, len[s.b] + tt) : 0;
-          if (++g == p.group) {
-            g = 0;
-            ++tt;
-          }
-          m[j] = 0.f;
-          l[j] = 0.f;
-          cq[j] = p.qscale;
-        }
-      }
-      for (int t = s.t0; t < s.t1; ++t, ++i) {
-        const int b = i & 1;
-        const bool first = t == s.t0;
-        const int key = t * BN + tid;
+      for (int j = 0; j < NQT; ++j) m[j] = l[j] = 0.f;
+      bool first = true;
+      for (int i = seg0 + ((seg0 ^ b) & 1); i < seg0 + s.t1 - s.t0; i += 2) {
+        const int t = s.t0 + i - seg0;
+        const int key = t * BN + key_in;
         wait(&ctl.s_full[b], (i >> 1) & 1);
         float ks = 1.f, ev = 0.f, iv = 1.f;
         if constexpr (FP8) {
           const int st = i % kScaleStages;
           wait(&ctl.sc_full[st], (i / kScaleStages) & 1);
           const unsigned char* sc = smem + C::SC_OFF + st * 2 * BN;
-          ks = __uint_as_float((uint32_t)sc[tid] << 23);
-          const int eb = sc[BN + tid];
+          ks = __uint_as_float((uint32_t)sc[key_in] << 23);
+          const int eb = sc[BN + key_in];
           ev = (float)(eb - 127);
           iv = __uint_as_float((uint32_t)(254 - eb) << 23);
           __syncwarp();
           if (lane == 0) mbar_arrive(&ctl.sc_empty[st]);
-          if (first) {
-#pragma unroll
-            for (int j = 0; j < NQT; ++j) cq[j] = ctl.cq[n & 3][j];
-          }
         }
         tc_fence_after();
         __syncwarp();
@@ -694,32 +713,45 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int c = 0; c < N / 16; ++c) tmem_ld16(tbase + lane_off + b * N + c * 16, sv + c * 16);
         tc_fence_before();
-        mbar_arrive(&ctl.s_free[b]);
         float x[NQT];
+#pragma unroll
+        for (int j = 0; j < NQT; ++j) {
+          if constexpr (FP8) x[j] = fmaf(fmaf(sv[NQT + j], 0.0625f, sv[j]) * ks, ctl.cq[n & 3][j], ev);
+          else x[j] = sv[j] * p.qscale;
+        }
+        mbar_arrive(&ctl.s_free[b]);  // (after the last read of the queries' factors, too)
+        if (NQT > ncol || (t + 1) * BN > lim0) {  // spare columns, or keys that some column does not see
+          int tt = 0, g = col0 - tok0 * p.group;
+#pragma unroll
+          for (int j = 0; j < NQT; ++j) {
+            if (j >= ncol || key >= min(need, lim0 + tt)) x[j] = -INFINITY;
+            if (++g == p.group) {
+              g = 0;
+              ++tt;
+            }
+          }
+        }
         bool over = FP8 && first;
 #pragma unroll
         for (int j = 0; j < NQT; ++j) {
-          if constexpr (FP8) {
-            const float raw = fmaf(sv[NQT + j], 0.0625f, sv[j]);
-            x[j] = key < lim[j] ? fmaf(raw * ks, cq[j], ev) : -INFINITY;
-            if (!first) over |= x[j] > m[j] + kRaise;
+          if (FP8) {
+            over |= x[j] > m[j] + kRaise;
           } else {
-            x[j] = key < lim[j] ? sv[j] * p.qscale : -INFINITY;
             over |= x[j] > m[j] + kRaise;
             if (first) over |= x[j] > -INFINITY && x[j] < m[j] - kBelow;
           }
         }
         const bool saw = abort_flag != 0;
-        if (sync_or(1, 128, over || saw)) {
+        if (sync_or(bar, 128, over || saw)) {
           float v[NQT];
 #pragma unroll
           for (int j = 0; j < NQT; ++j) v[j] = x[j];
           warp_all<NQT, true>(v);
           if (lane == 0) {
 #pragma unroll
-            for (int j = 0; j < NQT; ++j) ctl.red[warp][j] = v[j];
+            for (int j = 0; j < NQT; ++j) ctl.red[b][wq][j] = v[j];
           }
-          if (sync_or(1, 128, saw)) {
+          if (sync_or(bar, 128, saw)) {
             quit = true;
             break;
           }
@@ -727,7 +759,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           bool any = false;
 #pragma unroll
           for (int j = 0; j < NQT; ++j) {
-            const float top = fmaxf(fmaxf(ctl.red[0][j], ctl.red[1][j]), fmaxf(ctl.red[2][j], ctl.red[3][j]));
+            const float top = fmaxf(fmaxf(ctl.red[b][0][j], ctl.red[b][1][j]), fmaxf(ctl.red[b][2][j], ctl.red[b][3][j]));
             float mn = m[j];
             if (top != -INFINITY) {
               if (FP8) mn = first ? top - kHead8 : (top > m[j] + kRaise ? top - kHead8 : m[j]);
@@ -739,12 +771,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             l[j] *= scl[j];
           }
           if (any && !first) {  // the same in every thread: the maxima are
-            wait(&ctl.pv_done[b ^ 1], ((i - 1) >> 1) & 1);  // O holds every earlier tile of the unit
+            wait(&ctl.pv_done[b], ((i >> 1) - 1) & 1);  // O holds every earlier tile of the segment and group
             tc_fence_after();
             __syncwarp();
 #pragma unroll 1
             for (int c = 0; c < DC; ++c) {
-              const uint32_t o = tbase + lane_off + C::S_COLS + ((n & 1) * DC + c) * N;
+              const uint32_t o = tbase + lane_off + C::S_COLS + ((ob * 2 + b) * DC + c) * N;
               float ov[N];
 #pragma unroll
               for (int k = 0; k < N / 16; ++k) tmem_ld16(o + k * 16, ov + k * 16);
@@ -758,7 +790,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
           }
-          named_sync(1, 128);  // the maxima are read before the next tile writes them
+          named_sync(bar, 128);  // the maxima are read before the next tile writes them
         }
         float pr[NQT];
 #pragma unroll
@@ -797,8 +829,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           } else {
             w0 = make_uint4((hw[0] & 0xffu) | ((lw[0] & 0xffu) << 8), 0u, 0u, 0u);
           }
-          *reinterpret_cast<uint4*>(pb + tid * 16) = w0;
-          if constexpr (N == 32) *reinterpret_cast<uint4*>(pb + 2048 + tid * 16) = w1;
+          *reinterpret_cast<uint4*>(pb + key_in * 16) = w0;
+          if constexpr (N == 32) *reinterpret_cast<uint4*>(pb + 2048 + key_in * 16) = w1;
         } else {
           uint32_t wv[8];
 #pragma unroll
@@ -808,26 +840,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             const __nv_bfloat162 v2 = __floats2bfloat162_rn(lo, hi);
             wv[k] = *reinterpret_cast<const uint32_t*>(&v2);
           }
-          *reinterpret_cast<uint4*>(pb + tid * 16) = make_uint4(wv[0], wv[1], wv[2], wv[3]);
-          *reinterpret_cast<uint4*>(pb + 2048 + tid * 16) = make_uint4(wv[4], wv[5], wv[6], wv[7]);
+          *reinterpret_cast<uint4*>(pb + key_in * 16) = make_uint4(wv[0], wv[1], wv[2], wv[3]);
+          *reinterpret_cast<uint4*>(pb + 2048 + key_in * 16) = make_uint4(wv[4], wv[5], wv[6], wv[7]);
         }
         if (t * BN + BN > need) {
           // The row's last tile: V rows past its keys may hold anything, and 0 x NaN is NaN. Cleared once loaded (the
           // producer has issued the chunk, so the slot's phase is the chunk's).
           const int vc = v_chunk(i);
           for (int c = 0; c < DC; ++c) {
-            const uint64_t t_start = global_ns();
-            while (issued <= vc + c) {
-              if (abort_flag) break;
-              if (global_ns() - t_start > kWaitLimitNs) {
-                abort_flag = 1;
-                break;
-              }
-            }
-            if (abort_flag) break;
+            if (!wait_issued((vc + c) % SLOTS, (vc + c) / SLOTS + 1)) break;
             wait(&ctl.full[(vc + c) % SLOTS], ((vc + c) / SLOTS) & 1);
             if (key >= need) {
-              unsigned char* row = smem + ((vc + c) % SLOTS) * SLOT + tid * 128;
+              unsigned char* row = smem + ((vc + c) % SLOTS) * SLOT + key_in * 128;
 #pragma unroll
               for (int k = 0; k < 8; ++k) {
 #pragma unroll
@@ -839,18 +863,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         fence_async_smem();
         tc_fence_before();
         mbar_arrive(&ctl.p_full[b]);
+        first = false;
       }
       if (quit) break;
-      // The segment's sums and maxima, once the epilogue has read those of two segments before.
-      if (n >= 2) wait(&ctl.o_free[n & 1], ((n >> 1) - 1) & 1);
+      seg0 += s.t1 - s.t0;
+      // The segment's sums and maxima (sums of zero where the group had no tile), once the epilogue has read those of two
+      // segments before.
+      if (n >= 2) wait(&ctl.ml_free[n & 1], ((n >> 1) - 1) & 1);
       warp_all<NQT, false>(l);
       if (lane == 0) {
 #pragma unroll
-        for (int j = 0; j < NQT; ++j) ctl.sum[n & 1][warp][j] = l[j];
+        for (int j = 0; j < NQT; ++j) ctl.sum[n & 1][b][wq][j] = l[j];
       }
-      if (tid == 0) {
+      if (key_in == 0) {
 #pragma unroll
-        for (int j = 0; j < NQT; ++j) ctl.top[n & 1][j] = m[j];
+        for (int j = 0; j < NQT; ++j) ctl.top[n & 1][b][j] = m[j];
       }
       mbar_arrive(&ctl.ml_full[n & 1]);
     }
@@ -862,18 +889,30 @@ __global__ void __launch_bounds__(kThreads, 1)
     w.init(pre, p.rows, per_row, c0, c1);
     Seg s{};
     for (int n = 0; w.next(s); ++n) {
-      wait(&ctl.o_full[n & 1], (n >> 1) & 1);
+      const int ob = C::OB == 2 ? n & 1 : 0;
+      wait(&ctl.o_full[ob], (n / C::OB) & 1);
       wait(&ctl.ml_full[n & 1], (n >> 1) & 1);
       if (sync_or(2, 128, abort_flag != 0)) break;  // all of these warps leave together
       tc_fence_after();
       const int h = s.u / p.chunks, col0 = (s.u - h * p.chunks) * p.chunk_cols;
       const int ncol = min(p.chunk_cols, p.cols - col0);
-      float l[NQT], m[NQT];
+      // The two softmax groups' parts as one: weights 2^(m_b - m); a group that saw no key takes no part.
+      float l[NQT], m[NQT], wt[2][NQT];
 #pragma unroll
       for (int j = 0; j < NQT; ++j) {
-        l[j] = (ctl.sum[n & 1][0][j] + ctl.sum[n & 1][1][j]) + (ctl.sum[n & 1][2][j] + ctl.sum[n & 1][3][j]);
-        m[j] = ctl.top[n & 1][j];
+        float ls[2], ms[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const auto& sum = ctl.sum[n & 1][b];
+          ls[b] = (sum[0][j] + sum[1][j]) + (sum[2][j] + sum[3][j]);
+          ms[b] = ls[b] != 0.f ? ctl.top[n & 1][b][j] : -INFINITY;
+        }
+        m[j] = fmaxf(ms[0], ms[1]);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) wt[b][j] = ls[b] != 0.f ? ex2(ms[b] - m[j]) : 0.f;
+        l[j] = ls[0] * wt[0][j] + ls[1] * wt[1][j];
       }
+      mbar_arrive(&ctl.ml_free[n & 1]);
       unsigned bad = 0;  // columns with a result that is not finite
       auto store = [&](int c, const float (&o)[NQT], const float (&sum)[NQT]) {
         int tt = col0 / p.group, g = col0 - tt * p.group;
@@ -898,13 +937,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int c = 0; c < DC; ++c) {
         float v[N], o[NQT];
 #pragma unroll
-        for (int k = 0; k < N / 16; ++k) tmem_ld16(tbase + lane_off + C::S_COLS + ((n & 1) * DC + c) * N + k * 16, v + k * 16);
+        for (int b = 0; b < 2; ++b) {
+#pragma unroll
+          for (int k = 0; k < N / 16; ++k)
+            tmem_ld16(tbase + lane_off + C::S_COLS + ((ob * 2 + b) * DC + c) * N + k * 16, v + k * 16);
+#pragma unroll
+          for (int j = 0; j < NQT; ++j) {
+            const float x = FP8 ? fmaf(v[NQT + j], 0.0625f, v[j]) : v[j];
+            const float add = wt[b][j] != 0.f ? x * wt[b][j] : 0.f;  // (a group without a tile: its O is stale)
+            o[j] = b == 0 ? add : o[j] + add;
+          }
+        }
         if (c == DC - 1) {
           tc_fence_before();
-          mbar_arrive(&ctl.o_free[n & 1]);
+          mbar_arrive(&ctl.o_free[ob]);
         }
-#pragma unroll
-        for (int j = 0; j < NQT; ++j) o[j] = FP8 ? fmaf(v[NQT + j], 0.0625f, v[j]) : v[j];
         if (emit) {
           store(c, o, l);
         } else {
@@ -994,7 +1041,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_wait(&ctl.drain, 0);
     }
     if (tid == W_LOAD * 32)  // the latest load of every slot lands before the shared memory goes away
-      for (int i = issued > SLOTS ? issued - SLOTS : 0; i < issued; ++i) mbar_wait(&ctl.full[i % SLOTS], (i / SLOTS) & 1);
+      for (int i = 0; i < SLOTS; ++i)
+        if (loads[i] > 0) mbar_wait(&ctl.full[i], (loads[i] - 1) & 1);
   }
   tc_fence_before();
   __syncthreads();

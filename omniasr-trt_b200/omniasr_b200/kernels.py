@@ -31,6 +31,7 @@ the built library every function raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -125,10 +126,10 @@ _ATTN_WS: dict = {}  # (device, stream) -> decode / draft workspace; its unit co
 _ATTN_WS_RETIRED: list = []  # outgrown workspaces, kept alive for CUDA graphs that captured them
 
 
-def _attn_workspace(nbytes: int, device: torch.device) -> torch.Tensor:
+def _attn_workspace(nbytes: int, device: torch.device, stream: int | None = None) -> torch.Tensor:
     """The decode / draft workspace of the current stream: zeroed once when allocated (its leading unit counters
     must be zero on entry, and every call leaves them zero), reused by the stream's calls in order."""
-    key = (device.index, torch.cuda.current_stream(device).cuda_stream)
+    key = (device.index, torch.cuda.current_stream(device).cuda_stream if stream is None else stream)
     ws = _ATTN_WS.get(key)
     if ws is None or ws.numel() < nbytes:
         if ws is not None:
@@ -497,33 +498,46 @@ def reorder_gather(src: torch.Tensor, parent: torch.Tensor, out: torch.Tensor | 
     return out
 
 
+def _launch(device: torch.device) -> tuple[int, int]:
+    """(the device's status word, the current stream) as the C ABI takes them; a few hundred nanoseconds, as the host's
+    time is what a small call waits for."""
+    index = device.index
+    word = _status.get(index)
+    if word is None:
+        word = status_word(index)
+    return word.data_ptr(), _raw_stream(index)
+
+
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 def _pages(k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None, v_scale: torch.Tensor | None, dtype: int,
            name: str) -> tuple:
     """A paged cache's arguments: (k, v, k_scale, v_scale, pages, page, strides), kv heads, head_dim and type code."""
-    if k.dim() != 4 or v.shape != k.shape or v.stride() != k.stride() or k.stride(3) != 1 or v.dtype != k.dtype:
+    shape, stride, kind = k.shape, k.stride(), k.dtype
+    if len(shape) != 4 or v.shape != shape or v.stride() != stride or stride[3] != 1 or v.dtype != kind:
         raise ValueError(f"{name}: k and v pages must be [pages, kv_heads, page, D] views of one dtype with the same "
                          "strides and unit stride in D")
-    pages, kv_heads, page, dim = k.shape
-    if k.dtype == torch.float8_e4m3fn:
-        code = _lib.FP8
+    pages, kv_heads, page, dim = shape
+    geometry = (pages, page, stride[0], stride[1], stride[2])
+    if kind == torch.float8_e4m3fn:
         for t in (k_scale, v_scale):
-            if t is None or t.dtype != torch.uint8 or t.shape != (pages, kv_heads, page) or not t.is_contiguous():
+            if t is None or t.dtype != torch.uint8 or t.shape != shape[:3] or not t.is_contiguous():
                 raise ValueError(f"{name}: float8_e4m3fn pages need contiguous uint8 scales [pages, kv_heads, page]")
-    else:
-        code = _DTYPES.get(k.dtype)
-        if code != dtype:
-            raise ValueError(f"{name}: pages of {k.dtype} (supported: the queries' dtype, float8_e4m3fn)")
-        if k_scale is not None or v_scale is not None:
-            raise ValueError(f"{name}: scales belong to float8_e4m3fn pages")
-    sp, sh, st, _ = k.stride()
-    return ((k.data_ptr(), v.data_ptr(), None if k_scale is None else k_scale.data_ptr(),
-             None if v_scale is None else v_scale.data_ptr()), (pages, page, sp, sh, st), kv_heads, dim, code)
+        return (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr()), geometry, kv_heads, dim, _lib.FP8
+    code = _DTYPES.get(kind)
+    if code != dtype:
+        raise ValueError(f"{name}: pages of {kind} (supported: the queries' dtype, float8_e4m3fn)")
+    if k_scale is not None or v_scale is not None:
+        raise ValueError(f"{name}: scales belong to float8_e4m3fn pages")
+    return (k.data_ptr(), v.data_ptr(), None, None), geometry, kv_heads, dim, code
 
 
 def _table(table: torch.Tensor, rows: int, name: str) -> tuple[int, int, int]:
-    if table.dtype != torch.int32 or table.dim() != 2 or table.size(0) < rows or (table.size(1) > 1 and table.stride(1) != 1):
+    shape, stride = table.shape, table.stride()
+    if table.dtype != torch.int32 or len(shape) != 2 or shape[0] < rows or (shape[1] > 1 and stride[1] != 1):
         raise ValueError(f"{name}: page_table must be int32 [rows, width] with unit inner stride")
-    return table.data_ptr(), table.stride(0), table.size(1)
+    return table.data_ptr(), stride[0], shape[1]
 
 
 def paged_rope_kv(qkv: torch.Tensor, cs: torch.Tensor, pos: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -551,8 +565,7 @@ def paged_rope_kv(qkv: torch.Tensor, cs: torch.Tensor, pos: torch.Tensor, k_page
     cs = cs if cs.dtype == torch.float32 and cs.is_contiguous() else cs.float().contiguous()
     pos, slots = _index(pos), _index(slots)
     _lib.call("omniasr_paged_rope_kv", qkv.data_ptr(), qkv.stride(0), cs.data_ptr(), cs.size(0), pos.data_ptr(),
-              slots.data_ptr(), q.data_ptr(), *ptrs, *geo, n, heads, kv_heads, dim, dtype, code,
-              status_word(device).data_ptr(), _stream(device))
+              slots.data_ptr(), q.data_ptr(), *ptrs, *geo, n, heads, kv_heads, dim, dtype, code, *_launch(device))
     return q
 
 
@@ -579,8 +592,14 @@ def paged_kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torc
         return k, v
     offsets = _index(offsets)
     _lib.call("omniasr_paged_kv_read", *ptrs, *geo, *table, rows, offsets.data_ptr(), tokens, k.data_ptr(), v.data_ptr(),
-              kvh, dim, out_code, code, status_word(device).data_ptr(), _stream(device))
+              kvh, dim, out_code, code, *_launch(device))
     return k, v
+
+
+@functools.lru_cache(maxsize=4096)
+def _paged_ws(*shape: int) -> int:
+    """Workspace bytes of a paged_attention call (a function of host sizes alone)."""
+    return _lib.load().omniasr_paged_attention_workspace(*shape)
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -606,10 +625,10 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         return out
     device = q.device
     lengths = _index(lengths)
-    nbytes = _lib.load().omniasr_paged_attention_workspace(dtype, code, rows, tokens, heads, kvh, dim, geo[1], table[2])
-    ws = _attn_workspace(nbytes, device)
+    status, stream = _launch(device)
+    ws = _attn_workspace(_paged_ws(dtype, code, rows, tokens, heads, kvh, dim, geo[1], table[2]), device, stream)
     _lib.call("omniasr_paged_attention", q.data_ptr(), *ptrs, *geo, *table, lengths.data_ptr(), out.data_ptr(), rows, tokens,
-              heads, kvh, dim, scale, dtype, code, ws.data_ptr(), ws.numel(), status_word(device).data_ptr(), _stream(device))
+              heads, kvh, dim, scale, dtype, code, ws.data_ptr(), ws.numel(), status, stream)
     return out
 
 
@@ -639,11 +658,12 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offset
         return out
     device = q.device
     q_offsets, k_offsets = _index(q_offsets), _index(k_offsets)
-    ws = _attn_workspace(_PACKED_WS, device)
+    status, stream = _launch(device)
+    ws = _attn_workspace(_PACKED_WS, device, stream)
     _lib.call("omniasr_packed_attention", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
               v.data_ptr(), v.stride(0), v.stride(1), out.data_ptr(), q_offsets.data_ptr(), k_offsets.data_ptr(), tq, tk,
               seqs, heads, kv_heads, dim, dim**-0.5 if scale is None else scale, dtype, ws.data_ptr(), ws.numel(),
-              status_word(device).data_ptr(), _stream(device))
+              status, stream)
     return out
 
 
