@@ -58,6 +58,8 @@ int check_pages(const char* name, const omni::PageCache& c) {
   if (c.page > 1 && c.s_pos < c.dim) return fail(OMNIASR_ERR_ARGUMENT, "%s: positions overlap", name);
   if (c.type == OMNIASR_FP8 && (!c.k_scale || !c.v_scale))
     return fail(OMNIASR_ERR_ARGUMENT, "%s: an fp8 cache needs its scale bytes", name);
+  if (c.type == OMNIASR_FP8 && (!aligned16(c.k_scale) || !aligned16(c.v_scale)))
+    return fail(OMNIASR_ERR_ARGUMENT, "%s: scale bytes must be 16-byte aligned", name);
   return OMNIASR_OK;
 }
 
