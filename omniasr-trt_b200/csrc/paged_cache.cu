@@ -16,6 +16,8 @@
 
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "attention.cuh"
 #include "common.cuh"
 #include "paged.cuh"
@@ -76,6 +78,19 @@ __global__ void __launch_bounds__(kRopeThreads) paged_rope_kernel(const PagedRop
   const int items = a.heads + 2 * kvh;
   const int i0 = blockIdx.y * per, i1 = min(items, i0 + per);
   const int lane = threadIdx.x % L, team = threadIdx.x / L;
+  const T* src = reinterpret_cast<const T*>(a.qkv) + n * a.qkv_stride;
+  uint4 u[IL][NV];
+  auto load = [&](int base) {
+#pragma unroll
+    for (int j = 0; j < IL; ++j) {
+      const int it = base + j * TEAMS + team;
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+        u[j][v] = it < i1 ? __ldg(reinterpret_cast<const uint4*>(src + (int64_t)it * D) + v * L + lane)
+                          : make_uint4(0u, 0u, 0u, 0u);
+    }
+  };
+  load(i0);  // before the position is waited for
   const int64_t p = a.pos[n];
   const int64_t slot = a.slots[n];
   const bool pos_ok = p >= 0 && p < a.cs_positions;
@@ -83,7 +98,6 @@ __global__ void __launch_bounds__(kRopeThreads) paged_rope_kernel(const PagedRop
   if (threadIdx.x == 0 && (!pos_ok || slot >= a.c.pages * a.c.page)) raise_status(a.status, kStatusIndex);
   const int64_t pg = slot_ok ? slot / a.c.page : 0;
   const int off = slot_ok ? (int)(slot - pg * a.c.page) : 0;
-  const T* src = reinterpret_cast<const T*>(a.qkv) + n * a.qkv_stride;
 
   float cs[NV][kVec];
 #pragma unroll
@@ -99,15 +113,7 @@ __global__ void __launch_bounds__(kRopeThreads) paged_rope_kernel(const PagedRop
     }
   // Every team of a warp takes the same number of rounds (the scale's shuffles need the whole warp).
   for (int base = i0; base < i1; base += TEAMS * IL) {
-    uint4 u[IL][NV];
-#pragma unroll
-    for (int j = 0; j < IL; ++j) {
-      const int it = base + j * TEAMS + team;
-#pragma unroll
-      for (int v = 0; v < NV; ++v)
-        u[j][v] = it < i1 ? __ldg(reinterpret_cast<const uint4*>(src + (int64_t)it * D) + v * L + lane)
-                          : make_uint4(0u, 0u, 0u, 0u);
-    }
+    if (base > i0) load(base);
 #pragma unroll
     for (int j = 0; j < IL; ++j) {
       const int it = base + j * TEAMS + team;
@@ -137,6 +143,7 @@ __global__ void __launch_bounds__(kRopeThreads) paged_rope_kernel(const PagedRop
       const bool write = live && it >= a.heads && slot_ok && (pos_ok || !is_k);
       const int64_t dst = pg * a.c.s_page + (int64_t)h * a.c.s_head + (int64_t)off * a.c.s_pos;
       if constexpr (FP8) {
+        if (__all_sync(0xffffffffu, it < a.heads)) continue;  // a warp of query heads (the same for all its lanes)
         uint32_t amax = 0u;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
@@ -172,21 +179,26 @@ __global__ void __launch_bounds__(kRopeThreads) paged_rope_kernel(const PagedRop
 }
 
 constexpr int kReadThreads = 256;
-constexpr int kReadTokens = 16;  // most tokens of one CTA
 
-// One CTA: `tb` consecutive output tokens, K and V of every head. Threads 0 .. tb - 1 find the tokens' places (the
-// sequence by bisection in the offsets, the page in its table row); then 16 bytes of the cache per thread and step.
-template <typename T, int D, bool FP8>
-__global__ void __launch_bounds__(kReadThreads) paged_read_kernel(const PagedReadArgs a, int tb) {
-  constexpr int kElems = FP8 ? 16 : Elem<T>::kVec;  // elements of one 16-byte word of the cache
-  constexpr int W = D / kElems;                     // words per vector
+// One CTA: consecutive output tokens of one head (a page's positions of a head lie together), R rounds of TP tokens with
+// 16 bytes of the output per thread and round. Threads find the tokens' places first (the sequence by bisection in the
+// offsets, the page in its table row); then all rounds' loads are in flight together, and every store of a warp covers
+// whole lines: 195 MB of an fp8 context 44 us with 16-byte loads (two half-line stores each), token-major.
+template <typename T, int D, bool FP8, int R>
+__global__ void __launch_bounds__(kReadThreads) paged_read_kernel(const PagedReadArgs a) {
+  constexpr int kOut = 16 / sizeof(T);       // elements per thread and round
+  constexpr int W = D / kOut;                // threads per vector
+  constexpr int TP = kReadThreads / W;       // tokens per round
+  constexpr int TB = TP * R;
   grid_launch_dependents();
   grid_dependency_wait();
-  __shared__ int64_t s_page[kReadTokens];
-  __shared__ int s_off[kReadTokens];
-  const int64_t t0 = (int64_t)blockIdx.x * tb;
-  if (threadIdx.x < tb) {
-    const int64_t tok = t0 + threadIdx.x;
+  __shared__ int64_t s_page[TB];
+  __shared__ int s_off[TB];
+  const int kvh = a.c.kv_heads;
+  const int64_t t0 = (int64_t)(blockIdx.x / (unsigned)kvh) * TB;
+  const int h = blockIdx.x % (unsigned)kvh;
+  for (int i = threadIdx.x; i < TB; i += kReadThreads) {
+    const int64_t tok = t0 + i;
     int64_t page = -1;
     int off = 0;
     if (tok < a.tokens && tok >= a.offsets[0] && tok < a.offsets[a.rows]) {
@@ -201,62 +213,63 @@ __global__ void __launch_bounds__(kReadThreads) paged_read_kernel(const PagedRea
       off = (int)(j - pi * a.c.page);
       const int64_t id = j >= 0 && pi < a.table_width ? a.table[lo * a.table_stride + pi] : -1;
       if (id >= 0 && id < a.c.pages) page = id;
-      else raise_status(a.status, kStatusIndex);
+      else if (h == 0) raise_status(a.status, kStatusIndex);
     }
-    s_page[threadIdx.x] = page;
-    s_off[threadIdx.x] = off;
+    s_page[i] = page;
+    s_off[i] = off;
   }
   __syncthreads();
-  const int kvh = a.c.kv_heads;
-  const int per_tok = kvh * W;
-  const int total = tb * per_tok;
-#pragma unroll 2
-  for (int w = threadIdx.x; w < total; w += kReadThreads) {
-    const int ti = w / per_tok;
-    const int r = w - ti * per_tok;
-    const int h = r / W, c = r - h * W;
-    const int64_t tok = t0 + ti;
+  const int c = threadIdx.x % W;
+  using In = std::conditional_t<!FP8, uint4, std::conditional_t<kOut == 8, uint2, uint32_t>>;
+  In ku[R], vu[R];
+  float ks[R], vs[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int i = r * TP + threadIdx.x / W;
+    const int64_t page = s_page[i];
+    ku[r] = In{};
+    vu[r] = In{};
+    ks[r] = vs[r] = 0.f;
+    if (page >= 0) {
+      const int64_t at = page * a.c.s_page + (int64_t)h * a.c.s_head + (int64_t)s_off[i] * a.c.s_pos + c * kOut;
+      constexpr int es = FP8 ? 1 : sizeof(T);
+      ku[r] = __ldcs(reinterpret_cast<const In*>(reinterpret_cast<const char*>(a.c.k) + at * es));
+      vu[r] = __ldcs(reinterpret_cast<const In*>(reinterpret_cast<const char*>(a.c.v) + at * es));
+      if (FP8) {
+        const int64_t si = (page * kvh + h) * a.c.page + s_off[i];
+        ks[r] = __uint_as_float((uint32_t)__ldg(a.c.k_scale + si) << 23);
+        vs[r] = __uint_as_float((uint32_t)__ldg(a.c.v_scale + si) << 23);
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int64_t tok = t0 + r * TP + threadIdx.x / W;
     if (tok >= a.tokens) break;
-    const int64_t page = s_page[ti];
-    const int off = s_off[ti];
-    const int64_t src = page * a.c.s_page + (int64_t)h * a.c.s_head + (int64_t)off * a.c.s_pos + c * kElems;
-    const int64_t dst = (tok * kvh + h) * D + c * kElems;
-    T* ko = reinterpret_cast<T*>(a.k_out) + dst;
-    T* vo = reinterpret_cast<T*>(a.v_out) + dst;
+    const int64_t dst = (tok * kvh + h) * D + c * kOut;
+    uint4* ko = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.k_out) + dst);
+    uint4* vo = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.v_out) + dst);
     if constexpr (FP8) {
-      uint4 ku = make_uint4(0u, 0u, 0u, 0u), vu = ku;
-      float ks = 0.f, vs = 0.f;
-      if (page >= 0) {
-        ku = __ldcs(reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.c.k) + src));
-        vu = __ldcs(reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.c.v) + src));
-        const int64_t si = (page * kvh + h) * a.c.page + off;
-        ks = __uint_as_float((uint32_t)a.c.k_scale[si] << 23);
-        vs = __uint_as_float((uint32_t)a.c.v_scale[si] << 23);
+      uint32_t kw[2], vw[2];
+      if constexpr (kOut == 8) {
+        kw[0] = ku[r].x, kw[1] = ku[r].y, vw[0] = vu[r].x, vw[1] = vu[r].y;
+      } else {
+        kw[0] = ku[r], vw[0] = vu[r];
       }
-      const uint32_t kw[4] = {ku.x, ku.y, ku.z, ku.w}, vw[4] = {vu.x, vu.y, vu.z, vu.w};
-      float kf[16], vf[16];
+      float kf[kOut], vf[kOut];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < kOut / 2; ++i) {
         const float2 kk = values2(kw[i >> 1] >> (16 * (i & 1))), vv = values2(vw[i >> 1] >> (16 * (i & 1)));
-        kf[2 * i] = kk.x * ks;
-        kf[2 * i + 1] = kk.y * ks;
-        vf[2 * i] = vv.x * vs;
-        vf[2 * i + 1] = vv.y * vs;
+        kf[2 * i] = kk.x * ks[r];
+        kf[2 * i + 1] = kk.y * ks[r];
+        vf[2 * i] = vv.x * vs[r];
+        vf[2 * i + 1] = vv.y * vs[r];
       }
-      constexpr int kOut = Elem<T>::kVec;
-#pragma unroll
-      for (int i = 0; i < 16 / kOut; ++i) {
-        __stcs(reinterpret_cast<uint4*>(ko) + i, Pack<T>::pack(kf + i * kOut));
-        __stcs(reinterpret_cast<uint4*>(vo) + i, Pack<T>::pack(vf + i * kOut));
-      }
+      __stcs(ko, Pack<T>::pack(kf));
+      __stcs(vo, Pack<T>::pack(vf));
     } else {
-      uint4 ku = make_uint4(0u, 0u, 0u, 0u), vu = ku;
-      if (page >= 0) {
-        ku = __ldcs(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.c.k) + src));
-        vu = __ldcs(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.c.v) + src));
-      }
-      __stcs(reinterpret_cast<uint4*>(ko), ku);
-      __stcs(reinterpret_cast<uint4*>(vo), vu);
+      __stcs(ko, ku[r]);
+      __stcs(vo, vu[r]);
     }
   }
 }
@@ -278,15 +291,13 @@ cudaError_t rope_launch(const PagedRopeArgs& a, cudaStream_t s) {
 
 template <typename T, int D, bool FP8>
 cudaError_t read_launch(const PagedReadArgs& a, cudaStream_t s) {
-  constexpr int kElems = FP8 ? 16 : Elem<T>::kVec;
-  // About four steps per thread, less where that leaves SMs without work.
-  const int words = a.c.kv_heads * (D / kElems);
-  int tb = 4 * kReadThreads / words;
-  const int64_t spread = a.tokens / (2 * device_sm_count());
-  if (tb > spread) tb = (int)spread;
-  tb = tb < 1 ? 1 : (tb > kReadTokens ? kReadTokens : tb);
-  return launch_dependent(paged_read_kernel<T, D, FP8>, dim3((unsigned)((a.tokens + tb - 1) / tb)), dim3(kReadThreads),
-                          0, s, a, tb);
+  constexpr int TP = kReadThreads / (D / (16 / (int)sizeof(T)));
+  // Four rounds per CTA, one where four would leave SMs without work.
+  const int64_t four = (a.tokens + 4 * TP - 1) / (4 * TP) * a.c.kv_heads;
+  const int64_t one = (a.tokens + TP - 1) / TP * a.c.kv_heads;
+  if (four >= 2 * device_sm_count())
+    return launch_dependent(paged_read_kernel<T, D, FP8, 4>, dim3((unsigned)four), dim3(kReadThreads), 0, s, a);
+  return launch_dependent(paged_read_kernel<T, D, FP8, 1>, dim3((unsigned)one), dim3(kReadThreads), 0, s, a);
 }
 
 #define OMNI_DIM_SWITCH(DIM, CALL)      \

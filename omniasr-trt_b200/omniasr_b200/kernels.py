@@ -551,20 +551,21 @@ def paged_rope_kv(qkv: torch.Tensor, cs: torch.Tensor, pos: torch.Tensor, k_page
     [-40, 40])."""
     dtype = _dtype(qkv, "paged_rope_kv")
     ptrs, geo, kvh, dim, code = _pages(k_pages, v_pages, k_scale, v_scale, dtype, "paged_rope_kv")
-    n = qkv.size(0)
-    if kvh != kv_heads or qkv.dim() != 2 or qkv.size(1) != (heads + 2 * kv_heads) * dim or (n and qkv.stride(1) != 1):
+    shape, stride, table = qkv.shape, qkv.stride(), cs.shape
+    n = shape[0]
+    if kvh != kv_heads or len(shape) != 2 or shape[1] != (heads + 2 * kv_heads) * dim or (n and stride[1] != 1):
         raise ValueError("paged_rope_kv: qkv must be [N, (heads + 2 * kv_heads) * D] with unit inner stride")
     if pos.numel() != n or slots.numel() != n:
         raise ValueError("paged_rope_kv: pos and slots must hold one entry per token")
-    if cs.dim() != 3 or cs.size(1) != dim // 2 or cs.size(2) != 2:
+    if len(table) != 3 or table[1] != dim // 2 or table[2] != 2:
         raise ValueError("paged_rope_kv: cs must be [P, D / 2, 2]")
     device = qkv.device
-    q = torch.empty(n, heads, dim, device=device, dtype=qkv.dtype)
+    q = qkv.new_empty(n, heads, dim)
     if n == 0:
         return q
     cs = cs if cs.dtype == torch.float32 and cs.is_contiguous() else cs.float().contiguous()
     pos, slots = _index(pos), _index(slots)
-    _lib.call("omniasr_paged_rope_kv", qkv.data_ptr(), qkv.stride(0), cs.data_ptr(), cs.size(0), pos.data_ptr(),
+    _lib.call("omniasr_paged_rope_kv", qkv.data_ptr(), stride[0], cs.data_ptr(), table[0], pos.data_ptr(),
               slots.data_ptr(), q.data_ptr(), *ptrs, *geo, n, heads, kv_heads, dim, dtype, code, *_launch(device))
     return q
 
@@ -587,7 +588,7 @@ def paged_kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torc
     table = _table(page_table, rows, "paged_kv_read")
     device = k_pages.device
     k = torch.empty(tokens, kvh, dim, device=device, dtype=dtype)
-    v = torch.empty(tokens, kvh, dim, device=device, dtype=dtype)
+    v = torch.empty_like(k)
     if tokens == 0:
         return k, v
     offsets = _index(offsets)
@@ -639,13 +640,15 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offset
     query sees its last key, so a chunk of a prompt attends to the keys before it. Any token and head strides with
     16-byte alignment, unit stride in D; offsets ascending, on the device. Returns [Tq, heads, D] in q's dtype (a query
     that sees no key gets zeros; rows of no sequence are not written)."""
-    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or q.size(2) != k.size(2):
+    qs, ks, kind = q.shape, k.shape, q.dtype
+    if len(qs) != 3 or len(ks) != 3 or v.shape != ks or qs[2] != ks[2]:
         raise ValueError("packed_attention: q [Tq, heads, D], k and v [Tk, kv_heads, D]")
-    if k.dtype != q.dtype or v.dtype != q.dtype:
+    if k.dtype != kind or v.dtype != kind:
         raise ValueError("packed_attention: q, k and v must share a dtype")
-    tq, heads, dim = q.shape
-    tk, kv_heads, _ = k.shape
-    if (tq and q.stride(2) != 1) or (tk and (k.stride(2) != 1 or v.stride(2) != 1)):
+    tq, heads, dim = qs
+    tk, kv_heads, _ = ks
+    q_stride, k_stride, v_stride = q.stride(), k.stride(), v.stride()
+    if (tq and q_stride[2] != 1) or (tk and (k_stride[2] != 1 or v_stride[2] != 1)):
         raise ValueError("packed_attention: unit stride in D")
     dtype = _dtype(q, "packed_attention")
     if k_offsets is None:
@@ -653,15 +656,15 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offset
     seqs = q_offsets.numel() - 1
     if seqs < 0 or k_offsets.numel() != seqs + 1:
         raise ValueError("packed_attention: q_offsets and k_offsets must hold sequences + 1 entries")
-    out = torch.empty(tq, heads, dim, dtype=q.dtype, device=q.device)
+    out = q.new_empty(tq, heads, dim)
     if tq == 0:
         return out
     device = q.device
     q_offsets, k_offsets = _index(q_offsets), _index(k_offsets)
     status, stream = _launch(device)
     ws = _attn_workspace(_PACKED_WS, device, stream)
-    _lib.call("omniasr_packed_attention", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-              v.data_ptr(), v.stride(0), v.stride(1), out.data_ptr(), q_offsets.data_ptr(), k_offsets.data_ptr(), tq, tk,
+    _lib.call("omniasr_packed_attention", q.data_ptr(), q_stride[0], q_stride[1], k.data_ptr(), k_stride[0], k_stride[1],
+              v.data_ptr(), v_stride[0], v_stride[1], out.data_ptr(), q_offsets.data_ptr(), k_offsets.data_ptr(), tq, tk,
               seqs, heads, kv_heads, dim, dim**-0.5 if scale is None else scale, dtype, ws.data_ptr(), ws.numel(),
               status, stream)
     return out
