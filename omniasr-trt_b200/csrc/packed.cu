@@ -6,8 +6,10 @@
 // where that is not positive. q [Tq, H, D], k and v [Tk, Hkv, D], head h reads kv head h / (H / Hkv).
 //
 // One CTA: BM queries of one head; K and V tiles of BN keys go through shared memory as fp32; S = Q K^T and O += P V
-// in registers (256 threads as 16 x 16: thread (y, x) holds rows y + 16 i and keys / dims x + 16 j, so a row's softmax
-// statistics are a shuffle over half a warp). FMA-bound; fp32 throughout, as an fp32 model needs.
+// in registers (256 threads as 16 x 16: thread (y, x) holds rows y + 16 i, keys x + 16 j and groups of four dims, so a row's
+// softmax statistics are a shuffle over half a warp). FMA-bound; fp32 throughout, as an fp32 model needs. BM is 64 (32 for
+// head dims of 256 and more, whose tiles fill the shared memory), or 16 while larger tiles leave SMs idle: three prompts of
+// 17 to 131 tokens, 8 heads of 64, took 20 us with 64.
 
 #include <math.h>
 
@@ -23,10 +25,11 @@ namespace packed {
 
 constexpr int kThreads = 256;
 
-template <int D>
+template <int D, int BM_>
 struct Shape {
-  static constexpr int BM = D <= 128 ? 64 : 32;
+  static constexpr int BM = BM_;
   static constexpr int BN = D <= 128 ? 64 : 32;
+  static constexpr int VW = D >= 64 ? 4 : D / 16;  // consecutive head dims of O per thread
   static constexpr int LD = D + 4;  // row stride in shared memory (floats): 16-byte aligned, rows on different banks
   static constexpr int LP = BN + 4;
   static constexpr int BYTES = (BM * LD + 2 * BN * LD + BM * LP) * 4;
@@ -71,22 +74,35 @@ OMNI_DEV void load4<__nv_bfloat16>(const __nv_bfloat16* p, float* f) {
   f[2] = __uint_as_float(v.y << 16), f[3] = __uint_as_float(v.y & 0xffff0000u);
 }
 
-// `rows` rows of 4-element groups from global (row stride st) into shared memory; rows at or past `valid` are zeros.
-template <typename T, int D, int LD>
-OMNI_DEV void load_tile(float* dst, const T* src, int64_t st, int rows, int valid) {
-  for (int i = threadIdx.x; i < rows * (D / 4); i += kThreads) {
-    const int r = i / (D / 4), c = (i - r * (D / 4)) * 4;
-    float f[4] = {0.f, 0.f, 0.f, 0.f};
-    if (r < valid) load4(src + (int64_t)r * st + c, f);
-    *reinterpret_cast<float4*>(dst + r * LD + c) = make_float4(f[0], f[1], f[2], f[3]);
+// ROWS rows of 4-element groups from global (row stride st) into shared memory, all loads in flight together; rows at or
+// past `valid` are zeros.
+template <typename T, int D, int LD, int ROWS>
+OMNI_DEV void load_tile(float* dst, const T* src, int64_t st, int valid) {
+  constexpr int TOTAL = ROWS * (D / 4), N = (TOTAL + kThreads - 1) / kThreads, B = N < 8 ? N : 8;
+#pragma unroll 1
+  for (int i0 = 0; i0 < N; i0 += B) {
+    float f[B][4];
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      const int i = (i0 + b) * kThreads + threadIdx.x;
+      const int r = i / (D / 4), c = (i - r * (D / 4)) * 4;
+      f[b][0] = f[b][1] = f[b][2] = f[b][3] = 0.f;
+      if (r < valid && i < TOTAL) load4(src + (int64_t)r * st + c, f[b]);
+    }
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      const int i = (i0 + b) * kThreads + threadIdx.x;
+      const int r = i / (D / 4), c = (i - r * (D / 4)) * 4;
+      if (i < TOTAL) *reinterpret_cast<float4*>(dst + r * LD + c) = make_float4(f[b][0], f[b][1], f[b][2], f[b][3]);
+    }
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, int BM_>
 __global__ void __launch_bounds__(kThreads) packed_kernel(const PackedArgs a) {
-  using S = Shape<D>;
-  constexpr int BM = S::BM, BN = S::BN, LD = S::LD, LP = S::LP;
-  constexpr int MR = BM / 16, NR = BN / 16, DR = D / 16;
+  using S = Shape<D, BM_>;
+  constexpr int BM = S::BM, BN = S::BN, LD = S::LD, LP = S::LP, VW = S::VW;
+  constexpr int MR = BM / 16, NR = BN / 16, DR = D / 16, DG = DR / VW;
   extern __shared__ __align__(16) float sm[];
   float* qs = sm;
   float* ks = qs + BM * LD;
@@ -118,7 +134,7 @@ __global__ void __launch_bounds__(kThreads) packed_kernel(const PackedArgs a) {
   const int64_t lim0 = (q0 - qa) + 1 + (kb - ka) - (qb - qa);
   const int64_t keys = max((int64_t)0, lim0 + rows - 1);
   const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
-  load_tile<T, D, LD>(qs, reinterpret_cast<const T*>(a.q) + q0 * a.q_st + (int64_t)h * a.q_sh, a.q_st, BM, rows);
+  load_tile<T, D, LD, BM>(qs, reinterpret_cast<const T*>(a.q) + q0 * a.q_st + (int64_t)h * a.q_sh, a.q_st, rows);
   const T* kg = reinterpret_cast<const T*>(a.k) + ka * a.k_st + (int64_t)kvh * a.k_sh;
   const T* vg = reinterpret_cast<const T*>(a.v) + ka * a.v_st + (int64_t)kvh * a.v_sh;
   const float qscale = a.scale * kLog2e;
@@ -133,8 +149,8 @@ __global__ void __launch_bounds__(kThreads) packed_kernel(const PackedArgs a) {
   for (int64_t j0 = 0; j0 < keys; j0 += BN) {
     const int valid = (int)min((int64_t)BN, keys - j0);
     __syncthreads();  // the tile before is used up
-    load_tile<T, D, LD>(ks, kg + j0 * a.k_st, a.k_st, BN, valid);
-    load_tile<T, D, LD>(vs, vg + j0 * a.v_st, a.v_st, BN, valid);
+    load_tile<T, D, LD, BN>(ks, kg + j0 * a.k_st, a.k_st, valid);
+    load_tile<T, D, LD, BN>(vs, vg + j0 * a.v_st, a.v_st, valid);
     __syncthreads();
     float s[MR][NR];
 #pragma unroll
@@ -182,19 +198,39 @@ __global__ void __launch_bounds__(kThreads) packed_kernel(const PackedArgs a) {
       for (int d = 0; d < DR; ++d) o[i][d] *= f;
     }
     __syncwarp();  // a row's probabilities are written and read by the same half-warp
+    // Four keys at a time (rows past the valid ones hold zeros, their probabilities are zeros or hidden).
     auto values = [&](auto masked) {
 #pragma unroll 2
-      for (int k = 0; k < valid; ++k) {
-        float p[MR];
+      for (int k = 0; k < valid; k += 4) {
+        float p[MR][4];
 #pragma unroll
-        for (int i = 0; i < MR; ++i) p[i] = ps[(y + 16 * i) * LP + k];
+        for (int i = 0; i < MR; ++i) {
+          const float4 f = *reinterpret_cast<const float4*>(ps + (y + 16 * i) * LP + k);
+          p[i][0] = f.x, p[i][1] = f.y, p[i][2] = f.z, p[i][3] = f.w;
+        }
 #pragma unroll
-        for (int d = 0; d < DR; ++d) {
-          const float v = vs[k * LD + x + 16 * d];
+        for (int c = 0; c < 4; ++c) {
 #pragma unroll
-          for (int i = 0; i < MR; ++i) {
-            // A key past the row's does not enter, whatever its value holds.
-            if (!decltype(masked)::value || j0 + k < lim0 + y + 16 * i) o[i][d] = fmaf(p[i], v, o[i][d]);
+          for (int d = 0; d < DG; ++d) {
+            const float* src = vs + (k + c) * LD + (x + 16 * d) * VW;
+            float v[VW];
+            if constexpr (VW == 4) {
+              const float4 f = *reinterpret_cast<const float4*>(src);
+              v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+            } else if constexpr (VW == 2) {
+              const float2 f = *reinterpret_cast<const float2*>(src);
+              v[0] = f.x, v[1] = f.y;
+            } else {
+              v[0] = src[0];
+            }
+#pragma unroll
+            for (int i = 0; i < MR; ++i) {
+              // A key past the row's does not enter, whatever its value holds.
+              if (!decltype(masked)::value || j0 + k + c < lim0 + y + 16 * i) {
+#pragma unroll
+                for (int e = 0; e < VW; ++e) o[i][d * VW + e] = fmaf(p[i][c], v[e], o[i][d * VW + e]);
+              }
+            }
           }
         }
       }
@@ -211,34 +247,43 @@ __global__ void __launch_bounds__(kThreads) packed_kernel(const PackedArgs a) {
       const float inv = l[i] != 0.f ? 1.f / l[i] : 0.f;
       T* dst = reinterpret_cast<T*>(a.out) + ((q0 + r) * a.heads + h) * D;
 #pragma unroll
-      for (int d = 0; d < DR; ++d) dst[x + 16 * d] = Elem<T>::from_float(o[i][d] * inv);
+      for (int d = 0; d < DG; ++d)
+#pragma unroll
+        for (int e = 0; e < VW; ++e) dst[(x + 16 * d) * VW + e] = Elem<T>::from_float(o[i][d * VW + e] * inv);
     }
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, int BM>
 cudaError_t launch_t(const PackedArgs& a, cudaStream_t s) {
-  using S = Shape<D>;
+  using S = Shape<D, BM>;
   static bool configured = false;
   if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(packed_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES);
+    cudaError_t e = cudaFuncSetAttribute(packed_kernel<T, D, BM>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES);
     if (e != cudaSuccess) return e;
     configured = true;
   }
   // At most this many tiles: a sequence's last tile may be partly filled.
-  const int64_t tiles = a.q_tokens / S::BM + a.seqs;
-  return launch_dependent(packed_kernel<T, D>, dim3((unsigned)tiles, (unsigned)a.heads), dim3(kThreads), (size_t)S::BYTES, s, a);
+  const int64_t tiles = a.q_tokens / BM + a.seqs;
+  return launch_dependent(packed_kernel<T, D, BM>, dim3((unsigned)tiles, (unsigned)a.heads), dim3(kThreads), (size_t)S::BYTES, s, a);
+}
+
+template <typename T, int D>
+cudaError_t launch_bm(const PackedArgs& a, cudaStream_t s) {
+  constexpr int BM = D <= 128 ? 64 : 32;
+  if (a.q_tokens * a.heads < (int64_t)BM * 2 * device_sm_count()) return launch_t<T, D, 16>(a, s);
+  return launch_t<T, D, BM>(a, s);
 }
 
 template <typename T>
 cudaError_t launch_dim(const PackedArgs& a, cudaStream_t s) {
   switch (a.dim) {
-    case 16: return launch_t<T, 16>(a, s);
-    case 32: return launch_t<T, 32>(a, s);
-    case 64: return launch_t<T, 64>(a, s);
-    case 128: return launch_t<T, 128>(a, s);
-    case 256: return launch_t<T, 256>(a, s);
-    case 512: return launch_t<T, 512>(a, s);
+    case 16: return launch_bm<T, 16>(a, s);
+    case 32: return launch_bm<T, 32>(a, s);
+    case 64: return launch_bm<T, 64>(a, s);
+    case 128: return launch_bm<T, 128>(a, s);
+    case 256: return launch_bm<T, 256>(a, s);
+    case 512: return launch_bm<T, 512>(a, s);
     default: return cudaErrorInvalidValue;
   }
 }
