@@ -1,5 +1,5 @@
 // Causal attention of packed sequences with grouped heads: entry, and the CUDA-core kernel for what the tensor-core
-// kernels (prefill.cu, prefill_wide.cu) do not take (fp32, head dims other than 128 and 512).
+// kernels (prefill.cu, prefill_wide.cu) do not take (fp32, head dims under 64).
 //
 // Sequence s has queries q_offsets[s] .. q_offsets[s+1] - 1 and keys k_offsets[s] .. k_offsets[s+1] - 1; its last query
 // sees its last key (a chunk of a prompt attends to the keys before it), so query i sees i + 1 + lk - lq keys, none
@@ -291,8 +291,8 @@ cudaError_t launch_dim(const PackedArgs& a, cudaStream_t s) {
 }  // namespace packed
 
 cudaError_t launch_packed(int dtype, const PackedArgs& a, cudaStream_t stream) {
-  if (dtype == kBF16 && (a.dim == 128 || a.dim == 512) && a.heads / a.kv_heads <= 128 && a.k_tokens > 0) {
-    const cudaError_t e = a.dim == 128 ? launch_packed_tc(a, stream) : launch_packed_tc_wide(a, stream);
+  if (dtype == kBF16 && a.dim >= 64 && a.heads / a.kv_heads <= 128 && a.k_tokens > 0) {
+    const cudaError_t e = a.dim <= 128 ? launch_packed_tc(a, stream) : launch_packed_tc_wide(a, stream);
     if (e != cudaErrorNotSupported) return e;
   }
   return dtype == kBF16 ? packed::launch_dim<__nv_bfloat16>(a, stream) : packed::launch_dim<float>(a, stream);

@@ -88,7 +88,7 @@ struct PackedArgs {
   unsigned* counters;  // zero on entry, left zero (tensor-core kernels)
   int* status;
 };
-// Tensor-core kernels, bf16 head_dim 128 (prefill.cu) and 512 (prefill_wide.cu), at most 128 query heads per kv head;
+// Tensor-core kernels, bf16 head_dim 64 and 128 (prefill.cu), 256 and 512 (prefill_wide.cu), at most 128 query heads per kv head;
 // cudaErrorNotSupported where a tensor's strides have no tensor map.
 cudaError_t launch_packed_tc(const PackedArgs& a, cudaStream_t stream);
 cudaError_t launch_packed_tc_wide(const PackedArgs& a, cudaStream_t stream);

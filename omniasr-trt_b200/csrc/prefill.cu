@@ -48,27 +48,28 @@ namespace prefill {
 
 using namespace pfx;
 
-constexpr int D = 128;
 constexpr int BM = 128;  // queries per tile
 constexpr int BN = 128;  // keys per tile
-constexpr int TILE = BN * D * 2;
 constexpr int BOX = BN * 64 * 2;
-constexpr int QS = 2, KS = 3, VS = 2;  // query tiles (two units), K and V rings, in shared memory
-constexpr int Q_OFF = 0;
-constexpr int K_OFF = Q_OFF + QS * TILE;
-constexpr int V_OFF = K_OFF + KS * TILE;
-constexpr int SMEM_BYTES = V_OFF + VS * TILE;
+// What depends on the head dim: 128, or 64 (packed sequences; half the bytes per tile, so twice the tiles in flight).
+template <int D>
+struct Cfg {
+  static constexpr int TILE = BN * D * 2;
+  static constexpr int QS = 2, KS = D == 64 ? 6 : 3, VS = D == 64 ? 6 : 2;  // query tiles (two units), K and V rings
+  static constexpr int Q_OFF = 0;
+  static constexpr int K_OFF = Q_OFF + QS * TILE;
+  static constexpr int V_OFF = K_OFF + KS * TILE;
+  static constexpr int SMEM_BYTES = V_OFF + VS * TILE;
+};
 constexpr int NSB = 3;  // S buffers in TMEM: S(t + 3) needs only O += P(t) V to have completed
 constexpr int NWG = 2;        // softmax warpgroups; warpgroup x owns keys KW x .. KW x + KW - 1 of every tile
 constexpr int KW = BN / NWG;  // keys per softmax warpgroup (a multiple of the 16-key MMA step)
-constexpr int DW = D / NWG;   // head dims of O each softmax warpgroup rescales
 constexpr int W_EPI = 4 * NWG, W_LOADK = W_EPI + 4, W_MMA = W_LOADK + 1, W_LOADV = W_LOADK + 2, W_MMA_PV = W_LOADK + 3;
 constexpr int THREADS = 32 * (W_MMA_PV + 1);  // softmax, Q loader + epilogue, K loads, S MMAs, V loads, PV MMAs
 constexpr int SM_THREADS = 128 * NWG;
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t COL_S = 0, COL_O = 384;  // S buffer j at 128 j
 constexpr uint32_t IDESC_S = idesc_bf16(BM, BN, 0, 0);
-constexpr uint32_t IDESC_O = idesc_bf16(BM, D, 0, 1);
 constexpr float kRescale = 8.f;
 #ifndef OMNI_PREFILL_POLY_EVERY
 #define OMNI_PREFILL_POLY_EVERY 4
@@ -93,7 +94,9 @@ OMNI_DEV void unit_of(const Params& p, int u, int& b, int& h, int& qt) {
 // The CTA's control block: barriers, the row maxima exchanged between the softmax warpgroups, the unit's row sums
 // for the epilogue, flags. One static struct, padded to 1024 bytes, so that the dynamic tile ring after it starts
 // 1024-aligned (the kernel checks, and reports status bit 4 otherwise).
+template <int D>
 struct alignas(1024) Ctl {
+  static constexpr int QS = Cfg<D>::QS, KS = Cfg<D>::KS, VS = Cfg<D>::VS;
   uint64_t k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], q_full[QS], q_empty[QS];
   uint64_t s_full[NSB], p_full[NWG][NSB], pv_done[NSB], o_ready, o_free, l_full, l_free, drain;
   float tmax[NWG][BM];  // [warpgroup][row]: a tile's scaled row maxima, on the rare tiles that raise a max
@@ -103,17 +106,22 @@ struct alignas(1024) Ctl {
   uint64_t u_full[kUnitRing], u_empty[kUnitRing];  // packed: the units claimed, for all roles
   Unit unit[kUnitRing];
 };
-static_assert(sizeof(Ctl) + SMEM_BYTES <= 232448, "shared memory per block");
-static_assert(NSB * 128 + D <= TMEM_COLS, "S buffers and O in TMEM");
+static_assert(sizeof(Ctl<128>) + Cfg<128>::SMEM_BYTES <= 232448 && sizeof(Ctl<64>) + Cfg<64>::SMEM_BYTES <= 232448,
+              "shared memory per block");
+static_assert(NSB * 128 + 128 <= TMEM_COLS, "S buffers and O in TMEM");
 
 // Src: Sched (dense rows) or PackedSrc (packed sequences with grouped heads).
-template <typename Src>
+template <typename Src, int D>
 __global__ void __launch_bounds__(THREADS, 1)
     prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                    const __grid_constant__ CUtensorMap vmap, const Params p, const __grid_constant__ Src src) {
   constexpr bool PACKED = std::is_same_v<Src, PackedSrc>;
+  using C = Cfg<D>;
+  constexpr int TILE = C::TILE, QS = C::QS, KS = C::KS, VS = C::VS, Q_OFF = C::Q_OFF, K_OFF = C::K_OFF, V_OFF = C::V_OFF;
+  constexpr int DW = D / NWG;  // head dims of O each softmax warpgroup rescales
+  constexpr uint32_t IDESC_O = idesc_bf16(BM, D, 0, 1);
   extern __shared__ __align__(1024) unsigned char smem[];
-  __shared__ Ctl ctl;
+  __shared__ Ctl<D> ctl;
   uint64_t *k_full = ctl.k_full, *k_empty = ctl.k_empty, *v_full = ctl.v_full, *v_empty = ctl.v_empty;
   uint64_t *q_full = ctl.q_full, *q_empty = ctl.q_empty, *s_full = ctl.s_full, *pv_done = ctl.pv_done;
   uint64_t(*p_full)[NSB] = ctl.p_full;
@@ -223,9 +231,10 @@ __global__ void __launch_bounds__(THREADS, 1)
             const int qslot = n % QS;
             ok = n < QS || wait(&q_empty[qslot], (n / QS - 1) & 1);
             if (ok) {
-              mbar_arrive_expect_tx(&q_full[qslot], (uint32_t)(src.group * src.pos) * 256u);
-              tma_load_4d(smem + Q_OFF + qslot * TILE, &qmap, 0, 0, u.h, u.q0, &q_full[qslot]);
-              tma_load_4d(smem + Q_OFF + qslot * TILE + BOX, &qmap, 64, 0, u.h, u.q0, &q_full[qslot]);
+              mbar_arrive_expect_tx(&q_full[qslot], (uint32_t)(src.group * src.pos * D * 2));
+#pragma unroll
+              for (int x = 0; x < D / 64; ++x)
+                tma_load_4d(smem + Q_OFF + qslot * TILE + x * BOX, &qmap, 64 * x, 0, u.h, u.q0, &q_full[qslot]);
               issued_q = n + 1;
             }
             for (int kt = 0; kt < u.kt && ok; ++kt, ++tile) {
@@ -237,8 +246,9 @@ __global__ void __launch_bounds__(THREADS, 1)
                 break;
               }
               mbar_arrive_expect_tx(&k_full[slot], TILE);
-              tma_load_4d(smem + K_OFF + slot * TILE, &kmap, 0, u.k0 + kt * BN, u.h, 0, &k_full[slot]);
-              tma_load_4d(smem + K_OFF + slot * TILE + BOX, &kmap, 64, u.k0 + kt * BN, u.h, 0, &k_full[slot]);
+#pragma unroll
+              for (int x = 0; x < D / 64; ++x)
+                tma_load_4d(smem + K_OFF + slot * TILE + x * BOX, &kmap, 64 * x, u.k0 + kt * BN, u.h, 0, &k_full[slot]);
               issued_k = tile + 1;
             }
           }
@@ -275,8 +285,9 @@ __global__ void __launch_bounds__(THREADS, 1)
           const int slot = tile % ns, use = tile / ns;
           if (use >= 1 && !wait(&empty[slot], (use - 1) & 1)) break;
           mbar_arrive_expect_tx(&full[slot], TILE);
-          tma_load_4d(ring + slot * TILE, map, 0, row0 + kt * BN, u.h, b, &full[slot]);
-          tma_load_4d(ring + slot * TILE + BOX, map, 64, row0 + kt * BN, u.h, b, &full[slot]);
+#pragma unroll
+          for (int x = 0; x < D / 64; ++x)
+            tma_load_4d(ring + slot * TILE + x * BOX, map, 64 * x, row0 + kt * BN, u.h, b, &full[slot]);
           if (is_k) issued_k = tile + 1;
           else issued_v = tile + 1;
           OMNI_TRACE_AT(tile * 8 + (is_k ? 0 : 1));
@@ -527,8 +538,9 @@ __global__ void __launch_bounds__(THREADS, 1)
       unit_of(p, i, b, h, qt);
       const int qslot = n % QS;
       mbar_arrive_expect_tx(&q_full[qslot], TILE);
-      tma_load_4d(smem + Q_OFF + qslot * TILE, &qmap, 0, qt * BM, h, b, &q_full[qslot]);
-      tma_load_4d(smem + Q_OFF + qslot * TILE + BOX, &qmap, 64, qt * BM, h, b, &q_full[qslot]);
+#pragma unroll
+      for (int x = 0; x < D / 64; ++x)
+        tma_load_4d(smem + Q_OFF + qslot * TILE + x * BOX, &qmap, 64 * x, qt * BM, h, b, &q_full[qslot]);
       issued_q = n + 1;
     };
     if constexpr (!PACKED) {
@@ -580,12 +592,12 @@ __global__ void __launch_bounds__(THREADS, 1)
       // second half is in registers, before it is scaled and stored (measured: 183.0 us per config-4 call against
       // 186.5 us with four 32-column reads and the release after the last store).
 #pragma unroll 1
-      for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < D / 64; ++c) {
         uint32_t r0[64];
         tmem_ld32_async(tbase + lane_off + COL_O + c * 64, r0);
         tmem_ld32_async(tbase + lane_off + COL_O + c * 64 + 32, r0 + 32);
         tmem_wait_ld();
-        if (c == 1) {
+        if (c == D / 64 - 1) {
           tc_fence_before();
           mbar_arrive(&o_free);
         }
@@ -664,7 +676,7 @@ bool encode_map(CUtensorMap* map, const void* base, const cuuint64_t* dims, cons
 
 bool make_map(CUtensorMap* map, const void* base, int64_t b, int64_t h, int64_t w, int64_t sb, int64_t sh,
               int64_t sw) {
-  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)w, (cuuint64_t)h, (cuuint64_t)b};
+  cuuint64_t dims[4] = {128, (cuuint64_t)w, (cuuint64_t)h, (cuuint64_t)b};
   cuuint64_t strides[3] = {(cuuint64_t)sw * 2, (cuuint64_t)sh * 2, (cuuint64_t)sb * 2};
   cuuint32_t box[4] = {64, 128, 1, 1};
   return encode_map(map, base, dims, strides, box);
@@ -737,6 +749,7 @@ const pfx::Sched& prefill_round_robin() {
 
 cudaError_t launch_prefill(const PrefillArgs& a, cudaStream_t stream) {
   using namespace prefill;
+  constexpr int SMEM_BYTES = Cfg<128>::SMEM_BYTES;
   CUtensorMap qm, km, vm;
   if (!make_map(&qm, a.q, a.batch, a.heads, a.width, a.q_sb, a.q_sh, a.q_sw) ||
       !make_map(&km, a.k, a.batch, a.heads, a.width, a.k_sb, a.k_sh, a.k_sw) ||
@@ -744,7 +757,7 @@ cudaError_t launch_prefill(const PrefillArgs& a, cudaStream_t stream) {
     return cudaErrorInvalidValue;
   static bool configured = false;
   if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(prefill_kernel<Sched>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+    cudaError_t e = cudaFuncSetAttribute(prefill_kernel<Sched, 128>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
     if (e != cudaSuccess) return e;
     configured = true;
   }
@@ -769,7 +782,7 @@ cudaError_t launch_prefill(const PrefillArgs& a, cudaStream_t stream) {
   if (grid > units) grid = units;
   if (grid <= 0) return cudaSuccess;
   const Sched* sched = prefill_schedule(p.batch, p.heads, p.qtiles, p.group, grid);
-  return launch_dependent(prefill_kernel<Sched>, dim3(grid), dim3(THREADS), (size_t)SMEM_BYTES, stream, qm, km, vm, p,
+  return launch_dependent(prefill_kernel<Sched, 128>, dim3(grid), dim3(THREADS), (size_t)SMEM_BYTES, stream, qm, km, vm, p,
                           sched ? *sched : prefill_round_robin());
 }
 
@@ -814,14 +827,16 @@ int packed_grid(const PackedArgs& a, int positions) {
   return (int)std::min<int64_t>(device_sm_count(), units);
 }
 
-cudaError_t launch_packed_tc(const PackedArgs& a, cudaStream_t stream) {
+template <int D>
+cudaError_t launch_packed_d(const PackedArgs& a, cudaStream_t stream) {
   using namespace prefill;
+  constexpr int SMEM_BYTES = Cfg<D>::SMEM_BYTES;
   const int positions = BM / (a.heads / a.kv_heads);
   CUtensorMap qm, km, vm;
   if (!packed_maps(a, positions, &qm, &km, &vm)) return cudaErrorNotSupported;
   static bool configured = false;
   if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(prefill_kernel<PackedSrc>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+    cudaError_t e = cudaFuncSetAttribute(prefill_kernel<PackedSrc, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
     if (e != cudaSuccess) return e;
     configured = true;
   }
@@ -829,8 +844,12 @@ cudaError_t launch_packed_tc(const PackedArgs& a, cudaStream_t stream) {
   p.qscale = a.scale * kLog2e;
   p.out = reinterpret_cast<__nv_bfloat16*>(a.out);
   p.status = a.status;
-  return launch_dependent(prefill_kernel<PackedSrc>, dim3(packed_grid(a, positions)), dim3(THREADS), (size_t)SMEM_BYTES, stream,
-                          qm, km, vm, p, packed_source(a, positions));
+  return launch_dependent(prefill_kernel<PackedSrc, D>, dim3(packed_grid(a, positions)), dim3(THREADS), (size_t)SMEM_BYTES,
+                          stream, qm, km, vm, p, packed_source(a, positions));
+}
+
+cudaError_t launch_packed_tc(const PackedArgs& a, cudaStream_t stream) {
+  return a.dim == 64 ? launch_packed_d<64>(a, stream) : launch_packed_d<128>(a, stream);
 }
 
 }  // namespace omni

@@ -37,19 +37,24 @@ namespace prefillw {
 
 using namespace pfx;
 
-constexpr int D = 512;
-constexpr int DC = D / 128;        // 128-dim chunks of Q and K
-constexpr int DH = D / 2;          // head dims of O per pass
+constexpr int DH = 256;            // head dims of O per pass
 constexpr int NSUB = DH / 64;      // 64-dim V sub-chunks per pass
 constexpr int BM = 128;            // queries per tile
 constexpr int BN = 128;            // keys per tile
 constexpr int CHUNK = BN * 128 * 2;  // 128 rows x 128 dims
 constexpr int BOX = BN * 64 * 2;     // 128 rows x 64 dims: one TMA box
-constexpr int KS = 2, VS = 2;
-constexpr int Q_OFF = 0;
-constexpr int K_OFF = Q_OFF + DC * CHUNK;
-constexpr int V_OFF = K_OFF + KS * CHUNK;
-constexpr int SMEM_BYTES = V_OFF + VS * BOX;
+// What depends on the head dim: 512, or 256 (packed sequences; O of all 256 dims is one pass, and the query tile leaves room
+// for deeper rings).
+template <int D>
+struct Cfg {
+  static constexpr int DC = D / 128;   // 128-dim chunks of Q and K
+  static constexpr int PASSES = D / DH;
+  static constexpr int KS = D == 256 ? 3 : 2, VS = D == 256 ? 4 : 2;
+  static constexpr int Q_OFF = 0;
+  static constexpr int K_OFF = Q_OFF + DC * CHUNK;
+  static constexpr int V_OFF = K_OFF + KS * CHUNK;
+  static constexpr int SMEM_BYTES = V_OFF + VS * BOX;
+};
 constexpr int NSB = 2;
 constexpr int NWG = 2;
 constexpr int KW = BN / NWG;  // keys per softmax warpgroup
@@ -73,7 +78,9 @@ struct Params {
   int* status;
 };
 
+template <int D>
 struct alignas(1024) Ctl {
+  static constexpr int DC = Cfg<D>::DC, KS = Cfg<D>::KS, VS = Cfg<D>::VS;
   uint64_t k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], q_full[DC], q_empty[DC];
   uint64_t s_full[NSB], pv_done[NSB], p_full[NWG][NSB];
   uint64_t o_ready, o_free, l_full, l_free, drain;
@@ -84,17 +91,20 @@ struct alignas(1024) Ctl {
   uint64_t u_full[kUnitRing], u_empty[kUnitRing];  // packed: the units claimed, for all roles
   Unit unit[kUnitRing];
 };
-static_assert(sizeof(Ctl) + SMEM_BYTES <= 232448, "shared memory per block");
+static_assert(sizeof(Ctl<512>) + Cfg<512>::SMEM_BYTES <= 232448 && sizeof(Ctl<256>) + Cfg<256>::SMEM_BYTES <= 232448,
+              "shared memory per block");
 static_assert(NSB * 128 + DH <= TMEM_COLS, "S buffers and O in TMEM");
 
 // Src: Sched (dense rows) or PackedSrc (packed sequences with grouped heads).
-template <typename Src>
+template <typename Src, int D>
 __global__ void __launch_bounds__(THREADS, 1)
     prefill_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                         const __grid_constant__ CUtensorMap vmap, const Params p, const __grid_constant__ Src src) {
   constexpr bool PACKED = std::is_same_v<Src, PackedSrc>;
+  using C = Cfg<D>;
+  constexpr int DC = C::DC, PASSES = C::PASSES, KS = C::KS, VS = C::VS, Q_OFF = C::Q_OFF, K_OFF = C::K_OFF, V_OFF = C::V_OFF;
   extern __shared__ __align__(1024) unsigned char smem[];
-  __shared__ Ctl ctl;
+  __shared__ Ctl<D> ctl;
   uint64_t *k_full = ctl.k_full, *k_empty = ctl.k_empty, *v_full = ctl.v_full, *v_empty = ctl.v_empty;
   uint64_t *q_full = ctl.q_full, *q_empty = ctl.q_empty, *s_full = ctl.s_full, *pv_done = ctl.pv_done;
   uint64_t(*p_full)[NSB] = ctl.p_full;
@@ -198,10 +208,10 @@ __global__ void __launch_bounds__(THREADS, 1)
             ctl.unit[us] = u;
             mbar_arrive(&ctl.u_full[us]);
           }
-          for (int pass = 0; pass < 2 && ok; ++pass)
+          for (int pass = 0; pass < PASSES && ok; ++pass)
             for (int kt = 0; kt < u.kt && ok; ++kt) {
               // The next unit is claimed with the last tile, so that no CTA holds units it starts late.
-              if (pass == 1 && kt == u.kt - 1) claim = atomicAdd(src.counters, 1u);
+              if (pass == PASSES - 1 && kt == u.kt - 1) claim = atomicAdd(src.counters, 1u);
               for (int c = 0; c < DC && ok; ++c, ++kc) {
                 if (pass == 0 && kt == 0) {
                   ok = n < 1 || wait(&q_empty[c], (n - 1) & 1);
@@ -244,7 +254,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       int kc = 0;
       Unit u;
       for (int n = 0; get(n, u) && !abort_flag; ++n) {
-        for (int pass = 0; pass < 2 && !abort_flag; ++pass)
+        for (int pass = 0; pass < PASSES && !abort_flag; ++pass)
           for (int kt = 0; kt < u.kt && !abort_flag; ++kt)
             for (int c = 0; c < DC && !abort_flag; ++c, ++kc) {
               const int slot = kc % KS, use = kc / KS;
@@ -265,7 +275,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       int vc = 0;
       Unit u;
       for (int n = 0; get(n, u) && !abort_flag; ++n) {
-        for (int pass = 0; pass < 2 && !abort_flag; ++pass)
+        for (int pass = 0; pass < PASSES && !abort_flag; ++pass)
           for (int kt = 0; kt < u.kt && !abort_flag; ++kt)
             for (int sc = 0; sc < NSUB && !abort_flag; ++sc, ++vc) {
               const int slot = vc % VS, use = vc / VS;
@@ -288,7 +298,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       bool ok = true;
       Unit u;
       for (int n = 0; get(n, u) && ok && !abort_flag; ++n) {
-        for (int pass = 0; pass < 2 && ok; ++pass) {
+        for (int pass = 0; pass < PASSES && ok; ++pass) {
           for (int kt = 0; kt < u.kt && ok; ++kt, ++tile) {
             const int sb = tile % NSB;
             if (tile >= NSB && !wait(&pv_done[sb], ((tile - NSB) / NSB) & 1)) {
@@ -315,7 +325,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 mma_bf16_ss(dcol, qd + off, kd + off, IDESC_S, (c > 0 || kk > 0) ? 1u : 0u);
               }
               tc_commit(&k_empty[slot]);
-              if (pass == 1 && kt == u.kt - 1) tc_commit(&q_empty[c]);  // the unit's last read of query chunk c
+              if (pass == PASSES - 1 && kt == u.kt - 1) tc_commit(&q_empty[c]);  // the unit's last read of query chunk c
             }
             if (!ok) break;
             tc_commit(&s_full[sb]);
@@ -334,7 +344,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       bool ok = true;
       Unit u;
       for (int n = 0; get(n, u) && ok && !abort_flag; ++n) {
-        for (int pass = 0; pass < 2 && ok; ++pass, ++item) {
+        for (int pass = 0; pass < PASSES && ok; ++pass, ++item) {
           for (int kt = 0; kt < u.kt && ok; ++kt, ++tile) {
             const int pb = tile % NSB, pu = tile / NSB;
             if (kt == 0 && item >= 1 && !wait(&o_free, (item - 1) & 1)) {
@@ -391,7 +401,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (!more) break;
       __syncwarp();
       if (PACKED && lane == 0) put(n);
-      for (int pass = 0; pass < 2 && !quit; ++pass, ++item) {
+      for (int pass = 0; pass < PASSES && !quit; ++pass, ++item) {
         float m = -INFINITY, l = 0.f;
         for (int kt = 0; kt < u.kt; ++kt, ++tile) {
           const int sb = tile % NSB;
@@ -538,9 +548,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         live = q < p.width;
         row_out = p.out + (int64_t)u.b * p.out_sb + (int64_t)q * p.out_sw + (int64_t)u.h * p.out_sh;
       }
-      for (int pass = 0; pass < 2 && !abort_flag; ++pass, ++item) {
+      for (int pass = 0; pass < PASSES && !abort_flag; ++pass, ++item) {
         if constexpr (!PACKED) {
-          if (pass == 1 && q_loader) {  // the next unit's queries, as the last S MMAs of this one free the chunks
+          if (pass == PASSES - 1 && q_loader) {  // the next unit's queries, as the last S MMAs of this one free the chunks
             const int un = cta_unit(src, units, n + 1);
             if (un >= 0) load_q(n + 1, un);
           }
@@ -632,7 +642,7 @@ bool make_map(CUtensorMap* map, const void* base, int64_t b, int64_t h, int64_t 
     return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
   }();
   if (!fn) return false;
-  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)w, (cuuint64_t)h, (cuuint64_t)b};
+  cuuint64_t dims[4] = {512, (cuuint64_t)w, (cuuint64_t)h, (cuuint64_t)b};
   cuuint64_t strides[3] = {(cuuint64_t)sw * 2, (cuuint64_t)sh * 2, (cuuint64_t)sb * 2};
   cuuint32_t box[4] = {64, 128, 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
@@ -645,6 +655,7 @@ bool make_map(CUtensorMap* map, const void* base, int64_t b, int64_t h, int64_t 
 
 cudaError_t launch_prefill_wide(const PrefillArgs& a, cudaStream_t stream) {
   using namespace prefillw;
+  constexpr int SMEM_BYTES = Cfg<512>::SMEM_BYTES;
   CUtensorMap qm, km, vm;
   if (!make_map(&qm, a.q, a.batch, a.heads, a.width, a.q_sb, a.q_sh, a.q_sw) ||
       !make_map(&km, a.k, a.batch, a.heads, a.width, a.k_sb, a.k_sh, a.k_sw) ||
@@ -653,7 +664,7 @@ cudaError_t launch_prefill_wide(const PrefillArgs& a, cudaStream_t stream) {
   static bool configured = false;
   if (!configured) {
     cudaError_t e =
-        cudaFuncSetAttribute(prefill_wide_kernel<Sched>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+        cudaFuncSetAttribute(prefill_wide_kernel<Sched, 512>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
     if (e != cudaSuccess) return e;
     configured = true;
   }
@@ -674,19 +685,21 @@ cudaError_t launch_prefill_wide(const PrefillArgs& a, cudaStream_t stream) {
   if (grid > units) grid = units;
   if (grid <= 0) return cudaSuccess;
   const Sched* sched = prefill_schedule(p.batch, p.heads, p.qtiles, p.group, grid);
-  return launch_dependent(prefill_wide_kernel<Sched>, dim3(grid), dim3(THREADS), (size_t)SMEM_BYTES, stream, qm, km, vm, p,
+  return launch_dependent(prefill_wide_kernel<Sched, 512>, dim3(grid), dim3(THREADS), (size_t)SMEM_BYTES, stream, qm, km, vm, p,
                           sched ? *sched : prefill_round_robin());
 }
 
-cudaError_t launch_packed_tc_wide(const PackedArgs& a, cudaStream_t stream) {
+template <int D>
+cudaError_t launch_packed_wide_d(const PackedArgs& a, cudaStream_t stream) {
   using namespace prefillw;
+  constexpr int SMEM_BYTES = Cfg<D>::SMEM_BYTES;
   const int positions = BM / (a.heads / a.kv_heads);
   CUtensorMap qm, km, vm;
   if (!packed_maps(a, positions, &qm, &km, &vm)) return cudaErrorNotSupported;
   static bool configured = false;
   if (!configured) {
     cudaError_t e =
-        cudaFuncSetAttribute(prefill_wide_kernel<PackedSrc>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+        cudaFuncSetAttribute(prefill_wide_kernel<PackedSrc, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
     if (e != cudaSuccess) return e;
     configured = true;
   }
@@ -694,8 +707,12 @@ cudaError_t launch_packed_tc_wide(const PackedArgs& a, cudaStream_t stream) {
   p.qscale = a.scale * kLog2e;
   p.out = reinterpret_cast<__nv_bfloat16*>(a.out);
   p.status = a.status;
-  return launch_dependent(prefill_wide_kernel<PackedSrc>, dim3(packed_grid(a, positions)), dim3(THREADS), (size_t)SMEM_BYTES,
+  return launch_dependent(prefill_wide_kernel<PackedSrc, D>, dim3(packed_grid(a, positions)), dim3(THREADS), (size_t)SMEM_BYTES,
                           stream, qm, km, vm, p, packed_source(a, positions));
+}
+
+cudaError_t launch_packed_tc_wide(const PackedArgs& a, cudaStream_t stream) {
+  return a.dim == 256 ? launch_packed_wide_d<256>(a, stream) : launch_packed_wide_d<512>(a, stream);
 }
 
 }  // namespace omni
