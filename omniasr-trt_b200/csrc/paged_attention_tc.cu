@@ -1,5 +1,5 @@
 // Attention of each row's newest tokens over a paged KV cache on the 5th-generation tensor cores (tcgen05 + TMEM):
-// bf16 queries, bf16 or e4m3 pages, head_dim 128, 256 or 512, pages of 8 .. 64 positions (powers of two) or of a multiple
+// bf16 queries, bf16 or e4m3 pages, head_dim 64, 128, 256 or 512, pages of 8 .. 64 positions (powers of two) or of a multiple
 // of 128.
 //
 // A unit is (row, kv head, chunk of at most 16 query columns): the row's T * G query vectors on that kv head share every
@@ -42,25 +42,33 @@ namespace pagedtc {
 constexpr int BN = 128;            // keys per tile (the MMA's M)
 constexpr int kMaxCols = 16;       // query columns per unit
 constexpr int kMaxRows = 1024;     // rows of one launch
-constexpr int kBox = BN * 128;     // 128 keys x 128 bytes
-constexpr int kScaleStages = 8;    // tiles of scale bytes in shared memory
-constexpr int kCtlBytes = 3072;    // control block (below)
+constexpr int kScaleStages = 16;   // tiles of scale bytes in shared memory
+constexpr int kMaxSlots = 20;      // ring slots
+constexpr uint32_t kLayoutSw64 = 4;  // 64-byte swizzle (the TMA's CU_TENSOR_MAP_SWIZZLE_64B)
+constexpr int kCtlBytes = 3584;    // control block (below)
 constexpr float kRaise = 8.f;      // log2: a weight may reach 2^8 before its column's maximum is raised
 constexpr float kHead8 = 4.f;      // e4m3: the maximum kept this far (log2) below the largest exponent seen
 constexpr float kBelow = 64.f;     // bf16: a unit starts from maximum 0 unless its scores lie 2^64 below
 
 template <bool FP8, int DIM, int NQT>
 struct Cfg {
-  static constexpr int DC = DIM / 128;                     // 128-dim chunks
-  static constexpr int SLOT = FP8 ? kBox : 2 * kBox;       // one chunk of a K or V tile
+  static constexpr int CD = DIM < 128 ? DIM : 128;         // head dims of a chunk
+  static constexpr int DC = DIM / CD;                      // chunks
+  static constexpr int ES = FP8 ? 1 : 2;
+  static constexpr int ROWB = CD * ES < 128 ? CD * ES : 128;  // bytes of a box's row, the swizzle's width
+  static constexpr int NB = CD * ES / ROWB;                // boxes per chunk
+  static constexpr int BOX = BN * ROWB;                    // 128 keys of a box
+  static constexpr int GRP = 8 * ROWB;                     // eight of its rows
+  static constexpr uint32_t LAYOUT = ROWB == 128 ? kLayoutSw128 : kLayoutSw64;
+  static constexpr int SLOT = NB * BOX;                    // one chunk of a K or V tile
   static constexpr int N = FP8 ? (2 * NQT < 16 ? 16 : 2 * NQT) : 16;  // MMA columns
-  static constexpr int QBOX = N * 128;                     // N rows x 128 bytes of the query
-  static constexpr int QB = DC * (FP8 ? 1 : 2) * QBOX;     // one query buffer
+  static constexpr int QBOX = N * ROWB;                    // N rows of the query
+  static constexpr int QB = DC * NB * QBOX;                // one query buffer
   static constexpr int PB = BN * N * (FP8 ? 1 : 2);        // one P buffer
   static constexpr int QN = !FP8 && DIM == 128 ? 3 : QB <= 8192 ? 4 : 2;  // query buffers
   static constexpr int FIXED = QN * QB + 2 * PB + 2 * kMaxRows * 4 + 64 + (FP8 ? kScaleStages * 2 * BN : 0);
   static constexpr int FIT = (232448 - kCtlBytes - 1024 - FIXED) / SLOT;
-  static constexpr int SLOTS = FIT > 12 ? 12 : FIT;
+  static constexpr int SLOTS = FIT > kMaxSlots ? kMaxSlots : FIT;
   static constexpr int Q_OFF = SLOTS * SLOT;
   static constexpr int P_OFF = Q_OFF + QN * QB;
   static constexpr int SC_OFF = P_OFF + 2 * PB;            // scale bytes [stage][K, V][128]
@@ -207,7 +215,7 @@ struct Walk {
 };
 
 struct alignas(16) Ctl {
-  uint64_t full[12], empty[12];
+  uint64_t full[kMaxSlots], empty[kMaxSlots];
   uint64_t s_full[2], s_free[2], p_full[2], pv_done[2], q_full[4], q_empty[4], o_full[2], o_free[2], ml_full[2], ml_free[2];
   uint64_t sc_full[kScaleStages];
   uint64_t drain;
@@ -218,7 +226,7 @@ struct alignas(16) Ctl {
   int wsum[kThreads / 32];
   uint32_t tmem_base;
   int abort_flag;
-  int loads[12];                  // loads issued into each ring slot
+  int loads[kMaxSlots];                  // loads issued into each ring slot
   int last;                       // epilogue: this CTA joins the unit
   unsigned bad;                   // epilogue: columns to redo
 };
@@ -285,8 +293,7 @@ template <bool FP8, int DIM, int NQT>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ Params p) {
   using C = Cfg<FP8, DIM, NQT>;
-  constexpr int DC = C::DC, N = C::N, SLOTS = C::SLOTS, SLOT = C::SLOT;
-  constexpr int NB = FP8 ? 1 : 2;  // 128-byte boxes per chunk
+  constexpr int CD = C::CD, DC = C::DC, N = C::N, SLOTS = C::SLOTS, SLOT = C::SLOT, ROWB = C::ROWB, NB = C::NB;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ Ctl ctl;
@@ -319,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&ctl.drain, 2);
     mbar_fence_init();
     abort_flag = 0;
-    for (int s = 0; s < 12; ++s) loads[s] = 0;
+    for (int s = 0; s < kMaxSlots; ++s) loads[s] = 0;
     ctl.bad = 0;
   }
   if (warp == W_EPI) tmem_alloc(&ctl.tmem_base, C::TMEM);
@@ -468,20 +475,22 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = false;
           break;
         }
-        if (leader) mbar_arrive_expect_tx(&ctl.full[slot], (uint32_t)(x.live * rows_box * 128 * NB));
+        if (leader) mbar_arrive_expect_tx(&ctl.full[slot], (uint32_t)(x.live * rows_box * ROWB * NB));
         for (int k = 0; k < x.live; ++k) {
           const int id = __shfl_sync(0xffffffffu, x.id, k);
           if (leader) {
-            unsigned char* dst = smem + slot * SLOT + k * rows_box * 128;
+            unsigned char* dst = smem + slot * SLOT + k * rows_box * ROWB;
 #pragma unroll
-            for (int h = 0; h < NB; ++h) tma_load_4d(dst + h * kBox, map, c * 128 + h * 64, x.row, x.h, id, &ctl.full[slot]);
+            for (int h = 0; h < NB; ++h)
+              tma_load_4d(dst + h * C::BOX, map, c * CD + h * (ROWB / C::ES), x.row, x.h, id, &ctl.full[slot]);
           }
         }
         if (leader) loads[slot] = use + 1;
         __syncwarp();
         if (FP8 && is_k && c == 0) {
-          // Four keys' scale bytes per lane (within one page), copied without waiting for them. The stage is free: K of
-          // this tile went into a slot whose S^T, at most six tiles back, followed the reads of the stage's last tile.
+          // Four keys' scale bytes per lane (within one page), copied without waiting for them. The stage is free: this K
+          // chunk went into a slot whose last one, at most 20 chunks (ten tiles) back, has been used, and an S^T is issued
+          // after the reads of the scales two tiles before it.
           const int st = i % kScaleStages;
           const int pi = small ? (4 * lane) >> p.page_shift : 0;
           const int64_t id = __shfl_sync(0xffffffffu, x.id, pi);
@@ -510,8 +519,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // The issuing warps run converged, one elected lane issuing, so that the descriptors are warp-uniform: with a lone
     // thread issuing both products, four MMAs and their two commits took 520 clocks and a tile 1800.
     constexpr uint32_t IS = FP8 ? idesc_e4m3(128, N, 0, 0) : idesc_bf16(128, N, 0, 0);
-    const uint64_t kd0 = smem_desc(smem_addr(smem), 16, 1024, kLayoutSw128);
-    const uint64_t qd0 = smem_desc(smem_addr(smem + C::Q_OFF), 16, 1024, kLayoutSw128);
+    const uint64_t kd0 = smem_desc(smem_addr(smem), 16, C::GRP, C::LAYOUT);
+    const uint64_t qd0 = smem_desc(smem_addr(smem + C::Q_OFF), 16, C::GRP, C::LAYOUT);
     const bool leader = elect_one();
     Walk w;
     w.init(pre, p.rows, per_row, c0, c1);
@@ -534,9 +543,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint64_t kd = kd0 + (uint64_t)(slot * (SLOT >> 4));
             const uint32_t d = tbase + b * N;
 #pragma unroll
-            for (int kk = 0; kk < (FP8 ? 4 : 8); ++kk) {
-              const uint64_t ko = (uint64_t)(((kk >> 2) * kBox + (kk & 3) * 32) >> 4);
-              const uint64_t qo = (uint64_t)(((c * NB + (kk >> 2)) * C::QBOX + (kk & 3) * 32) >> 4);
+            for (int kk = 0; kk < CD * C::ES / 32; ++kk) {  // 32 bytes of each row per MMA
+              const int box = kk * 32 / ROWB, off = kk * 32 % ROWB;
+              const uint64_t ko = (uint64_t)((box * C::BOX + off) >> 4);
+              const uint64_t qo = (uint64_t)(((c * NB + box) * C::QBOX + off) >> 4);
               if constexpr (FP8) mma_f8_ss(d, kd + ko, qd + qo, IS, (c > 0 || kk > 0) ? 1u : 0u);
               else mma_bf16_ss(d, kd + ko, qd + qo, IS, (c > 0 || kk > 0) ? 1u : 0u);
             }
@@ -560,7 +570,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == W_PV) {
     // ------------------------------------------------------------------ O^T += V(i)^T P(i)^T
     constexpr uint32_t IO = FP8 ? idesc_e4m3(128, N, 1, 1) : idesc_bf16(128, N, 1, 1);
-    const uint64_t vd0 = smem_desc(smem_addr(smem), kBox, 1024, kLayoutSw128);
+    // (head_dim 64: the MMA's upper 64 rows read the same dims again, and nothing reads them.)
+    const uint64_t vd0 = smem_desc(smem_addr(smem), CD == 64 ? 0 : C::BOX, C::GRP, C::LAYOUT);
     const uint64_t pd0 = smem_desc(smem_addr(smem + C::P_OFF), 128, 2048, kLayoutNone);
     const bool leader = elect_one();
     Walk w;
@@ -587,8 +598,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t d = tbase + C::S_COLS + ((ob * 2 + b) * DC + c) * N;
 #pragma unroll
             for (int kk = 0; kk < (FP8 ? 4 : 8); ++kk) {
-              if constexpr (FP8) mma_f8_ss(d, vd + kk * (4096 >> 4), pd + kk * (512 >> 4), IO, kk > 0 ? 1u : fresh);
-              else mma_bf16_ss(d, vd + kk * (2048 >> 4), pd + kk * (256 >> 4), IO, kk > 0 ? 1u : fresh);
+              if constexpr (FP8) mma_f8_ss(d, vd + kk * (4 * C::GRP >> 4), pd + kk * (512 >> 4), IO, kk > 0 ? 1u : fresh);
+              else mma_bf16_ss(d, vd + kk * (2 * C::GRP >> 4), pd + kk * (256 >> 4), IO, kk > 0 ? 1u : fresh);
             }
             tc_commit(&ctl.empty[slot]);
           }
@@ -787,11 +798,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!wait_issued((vc + c) % SLOTS, (vc + c) / SLOTS + 1)) break;
             wait(&ctl.full[(vc + c) % SLOTS], ((vc + c) / SLOTS) & 1);
             if (key >= need) {
-              unsigned char* row = smem + ((vc + c) % SLOTS) * SLOT + key_in * 128;
+              unsigned char* row = smem + ((vc + c) % SLOTS) * SLOT + key_in * ROWB;
 #pragma unroll
-              for (int k = 0; k < 8; ++k) {
+              for (int k = 0; k < ROWB / 16; ++k) {
 #pragma unroll
-                for (int x2 = 0; x2 < NB; ++x2) *reinterpret_cast<uint4*>(row + x2 * kBox + k * 16) = make_uint4(0u, 0u, 0u, 0u);
+                for (int x2 = 0; x2 < NB; ++x2) *reinterpret_cast<uint4*>(row + x2 * C::BOX + k * 16) = make_uint4(0u, 0u, 0u, 0u);
               }
             }
           }
@@ -831,7 +842,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // those of segment n when segment n + QN's are written.)
     constexpr int QC = (NQT + 3) / 4;
     const int wq = warp - W_EPI;
-    uint2 qr[QC][DC];  // four dims per lane of each 128-dim chunk
+    uint2 qr[QC][DC];  // four dims per lane of each chunk (head_dim 64: of the first 16 lanes)
     auto query_load = [&]() {
       const int h = sq.u / p.chunks, col0 = (sq.u - h * p.chunks) * p.chunk_cols;
       const int ncol = min(p.chunk_cols, p.cols - col0);
@@ -842,10 +853,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           int tt;
           const uint2* src = reinterpret_cast<const uint2*>(p.q + query_row(p, sq.b, h, col0 + j, &tt) * DIM) + lane;
 #pragma unroll
-          for (int c = 0; c < DC; ++c) qr[k][c] = __ldg(src + c * 32);
+          for (int c = 0; c < DC; ++c) qr[k][c] = CD == 128 || lane < 16 ? __ldg(src + c * 32) : make_uint2(0u, 0u);
         }
       }
     };
+    // The 16-byte words of row r are stored at index ^ swizzle(r) (the 128- or 64-byte swizzle of the tensor maps).
+    auto swizzle = [](int r) { return ROWB == 128 ? r & 7 : (r >> 1) & 3; };
     auto query_store = [&](int n) {
       unsigned char* qb = smem + C::Q_OFF + (n % C::QN) * C::QB;
       const int h = sq.u / p.chunks, col0 = (sq.u - h * p.chunks) * p.chunk_cols;
@@ -887,15 +900,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             const int r2 = NQT + j;
             unsigned char* box = qb + c * C::QBOX;
-            *reinterpret_cast<uint32_t*>(box + j * 128 + (((lane >> 2) ^ (j & 7)) << 4) + (lane & 3) * 4) = hi;
-            *reinterpret_cast<uint32_t*>(box + r2 * 128 + (((lane >> 2) ^ (r2 & 7)) << 4) + (lane & 3) * 4) = lo;
+            if (CD == 128 || lane < 16) {
+              *reinterpret_cast<uint32_t*>(box + j * ROWB + (((lane >> 2) ^ swizzle(j)) << 4) + (lane & 3) * 4) = hi;
+              *reinterpret_cast<uint32_t*>(box + r2 * ROWB + (((lane >> 2) ^ swizzle(r2)) << 4) + (lane & 3) * 4) = lo;
+            }
           }
           if (lane == 0) ctl.cq[n & 7][j] = p.qscale * __uint_as_float((uint32_t)(e + 127) << 23);
         } else {
 #pragma unroll
           for (int c = 0; c < DC; ++c) {  // lanes 0-15 the chunk's first 64 dims, 16-31 the others
-            unsigned char* box = qb + (2 * c + (lane >> 4)) * C::QBOX;
-            *reinterpret_cast<uint2*>(box + j * 128 + ((((lane & 15) >> 1) ^ (j & 7)) << 4) + (lane & 1) * 8) = qr[k][c];
+            unsigned char* box = qb + (NB * c + (lane >> 4)) * C::QBOX;
+            if (CD == 128 || lane < 16)
+              *reinterpret_cast<uint2*>(box + j * ROWB + ((((lane & 15) >> 1) ^ swizzle(j)) << 4) + (lane & 1) * 8) = qr[k][c];
           }
         }
       }
@@ -946,8 +962,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (j < ncol) {
             const int64_t row = ((int64_t)s.b * p.tokens + tt) * p.heads + h * p.group + g;
             const float r = o[j] * (sum[j] != 0.f ? 1.f / sum[j] : 0.f);
-            if (!(fabsf(r) <= 3.3e38f)) bad |= 1u << j;
-            p.out[row * DIM + c * 128 + d] = __float2bfloat16_rn(r);
+            if (!(fabsf(r) <= 3.3e38f) && (CD == 128 || d < CD)) bad |= 1u << j;
+            if (CD == 128 || d < CD) p.out[row * DIM + c * CD + d] = __float2bfloat16_rn(r);
           }
           if (++g == p.group) {
             g = 0;
@@ -982,7 +998,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else {
 #pragma unroll
           for (int j = 0; j < NQT; ++j)
-            if (j < ncol) p.part_o[(at + j) * DIM + c * 128 + d] = o[j];
+            if (j < ncol && (CD == 128 || d < CD)) p.part_o[(at + j) * DIM + c * CD + d] = o[j];
         }
       }
       if (!emit) {
@@ -1020,7 +1036,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int j = 0; j < NQT; ++j) {
                 e[j] = j < ncol ? __ldcg(p.part_ml + src + j) : make_float2(0.f, 0.f);
-                v[j] = j < ncol ? __ldcg(p.part_o + (src + j) * DIM + c * 128 + d) : 0.f;
+                v[j] = j < ncol && (CD == 128 || d < CD) ? __ldcg(p.part_o + (src + j) * DIM + c * CD + d) : 0.f;
               }
 #pragma unroll
               for (int j = 0; j < NQT; ++j) {
@@ -1098,11 +1114,12 @@ bool page_map(CUtensorMap* map, const void* base, const PageCache& c) {
   auto st = [&](int64_t extent, int64_t stride) { return (cuuint64_t)(extent > 1 ? stride * es : 16); };
   const cuuint64_t dims[4] = {(cuuint64_t)c.dim, (cuuint64_t)c.page, (cuuint64_t)c.kv_heads, (cuuint64_t)c.pages};
   const cuuint64_t strides[3] = {st(c.page, c.s_pos), st(c.kv_heads, c.s_head), st(c.pages, c.s_page)};
-  const cuuint32_t box[4] = {(cuuint32_t)(fp8 ? 128 : 64), (cuuint32_t)(c.page < BN ? c.page : BN), 1, 1};
+  const bool half = fp8 && c.dim == 64;  // 64-byte rows
+  const cuuint32_t box[4] = {(cuuint32_t)(fp8 && !half ? 128 : 64), (cuuint32_t)(c.page < BN ? c.page : BN), 1, 1};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   if (!strides[0] || !strides[1] || !strides[2]) return false;
   return fn(map, fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides,
-            box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, half ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -1129,6 +1146,7 @@ cudaError_t launch_cols(const CUtensorMap& k, const CUtensorMap& v, const Params
 
 template <bool FP8>
 cudaError_t launch_dim(const CUtensorMap& k, const CUtensorMap& v, const Params& p, int grid, cudaStream_t s) {
+  if (p.c.dim == 64) return launch_cols<FP8, 64>(k, v, p, grid, s);
   if (p.c.dim == 128) return launch_cols<FP8, 128>(k, v, p, grid, s);
   if (p.c.dim == 256) return launch_cols<FP8, 256>(k, v, p, grid, s);
   return launch_cols<FP8, 512>(k, v, p, grid, s);
@@ -1138,7 +1156,7 @@ cudaError_t launch_dim(const CUtensorMap& k, const CUtensorMap& v, const Params&
 
 bool paged_tc_supported(int dtype, int type, int dim, int page) {
   const bool pages = page >= 128 ? page % 128 == 0 : page >= 8 && (page & (page - 1)) == 0;
-  return dtype == kBF16 && (type == kBF16 || type == kFp8) && (dim == 128 || dim == 256 || dim == 512) && pages;
+  return dtype == kBF16 && (type == kBF16 || type == kFp8) && dim >= 64 && pages;
 }
 
 size_t paged_tc_workspace(int dim) {
