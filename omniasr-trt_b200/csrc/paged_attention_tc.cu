@@ -44,6 +44,7 @@ constexpr int kMaxCols = 16;       // query columns per unit
 constexpr int kMaxRows = 1024;     // rows of one launch
 constexpr int kScaleStages = 16;   // tiles of scale bytes in shared memory
 constexpr int kMaxSlots = 20;      // ring slots
+constexpr int kJoin = 16;          // parts of a cut unit that one CTA joins at a time
 constexpr uint32_t kLayoutSw64 = 4;  // 64-byte swizzle (the TMA's CU_TENSOR_MAP_SWIZZLE_64B)
 constexpr int kCtlBytes = 3584;    // control block (below)
 constexpr float kRaise = 8.f;      // log2: a weight may reach 2^8 before its column's maximum is raised
@@ -98,7 +99,8 @@ struct Params {
   int cap;                         // keys a row can have
   int page_shift;                  // log2(page) for pages below 128, else -1
   float qscale;
-  unsigned* counters;              // per CTA: partial results published of the unit that starts there and is cut
+  unsigned* counters;              // [CTA]: parts (or runs of parts) published of the cut unit that begins there;
+                                   // [grid + 2 CTA + place]: parts of the run that begins with that slot's
   float* part_o;                   // [2 * CTA + place][column][DIM]; place 0: a unit begun in an earlier CTA, 1: in this one
   float2* part_ml;                 // [2 * CTA + place][column]
   int* status;
@@ -177,42 +179,76 @@ OMNI_DEV void warp_all(float (&v)[NV]) {
 // A CTA's part of one unit: tiles [t0, t1) of the unit's nt.
 struct Seg {
   int b, u;        // row; unit within the row (kv head * chunks + chunk)
+  int h, col0, ncol;  // the unit's kv head, first query column and columns
+  int need;        // keys of the row's last query
   int t0, t1, nt;
   int first;       // first tile of the unit in the global numbering
 };
 
+// The segments of a CTA, in order. One division, in init: the roles come here between their tiles.
 struct Walk {
-  const int* pre;
-  int rows, per_row, pos, end, b;
-  OMNI_DEV void init(const int* pre_, int rows_, int per_row_, int c0, int c1) {
+  const Params* p;
+  const int* pre;   // tiles before each row
+  const int* len;
+  int pos, end, b, u, nt, t, need;
+  OMNI_DEV void row() {  // the row's tiles
+    need = min(p->cap, len[b] + p->tokens - 1);
+    nt = (need + BN - 1) / BN;
+  }
+  OMNI_DEV void init(const Params& p_, const int* pre_, const int* len_, int c0, int c1) {
+    p = &p_;
     pre = pre_;
-    rows = rows_;
-    per_row = per_row_;
+    len = len_;
     pos = c0;
     end = c1;
-    int lo = 0, hi = rows - 1;  // the first row that ends past c0
+    int lo = 0, hi = p->rows - 1;  // the first row that ends past c0
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
       if (pre[mid + 1] > c0) hi = mid;
       else lo = mid + 1;
     }
     b = lo;
+    row();
+    const int r = c0 - pre[b];
+    u = nt > 0 ? r / nt : 0;
+    t = r - u * nt;
   }
   OMNI_DEV bool next(Seg& s) {
     if (pos >= end) return false;
-    while (pre[b + 1] <= pos) ++b;  // rows without keys have no tiles
-    const int nt = (pre[b + 1] - pre[b]) / per_row;
-    const int r = pos - pre[b];
+    if (t >= nt) {
+      t = 0;
+      if (++u >= p->c.kv_heads * p->chunks) {
+        u = 0;
+        do ++b;
+        while (pre[b + 1] <= pos);  // rows without keys have no tiles
+        row();
+      }
+    }
     s.b = b;
+    s.u = u;
+    s.need = need;
     s.nt = nt;
-    s.u = r / nt;
-    s.t0 = r - s.u * nt;
-    s.t1 = min(nt, s.t0 + (end - pos));
-    s.first = pos - s.t0;
+    s.t0 = t;
+    s.t1 = min(nt, t + (end - pos));
+    s.first = pos - t;
+    s.h = u;
+    s.col0 = 0;
+    if (p->chunks > 1) {
+      s.h = u / p->chunks;
+      s.col0 = (u - s.h * p->chunks) * p->chunk_cols;
+    }
+    s.ncol = min(p->chunk_cols, p->cols - s.col0);
+    t = s.t1;
     pos += s.t1 - s.t0;
     return true;
   }
 };
+
+// Token and head-of-group of query column `col` (a division only where a unit holds more than one token).
+OMNI_DEV void column(const Params& p, int col, int& tok, int& g) {
+  tok = p.tokens > 1 ? col / p.group : 0;
+  g = col - tok * p.group;
+}
 
 struct alignas(16) Ctl {
   uint64_t full[kMaxSlots], empty[kMaxSlots];
@@ -232,10 +268,11 @@ struct alignas(16) Ctl {
 };
 static_assert(sizeof(Ctl) <= kCtlBytes, "control block");
 
-// The query row and the keys that column `col` of row b, kv head h sees.
+// The query row of column `col` of row b, kv head h.
 OMNI_DEV int64_t query_row(const Params& p, int b, int h, int col, int* t) {
-  *t = col / p.group;
-  return ((int64_t)b * p.tokens + *t) * p.heads + h * p.group + (col - *t * p.group);
+  int g;
+  column(p, col, *t, g);
+  return ((int64_t)b * p.tokens + *t) * p.heads + h * p.group + g;
 }
 
 // One column straight from the formula, by one warp: for a draft column whose tensor-core result is not finite, because a
@@ -405,7 +442,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       ++use;
     }
   };
-  auto need_of = [&](int b) { return min(p.cap, len[b] + p.tokens - 1); };  // of a row that has tiles
   // Ring positions of tile i's first K and V chunk, in the MMAs' order: K0 K1 K2 V0 K3 V1 .. K(n-1) V(n-3) V(n-2) V(n-1).
   auto k_chunk = [&](int i) { return DC * (i < 2 ? i : 2 * i - 2); };
   auto v_chunk = [&](int i) { return DC * min(2 * i + 3, tiles + i); };
@@ -431,16 +467,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int rows_box = small ? p.c.page : BN;
     const int boxes = small ? BN >> p.page_shift : 1;
     Walk w;
-    w.init(pre, p.rows, per_row, c0, c1);
+    w.init(p, pre, len, c0, c1);
     Seg s{};
     int t = 0, ntile = 0;  // the tile in hand
     struct Tile {
       int h, live, row, id;  // kv head, boxes with keys, first row within the page, this lane's page
     };
     auto fetch = [&](Tile& x) {  // the tile (s, t): its page numbers start to load
-      const int need = need_of(s.b);
-      const int left = need - t * BN;
-      x.h = s.u / p.chunks;
+      const int left = s.need - t * BN;
+      x.h = s.h;
       x.live = small ? min(boxes, (left + rows_box - 1) >> p.page_shift) : 1;
       x.row = small ? 0 : (t * BN) % p.c.page;
       const int pi = small ? ((t * BN) >> p.page_shift) + lane : (t * BN) / p.c.page;
@@ -465,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         raise_status(p.status, kStatusIndex);
         x.id = 0;
       }
-      const int left = need_of(s.b) - t * BN;  // keys of this tile (before the walk goes on)
+      const int left = s.need - t * BN;  // keys of this tile (before the walk goes on)
       if (step()) fetch(nxt);
       bool ok = true;
       for (int c = 0; c < DC; ++c) {
@@ -523,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t qd0 = smem_desc(smem_addr(smem + C::Q_OFF), 16, C::GRP, C::LAYOUT);
     const bool leader = elect_one();
     Walk w;
-    w.init(pre, p.rows, per_row, c0, c1);
+    w.init(p, pre, len, c0, c1);
     Seg s{};
     int i = 0, slot = 0, use = 0;
     bool ok = true;
@@ -575,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t pd0 = smem_desc(smem_addr(smem + C::P_OFF), 128, 2048, kLayoutNone);
     const bool leader = elect_one();
     Walk w;
-    w.init(pre, p.rows, per_row, c0, c1);
+    w.init(p, pre, len, c0, c1);
     Seg s{};
     int i = 0, slot = v_chunk(0) % SLOTS, use = v_chunk(0) / SLOTS;
     bool ok = true;
@@ -625,15 +660,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int bar = b == 0 ? 1 : 3;
     const uint32_t lane_off = (uint32_t)(32 * wq) << 16;
     Walk w;
-    w.init(pre, p.rows, per_row, c0, c1);
+    w.init(p, pre, len, c0, c1);
     Seg s{};
     int seg0 = 0;  // the segment's first tile in this CTA's numbering
     bool quit = false;
     for (int n = 0; !quit && w.next(s); ++n) {
-      const int need = need_of(s.b);
-      const int h = s.u / p.chunks, col0 = (s.u - h * p.chunks) * p.chunk_cols;
-      const int ncol = min(p.chunk_cols, p.cols - col0);
-      const int tok0 = col0 / p.group;         // the first column's token
+      const int need = s.need, ncol = s.ncol;
+      int tok0, g0;                            // the first column's token and head
+      column(p, s.col0, tok0, g0);
       const int lim0 = len[s.b] + tok0;        // the keys it sees; later tokens see more
       const int ob = C::OB == 2 ? n & 1 : 0;
       float m[NQT], l[NQT];
@@ -668,7 +702,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         mbar_arrive(&ctl.s_free[b]);  // (after the last read of the queries' factors and the scales, too)
         if (NQT > ncol || (t + 1) * BN > lim0) {  // spare columns, or keys that some column does not see
-          int tt = 0, g = col0 - tok0 * p.group;
+          int tt = 0, g = g0;
 #pragma unroll
           for (int j = 0; j < NQT; ++j) {
             if (j >= ncol || key >= min(need, lim0 + tt)) x[j] = -INFINITY;
@@ -833,7 +867,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int d = tid - W_EPI * 32;
     const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
     Walk w, ahead;
-    w.init(pre, p.rows, per_row, c0, c1);
+    w.init(p, pre, len, c0, c1);
     ahead = w;
     Seg s{}, sq{};
     // These warps also load the queries, QN segments ahead: warp w the columns w, w + 4, .. of a segment. They are written
@@ -844,14 +878,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int wq = warp - W_EPI;
     uint2 qr[QC][DC];  // four dims per lane of each chunk (head_dim 64: of the first 16 lanes)
     auto query_load = [&]() {
-      const int h = sq.u / p.chunks, col0 = (sq.u - h * p.chunks) * p.chunk_cols;
-      const int ncol = min(p.chunk_cols, p.cols - col0);
 #pragma unroll
       for (int k = 0; k < QC; ++k) {
         const int j = wq + 4 * k;
-        if (j < ncol) {
+        if (j < sq.ncol) {
           int tt;
-          const uint2* src = reinterpret_cast<const uint2*>(p.q + query_row(p, sq.b, h, col0 + j, &tt) * DIM) + lane;
+          const uint2* src = reinterpret_cast<const uint2*>(p.q + query_row(p, sq.b, sq.h, sq.col0 + j, &tt) * DIM) + lane;
 #pragma unroll
           for (int c = 0; c < DC; ++c) qr[k][c] = CD == 128 || lane < 16 ? __ldg(src + c * 32) : make_uint2(0u, 0u);
         }
@@ -861,12 +893,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto swizzle = [](int r) { return ROWB == 128 ? r & 7 : (r >> 1) & 3; };
     auto query_store = [&](int n) {
       unsigned char* qb = smem + C::Q_OFF + (n % C::QN) * C::QB;
-      const int h = sq.u / p.chunks, col0 = (sq.u - h * p.chunks) * p.chunk_cols;
-      const int ncol = min(p.chunk_cols, p.cols - col0);
 #pragma unroll
       for (int k = 0; k < QC; ++k) {
         const int j = wq + 4 * k;
-        if (j >= ncol) continue;
+        if (j >= sq.ncol) continue;
         if constexpr (FP8) {
           float x[DC][4];
           uint32_t amax = 0u;
@@ -923,20 +953,25 @@ __global__ void __launch_bounds__(kThreads, 1)
       query_load();
       query_store(n);
     }
+    constexpr bool EARLY = QC * DC <= 8;  // loaded a segment before they are written out (while the registers hold them)
+    bool more = ahead.next(sq);  // segment n + QN
+    if (EARLY && more) query_load();
     for (int n = 0; w.next(s); ++n) {
       const int ob = C::OB == 2 ? n & 1 : 0;
-      const bool more = ahead.next(sq);
       if (more) {
-        query_load();
+        if (!EARLY) query_load();
         wait(&ctl.q_empty[n % C::QN], (n / C::QN) & 1);
         query_store(n + C::QN);
+        more = ahead.next(sq);
+        if (EARLY && more) query_load();
       }
       wait(&ctl.o_full[ob], (n / C::OB) & 1);
       wait(&ctl.ml_full[n & 1], (n >> 1) & 1);
       if (sync_or(2, 128, abort_flag != 0)) break;  // all of these warps leave together
       tc_fence_after();
-      const int h = s.u / p.chunks, col0 = (s.u - h * p.chunks) * p.chunk_cols;
-      const int ncol = min(p.chunk_cols, p.cols - col0);
+      const int h = s.h, col0 = s.col0, ncol = s.ncol;
+      int tok0, g0;
+      column(p, col0, tok0, g0);
       // The two softmax groups' parts as one: weights 2^(m_b - m); a group that saw no key takes no part.
       float l[NQT], m[NQT], wt[2][NQT];
 #pragma unroll
@@ -956,12 +991,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_arrive(&ctl.ml_free[n & 1]);
       unsigned bad = 0;  // columns with a result that is not finite
       auto store = [&](int c, const float (&o)[NQT], const float (&sum)[NQT]) {
-        int tt = col0 / p.group, g = col0 - tt * p.group;
+        int tt = tok0, g = g0;
+        const int64_t row0 = (int64_t)s.b * p.tokens * p.heads + h * p.group;
 #pragma unroll
         for (int j = 0; j < NQT; ++j) {
           if (j < ncol) {
-            const int64_t row = ((int64_t)s.b * p.tokens + tt) * p.heads + h * p.group + g;
-            const float r = o[j] * (sum[j] != 0.f ? 1.f / sum[j] : 0.f);
+            const int64_t row = row0 + tt * p.heads + g;
+            const float r = o[j] * (sum[j] != 0.f ? __fdividef(1.f, sum[j]) : 0.f);
             if (!(fabsf(r) <= 3.3e38f) && (CD == 128 || d < CD)) bad |= 1u << j;
             if (CD == 128 || d < CD) p.out[row * DIM + c * CD + d] = __float2bfloat16_rn(r);
           }
@@ -971,9 +1007,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       };
-      const int f0 = s.first / per, f1 = (s.first + s.nt - 1) / per;  // the unit's first and last CTA
-      bool emit = f0 == f1;
-      const int64_t at = ((int64_t)2 * blockIdx.x + ((int)blockIdx.x == f0 ? 1 : 0)) * kMaxCols;
+      const bool here = s.t0 == 0;  // the unit begins in this CTA
+      bool emit = here && s.t1 == s.nt;
+      const int place = (2 * (int)blockIdx.x + (here ? 1 : 0)) * kMaxCols;
 #pragma unroll 1
       for (int c = 0; c < DC; ++c) {
         float v[N], o[NQT];
@@ -998,28 +1034,35 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else {
 #pragma unroll
           for (int j = 0; j < NQT; ++j)
-            if (j < ncol && (CD == 128 || d < CD)) p.part_o[(at + j) * DIM + c * CD + d] = o[j];
+            if (j < ncol && (CD == 128 || d < CD)) p.part_o[(int64_t)(place + j) * DIM + c * CD + d] = o[j];
         }
       }
       if (!emit) {
+        // A cut unit: its parts are joined in the order of the keys, by the CTA that publishes last; where there are more
+        // than kJoin of them, in two steps (each run of kJoin parts by the last of its CTAs, then the runs).
         if (d == 0) {
 #pragma unroll
           for (int j = 0; j < NQT; ++j)
-            if (j < ncol) p.part_ml[at + j] = make_float2(m[j], l[j]);
+            if (j < ncol) p.part_ml[place + j] = make_float2(m[j], l[j]);
         }
-        __threadfence();
-        named_sync(2, 128);  // every thread's part is out before the count
-        if (d == 0) {
-          const unsigned before = atomicAdd(p.counters + f0, 1u);
-          const bool last = before == (unsigned)(f1 - f0);
-          if (last) p.counters[f0] = 0;  // zero again for the next call
-          ctl.last = last;
-        }
-        named_sync(2, 128);
-        emit = ctl.last != 0;
-        if (emit) {
-          __threadfence();
-          // Joined in the order of the keys, whichever CTA came last.
+        const int f0 = s.first / per, parts = (s.first + s.nt - 1) / per - f0 + 1, mine = (int)blockIdx.x - f0;
+        // True in the CTA that comes last of `of`; the parts of the others are visible to it then.
+        auto arrive = [&](unsigned* counter, int of) -> bool {
+          named_sync(2, 128);  // this CTA's part is written
+          if (d == 0) {
+            __threadfence();
+            const bool last = atomicAdd(counter, 1u) == (unsigned)(of - 1);
+            if (last) *counter = 0;  // zero again for the next call
+            __threadfence();
+            ctl.last = last;
+          }
+          named_sync(2, 128);
+          return ctl.last != 0;
+        };
+        auto slot_of = [&](int part) { return (2 * (f0 + part) + (part == 0 ? 1 : 0)) * kMaxCols; };
+        // Joins `count` parts from `begin`, every `by`-th; `to`: a part's slot, or -1: the output.
+        auto join = [&](int begin, int by, int count, int to) {
+          constexpr int U = NQT >= 16 ? 1 : NQT >= 8 ? 2 : 4;  // parts loaded together
 #pragma unroll 1
           for (int c = 0; c < DC; ++c) {
             float o[NQT];
@@ -1028,28 +1071,61 @@ __global__ void __launch_bounds__(kThreads, 1)
               m[j] = -INFINITY;
               l[j] = o[j] = 0.f;
             }
-#pragma unroll 2
-            for (int f = f0; f <= f1; ++f) {
-              const int64_t src = ((int64_t)2 * f + (f == f0 ? 1 : 0)) * kMaxCols;
-              float2 e[NQT];
-              float v[NQT];
+#pragma unroll 1
+            for (int k0 = 0; k0 < count; k0 += U) {
+              float2 e[U][NQT];
+              float v[U][NQT];
 #pragma unroll
-              for (int j = 0; j < NQT; ++j) {
-                e[j] = j < ncol ? __ldcg(p.part_ml + src + j) : make_float2(0.f, 0.f);
-                v[j] = j < ncol && (CD == 128 || d < CD) ? __ldcg(p.part_o + (src + j) * DIM + c * CD + d) : 0.f;
+              for (int k = 0; k < U; ++k) {
+                const int src = slot_of(begin + (k0 + k) * by);
+#pragma unroll
+                for (int j = 0; j < NQT; ++j) {
+                  const bool on = k0 + k < count && j < ncol;
+                  e[k][j] = on ? __ldcg(p.part_ml + src + j) : make_float2(0.f, 0.f);
+                  v[k][j] = on && (CD == 128 || d < CD) ? __ldcg(p.part_o + (int64_t)(src + j) * DIM + c * CD + d) : 0.f;
+                }
               }
 #pragma unroll
-              for (int j = 0; j < NQT; ++j) {
-                if (e[j].y != 0.f) {  // a part that saw no key takes no part
-                  const float mn = fmaxf(m[j], e[j].x);
-                  const float a = ex2(m[j] - mn), b = ex2(e[j].x - mn);
-                  l[j] = fmaf(l[j], a, e[j].y * b);
-                  m[j] = mn;
-                  o[j] = fmaf(o[j], a, v[j] * b);
+              for (int k = 0; k < U; ++k) {
+#pragma unroll
+                for (int j = 0; j < NQT; ++j) {
+                  if (e[k][j].y != 0.f) {  // a part that saw no key takes no part
+                    const float mn = fmaxf(m[j], e[k][j].x);
+                    const float a = ex2(m[j] - mn), b = ex2(e[k][j].x - mn);
+                    l[j] = fmaf(l[j], a, e[k][j].y * b);
+                    m[j] = mn;
+                    o[j] = fmaf(o[j], a, v[k][j] * b);
+                  }
                 }
               }
             }
-            store(c, o, l);
+            if (to < 0) {
+              store(c, o, l);
+            } else {
+#pragma unroll
+              for (int j = 0; j < NQT; ++j)
+                if (j < ncol && (CD == 128 || d < CD)) p.part_o[(int64_t)(to + j) * DIM + c * CD + d] = o[j];
+            }
+          }
+          if (to >= 0) {
+            named_sync(2, 128);  // the slot's statistics are read
+            if (d == 0) {
+#pragma unroll
+              for (int j = 0; j < NQT; ++j)
+                if (j < ncol) p.part_ml[to + j] = make_float2(m[j], l[j]);
+            }
+          }
+        };
+        if (parts <= kJoin) {
+          emit = arrive(p.counters + f0, parts);
+          if (emit) join(0, 1, parts, -1);
+        } else {
+          const int begin = mine - mine % kJoin, count = min(kJoin, parts - begin);
+          const int runs = (parts + kJoin - 1) / kJoin;
+          if (arrive(p.counters + gridDim.x + 2 * (f0 + begin) + (begin == 0 ? 1 : 0), count)) {
+            join(begin, 1, count, slot_of(begin));
+            emit = arrive(p.counters + f0, runs);
+            if (emit) join(0, kJoin, runs, -1);
           }
         }
       }
@@ -1064,7 +1140,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               int t2;
               const int64_t row = query_row(p, s.b, h, col0 + j, &t2);
               exact_column<FP8, DIM>(p.q + row * DIM, p.c, p.table + (int64_t)s.b * p.table_stride, h,
-                                     min(need_of(s.b), len[s.b] + t2), p.qscale, p.out + row * DIM);
+                                     min(s.need, len[s.b] + t2), p.qscale, p.out + row * DIM);
             }
             named_sync(2, 128);
             if (d == 0) ctl.bad = 0;
