@@ -153,6 +153,24 @@ OMNI_DEV void copy_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 
+OMNI_DEV unsigned add_acq_rel(unsigned* p) {
+  unsigned old;
+  asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(old) : "l"(p) : "memory");
+  return old;
+}
+
+// 16 columns of this thread's lane without waiting; complete after tmem_wait.
+OMNI_DEV void tmem_ld16_async(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+OMNI_DEV void tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
 // One lane of the (converged) warp.
 OMNI_DEV bool elect_one() {
   uint32_t e;
@@ -870,6 +888,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     w.init(p, pre, len, c0, c1);
     ahead = w;
     Seg s{}, sq{};
+    // (After an abort the waits return at once and these warps go through their segments all the same, so that no barrier
+    // of theirs is left to some of them.)
     // These warps also load the queries, QN segments ahead: warp w the columns w, w + 4, .. of a segment. They are written
     // out as soon as a segment's last S^T has released its buffer, not after its O: a V chunk may wait for the slot of a K
     // chunk two tiles on, whose S^T needs the queries. (The factors of 8 segments are kept, as the softmax may still read
@@ -967,8 +987,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       wait(&ctl.o_full[ob], (n / C::OB) & 1);
       wait(&ctl.ml_full[n & 1], (n >> 1) & 1);
-      if (sync_or(2, 128, abort_flag != 0)) break;  // all of these warps leave together
       tc_fence_after();
+      __syncwarp();
       const int h = s.h, col0 = s.col0, ncol = s.ncol;
       int tok0, g0;
       column(p, col0, tok0, g0);
@@ -1012,15 +1032,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int place = (2 * (int)blockIdx.x + (here ? 1 : 0)) * kMaxCols;
 #pragma unroll 1
       for (int c = 0; c < DC; ++c) {
-        float v[N], o[NQT];
+        uint32_t v[2][N];
+        float o[NQT];
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int k = 0; k < N / 16; ++k)
+            tmem_ld16_async(tbase + lane_off + C::S_COLS + ((ob * 2 + b) * DC + c) * N + k * 16, v[b] + k * 16);
+        tmem_wait();
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
 #pragma unroll
-          for (int k = 0; k < N / 16; ++k)
-            tmem_ld16(tbase + lane_off + C::S_COLS + ((ob * 2 + b) * DC + c) * N + k * 16, v + k * 16);
-#pragma unroll
           for (int j = 0; j < NQT; ++j) {
-            const float x = FP8 ? fmaf(v[NQT + j], 0.0625f, v[j]) : v[j];
+            const float x0 = __uint_as_float(v[b][j]);
+            const float x = FP8 ? fmaf(__uint_as_float(v[b][(FP8 ? NQT : 0) + j]), 0.0625f, x0) : x0;
             const float add = wt[b][j] != 0.f ? x * wt[b][j] : 0.f;  // (a group without a tile: its O is stale)
             o[j] = b == 0 ? add : o[j] + add;
           }
@@ -1050,10 +1075,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         auto arrive = [&](unsigned* counter, int of) -> bool {
           named_sync(2, 128);  // this CTA's part is written
           if (d == 0) {
-            __threadfence();
-            const bool last = atomicAdd(counter, 1u) == (unsigned)(of - 1);
+            // Releases what the barrier has ordered before, acquires what the others released: no fences of their own.
+            const bool last = add_acq_rel(counter) == (unsigned)(of - 1);
             if (last) *counter = 0;  // zero again for the next call
-            __threadfence();
             ctl.last = last;
           }
           named_sync(2, 128);
