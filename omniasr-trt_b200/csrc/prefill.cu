@@ -786,7 +786,7 @@ cudaError_t launch_prefill(const PrefillArgs& a, cudaStream_t stream) {
                           sched ? *sched : prefill_round_robin());
 }
 
-bool packed_maps(const PackedArgs& a, int positions, CUtensorMap* q, CUtensorMap* k, CUtensorMap* v) {
+bool packed_maps(const PackedArgs& a, int positions, int v_rows, CUtensorMap* q, CUtensorMap* k, CUtensorMap* v) {
   using prefill::encode_map;
   const int group = a.heads / a.kv_heads;
   // An extent of one has a stride that nothing reads; PyTorch leaves any number there.
@@ -797,10 +797,10 @@ bool packed_maps(const PackedArgs& a, int positions, CUtensorMap* q, CUtensorMap
   const cuuint64_t kd[4] = {(cuuint64_t)a.dim, (cuuint64_t)a.k_tokens, (cuuint64_t)a.kv_heads, 1};
   const cuuint64_t ks[3] = {st(a.k_tokens, a.k_st), st(a.kv_heads, a.k_sh), 16};
   const cuuint64_t vs[3] = {st(a.k_tokens, a.v_st), st(a.kv_heads, a.v_sh), 16};
-  const cuuint32_t kb[4] = {64, 128, 1, 1};
+  const cuuint32_t kb[4] = {64, 128, 1, 1}, vb[4] = {64, (cuuint32_t)v_rows, 1, 1};
   for (int i = 0; i < 3; ++i)
     if (!qs[i] || !ks[i] || !vs[i]) return false;
-  return encode_map(q, a.q, qd, qs, qb) && encode_map(k, a.k, kd, ks, kb) && encode_map(v, a.v, kd, vs, kb);
+  return encode_map(q, a.q, qd, qs, qb) && encode_map(k, a.k, kd, ks, kb) && encode_map(v, a.v, kd, vs, vb);
 }
 
 pfx::PackedSrc packed_source(const PackedArgs& a, int positions) {
@@ -833,7 +833,7 @@ cudaError_t launch_packed_d(const PackedArgs& a, cudaStream_t stream) {
   constexpr int SMEM_BYTES = Cfg<D>::SMEM_BYTES;
   const int positions = BM / (a.heads / a.kv_heads);
   CUtensorMap qm, km, vm;
-  if (!packed_maps(a, positions, &qm, &km, &vm)) return cudaErrorNotSupported;
+  if (!packed_maps(a, positions, BN, &qm, &km, &vm)) return cudaErrorNotSupported;
   static bool configured = false;
   if (!configured) {
     cudaError_t e = cudaFuncSetAttribute(prefill_kernel<PackedSrc, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);

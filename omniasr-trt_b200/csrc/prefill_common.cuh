@@ -324,9 +324,10 @@ int prefill_group(int bh_count);
 const pfx::Sched* prefill_schedule(int batch, int heads, int qtiles, int group, int grid);
 const pfx::Sched& prefill_round_robin();
 
-// The packed kernels' tensor maps (false where a stride has none), unit source and grid (prefill.cu).
+// The packed kernels' tensor maps (boxes of 128 keys, v_rows of V; false where a stride has none), unit source and grid
+// (prefill.cu).
 struct PackedArgs;
-bool packed_maps(const PackedArgs& a, int positions, CUtensorMap* q, CUtensorMap* k, CUtensorMap* v);
+bool packed_maps(const PackedArgs& a, int positions, int v_rows, CUtensorMap* q, CUtensorMap* k, CUtensorMap* v);
 pfx::PackedSrc packed_source(const PackedArgs& a, int positions);
 int packed_grid(const PackedArgs& a, int positions);
 

@@ -17,6 +17,8 @@
 // chunks, a 2-slot ring of 64-dim V sub-chunks (128 keys each; 128-byte swizzle throughout).
 // TMEM (512 columns): S double-buffered at [0, 128) and [128, 256), O of the pass's 256 dims at [256, 512); P (bf16
 // pairs) over S, read by the A-from-TMEM MMA.
+// Packed sequences use the same ring bytes in finer pieces: K in 64-dim boxes, so that more loads are in flight while one is
+// used, and V in slots of 32 keys x 256 dims, so that P V is 8 MMAs of N = 256 instead of 32 of N = 64.
 // Roles (512 threads), as in prefill.cu: warp 12 K chunk loads, warp 14 V sub-chunk loads, warp 13 S MMAs, warp 15
 // P V MMAs, warps 0-3 / 4-7 softmax warpgroups (thread = query row, warpgroup x the keys 64x .. 64x + 63 of every
 // tile, one running max per row shared through a barrier per tile), warps 8-11 the epilogue (and the query loads,
@@ -66,6 +68,8 @@ constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t COL_S = 0, COL_O = NSB * 128;
 constexpr uint32_t IDESC_S = idesc_bf16(BM, BN, 0, 0);
 constexpr uint32_t IDESC_O = idesc_bf16(BM, 64, 0, 1);
+constexpr uint32_t IDESC_O256 = idesc_bf16(BM, DH, 0, 1);
+constexpr int VK = 32;  // packed: keys of a V slot (all 256 dims of the pass)
 constexpr float kRescale = 8.f;
 constexpr int kPolyEvery = 4;  // probabilities of one pair in this many by ex2_fma
 
@@ -81,7 +85,7 @@ struct Params {
 template <int D>
 struct alignas(1024) Ctl {
   static constexpr int DC = Cfg<D>::DC, KS = Cfg<D>::KS, VS = Cfg<D>::VS;
-  uint64_t k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], q_full[DC], q_empty[DC];
+  uint64_t k_full[2 * KS], k_empty[2 * KS], v_full[VS], v_empty[VS], q_full[DC], q_empty[DC];
   uint64_t s_full[NSB], pv_done[NSB], p_full[NWG][NSB];
   uint64_t o_ready, o_free, l_full, l_free, drain;
   float tmax[NWG][BM];
@@ -123,7 +127,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     return;
   }
   if (tid == 0) {
-    for (int s = 0; s < KS; ++s) {
+    for (int s = 0; s < 2 * KS; ++s) {
       mbar_init(&k_full[s], 1);
       mbar_init(&k_empty[s], 1);
     }
@@ -222,14 +226,14 @@ __global__ void __launch_bounds__(THREADS, 1)
                   tma_load_4d(dst + BOX, &qmap, c * 128 + 64, 0, u.h, u.q0, &q_full[c]);
                   issued_q = n * DC + c + 1;
                 }
-                const int slot = kc % KS, use = kc / KS;
-                ok = use < 1 || wait(&k_empty[slot], (use - 1) & 1);
-                if (!ok) break;
-                mbar_arrive_expect_tx(&k_full[slot], CHUNK);
-                unsigned char* dst = smem + K_OFF + slot * CHUNK;
-                tma_load_4d(dst, &kmap, c * 128, u.k0 + kt * BN, u.h, 0, &k_full[slot]);
-                tma_load_4d(dst + BOX, &kmap, c * 128 + 64, u.k0 + kt * BN, u.h, 0, &k_full[slot]);
-                issued_k = kc + 1;
+                for (int x = 0; x < 2 && ok; ++x) {
+                  const int kb = 2 * kc + x, slot = kb % (2 * KS), use = kb / (2 * KS);
+                  ok = use < 1 || wait(&k_empty[slot], (use - 1) & 1);
+                  if (!ok) break;
+                  mbar_arrive_expect_tx(&k_full[slot], BOX);
+                  tma_load_4d(smem + K_OFF + slot * BOX, &kmap, c * 128 + 64 * x, u.k0 + kt * BN, u.h, 0, &k_full[slot]);
+                  issued_k = kb + 1;
+                }
               }
             }
         }
@@ -281,8 +285,14 @@ __global__ void __launch_bounds__(THREADS, 1)
               const int slot = vc % VS, use = vc / VS;
               if (use >= 1 && !wait(&v_empty[slot], (use - 1) & 1)) break;
               mbar_arrive_expect_tx(&v_full[slot], BOX);
-              tma_load_4d(smem + V_OFF + slot * BOX, &vmap, pass * DH + sc * 64, (PACKED ? u.k0 : 0) + kt * BN, u.h, u.b,
-                          &v_full[slot]);
+              unsigned char* dst = smem + V_OFF + slot * BOX;
+              if constexpr (PACKED) {  // keys VK sc .. of all the pass's dims, in 64-dim boxes
+#pragma unroll
+                for (int x = 0; x < DH / 64; ++x)
+                  tma_load_4d(dst + x * (VK * 128), &vmap, pass * DH + x * 64, u.k0 + kt * BN + VK * sc, u.h, 0, &v_full[slot]);
+              } else {
+                tma_load_4d(dst, &vmap, pass * DH + sc * 64, kt * BN, u.h, u.b, &v_full[slot]);
+              }
               issued_v = vc + 1;
             }
         put(n);
@@ -310,6 +320,25 @@ __global__ void __launch_bounds__(THREADS, 1)
               if (pass == 0 && kt == 0 && !wait(&q_full[c], n & 1)) {
                 ok = false;
                 break;
+              }
+              if constexpr (PACKED) {
+                for (int x = 0; x < 2; ++x) {
+                  const int kb = 2 * kc + x, slot = kb % (2 * KS);
+                  if (!wait(&k_full[slot], (kb / (2 * KS)) & 1)) {
+                    ok = false;
+                    break;
+                  }
+                  tc_fence_after();
+                  const uint64_t qd = qdesc0 + (uint64_t)((2 * c + x) * (BOX >> 4));
+                  const uint64_t kd = kdesc0 + (uint64_t)(slot * (BOX >> 4));
+#pragma unroll
+                  for (int kk = 0; kk < 4; ++kk)
+                    mma_bf16_ss(dcol, qd + kk * 2, kd + kk * 2, IDESC_S, (c > 0 || x > 0 || kk > 0) ? 1u : 0u);
+                  tc_commit(&k_empty[slot]);
+                }
+                if (!ok) break;
+                if (pass == PASSES - 1 && kt == u.kt - 1) tc_commit(&q_empty[c]);  // the unit's last read of query chunk c
+                continue;
               }
               const int slot = kc % KS;
               if (!wait(&k_full[slot], (kc / KS) & 1)) {
@@ -340,6 +369,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     // ------------------------------------------------------------------ O[:, 64 sc ..] += P(t) V(t)[:, sc]
     if (lane == 0) {
       const uint64_t vdesc0 = smem_desc(smem_addr(smem + V_OFF), BOX, 1024, kLayoutSw128);
+      const uint64_t vdesc32 = smem_desc(smem_addr(smem + V_OFF), VK * 128, 1024, kLayoutSw128);
       int tile = 0, vc = 0, item = 0;
       bool ok = true;
       Unit u;
@@ -351,10 +381,28 @@ __global__ void __launch_bounds__(THREADS, 1)
               ok = false;
               break;
             }
+            const uint32_t pcol = tbase + COL_S + pb * 128;
+            if constexpr (PACKED) {
+              for (int sc = 0; sc < BN / VK; ++sc, ++vc) {
+                const int slot = vc % VS, x = sc * VK / KW;
+                if (sc * VK % KW == 0) ok = wait(&p_full[x][pb], pu & 1);
+                ok = ok && wait(&v_full[slot], (vc / VS) & 1);
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t vd = vdesc32 + (uint64_t)(slot * (BOX >> 4));
+#pragma unroll
+                for (int kk = 0; kk < VK / 16; ++kk)
+                  mma_bf16_ts(tbase + COL_O, pcol + x * KW + (sc * VK % KW / 16 + kk) * 8, vd + (uint64_t)(kk * 128), IDESC_O256,
+                              (kt == 0 && sc == 0 && kk == 0) ? 0u : 1u);
+                tc_commit(&v_empty[slot]);
+              }
+              if (!ok) break;
+              tc_commit(&pv_done[pb]);
+              continue;
+            }
             for (int x = 0; x < NWG && ok; ++x) ok = wait(&p_full[x][pb], pu & 1);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t pcol = tbase + COL_S + pb * 128;
             for (int sc = 0; sc < NSUB; ++sc, ++vc) {
               const int slot = vc % VS;
               if (!wait(&v_full[slot], (vc / VS) & 1)) {
@@ -617,7 +665,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_wait(&drain, 0);
     }
     if (tid == W_LOADK * 32) {
-      for (int i = issued_k > KS ? issued_k - KS : 0; i < issued_k; ++i) mbar_wait(&k_full[i % KS], (i / KS) & 1);
+      constexpr int KR = PACKED ? 2 * KS : KS;  // K ring slots
+      for (int i = issued_k > KR ? issued_k - KR : 0; i < issued_k; ++i) mbar_wait(&k_full[i % KR], (i / KR) & 1);
       for (int i = issued_v > VS ? issued_v - VS : 0; i < issued_v; ++i) mbar_wait(&v_full[i % VS], (i / VS) & 1);
       // the latest load of every query chunk (load i fills chunk i % DC for the (i / DC)-th time)
       for (int i = issued_q > DC ? issued_q - DC : 0; i < issued_q; ++i) mbar_wait(&q_full[i % DC], (i / DC) & 1);
@@ -695,7 +744,7 @@ cudaError_t launch_packed_wide_d(const PackedArgs& a, cudaStream_t stream) {
   constexpr int SMEM_BYTES = Cfg<D>::SMEM_BYTES;
   const int positions = BM / (a.heads / a.kv_heads);
   CUtensorMap qm, km, vm;
-  if (!packed_maps(a, positions, &qm, &km, &vm)) return cudaErrorNotSupported;
+  if (!packed_maps(a, positions, VK, &qm, &km, &vm)) return cudaErrorNotSupported;
   static bool configured = false;
   if (!configured) {
     cudaError_t e =
