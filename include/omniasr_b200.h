@@ -300,8 +300,9 @@ int omniasr_paged_attention(const void* q, const void* k_pages, const void* v_pa
  * q [q_tokens, heads, dim] and keys k_offsets[s] .. k_offsets[s + 1] - 1 of k / v [k_tokens, kv_heads, dim] (token and
  * head strides in elements); its last query sees its last key, so query i of lq sees i + 1 + lk - lq keys (none where
  * that is not positive: zeros). out [q_tokens, heads, dim] contiguous; rows of no sequence are not written. Offsets are
- * int64, ascending, on the device. The workspace begins with counters under the rule of omniasr_attention_workspace(). */
-#define OMNIASR_PACKED_WORKSPACE_BYTES 256
+ * int64, ascending, on the device. The workspace (omniasr_packed_attention_workspace() bytes) begins with counters under the
+ * rule of omniasr_attention_workspace(). */
+size_t omniasr_packed_attention_workspace(int64_t q_tokens, int heads, int kv_heads, int dim, int dtype);
 int omniasr_packed_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k, int64_t k_stride_tok,
                              int64_t k_stride_head, const void* v, int64_t v_stride_tok, int64_t v_stride_head, void* out,
                              const int64_t* q_offsets, const int64_t* k_offsets, int64_t q_tokens, int64_t k_tokens, int seqs,

@@ -90,6 +90,7 @@ struct PackedArgs {
 };
 // Tensor-core kernels, bf16 head_dim 64 and 128 (prefill.cu), 256 and 512 (prefill_wide.cu), at most 128 query heads per kv head;
 // cudaErrorNotSupported where a tensor's strides have no tensor map.
+size_t packed_workspace(int dtype, int64_t q_tokens, int heads, int kv_heads, int dim);
 cudaError_t launch_packed_tc(const PackedArgs& a, cudaStream_t stream);
 cudaError_t launch_packed_tc_wide(const PackedArgs& a, cudaStream_t stream);
 cudaError_t launch_packed(int dtype, const PackedArgs& a, cudaStream_t stream);

@@ -193,6 +193,11 @@ int omniasr_paged_attention(const void* q, const void* k_pages, const void* v_pa
   return done(name, omni::launch_paged_attention(dtype, a, stream));
 }
 
+size_t omniasr_packed_attention_workspace(int64_t q_tokens, int heads, int kv_heads, int dim, int dtype) {
+  if (!omni::dim_supported(dtype, dim) || q_tokens < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 0;
+  return omni::packed_workspace(dtype, q_tokens, heads, kv_heads, dim);
+}
+
 int omniasr_packed_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k, int64_t k_stride_tok,
                              int64_t k_stride_head, const void* v, int64_t v_stride_tok, int64_t v_stride_head, void* out,
                              const int64_t* q_offsets, const int64_t* k_offsets, int64_t q_tokens, int64_t k_tokens, int seqs,
@@ -211,9 +216,9 @@ int omniasr_packed_attention(const void* q, int64_t q_stride_tok, int64_t q_stri
   const int64_t strides[6] = {q_stride_tok, q_stride_head, k_stride_tok, k_stride_head, v_stride_tok, v_stride_head};
   for (int64_t st : strides)
     if (!stride_ok(st, dtype)) return fail(OMNIASR_ERR_ARGUMENT, "%s: strides must keep 16-byte alignment", name);
-  if (!workspace || !aligned16(workspace) || workspace_bytes < OMNIASR_PACKED_WORKSPACE_BYTES)
-    return fail(OMNIASR_ERR_WORKSPACE, "%s: workspace of %zu bytes, %d needed", name, workspace_bytes,
-                OMNIASR_PACKED_WORKSPACE_BYTES);
+  const size_t need = omniasr_packed_attention_workspace(q_tokens, heads, kv_heads, dim, dtype);
+  if (!workspace || !aligned16(workspace) || workspace_bytes < need)
+    return fail(OMNIASR_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", name, workspace_bytes, need);
   omni::PackedArgs a;
   a.q = q;
   a.q_st = q_stride_tok;

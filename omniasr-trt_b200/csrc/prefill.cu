@@ -55,7 +55,7 @@ constexpr int BOX = BN * 64 * 2;
 template <int D>
 struct Cfg {
   static constexpr int TILE = BN * D * 2;
-  static constexpr int QS = 2, KS = D == 64 ? 6 : 3, VS = D == 64 ? 6 : 2;  // query tiles (two units), K and V rings
+  static constexpr int QS = 2, KS = D == 64 ? 5 : 3, VS = D == 64 ? 6 : 2;  // query tiles (two units), K and V rings
   static constexpr int Q_OFF = 0;
   static constexpr int K_OFF = Q_OFF + QS * TILE;
   static constexpr int V_OFF = K_OFF + KS * TILE;
@@ -100,6 +100,7 @@ struct alignas(1024) Ctl {
   uint64_t k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], q_full[QS], q_empty[QS];
   uint64_t s_full[NSB], p_full[NWG][NSB], pv_done[NSB], o_ready, o_free, l_full, l_free, drain;
   float tmax[NWG][BM];  // [warpgroup][row]: a tile's scaled row maxima, on the rare tiles that raise a max
+  float msum[BM];       // [row]: the maximum of a unit's part
   float lsum[NWG][BM];  // [warpgroup][row]: the unit's row sums for the epilogue
   uint32_t tmem_base;
   int abort_flag, issued_k, issued_v, issued_q;  // loads the producers issued
@@ -217,7 +218,14 @@ __global__ void __launch_bounds__(THREADS, 1)
       int tile = 0;
       long long next = blockIdx.x;
       for (int n = 0;; ++n) {
-        const Unit u = walk.find(src, next, lane, blockIdx.x == 0 ? p.status : nullptr);
+        const Unit u = walk.find_part(src, next, lane, blockIdx.x == 0 ? p.status : nullptr);
+        if (u.kt < 0) {  // a part without keys
+          unsigned c = 0;
+          if (lane == 0) c = atomicAdd(src.counters, 1u);
+          next = (long long)gridDim.x + __shfl_sync(0xffffffffu, c, 0);
+          --n;
+          continue;
+        }
         bool ok = true;
         unsigned claim = 0;
         if (lane == 0) {
@@ -524,6 +532,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       // two tiles can be finished before that, and l_full must not complete two phases ahead of its waiter).
       if (nunit >= 1) wait(&l_free, (nunit - 1) & 1);
       ctl.lsum[x][row] = l;
+      if (PACKED && x == 0) ctl.msum[row] = m;
       mbar_arrive(&l_full);
     }
   } else if (warp < W_EPI + 4) {
@@ -570,6 +579,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       float l = 0.f;
 #pragma unroll
       for (int y = 0; y < NWG; ++y) l += ctl.lsum[y][row];
+      const float m = PACKED ? ctl.msum[row] : 0.f;
       mbar_arrive(&l_free);
       float inv = l > 0.f ? 1.f / l : 0.f;
       const int q = u.qt * BM + row;
@@ -601,7 +611,17 @@ __global__ void __launch_bounds__(THREADS, 1)
           tc_fence_before();
           mbar_arrive(&o_free);
         }
-        if (live) {
+        if (PACKED && u.part >= 0) {  // a part: fp32, a column of rows at a time
+          if constexpr (PACKED) {
+            float* part = src.parts + (int64_t)u.part * ((D + 2) * BM) + row;
+#pragma unroll
+            for (int i = 0; i < 64; ++i) part[(c * 64 + i) * BM] = __uint_as_float(r0[i]);
+            if (c == 0) {
+              part[D * BM] = u.lim0 + pos > 0 ? m : -INFINITY;
+              part[(D + 1) * BM] = u.lim0 + pos > 0 ? l : 0.f;
+            }
+          }
+        } else if (live) {
           if constexpr (PACKED) {
 #pragma unroll
             for (int i = 0; i < 64; ++i) odd = fmaf(__uint_as_float(r0[i]), 0.f, odd);
@@ -619,7 +639,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       }
       if constexpr (PACKED) {
-        const bool redo = live && !(odd == 0.f && l - l == 0.f);
+        if (u.part >= 0 && u.part % u.b == 0 && row == 0)  // a unit's first part
+          reinterpret_cast<PartMeta*>(src.meta + 8)[u.part / u.b] = {u.qt, u.h, u.q0, u.npos, u.k0, u.lim0, {0, 0}};
+        const bool redo = live && u.part < 0 && !(odd == 0.f && l - l == 0.f);
         __syncwarp();  // the rows' first results are written before they are written again
         for (unsigned left = __ballot_sync(0xffffffffu, redo); left; left &= left - 1) {
           const int w = __ffs(left) - 1;
@@ -786,6 +808,101 @@ cudaError_t launch_prefill(const PrefillArgs& a, cudaStream_t stream) {
                           sched ? *sched : prefill_round_robin());
 }
 
+// Adds up the parts of a cut unit (block x: unit, y: 32 of its head dims; thread: tile row): o = sum 2^(m_s - m) O_s / sum
+// 2^(m_s - m) l_s, in the order of the keys. Rows whose result is not finite are redone from the formula.
+template <int D>
+__global__ void __launch_bounds__(128) packed_join_kernel(const __grid_constant__ pfx::PackedSrc src, float qscale,
+                                                          __nv_bfloat16* out) {
+  using namespace pfx;
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int units = src.meta[0], cut = src.meta[1];
+  if (cut <= 1 || (int)blockIdx.x >= units) return;
+  const PartMeta u = reinterpret_cast<const PartMeta*>(src.meta + 8)[blockIdx.x];
+  const int row = threadIdx.x, d0 = blockIdx.y * 32;
+  const int pos = row / src.group, head = u.h * src.group + row - pos * src.group;
+  const bool live = pos < u.npos;
+  const float* part = src.parts + (int64_t)blockIdx.x * cut * ((D + 2) * 128) + row;
+  float w[kMostParts], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int s = 0; s < kMostParts; ++s) {
+    w[s] = s < u.n ? part[(int64_t)s * ((D + 2) * 128) + D * 128] : -INFINITY;
+    m = fmaxf(m, w[s]);
+  }
+#pragma unroll
+  for (int s = 0; s < kMostParts; ++s) {
+    w[s] = w[s] > -INFINITY ? ex2(w[s] - m) : 0.f;
+    if (w[s] != 0.f) l = fmaf(w[s], part[(int64_t)s * ((D + 2) * 128) + (D + 1) * 128], l);
+  }
+  float o[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) o[i] = 0.f;
+#pragma unroll 1
+  for (int s = 0; s < u.n; ++s) {
+    float ws = 0.f;
+#pragma unroll
+    for (int k = 0; k < kMostParts; ++k) ws = k == s ? w[k] : ws;
+    float v[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = part[(int64_t)s * ((D + 2) * 128) + (d0 + i) * 128];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) o[i] = ws != 0.f ? fmaf(ws, v[i], o[i]) : o[i];
+  }
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  const int64_t at = ((int64_t)(u.q0 + pos) * src.heads + head) * D;
+  float odd = l * 0.f;
+  if (live) {
+    uint4* dst = reinterpret_cast<uint4*>(out + at + d0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t p4[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float a = o[8 * i + 2 * j] * inv, b = o[8 * i + 2 * j + 1] * inv;
+        odd = fmaf(a, 0.f, fmaf(b, 0.f, odd));
+        p4[j] = pack_bf16x2(a, b);
+      }
+      dst[i] = make_uint4(p4[0], p4[1], p4[2], p4[3]);
+    }
+  }
+  __syncwarp();
+  for (unsigned left = __ballot_sync(0xffffffffu, live && odd != 0.f); left; left &= left - 1) {
+    const int k = __ffs(left) - 1;
+    const int wp = __shfl_sync(0xffffffffu, pos, k), wh = __shfl_sync(0xffffffffu, head, k);
+    const int64_t tok = u.q0 + wp;
+    exact_row<D>(src.q + tok * src.q_st + wh * src.q_sh, src.k + u.k0 * src.k_st + u.h * src.k_sh, src.k_st,
+                 src.v + u.k0 * src.v_st + u.h * src.v_sh, src.v_st, u.lim0 + wp, qscale, out + (tok * src.heads + wh) * D);
+  }
+}
+
+cudaError_t launch_packed_join(const PackedArgs& a, const pfx::PackedSrc& src, cudaStream_t stream) {
+  if (!src.meta) return cudaSuccess;
+  const dim3 grid((unsigned)packed_cut_units(), (unsigned)(a.dim / 32));
+  const float qscale = a.scale * kLog2e;
+  __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out);
+  switch (a.dim) {
+    case 64: return launch_dependent(packed_join_kernel<64>, grid, dim3(128), 0, stream, src, qscale, out);
+    case 128: return launch_dependent(packed_join_kernel<128>, grid, dim3(128), 0, stream, src, qscale, out);
+    case 256: return launch_dependent(packed_join_kernel<256>, grid, dim3(128), 0, stream, src, qscale, out);
+    default: return launch_dependent(packed_join_kernel<512>, grid, dim3(128), 0, stream, src, qscale, out);
+  }
+}
+
+// Units are cut while there are at most this many.
+int packed_cut_units() { return device_sm_count() / 2; }
+
+// Whether a call may have that few units: it has one per tile of its queries at least.
+static bool may_cut(int64_t q_tokens, int heads, int kv_heads) {
+  const int positions = 128 / (heads / kv_heads);
+  return (q_tokens + positions - 1) / positions * kv_heads <= packed_cut_units();
+}
+
+size_t packed_workspace(int dtype, int64_t q_tokens, int heads, int kv_heads, int dim) {
+  if (dtype != kBF16 || dim < 64 || heads / kv_heads > 128 || !may_cut(q_tokens, heads, kv_heads)) return 256;
+  return kCounterBytes + 32 + sizeof(pfx::PartMeta) * packed_cut_units() + 256 +
+         sizeof(float) * 128 * (size_t)(dim + 2) * device_sm_count();
+}
+
 bool packed_maps(const PackedArgs& a, int positions, int v_rows, CUtensorMap* q, CUtensorMap* k, CUtensorMap* v) {
   using prefill::encode_map;
   const int group = a.heads / a.kv_heads;
@@ -815,6 +932,13 @@ pfx::PackedSrc packed_source(const PackedArgs& a, int positions) {
   s.group = a.heads / a.kv_heads;
   s.pos = positions;
   s.counters = a.counters;
+  s.meta = nullptr;
+  s.parts = nullptr;
+  if (may_cut(a.q_tokens, a.heads, a.kv_heads)) {
+    char* ws = reinterpret_cast<char*>(a.counters) + kCounterBytes;
+    s.meta = reinterpret_cast<int*>(ws);
+    s.parts = reinterpret_cast<float*>(ws + (32 + sizeof(pfx::PartMeta) * packed_cut_units() + 255) / 256 * 256);
+  }
   s.q = reinterpret_cast<const __nv_bfloat16*>(a.q);
   s.k = reinterpret_cast<const __nv_bfloat16*>(a.k);
   s.v = reinterpret_cast<const __nv_bfloat16*>(a.v);
@@ -823,7 +947,9 @@ pfx::PackedSrc packed_source(const PackedArgs& a, int positions) {
 }
 
 int packed_grid(const PackedArgs& a, int positions) {
-  const int64_t units = (a.q_tokens / positions + a.seqs) * a.kv_heads;  // at least as many as there are
+  // Units that are cut may give every CTA a part; others are at most this many.
+  const int64_t units = may_cut(a.q_tokens, a.heads, a.kv_heads) ? device_sm_count()
+                                                                 : (a.q_tokens / positions + a.seqs) * a.kv_heads;
   return (int)std::min<int64_t>(device_sm_count(), units);
 }
 
@@ -844,8 +970,10 @@ cudaError_t launch_packed_d(const PackedArgs& a, cudaStream_t stream) {
   p.qscale = a.scale * kLog2e;
   p.out = reinterpret_cast<__nv_bfloat16*>(a.out);
   p.status = a.status;
-  return launch_dependent(prefill_kernel<PackedSrc, D>, dim3(packed_grid(a, positions)), dim3(THREADS), (size_t)SMEM_BYTES,
-                          stream, qm, km, vm, p, packed_source(a, positions));
+  const pfx::PackedSrc src = packed_source(a, positions);
+  const cudaError_t e = launch_dependent(prefill_kernel<PackedSrc, D>, dim3(packed_grid(a, positions)), dim3(THREADS),
+                                         (size_t)SMEM_BYTES, stream, qm, km, vm, p, src);
+  return e != cudaSuccess ? e : launch_packed_join(a, src, stream);
 }
 
 cudaError_t launch_packed_tc(const PackedArgs& a, cudaStream_t stream) {

@@ -173,7 +173,9 @@ OMNI_DEV int cta_unit(const Sched& s, int units, int n) {
 // 128 rows. Units are claimed by the CTAs as they become free (an atomic counter; the first by block index): sequences in
 // order, each in groups of 16 kv heads, a group's longest query tiles first. Claiming keeps the CTAs' end times together
 // whatever the lengths, which the device alone knows; the warp that loads K claims, and hands the units to the other
-// roles through a ring in shared memory.
+// roles through a ring in shared memory. Where the units would leave half of the CTAs idle (a short chunk over many keys),
+// each is cut into up to grid / units parts along its keys; a part leaves its maxima, sums and unnormalised output in fp32,
+// and packed_join_kernel adds the parts up.
 struct PackedSrc {
   const int64_t* q_offsets;
   const int64_t* k_offsets;
@@ -181,18 +183,27 @@ struct PackedSrc {
   int seqs, heads, kv_heads, group;  // group: query heads per kv head
   int pos;                           // positions per query tile
   unsigned* counters;                // [0] units claimed, [1] CTAs done: zero on entry and left zero
+  int* meta;                         // null: no unit is cut. [0] units, [1] parts per unit; then PartMeta per unit
+  float* parts;                      // [unit * parts per unit + part][(D + 2) * 128]: O [D][128 rows], maxima, sums
   const __nv_bfloat16 *q, *k, *v;    // for rows that need the exact form
   int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;
 };
 
 struct Unit {
-  int b, h, qt;   // dense: row, head, query tile
+  int b, h, qt;   // row, head, query tile; packed: parts per unit, kv head, parts of this unit
   int kt;         // key tiles (0: no more units)
   int q0, npos;   // packed: first token of the tile, positions in it
   int k0, lim0;   // first key token; keys the tile's first position sees (the next ones see one more each)
+  int part;       // packed: the slot for this part's result, or -1: the unit is whole
 };
 
-constexpr int kUnitRing = 4;
+// What packed_join_kernel needs of a unit: the parts there are and the unit as PackedWalk gives it.
+struct PartMeta {
+  int n, h, q0, npos, k0, lim0, pad[2];
+};
+constexpr int kMostParts = 16;
+
+constexpr int kUnitRing = 3;
 constexpr int kUnitHeads = 16;  // kv heads per scheduling group (as prefill_group)
 
 // The claiming warp's place in the sequences: 32 of them at a time, one per lane.
@@ -202,6 +213,7 @@ struct PackedWalk {
   long long incl;     // units of the block's sequences up to this lane's
   int tiles;          // this lane's sequence: query tiles, first query / key token, queries, keys
   int q0, k0, lq, lk;
+  int cut;            // parts per unit
 
   OMNI_DEV void load(const PackedSrc& p, int lane, int* status) {
     const int s = s0 + lane;
@@ -224,15 +236,52 @@ struct PackedWalk {
     incl = c;
   }
   OMNI_DEV void init(const PackedSrc& p, int lane, int* status) {
-    s0 = 0;
     before = 0;
     q0 = k0 = lq = lk = 0;
+    cut = 1;
+    if (p.meta) {  // few enough units that they may be cut: how many, and how long
+      long long units = 0;
+      int most = 0;
+      for (s0 = 0; s0 < p.seqs; s0 += 32) {
+        load(p, lane, nullptr);
+        units += __shfl_sync(0xffffffffu, incl, 31);
+        most = max(most, (int)__reduce_max_sync(0xffffffffu, tiles > 0 ? (unsigned)((lk + 127) / 128) : 0u));
+      }
+      const long long room = units > 0 ? (long long)gridDim.x / units : 1;
+      cut = (int)max(1ll, min(min(room, (long long)kMostParts), (long long)(most / 2)));  // parts of two tiles at least
+      if (blockIdx.x == 0 && lane == 0) {
+        p.meta[0] = (int)units;
+        p.meta[1] = cut;
+      }
+    }
+    s0 = 0;
     load(p, lane, status);
+  }
+  // Part number `c` (ascending from call to call) of the units' parts; empty ones have kt = -1.
+  OMNI_DEV Unit find_part(const PackedSrc& p, long long c, int lane, int* status) {
+    if (cut == 1) return find(p, c, lane, status);
+    const long long whole = c / cut;
+    Unit r = find(p, whole, lane, status);
+    if (r.kt == 0) return r;
+    const int j = (int)(c - whole * cut), each = (r.kt + cut - 1) / cut;
+    const int t0 = j * each, t1 = min(r.kt, t0 + each);
+    if (t0 >= t1) {
+      r.kt = -1;
+      return r;
+    }
+    r.part = (int)c;
+    r.b = cut;
+    r.qt = (r.kt + each - 1) / each;
+    r.k0 += t0 * 128;
+    r.lim0 -= t0 * 128;
+    r.kt = t1 - t0;
+    return r;
   }
   // Unit number `u` (ascending from call to call); kt = 0 past the last. All lanes call it and get the same answer.
   OMNI_DEV Unit find(const PackedSrc& p, long long u, int lane, int* status) {
     Unit r;
     r.kt = 0;
+    r.part = -1;
     for (;;) {
       const unsigned hit = __ballot_sync(0xffffffffu, u < before + incl);
       if (!hit) {
@@ -330,5 +379,7 @@ struct PackedArgs;
 bool packed_maps(const PackedArgs& a, int positions, int v_rows, CUtensorMap* q, CUtensorMap* k, CUtensorMap* v);
 pfx::PackedSrc packed_source(const PackedArgs& a, int positions);
 int packed_grid(const PackedArgs& a, int positions);
+int packed_cut_units();
+cudaError_t launch_packed_join(const PackedArgs& a, const pfx::PackedSrc& src, cudaStream_t stream);
 
 }  // namespace omni

@@ -89,6 +89,7 @@ struct alignas(1024) Ctl {
   uint64_t s_full[NSB], pv_done[NSB], p_full[NWG][NSB];
   uint64_t o_ready, o_free, l_full, l_free, drain;
   float tmax[NWG][BM];
+  float msum[BM];  // [row]: the maximum of a unit's part
   float lsum[NWG][BM];
   uint32_t tmem_base;
   int abort_flag, issued_k, issued_v, issued_q;
@@ -202,7 +203,14 @@ __global__ void __launch_bounds__(THREADS, 1)
       int kc = 0;
       long long next = blockIdx.x;
       for (int n = 0;; ++n) {
-        const Unit u = walk.find(src, next, lane, blockIdx.x == 0 ? p.status : nullptr);
+        const Unit u = walk.find_part(src, next, lane, blockIdx.x == 0 ? p.status : nullptr);
+        if (u.kt < 0) {  // a part without keys
+          unsigned c = 0;
+          if (lane == 0) c = atomicAdd(src.counters, 1u);
+          next = (long long)gridDim.x + __shfl_sync(0xffffffffu, c, 0);
+          --n;
+          continue;
+        }
         bool ok = true;
         unsigned claim = 0;
         if (lane == 0) {
@@ -337,23 +345,22 @@ __global__ void __launch_bounds__(THREADS, 1)
                   tc_commit(&k_empty[slot]);
                 }
                 if (!ok) break;
-                if (pass == PASSES - 1 && kt == u.kt - 1) tc_commit(&q_empty[c]);  // the unit's last read of query chunk c
-                continue;
-              }
-              const int slot = kc % KS;
-              if (!wait(&k_full[slot], (kc / KS) & 1)) {
-                ok = false;
-                break;
-              }
-              tc_fence_after();
-              const uint64_t qd = qdesc0 + (uint64_t)(c * (CHUNK >> 4));
-              const uint64_t kd = kdesc0 + (uint64_t)(slot * (CHUNK >> 4));
+              } else {
+                const int slot = kc % KS;
+                if (!wait(&k_full[slot], (kc / KS) & 1)) {
+                  ok = false;
+                  break;
+                }
+                tc_fence_after();
+                const uint64_t qd = qdesc0 + (uint64_t)(c * (CHUNK >> 4));
+                const uint64_t kd = kdesc0 + (uint64_t)(slot * (CHUNK >> 4));
 #pragma unroll
-              for (int kk = 0; kk < 8; ++kk) {
-                const uint64_t off = (uint64_t)((((kk >> 2) * BOX + (kk & 3) * 32) >> 4));
-                mma_bf16_ss(dcol, qd + off, kd + off, IDESC_S, (c > 0 || kk > 0) ? 1u : 0u);
+                for (int kk = 0; kk < 8; ++kk) {
+                  const uint64_t off = (uint64_t)((((kk >> 2) * BOX + (kk & 3) * 32) >> 4));
+                  mma_bf16_ss(dcol, qd + off, kd + off, IDESC_S, (c > 0 || kk > 0) ? 1u : 0u);
+                }
+                tc_commit(&k_empty[slot]);
               }
-              tc_commit(&k_empty[slot]);
               if (pass == PASSES - 1 && kt == u.kt - 1) tc_commit(&q_empty[c]);  // the unit's last read of query chunk c
             }
             if (!ok) break;
@@ -398,30 +405,30 @@ __global__ void __launch_bounds__(THREADS, 1)
               }
               if (!ok) break;
               tc_commit(&pv_done[pb]);
-              continue;
-            }
-            for (int x = 0; x < NWG && ok; ++x) ok = wait(&p_full[x][pb], pu & 1);
-            if (!ok) break;
-            tc_fence_after();
-            for (int sc = 0; sc < NSUB; ++sc, ++vc) {
-              const int slot = vc % VS;
-              if (!wait(&v_full[slot], (vc / VS) & 1)) {
-                ok = false;
-                break;
-              }
+            } else {
+              for (int x = 0; x < NWG && ok; ++x) ok = wait(&p_full[x][pb], pu & 1);
+              if (!ok) break;
               tc_fence_after();
-              const uint64_t vd = vdesc0 + (uint64_t)(slot * (BOX >> 4));
+              for (int sc = 0; sc < NSUB; ++sc, ++vc) {
+                const int slot = vc % VS;
+                if (!wait(&v_full[slot], (vc / VS) & 1)) {
+                  ok = false;
+                  break;
+                }
+                tc_fence_after();
+                const uint64_t vd = vdesc0 + (uint64_t)(slot * (BOX >> 4));
 #pragma unroll
-              for (int x = 0; x < NWG; ++x)
+                for (int x = 0; x < NWG; ++x)
 #pragma unroll
-                for (int kk = 0; kk < KW / 16; ++kk)
-                  mma_bf16_ts(tbase + COL_O + sc * 64, pcol + x * KW + kk * 8,
-                              vd + (uint64_t)((KW / 16 * x + kk) * 128), IDESC_O,
-                              (kt == 0 && x == 0 && kk == 0) ? 0u : 1u);
-              tc_commit(&v_empty[slot]);
+                  for (int kk = 0; kk < KW / 16; ++kk)
+                    mma_bf16_ts(tbase + COL_O + sc * 64, pcol + x * KW + kk * 8,
+                                vd + (uint64_t)((KW / 16 * x + kk) * 128), IDESC_O,
+                                (kt == 0 && x == 0 && kk == 0) ? 0u : 1u);
+                tc_commit(&v_empty[slot]);
+              }
+              if (!ok) break;
+              tc_commit(&pv_done[pb]);
             }
-            if (!ok) break;
-            tc_commit(&pv_done[pb]);
           }
           if (ok) tc_commit(&o_ready);
         }
@@ -550,6 +557,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (quit) break;
         if (item >= 1) wait(&l_free, (item - 1) & 1);
         ctl.lsum[x][row] = l;
+        if (PACKED && x == 0) ctl.msum[row] = m;
         mbar_arrive(&l_full);
       }
     }
@@ -610,6 +618,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         float l = 0.f;
 #pragma unroll
         for (int y = 0; y < NWG; ++y) l += ctl.lsum[y][row];
+        const float m = PACKED ? ctl.msum[row] : 0.f;
         mbar_arrive(&l_free);
         // A packed row that sees no key: zeros (its masked probabilities are not exactly zero: ex2_fma's smallest is 2^-126).
         const float inv = l > 0.f && !(PACKED && u.lim0 + pos <= 0) ? 1.f / l : 0.f;
@@ -624,7 +633,17 @@ __global__ void __launch_bounds__(THREADS, 1)
             tc_fence_before();
             mbar_arrive(&o_free);
           }
-          if (live) {
+          if (PACKED && u.part >= 0) {  // a part: fp32, a column of rows at a time
+            if constexpr (PACKED) {
+              float* part = src.parts + (int64_t)u.part * ((D + 2) * BM) + row;
+#pragma unroll
+              for (int i = 0; i < 64; ++i) part[(pass * DH + c * 64 + i) * BM] = __uint_as_float(r0[i]);
+              if (c == 0) {
+                part[D * BM] = u.lim0 + pos > 0 ? m : -INFINITY;
+                part[(D + 1) * BM] = u.lim0 + pos > 0 ? l : 0.f;
+              }
+            }
+          } else if (live) {
             if constexpr (PACKED) {
 #pragma unroll
               for (int i = 0; i < 64; ++i) odd = fmaf(__uint_as_float(r0[i]), 0.f, odd);
@@ -644,7 +663,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         if constexpr (PACKED) odd = fmaf(l, 0.f, odd);
       }
       if constexpr (PACKED) {
-        const bool redo = live && odd != 0.f && !abort_flag;
+        if (u.part >= 0 && u.part % u.b == 0 && row == 0)  // a unit's first part
+          reinterpret_cast<PartMeta*>(src.meta + 8)[u.part / u.b] = {u.qt, u.h, u.q0, u.npos, u.k0, u.lim0, {0, 0}};
+        const bool redo = live && u.part < 0 && odd != 0.f && !abort_flag;
         __syncwarp();  // the rows' first results are written before they are written again
         for (unsigned left = __ballot_sync(0xffffffffu, redo); left; left &= left - 1) {
           const int w = __ffs(left) - 1;
@@ -756,8 +777,10 @@ cudaError_t launch_packed_wide_d(const PackedArgs& a, cudaStream_t stream) {
   p.qscale = a.scale * kLog2e;
   p.out = reinterpret_cast<__nv_bfloat16*>(a.out);
   p.status = a.status;
-  return launch_dependent(prefill_wide_kernel<PackedSrc, D>, dim3(packed_grid(a, positions)), dim3(THREADS), (size_t)SMEM_BYTES,
-                          stream, qm, km, vm, p, packed_source(a, positions));
+  const pfx::PackedSrc src = packed_source(a, positions);
+  const cudaError_t e = launch_dependent(prefill_wide_kernel<PackedSrc, D>, dim3(packed_grid(a, positions)), dim3(THREADS),
+                                         (size_t)SMEM_BYTES, stream, qm, km, vm, p, src);
+  return e != cudaSuccess ? e : launch_packed_join(a, src, stream);
 }
 
 cudaError_t launch_packed_tc_wide(const PackedArgs& a, cudaStream_t stream) {

@@ -62,6 +62,7 @@ SIGNATURES = {
     "omniasr_paged_attention_workspace": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i, _i]),
     "omniasr_paged_attention": (_i, [_p, _p, _p, _p, _p, _i64, _i, _i64, _i64, _i64, _p, _i64, _i, _p, _p, _i, _i, _i, _i,
                                      _i, _f, _i, _i, _p, _sz, _p, _p]),
+    "omniasr_packed_attention_workspace": (_sz, [_i64, _i, _i, _i, _i]),
     "omniasr_packed_attention": (_i, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _i64, _i, _i, _i,
                                       _i, _f, _i, _p, _sz, _p, _p]),
     "omniasr_decode_gemm_workspace": (_sz, [_i, _i, _i, _i]),

@@ -633,6 +633,12 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     return out
 
 
+@functools.lru_cache(maxsize=4096)
+def _packed_ws(*shape: int) -> int:
+    """Workspace bytes of a packed_attention call (a function of host sizes alone)."""
+    return _lib.load().omniasr_packed_attention_workspace(*shape)
+
+
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor,
                      k_offsets: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
     """Causal attention of packed sequences: sequence s has queries ``q_offsets[s]`` .. ``q_offsets[s + 1] - 1`` of ``q``
@@ -662,15 +668,12 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offset
     device = q.device
     q_offsets, k_offsets = _index(q_offsets), _index(k_offsets)
     status, stream = _launch(device)
-    ws = _attn_workspace(_PACKED_WS, device, stream)
+    ws = _attn_workspace(_packed_ws(tq, heads, kv_heads, dim, dtype), device, stream)
     _lib.call("omniasr_packed_attention", q.data_ptr(), q_stride[0], q_stride[1], k.data_ptr(), k_stride[0], k_stride[1],
               v.data_ptr(), v_stride[0], v_stride[1], out.data_ptr(), q_offsets.data_ptr(), k_offsets.data_ptr(), tq, tk,
               seqs, heads, kv_heads, dim, dim**-0.5 if scale is None else scale, dtype, ws.data_ptr(), ws.numel(),
               status, stream)
     return out
-
-
-_PACKED_WS = 256
 
 
 def splits_for(rows: int, heads: int, keys: int, block: int = 64, programs: int = 264) -> tuple[int, int]:

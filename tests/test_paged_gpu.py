@@ -76,7 +76,7 @@ LENS = [0, 1, 2, 15, 16, 17, 127, 128, 129, 300, 511, 700]
 @pytest.mark.parametrize("heads,kv,dim,page,dtype", [
     (8, 2, 128, 16, "bf16"), (4, 4, 128, 64, "bf16"), (6, 2, 128, 8, "bf16"), (32, 1, 128, 32, "bf16"), (16, 1, 128, 128, "bf16"),
     (4, 4, 512, 64, "bf16"), (8, 1, 512, 16, "bf16"), (4, 2, 256, 16, "bf16"), (3, 3, 64, 16, "bf16"), (4, 1, 128, 12, "bf16"),
-    (4, 2, 128, 256, "bf16"), (2, 2, 32, 4, "bf16"), (2, 1, 16, 1, "bf16"),
+    (4, 2, 128, 256, "bf16"), (2, 2, 32, 4, "bf16"), (2, 1, 16, 1, "bf16"), (8, 2, 64, 32, "bf16"), (16, 1, 64, 128, "bf16"), (20, 1, 256, 64, "bf16"),
     (4, 2, 64, 16, "f32"), (3, 1, 128, 16, "f32"), (2, 2, 512, 8, "f32"), (4, 4, 16, 5, "f32"), (8, 1, 256, 16, "f32")])
 def test_paged_one_token(heads, kv, dim, page, dtype, kind):
     run_paged(heads, kv, dim, page, LENS, 1, dtype, kind)
@@ -84,7 +84,7 @@ def test_paged_one_token(heads, kv, dim, page, dtype, kind):
 
 @pytest.mark.parametrize("kind", ["own", "fp8"])
 @pytest.mark.parametrize("heads,kv,dim,page,tokens,dtype", [
-    (4, 4, 128, 64, 5, "bf16"), (8, 2, 128, 16, 2, "bf16"), (8, 2, 128, 16, 4, "bf16"), (8, 2, 128, 16, 7, "bf16"),
+    (4, 4, 128, 64, 5, "bf16"), (8, 2, 128, 16, 2, "bf16"), (8, 2, 128, 16, 4, "bf16"), (8, 2, 128, 16, 7, "bf16"), (8, 2, 64, 16, 5, "bf16"), (4, 2, 256, 16, 3, "bf16"),
     (2, 2, 512, 32, 8, "bf16"), (4, 2, 64, 16, 3, "f32"), (6, 2, 128, 16, 1, "bf16"), (10, 2, 128, 32, 3, "bf16")])
 def test_paged_drafts(heads, kv, dim, page, tokens, dtype, kind):
     run_paged(heads, kv, dim, page, [0, 1, 3, 16, 120, 126, 127, 128, 130, 385], tokens, dtype, kind, seed=3)
@@ -92,7 +92,7 @@ def test_paged_drafts(heads, kv, dim, page, tokens, dtype, kind):
 
 @pytest.mark.parametrize("layout", ["token", "both"])
 @pytest.mark.parametrize("kind", ["own", "fp8"])
-@pytest.mark.parametrize("dim,dtype", [(128, "bf16"), (512, "bf16"), (64, "f32")])
+@pytest.mark.parametrize("dim,dtype", [(64, "bf16"), (128, "bf16"), (512, "bf16"), (64, "f32")])
 def test_paged_other_layouts(layout, kind, dim, dtype):
     run_paged(4, 2, dim, 16, [5, 40, 260], 1, dtype, kind, seed=4, layout=layout)
 
@@ -105,13 +105,48 @@ def test_paged_long_row(kind, heads, kv, dim):
 
 
 @pytest.mark.parametrize("kind", ["own", "fp8"])
+@pytest.mark.parametrize("heads,kv,dim,page,rows,n", [(8, 4, 128, 8, 40, 3000), (4, 4, 512, 16, 20, 1500), (4, 2, 256, 64, 40, 2500),
+                                                      (32, 2, 64, 32, 60, 2000), (32, 2, 128, 128, 40, 2500), (16, 1, 512, 32, 30, 2000)])
+def test_paged_batches(kind, heads, kv, dim, page, rows, n):
+    """Ragged batches that send every CTA through many tiles and several segments (ring slots that hold K and V in turn),
+    against the formula in float64 on the GPU."""
+    g = torch.Generator().manual_seed(rows)
+    lens = [n - (i * 977) % n for i in range(rows)]
+    table, pool = pu.table_for(lens, page, g)
+    cg = torch.Generator(device=DEV).manual_seed(1)
+    pages, scales, values = [], [], []
+    for _ in range(2):
+        x = torch.randn(pool, kv, page, dim, generator=cg, device=DEV).to(torch.bfloat16)
+        if kind == "fp8":
+            e = torch.frexp(x.float().abs().amax(-1))[1] - 8  # (any exponent that holds the vector)
+            codes = torch.ldexp(x.float(), -e[..., None]).to(torch.float8_e4m3fn)
+            pages.append(codes)
+            scales.append((e + 127).to(torch.uint8))
+            values.append(codes.float() * 2.0 ** e.float()[..., None])
+        else:
+            pages.append(x)
+            scales.append(None)
+            values.append(x)
+    q = torch.randn(rows, heads, dim, generator=cg, device=DEV).to(torch.bfloat16)
+    got = kernels.paged_attention(q, *pages, table.to(DEV), torch.tensor(lens, device=DEV), dim**-0.5, k_scale=scales[0],
+                                  v_scale=scales[1])
+    for r, m in enumerate(lens):
+        ids = table[r].long().to(DEV)[: -(-m // page)]
+        k, v = (t[ids].double().transpose(0, 1).reshape(kv, -1, dim)[:, :m] for t in values)
+        qr = q[r].double().view(kv, heads // kv, dim)
+        p = torch.softmax(qr @ k.transpose(1, 2) * dim**-0.5, -1)
+        want, size = ((p @ t).view(heads, dim).cpu() for t in (v, v.abs()))
+        check(got[r], want, size, torch.bfloat16, m if kind == "fp8" else 0, float(v.abs().max()))
+
+
+@pytest.mark.parametrize("kind", ["own", "fp8"])
 def test_paged_many_rows(kind):
     """More rows than one launch schedules at a time, most of them short, many empty."""
     run_paged(2, 2, 128, 16, [(i * 37) % 50 for i in range(1500)], 1, "bf16", kind, seed=6)
 
 
 @pytest.mark.parametrize("kind", ["own", "fp8"])
-@pytest.mark.parametrize("dim,dtype", [(128, "bf16"), (512, "bf16"), (32, "f32")])
+@pytest.mark.parametrize("dim,dtype", [(64, "bf16"), (128, "bf16"), (256, "bf16"), (512, "bf16"), (32, "f32")])
 def test_paged_scores_far_apart(kind, dim, dtype):
     """Scores that grow by hundreds along the keys, and a first key far below: the running maximum has to follow; values
     whose scales differ by 2^40."""
@@ -335,7 +370,8 @@ def test_packed_prompts(heads, kv, dim, dtype, fused):
 
 
 @pytest.mark.parametrize("heads,kv,dim,dtype", [(8, 2, 128, "bf16"), (4, 4, 128, "bf16"), (2, 1, 512, "bf16"), (4, 2, 64, "f32"),
-                                                (64, 1, 128, "bf16"), (100, 1, 128, "bf16"), (48, 1, 512, "bf16")])
+                                                (64, 1, 128, "bf16"), (100, 1, 128, "bf16"), (48, 1, 512, "bf16"), (130, 1, 64, "bf16"),
+                                                (4, 2, 64, "bf16"), (4, 1, 256, "bf16")])
 def test_packed_chunks(heads, kv, dim, dtype):
     """Chunks with keys before them, sequences with fewer keys than queries (rows that see nothing) or none."""
     new = [1, 5, 100, 33, 0, 9, 130]
@@ -343,9 +379,31 @@ def test_packed_chunks(heads, kv, dim, dtype):
     run_packed(heads, kv, dim, new, keys, dtype, seed=2)
 
 
-@pytest.mark.parametrize("heads,kv,dim", [(4, 1, 128), (2, 2, 512)])
+@pytest.mark.parametrize("heads,kv,dim", [(4, 1, 128), (2, 2, 512), (4, 2, 64), (2, 1, 256)])
 def test_packed_long(heads, kv, dim):
     run_packed(heads, kv, dim, [1111, 64], [1111 + 700, 2000], "bf16", seed=3)
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 64), (4, 4, 128), (6, 2, 128), (2, 1, 256), (2, 2, 512), (4, 1, 512)])
+def test_packed_few_rows_over_many_keys(heads, kv, dim):
+    """Few units: each is cut along its keys, and its parts are added up (the last parts of short sequences are empty)."""
+    run_packed(heads, kv, dim, [3, 40, 1, 7, 0, 5], [1500, 700, 2, 7, 30, 4], "bf16", seed=6)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256, 512])
+def test_packed_cut_units_with_hidden_values(dim):
+    """As test_packed_hidden_values_stay_out, where the units are cut."""
+    g = torch.Generator().manual_seed(9)
+    q = torch.randn(4, 2, dim, generator=g).to(torch.bfloat16)
+    k = torch.randn(900, 2, dim, generator=g).to(torch.bfloat16)
+    v = torch.randn(900, 2, dim, generator=g).to(torch.bfloat16)
+    off, k_off = [0, 4], [0, 900]
+    want = pu.packed(q, k, v, off, k_off, dim**-0.5)
+    size = pu.packed(q, k, v.abs(), off, k_off, dim**-0.5)
+    k[898], v[898] = float("nan"), float("nan")
+    got = kernels.packed_attention(q.to(DEV), k.to(DEV), v.to(DEV), torch.tensor(off, device=DEV), torch.tensor(k_off, device=DEV))
+    check(got[:2], want[:2], size[:2], torch.bfloat16)
+    assert bool(torch.isnan(got[2:]).all())
 
 
 @pytest.mark.parametrize("dim,dtype", [(128, "bf16"), (512, "bf16"), (64, "f32")])
@@ -354,7 +412,7 @@ def test_packed_large_scores(dim, dtype):
     run_packed(4, 2, dim, [150, 40], [400, 40], "bf16" if dtype == "bf16" else "f32", seed=4, big=30.0 if dtype == "bf16" else 3.0)
 
 
-@pytest.mark.parametrize("dim,dtype", [(128, "bf16"), (512, "bf16"), (64, "f32"), (64, "bf16")])
+@pytest.mark.parametrize("dim,dtype", [(128, "bf16"), (512, "bf16"), (64, "f32"), (64, "bf16"), (256, "bf16"), (32, "bf16")])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 def test_packed_hidden_values_stay_out(dim, dtype, bad):
     """What is not finite in the keys and values of a position reaches the queries that see it, and no other query and no
