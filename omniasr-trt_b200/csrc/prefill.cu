@@ -598,6 +598,27 @@ __global__ void __launch_bounds__(THREADS, 1)
         live = q < p.width;
       }
       float odd = 0.f;  // packed: turns NaN if a result of the row is not finite
+      if constexpr (PACKED) {
+        if (u.part >= 0) {  // a part of a unit: fp32, a column of rows at a time
+          if (u.part % u.b == 0 && row == 0)
+            reinterpret_cast<PartMeta*>(src.meta + 8)[u.part / u.b] = {u.qt, u.h, u.q0, u.npos, u.k0, u.lim0, {0, 0}};
+          float* part = src.parts + (int64_t)u.part * ((D + 2) * BM) + row;
+          part[D * BM] = u.lim0 + pos > 0 ? m : -INFINITY;
+          part[(D + 1) * BM] = u.lim0 + pos > 0 ? l : 0.f;
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c, part += 32 * BM) {
+            float o[32];
+            tmem_ld32(tbase + lane_off + COL_O + c * 32, o);
+            if (c == D / 32 - 1) {
+              tc_fence_before();
+              mbar_arrive(&o_free);
+            }
+#pragma unroll
+            for (int i = 0; i < 32; ++i) part[i * BM] = o[i];
+          }
+          continue;
+        }
+      }
       // O in two halves of 64 columns (two loads in flight per wait), released to the next unit's first P V once the
       // second half is in registers, before it is scaled and stored (measured: 183.0 us per config-4 call against
       // 186.5 us with four 32-column reads and the release after the last store).
@@ -611,17 +632,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           tc_fence_before();
           mbar_arrive(&o_free);
         }
-        if (PACKED && u.part >= 0) {  // a part: fp32, a column of rows at a time
-          if constexpr (PACKED) {
-            float* part = src.parts + (int64_t)u.part * ((D + 2) * BM) + row;
-#pragma unroll
-            for (int i = 0; i < 64; ++i) part[(c * 64 + i) * BM] = __uint_as_float(r0[i]);
-            if (c == 0) {
-              part[D * BM] = u.lim0 + pos > 0 ? m : -INFINITY;
-              part[(D + 1) * BM] = u.lim0 + pos > 0 ? l : 0.f;
-            }
-          }
-        } else if (live) {
+        if (live) {
           if constexpr (PACKED) {
 #pragma unroll
             for (int i = 0; i < 64; ++i) odd = fmaf(__uint_as_float(r0[i]), 0.f, odd);
@@ -639,9 +650,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       }
       if constexpr (PACKED) {
-        if (u.part >= 0 && u.part % u.b == 0 && row == 0)  // a unit's first part
-          reinterpret_cast<PartMeta*>(src.meta + 8)[u.part / u.b] = {u.qt, u.h, u.q0, u.npos, u.k0, u.lim0, {0, 0}};
-        const bool redo = live && u.part < 0 && !(odd == 0.f && l - l == 0.f);
+        const bool redo = live && !(odd == 0.f && l - l == 0.f);
         __syncwarp();  // the rows' first results are written before they are written again
         for (unsigned left = __ballot_sync(0xffffffffu, redo); left; left &= left - 1) {
           const int w = __ffs(left) - 1;

@@ -623,6 +623,26 @@ __global__ void __launch_bounds__(THREADS, 1)
         // A packed row that sees no key: zeros (its masked probabilities are not exactly zero: ex2_fma's smallest is 2^-126).
         const float inv = l > 0.f && !(PACKED && u.lim0 + pos <= 0) ? 1.f / l : 0.f;
         __nv_bfloat16* dst = row_out + pass * DH;
+        if constexpr (PACKED) {
+          if (u.part >= 0) {  // a part: fp32, a column of rows at a time
+            float* part = src.parts + (int64_t)u.part * ((D + 2) * BM) + row;
+            part[D * BM] = u.lim0 + pos > 0 ? m : -INFINITY;
+            part[(D + 1) * BM] = u.lim0 + pos > 0 ? l : 0.f;
+            part += pass * DH * BM;
+#pragma unroll 1
+            for (int c = 0; c < DH / 32; ++c, part += 32 * BM) {
+              float o[32];
+              tmem_ld32(tbase + lane_off + COL_O + c * 32, o);
+              if (c == DH / 32 - 1) {
+                tc_fence_before();
+                mbar_arrive(&o_free);
+              }
+#pragma unroll
+              for (int i = 0; i < 32; ++i) part[i * BM] = o[i];
+            }
+            continue;
+          }
+        }
 #pragma unroll 1
         for (int c = 0; c < DH / 64; ++c) {
           uint32_t r0[64];
@@ -633,17 +653,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             tc_fence_before();
             mbar_arrive(&o_free);
           }
-          if (PACKED && u.part >= 0) {  // a part: fp32, a column of rows at a time
-            if constexpr (PACKED) {
-              float* part = src.parts + (int64_t)u.part * ((D + 2) * BM) + row;
-#pragma unroll
-              for (int i = 0; i < 64; ++i) part[(pass * DH + c * 64 + i) * BM] = __uint_as_float(r0[i]);
-              if (c == 0) {
-                part[D * BM] = u.lim0 + pos > 0 ? m : -INFINITY;
-                part[(D + 1) * BM] = u.lim0 + pos > 0 ? l : 0.f;
-              }
-            }
-          } else if (live) {
+          if (live) {
             if constexpr (PACKED) {
 #pragma unroll
               for (int i = 0; i < 64; ++i) odd = fmaf(__uint_as_float(r0[i]), 0.f, odd);
