@@ -940,6 +940,7 @@ pfx::PackedSrc packed_source(const PackedArgs& a, int positions) {
   s.kv_heads = a.kv_heads;
   s.group = a.heads / a.kv_heads;
   s.pos = positions;
+  s.pos_magic = 0xffffffffu / (unsigned)positions + 1;
   s.counters = a.counters;
   s.meta = nullptr;
   s.parts = nullptr;

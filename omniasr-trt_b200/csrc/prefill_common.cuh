@@ -171,9 +171,12 @@ OMNI_DEV int cta_unit(const Sched& s, int units, int n) {
 // A unit's query tile holds `pos` consecutive positions of one kv head's G = heads / kv_heads query heads: tile row r is
 // position r / G, head kv * G + r % G, so that the G heads share every key tile and a short sequence fills more of the
 // 128 rows. Units are claimed by the CTAs as they become free (an atomic counter; the first by block index): sequences in
-// order, each in groups of 16 kv heads, a group's longest query tiles first. Claiming keeps the CTAs' end times together
-// whatever the lengths, which the device alone knows; the warp that loads K claims, and hands the units to the other
-// roles through a ring in shared memory. Where the units would leave half of the CTAs idle (a short chunk over many keys),
+// order, each in groups of 16 kv heads, a group's longest query tiles first, so that the CTAs at work share keys in L2; but
+// the last sequences, until they hold two units per CTA, as one, the longest units of all of them first: a last sequence
+// of its own ends with one long unit on some CTAs and nothing on the others (8 prompts of 1400-1500, 8 heads of 512: 277
+// against 253 us; all sequences as one lose the keys in L2, 16 heads of 128: 92 against 105).
+// Claiming keeps the CTAs' end times together whatever the lengths, which the device alone knows; the warp that loads K
+// claims, and hands the units to the other roles through a ring in shared memory. Where the units would leave half of the CTAs idle (a short chunk over many keys),
 // each is cut into up to grid / units parts along its keys; a part leaves its maxima, sums and unnormalised output in fp32,
 // and packed_join_kernel adds the parts up.
 struct PackedSrc {
@@ -182,6 +185,7 @@ struct PackedSrc {
   int64_t q_tokens, k_tokens;
   int seqs, heads, kv_heads, group;  // group: query heads per kv head
   int pos;                           // positions per query tile
+  unsigned pos_magic;                // ceil(2^32 / pos)
   unsigned* counters;                // [0] units claimed, [1] CTAs done: zero on entry and left zero
   int* meta;                         // null: no unit is cut. [0] units, [1] parts per unit; then PartMeta per unit
   float* parts;                      // [unit * parts per unit + part][(D + 2) * 128]: O [D][128 rows], maxima, sums
@@ -214,6 +218,10 @@ struct PackedWalk {
   int tiles;          // this lane's sequence: query tiles, first query / key token, queries, keys
   int q0, k0, lq, lk;
   int cut;            // parts per unit
+  int w0;             // first lane of the group that is taken as one (32: none; only in the last block)
+  int level;          // the group's units are found from the longest down: the key tiles in hand,
+  long long above;    // and the group's units longer than that
+  long long group;    // units of the group
 
   OMNI_DEV void load(const PackedSrc& p, int lane, int* status) {
     const int s = s0 + lane;
@@ -234,6 +242,26 @@ struct PackedWalk {
       if (lane >= o) c += y;
     }
     incl = c;
+    w0 = 32;
+    if (s0 + 32 >= p.seqs) {
+      // The last sequences until they hold two units per CTA.
+      const long long all = __shfl_sync(0xffffffffu, incl, 31);
+      const unsigned in = __ballot_sync(0xffffffffu, all - incl < 2ll * gridDim.x && lk < (1 << 24));
+      w0 = 32 - __clz(~in);  // the lanes from the top
+      group = all - (w0 > 0 ? __shfl_sync(0xffffffffu, incl, (w0 - 1) & 31) : 0);
+      level = (int)__reduce_max_sync(0xffffffffu, lane >= w0 && tiles > 0 ? (unsigned)max(1, (lk + 127) / 128) : 0u);
+      above = 0;
+    }
+  }
+  // This lane's query tiles of `l` key tiles and more, if it is of the group.
+  OMNI_DEV int at_least(const PackedSrc& p, int lane, int l) const {
+    if (lane < w0 || tiles == 0) return 0;
+    if (l <= 1) return tiles;
+    const int keys = 128 * (l - 1) + 1;  // tile qt sees min(lk, lk - lq + (qt + 1) pos) keys
+    if (lk < keys) return 0;
+    const int x = keys - (lk - lq);
+    const int q = x <= 0 ? 0 : (p.pos == 1 ? x : (int)__umulhi((unsigned)(x + p.pos - 1), p.pos_magic)) - 1;
+    return tiles - max(0, q);
   }
   OMNI_DEV void init(const PackedSrc& p, int lane, int* status) {
     before = 0;
@@ -283,6 +311,10 @@ struct PackedWalk {
     r.kt = 0;
     r.part = -1;
     for (;;) {
+      if (w0 < 32) {
+        const long long in_order = w0 > 0 ? __shfl_sync(0xffffffffu, incl, (w0 - 1) & 31) : 0;
+        if (u >= before + in_order) return find_in_group(p, u - before - in_order, lane);
+      }
       const unsigned hit = __ballot_sync(0xffffffffu, u < before + incl);
       if (!hit) {
         if (s0 + 32 >= p.seqs) return r;
@@ -299,18 +331,50 @@ struct PackedWalk {
       const int hg = rem / (kUnitHeads * nt);
       rem -= hg * kUnitHeads * nt;
       const int gs = min(kUnitHeads, p.kv_heads - hg * kUnitHeads);
-      const int qt = nt - 1 - rem / gs;
-      r.h = hg * kUnitHeads + rem % gs;
-      r.b = 0;
-      r.qt = qt;
-      r.q0 = sq + qt * p.pos;
-      r.npos = min(p.pos, nq - qt * p.pos);
-      r.k0 = sk;
-      r.lim0 = qt * p.pos + 1 + nk - nq;
-      const int seen = r.lim0 + r.npos - 1;
-      r.kt = seen > 128 ? (seen + 127) / 128 : 1;  // a tile that sees nothing still runs one (masked) key tile
+      fill(p, r, nt - 1 - rem / gs, hg * kUnitHeads + rem % gs, sq, sk, nq, nk);
       return r;
     }
+  }
+  OMNI_DEV void fill(const PackedSrc& p, Unit& r, int qt, int h, int sq, int sk, int nq, int nk) {
+    r.h = h;
+    r.b = 0;
+    r.qt = qt;
+    r.q0 = sq + qt * p.pos;
+    r.npos = min(p.pos, nq - qt * p.pos);
+    r.k0 = sk;
+    r.lim0 = qt * p.pos + 1 + nk - nq;
+    const int seen = r.lim0 + r.npos - 1;
+    r.kt = seen > 128 ? (seen + 127) / 128 : 1;  // a tile that sees nothing still runs one (masked) key tile
+  }
+  // Unit number `u` of the group (ascending from call to call): levels from the longest down, within a level the lanes'
+  // sequences in order, within a sequence tile by tile, the heads innermost.
+  OMNI_DEV Unit find_in_group(const PackedSrc& p, long long u, int lane) {
+    Unit r;
+    r.kt = 0;
+    r.part = -1;
+    if (u >= group) return r;
+    int longer, mine;  // this lane's tiles above the level, and of it and above
+    for (;; --level) {
+      longer = at_least(p, lane, level + 1);
+      mine = at_least(p, lane, level);
+      const long long n = (long long)__reduce_add_sync(0xffffffffu, (unsigned)(mine - longer)) * p.kv_heads;
+      if (u < above + n) break;
+      above += n;
+    }
+    int upto = mine - longer;  // tiles of the level up to this lane's
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += y;
+    }
+    const int rem = (int)(u - above);
+    const int tile = rem / p.kv_heads;
+    const int w = __ffs(__ballot_sync(0xffffffffu, tile < upto)) - 1;
+    const int in_lane = tile - __shfl_sync(0xffffffffu, upto - (mine - longer), w);
+    const int qt = __shfl_sync(0xffffffffu, tiles - longer, w) - 1 - in_lane;
+    fill(p, r, qt, rem - tile * p.kv_heads, __shfl_sync(0xffffffffu, q0, w), __shfl_sync(0xffffffffu, k0, w),
+         __shfl_sync(0xffffffffu, lq, w), __shfl_sync(0xffffffffu, lk, w));
+    return r;
   }
 };
 

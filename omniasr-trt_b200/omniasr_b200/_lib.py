@@ -7,10 +7,12 @@ is no other implementation behind these functions, so a missing library is an er
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import threading
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent.parent / "lib" / "libomniasr_b200.so"
+BINDING_PATH = LIB_PATH.parent / "_omniasr_torch.so"  # csrc/binding.cpp: the calls that take torch tensors themselves
 
 BF16, F32, FP8 = 0, 1, 2
 OK, ERR_ARGUMENT, ERR_UNSUPPORTED, ERR_WORKSPACE, ERR_CUDA, ERR_DEVICE = range(6)
@@ -98,6 +100,18 @@ def load() -> ctypes.CDLL:
                 fn.argtypes = args
             _lib = lib
     return _lib
+
+
+def load_binding():
+    """The extension module ``_omniasr_torch`` beside the library (raises if it was not built)."""
+    load()
+    if not BINDING_PATH.exists():
+        raise RuntimeError(f"{BINDING_PATH} is missing: build it with `make -C omniasr-trt_b200/csrc` "
+                           "or `python -c 'import __graft_entry__ as g; g.build()'`")
+    spec = importlib.util.spec_from_file_location("_omniasr_torch", BINDING_PATH)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
 
 
 def call(name: str, *args) -> None:

@@ -31,7 +31,6 @@ the built library every function raises.
 from __future__ import annotations
 
 import ctypes
-import functools
 
 import torch
 
@@ -498,46 +497,29 @@ def reorder_gather(src: torch.Tensor, parent: torch.Tensor, out: torch.Tensor | 
     return out
 
 
-def _launch(device: torch.device) -> tuple[int, int]:
-    """(the device's status word, the current stream) as the C ABI takes them; a few hundred nanoseconds, as the host's
-    time is what a small call waits for."""
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_native = None
+
+
+def _binding():
+    """The native calls (csrc/binding.cpp) behind the paged cache and the packed prompts."""
+    global _native
+    if _native is None:
+        _native = _lib.load_binding()
+    return _native
+
+
+def _context(device: torch.device) -> tuple:
+    """(the device's status word, the current stream, the stream's workspace or None) for the native calls, which refuse
+    tensors that are on no CUDA device."""
     index = device.index
+    if index is None:
+        return 0, 0, None
     word = _status.get(index)
     if word is None:
         word = status_word(index)
-    return word.data_ptr(), _raw_stream(index)
-
-
-_raw_stream = torch._C._cuda_getCurrentRawStream
-
-
-def _pages(k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None, v_scale: torch.Tensor | None, dtype: int,
-           name: str) -> tuple:
-    """A paged cache's arguments: (k, v, k_scale, v_scale, pages, page, strides), kv heads, head_dim and type code."""
-    shape, stride, kind = k.shape, k.stride(), k.dtype
-    if len(shape) != 4 or v.shape != shape or v.stride() != stride or stride[3] != 1 or v.dtype != kind:
-        raise ValueError(f"{name}: k and v pages must be [pages, kv_heads, page, D] views of one dtype with the same "
-                         "strides and unit stride in D")
-    pages, kv_heads, page, dim = shape
-    geometry = (pages, page, stride[0], stride[1], stride[2])
-    if kind == torch.float8_e4m3fn:
-        for t in (k_scale, v_scale):
-            if t is None or t.dtype != torch.uint8 or t.shape != shape[:3] or not t.is_contiguous():
-                raise ValueError(f"{name}: float8_e4m3fn pages need contiguous uint8 scales [pages, kv_heads, page]")
-        return (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr()), geometry, kv_heads, dim, _lib.FP8
-    code = _DTYPES.get(kind)
-    if code != dtype:
-        raise ValueError(f"{name}: pages of {kind} (supported: the queries' dtype, float8_e4m3fn)")
-    if k_scale is not None or v_scale is not None:
-        raise ValueError(f"{name}: scales belong to float8_e4m3fn pages")
-    return (k.data_ptr(), v.data_ptr(), None, None), geometry, kv_heads, dim, code
-
-
-def _table(table: torch.Tensor, rows: int, name: str) -> tuple[int, int, int]:
-    shape, stride = table.shape, table.stride()
-    if table.dtype != torch.int32 or len(shape) != 2 or shape[0] < rows or (shape[1] > 1 and stride[1] != 1):
-        raise ValueError(f"{name}: page_table must be int32 [rows, width] with unit inner stride")
-    return table.data_ptr(), stride[0], shape[1]
+    stream = _raw_stream(index)
+    return word.data_ptr(), stream, _ATTN_WS.get((index, stream))
 
 
 def paged_rope_kv(qkv: torch.Tensor, cs: torch.Tensor, pos: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -549,25 +531,8 @@ def paged_rope_kv(qkv: torch.Tensor, cs: torch.Tensor, pos: torch.Tensor, k_page
     float8_e4m3fn codes with one scale byte per vector in ``k_scale``/``v_scale`` (uint8 [pages, kv_heads, page]): the
     vector x is held as codes of x * 2^-e and the byte e + 127, e the smallest integer with max|x| <= 448 * 2^e (within
     [-40, 40])."""
-    dtype = _dtype(qkv, "paged_rope_kv")
-    ptrs, geo, kvh, dim, code = _pages(k_pages, v_pages, k_scale, v_scale, dtype, "paged_rope_kv")
-    shape, stride, table = qkv.shape, qkv.stride(), cs.shape
-    n = shape[0]
-    if kvh != kv_heads or len(shape) != 2 or shape[1] != (heads + 2 * kv_heads) * dim or (n and stride[1] != 1):
-        raise ValueError("paged_rope_kv: qkv must be [N, (heads + 2 * kv_heads) * D] with unit inner stride")
-    if pos.numel() != n or slots.numel() != n:
-        raise ValueError("paged_rope_kv: pos and slots must hold one entry per token")
-    if len(table) != 3 or table[1] != dim // 2 or table[2] != 2:
-        raise ValueError("paged_rope_kv: cs must be [P, D / 2, 2]")
-    device = qkv.device
-    q = qkv.new_empty(n, heads, dim)
-    if n == 0:
-        return q
-    cs = cs if cs.dtype == torch.float32 and cs.is_contiguous() else cs.float().contiguous()
-    pos, slots = _index(pos), _index(slots)
-    _lib.call("omniasr_paged_rope_kv", qkv.data_ptr(), stride[0], cs.data_ptr(), table[0], pos.data_ptr(),
-              slots.data_ptr(), q.data_ptr(), *ptrs, *geo, n, heads, kv_heads, dim, dtype, code, *_launch(device))
-    return q
+    status, stream, _ = _context(qkv.device)
+    return _binding().paged_rope_kv(qkv, cs, pos, k_pages, v_pages, slots, heads, kv_heads, k_scale, v_scale, status, stream)
 
 
 def paged_kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, offsets: torch.Tensor,
@@ -578,29 +543,8 @@ def paged_kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torc
     outside them are zeros). 8-bit pages are read as ``dtype`` (default bfloat16), others as what they hold."""
     if dtype is None:
         dtype = torch.bfloat16 if k_pages.dtype == torch.float8_e4m3fn else k_pages.dtype
-    out_code = _DTYPES.get(dtype)
-    if out_code is None:
-        raise ValueError(f"paged_kv_read: dtype {dtype} (supported: bfloat16, float32)")
-    ptrs, geo, kvh, dim, code = _pages(k_pages, v_pages, k_scale, v_scale, out_code, "paged_kv_read")
-    rows = offsets.numel() - 1
-    if rows < 0:
-        raise ValueError("paged_kv_read: offsets must hold rows + 1 entries")
-    table = _table(page_table, rows, "paged_kv_read")
-    device = k_pages.device
-    k = torch.empty(tokens, kvh, dim, device=device, dtype=dtype)
-    v = torch.empty_like(k)
-    if tokens == 0:
-        return k, v
-    offsets = _index(offsets)
-    _lib.call("omniasr_paged_kv_read", *ptrs, *geo, *table, rows, offsets.data_ptr(), tokens, k.data_ptr(), v.data_ptr(),
-              kvh, dim, out_code, code, *_launch(device))
-    return k, v
-
-
-@functools.lru_cache(maxsize=4096)
-def _paged_ws(*shape: int) -> int:
-    """Workspace bytes of a paged_attention call (a function of host sizes alone)."""
-    return _lib.load().omniasr_paged_attention_workspace(*shape)
+    status, stream, _ = _context(k_pages.device)
+    return _binding().paged_kv_read(k_pages, v_pages, page_table, offsets, tokens, k_scale, v_scale, dtype, status, stream)
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -610,33 +554,14 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     b * tokens ..; query i of row b sees positions [0, ``lengths[b]`` + i) of the pages that ``page_table`` [B, width]
     (int32) names, head h those of kv head h // (heads / kv_heads). Pages as :func:`paged_rope_kv` writes them. Returns
     q's shape and dtype; a query that sees nothing gets zeros."""
-    if q.dim() != 3 or not q.is_contiguous():
-        raise ValueError("paged_attention: q must be contiguous [B * tokens, heads, D]")
-    rows_q, heads, dim = q.shape
-    dtype = _dtype(q, "paged_attention")
-    ptrs, geo, kvh, pdim, code = _pages(k_pages, v_pages, k_scale, v_scale, dtype, "paged_attention")
-    if pdim != dim:
-        raise ValueError("paged_attention: q and the pages differ in head_dim")
-    if tokens < 1 or rows_q % tokens or lengths.numel() * tokens != rows_q:
-        raise ValueError(f"paged_attention: {rows_q} queries are not {lengths.numel()} rows of {tokens} tokens")
-    rows = rows_q // tokens
-    table = _table(page_table, rows, "paged_attention")
-    out = torch.empty_like(q)
-    if rows == 0:
-        return out
     device = q.device
-    lengths = _index(lengths)
-    status, stream = _launch(device)
-    ws = _attn_workspace(_paged_ws(dtype, code, rows, tokens, heads, kvh, dim, geo[1], table[2]), device, stream)
-    _lib.call("omniasr_paged_attention", q.data_ptr(), *ptrs, *geo, *table, lengths.data_ptr(), out.data_ptr(), rows, tokens,
-              heads, kvh, dim, scale, dtype, code, ws.data_ptr(), ws.numel(), status, stream)
+    status, stream, ws = _context(device)
+    out = _binding().paged_attention(q, k_pages, v_pages, page_table, lengths, scale, tokens, k_scale, v_scale, status, stream, ws)
+    if out.__class__ is int:  # the bytes of workspace it takes: nothing ran
+        ws = _attn_workspace(out, device, stream)
+        out = _binding().paged_attention(q, k_pages, v_pages, page_table, lengths, scale, tokens, k_scale, v_scale, status,
+                                         stream, ws)
     return out
-
-
-@functools.lru_cache(maxsize=4096)
-def _packed_ws(*shape: int) -> int:
-    """Workspace bytes of a packed_attention call (a function of host sizes alone)."""
-    return _lib.load().omniasr_packed_attention_workspace(*shape)
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor,
@@ -645,34 +570,13 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offset
     [Tq, heads, D] and keys ``k_offsets[s]`` .. (default: the queries' offsets) of ``k``/``v`` [Tk, kv_heads, D]; its last
     query sees its last key, so a chunk of a prompt attends to the keys before it. Any token and head strides with
     16-byte alignment, unit stride in D; offsets ascending, on the device. Returns [Tq, heads, D] in q's dtype (a query
-    that sees no key gets zeros; rows of no sequence are not written)."""
-    qs, ks, kind = q.shape, k.shape, q.dtype
-    if len(qs) != 3 or len(ks) != 3 or v.shape != ks or qs[2] != ks[2]:
-        raise ValueError("packed_attention: q [Tq, heads, D], k and v [Tk, kv_heads, D]")
-    if k.dtype != kind or v.dtype != kind:
-        raise ValueError("packed_attention: q, k and v must share a dtype")
-    tq, heads, dim = qs
-    tk, kv_heads, _ = ks
-    q_stride, k_stride, v_stride = q.stride(), k.stride(), v.stride()
-    if (tq and q_stride[2] != 1) or (tk and (k_stride[2] != 1 or v_stride[2] != 1)):
-        raise ValueError("packed_attention: unit stride in D")
-    dtype = _dtype(q, "packed_attention")
-    if k_offsets is None:
-        k_offsets = q_offsets
-    seqs = q_offsets.numel() - 1
-    if seqs < 0 or k_offsets.numel() != seqs + 1:
-        raise ValueError("packed_attention: q_offsets and k_offsets must hold sequences + 1 entries")
-    out = q.new_empty(tq, heads, dim)
-    if tq == 0:
-        return out
+    that sees no key gets zeros; rows of no sequence are not written). ``scale`` defaults to D ** -0.5."""
     device = q.device
-    q_offsets, k_offsets = _index(q_offsets), _index(k_offsets)
-    status, stream = _launch(device)
-    ws = _attn_workspace(_packed_ws(tq, heads, kv_heads, dim, dtype), device, stream)
-    _lib.call("omniasr_packed_attention", q.data_ptr(), q_stride[0], q_stride[1], k.data_ptr(), k_stride[0], k_stride[1],
-              v.data_ptr(), v_stride[0], v_stride[1], out.data_ptr(), q_offsets.data_ptr(), k_offsets.data_ptr(), tq, tk,
-              seqs, heads, kv_heads, dim, dim**-0.5 if scale is None else scale, dtype, ws.data_ptr(), ws.numel(),
-              status, stream)
+    status, stream, ws = _context(device)
+    out = _binding().packed_attention(q, k, v, q_offsets, k_offsets, scale, status, stream, ws)
+    if out.__class__ is int:  # the bytes of workspace it takes: nothing ran
+        ws = _attn_workspace(out, device, stream)
+        out = _binding().packed_attention(q, k, v, q_offsets, k_offsets, scale, status, stream, ws)
     return out
 
 
