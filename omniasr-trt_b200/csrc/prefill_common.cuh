@@ -173,8 +173,8 @@ OMNI_DEV int cta_unit(const Sched& s, int units, int n) {
 // 128 rows. Units are claimed by the CTAs as they become free (an atomic counter; the first by block index): sequences in
 // order, each in groups of 16 kv heads, a group's longest query tiles first, so that the CTAs at work share keys in L2; but
 // the last sequences, until they hold two units per CTA, as one, the longest units of all of them first: a last sequence
-// of its own ends with one long unit on some CTAs and nothing on the others (8 prompts of 1400-1500, 8 heads of 512: 277
-// against 253 us; all sequences as one lose the keys in L2, 16 heads of 128: 92 against 105).
+// of its own ends with one long unit on some CTAs and nothing on the others (8 prompts of 1400-1500, 8 heads of 512: 280
+// against 268 us; all sequences as one lose the keys in L2, 16 heads of 128: 92 against 105).
 // Claiming keeps the CTAs' end times together whatever the lengths, which the device alone knows; the warp that loads K
 // claims, and hands the units to the other roles through a ring in shared memory. Where the units would leave half of the CTAs idle (a short chunk over many keys),
 // each is cut into up to grid / units parts along its keys; a part leaves its maxima, sums and unnormalised output in fp32,
