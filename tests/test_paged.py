@@ -110,3 +110,43 @@ def test_workspace_sizes():
     assert size(_lib.BF16, _lib.FP8, 4, 1, 8, 2, 128, 16, 100) > 65536
     assert size(_lib.BF16, _lib.BF16, 4, 1, 8, 3, 128, 16, 100) == 0  # heads not a multiple
     assert size(_lib.BF16, _lib.BF16, 4, 1, 8, 2, 96, 16, 100) == 0  # head_dim
+
+
+def test_paged_cache_hands_out_pages():
+    """Pages, slots and offsets of a batch; nothing changes when the pages do not suffice; freed pages come back."""
+    from omniasr_b200.paged import PagedCache
+
+    c = PagedCache(2, 7, 4, 2, 16, device="cpu")
+    a, b = c.add(), c.add()
+    step = c.extend([a, b], [5, 0])
+    assert step.tokens == 5 and step.total == 5 and step.fresh
+    assert step.pos.tolist() == [0, 1, 2, 3, 4]
+    assert step.lengths.tolist() == [1, 1]
+    assert step.q_offsets.tolist() == [0, 5, 5] == step.k_offsets.tolist()
+    pages = step.table[0].tolist()
+    assert len(set(pages)) == 2
+    assert step.slots.tolist() == [pages[0] * 4 + i for i in range(4)] + [pages[1] * 4]
+    step = c.extend([b, a], [9, 4])
+    assert step.pos.tolist() == [*range(9), 5, 6, 7, 8]
+    assert step.k_offsets.tolist() == [0, 9, 18] and step.lengths.tolist() == [1, 6] and not step.fresh
+    assert sorted(set(step.table[0].tolist()) | set(step.table[1].tolist())) == sorted(set(range(7)) - set(c._free))
+    assert len(set((step.slots).tolist())) == 13
+    with pytest.raises(RuntimeError, match="full"):
+        c.extend([a, b], [4, 8])
+    assert c.length(a) == 9 and c.length(b) == 9 and c.free_pages == 1
+    with pytest.raises(ValueError, match="different"):
+        c.extend([a, a], [1, 1])
+    c.free(a)
+    assert c.free_pages == 4
+    assert c.extend([b], [3]).total == 12
+    c.free(b)
+    assert c.free_pages == 7
+
+
+def test_paged_cache_decode_wants_even_steps():
+    from omniasr_b200.paged import PagedCache
+
+    c = PagedCache(1, 4, 4, 1, 16, device="cpu")
+    batch = c.extend([c.add(), c.add()], [1, 2])
+    with pytest.raises(ValueError, match="same number"):
+        c.decode(0, torch.zeros(3, 48), torch.zeros(8, 8, 2), batch, 1)
