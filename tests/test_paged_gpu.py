@@ -390,6 +390,43 @@ def test_packed_few_rows_over_many_keys(heads, kv, dim):
     run_packed(heads, kv, dim, [3, 40, 1, 7, 0, 5], [1500, 700, 2, 7, 30, 4], "bf16", seed=6)
 
 
+MANY = [  # more units than CTAs; some sequences see fewer keys than queries
+    (32, 4, [300, 1, 0, 65, 500, 128, 250, 16, 17], [300, 200, 3, 20, 900, 0, 251, 16, 145]),
+    (60, 20, [430, 1, 300, 90], [430, 130, 260, 300]), (32, 32, [1100, 513], [1100, 600])]
+
+
+@pytest.mark.parametrize("heads,kv,new,keys", MANY)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_packed_many_units(heads, kv, new, keys, dim):
+    run_packed(heads, kv, dim, new, keys, "bf16", seed=7)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_packed_many_units_with_large_scores(dim):
+    run_packed(*MANY[0][:2], dim, *MANY[0][2:], "bf16", seed=8, big=30.0)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_packed_many_units_with_hidden_values(dim, bad):
+    """As test_packed_hidden_values_stay_out, where a sequence has many query tiles."""
+    g = torch.Generator().manual_seed(10)
+    off = [0, 600, 1300]
+    q = torch.randn(1300, 32, dim, generator=g).to(torch.bfloat16)
+    k = torch.randn(1300, 4, dim, generator=g).to(torch.bfloat16)
+    v = torch.randn(1300, 4, dim, generator=g).to(torch.bfloat16)
+    want = pu.packed(q, k, v, off, off, dim**-0.5)
+    size = pu.packed(q, k, v.abs(), off, off, dim**-0.5)
+    for at in (410, 600 + 690):
+        k[at], v[at] = bad, bad
+    got = kernels.packed_attention(q.to(DEV), k.to(DEV), v.to(DEV), torch.tensor(off, device=DEV))
+    blind = [*range(0, 410), *range(600, 1290)]
+    check(got[blind], want[blind], size[blind], torch.bfloat16)
+    if bad != bad:
+        assert bool(torch.isnan(got[410:600]).all()) and bool(torch.isnan(got[1290:]).all())
+    kernels.read_status()
+
+
 @pytest.mark.parametrize("dim", [64, 128, 256, 512])
 def test_packed_cut_units_with_hidden_values(dim):
     """As test_packed_hidden_values_stay_out, where the units are cut."""
