@@ -171,17 +171,6 @@ OMNI_DEV void tmem_ld16_async(uint32_t taddr, uint32_t* r) {
 }
 OMNI_DEV void tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
-// One lane of the (converged) warp.
-OMNI_DEV bool elect_one() {
-  uint32_t e;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "elect.sync _|p, 0xffffffff;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(e));
-  return e != 0;
-}
-
 // Column totals over a warp of NV values per lane; every lane gets every column's (maximum or sum).
 template <int NV, bool MAX>
 OMNI_DEV void warp_all(float (&v)[NV]) {
@@ -609,7 +598,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int i = 0, slot = 0, use = 0;
     bool ok = true;
     for (int n = 0; ok && w.next(s); ++n) {
-      ok = wait(&ctl.q_full[n % C::QN], (n / C::QN) & 1);
+      ok = __all_sync(0xffffffffu, wait(&ctl.q_full[n % C::QN], (n / C::QN) & 1));
       const uint64_t qd = qd0 + (uint64_t)((n % C::QN) * (C::QB >> 4));
       const int end = i + s.t1 - s.t0;
       for (; ok && i < end; ++i) {
@@ -617,7 +606,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (i >= 2) ok = wait(&ctl.s_free[b], ((i >> 1) - 1) & 1);
 #pragma unroll
         for (int c = 0; c < DC; ++c) {
-          ok = ok && wait_issued(slot, use + 1) && wait(&ctl.full[slot], use & 1);
+          // The lanes leave their waits together, with one answer: none is still at a barrier that these MMAs move on.
+          ok = __all_sync(0xffffffffu, ok && wait_issued(slot, use + 1) && wait(&ctl.full[slot], use & 1));
           if (!ok) break;
           tc_fence_after();
           if (leader) {
@@ -662,7 +652,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (int n = 0; ok && w.next(s); ++n) {
       const int ob = C::OB == 2 ? n & 1 : 0;
-      if (n >= C::OB) ok = wait(&ctl.o_free[ob], (n / C::OB - 1) & 1);
+      if (n >= C::OB) ok = __all_sync(0xffffffffu, wait(&ctl.o_free[ob], (n / C::OB - 1) & 1));
       const int begin = i, end = i + s.t1 - s.t0;
       for (; ok && i < end; ++i) {
         const int b = i & 1;
@@ -671,7 +661,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t fresh = i - begin < 2 ? 0u : 1u;  // a softmax group's first tile of the segment overwrites
 #pragma unroll
         for (int c = 0; c < DC; ++c) {
-          ok = ok && wait_issued(slot, use + 1) && wait(&ctl.full[slot], use & 1);
+          ok = __all_sync(0xffffffffu, ok && wait_issued(slot, use + 1) && wait(&ctl.full[slot], use & 1));
           if (!ok) break;
           tc_fence_after();
           if (leader) {
@@ -1221,7 +1211,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   if (abort_flag) {
     if (tid == 0) raise_status(p.status, kStatusTimeout);
-    if (tid == W_MMA * 32 || tid == W_PV * 32) {
+    if ((warp == W_MMA || warp == W_PV) && elect_one()) {
       tc_commit(&ctl.drain);  // every MMA issued has completed once this arrives
       mbar_wait(&ctl.drain, 0);
     }

@@ -202,6 +202,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       return true;
     }
   };
+  // The same for a warp that runs converged: its lanes leave their waits together, with one answer, so that none is still at
+  // a barrier that the MMAs issued next move on.
+  auto wwait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+  auto wget = [&](int n, Unit& u) { return __all_sync(0xffffffffu, get(n, u)) != 0; };
   auto put = [&](int n) {
     if constexpr (PACKED) mbar_arrive(&ctl.u_empty[n % kUnitRing]);
   };
@@ -307,63 +311,67 @@ __global__ void __launch_bounds__(THREADS, 1)
   } else if (warp == W_MMA) {
     // ------------------------------------------------------------------ S issuer: S[t % NSB] = Q K(t)^T
     // S[t % NSB] is free once O += P(t - NSB) V has completed (P(t - NSB) lies over it); the unit's Q slot is
-    // released after its last S (q_empty).
-    if (lane == 0) {
+    // released after its last S (q_empty). Both issuing warps run converged, one elected lane issuing, so that the
+    // descriptors are warp-uniform.
+    {
+      const bool leader = elect_one();
       // Slot s's descriptor is slot 0's with the start address (in 16-byte units, 14 bits) moved on by s tiles.
       const uint64_t kdesc0 = smem_desc(smem_addr(smem + K_OFF), 16, 1024, kLayoutSw128);
       const uint64_t qdesc0 = smem_desc(smem_addr(smem + Q_OFF), 16, 1024, kLayoutSw128);
       int tile = 0, nunit = 0, sb = 0;
       bool ok = true;
       Unit u;
-      for (; get(nunit, u) && ok && !abort_flag; ++nunit) {
+      for (; wget(nunit, u) && ok; ++nunit) {
         const int qslot = nunit % QS;
-        if (!wait(&q_full[qslot], (nunit / QS) & 1)) break;
+        if (!wwait(&q_full[qslot], (nunit / QS) & 1)) break;
         const uint64_t qd = qdesc0 + (uint64_t)(qslot * (TILE >> 4));
         for (int kt = 0; kt < u.kt; ++kt, ++tile, sb = sb == NSB - 1 ? 0 : sb + 1) {
           const int slot = tile % KS;
-          if (tile >= NSB && !wait(&pv_done[sb], ((tile - NSB) / NSB) & 1)) {
+          if (tile >= NSB && !wwait(&pv_done[sb], ((tile - NSB) / NSB) & 1)) {
             ok = false;
             break;
           }
-          if (!wait(&k_full[slot], (tile / KS) & 1)) {
+          if (!wwait(&k_full[slot], (tile / KS) & 1)) {
             ok = false;
             break;
           }
           tc_fence_after();
           const uint32_t dcol = tbase + COL_S + sb * 128;
           const uint64_t kd = kdesc0 + (uint64_t)(slot * (TILE >> 4));
+          if (leader) {
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint64_t off = (uint64_t)((((kk >> 2) * BOX + (kk & 3) * 32) >> 4));
-            mma_bf16_ss(dcol, qd + off, kd + off, IDESC_S, kk > 0 ? 1u : 0u);
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint64_t off = (uint64_t)((((kk >> 2) * BOX + (kk & 3) * 32) >> 4));
+              mma_bf16_ss(dcol, qd + off, kd + off, IDESC_S, kk > 0 ? 1u : 0u);
+            }
+            tc_commit(&s_full[sb]);
+            tc_commit(&k_empty[slot]);
+            if (kt == u.kt - 1) tc_commit(&q_empty[qslot]);  // the unit's last read of its query tile
+            OMNI_TRACE_AT(tile * 8 + 2);
           }
-          tc_commit(&s_full[sb]);
-          tc_commit(&k_empty[slot]);
-          if (kt == u.kt - 1) tc_commit(&q_empty[qslot]);  // the unit's last read of its query tile
-          OMNI_TRACE_AT(tile * 8 + 2);
         }
-        put(nunit);
+        if (leader) put(nunit);
       }
     }
-    __syncwarp();
   } else if (warp == W_MMA_PV) {
     // ------------------------------------------------------------------ PV issuer: O += P(t) V(t)
     // The two key halves in turn, as their softmax warpgroups finish; a unit's first tile overwrites O once the
     // epilogue has read the previous unit's (o_free).
-    if (lane == 0) {
+    {
+      const bool leader = elect_one();
       const uint64_t vdesc0 = smem_desc(smem_addr(smem + V_OFF), BOX, 1024, kLayoutSw128);
       int tile = 0, nunit = 0;
       bool ok = true;
       Unit u;
-      for (; get(nunit, u) && ok && !abort_flag; ++nunit) {
+      for (; wget(nunit, u) && ok; ++nunit) {
         for (int kt = 0; kt < u.kt; ++kt, ++tile) {
           const int pb = tile % NSB, pu = tile / NSB;
           const int slot = tile % VS;
-          if (kt == 0 && nunit >= 1 && !wait(&o_free, (nunit - 1) & 1)) {
+          if (kt == 0 && nunit >= 1 && !wwait(&o_free, (nunit - 1) & 1)) {
             ok = false;
             break;
           }
-          if (!wait(&v_full[slot], (tile / VS) & 1)) {
+          if (!wwait(&v_full[slot], (tile / VS) & 1)) {
             ok = false;
             break;
           }
@@ -371,23 +379,29 @@ __global__ void __launch_bounds__(THREADS, 1)
           const uint32_t pcol = tbase + COL_S + pb * 128;
 #pragma unroll
           for (int x = 0; x < NWG; ++x) {
-            if (!wait(&p_full[x][pb], pu & 1)) {
+            if (!wwait(&p_full[x][pb], pu & 1)) {
               ok = false;
               break;
             }
             tc_fence_after();
+            if (leader) {
 #pragma unroll
-            for (int kk = 0; kk < KW / 16; ++kk)
-              mma_bf16_ts(tbase + COL_O, pcol + x * KW + kk * 8, vd + (uint64_t)((KW / 16 * x + kk) * 128), IDESC_O,
-                          (kt == 0 && x == 0 && kk == 0) ? 0u : 1u);
+              for (int kk = 0; kk < KW / 16; ++kk)
+                mma_bf16_ts(tbase + COL_O, pcol + x * KW + kk * 8, vd + (uint64_t)((KW / 16 * x + kk) * 128), IDESC_O,
+                            (kt == 0 && x == 0 && kk == 0) ? 0u : 1u);
+            }
           }
           if (!ok) break;
-          tc_commit(&pv_done[pb]);
-          tc_commit(&v_empty[slot]);
-          OMNI_TRACE_AT(tile * 8 + 3);
+          if (leader) {
+            tc_commit(&pv_done[pb]);
+            tc_commit(&v_empty[slot]);
+            OMNI_TRACE_AT(tile * 8 + 3);
+          }
         }
-        if (ok) tc_commit(&o_ready);
-        put(nunit);
+        if (leader) {
+          if (ok) tc_commit(&o_ready);
+          put(nunit);
+        }
       }
     }
     __syncwarp();
@@ -667,7 +681,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   __syncthreads();
   if (abort_flag) {
     if (tid == 0) raise_status(p.status, kStatusTimeout);
-    if (tid == W_MMA * 32 || tid == W_MMA_PV * 32) {
+    if ((warp == W_MMA || warp == W_MMA_PV) && elect_one()) {
       // Every MMA an issuer thread issued has completed once its commit arrives (two issuers: two arrivals).
       tc_commit(&drain);
       mbar_wait(&drain, 0);

@@ -187,6 +187,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       return true;
     }
   };
+  // The same for a warp that runs converged: its lanes leave their waits together, with one answer, so that none is still at
+  // a barrier that the MMAs issued next move on.
+  auto wwait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+  auto wget = [&](int n, Unit& u) { return __all_sync(0xffffffffu, get(n, u)) != 0; };
   auto put = [&](int n) {
     if constexpr (PACKED) mbar_arrive(&ctl.u_empty[n % kUnitRing]);
   };
@@ -309,82 +313,88 @@ __global__ void __launch_bounds__(THREADS, 1)
     __syncwarp();
   } else if (warp == W_MMA) {
     // ------------------------------------------------------------------ S[t % NSB] = sum over chunks Q_c K_c(t)^T
-    if (lane == 0) {
+    {
+      const bool leader = elect_one();  // the issuing warps run converged (prefill.cu)
       const uint64_t kdesc0 = smem_desc(smem_addr(smem + K_OFF), 16, 1024, kLayoutSw128);
       const uint64_t qdesc0 = smem_desc(smem_addr(smem + Q_OFF), 16, 1024, kLayoutSw128);
       int tile = 0, kc = 0;
       bool ok = true;
       Unit u;
-      for (int n = 0; get(n, u) && ok && !abort_flag; ++n) {
+      for (int n = 0; wget(n, u) && ok; ++n) {
         for (int pass = 0; pass < PASSES && ok; ++pass) {
           for (int kt = 0; kt < u.kt && ok; ++kt, ++tile) {
             const int sb = tile % NSB;
-            if (tile >= NSB && !wait(&pv_done[sb], ((tile - NSB) / NSB) & 1)) {
+            if (tile >= NSB && !wwait(&pv_done[sb], ((tile - NSB) / NSB) & 1)) {
               ok = false;
               break;
             }
             const uint32_t dcol = tbase + COL_S + sb * 128;
             for (int c = 0; c < DC; ++c, ++kc) {
-              if (pass == 0 && kt == 0 && !wait(&q_full[c], n & 1)) {
+              if (pass == 0 && kt == 0 && !wwait(&q_full[c], n & 1)) {
                 ok = false;
                 break;
               }
               if constexpr (PACKED) {
                 for (int x = 0; x < 2; ++x) {
                   const int kb = 2 * kc + x, slot = kb % (2 * KS);
-                  if (!wait(&k_full[slot], (kb / (2 * KS)) & 1)) {
+                  if (!wwait(&k_full[slot], (kb / (2 * KS)) & 1)) {
                     ok = false;
                     break;
                   }
                   tc_fence_after();
                   const uint64_t qd = qdesc0 + (uint64_t)((2 * c + x) * (BOX >> 4));
                   const uint64_t kd = kdesc0 + (uint64_t)(slot * (BOX >> 4));
+                  if (leader) {
 #pragma unroll
-                  for (int kk = 0; kk < 4; ++kk)
-                    mma_bf16_ss(dcol, qd + kk * 2, kd + kk * 2, IDESC_S, (c > 0 || x > 0 || kk > 0) ? 1u : 0u);
-                  tc_commit(&k_empty[slot]);
+                    for (int kk = 0; kk < 4; ++kk)
+                      mma_bf16_ss(dcol, qd + kk * 2, kd + kk * 2, IDESC_S, (c > 0 || x > 0 || kk > 0) ? 1u : 0u);
+                    tc_commit(&k_empty[slot]);
+                  }
                 }
                 if (!ok) break;
               } else {
                 const int slot = kc % KS;
-                if (!wait(&k_full[slot], (kc / KS) & 1)) {
+                if (!wwait(&k_full[slot], (kc / KS) & 1)) {
                   ok = false;
                   break;
                 }
                 tc_fence_after();
                 const uint64_t qd = qdesc0 + (uint64_t)(c * (CHUNK >> 4));
                 const uint64_t kd = kdesc0 + (uint64_t)(slot * (CHUNK >> 4));
+                if (leader) {
 #pragma unroll
-                for (int kk = 0; kk < 8; ++kk) {
-                  const uint64_t off = (uint64_t)((((kk >> 2) * BOX + (kk & 3) * 32) >> 4));
-                  mma_bf16_ss(dcol, qd + off, kd + off, IDESC_S, (c > 0 || kk > 0) ? 1u : 0u);
+                  for (int kk = 0; kk < 8; ++kk) {
+                    const uint64_t off = (uint64_t)((((kk >> 2) * BOX + (kk & 3) * 32) >> 4));
+                    mma_bf16_ss(dcol, qd + off, kd + off, IDESC_S, (c > 0 || kk > 0) ? 1u : 0u);
+                  }
+                  tc_commit(&k_empty[slot]);
                 }
-                tc_commit(&k_empty[slot]);
               }
-              if (pass == PASSES - 1 && kt == u.kt - 1) tc_commit(&q_empty[c]);  // the unit's last read of query chunk c
+              if (leader && pass == PASSES - 1 && kt == u.kt - 1) tc_commit(&q_empty[c]);  // the unit's last read of query chunk c
             }
             if (!ok) break;
-            tc_commit(&s_full[sb]);
+            if (leader) tc_commit(&s_full[sb]);
+            __syncwarp();
           }
         }
-        put(n);
+        if (leader) put(n);
       }
       if (!ok) abort_flag = 1;
     }
-    __syncwarp();
   } else if (warp == W_MMA_PV) {
     // ------------------------------------------------------------------ O[:, 64 sc ..] += P(t) V(t)[:, sc]
-    if (lane == 0) {
+    {
+      const bool leader = elect_one();
       const uint64_t vdesc0 = smem_desc(smem_addr(smem + V_OFF), BOX, 1024, kLayoutSw128);
       const uint64_t vdesc32 = smem_desc(smem_addr(smem + V_OFF), VK * 128, 1024, kLayoutSw128);
       int tile = 0, vc = 0, item = 0;
       bool ok = true;
       Unit u;
-      for (int n = 0; get(n, u) && ok && !abort_flag; ++n) {
+      for (int n = 0; wget(n, u) && ok; ++n) {
         for (int pass = 0; pass < PASSES && ok; ++pass, ++item) {
           for (int kt = 0; kt < u.kt && ok; ++kt, ++tile) {
             const int pb = tile % NSB, pu = tile / NSB;
-            if (kt == 0 && item >= 1 && !wait(&o_free, (item - 1) & 1)) {
+            if (kt == 0 && item >= 1 && !wwait(&o_free, (item - 1) & 1)) {
               ok = false;
               break;
             }
@@ -392,47 +402,53 @@ __global__ void __launch_bounds__(THREADS, 1)
             if constexpr (PACKED) {
               for (int sc = 0; sc < BN / VK; ++sc, ++vc) {
                 const int slot = vc % VS, x = sc * VK / KW;
-                if (sc * VK % KW == 0) ok = wait(&p_full[x][pb], pu & 1);
-                ok = ok && wait(&v_full[slot], (vc / VS) & 1);
+                if (sc * VK % KW == 0) ok = wwait(&p_full[x][pb], pu & 1);
+                ok = ok && wwait(&v_full[slot], (vc / VS) & 1);
                 if (!ok) break;
                 tc_fence_after();
                 const uint64_t vd = vdesc32 + (uint64_t)(slot * (BOX >> 4));
+                if (leader) {
 #pragma unroll
-                for (int kk = 0; kk < VK / 16; ++kk)
-                  mma_bf16_ts(tbase + COL_O, pcol + x * KW + (sc * VK % KW / 16 + kk) * 8, vd + (uint64_t)(kk * 128), IDESC_O256,
-                              (kt == 0 && sc == 0 && kk == 0) ? 0u : 1u);
-                tc_commit(&v_empty[slot]);
+                  for (int kk = 0; kk < VK / 16; ++kk)
+                    mma_bf16_ts(tbase + COL_O, pcol + x * KW + (sc * VK % KW / 16 + kk) * 8, vd + (uint64_t)(kk * 128), IDESC_O256,
+                                (kt == 0 && sc == 0 && kk == 0) ? 0u : 1u);
+                  tc_commit(&v_empty[slot]);
+                }
               }
               if (!ok) break;
-              tc_commit(&pv_done[pb]);
+              if (leader) tc_commit(&pv_done[pb]);
+              __syncwarp();
             } else {
-              for (int x = 0; x < NWG && ok; ++x) ok = wait(&p_full[x][pb], pu & 1);
+              for (int x = 0; x < NWG && ok; ++x) ok = wwait(&p_full[x][pb], pu & 1);
               if (!ok) break;
               tc_fence_after();
               for (int sc = 0; sc < NSUB; ++sc, ++vc) {
                 const int slot = vc % VS;
-                if (!wait(&v_full[slot], (vc / VS) & 1)) {
+                if (!wwait(&v_full[slot], (vc / VS) & 1)) {
                   ok = false;
                   break;
                 }
                 tc_fence_after();
                 const uint64_t vd = vdesc0 + (uint64_t)(slot * (BOX >> 4));
+                if (leader) {
 #pragma unroll
-                for (int x = 0; x < NWG; ++x)
+                  for (int x = 0; x < NWG; ++x)
 #pragma unroll
-                  for (int kk = 0; kk < KW / 16; ++kk)
-                    mma_bf16_ts(tbase + COL_O + sc * 64, pcol + x * KW + kk * 8,
-                                vd + (uint64_t)((KW / 16 * x + kk) * 128), IDESC_O,
-                                (kt == 0 && x == 0 && kk == 0) ? 0u : 1u);
-                tc_commit(&v_empty[slot]);
+                    for (int kk = 0; kk < KW / 16; ++kk)
+                      mma_bf16_ts(tbase + COL_O + sc * 64, pcol + x * KW + kk * 8,
+                                  vd + (uint64_t)((KW / 16 * x + kk) * 128), IDESC_O,
+                                  (kt == 0 && x == 0 && kk == 0) ? 0u : 1u);
+                  tc_commit(&v_empty[slot]);
+                }
               }
               if (!ok) break;
-              tc_commit(&pv_done[pb]);
+              if (leader) tc_commit(&pv_done[pb]);
+              __syncwarp();
             }
           }
-          if (ok) tc_commit(&o_ready);
+          if (ok && leader) tc_commit(&o_ready);
         }
-        put(n);
+        if (leader) put(n);
       }
       if (!ok) abort_flag = 1;
     }
@@ -691,7 +707,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   __syncthreads();
   if (abort_flag) {
     if (tid == 0) raise_status(p.status, kStatusTimeout);
-    if (tid == W_MMA * 32 || tid == W_MMA_PV * 32) {
+    if ((warp == W_MMA || warp == W_MMA_PV) && elect_one()) {
       tc_commit(&drain);
       mbar_wait(&drain, 0);
     }

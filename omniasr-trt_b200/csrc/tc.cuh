@@ -94,6 +94,17 @@ OMNI_DEV void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;
 // Generic-proxy shared-memory writes -> visible to the tensor core / TMA (async proxy).
 OMNI_DEV void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// One lane of the (converged) warp.
+OMNI_DEV bool elect_one() {
+  uint32_t e;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(e));
+  return e != 0;
+}
+
 // Warp-wide: allocate `ncols` TMEM columns (power of two >= 32); the base address goes to *dst.
 OMNI_DEV void tmem_alloc(uint32_t* dst, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(dst)),
