@@ -262,7 +262,7 @@ int omniasr_noalloc_reset(cudaStream_t stream);
  * shared by K and V, 16-byte aligned); a sequence's position j is offset j % page of the page its int32 table row names
  * at j / page. cache_type is the dtype itself, or OMNIASR_FP8: each vector x (one position of one kv head) is held as
  * e4m3 codes of x * 2^-e, e = the smallest integer with max|x| <= 448 * 2^e held to [-40, 40], and the byte e + 127 in
- * k_scale / v_scale [pages, kv_heads, page] (contiguous; NULL for the other types). Infinities, NaN and values past
+ * k_scale / v_scale [pages, kv_heads, page] (contiguous, 16-byte aligned; NULL for the other types). Infinities, NaN and values past
  * 448 * 2^40 are held as NaN and do not count for the scale. heads must be a multiple of kv_heads; query head h reads kv
  * head h / (heads / kv_heads). A page number outside the pool (or a length past the table) raises status bit 1, the
  * row's result is then unspecified, and nothing outside the tensors is touched. */

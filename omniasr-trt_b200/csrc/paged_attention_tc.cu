@@ -23,7 +23,11 @@
 // with m the running maximum of x + ev, so that w stays in e4m3's range whatever the scales are. m is kept 2^4 below the
 // maximum, w up to 2^8: the pieces' smallest step is then 2^-17 of a typical largest weight.
 //
-// What bounds it: HBM. bytes = keys * kv_heads * D * 2 * element (+ 2 scale bytes a key).
+// What bounds it: HBM. bytes = keys * kv_heads * D * 2 * element (+ 2 scale bytes a key). 48 rows of 4096 keys, 8 kv heads of
+// 128, 32 query heads: bf16 126.5 us (6369 GB/s), e4m3 72 us (5612 GB/s); 48 rows of 61 to 4093 in pages of 16, bf16, 72 us
+// (5670 GB/s: 9 us of entry, schedule and last join); with 16 query heads to a kv head e4m3 takes 4.3 TB/s (N = 64, whose
+// softmax spills at these registers). One row of a few hundred keys is latency: 12 us, of which a unit's ends are about 4000
+// clocks.
 
 #include <cudaTypedefs.h>
 #include <math.h>

@@ -190,7 +190,7 @@ constexpr int kReadThreads = 256;
 // One CTA: consecutive output tokens of one head (a page's positions of a head lie together), R rounds of TP tokens with
 // 16 bytes of the output per thread and round. Threads find the tokens' places first (the sequence by bisection in the
 // offsets, the page in its table row); then all rounds' loads are in flight together, and every store of a warp covers
-// whole lines: 195 MB of an fp8 context 44 us with 16-byte loads (two half-line stores each), token-major.
+// whole lines: 195 MB of an fp8 context 34 us (5741 GB/s); 44 us with 16-byte loads (two half-line stores each), token-major.
 template <typename T, int D, bool FP8, int R>
 __global__ void __launch_bounds__(kReadThreads) paged_read_kernel(const PagedReadArgs a) {
   constexpr int kOut = 16 / sizeof(T);       // elements per thread and round

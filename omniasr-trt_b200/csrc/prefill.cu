@@ -1,4 +1,5 @@
-// Causal prefill attention on the 5th-generation tensor cores (tcgen05 + TMEM), bf16, head_dim 128.
+// Causal prefill attention on the 5th-generation tensor cores (tcgen05 + TMEM), bf16: dense rows of head_dim 128, and packed
+// sequences with grouped heads of head_dim 64 and 128 (PackedSrc, prefill_common.cuh; packed.cu has the formula).
 //
 // out[b, w, h] = softmax(q[b, h, w] . k[b, h, :w+1]^T * scale) . v[b, h, :w+1]   for w < W
 // (F.scaled_dot_product_attention(q, k, v, is_causal=True) of the reference's prefill, decode.py:171; the
@@ -11,9 +12,11 @@
 //           the query tiles (2 slots) are loaded two units ahead by the first epilogue thread
 //   warp 13 MMA: S = Q K^T into TMEM (M=128 queries, N=128 keys), triple-buffered, so that S(t + 3) needs only
 //           O += P(t) V to have completed and the scores are ready before the softmax asks for them;
-//   warp 15 MMA: O += P V with P read from TMEM (the tcgen05 "A in TMEM" form). Two issuing threads, because one
+//   warp 15 MMA: O += P V with P read from TMEM (the tcgen05 "A in TMEM" form). Two issuing warps, because one
 //           thread issues a tcgen05.mma in about 55 clocks at best (measured), while a 128x128x16 MMA takes the
-//           tensor core about 64: a single issuer with its waits left the tensor core idle half the time.
+//           tensor core about 64: a single issuer with its waits left the tensor core idle half the time. Each runs
+//           converged with one elected lane issuing, its descriptors warp-uniform (12 packed prompts of 60 to 2047
+//           tokens 172 -> 166 us, dense 752 -> 770 TFLOP/s over a lone thread).
 //   warps 0-3 / 4-7  softmax warpgroups x = 0 / 1: thread t of warpgroup x owns query row t and the keys 64x .. 64x+63
 //           of every tile, so twice the softmax warps per SM each form half a tile's exponentials. The two keep one
 //           running max per row: each tile one barrier over both warpgroups asks whether any row's scores pass its
@@ -23,6 +26,10 @@
 //           and one probability pair in four is exponentiated on the FMA pipe (ex2_fma) instead of the
 //           special-function unit, which the exponentials otherwise saturate.
 //   warps 8-11 epilogue: O / (l_0 + l_1) of each unit as bf16 rows, while the softmax warpgroups go on with the next.
+// What bounds it: the softmax's chain. At head_dim 128 a tile is 1024 clocks of the tensor core and took 1930: 165 until the
+// wait sees S, 120 to read it, 300 for maxima and the barrier, 1000 for the exponentials (768 of them the special-function
+// unit's), the rest stores and hand-over. More of them on the FMA pipe (one pair in two: 172 -> 180 us) lose. Long calls
+// are held by the power limit besides.
 // TMEM: S0 [0,128) S1 [128,256) S2 [256,384) O [384,512); P of S buffer j, half x at 128j + 64x .. +32.
 
 #include <cudaTypedefs.h>

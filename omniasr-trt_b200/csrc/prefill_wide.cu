@@ -1,5 +1,6 @@
-// Causal prefill attention on the 5th-generation tensor cores (tcgen05 + TMEM), bf16, head_dim 512 -- the shipped
-// omniASR-LLM decoder's 8 heads x 512 (omniasr_trt/modeling.py:30-35).
+// Causal prefill attention on the 5th-generation tensor cores (tcgen05 + TMEM), bf16: dense rows of head_dim 512 -- the shipped
+// omniASR-LLM decoder's 8 heads x 512 (omniasr_trt/modeling.py:30-35) -- and packed sequences with grouped heads of head_dim
+// 256 (one pass) and 512 (two; PackedSrc, prefill_common.cuh; packed.cu has the formula).
 //
 // out[b, w, h] = softmax(q[b, h, w] . k[b, h, :w+1]^T * scale) . v[b, h, :w+1]   for w < W
 // (F.scaled_dot_product_attention(q, k, v, is_causal=True) of the reference's prefill, decode.py:171).
@@ -18,7 +19,8 @@
 // TMEM (512 columns): S double-buffered at [0, 128) and [128, 256), O of the pass's 256 dims at [256, 512); P (bf16
 // pairs) over S, read by the A-from-TMEM MMA.
 // Packed sequences use the same ring bytes in finer pieces: K in 64-dim boxes, so that more loads are in flight while one is
-// used, and V in slots of 32 keys x 256 dims, so that P V is 8 MMAs of N = 256 instead of 32 of N = 64.
+// used, and V in slots of 32 keys x 256 dims, so that P V is 8 MMAs of N = 256 instead of 32 of N = 64. Issuing from converged
+// warps (prefill.cu): 8 prompts of 1500, 16 heads of 256 on 4, 177 -> 157 us (939 TFLOP/s), of 512 454 -> 421 (702).
 // Roles (512 threads), as in prefill.cu: warp 12 K chunk loads, warp 14 V sub-chunk loads, warp 13 S MMAs, warp 15
 // P V MMAs, warps 0-3 / 4-7 softmax warpgroups (thread = query row, warpgroup x the keys 64x .. 64x + 63 of every
 // tile, one running max per row shared through a barrier per tile), warps 8-11 the epilogue (and the query loads,

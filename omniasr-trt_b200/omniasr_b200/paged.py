@@ -63,6 +63,16 @@ class PagedCache:
         self._free.extend(reversed(self._pages.pop(seq)))
         del self._length[seq]
 
+    def trim(self, seq: int, length: int) -> None:
+        """Keeps the sequence's first ``length`` positions (drops drafts that were not accepted) and gives back the pages past
+        them."""
+        if not 0 <= length <= self._length[seq]:
+            raise ValueError(f"trim: {length} of {self._length[seq]} positions")
+        keep = -(-length // self.page)
+        self._free.extend(reversed(self._pages[seq][keep:]))
+        del self._pages[seq][keep:]
+        self._length[seq] = length
+
     def length(self, seq: int) -> int:
         return self._length[seq]
 

@@ -143,6 +143,25 @@ def test_paged_cache_hands_out_pages():
     assert c.free_pages == 7
 
 
+def test_paged_cache_drops_drafts():
+    from omniasr_b200.paged import PagedCache
+
+    c = PagedCache(1, 5, 4, 1, 16, device="cpu")
+    a = c.add()
+    pages = c.extend([a], [7]).table[0].tolist()
+    c.extend([a], [6])  # to 13 positions: two more pages
+    assert c.free_pages == 1
+    c.trim(a, 8)  # the first 8 fill two pages
+    assert c.length(a) == 8 and c.free_pages == 3
+    step = c.extend([a], [1])
+    assert step.table[0, :2].tolist() == pages and step.pos.tolist() == [8] and step.lengths.tolist() == [9]
+    for n in (-1, 10):
+        with pytest.raises(ValueError, match="trim"):
+            c.trim(a, n)
+    c.trim(a, 0)
+    assert c.free_pages == 5 and c.extend([a], [1]).fresh
+
+
 def test_paged_cache_decode_wants_even_steps():
     from omniasr_b200.paged import PagedCache
 

@@ -474,6 +474,46 @@ def test_packed_hidden_values_stay_out(dim, dtype, bad):
     kernels.read_status()
 
 
+@pytest.mark.parametrize("heads,kv,dim,dtype,lens", [
+    (4, 2, 128, "bf16", [1, 130, 300]), (32, 4, 128, "bf16", [700, 600]), (32, 4, 64, "bf16", [1, 700, 600]), (4, 2, 256, "bf16", [1, 300]),
+    (4, 2, 512, "bf16", [1, 300]), (4, 2, 64, "f32", [1, 130]), (4, 2, 32, "bf16", [1, 130])])
+def test_packed_scores_of_minus_infinity(heads, kv, dim, dtype, lens):
+    """The first key of each sequence scores -inf: a query that sees it alone has no softmax (NaN), the others leave it out."""
+    g = torch.Generator().manual_seed(11)
+    dt, n = DT[dtype], sum(lens)
+    off = [sum(lens[:i]) for i in range(len(lens) + 1)]
+    q, k, v = (torch.randn(n, h, dim, generator=g).to(dt) for h in (heads, kv, kv))
+    q[:, :, 3] = 1.0
+    k[off[:-1], :, 3] = float("-inf")
+    want = pu.packed(q, k, v, off, off, dim**-0.5)
+    size = pu.packed(q, k, v.abs(), off, off, dim**-0.5)
+    got = kernels.packed_attention(q.to(DEV), k.to(DEV), v.to(DEV), torch.tensor(off, device=DEV)).cpu()
+    first = torch.zeros(n, dtype=torch.bool)
+    first[off[:-1]] = True
+    assert bool(torch.isnan(want[first]).all()) and bool(torch.isnan(got[first]).all())
+    check(got[~first], want[~first], size[~first], dt)
+
+
+@pytest.mark.parametrize("heads,kv,dim,page,dtype", [
+    (4, 2, 128, 16, "bf16"), (4, 4, 512, 64, "bf16"), (8, 1, 64, 16, "bf16"), (4, 1, 256, 128, "bf16"), (4, 2, 64, 16, "f32"), (4, 2, 32, 16, "bf16")])
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_paged_scores_of_minus_infinity(heads, kv, dim, page, dtype, tokens):
+    """As test_packed_scores_of_minus_infinity, over pages."""
+    g = torch.Generator().manual_seed(12)
+    dt, lens = DT[dtype], [1, 2, 300, 131]
+    table, pool = pu.table_for([n + tokens - 1 for n in lens], page, g)
+    k, v, _, _, _, _ = pu.cache(pool, kv, page, dim, "own", g, dt)
+    q = torch.randn(len(lens) * tokens, heads, dim, generator=g).to(dt)
+    q[:, :, 3] = 1.0
+    k[table[:, 0].long(), :, 0, 3] = float("-inf")
+    length = torch.tensor(lens)
+    want = pu.paged(q, k, v, table, length, dim**-0.5, tokens)
+    size = pu.paged(q, k, v.abs(), table, length, dim**-0.5, tokens)
+    got = kernels.paged_attention(q.to(DEV), k.to(DEV), v.to(DEV), table.to(DEV), length.to(DEV), dim**-0.5, tokens=tokens).cpu()
+    assert bool(torch.isnan(want[0]).all()) and bool(torch.isnan(got[0]).all())
+    check(got[1:], want[1:], size[1:], dt)
+
+
 def test_packed_bad_offsets_are_reported():
     q = torch.randn(10, 2, 128).to(torch.bfloat16).to(DEV)
     kernels.packed_attention(q, q, q, torch.tensor([0, 4, 10], device=DEV), torch.tensor([0, 4, 11], device=DEV))
