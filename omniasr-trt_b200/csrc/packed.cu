@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(kThreads) packed_kernel(const PackedArgs a) {
     for (int w = 8; w > 0; w >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], w);
     const int r = y + 16 * i;
     if (r < rows) {
-      const float inv = l[i] != 0.f ? 1.f / l[i] : 0.f;
+      const float inv = l[i] != 0.f ? 1.f / l[i] : (lim0 + r > 0 ? NAN : 0.f);  // (keys that all score -inf: no softmax)
       T* dst = reinterpret_cast<T*>(a.out) + ((q0 + r) * a.heads + h) * D;
 #pragma unroll
       for (int d = 0; d < DG; ++d)

@@ -66,6 +66,13 @@ struct Split {
   float* part_ml;            // ... [split][2]
 };
 
+// The result of query vector `row` where nothing was summed: zeros if it sees no key, else all its keys score -inf and it
+// has no softmax.
+OMNI_DEV float nothing(const int64_t* lengths, int tokens, int heads, int64_t row) {
+  const int64_t t = row / heads;
+  return lengths[t / tokens] + t % tokens > 0 ? NAN : 0.f;
+}
+
 // TQ: the queries' and output's type; TC: the cache's; NC: columns per unit.
 template <typename TQ, typename TC, int D, int NC>
 __global__ void __launch_bounds__(kThreads) split_kernel(const PagedAttnArgs a, const Split sp) {
@@ -237,7 +244,7 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const PagedAttnArgs a, 
       float acc = 0.f;
       for (int t = 0; t < TEAMS; ++t) acc = fmaf(s_o[t][d], ex2(s_m[t] - base), acc);
       if (sp.splits == 1) {
-        const float r = sum != 0.f ? acc / sum : 0.f;
+        const float r = sum != 0.f ? acc / sum : nothing(a.lengths, a.tokens, a.heads, qrow[c]);
         reinterpret_cast<TQ*>(a.out)[qrow[c] * D + d] = Elem<TQ>::from_float(r);
       } else {
         sp.part_o[(qrow[c] * sp.splits + split) * D + d] = acc;
@@ -250,7 +257,8 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const PagedAttnArgs a, 
 }
 
 template <typename TQ>
-__global__ void __launch_bounds__(kThreads) join_kernel(const Split sp, int dim, TQ* __restrict__ out) {
+__global__ void __launch_bounds__(kThreads) join_kernel(const Split sp, int dim, const int64_t* lengths, int tokens, int heads,
+                                                        TQ* __restrict__ out) {
   grid_launch_dependents();
   grid_dependency_wait();
   const int64_t row = blockIdx.x;
@@ -263,7 +271,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Split sp, int dim,
   for (int d = threadIdx.x; d < dim; d += kThreads) {
     float acc = 0.f;
     for (int s = 0; s < sp.splits; ++s) acc = fmaf(sp.part_o[(row * sp.splits + s) * dim + d], ex2(ml[s].x - base), acc);
-    out[row * dim + d] = Elem<TQ>::from_float(sum != 0.f ? acc / sum : 0.f);
+    out[row * dim + d] = Elem<TQ>::from_float(sum != 0.f ? acc / sum : nothing(lengths, tokens, heads, row));
   }
 }
 
@@ -333,9 +341,9 @@ cudaError_t launch_paged_attention(int dtype, const PagedAttnArgs& a, cudaStream
   if (e != cudaSuccess || sp.splits == 1) return e;
   if (dtype == kBF16)
     return launch_dependent(paged::join_kernel<__nv_bfloat16>, dim3((unsigned)qrows), dim3(paged::kThreads), 0, stream, sp,
-                            a.c.dim, reinterpret_cast<__nv_bfloat16*>(a.out));
+                            a.c.dim, a.lengths, a.tokens, a.heads, reinterpret_cast<__nv_bfloat16*>(a.out));
   return launch_dependent(paged::join_kernel<float>, dim3((unsigned)qrows), dim3(paged::kThreads), 0, stream, sp, a.c.dim,
-                          reinterpret_cast<float*>(a.out));
+                          a.lengths, a.tokens, a.heads, reinterpret_cast<float*>(a.out));
 }
 
 }  // namespace omni

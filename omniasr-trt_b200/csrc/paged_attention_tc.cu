@@ -335,7 +335,7 @@ __device__ __noinline__ void exact_column(const __nv_bfloat16* q, const PageCach
     for (int i = 0; i < NV; ++i) o[i] = fmaf(pr * vs, value(c.v, at + i * 32 + lane), o[i] * f);
     if (l != l) break;  // a NaN score: the whole row is NaN
   }
-  const float inv = l != 0.f ? 1.f / l : 0.f;
+  const float inv = l != 0.f ? 1.f / l : (lim > 0 ? NAN : 0.f);
 #pragma unroll
   for (int i = 0; i < NV; ++i) out[i * 32 + lane] = __float2bfloat16_rn(l != l ? l : o[i] * inv);
 }
@@ -1042,7 +1042,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 0; j < NQT; ++j) {
           if (j < ncol) {
             const int64_t row = row0 + tt * p.heads + g;
-            const float r = o[j] * (sum[j] != 0.f ? __fdividef(1.f, sum[j]) : 0.f);
+            // Nothing summed: a query that sees no key gets zeros, one whose keys all score -inf has no softmax.
+            const float r = sum[j] != 0.f ? o[j] * __fdividef(1.f, sum[j]) : (len[s.b] + tt > 0 ? NAN : 0.f);
             if (!(fabsf(r) <= 3.3e38f) && (CD == 128 || d < CD)) bad |= 1u << j;
             if (CD == 128 || d < CD) p.out[row * DIM + c * CD + d] = __float2bfloat16_rn(r);
           }

@@ -613,6 +613,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         live = pos < u.npos;
         // A row that sees no key: zeros (its masked probabilities are not exactly zero: ex2_fma's smallest is 2^-126).
         if (u.lim0 + pos <= 0) inv = 0.f;
+        else if (m == -INFINITY) inv = NAN;  // every key it sees scores -inf: no softmax
         dst = p.out + ((int64_t)(u.q0 + pos) * src.heads + head) * D;
       } else {
         dst = p.out + (int64_t)u.b * p.out_sb + (int64_t)q * p.out_sw + (int64_t)u.h * p.out_sh;
@@ -878,7 +879,7 @@ __global__ void __launch_bounds__(128) packed_join_kernel(const __grid_constant_
 #pragma unroll
     for (int i = 0; i < 32; ++i) o[i] = ws != 0.f ? fmaf(ws, v[i], o[i]) : o[i];
   }
-  const float inv = l != 0.f ? 1.f / l : 0.f;
+  const float inv = l != 0.f ? 1.f / l : (u.lim0 + pos > 0 ? NAN : 0.f);  // (keys that all score -inf: no softmax)
   const int64_t at = ((int64_t)(u.q0 + pos) * src.heads + head) * D;
   float odd = l * 0.f;
   if (live) {

@@ -422,7 +422,7 @@ __device__ __noinline__ void exact_row(const __nv_bfloat16* q, const __nv_bfloat
     }
     if (l != l) break;  // a NaN score: the whole row is NaN
   }
-  const float inv = l != 0.f ? 1.f / l : 0.f;
+  const float inv = l != 0.f ? 1.f / l : (lim > 0 ? NAN : 0.f);  // every key it sees scores -inf: no softmax
 #pragma unroll
   for (int i = 0; i < N; ++i) out[i * 32 + lane] = __float2bfloat16_rn(l != l ? l : o[i] * inv);
 }

@@ -639,7 +639,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         const float m = PACKED ? ctl.msum[row] : 0.f;
         mbar_arrive(&l_free);
         // A packed row that sees no key: zeros (its masked probabilities are not exactly zero: ex2_fma's smallest is 2^-126).
-        const float inv = l > 0.f && !(PACKED && u.lim0 + pos <= 0) ? 1.f / l : 0.f;
+        float inv = l > 0.f && !(PACKED && u.lim0 + pos <= 0) ? 1.f / l : 0.f;
+        if (PACKED && m == -INFINITY && u.lim0 + pos > 0) inv = NAN;  // every key it sees scores -inf: no softmax
         __nv_bfloat16* dst = row_out + pass * DH;
         if constexpr (PACKED) {
           if (u.part >= 0) {  // a part: fp32, a column of rows at a time
