@@ -6,10 +6,11 @@
 // where that is not positive. q [Tq, H, D], k and v [Tk, Hkv, D], head h reads kv head h / (H / Hkv).
 //
 // One CTA: BM queries of one head; K and V tiles of BN keys go through shared memory as fp32; S = Q K^T and O += P V
-// in registers (256 threads as 16 x 16: thread (y, x) holds rows y + 16 i, keys x + 16 j and groups of four dims, so a row's
+// in registers (256 threads as 16 x 16, for 16 queries 128 as 8 x 16: thread (y, x) holds rows y + 16 i, keys x + 16 j and groups of four dims, so a row's
 // softmax statistics are a shuffle over half a warp). FMA-bound; fp32 throughout, as an fp32 model needs. BM is 64 (32 for
 // head dims of 256 and more, whose tiles fill the shared memory), or 16 while larger tiles leave SMs idle: three prompts of
-// 17 to 131 tokens, 8 heads of 64, take 12 us, 20 with 64.
+// 17 to 131 tokens, 8 heads of 64, take 11 us: 22 with 256 threads of one row each (a K or V value from shared memory then
+// serves one product, not two) and no copy of the next tile in flight.
 
 #include <math.h>
 
@@ -23,16 +24,19 @@
 namespace omni {
 namespace packed {
 
-constexpr int kThreads = 256;
-
-template <int D, int BM_>
+template <typename T, int D, int BM_>
 struct Shape {
   static constexpr int BM = BM_;
+  static constexpr int THREADS = BM == 16 ? 128 : 256, YR = THREADS / 16;
   static constexpr int BN = D <= 128 ? 64 : 32;
   static constexpr int VW = D >= 64 ? 4 : D / 16;  // consecutive head dims of O per thread
   static constexpr int LD = D + 4;  // row stride in shared memory (floats): 16-byte aligned, rows on different banks
   static constexpr int LP = BN + 4;
-  static constexpr int BYTES = (BM * LD + 2 * BN * LD + BM * LP) * 4;
+  static constexpr int KV = 2 * BN * LD;  // floats of a K and a V tile
+  // fp32 tiles are copied asynchronously, for small tiles (which wait for nothing else) the next one during this one's work.
+  static constexpr bool ASYNC = sizeof(T) == 4;
+  static constexpr int STAGES = ASYNC && BM == 16 && (BM * (LD + LP) + 2 * KV) * 4 <= 232448 - 1024 ? 2 : 1;
+  static constexpr int BYTES = (BM * (LD + LP) + STAGES * KV) * 4;
 };
 
 // Tile `slot` of the packed queries -> sequence and first query: the sequences' tile counts, summed 32 at a time by one
@@ -76,9 +80,19 @@ OMNI_DEV void load4<__nv_bfloat16>(const __nv_bfloat16* p, float* f) {
 
 // ROWS rows of 4-element groups from global (row stride st) into shared memory, all loads in flight together; rows at or
 // past `valid` are zeros.
-template <typename T, int D, int LD, int ROWS>
+template <typename T, int D, int LD, int ROWS, int kThreads>
 OMNI_DEV void load_tile(float* dst, const T* src, int64_t st, int valid) {
   constexpr int TOTAL = ROWS * (D / 4), N = (TOTAL + kThreads - 1) / kThreads, B = N < 8 ? N : 8;
+  if constexpr (sizeof(T) == 4) {  // asynchronously: the caller waits (nothing is read for the rows of zeros)
+#pragma unroll 4
+    for (int i = threadIdx.x; i < TOTAL; i += kThreads) {
+      const int r = i / (D / 4), c = (i - r * (D / 4)) * 4;
+      const int size = r < valid ? 16 : 0;
+      const T* from = size ? src + (int64_t)r * st + c : src;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst + r * LD + c)), "l"(from), "r"(size) : "memory");
+    }
+    return;
+  }
 #pragma unroll 1
   for (int i0 = 0; i0 < N; i0 += B) {
     float f[B][4];
@@ -99,15 +113,14 @@ OMNI_DEV void load_tile(float* dst, const T* src, int64_t st, int valid) {
 }
 
 template <typename T, int D, int BM_>
-__global__ void __launch_bounds__(kThreads) packed_kernel(const PackedArgs a) {
-  using S = Shape<D, BM_>;
-  constexpr int BM = S::BM, BN = S::BN, LD = S::LD, LP = S::LP, VW = S::VW;
-  constexpr int MR = BM / 16, NR = BN / 16, DR = D / 16, DG = DR / VW;
+__global__ void __launch_bounds__(Shape<T, D, BM_>::THREADS) packed_kernel(const PackedArgs a) {
+  using S = Shape<T, D, BM_>;
+  constexpr int BM = S::BM, BN = S::BN, LD = S::LD, LP = S::LP, VW = S::VW, YR = S::YR;
+  constexpr int MR = BM / YR, NR = BN / 16, DR = D / 16, DG = DR / VW;
   extern __shared__ __align__(16) float sm[];
   float* qs = sm;
-  float* ks = qs + BM * LD;
-  float* vs = ks + BN * LD;
-  float* ps = vs + BN * LD;
+  float* ps = qs + BM * LD;
+  float* ring = ps + BM * LP;  // [stage][K, V]
   __shared__ int s_seq, s_tile;
   grid_launch_dependents();
   grid_dependency_wait();
@@ -134,10 +147,15 @@ __global__ void __launch_bounds__(kThreads) packed_kernel(const PackedArgs a) {
   const int64_t lim0 = (q0 - qa) + 1 + (kb - ka) - (qb - qa);
   const int64_t keys = max((int64_t)0, lim0 + rows - 1);
   const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
-  load_tile<T, D, LD, BM>(qs, reinterpret_cast<const T*>(a.q) + q0 * a.q_st + (int64_t)h * a.q_sh, a.q_st, rows);
+  load_tile<T, D, LD, BM, S::THREADS>(qs, reinterpret_cast<const T*>(a.q) + q0 * a.q_st + (int64_t)h * a.q_sh, a.q_st, rows);
   const T* kg = reinterpret_cast<const T*>(a.k) + ka * a.k_st + (int64_t)kvh * a.k_sh;
   const T* vg = reinterpret_cast<const T*>(a.v) + ka * a.v_st + (int64_t)kvh * a.v_sh;
   const float qscale = a.scale * kLog2e;
+  auto fetch = [&](float* to, int64_t j0) {  // the K and V tile of keys j0 ..
+    const int valid = (int)min((int64_t)BN, keys - j0);
+    load_tile<T, D, LD, BN, S::THREADS>(to, kg + j0 * a.k_st, a.k_st, valid);
+    load_tile<T, D, LD, BN, S::THREADS>(to + BN * LD, vg + j0 * a.v_st, a.v_st, valid);
+  };
   float m[MR], l[MR], o[MR][DR];
 #pragma unroll
   for (int i = 0; i < MR; ++i) {
@@ -148,9 +166,18 @@ __global__ void __launch_bounds__(kThreads) packed_kernel(const PackedArgs a) {
   }
   for (int64_t j0 = 0; j0 < keys; j0 += BN) {
     const int valid = (int)min((int64_t)BN, keys - j0);
+    float* ks = ring + (S::STAGES == 2 && (j0 / BN & 1) ? S::KV : 0);
+    const float* vs = ks + BN * LD;
     __syncthreads();  // the tile before is used up
-    load_tile<T, D, LD, BN>(ks, kg + j0 * a.k_st, a.k_st, valid);
-    load_tile<T, D, LD, BN>(vs, vg + j0 * a.v_st, a.v_st, valid);
+    if (S::STAGES == 1 || j0 == 0) {
+      fetch(ks, j0);
+      if (S::ASYNC) asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    if (S::STAGES == 2) {
+      if (j0 + BN < keys) fetch(ring + (j0 / BN & 1 ? 0 : S::KV), j0 + BN);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    if (S::ASYNC) asm volatile("cp.async.wait_group %0;" ::"n"(S::STAGES - 1) : "memory");
     __syncthreads();
     float s[MR][NR];
 #pragma unroll
@@ -161,7 +188,7 @@ __global__ void __launch_bounds__(kThreads) packed_kernel(const PackedArgs a) {
     for (int d = 0; d < D; d += 4) {
       float4 qv[MR], kv[NR];
 #pragma unroll
-      for (int i = 0; i < MR; ++i) qv[i] = *reinterpret_cast<const float4*>(qs + (y + 16 * i) * LD + d);
+      for (int i = 0; i < MR; ++i) qv[i] = *reinterpret_cast<const float4*>(qs + (y + YR * i) * LD + d);
 #pragma unroll
       for (int j = 0; j < NR; ++j) kv[j] = *reinterpret_cast<const float4*>(ks + (x + 16 * j) * LD + d);
 #pragma unroll
@@ -173,7 +200,7 @@ __global__ void __launch_bounds__(kThreads) packed_kernel(const PackedArgs a) {
     const bool edge = j0 + BN > lim0;  // some row does not see all of the tile
 #pragma unroll
     for (int i = 0; i < MR; ++i) {
-      const int64_t lim = lim0 + y + 16 * i - j0;
+      const int64_t lim = lim0 + y + YR * i - j0;
       float top = -INFINITY;
 #pragma unroll
       for (int j = 0; j < NR; ++j) {
@@ -191,7 +218,7 @@ __global__ void __launch_bounds__(kThreads) packed_kernel(const PackedArgs a) {
       for (int j = 0; j < NR; ++j) {
         const float p = ex2(s[i][j] - base);  // a NaN score gives NaN: the row is NaN, as the formula is
         sum += p;
-        ps[(y + 16 * i) * LP + x + 16 * j] = p;
+        ps[(y + YR * i) * LP + x + 16 * j] = p;
       }
       l[i] = fmaf(l[i], f, sum);
 #pragma unroll
@@ -205,7 +232,7 @@ __global__ void __launch_bounds__(kThreads) packed_kernel(const PackedArgs a) {
         float p[MR][4];
 #pragma unroll
         for (int i = 0; i < MR; ++i) {
-          const float4 f = *reinterpret_cast<const float4*>(ps + (y + 16 * i) * LP + k);
+          const float4 f = *reinterpret_cast<const float4*>(ps + (y + YR * i) * LP + k);
           p[i][0] = f.x, p[i][1] = f.y, p[i][2] = f.z, p[i][3] = f.w;
         }
 #pragma unroll
@@ -226,7 +253,7 @@ __global__ void __launch_bounds__(kThreads) packed_kernel(const PackedArgs a) {
 #pragma unroll
             for (int i = 0; i < MR; ++i) {
               // A key past the row's does not enter, whatever its value holds.
-              if (!decltype(masked)::value || j0 + k + c < lim0 + y + 16 * i) {
+              if (!decltype(masked)::value || j0 + k + c < lim0 + y + YR * i) {
 #pragma unroll
                 for (int e = 0; e < VW; ++e) o[i][d * VW + e] = fmaf(p[i][c], v[e], o[i][d * VW + e]);
               }
@@ -238,11 +265,12 @@ __global__ void __launch_bounds__(kThreads) packed_kernel(const PackedArgs a) {
     if (edge) values(std::true_type{});
     else values(std::false_type{});
   }
+  if (S::ASYNC) asm volatile("cp.async.wait_all;" ::: "memory");  // (a sequence without keys: the queries')
 #pragma unroll
   for (int i = 0; i < MR; ++i) {
 #pragma unroll
     for (int w = 8; w > 0; w >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], w);
-    const int r = y + 16 * i;
+    const int r = y + YR * i;
     if (r < rows) {
       const float inv = l[i] != 0.f ? 1.f / l[i] : (lim0 + r > 0 ? NAN : 0.f);  // (keys that all score -inf: no softmax)
       T* dst = reinterpret_cast<T*>(a.out) + ((q0 + r) * a.heads + h) * D;
@@ -256,7 +284,7 @@ __global__ void __launch_bounds__(kThreads) packed_kernel(const PackedArgs a) {
 
 template <typename T, int D, int BM>
 cudaError_t launch_t(const PackedArgs& a, cudaStream_t s) {
-  using S = Shape<D, BM>;
+  using S = Shape<T, D, BM>;
   static bool configured = false;
   if (!configured) {
     cudaError_t e = cudaFuncSetAttribute(packed_kernel<T, D, BM>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES);
@@ -265,7 +293,7 @@ cudaError_t launch_t(const PackedArgs& a, cudaStream_t s) {
   }
   // At most this many tiles: a sequence's last tile may be partly filled.
   const int64_t tiles = a.q_tokens / BM + a.seqs;
-  return launch_dependent(packed_kernel<T, D, BM>, dim3((unsigned)tiles, (unsigned)a.heads), dim3(kThreads), (size_t)S::BYTES, s, a);
+  return launch_dependent(packed_kernel<T, D, BM>, dim3((unsigned)tiles, (unsigned)a.heads), dim3(S::THREADS), (size_t)S::BYTES, s, a);
 }
 
 template <typename T, int D>
