@@ -6,11 +6,12 @@
 // where that is not positive. q [Tq, H, D], k and v [Tk, Hkv, D], head h reads kv head h / (H / Hkv).
 //
 // One CTA: BM queries of one head; K and V tiles of BN keys go through shared memory as fp32; S = Q K^T and O += P V
-// in registers (256 threads as 16 x 16, for 16 queries 128 as 8 x 16: thread (y, x) holds rows y + 16 i, keys x + 16 j and groups of four dims, so a row's
-// softmax statistics are a shuffle over half a warp). FMA-bound; fp32 throughout, as an fp32 model needs. BM is 64 (32 for
-// head dims of 256 and more, whose tiles fill the shared memory), or 16 while larger tiles leave SMs idle: three prompts of
-// 17 to 131 tokens, 8 heads of 64, take 11 us: 22 with 256 threads of one row each (a K or V value from shared memory then
-// serves one product, not two) and no copy of the next tile in flight.
+// in registers (16 lanes across keys and head dims: thread (y, x) holds rows y + YR i, keys x + 16 j and groups of four dims,
+// so a row's softmax statistics are a shuffle over half a warp). Bound by shared-memory reads and FMA; fp32 throughout, as an
+// fp32 model needs. BM is 64 (32 for head dims of 256 and more, whose tiles fill the shared memory), or 16, of 128 threads,
+// while larger tiles leave SMs idle: three prompts of 17 to 131 tokens, 8 heads of 64, take 11 us; 22
+// with 256 threads of one row each (a value read from shared memory then serves one product, not two) and no copy of the
+// next tile in flight.
 
 #include <math.h>
 
