@@ -113,8 +113,24 @@ OMNI_DEV void load_tile(float* dst, const T* src, int64_t st, int valid) {
   }
 }
 
+// Parts of a query tile's keys for the calls of few tiles over many keys (part z of them: blockIdx.z); each leaves its rows'
+// maxima, sums and unnormalised outputs, and join_kernel adds them up in the order of the keys.
+struct Parts {
+  int n;
+  float* ml;  // [row * heads + head][part][2]
+  float* o;   // ... [D]
+};
+constexpr int kMostParts = 32;
+
+// At most this many parts: two CTAs per SM.
+int most_parts(int dtype, int64_t q_tokens, int heads, int kv_heads, int dim) {
+  if (dtype == kBF16 && dim >= 64 && heads / kv_heads <= 128) return 1;  // the tensor-core kernels' calls
+  const int64_t units = heads * ((q_tokens + 15) / 16);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(kMostParts, units > 0 ? 2 * device_sm_count() / units : 1));
+}
+
 template <typename T, int D, int BM_>
-__global__ void __launch_bounds__(Shape<T, D, BM_>::THREADS) packed_kernel(const PackedArgs a) {
+__global__ void __launch_bounds__(Shape<T, D, BM_>::THREADS) packed_kernel(const PackedArgs a, const Parts parts) {
   using S = Shape<T, D, BM_>;
   constexpr int BM = S::BM, BN = S::BN, LD = S::LD, LP = S::LP, VW = S::VW, YR = S::YR;
   constexpr int MR = BM / YR, NR = BN / 16, DR = D / 16, DG = DR / VW;
@@ -146,7 +162,12 @@ __global__ void __launch_bounds__(Shape<T, D, BM_>::THREADS) packed_kernel(const
   const int rows = (int)min((int64_t)BM, qb - q0);
   // Row r of the tile sees keys [0, lim0 + r) of the sequence.
   const int64_t lim0 = (q0 - qa) + 1 + (kb - ka) - (qb - qa);
-  const int64_t keys = max((int64_t)0, lim0 + rows - 1);
+  int64_t keys = max((int64_t)0, lim0 + rows - 1), first = 0;
+  if (BM == 16 && parts.n > 1) {
+    const int64_t each = ((keys + BN - 1) / BN + parts.n - 1) / parts.n * BN;
+    first = min(keys, blockIdx.z * each);
+    keys = min(keys, first + each);
+  }
   const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
   load_tile<T, D, LD, BM, S::THREADS>(qs, reinterpret_cast<const T*>(a.q) + q0 * a.q_st + (int64_t)h * a.q_sh, a.q_st, rows);
   const T* kg = reinterpret_cast<const T*>(a.k) + ka * a.k_st + (int64_t)kvh * a.k_sh;
@@ -165,12 +186,12 @@ __global__ void __launch_bounds__(Shape<T, D, BM_>::THREADS) packed_kernel(const
 #pragma unroll
     for (int d = 0; d < DR; ++d) o[i][d] = 0.f;
   }
-  for (int64_t j0 = 0; j0 < keys; j0 += BN) {
+  for (int64_t j0 = first; j0 < keys; j0 += BN) {
     const int valid = (int)min((int64_t)BN, keys - j0);
     float* ks = ring + (S::STAGES == 2 && (j0 / BN & 1) ? S::KV : 0);
     const float* vs = ks + BN * LD;
     __syncthreads();  // the tile before is used up
-    if (S::STAGES == 1 || j0 == 0) {
+    if (S::STAGES == 1 || j0 == first) {
       fetch(ks, j0);
       if (S::ASYNC) asm volatile("cp.async.commit_group;" ::: "memory");
     }
@@ -272,6 +293,17 @@ __global__ void __launch_bounds__(Shape<T, D, BM_>::THREADS) packed_kernel(const
 #pragma unroll
     for (int w = 8; w > 0; w >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], w);
     const int r = y + YR * i;
+    if (BM == 16 && parts.n > 1) {
+      if (r < rows) {
+        const int64_t at = ((q0 + r) * a.heads + h) * parts.n + blockIdx.z;
+        if (x == 0) reinterpret_cast<float2*>(parts.ml)[at] = make_float2(m[i], l[i]);
+#pragma unroll
+        for (int d = 0; d < DG; ++d)
+#pragma unroll
+          for (int e = 0; e < VW; ++e) parts.o[at * D + (x + 16 * d) * VW + e] = o[i][d * VW + e];
+      }
+      continue;
+    }
     if (r < rows) {
       const float inv = l[i] != 0.f ? 1.f / l[i] : (lim0 + r > 0 ? NAN : 0.f);  // (keys that all score -inf: no softmax)
       T* dst = reinterpret_cast<T*>(a.out) + ((q0 + r) * a.heads + h) * D;
@@ -283,8 +315,55 @@ __global__ void __launch_bounds__(Shape<T, D, BM_>::THREADS) packed_kernel(const
   }
 }
 
+// One warp per query and head: o = sum 2^(m_p - m) o_p / sum 2^(m_p - m) l_p over its parts. Rows of no sequence (or of one
+// whose offsets are bad) have no parts and are not written.
+template <typename T>
+__global__ void __launch_bounds__(256) join_kernel(const PackedArgs a, const Parts parts) {
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t at = blockIdx.x * 8ll + (threadIdx.x >> 5), row = at / a.heads;
+  if (row >= a.q_tokens) return;
+  int64_t lim = -1;  // keys the query sees
+  bool mine = false;
+  for (int s0 = 0; s0 < a.seqs && !mine; s0 += 32) {
+    const int s = s0 + lane;
+    bool hit = false;
+    if (s < a.seqs) {
+      const int64_t qa = a.q_offsets[s], qb = a.q_offsets[s + 1], ka = a.k_offsets[s], kb = a.k_offsets[s + 1];
+      hit = qa <= row && row < qb && qa >= 0 && qb <= a.q_tokens && ka >= 0 && kb <= a.k_tokens && kb >= ka;
+      if (hit) lim = row - qa + 1 + (kb - ka) - (qb - qa);
+    }
+    const unsigned who = __ballot_sync(0xffffffffu, hit);
+    if (who) {
+      mine = true;
+      lim = __shfl_sync(0xffffffffu, lim, __ffs(who) - 1);
+    }
+  }
+  if (!mine) return;
+  const float2* ml = reinterpret_cast<const float2*>(parts.ml) + at * parts.n;
+  const float2 own = lane < parts.n ? ml[lane] : make_float2(-INFINITY, 0.f);  // (at most 32 parts)
+  float top = own.x;
+#pragma unroll
+  for (int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+  const float weight = ex2(own.x - (top == -INFINITY ? 0.f : top));
+  float sum = weight * own.y;
+#pragma unroll
+  for (int w = 16; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+  const float inv = sum != 0.f ? 1.f / sum : (lim > 0 ? NAN : 0.f);
+  for (int d0 = 0; d0 < a.dim; d0 += 32) {
+    const int d = d0 + lane;
+    float o = 0.f;
+    for (int p = 0; p < parts.n; ++p) {
+      const float w = __shfl_sync(0xffffffffu, weight, p);
+      if (d < a.dim) o = fmaf(w, parts.o[(at * parts.n + p) * a.dim + d], o);
+    }
+    if (d < a.dim) reinterpret_cast<T*>(a.out)[at * a.dim + d] = Elem<T>::from_float(o * inv);
+  }
+}
+
 template <typename T, int D, int BM>
-cudaError_t launch_t(const PackedArgs& a, cudaStream_t s) {
+cudaError_t launch_t(const PackedArgs& a, const Parts& parts, cudaStream_t s) {
   using S = Shape<T, D, BM>;
   static bool configured = false;
   if (!configured) {
@@ -294,14 +373,23 @@ cudaError_t launch_t(const PackedArgs& a, cudaStream_t s) {
   }
   // At most this many tiles: a sequence's last tile may be partly filled.
   const int64_t tiles = a.q_tokens / BM + a.seqs;
-  return launch_dependent(packed_kernel<T, D, BM>, dim3((unsigned)tiles, (unsigned)a.heads), dim3(S::THREADS), (size_t)S::BYTES, s, a);
+  const cudaError_t e = launch_dependent(packed_kernel<T, D, BM>, dim3((unsigned)tiles, (unsigned)a.heads, (unsigned)parts.n),
+                                         dim3(S::THREADS), (size_t)S::BYTES, s, a, parts);
+  if (e != cudaSuccess || parts.n == 1) return e;
+  return launch_dependent(join_kernel<T>, dim3((unsigned)((a.q_tokens * a.heads + 7) / 8)), dim3(256), 0, s, a, parts);
 }
 
 template <typename T, int D>
 cudaError_t launch_bm(const PackedArgs& a, cudaStream_t s) {
   constexpr int BM = D <= 128 ? 64 : 32;
-  if (a.q_tokens * a.heads < (int64_t)BM * 2 * device_sm_count()) return launch_t<T, D, 16>(a, s);
-  return launch_t<T, D, BM>(a, s);
+  Parts parts{1, nullptr, nullptr};
+  if (a.q_tokens * a.heads >= (int64_t)BM * 2 * device_sm_count()) return launch_t<T, D, BM>(a, parts, s);
+  // Parts of 128 keys at least, in the mean: 16 queries of 8 heads of 64 over 1516 keys take 22 us in 11 parts, 64 whole.
+  const int dtype = sizeof(T) == 4 ? kF32 : kBF16;
+  parts.n = (int)std::max<int64_t>(1, std::min<int64_t>(most_parts(dtype, a.q_tokens, a.heads, a.kv_heads, D), a.k_tokens / a.seqs / 128));
+  parts.ml = reinterpret_cast<float*>(reinterpret_cast<char*>(a.counters) + kCounterBytes);
+  parts.o = parts.ml + (a.q_tokens * a.heads * parts.n * 2 + 3) / 4 * 4;
+  return launch_t<T, D, 16>(a, parts, s);
 }
 
 template <typename T>
@@ -318,6 +406,11 @@ cudaError_t launch_dim(const PackedArgs& a, cudaStream_t s) {
 }
 
 }  // namespace packed
+
+size_t packed_parts_bytes(int dtype, int64_t q_tokens, int heads, int kv_heads, int dim) {
+  const int n = packed::most_parts(dtype, q_tokens, heads, kv_heads, dim);
+  return n > 1 ? sizeof(float) * ((size_t)q_tokens * heads * n * (dim + 2) + 4) : 0;
+}
 
 cudaError_t launch_packed(int dtype, const PackedArgs& a, cudaStream_t stream) {
   if (dtype == kBF16 && a.dim >= 64 && a.heads / a.kv_heads <= 128 && a.k_tokens > 0) {

@@ -93,6 +93,8 @@ struct PackedArgs {
 size_t packed_workspace(int dtype, int64_t q_tokens, int heads, int kv_heads, int dim);
 cudaError_t launch_packed_tc(const PackedArgs& a, cudaStream_t stream);
 cudaError_t launch_packed_tc_wide(const PackedArgs& a, cudaStream_t stream);
+// What the parts of the CUDA-core kernel's calls take (packed.cu).
+size_t packed_parts_bytes(int dtype, int64_t q_tokens, int heads, int kv_heads, int dim);
 cudaError_t launch_packed(int dtype, const PackedArgs& a, cudaStream_t stream);
 
 }  // namespace omni

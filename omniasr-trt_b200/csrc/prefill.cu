@@ -929,6 +929,7 @@ static bool may_cut(int64_t q_tokens, int heads, int kv_heads) {
 }
 
 size_t packed_workspace(int dtype, int64_t q_tokens, int heads, int kv_heads, int dim) {
+  if (const size_t parts = packed_parts_bytes(dtype, q_tokens, heads, kv_heads, dim)) return kCounterBytes + parts;
   if (dtype != kBF16 || dim < 64 || heads / kv_heads > 128 || !may_cut(q_tokens, heads, kv_heads)) return 256;
   return kCounterBytes + 32 + sizeof(pfx::PartMeta) * packed_cut_units() + 256 +
          sizeof(float) * 128 * (size_t)(dim + 2) * device_sm_count();

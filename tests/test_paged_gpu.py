@@ -390,6 +390,14 @@ def test_packed_few_rows_over_many_keys(heads, kv, dim):
     run_packed(heads, kv, dim, [3, 40, 1, 7, 0, 5], [1500, 700, 2, 7, 30, 4], "bf16", seed=6)
 
 
+@pytest.mark.parametrize("heads,kv,dim,dtype", [(8, 4, 64, "f32"), (3, 1, 128, "f32"), (2, 1, 512, "f32"), (2, 2, 256, "f32"), (4, 4, 16, "bf16"),
+                                                (6, 2, 32, "bf16"), (130, 1, 64, "bf16")])
+@pytest.mark.parametrize("new,keys", [([16], [1516]), ([3, 40, 1, 7, 0, 5], [1500, 700, 2, 3, 30, 4]), ([1, 20], [2600, 5])])
+def test_packed_parts_without_tensor_cores(heads, kv, dim, dtype, new, keys):
+    """Few queries over many keys where no tensor-core kernel takes the call: parts of the keys, some of them empty."""
+    run_packed(heads, kv, dim, new, keys, dtype, seed=13)
+
+
 MANY = [  # more units than CTAs; some sequences see fewer keys than queries
     (32, 4, [300, 1, 0, 65, 500, 128, 250, 16, 17], [300, 200, 3, 20, 900, 0, 251, 16, 145]),
     (60, 20, [430, 1, 300, 90], [430, 130, 260, 300]), (32, 32, [1100, 513], [1100, 600])]
