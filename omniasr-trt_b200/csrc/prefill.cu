@@ -611,7 +611,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         pos = row / src.group;
         head = u.h * src.group + row - pos * src.group;
         live = pos < u.npos;
-        // A row that sees no key: zeros (its masked probabilities are not exactly zero: ex2_fma's smallest is 2^-126).
+        // A row that sees no key: zeros.
         if (u.lim0 + pos <= 0) inv = 0.f;
         else if (m == -INFINITY) inv = NAN;  // every key it sees scores -inf: no softmax
         dst = p.out + ((int64_t)(u.q0 + pos) * src.heads + head) * D;

@@ -50,15 +50,16 @@ OMNI_DEV void tmem_ld32_async(uint32_t taddr, uint32_t* r) {
 
 // 2^x on the FMA and integer pipes, for x <= 127 (the softmax's arguments are at most 8): x = j + f with j the
 // nearest integer (the 1.5 * 2^23 addition leaves j in the low mantissa bits of t) and f in [-0.5, 0.5]; 2^f from a
-// cubic fitted here for relative error on [-0.5, 0.5] (7.5e-5 at most, far below bf16's 2^-9); 2^j added to the
-// exponent field. x is clamped to -126 (2^-126 or a denormal below it: zero to a probability), so that the exponent
-// field never wraps. Used for part of the probabilities, so that the special-function unit, which forms the others
+// cubic fitted here for relative error on [-0.5, 0.5] under the condition that it is 1 at 0 (1.02e-4 at most, far below
+// bf16's 2^-9); 2^j added to the exponent field. x is clamped to -127, where the fields then cancel to exactly 0 (a masked
+// key's weight must be zero: 2^-126 times the type's largest value is about 4); between -127 and -126 the result is a
+// denormal below 2^-126. Used for part of the probabilities, so that the special-function unit, which forms the others
 // with ex2, is not the only pipe the exponentials load.
 OMNI_DEV float ex2_fma(float x) {
-  x = fmaxf(x, -126.f);
+  x = fmaxf(x, -127.f);
   const float t = x + 12582912.f;
   const float f = x - (t - 12582912.f);
-  const float q = fmaf(fmaf(fmaf(0.055174146f, f, 0.24261758f), f, 0.69326109f), f, 0.99992758f);
+  const float q = fmaf(fmaf(fmaf(0.05500906f, f, 0.24221097f), f, 0.6932829f), f, 1.f);
   return __uint_as_float(__float_as_uint(q) + (__float_as_uint(t) << 23));
 }
 

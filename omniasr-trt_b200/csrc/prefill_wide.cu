@@ -638,7 +638,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int y = 0; y < NWG; ++y) l += ctl.lsum[y][row];
         const float m = PACKED ? ctl.msum[row] : 0.f;
         mbar_arrive(&l_free);
-        // A packed row that sees no key: zeros (its masked probabilities are not exactly zero: ex2_fma's smallest is 2^-126).
+        // A packed row that sees no key: zeros.
         float inv = l > 0.f && !(PACKED && u.lim0 + pos <= 0) ? 1.f / l : 0.f;
         if (PACKED && m == -INFINITY && u.lim0 + pos > 0) inv = NAN;  // every key it sees scores -inf: no softmax
         __nv_bfloat16* dst = row_out + pass * DH;

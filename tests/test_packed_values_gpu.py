@@ -1,0 +1,70 @@
+"""Packed attention where keys or values are not ordinary numbers: scores that are NaN or +inf, hidden values that are NaN,
+infinite or the type's largest, one NaN in a long sequence.
+
+Tolerances as in test_paged_gpu: bf16 outputs and probabilities of 8 significant bits, 2^-8 (|o| + A) with A = sum p |v| / sum p,
+and 2^-10 A for the exponential and the fp32 sums. References are float64, by masked matrix products on the GPU."""
+
+import pytest
+import torch
+
+from omniasr_b200 import kernels
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+NAN, INF = float("nan"), float("inf")
+
+
+def randn(gen, *shape):
+    return torch.randn(*shape, generator=gen, device=DEV).to(torch.bfloat16)
+
+
+def offsets(lens):
+    return [sum(lens[:i]) for i in range(len(lens) + 1)]
+
+
+def packed(q, k, v, new, keys, scale=None):
+    return kernels.packed_attention(q, k, v, torch.tensor(offsets(new), device=DEV), torch.tensor(offsets(keys), device=DEV), scale)
+
+
+def plain(q, k, v, new, keys, scale=None):
+    """(o, A) in float64; keys that a query does not see take no part (k and v finite)."""
+    heads, kv, dim = q.size(1), k.size(1), q.size(2)
+    scale = dim**-0.5 if scale is None else scale
+    out, size = torch.zeros(q.shape, dtype=torch.float64, device=DEV), torch.zeros(q.shape, dtype=torch.float64, device=DEV)
+    for a, b, c, d in zip(offsets(new), offsets(new)[1:], offsets(keys), offsets(keys)[1:]):
+        if b == a or d == c:
+            continue
+        seen = torch.arange(1, b - a + 1, device=DEV) + (d - c) - (b - a)
+        mask = torch.arange(d - c, device=DEV)[None] >= seen[:, None]
+        for h in range(heads):
+            j = h // (heads // kv)
+            x = (q[a:b, h].double() @ k[c:d, j].double().t() * scale).masked_fill(mask, -INF)
+            p = torch.nan_to_num(torch.softmax(x, -1))  # (a query that sees nothing: zeros)
+            out[a:b, h], size[a:b, h] = p @ v[c:d, j].double(), p @ v[c:d, j].double().abs()
+    return out, size
+
+
+def check(got, want, size):
+    bound = 2.0**-8 * (want.abs() + size) + 2.0**-10 * size + 1e-30
+    got = got.double()
+    assert bool(torch.isfinite(got).all()), f"{int((~torch.isfinite(got)).sum())} of {got.numel()} not finite"
+    worst = float(((got - want).abs() / bound).max())
+    assert worst <= 1, f"{worst:.3g} times the bound"
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256, 512])
+@pytest.mark.parametrize("new,keys", [([152, 128, 72], [152, 128, 72]), ([4], [904])])
+def test_hidden_values_of_the_largest_magnitude(dim, new, keys):
+    """A hidden key's weight is zero, not merely small: 2^-126 of the type's largest value would be a number like 4. (The keys
+    have the places 6 modulo 8.)"""
+    g = torch.Generator(device=DEV).manual_seed(4)
+    q, k, v = randn(g, sum(new), 4, dim), randn(g, sum(keys), 2, dim), randn(g, sum(keys), 2, dim)
+    want, size = plain(q, k, v, new, keys)
+    blind = torch.ones(sum(new), dtype=torch.bool, device=DEV)
+    for s, (a, c, d) in enumerate(zip(offsets(new), offsets(keys), keys)):
+        v[c + d - 2] = torch.finfo(torch.bfloat16).min if s % 2 else torch.finfo(torch.bfloat16).max
+        blind[a + new[s] - 2:a + new[s]] = False  # the queries that see it
+    got = packed(q, k, v, new, keys)
+    check(got[blind], want[blind], size[blind])
+    assert kernels.read_status() == 0
