@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
           for (int j = 0; j < 8; ++j) part[j] = max3(part[j], v[i + j], v[i + 8 + j]);
         const float tmax = max3(max3(part[0], part[1], part[2]), max3(part[3], part[4], part[5]),
-                                fmaxf(part[6], part[7])) * p.qscale;
+                                max2(part[6], part[7])) * p.qscale;
         // One barrier per tile over the warpgroups: does any row need a higher max, or has any thread seen an abort?
         const bool saw_abort = abort_flag != 0;
         float mnew = m;
@@ -538,6 +538,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           m = mnew;
         }
         l += ((ls[0] + ls[1]) + (ls[2] + ls[3])) + ((ls[4] + ls[5]) + (ls[6] + ls[7]));
+        if (!row_finite(tmax)) l = NAN;
         if (row == 0 && x == 0 && tile < 400) OMNI_TRACE_AT(2402 + tile * 4);
         // P over this warpgroup's scores, which are in registers already.
         if constexpr (KW / 2 == 32) tmem_st32(scol, w);
@@ -602,7 +603,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int y = 0; y < NWG; ++y) l += ctl.lsum[y][row];
       const float m = PACKED ? ctl.msum[row] : 0.f;
       mbar_arrive(&l_free);
-      float inv = l > 0.f ? 1.f / l : 0.f;
+      float inv = l > 0.f ? 1.f / l : l;  // (l is 0, or NaN)
       const int q = u.qt * BM + row;
       __nv_bfloat16* dst;
       bool live;
@@ -625,7 +626,8 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (u.part % u.b == 0 && row == 0)
             reinterpret_cast<PartMeta*>(src.meta + 8)[u.part / u.b] = {u.qt, u.h, u.q0, u.npos, u.k0, u.lim0, {0, 0}};
           float* part = src.parts + (int64_t)u.part * ((D + 2) * BM) + row;
-          part[D * BM] = u.lim0 + pos > 0 ? m : -INFINITY;
+          // (A row whose sum is NaN takes part whatever its maximum is, and makes the whole NaN.)
+          part[D * BM] = u.lim0 + pos <= 0 ? -INFINITY : l == l ? m : INFINITY;
           part[(D + 1) * BM] = u.lim0 + pos > 0 ? l : 0.f;
 #pragma unroll 1
           for (int c = 0; c < D / 32; ++c, part += 32 * BM) {

@@ -53,8 +53,9 @@ OMNI_DEV void tmem_ld32_async(uint32_t taddr, uint32_t* r) {
 // cubic fitted here for relative error on [-0.5, 0.5] under the condition that it is 1 at 0 (1.02e-4 at most, far below
 // bf16's 2^-9); 2^j added to the exponent field. x is clamped to -127, where the fields then cancel to exactly 0 (a masked
 // key's weight must be zero: 2^-126 times the type's largest value is about 4); between -127 and -126 the result is a
-// denormal below 2^-126. Used for part of the probabilities, so that the special-function unit, which forms the others
-// with ex2, is not the only pipe the exponentials load.
+// denormal below 2^-126. A NaN gives 0: what is not finite is carried into the row's sum (row_finite). Used for part of the
+// probabilities, so that the special-function unit, which forms the others with ex2, is not the only pipe the
+// exponentials load.
 OMNI_DEV float ex2_fma(float x) {
   x = fmaxf(x, -127.f);
   const float t = x + 12582912.f;
@@ -80,11 +81,19 @@ OMNI_DEV uint64_t f2_add(uint64_t a, uint64_t b) {
   asm("add.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
+// Maxima that are NaN where an argument is.
 OMNI_DEV float max3(float a, float b, float c) {
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+OMNI_DEV float max2(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+// False where a row's scores, whose maximum this is, hold a NaN or +inf: the row has no softmax (NaN).
+OMNI_DEV bool row_finite(float max) { return max < INFINITY; }
 
 // Two floats rounded to bf16 and packed (lo in the low half).
 OMNI_DEV uint32_t pack_bf16x2(float lo, float hi) {

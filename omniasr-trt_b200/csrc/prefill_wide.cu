@@ -509,7 +509,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
             for (int j = 0; j < 8; ++j) part[j] = max3(part[j], v[i + j], v[i + 8 + j]);
           const float tmax = max3(max3(part[0], part[1], part[2]), max3(part[3], part[4], part[5]),
-                                  fmaxf(part[6], part[7])) * p.qscale;
+                                  max2(part[6], part[7])) * p.qscale;
           const bool saw_abort = abort_flag != 0;
           float mnew = m;
           bool slow = false;
@@ -567,6 +567,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             m = mnew;
           }
           l += ((ls[0] + ls[1]) + (ls[2] + ls[3])) + ((ls[4] + ls[5]) + (ls[6] + ls[7]));
+          if (!row_finite(tmax)) l = NAN;
           tmem_st32(scol, w);
           tmem_wait_st();
           tc_fence_before();
@@ -639,13 +640,14 @@ __global__ void __launch_bounds__(THREADS, 1)
         const float m = PACKED ? ctl.msum[row] : 0.f;
         mbar_arrive(&l_free);
         // A packed row that sees no key: zeros.
-        float inv = l > 0.f && !(PACKED && u.lim0 + pos <= 0) ? 1.f / l : 0.f;
+        float inv = PACKED && u.lim0 + pos <= 0 ? 0.f : l > 0.f ? 1.f / l : l;  // (l is 0, or NaN)
         if (PACKED && m == -INFINITY && u.lim0 + pos > 0) inv = NAN;  // every key it sees scores -inf: no softmax
         __nv_bfloat16* dst = row_out + pass * DH;
         if constexpr (PACKED) {
           if (u.part >= 0) {  // a part: fp32, a column of rows at a time
             float* part = src.parts + (int64_t)u.part * ((D + 2) * BM) + row;
-            part[D * BM] = u.lim0 + pos > 0 ? m : -INFINITY;
+            // (A row whose sum is NaN takes part whatever its maximum is, and makes the whole NaN.)
+            part[D * BM] = u.lim0 + pos <= 0 ? -INFINITY : l == l ? m : INFINITY;
             part[(D + 1) * BM] = u.lim0 + pos > 0 ? l : 0.f;
             part += pass * DH * BM;
 #pragma unroll 1

@@ -68,3 +68,53 @@ def test_hidden_values_of_the_largest_magnitude(dim, new, keys):
     got = packed(q, k, v, new, keys)
     check(got[blind], want[blind], size[blind])
     assert kernels.read_status() == 0
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256, 512])
+@pytest.mark.parametrize("bad", [NAN, INF])
+def test_scores_that_are_not_finite(dim, bad):
+    """A key whose score is NaN or +inf, its value finite, at each of eight consecutive positions: queries that see it are
+    NaN, the others and the other sequences know nothing of it."""
+    g = torch.Generator(device=DEV).manual_seed(1)
+    new = [150 + i for i in range(8)]
+    n, off = sum(new), offsets(new)
+    q, k, v = randn(g, n, 4, dim), randn(g, n, 2, dim), randn(g, n, 2, dim)
+    q[:, :, 3] = 1.0
+    want, size = plain(q, k, v, new, new)
+    sees = torch.zeros(n, dtype=torch.bool, device=DEV)
+    for s in range(8):
+        at = off[s] + 64 + s
+        k[at, :, 3] = bad
+        sees[at:off[s + 1]] = True
+    got = packed(q, k, v, new, new)
+    assert bool(torch.isnan(got[sees]).all()), f"{int((~torch.isnan(got[sees])).sum())} results know nothing of the key"
+    check(got[~sees], want[~sees], size[~sees])
+    assert kernels.read_status() == 0
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256, 512])
+@pytest.mark.parametrize("bad", [NAN, INF])
+def test_scores_that_are_not_finite_in_cut_units(dim, bad):
+    """The same where the units are cut along the keys."""
+    g = torch.Generator(device=DEV).manual_seed(2)
+    q, k, v = randn(g, 3, 2, dim), randn(g, 900, 2, dim), randn(g, 900, 2, dim)
+    q[:, :, 3] = 1.0
+    want, size = plain(q, k, v, [3], [900])
+    for at in [*range(500, 508), 898]:
+        kk = k.clone()
+        kk[at, :, 3] = bad
+        got = packed(q, kk, v, [3], [900])
+        blind = 1 if at == 898 else 0  # query 0 does not see key 898
+        assert bool(torch.isnan(got[blind:]).all()), f"key {at}"
+        check(got[:blind], want[:blind], size[:blind]) if blind else None
+    assert kernels.read_status() == 0
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256, 512])
+def test_a_part_whose_only_visible_key_is_nan(dim):
+    """769 keys are seven tiles: the last part of a cut unit holds one key that the query sees."""
+    g = torch.Generator(device=DEV).manual_seed(3)
+    q, k, v = randn(g, 1, 1, dim), randn(g, 769, 1, dim), randn(g, 769, 1, dim)
+    k[768] = NAN
+    assert bool(torch.isnan(packed(q, k, v, [1], [769])).all())
+    assert kernels.read_status() == 0
