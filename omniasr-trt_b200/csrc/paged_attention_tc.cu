@@ -18,7 +18,12 @@
 // e4m3 pages are fed to the tensor core as they are (kind::f8f6f4), at half the bytes of bf16; the query and the
 // probabilities become two e4m3 pieces each, in columns of their own: q = 2^e (q1 + q2 / 16), q1 = rn(q 2^-e), q2 =
 // rn(16 (q 2^-e - q1)), 4 + 4 significant bits, which hold a bf16 q exactly (down to 2^-22 of the vector's largest) and
-// a probability as well as bf16 does. The columns are there anyway: N is at least 16. A key's scale 2^ek multiplies its
+// a probability to 8 bits down to 2^-5 (the largest lies between 2^4 and 2^8); below that in steps of 2^-13. Rounded to the
+// nearest, the weights of a long flat tail would all be lost, or all counted half or twice (32,767 keys 12.5 nats below one
+// other are a tenth of the sum), so the second piece is rounded by a threshold that runs evenly over the keys (dither):
+// each weight's error then has mean zero, and a sum of n of them a deviation of at most sqrt(n) 2^-14 against a sum of 2^4 or
+// more. The threshold goes by the key's place alone, so equal calls give equal bits; it costs nothing beside the multiply-add.
+// The columns are there anyway: N is at least 16. A key's scale 2^ek multiplies its
 // scores; a value's scale 2^ev joins the probability as an exponent: w = 2^(x + ev - m), O = sum w v8, l = sum w 2^-ev,
 // with m the running maximum of x + ev, so that w stays in e4m3's range whatever the scales are. m is kept 2^4 below the
 // maximum, w up to 2^8: the pieces' smallest step is then 2^-17 of a typical largest weight.
@@ -822,6 +827,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (i >= 2) wait(&ctl.pv_done[b], ((i >> 1) - 1) & 1);  // P(i - 2) is used up
         unsigned char* pb = smem + C::P_OFF + b * C::PB;
         if constexpr (FP8) {
+          // The dither of this key, within half of the second piece's smallest step (2^-9): the tile's 128 keys in bit-reversed
+          // order, moved on by a golden section from tile to tile. (A weight of 0 stays 0: half a step is rounded to even.)
+          const float dither = (float)(int)(__brev(key_in) + (uint32_t)t * 0x9e3779b9u) * 0x1p-41f;
           uint32_t hw[NQT >= 4 ? NQT / 4 : 1], lw[NQT >= 4 ? NQT / 4 : 1];
 #pragma unroll
           for (int k = 0; k < (NQT >= 4 ? NQT / 4 : 1); ++k) hw[k] = lw[k] = 0u;
@@ -831,8 +839,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t a = __nv_cvt_float2_to_fp8x2(make_float2(p0, p1), __NV_SATFINITE, __NV_E4M3);
             const __half2_raw hr = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)a, __NV_E4M3);
             const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hr));
-            const uint32_t r =
-                __nv_cvt_float2_to_fp8x2(make_float2((p0 - f.x) * 16.f, (p1 - f.y) * 16.f), __NV_SATFINITE, __NV_E4M3);
+            const uint32_t r = __nv_cvt_float2_to_fp8x2(
+                make_float2(fmaf(p0 - f.x, 16.f, dither), fmaf(p1 - f.y, 16.f, dither)), __NV_SATFINITE, __NV_E4M3);
             hw[j >> 2] |= a << (8 * (j & 3));
             lw[j >> 2] |= r << (8 * (j & 3));
           }
