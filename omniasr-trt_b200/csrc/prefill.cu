@@ -680,9 +680,9 @@ __global__ void __launch_bounds__(THREADS, 1)
           const int w = __ffs(left) - 1;
           const int wp = __shfl_sync(0xffffffffu, pos, w), wh = __shfl_sync(0xffffffffu, head, w);
           const int64_t tok = u.q0 + wp;
-          exact_row<D>(src.q + tok * src.q_st + wh * src.q_sh, src.k + u.k0 * src.k_st + u.h * src.k_sh, src.k_st,
-                       src.v + u.k0 * src.v_st + u.h * src.v_sh, src.v_st, u.lim0 + wp, p.qscale,
-                       p.out + (tok * src.heads + wh) * D);
+          exact_row<D, D>(src.q + tok * src.q_st + wh * src.q_sh, src.k + u.k0 * src.k_st + u.h * src.k_sh, src.k_st,
+                          src.v + u.k0 * src.v_st + u.h * src.v_sh, src.v_st, u.lim0 + wp, p.qscale,
+                          p.out + (tok * src.heads + wh) * D, 0);
         }
       }
       if (row == 0) OMNI_TRACE_AT(1601 + nunit * 2);
@@ -842,7 +842,8 @@ cudaError_t launch_prefill(const PrefillArgs& a, cudaStream_t stream) {
 }
 
 // Adds up the parts of a cut unit (block x: unit, y: 32 of its head dims; thread: tile row): o = sum 2^(m_s - m) O_s / sum
-// 2^(m_s - m) l_s, in the order of the keys. Rows whose result is not finite are redone from the formula.
+// 2^(m_s - m) l_s, in the order of the keys. Rows whose result is not finite are redone from the formula, in the block's dims
+// (the other blocks write theirs).
 template <int D>
 __global__ void __launch_bounds__(128) packed_join_kernel(const __grid_constant__ pfx::PackedSrc src, float qscale,
                                                           __nv_bfloat16* out) {
@@ -903,8 +904,9 @@ __global__ void __launch_bounds__(128) packed_join_kernel(const __grid_constant_
     const int k = __ffs(left) - 1;
     const int wp = __shfl_sync(0xffffffffu, pos, k), wh = __shfl_sync(0xffffffffu, head, k);
     const int64_t tok = u.q0 + wp;
-    exact_row<D>(src.q + tok * src.q_st + wh * src.q_sh, src.k + u.k0 * src.k_st + u.h * src.k_sh, src.k_st,
-                 src.v + u.k0 * src.v_st + u.h * src.v_sh, src.v_st, u.lim0 + wp, qscale, out + (tok * src.heads + wh) * D);
+    exact_row<D, 32>(src.q + tok * src.q_st + wh * src.q_sh, src.k + u.k0 * src.k_st + u.h * src.k_sh, src.k_st,
+                     src.v + u.k0 * src.v_st + u.h * src.v_sh, src.v_st, u.lim0 + wp, qscale,
+                     out + (tok * src.heads + wh) * D, d0);
   }
 }
 

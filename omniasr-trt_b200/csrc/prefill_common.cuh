@@ -388,30 +388,30 @@ struct PackedWalk {
   }
 };
 
-// Attention of one query row over its first `lim` keys, by one warp, straight from the formula: for rows whose tensor-core
-// result is not finite, because 0 x NaN (or infinity) of a key the row does not see got into it, or because the row's own
-// keys are so. Keys past `lim` are not read. Rare, so it only has to be right.
-template <int D>
+// Attention of one query row over its first `lim` keys, by one warp, straight from the formula: ND head dims from d0 on,
+// into out[d0 ..]. For rows whose tensor-core result is not finite, because 0 x NaN (or infinity) of a key the row does not
+// see got into it, or because the row's own keys are so. Keys past `lim` are not read. Rare, so it only has to be right.
+template <int D, int ND>
 __device__ __noinline__ void exact_row(const __nv_bfloat16* q, const __nv_bfloat16* k, int64_t k_st, const __nv_bfloat16* v,
-                                       int64_t v_st, int lim, float qscale, __nv_bfloat16* out) {
-  constexpr int N = D / 32;
+                                       int64_t v_st, int lim, float qscale, __nv_bfloat16* out, int d0) {
+  constexpr int N = D / 32, NO = ND / 32;
   const int lane = threadIdx.x & 31;
-  float qv[N], o[N], m = -INFINITY, l = 0.f;
+  v += d0;
+  out += d0;
+  float qv[N], o[NO], m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    qv[i] = __bfloat162float(q[i * 32 + lane]);
-    o[i] = 0.f;
-  }
+  for (int i = 0; i < N; ++i) qv[i] = __bfloat162float(q[i * 32 + lane]);
+#pragma unroll
+  for (int i = 0; i < NO; ++i) o[i] = 0.f;
   for (int j0 = 0; j0 < lim; j0 += 4) {  // four keys' loads in flight
-    __nv_bfloat16 kv[4][N], vv[4][N];
+    __nv_bfloat16 kv[4][N], vv[4][NO];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const int64_t j = min(j0 + c, lim - 1);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        kv[c][i] = k[j * k_st + i * 32 + lane];
-        vv[c][i] = v[j * v_st + i * 32 + lane];
-      }
+      for (int i = 0; i < N; ++i) kv[c][i] = k[j * k_st + i * 32 + lane];
+#pragma unroll
+      for (int i = 0; i < NO; ++i) vv[c][i] = v[j * v_st + i * 32 + lane];
     }
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
@@ -428,13 +428,13 @@ __device__ __noinline__ void exact_row(const __nv_bfloat16* q, const __nv_bfloat
       m = mn;
       l = fmaf(l, f, pr);
 #pragma unroll
-      for (int i = 0; i < N; ++i) o[i] = fmaf(pr, __bfloat162float(vv[c][i]), o[i] * f);
+      for (int i = 0; i < NO; ++i) o[i] = fmaf(pr, __bfloat162float(vv[c][i]), o[i] * f);
     }
     if (l != l) break;  // a NaN score: the whole row is NaN
   }
   const float inv = l != 0.f ? 1.f / l : (lim > 0 ? NAN : 0.f);  // every key it sees scores -inf: no softmax
 #pragma unroll
-  for (int i = 0; i < N; ++i) out[i * 32 + lane] = __float2bfloat16_rn(l != l ? l : o[i] * inv);
+  for (int i = 0; i < NO; ++i) out[i * 32 + lane] = __float2bfloat16_rn(l != l ? l : o[i] * inv);
 }
 
 }  // namespace pfx

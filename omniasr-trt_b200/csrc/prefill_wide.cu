@@ -702,9 +702,9 @@ __global__ void __launch_bounds__(THREADS, 1)
           const int w = __ffs(left) - 1;
           const int wp = __shfl_sync(0xffffffffu, pos, w), wh = __shfl_sync(0xffffffffu, head, w);
           const int64_t tok = u.q0 + wp;
-          exact_row<D>(src.q + tok * src.q_st + wh * src.q_sh, src.k + u.k0 * src.k_st + u.h * src.k_sh, src.k_st,
-                       src.v + u.k0 * src.v_st + u.h * src.v_sh, src.v_st, u.lim0 + wp, p.qscale,
-                       p.out + (tok * src.heads + wh) * D);
+          exact_row<D, D>(src.q + tok * src.q_st + wh * src.q_sh, src.k + u.k0 * src.k_st + u.h * src.k_sh, src.k_st,
+                          src.v + u.k0 * src.v_st + u.h * src.v_sh, src.v_st, u.lim0 + wp, p.qscale,
+                          p.out + (tok * src.heads + wh) * D, 0);
         }
       }
     }

@@ -118,3 +118,19 @@ def test_a_part_whose_only_visible_key_is_nan(dim):
     k[768] = NAN
     assert bool(torch.isnan(packed(q, k, v, [1], [769])).all())
     assert kernels.read_status() == 0
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256, 512])
+def test_cut_units_redo_the_dims_that_need_it(dim):
+    """A hidden NaN in one dim of a cut unit's value: the blocks of 32 dims without it keep their bits, in every call."""
+    g = torch.Generator(device=DEV).manual_seed(8)
+    q, k, v = randn(g, 40, 2, dim), randn(g, 5000, 2, dim), randn(g, 5000, 2, dim)
+    want, size = plain(q, k, v, [40], [5000])
+    clean = packed(q, k, v, [40], [5000])
+    v[4998, :, 5] = NAN
+    for _ in range(20):
+        got = packed(q, k, v, [40], [5000])
+        assert torch.equal(got[:38, :, 32:], clean[:38, :, 32:])
+        check(got[:38], want[:38], size[:38])
+        assert bool(torch.isnan(got[38:, :, 5]).all())
+    assert kernels.read_status() == 0
