@@ -1,5 +1,5 @@
 // Causal attention of packed sequences with grouped heads: entry, and the CUDA-core kernel for what the tensor-core
-// kernels (prefill.cu, prefill_wide.cu) do not take (fp32, head dims under 64).
+// kernels (prefill.cu, prefill_wide.cu) do not take (fp32, head dims under 64, scales that are not positive).
 //
 // Sequence s has queries q_offsets[s] .. q_offsets[s+1] - 1 and keys k_offsets[s] .. k_offsets[s+1] - 1; its last query
 // sees its last key (a chunk of a prompt attends to the keys before it), so query i sees i + 1 + lk - lq keys, none
@@ -413,7 +413,8 @@ size_t packed_parts_bytes(int dtype, int64_t q_tokens, int heads, int kv_heads, 
 }
 
 cudaError_t launch_packed(int dtype, const PackedArgs& a, cudaStream_t stream) {
-  if (dtype == kBF16 && a.dim >= 64 && a.heads / a.kv_heads <= 128 && a.k_tokens > 0) {
+  // (The tensor-core kernels take the maximum of a row's products before they scale them.)
+  if (dtype == kBF16 && a.dim >= 64 && a.heads / a.kv_heads <= 128 && a.k_tokens > 0 && a.scale > 0.f) {
     const cudaError_t e = a.dim <= 128 ? launch_packed_tc(a, stream) : launch_packed_tc_wide(a, stream);
     if (e != cudaErrorNotSupported) return e;
   }

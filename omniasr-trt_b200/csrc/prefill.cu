@@ -674,8 +674,14 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       }
       if constexpr (PACKED) {
-        const bool redo = live && !(odd == 0.f && l - l == 0.f);
+        bool redo = live && odd != 0.f && l == l;  // (a row whose sum is NaN is NaN)
         __syncwarp();  // the rows' first results are written before they are written again
+        if (__any_sync(0xffffffffu, redo)) {
+          const int64_t end = min((int64_t)u.kt * BN, src.k_tokens - u.k0);
+          const BadValues bad =
+              bad_values<D>(src.v + u.k0 * src.v_st + u.h * src.v_sh, src.v_st, max(u.lim0, 0), (int)end, 0);
+          redo = redo && must_redo(bad, u.lim0 + pos);
+        }
         for (unsigned left = __ballot_sync(0xffffffffu, redo); left; left &= left - 1) {
           const int w = __ffs(left) - 1;
           const int wp = __shfl_sync(0xffffffffu, pos, w), wh = __shfl_sync(0xffffffffu, head, w);
@@ -884,7 +890,7 @@ __global__ void __launch_bounds__(128) packed_join_kernel(const __grid_constant_
   }
   const float inv = l != 0.f ? 1.f / l : (u.lim0 + pos > 0 ? NAN : 0.f);  // (keys that all score -inf: no softmax)
   const int64_t at = ((int64_t)(u.q0 + pos) * src.heads + head) * D;
-  float odd = l * 0.f;
+  float odd = 0.f;
   if (live) {
     uint4* dst = reinterpret_cast<uint4*>(out + at + d0);
 #pragma unroll
@@ -899,8 +905,15 @@ __global__ void __launch_bounds__(128) packed_join_kernel(const __grid_constant_
       dst[i] = make_uint4(p4[0], p4[1], p4[2], p4[3]);
     }
   }
+  bool redo = live && odd != 0.f && l == l;
   __syncwarp();
-  for (unsigned left = __ballot_sync(0xffffffffu, live && odd != 0.f); left; left &= left - 1) {
+  if (__any_sync(0xffffffffu, redo)) {
+    const int seen = u.lim0 + u.npos - 1;
+    const int64_t end = min((int64_t)max(1, (seen + 127) / 128) * 128, src.k_tokens - u.k0);
+    const BadValues bad = bad_values<32>(src.v + u.k0 * src.v_st + u.h * src.v_sh, src.v_st, max(u.lim0, 0), (int)end, d0);
+    redo = redo && must_redo(bad, u.lim0 + pos);
+  }
+  for (unsigned left = __ballot_sync(0xffffffffu, redo); left; left &= left - 1) {
     const int k = __ffs(left) - 1;
     const int wp = __shfl_sync(0xffffffffu, pos, k), wh = __shfl_sync(0xffffffffu, head, k);
     const int64_t tok = u.q0 + wp;

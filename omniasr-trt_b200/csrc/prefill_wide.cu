@@ -608,7 +608,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     Unit u;
     for (int n = 0; get(n, u) && !abort_flag; ++n) {
       int pos = 0, head = 0;
-      float odd = 0.f;  // packed: turns NaN if a result of the row is not finite
+      float odd = 0.f, sum = 0.f;  // packed: turns NaN if a result of the row is not finite; the row's sum
       bool live;
       __nv_bfloat16* row_out;
       if constexpr (PACKED) {
@@ -691,13 +691,19 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
           }
         }
-        if constexpr (PACKED) odd = fmaf(l, 0.f, odd);
+        if constexpr (PACKED) sum = l;
       }
       if constexpr (PACKED) {
         if (u.part >= 0 && u.part % u.b == 0 && row == 0)  // a unit's first part
           reinterpret_cast<PartMeta*>(src.meta + 8)[u.part / u.b] = {u.qt, u.h, u.q0, u.npos, u.k0, u.lim0, {0, 0}};
-        const bool redo = live && u.part < 0 && odd != 0.f && !abort_flag;
+        bool redo = live && u.part < 0 && odd != 0.f && sum == sum && !abort_flag;  // (a row whose sum is NaN is NaN)
         __syncwarp();  // the rows' first results are written before they are written again
+        if (__any_sync(0xffffffffu, redo)) {
+          const int64_t end = min((int64_t)u.kt * BN, src.k_tokens - u.k0);
+          const BadValues bad =
+              bad_values<D>(src.v + u.k0 * src.v_st + u.h * src.v_sh, src.v_st, max(u.lim0, 0), (int)end, 0);
+          redo = redo && must_redo(bad, u.lim0 + pos);
+        }
         for (unsigned left = __ballot_sync(0xffffffffu, redo); left; left &= left - 1) {
           const int w = __ffs(left) - 1;
           const int wp = __shfl_sync(0xffffffffu, pos, w), wh = __shfl_sync(0xffffffffu, head, w);

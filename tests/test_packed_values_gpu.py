@@ -4,6 +4,8 @@ infinite or the type's largest, one NaN in a long sequence.
 Tolerances as in test_paged_gpu: bf16 outputs and probabilities of 8 significant bits, 2^-8 (|o| + A) with A = sum p |v| / sum p,
 and 2^-10 A for the exponential and the fp32 sums. References are float64, by masked matrix products on the GPU."""
 
+import time
+
 import pytest
 import torch
 
@@ -133,4 +135,69 @@ def test_cut_units_redo_the_dims_that_need_it(dim):
         assert torch.equal(got[:38, :, 32:], clean[:38, :, 32:])
         check(got[:38], want[:38], size[:38])
         assert bool(torch.isnan(got[38:, :, 5]).all())
+    assert kernels.read_status() == 0
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256, 512])
+def test_one_nan_value_that_most_queries_see(dim):
+    """A NaN in one dim of an early value: NaN in that dim of the queries that see it, at a cost that does not grow with
+    the keys of every query (each redone by itself over 30,000 keys took hundreds of milliseconds)."""
+    g = torch.Generator(device=DEV).manual_seed(5)
+    new, keys = [2048], [30000]
+    q, k, v = randn(g, 2048, 8, dim), randn(g, 30000, 2, dim), randn(g, 30000, 2, dim)
+    clean = packed(q, k, v, new, keys)
+    v[7, 0, 5] = NAN
+    v[20000, 1, 6] = INF
+    got = packed(q, k, v, new, keys)
+    torch.cuda.synchronize()
+    start = time.perf_counter()
+    got = packed(q, k, v, new, keys)
+    torch.cuda.synchronize()
+    took = time.perf_counter() - start
+    same = torch.ones_like(got, dtype=torch.bool)
+    same[:, :4, 5] = False
+    same[:, 4:, 6] = False
+    assert torch.equal(got[same], clean[same])
+    assert bool(torch.isnan(got[:, :4, 5]).all()) and bool((got[:, 4:, 6] == INF).all())
+    assert kernels.read_status() == 0
+    assert took < 0.1, f"{took:.3f} s"
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256, 512])
+def test_values_whose_weighted_sum_overflows(dim):
+    """Large values in a row whose running maximum lags behind its scores, so that the weights reach 2^7: the sum of the
+    weighted values overflows, the result does not."""
+    g = torch.Generator(device=DEV).manual_seed(6)
+    n = 300
+    q, k = randn(g, n, 2, dim), randn(g, n, 2, dim)
+    k[:, :, 0] = torch.linspace(-2, 3, n, device=DEV)[:, None].to(torch.bfloat16)
+    q[:, :, 0] = dim**0.5
+    v = (randn(g, n, 2, dim).sign() * 2.0**118).to(torch.bfloat16)
+    want, size = plain(q, k, v, [n], [n])
+    check(packed(q, k, v, [n], [n]), want, size)
+    assert kernels.read_status() == 0
+
+
+def test_hidden_nan_after_many_keys():
+    """The queries before a NaN value are redone from the formula, over as many keys as they see."""
+    g = torch.Generator(device=DEV).manual_seed(7)
+    new, keys = [200], [60000]
+    q, k, v = randn(g, 200, 2, 128), randn(g, 60000, 1, 128), randn(g, 60000, 1, 128)
+    want, size = plain(q, k, v, new, keys)
+    v[59980] = NAN
+    got = packed(q, k, v, new, keys)
+    check(got[:180], want[:180], size[:180])
+    assert bool(torch.isnan(got[180:]).all())
+    assert kernels.read_status() == 0
+
+
+@pytest.mark.parametrize("dim", [32, 64, 128, 256, 512])
+@pytest.mark.parametrize("scale", [0.0, -0.3])
+def test_scales_that_are_not_positive(dim, scale):
+    """A scale of zero weighs all visible keys alike; a negative one prefers the smallest products."""
+    g = torch.Generator(device=DEV).manual_seed(9)
+    new, keys = [150, 40], [150, 300]
+    q, k, v = randn(g, 190, 4, dim), randn(g, 450, 2, dim), randn(g, 450, 2, dim)
+    want, size = plain(q, k, v, new, keys, scale)
+    check(packed(q, k, v, new, keys, scale), want, size)
     assert kernels.read_status() == 0
