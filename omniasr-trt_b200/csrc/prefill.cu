@@ -581,6 +581,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     }
     int nunit = 0;
+    RedoList list;  // packed
     Unit u;
     for (; get(nunit, u) && !abort_flag; ++nunit) {
       if constexpr (!PACKED) {
@@ -674,24 +675,14 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       }
       if constexpr (PACKED) {
-        bool redo = live && odd != 0.f && l == l;  // (a row whose sum is NaN is NaN)
-        __syncwarp();  // the rows' first results are written before they are written again
-        if (__any_sync(0xffffffffu, redo)) {
-          const int64_t end = min((int64_t)u.kt * BN, src.k_tokens - u.k0);
-          const BadValues bad =
-              bad_values<D>(src.v + u.k0 * src.v_st + u.h * src.v_sh, src.v_st, max(u.lim0, 0), (int)end, 0);
-          redo = redo && must_redo(bad, u.lim0 + pos);
-        }
-        for (unsigned left = __ballot_sync(0xffffffffu, redo); left; left &= left - 1) {
-          const int w = __ffs(left) - 1;
-          const int wp = __shfl_sync(0xffffffffu, pos, w), wh = __shfl_sync(0xffffffffu, head, w);
-          const int64_t tok = u.q0 + wp;
-          exact_row<D, D>(src.q + tok * src.q_st + wh * src.q_sh, src.k + u.k0 * src.k_st + u.h * src.k_sh, src.k_st,
-                          src.v + u.k0 * src.v_st + u.h * src.v_sh, src.v_st, u.lim0 + wp, p.qscale,
-                          p.out + (tok * src.heads + wh) * D, 0);
-        }
+        const bool redo = live && odd != 0.f && l == l;  // (a row whose sum is NaN is NaN)
+        const unsigned rows = __ballot_sync(0xffffffffu, redo);
+        if (rows && list.add(u, rows, lane)) list.run<D>(src, row - lane, p.qscale, p.out);
       }
       if (row == 0) OMNI_TRACE_AT(1601 + nunit * 2);
+    }
+    if constexpr (PACKED) {
+      if (!__any_sync(0xffffffffu, abort_flag != 0)) list.run<D>(src, row - lane, p.qscale, p.out);
     }
   }
   __syncthreads();
@@ -905,22 +896,11 @@ __global__ void __launch_bounds__(128) packed_join_kernel(const __grid_constant_
       dst[i] = make_uint4(p4[0], p4[1], p4[2], p4[3]);
     }
   }
-  bool redo = live && odd != 0.f && l == l;
-  __syncwarp();
-  if (__any_sync(0xffffffffu, redo)) {
-    const int seen = u.lim0 + u.npos - 1;
-    const int64_t end = min((int64_t)max(1, (seen + 127) / 128) * 128, src.k_tokens - u.k0);
-    const BadValues bad = bad_values<32>(src.v + u.k0 * src.v_st + u.h * src.v_sh, src.v_st, max(u.lim0, 0), (int)end, d0);
-    redo = redo && must_redo(bad, u.lim0 + pos);
-  }
-  for (unsigned left = __ballot_sync(0xffffffffu, redo); left; left &= left - 1) {
-    const int k = __ffs(left) - 1;
-    const int wp = __shfl_sync(0xffffffffu, pos, k), wh = __shfl_sync(0xffffffffu, head, k);
-    const int64_t tok = u.q0 + wp;
-    exact_row<D, 32>(src.q + tok * src.q_st + wh * src.q_sh, src.k + u.k0 * src.k_st + u.h * src.k_sh, src.k_st,
-                     src.v + u.k0 * src.v_st + u.h * src.v_sh, src.v_st, u.lim0 + wp, qscale,
-                     out + (tok * src.heads + wh) * D, d0);
-  }
+  const bool redo = live && odd != 0.f && l == l;
+  __syncwarp();  // the rows' first results are written before they are written again
+  const unsigned rows = __ballot_sync(0xffffffffu, redo);
+  if (rows)
+    redo_rows<D, 32>(src, rows, row & ~31, u.q0, u.k0, u.lim0, u.h, max(1, (u.lim0 + u.npos - 1 + 127) / 128), qscale, out, d0);
 }
 
 cudaError_t launch_packed_join(const PackedArgs& a, const pfx::PackedSrc& src, cudaStream_t stream) {

@@ -475,6 +475,44 @@ __device__ __noinline__ void exact_row(const __nv_bfloat16* q, const __nv_bfloat
   for (int i = 0; i < NO; ++i) out[i * 32 + lane] = __float2bfloat16_rn(l != l ? l : o[i] * inv);
 }
 
+// Rows `rows` (a bit each, from tile row row0 on) of a unit that are not finite: redone where must_redo says so. One warp.
+template <int D, int ND>
+__device__ __noinline__ void redo_rows(const PackedSrc& src, unsigned rows, int row0, int q0, int k0, int lim0, int h, int kt,
+                                       float qscale, __nv_bfloat16* out, int d0) {
+  const __nv_bfloat16* k = src.k + k0 * src.k_st + h * src.k_sh;
+  const __nv_bfloat16* v = src.v + k0 * src.v_st + h * src.v_sh;
+  const int end = (int)min((int64_t)kt * 128, src.k_tokens - k0);
+  const BadValues bad = bad_values<ND>(v, src.v_st, max(lim0, 0), end, d0);
+  for (; rows; rows &= rows - 1) {
+    const int row = row0 + __ffs(rows) - 1, pos = row / src.group, head = h * src.group + row - pos * src.group;
+    if (!must_redo(bad, lim0 + pos)) continue;
+    const int64_t tok = q0 + pos;
+    exact_row<D, ND>(src.q + tok * src.q_st + head * src.q_sh, k, src.k_st, v, src.v_st, lim0 + pos, qscale,
+                     out + (tok * src.heads + head) * D, d0);
+  }
+}
+
+// Such rows of a CTA's units, up to 32 units per warp (a lane holds one): they may take longer than the other roles wait for the
+// epilogue, so they are redone when the CTA's units are done.
+struct RedoList {
+  unsigned rows = 0;
+  int q0, k0, lim0, h, kt;
+  int count = 0;
+  OMNI_DEV bool add(const Unit& u, unsigned rows_, int lane) {  // true: the list is full
+    if (lane == count) rows = rows_, q0 = u.q0, k0 = u.k0, lim0 = u.lim0, h = u.h, kt = u.kt;
+    return ++count == 32;
+  }
+  template <int D>
+  OMNI_DEV void run(const PackedSrc& src, int row0, float qscale, __nv_bfloat16* out) {
+    __syncwarp();  // the rows' first results are written before they are written again
+    for (int i = 0; i < count; ++i)
+      redo_rows<D, D>(src, __shfl_sync(0xffffffffu, rows, i), row0, __shfl_sync(0xffffffffu, q0, i),
+                      __shfl_sync(0xffffffffu, k0, i), __shfl_sync(0xffffffffu, lim0, i), __shfl_sync(0xffffffffu, h, i),
+                      __shfl_sync(0xffffffffu, kt, i), qscale, out, 0);
+    count = 0;
+  }
+};
+
 }  // namespace pfx
 
 // (row, head) pairs per scheduling group of the prefill kernels (prefill.cu).

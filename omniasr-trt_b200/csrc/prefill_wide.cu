@@ -605,6 +605,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     }
     int item = 0;
+    RedoList list;  // packed
     Unit u;
     for (int n = 0; get(n, u) && !abort_flag; ++n) {
       int pos = 0, head = 0;
@@ -696,23 +697,13 @@ __global__ void __launch_bounds__(THREADS, 1)
       if constexpr (PACKED) {
         if (u.part >= 0 && u.part % u.b == 0 && row == 0)  // a unit's first part
           reinterpret_cast<PartMeta*>(src.meta + 8)[u.part / u.b] = {u.qt, u.h, u.q0, u.npos, u.k0, u.lim0, {0, 0}};
-        bool redo = live && u.part < 0 && odd != 0.f && sum == sum && !abort_flag;  // (a row whose sum is NaN is NaN)
-        __syncwarp();  // the rows' first results are written before they are written again
-        if (__any_sync(0xffffffffu, redo)) {
-          const int64_t end = min((int64_t)u.kt * BN, src.k_tokens - u.k0);
-          const BadValues bad =
-              bad_values<D>(src.v + u.k0 * src.v_st + u.h * src.v_sh, src.v_st, max(u.lim0, 0), (int)end, 0);
-          redo = redo && must_redo(bad, u.lim0 + pos);
-        }
-        for (unsigned left = __ballot_sync(0xffffffffu, redo); left; left &= left - 1) {
-          const int w = __ffs(left) - 1;
-          const int wp = __shfl_sync(0xffffffffu, pos, w), wh = __shfl_sync(0xffffffffu, head, w);
-          const int64_t tok = u.q0 + wp;
-          exact_row<D, D>(src.q + tok * src.q_st + wh * src.q_sh, src.k + u.k0 * src.k_st + u.h * src.k_sh, src.k_st,
-                          src.v + u.k0 * src.v_st + u.h * src.v_sh, src.v_st, u.lim0 + wp, p.qscale,
-                          p.out + (tok * src.heads + wh) * D, 0);
-        }
+        const bool redo = live && u.part < 0 && odd != 0.f && sum == sum && !abort_flag;  // (a row whose sum is NaN is NaN)
+        const unsigned rows = __ballot_sync(0xffffffffu, redo);
+        if (rows && list.add(u, rows, lane)) list.run<D>(src, row - lane, p.qscale, p.out);
       }
+    }
+    if constexpr (PACKED) {
+      if (!__any_sync(0xffffffffu, abort_flag != 0)) list.run<D>(src, row - lane, p.qscale, p.out);
     }
   }
   __syncthreads();

@@ -201,3 +201,21 @@ def test_scales_that_are_not_positive(dim, scale):
     want, size = plain(q, k, v, new, keys, scale)
     check(packed(q, k, v, new, keys, scale), want, size)
     assert kernels.read_status() == 0
+
+
+@pytest.mark.parametrize("dim", [128, 512])
+def test_rows_redone_for_longer_than_a_wait_may_last(dim):
+    """127 queries over 260,000 keys do not see the last, NaN: their block redoes them for seconds, with a unit of a short
+    sequence behind them, and no wait of the other warps gives up."""
+    g = torch.Generator(device=DEV).manual_seed(11)
+    n = 260000 if dim == 128 else 100000
+    new, keys = [128] * 401, [n] + [128] * 400
+    q, k, v = randn(g, sum(new), 1, dim), randn(g, sum(keys), 1, dim), randn(g, sum(keys), 1, dim)
+    v[n - 1] = NAN
+    got = packed(q, k, v, new, keys)
+    assert kernels.read_status() == 0
+    assert bool(torch.isnan(got[127]).all())
+    v[n - 1] = 0.0
+    want, size = plain(q, k, v, new, keys)
+    rest = torch.arange(sum(new), device=DEV) != 127
+    check(got[rest], want[rest], size[rest])
