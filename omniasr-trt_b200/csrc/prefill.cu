@@ -473,11 +473,11 @@ __global__ void __launch_bounds__(THREADS, 1)
           for (int j = 0; j < 8; ++j) part[j] = max3(part[j], v[i + j], v[i + 8 + j]);
         const float tmax = max3(max3(part[0], part[1], part[2]), max3(part[3], part[4], part[5]),
                                 max2(part[6], part[7])) * p.qscale;
-        // One barrier per tile over the warpgroups: does any row need a higher max, or has any thread seen an abort?
+        // One barrier per tile over the warpgroups: does any row need a higher max (or has a NaN), or has any thread seen an abort?
         const bool saw_abort = abort_flag != 0;
         float mnew = m;
         bool slow = false;
-        const bool any_raise = sync_or(1, SM_THREADS, tmax > m + kRescale || saw_abort);
+        const bool any_raise = sync_or(1, SM_THREADS, !(tmax <= m + kRescale) || saw_abort);
         if (row == 0 && x == 0 && tile < 400) OMNI_TRACE_AT(2401 + tile * 4);
         if (any_raise) {
           if (sync_or(1, SM_THREADS, saw_abort)) {
@@ -485,6 +485,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             break;
           }
           ctl.tmax[x][row] = tmax;
+          if (!row_finite(tmax)) l = NAN;
           named_sync(2, SM_THREADS);
           float t2 = ctl.tmax[0][row];  // the same in every warpgroup
 #pragma unroll
@@ -538,7 +539,6 @@ __global__ void __launch_bounds__(THREADS, 1)
           m = mnew;
         }
         l += ((ls[0] + ls[1]) + (ls[2] + ls[3])) + ((ls[4] + ls[5]) + (ls[6] + ls[7]));
-        if (!row_finite(tmax)) l = NAN;
         if (row == 0 && x == 0 && tile < 400) OMNI_TRACE_AT(2402 + tile * 4);
         // P over this warpgroup's scores, which are in registers already.
         if constexpr (KW / 2 == 32) tmem_st32(scol, w);

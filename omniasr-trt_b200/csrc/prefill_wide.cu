@@ -513,12 +513,13 @@ __global__ void __launch_bounds__(THREADS, 1)
           const bool saw_abort = abort_flag != 0;
           float mnew = m;
           bool slow = false;
-          if (sync_or(1, SM_THREADS, tmax > m + kRescale || saw_abort)) {
+          if (sync_or(1, SM_THREADS, !(tmax <= m + kRescale) || saw_abort)) {
             if (sync_or(1, SM_THREADS, saw_abort)) {
               quit = true;
               break;
             }
             ctl.tmax[x][row] = tmax;
+            if (!row_finite(tmax)) l = NAN;
             named_sync(2, SM_THREADS);
             float t2 = ctl.tmax[0][row];
 #pragma unroll
@@ -567,7 +568,6 @@ __global__ void __launch_bounds__(THREADS, 1)
             m = mnew;
           }
           l += ((ls[0] + ls[1]) + (ls[2] + ls[3])) + ((ls[4] + ls[5]) + (ls[6] + ls[7]));
-          if (!row_finite(tmax)) l = NAN;
           tmem_st32(scol, w);
           tmem_wait_st();
           tc_fence_before();
