@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
         }
         ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-        if (!ok || u.kt == 0 || abort_flag) break;
+        if (!ok || u.kt == 0 || __any_sync(0xffffffffu, abort_flag != 0)) break;
         tile = __shfl_sync(0xffffffffu, tile, 0);
         next = (long long)gridDim.x + __shfl_sync(0xffffffffu, claim, 0);
       }
@@ -583,19 +583,22 @@ __global__ void __launch_bounds__(THREADS, 1)
     int nunit = 0;
     RedoList list;  // packed
     Unit u;
-    for (; get(nunit, u) && !abort_flag; ++nunit) {
+    // (Converged, as the issuers: the warp's loads from TMEM and its votes want all lanes.)
+    for (; wget(nunit, u); ++nunit) {
       if constexpr (!PACKED) {
         const int ahead = q_loader ? cta_unit(src, units, nunit + QS) : -1;
+        bool ok = true;
         if (ahead >= 0) {
-          if (!wait(&q_empty[nunit % QS], (nunit / QS) & 1)) break;
-          load_q(nunit + QS, ahead);
+          ok = wait(&q_empty[nunit % QS], (nunit / QS) & 1);
+          if (ok) load_q(nunit + QS, ahead);
         }
+        if (!__all_sync(0xffffffffu, ok)) break;
       } else {
         __syncwarp();
         if (lane == 0) put(nunit);
       }
-      if (!wait(&o_ready, nunit & 1)) break;
-      if (!wait(&l_full, nunit & 1)) break;
+      if (!wwait(&o_ready, nunit & 1)) break;
+      if (!wwait(&l_full, nunit & 1)) break;
       if (row == 0) OMNI_TRACE_AT(1600 + nunit * 2);
       tc_fence_after();
       __syncwarp();

@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
         }
         ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-        if (!ok || u.kt == 0 || abort_flag) break;
+        if (!ok || u.kt == 0 || __any_sync(0xffffffffu, abort_flag != 0)) break;
         kc = __shfl_sync(0xffffffffu, kc, 0);
         next = (long long)gridDim.x + __shfl_sync(0xffffffffu, claim, 0);
       }
@@ -607,7 +607,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     int item = 0;
     RedoList list;  // packed
     Unit u;
-    for (int n = 0; get(n, u) && !abort_flag; ++n) {
+    bool ok = true;  // (converged, as in prefill.cu)
+    for (int n = 0; ok && wget(n, u); ++n) {
       int pos = 0, head = 0;
       float odd = 0.f, sum = 0.f;  // packed: turns NaN if a result of the row is not finite; the row's sum
       bool live;
@@ -624,15 +625,15 @@ __global__ void __launch_bounds__(THREADS, 1)
         live = q < p.width;
         row_out = p.out + (int64_t)u.b * p.out_sb + (int64_t)q * p.out_sw + (int64_t)u.h * p.out_sh;
       }
-      for (int pass = 0; pass < PASSES && !abort_flag; ++pass, ++item) {
+      for (int pass = 0; pass < PASSES; ++pass, ++item) {
         if constexpr (!PACKED) {
           if (pass == PASSES - 1 && q_loader) {  // the next unit's queries, as the last S MMAs of this one free the chunks
             const int un = cta_unit(src, units, n + 1);
             if (un >= 0) load_q(n + 1, un);
           }
         }
-        if (!wait(&o_ready, item & 1)) break;
-        if (!wait(&l_full, item & 1)) break;
+        ok = wwait(&o_ready, item & 1) && wwait(&l_full, item & 1);
+        if (!ok) break;
         tc_fence_after();
         __syncwarp();
         float l = 0.f;
@@ -697,7 +698,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       if constexpr (PACKED) {
         if (u.part >= 0 && u.part % u.b == 0 && row == 0)  // a unit's first part
           reinterpret_cast<PartMeta*>(src.meta + 8)[u.part / u.b] = {u.qt, u.h, u.q0, u.npos, u.k0, u.lim0, {0, 0}};
-        const bool redo = live && u.part < 0 && odd != 0.f && sum == sum && !abort_flag;  // (a row whose sum is NaN is NaN)
+        const bool redo = live && u.part < 0 && odd != 0.f && sum == sum && ok;  // (a row whose sum is NaN is NaN)
         const unsigned rows = __ballot_sync(0xffffffffu, redo);
         if (rows && list.add(u, rows, lane)) list.run<D>(src, row - lane, p.qscale, p.out);
       }
