@@ -146,6 +146,34 @@ struct Elem<__nv_bfloat16> {
   OMNI_DEV static __nv_bfloat16 from_float(float x) { return __float2bfloat16_rn(x); }
 };
 
+// ---------------------------------------------------------------------------------------------
+// Rows of an attention on the tensor cores that are not finite, and what they may owe it to.
+
+// The first and the last key with a value that is not finite: `first` of the keys [0, end) (INT_MAX: none), `last` of
+// [from, end) (-1: none).
+struct BadValues {
+  int first, last;
+};
+// By one warp; bad(j): whether key j has such a value.
+template <typename F>
+OMNI_DEV BadValues find_bad(int from, int end, F bad) {
+  const int lane = threadIdx.x & 31;
+  BadValues r{0x7fffffff, -1};
+  for (int j0 = end - 1; j0 >= from && r.last < 0; j0 -= 32) {
+    const unsigned hit = __ballot_sync(0xffffffffu, j0 - lane >= from && bad(max(j0 - lane, 0)));
+    if (hit) r.last = j0 - (__ffs(hit) - 1);
+  }
+  for (int j0 = 0; j0 < end && r.first == 0x7fffffff; j0 += 32) {
+    const unsigned hit = __ballot_sync(0xffffffffu, j0 + lane < end && bad(min(j0 + lane, end - 1)));
+    if (hit) r.first = j0 + (__ffs(hit) - 1);
+  }
+  return r;
+}
+// Whether a row of `lim` visible keys whose tensor-core result is not finite, its row sum being so, may owe that to the kernel:
+// to 0 x NaN (or infinity) of a key it does not see, or, where no value is bad at all, to a sum that passed fp32's range before it
+// was divided. Otherwise a value that it sees is not finite, and the result stands.
+OMNI_DEV bool must_redo(const BadValues& bad, int lim) { return bad.last >= lim || bad.first >= lim; }
+
 // 2^x on the special-function unit (MUFU.EX2); ex2(-inf) = 0.
 OMNI_DEV float ex2(float x) {
   float y;

@@ -283,7 +283,9 @@ struct alignas(16) Ctl {
   float weight[kJoin][kMaxCols];  // their weights,
   float2 joined[kMaxCols];        // and the whole's
   int last;                       // epilogue: this CTA joins the unit
-  unsigned bad;                   // epilogue: columns to redo
+  int odd;                        // epilogue: some whole unit has a column that is not finite
+  int odd_cuts;                   // cut units that this CTA joined and that have one (it has a part of two at most):
+  unsigned odd_cut[2];            // row << 16 | unit within the row
 };
 static_assert(sizeof(Ctl) <= kCtlBytes, "control block");
 
@@ -294,8 +296,31 @@ OMNI_DEV int64_t query_row(const Params& p, int b, int h, int col, int* t) {
   return ((int64_t)b * p.tokens + *t) * p.heads + h * p.group + g;
 }
 
-// One column straight from the formula, by one warp: for a draft column whose tensor-core result is not finite, because a
-// later draft position that it does not see holds something that is not (0 x NaN), or its own keys do. Rare.
+// BadValues of a row's kv head (a value's scale that is infinite among them), by one warp; a lane looks at a key.
+template <bool FP8, int DIM>
+__device__ __noinline__ BadValues bad_page_values(const PageCache& c, const int32_t* table, int h, int from, int end) {
+  return find_bad(from, end, [&](int j) {
+    const int pi = j / c.page, off = j - pi * c.page;
+    int64_t id = table[pi];
+    if (id < 0 || id >= c.pages) id = 0;
+    const int64_t at = id * c.s_page + (int64_t)h * c.s_head + (int64_t)off * c.s_pos;
+    const uint4* row = reinterpret_cast<const uint4*>(reinterpret_cast<const unsigned char*>(c.v) + at * (FP8 ? 1 : 2));
+    uint32_t any = FP8 && c.v_scale[(id * c.kv_heads + h) * c.page + off] == 255 ? 1u : 0u;
+#pragma unroll 8
+    for (int i = 0; i < DIM * (FP8 ? 1 : 2) / 16; ++i) {
+      const uint4 u = __ldg(row + i);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {  // a code that is NaN; a half whose exponent bits are all ones
+        const uint32_t z = ~w[k] & (FP8 ? 0x7f7f7f7fu : 0x7f807f80u);
+        any |= (z - (FP8 ? 0x01010101u : 0x00010001u)) & ~z & (FP8 ? 0x80808080u : 0x80008000u);
+      }
+    }
+    return any != 0u;
+  });
+}
+
+// One column straight from the formula, by one warp, for the draft columns of must_redo. Rare.
 template <bool FP8, int DIM>
 __device__ __noinline__ void exact_column(const __nv_bfloat16* q, const PageCache& c, const int32_t* table, int h, int lim,
                                           float qscale, __nv_bfloat16* out) {
@@ -345,6 +370,35 @@ __device__ __noinline__ void exact_column(const __nv_bfloat16* q, const PageCach
   for (int i = 0; i < NV; ++i) out[i * 32 + lane] = __float2bfloat16_rn(l != l ? l : o[i] * inv);
 }
 
+// Every fourth column of unit u of row b, from `first` on, by one warp: those that are not finite are redone where must_redo says
+// so. (NaN in every dim without a bad value: the column's sum is NaN, as a NaN score has it.)
+template <bool FP8, int DIM>
+__device__ __noinline__ void redo_columns(const Params& p, const int* len, int b, int u, int first) {
+  const int lane = threadIdx.x & 31;
+  const int h = u / p.chunks, col0 = (u - h * p.chunks) * p.chunk_cols, ncol = min(p.chunk_cols, p.cols - col0);
+  const int need = min(p.cap, len[b] + p.tokens - 1);
+  const int32_t* table = p.table + (int64_t)b * p.table_stride;
+  BadValues bad{};
+  bool known = false;
+  for (int j = first; j < ncol; j += 4) {
+    int t;
+    const int64_t row = query_row(p, b, h, col0 + j, &t);
+    bool odd = false, nan = true;
+#pragma unroll
+    for (int i = 0; i < DIM / 32; ++i) {
+      const float x = __bfloat162float(p.out[row * DIM + i * 32 + lane]);
+      odd |= !(fabsf(x) <= 3.3e38f);
+      nan &= x != x;
+    }
+    if (!__any_sync(0xffffffffu, odd)) continue;
+    if (!known) bad = bad_page_values<FP8, DIM>(p.c, table, h, max(0, len[b]), need);
+    known = true;
+    const int lim = min(need, len[b] + t);
+    if (must_redo(bad, lim) && (bad.last >= lim || !__all_sync(0xffffffffu, nan)))
+      exact_column<FP8, DIM>(p.q + row * DIM, p.c, table, h, lim, p.qscale, p.out + row * DIM);
+  }
+}
+
 template <bool FP8, int DIM, int NQT>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ Params p) {
@@ -383,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_fence_init();
     abort_flag = 0;
     for (int s = 0; s < kMaxSlots; ++s) loads[s] = 0;
-    ctl.bad = 0;
+    ctl.odd = ctl.odd_cuts = 0;
   }
   if (warp == W_EPI) tmem_alloc(&ctl.tmem_base, C::TMEM);
   if (warp == W_LOADK && lane == 0) {
@@ -1006,6 +1060,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       query_load();
       query_store(n);
     }
+    constexpr bool DRAFTS = NQT > 1;  // (one column is one token, which sees every key)
     constexpr bool EARLY = QC * DC <= 8;  // loaded a segment before they are written out (while the registers hold them)
     bool more = ahead.next(sq);  // segment n + QN
     if (EARLY && more) query_load();
@@ -1042,7 +1097,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         l[j] = ls[0] * wt[0][j] + ls[1] * wt[1][j];
       }
       mbar_arrive(&ctl.ml_free[n & 1]);
-      unsigned bad = 0;  // columns with a result that is not finite
+      bool bad = false;  // some result is not finite
       auto store = [&](int c, const float (&o)[NQT], const float (&sum)[NQT]) {
         int tt = tok0, g = g0;
         const int64_t row0 = (int64_t)s.b * p.tokens * p.heads + h * p.group;
@@ -1052,7 +1107,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int64_t row = row0 + tt * p.heads + g;
             // Nothing summed: a query that sees no key gets zeros, one whose keys all score -inf has no softmax.
             const float r = sum[j] != 0.f ? o[j] * __fdividef(1.f, sum[j]) : (len[s.b] + tt > 0 ? NAN : 0.f);
-            if (!(fabsf(r) <= 3.3e38f) && (CD == 128 || d < CD)) bad |= 1u << j;
+            if (DRAFTS && !(fabsf(r) <= 3.3e38f) && (CD == 128 || d < CD)) bad = true;
             if (CD == 128 || d < CD) p.out[row * DIM + c * CD + d] = __float2bfloat16_rn(r);
           }
           if (++g == p.group) {
@@ -1201,23 +1256,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (emit) {
-        if (p.tokens > 1) {  // a column may have met a key it does not see
-          if (sync_or(2, 128, bad != 0)) {
-            if (bad) atomicOr(&ctl.bad, bad);
-            named_sync(2, 128);
-            const unsigned all = *(volatile unsigned*)&ctl.bad;
-            for (int j = warp - W_EPI; j < ncol; j += 4) {
-              if (!(all >> j & 1)) continue;
-              int t2;
-              const int64_t row = query_row(p, s.b, h, col0 + j, &t2);
-              exact_column<FP8, DIM>(p.q + row * DIM, p.c, p.table + (int64_t)s.b * p.table_stride, h,
-                                     min(s.need, len[s.b] + t2), p.qscale, p.out + row * DIM);
-            }
-            named_sync(2, 128);
-            if (d == 0) ctl.bad = 0;
-            named_sync(2, 128);
+        if (DRAFTS && p.tokens > 1) {  // a column may have met a key it does not see
+          // Redone when the CTA's units are done: it may take longer than the other roles wait for this one.
+          if (sync_or(2, 128, bad) && d == 0) {
+            if (here && s.t1 == s.nt) ctl.odd = 1;
+            else ctl.odd_cut[ctl.odd_cuts++] = (unsigned)s.b << 16 | (unsigned)s.u;
           }
         }
+      }
+    }
+    if (DRAFTS && p.tokens > 1 && !sync_or(2, 128, abort_flag != 0)) {
+      for (int i = 0; i < ctl.odd_cuts; ++i) redo_columns<FP8, DIM>(p, len, ctl.odd_cut[i] >> 16, ctl.odd_cut[i] & 0xffff, wq);
+      if (ctl.odd) {
+        w.init(p, pre, len, c0, c1);
+        while (w.next(s))
+          if (s.t0 == 0 && s.t1 == s.nt) redo_columns<FP8, DIM>(p, len, s.b, s.u, wq);
       }
     }
   }

@@ -388,14 +388,9 @@ struct PackedWalk {
   }
 };
 
-// The first and the last key with a value that is not finite, by one warp, of ND head dims from d0 on: `first` of the keys
-// [0, end) (INT_MAX: none), `last` of [from, end) (-1: none). A lane looks at a key.
-struct BadValues {
-  int first, last;
-};
+// BadValues of ND head dims from d0 on, by one warp; a lane looks at a key.
 template <int ND>
 __device__ __noinline__ BadValues bad_values(const __nv_bfloat16* v, int64_t v_st, int from, int end, int d0) {
-  const int lane = threadIdx.x & 31;
   auto bad = [&](int j) {
     const uint4* row = reinterpret_cast<const uint4*>(v + j * v_st + d0);
     uint32_t any = 0u;
@@ -411,22 +406,8 @@ __device__ __noinline__ BadValues bad_values(const __nv_bfloat16* v, int64_t v_s
     }
     return any != 0u;
   };
-  BadValues r{0x7fffffff, -1};
-  for (int j0 = end - 1; j0 >= from && r.last < 0; j0 -= 32) {
-    const unsigned hit = __ballot_sync(0xffffffffu, j0 - lane >= from && bad(max(j0 - lane, 0)));
-    if (hit) r.last = j0 - (__ffs(hit) - 1);
-  }
-  for (int j0 = 0; j0 < end && r.first == 0x7fffffff; j0 += 32) {
-    const unsigned hit = __ballot_sync(0xffffffffu, j0 + lane < end && bad(min(j0 + lane, end - 1)));
-    if (hit) r.first = j0 + (__ffs(hit) - 1);
-  }
-  return r;
+  return find_bad(from, end, bad);
 }
-// Whether a row of `lim` visible keys whose tensor-core result is not finite, its row sum being so, may owe that to the kernel:
-// to 0 x NaN (or infinity) of a key it does not see, or, where no value is bad at all, to a sum that passed fp32's range before it
-// was divided. Otherwise a value that it sees is not finite, and the result stands.
-OMNI_DEV bool must_redo(const BadValues& bad, int lim) { return bad.last >= lim || bad.first >= lim; }
-
 // Attention of one query row over its first `lim` keys, by one warp, straight from the formula: ND head dims from d0 on,
 // into out[d0 ..], for the rows of must_redo. Keys past `lim` are not read. Rare, so it only has to be right.
 template <int D, int ND>

@@ -2,6 +2,8 @@
 
 Tolerances: see test_paged_gpu for the rounding of outputs, probabilities and sums."""
 
+import time
+
 import pytest
 import torch
 
@@ -10,6 +12,7 @@ from omniasr_b200 import kernels
 pytestmark = pytest.mark.gpu
 
 DEV = "cuda"
+NAN = float("nan")
 
 
 @pytest.mark.parametrize("heads,kv,dim,rows", [(8, 8, 128, 32), (16, 4, 128, 48), (16, 2, 64, 40), (32, 2, 128, 40), (8, 8, 512, 20), (8, 2, 256, 40)])
@@ -44,3 +47,92 @@ def test_a_key_far_above_a_long_tail(heads, kv, dim, rows, nats):
     worst = float(((got - want).abs() / bound).max())
     assert worst <= 1, f"{worst:.3g} times the bound"
     assert kernels.read_status() == 0
+
+
+@pytest.mark.parametrize("kind", ["own", "fp8"])
+@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 128), (4, 4, 64), (2, 2, 512), (4, 2, 256)])
+def test_one_nan_value_that_all_drafts_see(kind, heads, kv, dim):
+    """A NaN in one dim of an early value of long rows, five draft tokens: NaN in that dim, the other dims as without it, and
+    no column walks its 60,000 keys one after the other for it (which took tens of milliseconds)."""
+    g = torch.Generator(device=DEV).manual_seed(3)
+    n, page, t, rows = 60000, 32, 5, 4
+    k, v = (torch.randn(n // page, kv, page, dim, generator=g, device=DEV).to(torch.bfloat16) for _ in range(2))
+    ones = None
+    if kind == "fp8":
+        k, v = k.to(torch.float8_e4m3fn), v.to(torch.float8_e4m3fn)
+        ones = torch.full(k.shape[:3], 127, dtype=torch.uint8, device=DEV)
+    table = torch.arange(n // page, dtype=torch.int32, device=DEV).expand(rows, -1).contiguous()
+    q = torch.randn(rows * t, heads, dim, generator=g, device=DEV).to(torch.bfloat16)
+    run = lambda: kernels.paged_attention(q, k, v, table, torch.full((rows,), n - t + 1, device=DEV), dim**-0.5, tokens=t,  # noqa: E731
+                                          k_scale=ones, v_scale=ones)
+    clean = run()
+    v.view(torch.uint8 if kind == "fp8" else v.dtype)[0, :, 7, 5] = 0x7F if kind == "fp8" else NAN
+    run()
+    torch.cuda.synchronize()
+    start = time.perf_counter()
+    got = run()
+    torch.cuda.synchronize()
+    took = time.perf_counter() - start
+    same = torch.arange(dim, device=DEV) != 5
+    assert torch.equal(got[..., same], clean[..., same])
+    assert bool(torch.isnan(got[..., 5]).all())
+    assert kernels.read_status() == 0
+    assert took < 5e-3, f"{took:.4f} s"
+
+
+@pytest.mark.parametrize("kind", ["own", "fp8"])
+def test_drafts_after_many_keys_leave_a_hidden_nan_out(kind):
+    """The draft columns before a NaN are redone over all their keys."""
+    g = torch.Generator(device=DEV).manual_seed(4)
+    n, page, t, kv, dim = 60000, 32, 5, 2, 128
+    k, v = (torch.randn(n // page, kv, page, dim, generator=g, device=DEV).to(torch.bfloat16) for _ in range(2))
+    ones = None
+    if kind == "fp8":
+        k, v = k.to(torch.float8_e4m3fn), v.to(torch.float8_e4m3fn)
+        ones = torch.full(k.shape[:3], 127, dtype=torch.uint8, device=DEV)
+    kk, vv = (x.double().transpose(0, 1).reshape(kv, n, dim) for x in (k, v))
+    table = torch.arange(n // page, dtype=torch.int32, device=DEV)[None]
+    q = torch.randn(t, 4, dim, generator=g, device=DEV).to(torch.bfloat16)
+    v.view(torch.uint8 if kind == "fp8" else v.dtype)[-1, :, page - 2] = 0x7F if kind == "fp8" else NAN  # key n - 2
+    got = kernels.paged_attention(q, k, v, table, torch.full((1,), n - t + 1, device=DEV), dim**-0.5, tokens=t, k_scale=ones,
+                                  v_scale=ones).double()
+    for i in range(t - 2):
+        m = n - t + 1 + i
+        p = torch.softmax(q[i].double().view(kv, 2, dim) @ kk[:, :m].transpose(1, 2) * dim**-0.5, -1)
+        want, size = ((p @ x[:, :m]).view(4, dim) for x in (vv, vv.abs()))
+        assert float(((got[i] - want).abs() / (2.0**-8 * (want.abs() + size) + 2.0**-10 * size)).max()) <= 1
+    assert bool(torch.isnan(got[t - 2:]).all())
+    assert kernels.read_status() == 0
+
+
+@pytest.mark.parametrize("kind", ["own", "fp8"])
+def test_columns_redone_for_longer_than_a_wait_may_last(kind):
+    """Draft columns over a million and a half keys (a few pages, over and over) with a hidden NaN behind them, and short rows
+    after them: the redo takes seconds, and no wait gives up."""
+    g = torch.Generator(device=DEV).manual_seed(5)
+    page, t, kv, dim, real, width, short = 64, 5, 1, 128, 8, 24000, 300
+    k, v = (torch.randn(real + 1, kv, page, dim, generator=g, device=DEV).to(torch.bfloat16) for _ in range(2))
+    ones = None
+    if kind == "fp8":
+        k, v = k.to(torch.float8_e4m3fn), v.to(torch.float8_e4m3fn)
+        ones = torch.full(k.shape[:3], 127, dtype=torch.uint8, device=DEV)
+    table = (torch.arange(width, dtype=torch.int32, device=DEV) % real).expand(1 + short, -1).contiguous()
+    table[0, width - 1] = real
+    n = width * page
+    lengths = torch.full((1 + short,), 3 * page, device=DEV)
+    lengths[0] = n - t + 1
+    kk, vv = (torch.cat([x[i % real] if i < width - 1 else x[real] for i in range(width - 2 * real, width)], 1).double() for x in (k, v))
+    copies = torch.ones(kk.size(1), dtype=torch.float64, device=DEV)  # of each of these keys in the row
+    copies[:real * page] += width // real - 2
+    q = torch.randn((1 + short) * t, 4, dim, generator=g, device=DEV).to(torch.bfloat16)
+    v.view(torch.uint8 if kind == "fp8" else v.dtype)[real, :, page - 1] = 0x7F if kind == "fp8" else NAN
+    got = kernels.paged_attention(q, k, v, table, lengths, dim**-0.5, tokens=t, k_scale=ones, v_scale=ones).double()
+    assert kernels.read_status() == 0
+    assert bool(torch.isnan(got[t - 1]).all()) and bool(torch.isfinite(got[t:]).all())
+    for i in range(t - 1):
+        m = kk.size(1) - t + 1 + i
+        x = q[i].double() @ kk[0, :m].t() * dim**-0.5 + copies[:m].log()
+        p = torch.softmax(x, -1)
+        want, size = p @ vv[0, :m], p @ vv[0, :m].abs()
+        # (fp32 sums over 1.5 million keys one after the other: 2^-24 of the sum each, in a direction that wanders)
+        assert float(((got[i] - want).abs() / (2.0**-8 * (want.abs() + size) + 2.0**-10 * size)).max()) <= 1
