@@ -58,6 +58,7 @@ constexpr uint32_t kLayoutSw64 = 4;  // 64-byte swizzle (the TMA's CU_TENSOR_MAP
 constexpr int kCtlBytes = 6400;    // control block (below)
 constexpr float kRaise = 8.f;      // log2: a weight may reach 2^8 before its column's maximum is raised
 constexpr float kHead8 = 4.f;      // e4m3: the maximum kept this far (log2) below the largest exponent seen
+constexpr float kNone = -1e30f;    // bf16: the maximum of a column whose scores so far are all -inf
 constexpr float kBelow = 64.f;     // bf16: a unit starts from maximum 0 unless its scores lie 2^64 below
 
 template <bool FP8, int DIM, int NQT>
@@ -800,6 +801,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           else x[j] = sv[j] * p.qscale;
         }
         mbar_arrive(&ctl.s_free[b]);  // (after the last read of the queries' factors and the scales, too)
+        bool over = FP8 && first;
+        if (!FP8 && first) {  // a unit starts from maximum 0 unless its scores lie far below; -inf is such a score
+#pragma unroll
+          for (int j = 0; j < NQT; ++j) over |= x[j] < -kBelow && j < ncol && key < need;
+        }
         if (NQT > ncol || (t + 1) * BN > lim0) {  // spare columns, or keys that some column does not see
           int tt = 0, g = g0;
 #pragma unroll
@@ -811,16 +817,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        bool over = FP8 && first;
 #pragma unroll
-        for (int j = 0; j < NQT; ++j) {
-          if (FP8) {
-            over |= x[j] > m[j] + kRaise;
-          } else {
-            over |= x[j] > m[j] + kRaise;
-            if (first) over |= x[j] > -INFINITY && x[j] < m[j] - kBelow;
-          }
-        }
+        for (int j = 0; j < NQT; ++j) over |= x[j] > m[j] + kRaise;
         const bool saw = abort_flag != 0;
         if (sync_or(bar, 128, over || saw)) {
           float v[NQT];
@@ -841,9 +839,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int j = 0; j < NQT; ++j) {
             const float top = fmaxf(fmaxf(ctl.red[b][0][j], ctl.red[b][1][j]), fmaxf(ctl.red[b][2][j], ctl.red[b][3][j]));
             float mn = m[j];
-            if (top != -INFINITY) {
-              if (FP8) mn = first ? top - kHead8 : (top > m[j] + kRaise ? top - kHead8 : m[j]);
-              else mn = first ? top : fmaxf(m[j], top);
+            if (FP8) {
+              if (top != -INFINITY) mn = first ? top - kHead8 : (top > m[j] + kRaise ? top - kHead8 : m[j]);
+            } else {
+              // (No score but -inf yet: below whatever comes, and -inf less it is -inf.)
+              mn = fmaxf(first ? kNone : m[j], top);
             }
             scl[j] = first ? 1.f : ex2(m[j] - mn);
             any |= scl[j] != 1.f;

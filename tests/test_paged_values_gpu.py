@@ -7,12 +7,13 @@ import time
 import pytest
 import torch
 
+import paged_util as pu
 from omniasr_b200 import kernels
 
 pytestmark = pytest.mark.gpu
 
 DEV = "cuda"
-NAN = float("nan")
+NAN, INF = float("nan"), float("inf")
 
 
 @pytest.mark.parametrize("heads,kv,dim,rows", [(8, 8, 128, 32), (16, 4, 128, 48), (16, 2, 64, 40), (32, 2, 128, 40), (8, 8, 512, 20), (8, 2, 256, 40)])
@@ -136,3 +137,29 @@ def test_columns_redone_for_longer_than_a_wait_may_last(kind):
         want, size = p @ vv[0, :m], p @ vv[0, :m].abs()
         # (fp32 sums over 1.5 million keys one after the other: 2^-24 of the sum each, in a direction that wanders)
         assert float(((got[i] - want).abs() / (2.0**-8 * (want.abs() + size) + 2.0**-10 * size)).max()) <= 1
+
+
+@pytest.mark.parametrize("heads,kv,dim,page", [(4, 2, 128, 16), (16, 1, 128, 64), (4, 4, 512, 64), (8, 1, 64, 16), (4, 1, 256, 128)])
+def test_minus_infinity_before_scores_far_below_zero(heads, kv, dim, page):
+    """The first 256 keys score -inf, the later ones about -250: a column's maximum starts at the first score that is one. (The
+    rows are short enough to stay whole: each softmax group meets -inf alone in its first tile.)"""
+    g = torch.Generator().manual_seed(2)
+    lens = [600, 300, 520]
+    table, pool = pu.table_for(lens, page, g)
+    k, v, _, _, _, _ = pu.cache(pool, kv, page, dim, "own", g)
+    q = torch.randn(len(lens), heads, dim, generator=g).to(torch.bfloat16)
+    q[:, :, 3], q[:, :, 4] = 1.0, 16.0
+    for r, n in enumerate(lens):
+        for j in range(n):
+            k[int(table[r, j // page]), :, j % page, 4] = -16.0
+            if j < 256:
+                k[int(table[r, j // page]), :, j % page, 3] = -INF
+    length = torch.tensor(lens)
+    want = pu.paged(q, k, v, table, length, 1.0, 1)
+    size = pu.paged(q, k, v.abs(), table, length, 1.0, 1)
+    got = kernels.paged_attention(q.to(DEV), k.to(DEV), v.to(DEV), table.to(DEV), length.to(DEV), 1.0).double().cpu()
+    # (fp32 scores of about 370 in log2 units: a relative 2^-24 of them is 2^-15 of a weight)
+    bound = 2.0**-8 * (want.abs() + size) + 2.0**-10 * size
+    worst = float(((got - want).abs() / bound).nan_to_num(INF).max())
+    assert worst <= 1, f"{worst:.3g} times the bound"
+    assert kernels.read_status() == 0
