@@ -90,10 +90,10 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const PagedAttnArgs a, 
   const int c0 = chunk * sp.cols;
   const int lane = threadIdx.x % L, team = threadIdx.x / L;
   const int64_t cap = (int64_t)a.table_width * a.c.page;
-  const int64_t len = a.lengths[b];
-  int64_t need = len + a.tokens - 1;
-  if (threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0 && (len < 0 || need > cap)) raise_status(a.status, kStatusIndex);
-  need = need < 0 ? 0 : (need > cap ? cap : need);
+  const int64_t given = a.lengths[b], len = min(given, cap);  // (past the table: reported, and no key past it)
+  if (threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0 && (given < 0 || given > cap - (a.tokens - 1)))
+    raise_status(a.status, kStatusIndex);
+  const int64_t need = max((int64_t)0, min(cap, len + a.tokens - 1));
 
   float q[NC][NV][8];
   int64_t lim[NC];  // keys column c sees

@@ -456,13 +456,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < each; ++i) {
       const int b = tid * each + i;
       if (b >= p.rows) break;
-      const int64_t raw = p.lengths[b], most = raw + p.tokens - 1;
-      if (blockIdx.x == 0 && (raw < 0 || most > p.cap)) raise_status(p.status, kStatusIndex);
-      // The keys of the row's last query; a length out of range is clamped (and was reported).
-      const int64_t lim = raw < -(int64_t)p.tokens ? -(int64_t)p.tokens : (raw > p.cap ? (int64_t)p.cap : raw);
-      len[b] = (int)lim;
-      const int64_t need = most < 0 ? 0 : (most > p.cap ? (int64_t)p.cap : most);
-      const int nt = (int)((need + BN - 1) / BN);
+      const int64_t raw = p.lengths[b];
+      if (blockIdx.x == 0 && (raw < 0 || raw > p.cap - (p.tokens - 1))) raise_status(p.status, kStatusIndex);
+      // The keys of the row's last query; a length out of range is clamped (and was reported), so that len + tokens is an int.
+      const int64_t high = min(p.cap, 0x7fffffff - p.tokens);
+      len[b] = (int)max(-(int64_t)p.tokens, min(raw, high));
+      const int nt = (max(0, min(p.cap, len[b] + p.tokens - 1)) + BN - 1) / BN;
       most_tiles = max(most_tiles, nt);
       mine += nt * per_row;
       pre[b + 1] = mine;

@@ -163,3 +163,38 @@ def test_minus_infinity_before_scores_far_below_zero(heads, kv, dim, page):
     worst = float(((got - want).abs() / bound).nan_to_num(INF).max())
     assert worst <= 1, f"{worst:.3g} times the bound"
     assert kernels.read_status() == 0
+
+
+def test_rows_of_two_billion_keys():
+    """A table of one page 16.8 million times over: keys up to the largest that a row may have, and lengths past it, which are
+    reported and stay within the table."""
+    g = torch.Generator(device=DEV).manual_seed(6)
+    page, dim, t = 128, 64, 2
+    width = 0x7fffff00 // page
+    k, v = (torch.randn(1, 1, page, dim, generator=g, device=DEV).to(torch.bfloat16) for _ in range(2))
+    q = torch.randn(t, 2, dim, generator=g, device=DEV).to(torch.bfloat16)
+    table = torch.zeros(1, width, dtype=torch.int32, device=DEV)
+    run = lambda n: kernels.paged_attention(q, k, v, table, torch.tensor([n], device=DEV), dim**-0.5, tokens=t).double()  # noqa: E731
+    got = run(width * page - 1)
+    assert kernels.read_status() == 0
+    p = torch.softmax(q.double() @ k[0, 0].double().t() * dim**-0.5, -1)
+    want, size = p @ v[0, 0].double(), p @ v[0, 0].double().abs()
+    # Beside the usual rounding, sums of 57,000 tiles per block, each added to 2^-24 of the sum at most: 57000 x 2^-24 < 2^-8.
+    assert float(((got - want).abs() / (2.0**-8 * (want.abs() + 2 * size) + 2.0**-10 * size)).max()) <= 1
+    for n in (width * page, 2**31 - 1, 2**31, 2**40, 2**63 - 1):
+        run(n)
+        assert kernels.read_status() == 1
+
+
+@pytest.mark.parametrize("dtype,dim,page", [(torch.bfloat16, 64, 16), (torch.float32, 64, 16), (torch.bfloat16, 32, 5)])
+def test_lengths_at_the_ends_of_their_type(dtype, dim, page):
+    g = torch.Generator(device=DEV).manual_seed(7)
+    k, v = (torch.randn(3, 1, page, dim, generator=g, device=DEV).to(dtype) for _ in range(2))
+    q = torch.randn(6, 2, dim, generator=g, device=DEV).to(dtype)
+    table = torch.zeros(3, 2, dtype=torch.int32, device=DEV)
+    good = kernels.paged_attention(q, k, v, table, torch.tensor([3, 4, 2], device=DEV), 0.1, tokens=2)
+    assert kernels.read_status() == 0
+    for n in (2**63 - 1, -2**63):
+        out = kernels.paged_attention(q, k, v, table, torch.tensor([3, n, 2], device=DEV), 0.1, tokens=2)
+        assert kernels.read_status() == 1
+        assert torch.equal(out[:2], good[:2]) and torch.equal(out[4:], good[4:])
