@@ -40,6 +40,11 @@ struct Shape {
   static constexpr int BYTES = (BM * (LD + LP) + STAGES * KV) * 4;
 };
 
+OMNI_DEV bool offsets_ok(const PackedArgs& a, int s) {
+  const int64_t qa = a.q_offsets[s], qb = a.q_offsets[s + 1], ka = a.k_offsets[s], kb = a.k_offsets[s + 1];
+  return qa >= 0 && qb >= qa && qb <= a.q_tokens && ka >= 0 && kb >= ka && kb <= a.k_tokens;
+}
+
 // Tile `slot` of the packed queries -> sequence and first query: the sequences' tile counts, summed 32 at a time by one
 // warp. Returns the sequence, or -1 past the last tile.
 OMNI_DEV int find_tile(const int64_t* offsets, int seqs, int bm, int slot, int lane, int* tile) {
@@ -141,6 +146,10 @@ __global__ void __launch_bounds__(Shape<T, D, BM_>::THREADS) packed_kernel(const
   __shared__ int s_seq, s_tile;
   grid_launch_dependents();
   grid_dependency_wait();
+  if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 && blockIdx.z == 0) {  // one CTA looks all offsets over
+    for (int s = threadIdx.x; s < a.seqs; s += S::THREADS)
+      if (!offsets_ok(a, s)) raise_status(a.status, kStatusIndex);
+  }
   if (threadIdx.x < 32) {
     int tile = 0;
     const int seq = find_tile(a.q_offsets, a.seqs, BM, blockIdx.x, threadIdx.x, &tile);
@@ -154,10 +163,7 @@ __global__ void __launch_bounds__(Shape<T, D, BM_>::THREADS) packed_kernel(const
   const int h = blockIdx.y, kvh = h / (a.heads / a.kv_heads);
   const int64_t qa = a.q_offsets[s_seq], qb = a.q_offsets[s_seq + 1];
   const int64_t ka = a.k_offsets[s_seq], kb = a.k_offsets[s_seq + 1];
-  if (qa < 0 || qb > a.q_tokens || ka < 0 || kb > a.k_tokens || kb < ka) {
-    if (threadIdx.x == 0) raise_status(a.status, kStatusIndex);
-    return;
-  }
+  if (!offsets_ok(a, s_seq)) return;
   const int64_t q0 = qa + (int64_t)s_tile * BM;
   const int rows = (int)min((int64_t)BM, qb - q0);
   // Row r of the tile sees keys [0, lim0 + r) of the sequence.
@@ -331,7 +337,7 @@ __global__ void __launch_bounds__(256) join_kernel(const PackedArgs a, const Par
     bool hit = false;
     if (s < a.seqs) {
       const int64_t qa = a.q_offsets[s], qb = a.q_offsets[s + 1], ka = a.k_offsets[s], kb = a.k_offsets[s + 1];
-      hit = qa <= row && row < qb && qa >= 0 && qb <= a.q_tokens && ka >= 0 && kb <= a.k_tokens && kb >= ka;
+      hit = qa <= row && row < qb && offsets_ok(a, s);
       if (hit) lim = row - qa + 1 + (kb - ka) - (qb - qa);
     }
     const unsigned who = __ballot_sync(0xffffffffu, hit);

@@ -219,3 +219,14 @@ def test_rows_redone_for_longer_than_a_wait_may_last(dim):
     want, size = plain(q, k, v, new, keys)
     rest = torch.arange(sum(new), device=DEV) != 127
     check(got[rest], want[rest], size[rest])
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.float32, 64), (torch.bfloat16, 32), (torch.bfloat16, 64), (torch.bfloat16, 512)])
+@pytest.mark.parametrize("tokens", [10, 5000])
+def test_offsets_that_descend_are_reported(dtype, dim, tokens):
+    q = torch.zeros(tokens, 2, dim, dtype=dtype, device=DEV)
+    good = torch.tensor([0, 4, 4, tokens], device=DEV)
+    kernels.packed_attention(q, q, q, good)
+    assert kernels.read_status() == 0
+    kernels.packed_attention(q, q, q, torch.tensor([0, 6, 4, tokens], device=DEV), good)
+    assert kernels.read_status() == 1
