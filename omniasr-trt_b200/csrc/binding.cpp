@@ -47,6 +47,9 @@ void same_device(const char* name, const at::Tensor& a, std::initializer_list<co
     if (t->device() != a.device()) refuse(name, "tensors must be on one device");
 }
 
+// The stride of a dimension; nothing reads that of an extent of one, where PyTorch leaves any number.
+int64_t stride_of(const at::Tensor& t, int64_t dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }
+
 struct Pages {
   const void *k, *v, *ks, *vs;
   int64_t pages, kv, page, dim, sp, sh, st;
@@ -54,9 +57,12 @@ struct Pages {
 };
 
 Pages pages_of(const char* name, const at::Tensor& k, const at::Tensor& v, const Opt& ks, const Opt& vs, int dtype) {
-  if (k.dim() != 4 || v.sizes() != k.sizes() || v.strides() != k.strides() || k.stride(3) != 1 || v.scalar_type() != k.scalar_type())
+  bool same = k.dim() == 4 && v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type();
+  for (int64_t i = 0; same && i < 3; ++i) same = stride_of(k, i) == stride_of(v, i);
+  if (!same || k.stride(3) != 1 || v.stride(3) != 1)
     refuse(name, "k and v pages must be [pages, kv_heads, page, D] views of one dtype with the same strides and unit stride in D");
-  Pages p{k.data_ptr(), v.data_ptr(), nullptr, nullptr, k.size(0), k.size(1), k.size(2), k.size(3), k.stride(0), k.stride(1), k.stride(2), 0};
+  Pages p{k.data_ptr(), v.data_ptr(), nullptr, nullptr, k.size(0), k.size(1), k.size(2), k.size(3),
+          stride_of(k, 0), stride_of(k, 1), stride_of(k, 2), 0};
   if (k.scalar_type() == at::kFloat8_e4m3fn) {
     for (const Opt* s : {&ks, &vs}) {
       if (!*s || (*s)->scalar_type() != at::kByte || (*s)->sizes() != k.sizes().slice(0, 3) || !(*s)->is_contiguous())
@@ -101,7 +107,7 @@ at::Tensor paged_rope_kv(const at::Tensor& qkv, const at::Tensor& cs_in, const a
   const at::Tensor cs = cs_in.scalar_type() == at::kFloat && cs_in.is_contiguous() ? cs_in : cs_in.to(at::kFloat).contiguous();
   const at::Tensor pos = index_of(pos_in), slots = index_of(slots_in);
   done("omniasr_paged_rope_kv",
-       omniasr_paged_rope_kv(qkv.data_ptr(), qkv.stride(0), cs.data_ptr<float>(), cs.size(0), pos.data_ptr<int64_t>(),
+       omniasr_paged_rope_kv(qkv.data_ptr(), stride_of(qkv, 0), cs.data_ptr<float>(), cs.size(0), pos.data_ptr<int64_t>(),
                              slots.data_ptr<int64_t>(), q.data_ptr(), const_cast<void*>(p.k), const_cast<void*>(p.v),
                              const_cast<void*>(p.ks), const_cast<void*>(p.vs), p.pages, (int)p.page, p.sp, p.sh, p.st, (int)n,
                              (int)heads, (int)kv_heads, (int)p.dim, dtype, p.type, status_of(status), stream_of(stream)));
@@ -182,8 +188,8 @@ py::object packed_attention(const at::Tensor& q, const at::Tensor& k, const at::
   at::Tensor out = at::empty({tq, heads, dim}, q.options());
   const double s = scale ? *scale : 1.0 / std::sqrt((double)dim);
   done("omniasr_packed_attention",
-       omniasr_packed_attention(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-                                v.stride(1), out.data_ptr(), qo.data_ptr<int64_t>(), ko.data_ptr<int64_t>(), tq, tk, (int)seqs, (int)heads,
+       omniasr_packed_attention(q.data_ptr(), stride_of(q, 0), stride_of(q, 1), k.data_ptr(), stride_of(k, 0), stride_of(k, 1),
+                                v.data_ptr(), stride_of(v, 0), stride_of(v, 1), out.data_ptr(), qo.data_ptr<int64_t>(), ko.data_ptr<int64_t>(), tq, tk, (int)seqs, (int)heads,
                                 (int)kv, (int)dim, (float)s, dtype, ws->data_ptr(), ws->numel(), status_of(status), stream_of(stream)));
   return py::cast(out);
 }

@@ -230,3 +230,27 @@ def test_offsets_that_descend_are_reported(dtype, dim, tokens):
     assert kernels.read_status() == 0
     kernels.packed_attention(q, q, q, torch.tensor([0, 6, 4, tokens], device=DEV), good)
     assert kernels.read_status() == 1
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.float32, 64), (torch.bfloat16, 32), (torch.bfloat16, 128), (torch.bfloat16, 512)])
+def test_strides_of_extents_of_one(dtype, dim):
+    """The stride of an extent of one is not read, so it may be any number."""
+    g = torch.Generator(device=DEV).manual_seed(10)
+    q, k, v = (torch.randn(1, 1, dim, generator=g, device=DEV).to(dtype) for _ in range(3))
+    odd = [torch.as_strided(t, t.shape, (3, 7, 1)) for t in (q, k, v)]
+    off = torch.tensor([0, 1], device=DEV)
+    assert torch.equal(kernels.packed_attention(*odd, off), v)
+    pages = [torch.as_strided(t.view(1, 1, 1, dim), (1, 1, 1, dim), (5, 3, 1, 1)) for t in (k, v)]
+    table, one = torch.zeros(1, 1, dtype=torch.int32, device=DEV), torch.ones(1, dtype=torch.int64, device=DEV)
+    assert torch.equal(kernels.paged_attention(q, *pages, table, one, 0.1), v)
+    kb, vb = kernels.paged_kv_read(*pages, table, off, 1)
+    assert torch.equal(kb, k) and torch.equal(vb, v)
+    cs = torch.zeros(1, dim // 2, 2, device=DEV)
+    cs[..., 0] = 1
+    qkv = torch.cat([q, k, v], -1).view(1, 3 * dim)
+    fresh = [torch.zeros(1, 1, 1, dim, dtype=dtype, device=DEV) for _ in range(2)]
+    into = [torch.as_strided(t, t.shape, (5, 3, 1, 1)) for t in fresh]
+    zero = torch.zeros(1, dtype=torch.int64, device=DEV)
+    got = kernels.paged_rope_kv(torch.as_strided(qkv, qkv.shape, (1, 1)), cs, zero, *into, zero, 1, 1)
+    assert torch.equal(got, q) and torch.equal(fresh[0].view(-1), k.view(-1)) and torch.equal(fresh[1].view(-1), v.view(-1))
+    assert kernels.read_status() == 0
