@@ -336,12 +336,8 @@ template <typename T, int D, int NQB, bool GATHER>
 cudaError_t launch_split_t(const SplitPlan& p, const SplitArgs& a, int groups, cudaStream_t stream) {
   using S = SplitShape<T, D>;
   auto kern = split_attention_kernel<T, D, NQB, GATHER>;
-  static bool configured = false;
-  if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmemBytes);
-    if (e != cudaSuccess) return e;
-    configured = true;
-  }
+  static PerDevice configured;
+  if (const cudaError_t e = allow_smem(kern, S::kSmemBytes, configured)) return e;
   dim3 grid((unsigned)(groups * p.qblocks), (unsigned)a.heads, (unsigned)p.splits);
   kern<<<grid, S::kThreads, S::kSmemBytes, stream>>>(a);
   return cudaGetLastError();

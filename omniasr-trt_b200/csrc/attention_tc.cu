@@ -1490,12 +1490,8 @@ cudaError_t launch_tc_pass(const void* k, const void* v, int64_t cache_rows, int
   const int ci = p.nq <= 1 ? 0 : p.nq <= 2 ? 1 : p.nq <= 4 ? 2 : p.nq <= 8 ? 3 : 4;
   const Kern kern = table[di][ci];
   const int bytes = di == 0 ? Smem<6, 128>::BYTES : Smem<4, 512>::BYTES;
-  static bool configured[2][5] = {};
-  if (!configured[di][ci]) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != cudaSuccess) return e;
-    configured[di][ci] = true;
-  }
+  static PerDevice configured[2][5];
+  if (const cudaError_t e = allow_smem(kern, bytes, configured[di][ci])) return e;
   // Programmatic dependent launch: the set-up above griddepcontrol.wait overlaps the previous kernel.
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)p.grid);

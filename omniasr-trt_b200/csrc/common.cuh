@@ -13,6 +13,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "per_device.h"
+
 #define OMNI_DEV __device__ __forceinline__
 
 namespace omni {
@@ -182,6 +184,16 @@ OMNI_DEV float ex2(float x) {
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
+
+// Lets the kernel take `bytes` of dynamic shared memory on the current device; `done` is a static of the launcher.
+template <typename Kern>
+inline cudaError_t allow_smem(Kern kern, int bytes, PerDevice& done) {
+  int device = 0;
+  const cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  return (cudaError_t)done.once(
+      device, [&] { return (int)cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
+}
 
 // Launches `kern` as a programmatic dependent of the stream's previous kernel: its blocks may start while that
 // kernel drains, and must execute griddepcontrol.wait before reading anything an earlier kernel wrote.

@@ -371,12 +371,8 @@ __global__ void __launch_bounds__(256) join_kernel(const PackedArgs a, const Par
 template <typename T, int D, int BM>
 cudaError_t launch_t(const PackedArgs& a, const Parts& parts, cudaStream_t s) {
   using S = Shape<T, D, BM>;
-  static bool configured = false;
-  if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(packed_kernel<T, D, BM>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES);
-    if (e != cudaSuccess) return e;
-    configured = true;
-  }
+  static PerDevice configured;
+  if (const cudaError_t e = allow_smem(packed_kernel<T, D, BM>, S::BYTES, configured)) return e;
   // At most this many tiles: a sequence's last tile may be partly filled.
   const int64_t tiles = a.q_tokens / BM + a.seqs;
   const cudaError_t e = launch_dependent(packed_kernel<T, D, BM>, dim3((unsigned)tiles, (unsigned)a.heads, (unsigned)parts.n),

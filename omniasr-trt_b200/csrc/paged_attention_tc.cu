@@ -1325,12 +1325,8 @@ bool page_map(CUtensorMap* map, const void* base, const PageCache& c) {
 template <bool FP8, int DIM, int NQT>
 cudaError_t launch_t(const CUtensorMap& k, const CUtensorMap& v, const Params& p, int grid, cudaStream_t stream) {
   using C = Cfg<FP8, DIM, NQT>;
-  static bool configured = false;
-  if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(paged_tc_kernel<FP8, DIM, NQT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES);
-    if (e != cudaSuccess) return e;
-    configured = true;
-  }
+  static PerDevice configured;
+  if (const cudaError_t e = allow_smem(paged_tc_kernel<FP8, DIM, NQT>, C::BYTES, configured)) return e;
   return launch_dependent(paged_tc_kernel<FP8, DIM, NQT>, dim3(grid), dim3(kThreads), (size_t)C::BYTES, stream, k, v, p);
 }
 

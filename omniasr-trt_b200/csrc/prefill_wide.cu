@@ -760,13 +760,8 @@ cudaError_t launch_prefill_wide(const PrefillArgs& a, cudaStream_t stream) {
       !make_map(&km, a.k, a.batch, a.heads, a.width, a.k_sb, a.k_sh, a.k_sw) ||
       !make_map(&vm, a.v, a.batch, a.heads, a.width, a.v_sb, a.v_sh, a.v_sw))
     return cudaErrorInvalidValue;
-  static bool configured = false;
-  if (!configured) {
-    cudaError_t e =
-        cudaFuncSetAttribute(prefill_wide_kernel<Sched, 512>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
-    if (e != cudaSuccess) return e;
-    configured = true;
-  }
+  static PerDevice configured;
+  if (const cudaError_t e = allow_smem(prefill_wide_kernel<Sched, 512>, SMEM_BYTES, configured)) return e;
   Params p;
   p.batch = a.batch;
   p.heads = a.heads;
@@ -795,13 +790,8 @@ cudaError_t launch_packed_wide_d(const PackedArgs& a, cudaStream_t stream) {
   const int positions = BM / (a.heads / a.kv_heads);
   CUtensorMap qm, km, vm;
   if (!packed_maps(a, positions, VK, &qm, &km, &vm)) return cudaErrorNotSupported;
-  static bool configured = false;
-  if (!configured) {
-    cudaError_t e =
-        cudaFuncSetAttribute(prefill_wide_kernel<PackedSrc, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
-    if (e != cudaSuccess) return e;
-    configured = true;
-  }
+  static PerDevice configured;
+  if (const cudaError_t e = allow_smem(prefill_wide_kernel<PackedSrc, D>, SMEM_BYTES, configured)) return e;
   Params p{};
   p.qscale = a.scale * kLog2e;
   p.out = reinterpret_cast<__nv_bfloat16*>(a.out);

@@ -682,12 +682,8 @@ bool make_map_2d(CUtensorMap* map, const void* base, int64_t cols, int64_t rows,
 template <int NT, int MODE>
 cudaError_t launch_t(const CUtensorMap& wm, const CUtensorMap& xm, const GemmArgs& a, cudaStream_t stream) {
   using L = Layout<NT>;
-  static bool configured = false;
-  if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(wgemm_kernel<NT, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::BYTES);
-    if (e != cudaSuccess) return e;
-    configured = true;
-  }
+  static PerDevice configured;
+  if (const cudaError_t e = allow_smem(wgemm_kernel<NT, MODE>, L::BYTES, configured)) return e;
   if (a.cluster <= 1)
     return launch_dependent(wgemm_kernel<NT, MODE>, dim3((unsigned)a.grid), dim3(THREADS), (size_t)L::BYTES, stream,
                             wm, xm, a);
