@@ -31,6 +31,7 @@ the built library every function raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -83,6 +84,25 @@ def read_status(device=None, clear: bool = True) -> int:
         for key in [k for k in _GEMM_WS if k[0] == index]:
             _GEMM_WS_RETIRED.append(_GEMM_WS.pop(key))
     return value
+
+
+_current = getattr(torch._C, "_cuda_getDevice", None)  # (torch.cuda.current_device() takes half a microsecond more)
+
+
+def _on_its_device(fn):
+    """Makes the device of the call's first tensor the current one while it runs: kernels are launched, and a stream's handle
+    and what is allocated mean, on the current device."""
+    first = fn.__code__.co_varnames[0]  # its name, for a call by keywords
+
+    @functools.wraps(fn)
+    def call(*args, **kwargs):
+        device = getattr(args[0] if args else kwargs.get(first), "device", None)
+        if device is None or device.type != "cuda" or device.index == _current():
+            return fn(*args, **kwargs)
+        with torch.cuda.device(device):
+            return fn(*args, **kwargs)
+
+    return call
 
 
 def _ptr(t: torch.Tensor | None) -> ctypes.c_void_p | None:
@@ -139,6 +159,7 @@ def _attn_workspace(nbytes: int, device: torch.device, stream: int | None = None
     return ws
 
 
+@_on_its_device
 def rope_kv(qkv: torch.Tensor, cs: torch.Tensor, pos: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
             heads: int, slots: torch.Tensor | None = None, cache_pos: torch.Tensor | None = None) -> torch.Tensor:
     """``qkv`` [N, 3*H*D] (q|k|v of N tokens), ``cs`` [P, D/2, 2] fp32, ``pos`` [N]; ``k_cache``/``v_cache``
@@ -164,6 +185,7 @@ def rope_kv(qkv: torch.Tensor, cs: torch.Tensor, pos: torch.Tensor, k_cache: tor
     return q
 
 
+@_on_its_device
 def decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
                      keys: int, scale: float, block: int | None = None, warps: int | None = None,
                      stages: int | None = None, programs: int | None = None) -> torch.Tensor:
@@ -188,6 +210,7 @@ def decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     return out
 
 
+@_on_its_device
 def draft_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
                     tokens: int, keys: int, scale: float, **launch) -> torch.Tensor:
     """Draft verification: ``q`` [B*T, H, D], row b's T queries at rows b*T .. b*T+T-1; query i of row b attends
@@ -214,6 +237,7 @@ def draft_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     return out
 
 
+@_on_its_device
 def beam_attention(q: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor, ctx_len: torch.Tensor, kg: torch.Tensor,
                    vg: torch.Tensor, ptr: torch.Tensor, gen_len: torch.Tensor, beams: int, ctx_keys: int,
                    scale: float) -> torch.Tensor:
@@ -247,6 +271,7 @@ def beam_attention(q: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor, ctx_len:
     return out
 
 
+@_on_its_device
 def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | None = None) -> torch.Tensor:
     """Causal attention of prefilled contexts: ``q``/``k``/``v`` [B, H, W, D] (any strides, unit stride in D; k and
     v typically cache views); query w sees keys [0, w]. Returns [B, H, W, D] in q's dtype -- a view of a
@@ -279,6 +304,7 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: 
 _PREFILL_GROUP = 16  # query positions per group of the grouped prefill
 
 
+@_on_its_device
 def prefill_attention_grouped(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                               scale: float | None = None) -> torch.Tensor:
     """bf16 head_dim 512: every row's queries as groups of 16 consecutive positions on the tensor-core decode pass
@@ -315,6 +341,7 @@ def _vec(t: torch.Tensor, dtype: torch.dtype, name: str) -> torch.Tensor:
     return t
 
 
+@_on_its_device
 def propose(out: torch.Tensor, draft: torch.Tensor, draft_len: torch.Tensor, last: torch.Tensor,
             first: torch.Tensor, nxt: torch.Tensor, start: torch.Tensor, tokens: int, ngram: int, behind: int,
             ahead: int, reach: tuple, self_window: int, self_min: int) -> tuple[torch.Tensor, torch.Tensor]:
@@ -343,6 +370,7 @@ def propose(out: torch.Tensor, draft: torch.Tensor, draft_len: torch.Tensor, las
     return prop, use_draft
 
 
+@_on_its_device
 def accept(tokens: torch.Tensor, nxt: torch.Tensor, out: torch.Tensor, tok: torch.Tensor, last: torch.Tensor,
            done: torch.Tensor, draft_next: torch.Tensor, start: torch.Tensor, use_draft: torch.Tensor, limit: int,
            eos: int) -> None:
@@ -366,6 +394,7 @@ def accept(tokens: torch.Tensor, nxt: torch.Tensor, out: torch.Tensor, tok: torc
               int(eos), _ptr(status_word(out.device)), _stream(out.device))
 
 
+@_on_its_device
 def beam_select(logp: torch.Tensor, score: torch.Tensor, ended: torch.Tensor, count: torch.Tensor, tok: torch.Tensor,
                 hist: torch.Tensor, ptr: torch.Tensor, k_step: torch.Tensor, ctx: torch.Tensor, gdone: torch.Tensor,
                 beams: int, length_norm: bool, eos: int, pad: int, limit: int) -> None:
@@ -413,6 +442,7 @@ def _gemm_workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     return ws
 
 
+@_on_its_device
 def decode_gemm(x: torch.Tensor, w: torch.Tensor, mode: str = "store", residual: torch.Tensor | None = None,
                 out: torch.Tensor | None = None) -> torch.Tensor:
     """The decoder step's weight GEMMs for at most 64 token rows (bf16): ``x @ w.t()`` ("store"),
@@ -443,6 +473,7 @@ def decode_gemm(x: torch.Tensor, w: torch.Tensor, mode: str = "store", residual:
     return out
 
 
+@_on_its_device
 def decode_gemm_rope(x: torch.Tensor, w: torch.Tensor, cs: torch.Tensor, pos: torch.Tensor, k_cache: torch.Tensor,
                      v_cache: torch.Tensor, heads: int, slots: torch.Tensor | None = None,
                      cache_pos: torch.Tensor | None = None) -> torch.Tensor:
@@ -475,6 +506,7 @@ def decode_gemm_rope(x: torch.Tensor, w: torch.Tensor, cs: torch.Tensor, pos: to
     return q
 
 
+@_on_its_device
 def reorder_gather(src: torch.Tensor, parent: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
     """``out[r] = src[parent[r]]`` along dim 0, byte-exact (``torch.index_select(src, 0, parent)``); each row of
     ``src`` / ``out`` must be contiguous. ``out`` (optional) must not overlap ``src``."""
@@ -509,17 +541,35 @@ def _binding():
     return _native
 
 
+class _Elsewhere:
+    """The native calls, on a device that is not the current one."""
+
+    def __init__(self, index: int):
+        self._index = index
+
+    def __getattr__(self, name: str):
+        fn = getattr(_binding(), name)
+
+        def call(*args):
+            with torch.cuda.device(self._index):
+                return fn(*args)
+
+        return call
+
+
 def _context(device: torch.device) -> tuple:
-    """(the device's status word, the current stream, the stream's workspace or None) for the native calls, which refuse
-    tensors that are on no CUDA device."""
+    """(the native calls on the device, its status word, its current stream, the stream's workspace or None); tensors that are
+    on no CUDA device are refused by the calls."""
     index = device.index
     if index is None:
-        return 0, 0, None
+        return _binding(), 0, 0, None
     word = _status.get(index)
     if word is None:
         word = status_word(index)
     stream = _raw_stream(index)
-    return word.data_ptr(), stream, _ATTN_WS.get((index, stream))
+    # (As _on_its_device, which would cost these calls a tenth of their time.)
+    native = _binding() if index == _current() else _Elsewhere(index)
+    return native, word.data_ptr(), stream, _ATTN_WS.get((index, stream))
 
 
 def paged_rope_kv(qkv: torch.Tensor, cs: torch.Tensor, pos: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -531,8 +581,8 @@ def paged_rope_kv(qkv: torch.Tensor, cs: torch.Tensor, pos: torch.Tensor, k_page
     float8_e4m3fn codes with one scale byte per vector in ``k_scale``/``v_scale`` (uint8 [pages, kv_heads, page]): the
     vector x is held as codes of x * 2^-e and the byte e + 127, e the smallest integer with max|x| <= 448 * 2^e (within
     [-40, 40])."""
-    status, stream, _ = _context(qkv.device)
-    return _binding().paged_rope_kv(qkv, cs, pos, k_pages, v_pages, slots, heads, kv_heads, k_scale, v_scale, status, stream)
+    native, status, stream, _ = _context(qkv.device)
+    return native.paged_rope_kv(qkv, cs, pos, k_pages, v_pages, slots, heads, kv_heads, k_scale, v_scale, status, stream)
 
 
 def paged_kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, offsets: torch.Tensor,
@@ -543,8 +593,8 @@ def paged_kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torc
     outside them are zeros). 8-bit pages are read as ``dtype`` (default bfloat16), others as what they hold."""
     if dtype is None:
         dtype = torch.bfloat16 if k_pages.dtype == torch.float8_e4m3fn else k_pages.dtype
-    status, stream, _ = _context(k_pages.device)
-    return _binding().paged_kv_read(k_pages, v_pages, page_table, offsets, tokens, k_scale, v_scale, dtype, status, stream)
+    native, status, stream, _ = _context(k_pages.device)
+    return native.paged_kv_read(k_pages, v_pages, page_table, offsets, tokens, k_scale, v_scale, dtype, status, stream)
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -555,12 +605,11 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     (int32) names, head h those of kv head h // (heads / kv_heads). Pages as :func:`paged_rope_kv` writes them. Returns
     q's shape and dtype; a query that sees nothing gets zeros."""
     device = q.device
-    status, stream, ws = _context(device)
-    out = _binding().paged_attention(q, k_pages, v_pages, page_table, lengths, scale, tokens, k_scale, v_scale, status, stream, ws)
+    native, status, stream, ws = _context(device)
+    out = native.paged_attention(q, k_pages, v_pages, page_table, lengths, scale, tokens, k_scale, v_scale, status, stream, ws)
     if out.__class__ is int:  # the bytes of workspace it takes: nothing ran
         ws = _attn_workspace(out, device, stream)
-        out = _binding().paged_attention(q, k_pages, v_pages, page_table, lengths, scale, tokens, k_scale, v_scale, status,
-                                         stream, ws)
+        out = native.paged_attention(q, k_pages, v_pages, page_table, lengths, scale, tokens, k_scale, v_scale, status, stream, ws)
     return out
 
 
@@ -572,11 +621,11 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offset
     16-byte alignment, unit stride in D; offsets ascending, on the device. Returns [Tq, heads, D] in q's dtype (a query
     that sees no key gets zeros; rows of no sequence are not written). ``scale`` defaults to D ** -0.5."""
     device = q.device
-    status, stream, ws = _context(device)
-    out = _binding().packed_attention(q, k, v, q_offsets, k_offsets, scale, status, stream, ws)
+    native, status, stream, ws = _context(device)
+    out = native.packed_attention(q, k, v, q_offsets, k_offsets, scale, status, stream, ws)
     if out.__class__ is int:  # the bytes of workspace it takes: nothing ran
         ws = _attn_workspace(out, device, stream)
-        out = _binding().packed_attention(q, k, v, q_offsets, k_offsets, scale, status, stream, ws)
+        out = native.packed_attention(q, k, v, q_offsets, k_offsets, scale, status, stream, ws)
     return out
 
 
