@@ -529,7 +529,7 @@ def reorder_gather(src: torch.Tensor, parent: torch.Tensor, out: torch.Tensor | 
     return out
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # (builds of PyTorch without CUDA lack it)
 _native = None
 
 

@@ -2,7 +2,11 @@
 current when it is reached."""
 
 import contextlib
+import os
+import subprocess
+import sys
 import types
+from pathlib import Path
 
 import pytest
 import torch
@@ -69,3 +73,16 @@ def test_every_call_of_the_library_is_guarded():
     for n in names:
         fn = getattr(kernels, n)
         assert fn.__wrapped__.__name__ == n and fn.__doc__ == fn.__wrapped__.__doc__
+
+
+def test_import_without_cuda_in_pytorch():
+    """A build of PyTorch without CUDA has none of the private CUDA functions: the package still imports, and says that no
+    device is available."""
+    code = ("import torch\n"
+            "for name in [n for n in dir(torch._C) if n.startswith('_cuda_')]:\n"
+            "    delattr(torch._C, name)\n"
+            "from omniasr_b200 import kernels\n"
+            "assert not kernels.available(torch.device('cpu'))\n")
+    root = Path(kernels.__file__).resolve().parent.parent
+    r = subprocess.run([sys.executable, "-c", code], env={**os.environ, "PYTHONPATH": str(root)}, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
