@@ -147,12 +147,14 @@ _ATTN_WS_RETIRED: list = []  # outgrown workspaces, kept alive for CUDA graphs t
 
 def _attn_workspace(nbytes: int, device: torch.device, stream: int | None = None) -> torch.Tensor:
     """The decode / draft workspace of the current stream: zeroed once when allocated (its leading unit counters
-    must be zero on entry, and every call leaves them zero), reused by the stream's calls in order."""
+    must be zero on entry, and every call leaves them zero), reused by the stream's calls in order. It grows by half at
+    least, so that the outgrown ones, which are kept, stay below twice the last one's size however the calls grow."""
     key = (device.index, torch.cuda.current_stream(device).cuda_stream if stream is None else stream)
     ws = _ATTN_WS.get(key)
     if ws is None or ws.numel() < nbytes:
         if ws is not None:
             _ATTN_WS_RETIRED.append(ws)
+            nbytes = max(nbytes, ws.numel() + ws.numel() // 2)
         with torch.inference_mode(False):
             ws = torch.zeros(max(int(nbytes), 1 << 20), dtype=torch.uint8, device=device)
         _ATTN_WS[key] = ws
