@@ -309,6 +309,10 @@ int omniasr_packed_attention(const void* q, int64_t q_stride_tok, int64_t q_stri
                              int heads, int kv_heads, int dim, float scale, int dtype, void* workspace, size_t workspace_bytes,
                              int* status, cudaStream_t stream);
 
+/* The id of the capture that the stream is in (never 0), or 0: for callers that keep workspaces. One that is zeroed by a
+ * memset inside a capture is zero for that graph alone, once it is replayed. No counterpart in the reference. */
+unsigned long long omniasr_capture_id(cudaStream_t stream);
+
 /* Self-test of the bounded device wait every kernel here uses (no counterpart in the reference): one kernel waits
  * on an mbarrier that nothing completes, gives up after limit_ns (0 < limit_ns <= 1e8), ORs the timeout bit (2)
  * into *status and returns; *waited_ns (may be NULL; device memory) gets the time it waited. The context stays

@@ -91,6 +91,16 @@ extern "C" {
 
 int omniasr_abi_version(void) { return 2; }
 
+unsigned long long omniasr_capture_id(cudaStream_t stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(stream, &status, &id) != cudaSuccess) {
+    cudaGetLastError();  // (the legacy stream beside a capture, or no device)
+    return 0;
+  }
+  return status == cudaStreamCaptureStatusActive ? id : 0;
+}
+
 const char* omniasr_last_error(void) { return g_error.c_str(); }
 
 int omniasr_device_supported(int device) {

@@ -49,6 +49,7 @@ SIGNATURES = {
                                               _i, _p, _p]),
     "omniasr_noalloc_scratch_bytes": (_sz, []),
     "omniasr_noalloc_reset": (_i, [_p]),
+    "omniasr_capture_id": (ctypes.c_ulonglong, [_p]),
     "omniasr_selftest_wait_timeout": (_i, [_i64, _p, _p, _p]),
     "omniasr_propose": (_i, [_p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p, _i,
                              _i, _p, _p]),

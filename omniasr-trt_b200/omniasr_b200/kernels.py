@@ -143,22 +143,46 @@ def _workspace(nbytes: int, device: torch.device) -> torch.Tensor:
 
 _ATTN_WS: dict = {}  # (device, stream) -> decode / draft workspace; its unit counters start zero and stay zero
 _ATTN_WS_RETIRED: list = []  # outgrown workspaces, kept alive for CUDA graphs that captured them
+_CAPTURE_WS: dict = {}  # (kind, device, stream) -> (capture, workspace) of the stream's latest capture that needed its own
+
+
+def _capture_id(stream: int) -> int:
+    """The id of the CUDA graph capture that the stream is in, 0 outside one."""
+    return _lib.load().omniasr_capture_id(ctypes.c_void_p(stream))
+
+
+def _zeroed_workspace(kind: str, kept: dict, retired: list, nbytes: int, device: torch.device, stream: int) -> torch.Tensor:
+    """The stream's workspace in ``kept``, zeroed once when allocated (its leading counters must be zero on entry, and every
+    call leaves them zero), reused by the stream's calls in order. It grows by half at least, so that the outgrown ones,
+    which are kept, stay below twice the last one's size however the calls grow.
+
+    A workspace that is first needed during a capture belongs to that capture: its zeroing becomes a node of that graph, so
+    no other graph and no eager call may count on it."""
+    key = (device.index, stream)
+    ws = kept.get(key)
+    if ws is not None and ws.numel() >= nbytes:
+        return ws
+    capture = _capture_id(stream)
+    if capture:
+        of, ws = _CAPTURE_WS.get((kind, *key), (0, None))
+        if of == capture and ws.numel() >= nbytes:
+            return ws
+    elif ws is not None:
+        retired.append(ws)
+        nbytes = max(nbytes, ws.numel() + ws.numel() // 2)
+    with torch.inference_mode(False):
+        ws = torch.zeros(max(int(nbytes), 1 << 20), dtype=torch.uint8, device=device)
+    if capture:
+        _CAPTURE_WS[(kind, *key)] = (capture, ws)
+    else:
+        kept[key] = ws
+    return ws
 
 
 def _attn_workspace(nbytes: int, device: torch.device, stream: int | None = None) -> torch.Tensor:
-    """The decode / draft workspace of the current stream: zeroed once when allocated (its leading unit counters
-    must be zero on entry, and every call leaves them zero), reused by the stream's calls in order. It grows by half at
-    least, so that the outgrown ones, which are kept, stay below twice the last one's size however the calls grow."""
-    key = (device.index, torch.cuda.current_stream(device).cuda_stream if stream is None else stream)
-    ws = _ATTN_WS.get(key)
-    if ws is None or ws.numel() < nbytes:
-        if ws is not None:
-            _ATTN_WS_RETIRED.append(ws)
-            nbytes = max(nbytes, ws.numel() + ws.numel() // 2)
-        with torch.inference_mode(False):
-            ws = torch.zeros(max(int(nbytes), 1 << 20), dtype=torch.uint8, device=device)
-        _ATTN_WS[key] = ws
-    return ws
+    """The decode / draft workspace of the current stream."""
+    stream = torch.cuda.current_stream(device).cuda_stream if stream is None else stream
+    return _zeroed_workspace("attention", _ATTN_WS, _ATTN_WS_RETIRED, nbytes, device, stream)
 
 
 @_on_its_device
@@ -433,15 +457,7 @@ _GEMM_WS_RETIRED: list = []  # outgrown workspaces, kept alive for CUDA graphs t
 
 
 def _gemm_workspace(nbytes: int, device: torch.device) -> torch.Tensor:
-    key = (device.index, torch.cuda.current_stream(device).cuda_stream)
-    ws = _GEMM_WS.get(key)
-    if ws is None or ws.numel() < nbytes:
-        if ws is not None:
-            _GEMM_WS_RETIRED.append(ws)
-        with torch.inference_mode(False):
-            ws = torch.zeros(max(int(nbytes), 1 << 20), dtype=torch.uint8, device=device)
-        _GEMM_WS[key] = ws
-    return ws
+    return _zeroed_workspace("gemm", _GEMM_WS, _GEMM_WS_RETIRED, nbytes, device, torch.cuda.current_stream(device).cuda_stream)
 
 
 @_on_its_device
