@@ -130,6 +130,8 @@ class PagedCache:
         if len(set(batch.new)) > 1:
             raise ValueError("decode: the same number of new tokens for every sequence (prefill takes others)")
         q = self.write(layer, qkv, cs, batch, heads)
+        if not any(batch.new):
+            return q  # no queries
         k, v, (ks, vs) = self._layer(layer)
         return kernels.paged_attention(q, k, v, batch.table, batch.lengths, self.dim**-0.5 if scale is None else scale,
-                                       tokens=max(batch.new, default=1) or 1, k_scale=ks, v_scale=vs)
+                                       tokens=batch.new[0], k_scale=ks, v_scale=vs)
