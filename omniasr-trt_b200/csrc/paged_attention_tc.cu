@@ -29,10 +29,11 @@
 // maximum, w up to 2^8: the pieces' smallest step is then 2^-17 of a typical largest weight.
 //
 // What bounds it: HBM. bytes = keys * kv_heads * D * 2 * element (+ 2 scale bytes a key). 48 rows of 4096 keys, 8 kv heads of
-// 128, 32 query heads: bf16 126.5 us (6369 GB/s), e4m3 72 us (5612 GB/s); 48 rows of 61 to 4093 in pages of 16, bf16, 72 us
-// (5670 GB/s: 9 us of entry, schedule and last join); with 16 query heads to a kv head e4m3 takes 4.3 TB/s (N = 64, whose
-// softmax spills at these registers). One row of a few hundred keys is latency: 12 us, of which a unit's ends are about 4000
-// clocks.
+// 128, 32 query heads, pages of 64: bf16 127 us (6346 GB/s), e4m3 71.5 us (5690 GB/s); 48 rows of 61 to 4093 in pages of 16,
+// bf16, 74 us (5540 GB/s: 9 us of entry, schedule and last join). With 16 query heads to a kv head e4m3 takes 4.2 TB/s (a
+// thread's 16 columns of two pieces each spill registers, as those of bf16 at head_dim 256 and 512 do). More than 16 query
+// columns on a kv head are several units, each of which reads the keys: 5 tokens of 4 heads 260 us against 131 of one token
+// (pages of 16). One row of a few hundred keys is latency: 12 us, of which a unit's ends are about 4000 clocks.
 
 #include <cudaTypedefs.h>
 #include <math.h>
