@@ -607,8 +607,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     int item = 0;
     RedoList list;  // packed
     Unit u;
-    bool ok = true;  // (converged, as in prefill.cu)
-    for (int n = 0; ok && wget(n, u); ++n) {
+    bool ok = true;  // (no lane leaves alone: prefill.cu)
+    for (int n = 0; PACKED ? ok && wget(n, u) : get(n, u); ++n) {
       int pos = 0, head = 0;
       float odd = 0.f, sum = 0.f;  // packed: turns NaN if a result of the row is not finite; the row's sum
       bool live;
@@ -632,8 +632,13 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (un >= 0) load_q(n + 1, un);
           }
         }
-        ok = wwait(&o_ready, item & 1) && wwait(&l_full, item & 1);
-        if (!ok) break;
+        if constexpr (PACKED) {
+          ok = wwait(&o_ready, item & 1) && wwait(&l_full, item & 1);
+          if (!ok) break;
+        } else {
+          wait(&o_ready, item & 1);
+          wait(&l_full, item & 1);
+        }
         tc_fence_after();
         __syncwarp();
         float l = 0.f;
