@@ -17,16 +17,16 @@ NAN, INF = float("nan"), float("inf")
 
 
 @pytest.mark.parametrize("heads,kv,dim,rows", [(8, 8, 128, 32), (16, 4, 128, 48), (16, 2, 64, 40), (32, 2, 128, 40), (8, 8, 512, 20), (8, 2, 256, 40)])
-@pytest.mark.parametrize("nats", [11.0, 11.4, 11.8, 12.2, 12.5, 13.0])
-def test_a_key_far_above_a_long_tail(heads, kv, dim, rows, nats):
-    """8-bit pages, one key 11 to 13 nats above 32767 others that score alike, values with a common mean: each weight of the
-    tail lies below the smallest step of the two e4m3 pieces (2^-13; the key's weight is 2^4 to 2^8), yet together they are
-    a tenth of the sum and more. The units are long enough that few are cut.
+@pytest.mark.parametrize("n,nats", [*((32768, x) for x in (11.0, 11.4, 11.8, 12.2, 12.5, 13.0)), (131072, 13.0), (131072, 13.75)])
+def test_a_key_far_above_a_long_tail(heads, kv, dim, rows, n, nats):
+    """8-bit pages, one key 11 to 14 nats above the 32767 or 131071 others that score alike, values with a common mean: each
+    weight of the tail lies around or below the smallest step of the two e4m3 pieces (2^-13; the key's weight is 2^4 to
+    2^8), yet together they are 7 to 35% of the sum. The units are long enough that few are cut.
 
     Beside the rounding of the output and of the weights' 8 significant bits (2^-8 (|o| + A), 2^-10 A), a weight's last piece
     is off by an error of mean zero within one step, a standard deviation of at most half of one: over n keys and a sum l >= 2^4
     that is sqrt(n) 2^-14 / l of a value; six of them (2.4e5 results, about 5e-4 of one expected past it)."""
-    n, page = 32768, 128
+    page = 128
     g = torch.Generator(device=DEV).manual_seed(1)
     k = torch.zeros(n // page, kv, page, dim, device=DEV)
     k[3, :, 77, 0] = 1.0
