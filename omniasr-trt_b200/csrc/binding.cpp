@@ -189,8 +189,9 @@ py::object packed_attention(const at::Tensor& q, const at::Tensor& k, const at::
   const double s = scale ? *scale : 1.0 / std::sqrt((double)dim);
   done("omniasr_packed_attention",
        omniasr_packed_attention(q.data_ptr(), stride_of(q, 0), stride_of(q, 1), k.data_ptr(), stride_of(k, 0), stride_of(k, 1),
-                                v.data_ptr(), stride_of(v, 0), stride_of(v, 1), out.data_ptr(), qo.data_ptr<int64_t>(), ko.data_ptr<int64_t>(), tq, tk, (int)seqs, (int)heads,
-                                (int)kv, (int)dim, (float)s, dtype, ws->data_ptr(), ws->numel(), status_of(status), stream_of(stream)));
+                                v.data_ptr(), stride_of(v, 0), stride_of(v, 1), out.data_ptr(), qo.data_ptr<int64_t>(),
+                                ko.data_ptr<int64_t>(), tq, tk, (int)seqs, (int)heads, (int)kv, (int)dim, (float)s, dtype,
+                                ws->data_ptr(), ws->numel(), status_of(status), stream_of(stream)));
   return py::cast(out);
 }
 
