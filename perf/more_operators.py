@@ -27,6 +27,7 @@ import torch
 own = False
 
 MAX_KEYS = 5.4e8  # rows x longest x kv_heads x dim of the largest listed cache
+MAX_BYTES, MAX_FLOPS = 4.4e8, 6.2e9  # of the largest listed case
 MAX_NEW = 1.6e8  # numbers of the largest listed append
 
 
@@ -108,7 +109,7 @@ def draw(rng):
             hi = _log(rng, 1, 131072)
             c |= {"rows": _log(rng, 1, 256), "tokens": rng.choice([1, 1, 1, 1, 2, 5, 8]), "lo": rng.randint(0, hi), "hi": hi}
             keys = sum(_spread(c["lo"], c["hi"], c["rows"]))
-            if c["rows"] * hi * kv * dim > MAX_KEYS or keys * heads * c["tokens"] > 2e8:
+            if c["rows"] * hi * kv * dim > MAX_KEYS or work(c)["bytes"] > MAX_BYTES or work(c)["flops"] > MAX_FLOPS:
                 continue  # the plain form holds every key in 32 bits
             if dtype == "f32" and keys * kv * dim > 6e7:
                 continue
