@@ -34,7 +34,8 @@ extern "C" {
 
 #define OMNIASR_BF16 0
 #define OMNIASR_F32 1
-#define OMNIASR_FP8 2 /* a paged cache's element type: e4m3 codes with one scale byte per vector */
+#define OMNIASR_FP8 2  /* a paged cache's element type: e4m3 codes with one scale byte per vector */
+#define OMNIASR_INT4 3 /* a paged cache's element type: 4-bit codes with one bf16 scale per 32 dims */
 
 #define OMNIASR_OK 0
 #define OMNIASR_ERR_ARGUMENT 1    /* a shape, stride, pointer alignment or size is invalid */
@@ -263,7 +264,13 @@ int omniasr_noalloc_reset(cudaStream_t stream);
  * at j / page. cache_type is the dtype itself, or OMNIASR_FP8: each vector x (one position of one kv head) is held as
  * e4m3 codes of x * 2^-e, e = the smallest integer with max|x| <= 448 * 2^e held to [-40, 40], and the byte e + 127 in
  * k_scale / v_scale [pages, kv_heads, page] (contiguous, 16-byte aligned; NULL for the other types). Infinities, NaN and values past
- * 448 * 2^40 are held as NaN and do not count for the scale. heads must be a multiple of kv_heads; query head h reads kv
+ * 448 * 2^40 are held as NaN and do not count for the scale. OMNIASR_INT4 (dim 32 and more): a page holds dim / 2 bytes of codes per
+ * vector (strides in bytes), and k_scale / v_scale are bf16 [pages, kv_heads, page, dim / 32] (contiguous, 16-byte aligned). Each
+ * group of 32 dims x is held as s = -m / 8 rounded to bf16, m its value of largest magnitude (the negative one of two), and the
+ * codes c = x / s (one fp32 division) rounded to the nearest whole number of [-8, 7], plus 8 (8 where s is 0), which stand for
+ * s (c - 8); a group with an infinity or a NaN has s = NaN. Codes lie two to a byte, the low bits first; with quads
+ * u = d / 4 in blocks of 32, NG = min(4, dim / 32), g = u % 32 / 8, i = u % 8, dims 4u .. 4u + 3 are the 16-bit word
+ * (i / 2 * NG + g) * 2 + i % 2 of the quad's block in K, the word i * NG + g in V. heads must be a multiple of kv_heads; query head h reads kv
  * head h / (heads / kv_heads). A page number outside the pool (or a length past the table) raises status bit 1, the
  * row's result is then unspecified, and nothing outside the tensors is touched. */
 
@@ -274,6 +281,15 @@ int omniasr_paged_rope_kv(const void* qkv, int64_t qkv_stride, const float* cs, 
                           const int64_t* slots, void* q_out, void* k_pages, void* v_pages, void* k_scale, void* v_scale,
                           int64_t pages, int page, int64_t stride_page, int64_t stride_head, int64_t stride_pos, int n,
                           int heads, int kv_heads, int dim, int dtype, int cache_type, int* status, cudaStream_t stream);
+
+/* omniasr_paged_rope_kv() of a model that norms its queries and keys: each q and k vector x (one head of one token) becomes
+ * x * rsqrt(mean(x^2) + eps) * w before it is rotated, w being q_norm or k_norm [dim] of dtype (16-byte aligned), in fp32 with one
+ * rounding, after the rotation. v is not normed. No counterpart in the reference. */
+int omniasr_paged_norm_rope_kv(const void* qkv, int64_t qkv_stride, const void* q_norm, const void* k_norm, float eps,
+                               const float* cs, int64_t cs_positions, const int64_t* pos, const int64_t* slots, void* q_out,
+                               void* k_pages, void* v_pages, void* k_scale, void* v_scale, int64_t pages, int page,
+                               int64_t stride_page, int64_t stride_head, int64_t stride_pos, int n, int heads, int kv_heads,
+                               int dim, int dtype, int cache_type, int* status, cudaStream_t stream);
 
 /* Reads pages back: rows offsets[i] .. offsets[i + 1] - 1 of k_out / v_out [tokens, kv_heads, dim] (contiguous, dtype)
  * get the first offsets[i + 1] - offsets[i] positions of table row i, for i < rows (offsets ascending, rows + 1 of

@@ -61,7 +61,8 @@ Pages pages_of(const char* name, const at::Tensor& k, const at::Tensor& v, const
   for (int64_t i = 0; same && i < 3; ++i) same = stride_of(k, i) == stride_of(v, i);
   if (!same || k.stride(3) != 1 || v.stride(3) != 1)
     refuse(name, "k and v pages must be [pages, kv_heads, page, D] views of one dtype with the same strides and unit stride in D");
-  Pages p{k.data_ptr(), v.data_ptr(), nullptr, nullptr, k.size(0), k.size(1), k.size(2), k.size(3),
+  const bool int4 = k.scalar_type() == at::kByte;  // 4-bit codes, two to a byte
+  Pages p{k.data_ptr(), v.data_ptr(), nullptr, nullptr, k.size(0), k.size(1), k.size(2), int4 ? 2 * k.size(3) : k.size(3),
           stride_of(k, 0), stride_of(k, 1), stride_of(k, 2), 0};
   if (k.scalar_type() == at::kFloat8_e4m3fn) {
     for (const Opt* s : {&ks, &vs}) {
@@ -74,10 +75,23 @@ Pages pages_of(const char* name, const at::Tensor& k, const at::Tensor& v, const
     p.type = OMNIASR_FP8;
     return p;
   }
+  if (int4) {
+    const int64_t shape[4] = {k.size(0), k.size(1), k.size(2), p.dim / 32};
+    for (const Opt* s : {&ks, &vs}) {
+      if (!*s || (*s)->scalar_type() != at::kBFloat16 || (*s)->sizes() != at::IntArrayRef(shape, 4) || !(*s)->is_contiguous())
+        refuse(name, "uint8 pages (4-bit codes) need contiguous bfloat16 scales [pages, kv_heads, page, D / 32]");
+    }
+    same_device(name, k, {&v, &*ks, &*vs});
+    p.ks = ks->data_ptr();
+    p.vs = vs->data_ptr();
+    p.type = OMNIASR_INT4;
+    return p;
+  }
   p.type = code_of(k.scalar_type());
   if (p.type != dtype)
-    refuse(name, "pages of " + std::string(c10::toString(k.scalar_type())) + " (supported: the queries' dtype, float8_e4m3fn)");
-  if (ks || vs) refuse(name, "scales belong to float8_e4m3fn pages");
+    refuse(name, "pages of " + std::string(c10::toString(k.scalar_type())) +
+                     " (supported: the queries' dtype, float8_e4m3fn, uint8 of 4-bit codes)");
+  if (ks || vs) refuse(name, "scales belong to float8_e4m3fn and uint8 pages");
   return p;
 }
 
@@ -89,10 +103,10 @@ void check_table(const char* name, const at::Tensor& t, int64_t rows) {
 int* status_of(int64_t p) { return reinterpret_cast<int*>(p); }
 cudaStream_t stream_of(int64_t p) { return reinterpret_cast<cudaStream_t>(p); }
 
-at::Tensor paged_rope_kv(const at::Tensor& qkv, const at::Tensor& cs_in, const at::Tensor& pos_in, const at::Tensor& k,
-                         const at::Tensor& v, const at::Tensor& slots_in, int64_t heads, int64_t kv_heads, const Opt& ks,
-                         const Opt& vs, int64_t status, int64_t stream) {
-  const char* name = "paged_rope_kv";
+// paged_rope_kv, and paged_norm_rope_kv where the norms' weights are given.
+at::Tensor rope(const char* name, const at::Tensor& qkv, const Opt& q_norm, const Opt& k_norm, double eps, const at::Tensor& cs_in,
+                const at::Tensor& pos_in, const at::Tensor& k, const at::Tensor& v, const at::Tensor& slots_in, int64_t heads,
+                int64_t kv_heads, const Opt& ks, const Opt& vs, int64_t status, int64_t stream) {
   const int dtype = dtype_of(name, qkv);
   const Pages p = pages_of(name, k, v, ks, vs, dtype);
   const int64_t n = qkv.dim() == 2 ? qkv.size(0) : 0;
@@ -100,18 +114,45 @@ at::Tensor paged_rope_kv(const at::Tensor& qkv, const at::Tensor& cs_in, const a
     refuse(name, "qkv must be [N, (heads + 2 * kv_heads) * D] with unit inner stride");
   if (pos_in.numel() != n || slots_in.numel() != n) refuse(name, "pos and slots must hold one entry per token");
   if (cs_in.dim() != 3 || cs_in.size(1) != p.dim / 2 || cs_in.size(2) != 2) refuse(name, "cs must be [P, D / 2, 2]");
+  if (q_norm) {
+    for (const Opt* w : {&q_norm, &k_norm})
+      if ((*w)->dim() != 1 || (*w)->size(0) != p.dim || (*w)->scalar_type() != qkv.scalar_type() || (*w)->stride(0) != 1)
+        refuse(name, "q_norm and k_norm must be contiguous [D] of qkv's dtype");
+  }
   if (n > 0x7fffffff) refuse(name, "too many tokens");
   at::Tensor q = at::empty({n, heads, p.dim}, qkv.options());
   if (n == 0) return q;
   same_device(name, qkv, {&cs_in, &pos_in, &k, &v, &slots_in});
   const at::Tensor cs = cs_in.scalar_type() == at::kFloat && cs_in.is_contiguous() ? cs_in : cs_in.to(at::kFloat).contiguous();
   const at::Tensor pos = index_of(pos_in), slots = index_of(slots_in);
-  done("omniasr_paged_rope_kv",
-       omniasr_paged_rope_kv(qkv.data_ptr(), stride_of(qkv, 0), cs.data_ptr<float>(), cs.size(0), pos.data_ptr<int64_t>(),
-                             slots.data_ptr<int64_t>(), q.data_ptr(), const_cast<void*>(p.k), const_cast<void*>(p.v),
-                             const_cast<void*>(p.ks), const_cast<void*>(p.vs), p.pages, (int)p.page, p.sp, p.sh, p.st, (int)n,
-                             (int)heads, (int)kv_heads, (int)p.dim, dtype, p.type, status_of(status), stream_of(stream)));
+  void *kp = const_cast<void*>(p.k), *vp = const_cast<void*>(p.v), *ksp = const_cast<void*>(p.ks), *vsp = const_cast<void*>(p.vs);
+  if (q_norm) {
+    same_device(name, qkv, {&*q_norm, &*k_norm});
+    done("omniasr_paged_norm_rope_kv",
+         omniasr_paged_norm_rope_kv(qkv.data_ptr(), stride_of(qkv, 0), q_norm->data_ptr(), k_norm->data_ptr(), (float)eps,
+                                    cs.data_ptr<float>(), cs.size(0), pos.data_ptr<int64_t>(), slots.data_ptr<int64_t>(),
+                                    q.data_ptr(), kp, vp, ksp, vsp, p.pages, (int)p.page, p.sp, p.sh, p.st, (int)n, (int)heads,
+                                    (int)kv_heads, (int)p.dim, dtype, p.type, status_of(status), stream_of(stream)));
+  } else {
+    done("omniasr_paged_rope_kv",
+         omniasr_paged_rope_kv(qkv.data_ptr(), stride_of(qkv, 0), cs.data_ptr<float>(), cs.size(0), pos.data_ptr<int64_t>(),
+                               slots.data_ptr<int64_t>(), q.data_ptr(), kp, vp, ksp, vsp, p.pages, (int)p.page, p.sp, p.sh, p.st,
+                               (int)n, (int)heads, (int)kv_heads, (int)p.dim, dtype, p.type, status_of(status), stream_of(stream)));
+  }
   return q;
+}
+
+at::Tensor paged_rope_kv(const at::Tensor& qkv, const at::Tensor& cs, const at::Tensor& pos, const at::Tensor& k,
+                         const at::Tensor& v, const at::Tensor& slots, int64_t heads, int64_t kv_heads, const Opt& ks,
+                         const Opt& vs, int64_t status, int64_t stream) {
+  return rope("paged_rope_kv", qkv, std::nullopt, std::nullopt, 0., cs, pos, k, v, slots, heads, kv_heads, ks, vs, status, stream);
+}
+
+at::Tensor paged_norm_rope_kv(const at::Tensor& qkv, const at::Tensor& q_norm, const at::Tensor& k_norm, const at::Tensor& cs,
+                              const at::Tensor& pos, const at::Tensor& k, const at::Tensor& v, const at::Tensor& slots,
+                              int64_t heads, int64_t kv_heads, double eps, const Opt& ks, const Opt& vs, int64_t status,
+                              int64_t stream) {
+  return rope("paged_norm_rope_kv", qkv, q_norm, k_norm, eps, cs, pos, k, v, slots, heads, kv_heads, ks, vs, status, stream);
 }
 
 std::pair<at::Tensor, at::Tensor> paged_kv_read(const at::Tensor& k, const at::Tensor& v, const at::Tensor& table,
@@ -199,6 +240,7 @@ py::object packed_attention(const at::Tensor& q, const at::Tensor& k, const at::
 
 PYBIND11_MODULE(_omniasr_torch, m) {
   m.def("paged_rope_kv", &paged_rope_kv);
+  m.def("paged_norm_rope_kv", &paged_norm_rope_kv);
   m.def("paged_kv_read", &paged_kv_read);
   m.def("paged_attention", &paged_attention);
   m.def("packed_attention", &packed_attention);

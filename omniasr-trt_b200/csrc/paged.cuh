@@ -8,10 +8,11 @@
 
 namespace omni {
 
-constexpr int kFp8 = 2;  // cache element type code beside kBF16 / kF32: e4m3 codes with a scale byte per vector
+constexpr int kFp8 = 2;   // cache element type codes beside kBF16 / kF32: e4m3 codes with a scale byte per vector,
+constexpr int kInt4 = 3;  // 4-bit codes with a bf16 scale per 32 dims (int4.cuh)
 
-// A cache of pages [pages, kv_heads, page, dim] (K and V share their strides, in elements); scale bytes
-// [pages, kv_heads, page] contiguous, or null.
+// A cache of pages [pages, kv_heads, page, dim] (K and V share their strides, in elements; of 4-bit pages in bytes); scale bytes
+// [pages, kv_heads, page], bf16 scales [pages, kv_heads, page, dim / 32], contiguous, or null.
 struct PageCache {
   void* k;
   void* v;
@@ -19,7 +20,7 @@ struct PageCache {
   uint8_t* v_scale;
   int64_t pages, s_page, s_head, s_pos;
   int page, kv_heads, dim;
-  int type;  // kBF16, kF32 or kFp8
+  int type;  // kBF16, kF32, kFp8 or kInt4
 };
 
 struct PagedRopeArgs {
@@ -32,9 +33,13 @@ struct PagedRopeArgs {
   void* q_out;
   PageCache c;
   int n, heads;
+  const void* q_norm;  // [dim] weights of the norms (paged_norm_rope_kv alone)
+  const void* k_norm;
+  float eps;
   int* status;
 };
 cudaError_t launch_paged_rope_kv(int dtype, const PagedRopeArgs& a, cudaStream_t stream);
+cudaError_t launch_paged_norm_rope_kv(int dtype, const PagedRopeArgs& a, cudaStream_t stream);
 
 struct PagedReadArgs {
   PageCache c;

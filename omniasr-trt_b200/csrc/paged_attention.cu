@@ -14,9 +14,11 @@
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "attention.cuh"
 #include "common.cuh"
+#include "int4.cuh"
 #include "paged.cuh"
 
 namespace omni {
@@ -60,6 +62,27 @@ struct Row8<__nv_fp8_e4m3> {
   }
 };
 
+// A lane's eight dims of a key's or value's row: dims 8w .. 8w + 7 of the row that starts at element `row`.
+template <typename TC, int D, bool KEYS>
+struct CacheRow8 {
+  Row8<TC> r;
+  OMNI_DEV void load(const void* base, int64_t row, int w) { r.load(base, row + w * 8); }
+  OMNI_DEV void get(float* f) const { r.get(f); }
+};
+struct Int4 {};  // 4-bit codes (int4.cuh); `row` counts bytes, the values are those under a scale of 1
+template <int D, bool KEYS>
+struct CacheRow8<Int4, D, KEYS> {
+  uint32_t u;
+  OMNI_DEV void load(const void* base, int64_t row, int w) {
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(reinterpret_cast<const uint8_t*>(base) + row);
+    u = (uint32_t)__ldg(q + quad_at<D, KEYS>(2 * w)) | (uint32_t)__ldg(q + quad_at<D, KEYS>(2 * w + 1)) << 16;
+  }
+  OMNI_DEV void get(float* f) const {
+    int4_values(u, 1.f, f);
+    int4_values(u >> 16, 1.f, f + 4);
+  }
+};
+
 struct Split {
   int splits, chunks, cols;  // key splits per unit, column chunks per (row, kv head), columns per chunk
   float* part_o;             // [row * T * heads + column's query][split][D]
@@ -79,7 +102,7 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const PagedAttnArgs a, 
   constexpr int L = D / 8 < 32 ? D / 8 : 32;  // lanes per key
   constexpr int NV = D / 8 / L;               // steps of 8 dims per lane
   constexpr int TEAMS = kThreads / L;
-  constexpr bool FP8 = sizeof(TC) == 1;
+  constexpr bool FP8 = std::is_same_v<TC, __nv_fp8_e4m3>, INT4 = std::is_same_v<TC, Int4>;
   grid_launch_dependents();
   grid_dependency_wait();
   const int split = blockIdx.x;
@@ -150,15 +173,17 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const PagedAttnArgs a, 
       }
     }
     float s[NC];
-    Row8<TC> kr[NV], vr[NV];
+    CacheRow8<TC, D, true> kr[NV];
+    CacheRow8<TC, D, false> vr[NV];
 #pragma unroll
     for (int c = 0; c < NC; ++c) s[c] = 0.f;
     float ks = 1.f, vs = 1.f;
+    float kg[NV], vg[NV];  // 4-bit groups' scales
     if (page_ok) {
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        kr[v].load(a.c.k, at + (v * L + lane) * 8);
-        vr[v].load(a.c.v, at + (v * L + lane) * 8);
+        kr[v].load(a.c.k, at, v * L + lane);
+        vr[v].load(a.c.v, at, v * L + lane);
       }
       if (FP8) {
         ks = __uint_as_float((uint32_t)a.c.k_scale[si] << 23);
@@ -168,6 +193,13 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const PagedAttnArgs a, 
       for (int v = 0; v < NV; ++v) {
         float kf[8];
         kr[v].get(kf);
+        if constexpr (INT4) {
+          const int64_t g = si * (D / 32) + (v * L + lane) / 4;
+          kg[v] = bf16_value(__ldg(reinterpret_cast<const uint16_t*>(a.c.k_scale) + g));
+          vg[v] = bf16_value(__ldg(reinterpret_cast<const uint16_t*>(a.c.v_scale) + g));
+#pragma unroll
+          for (int i = 0; i < 8; ++i) kf[i] *= kg[v];
+        }
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -202,6 +234,10 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const PagedAttnArgs a, 
       for (int v = 0; v < NV; ++v) {
         float vf[8];
         vr[v].get(vf);
+        if constexpr (INT4) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) vf[i] *= vg[v];
+        }
 #pragma unroll
         for (int c = 0; c < NC; ++c)
           if (j < lim[c]) {
@@ -306,8 +342,9 @@ cudaError_t launch_cols(const PagedAttnArgs& a, const Split& sp, cudaStream_t s)
 
 template <typename TQ, typename TC>
 cudaError_t launch_dim(const PagedAttnArgs& a, const Split& sp, cudaStream_t s) {
+  if constexpr (!std::is_same_v<TC, Int4>)
+    if (a.c.dim == 16) return launch_cols<TQ, TC, 16>(a, sp, s);
   switch (a.c.dim) {
-    case 16: return launch_cols<TQ, TC, 16>(a, sp, s);
     case 32: return launch_cols<TQ, TC, 32>(a, sp, s);
     case 64: return launch_cols<TQ, TC, 64>(a, sp, s);
     case 128: return launch_cols<TQ, TC, 128>(a, sp, s);
@@ -333,11 +370,13 @@ cudaError_t launch_paged_attention(int dtype, const PagedAttnArgs& a, cudaStream
   sp.part_ml = sp.part_o + qrows * sp.splits * a.c.dim;
   cudaError_t e;
   if (dtype == kBF16)
-    e = a.c.type == kFp8 ? paged::launch_dim<__nv_bfloat16, __nv_fp8_e4m3>(a, sp, stream)
-                         : paged::launch_dim<__nv_bfloat16, __nv_bfloat16>(a, sp, stream);
+    e = a.c.type == kInt4  ? paged::launch_dim<__nv_bfloat16, paged::Int4>(a, sp, stream)
+        : a.c.type == kFp8 ? paged::launch_dim<__nv_bfloat16, __nv_fp8_e4m3>(a, sp, stream)
+                           : paged::launch_dim<__nv_bfloat16, __nv_bfloat16>(a, sp, stream);
   else
-    e = a.c.type == kFp8 ? paged::launch_dim<float, __nv_fp8_e4m3>(a, sp, stream)
-                         : paged::launch_dim<float, float>(a, sp, stream);
+    e = a.c.type == kInt4  ? paged::launch_dim<float, paged::Int4>(a, sp, stream)
+        : a.c.type == kFp8 ? paged::launch_dim<float, __nv_fp8_e4m3>(a, sp, stream)
+                           : paged::launch_dim<float, float>(a, sp, stream);
   if (e != cudaSuccess || sp.splits == 1) return e;
   if (dtype == kBF16)
     return launch_dependent(paged::join_kernel<__nv_bfloat16>, dim3((unsigned)qrows), dim3(paged::kThreads), 0, stream, sp,

@@ -8,7 +8,8 @@
 // A power of two loses nothing over an arbitrary scale in a floating-point code (e4m3 keeps its 4 significant bits
 // whatever the exponent), is exact to apply and to undo, and takes one byte. The range keeps every product of a scale
 // with a softmax weight inside fp32; finite values past 448 * 2^40, infinities and NaN are held as NaN and do not
-// count for the scale. paged_kv_read gives the values code * 2^e (exact in fp32, rounded to the output's type).
+// count for the scale. paged_kv_read gives the values code * 2^e (exact in fp32, rounded to the output's type). With a 4-bit cache a
+// group of 32 dims is held as 4-bit codes and a bf16 scale (int4.cuh); read back, s (c - 8), exact in fp32 too.
 //
 // Both move each byte once and compute next to nothing: HBM for prompts, latency for single tokens.
 
@@ -18,171 +19,15 @@
 
 #include <type_traits>
 
-#include "attention.cuh"
-#include "common.cuh"
-#include "paged.cuh"
-#include "rope_kv.cuh"
+#include "paged_rope.cuh"
 
 namespace omni {
 namespace {
-
-// The scale exponent of a vector whose largest finite magnitude has these bits.
-OMNI_DEV int scale_exponent(uint32_t amax_bits) {
-  const int e = (int)(amax_bits >> 23) - 135 + ((amax_bits & 0x7fffffu) > 0x600000u ? 1 : 0);
-  return e < -40 ? -40 : (e > 40 ? 40 : e);
-}
-
-OMNI_DEV float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
-
-// Four e4m3 codes of x * inv.
-OMNI_DEV uint32_t codes4(const float* x, float inv) {
-  float y[4];
-  bool bad[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    y[i] = x[i] * inv;
-    bad[i] = !(fabsf(y[i]) <= 448.f);
-  }
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
-  uint32_t r = lo | (hi << 16);
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (bad[i]) r |= 0x7fu << (8 * i);
-  return r;
-}
 
 // Two e4m3 codes as floats.
 OMNI_DEV float2 values2(uint32_t codes) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes & 0xffffu), __NV_E4M3);
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
-}
-
-constexpr int kRopeThreads = 256;
-
-// One CTA: the vectors [item0, item0 + per) of one token (heads of q, then k, then v). A vector is taken by L lanes,
-// 16 bytes per lane and step, so a thread keeps the same dims for all its vectors and loads their cos / sin once.
-// IL vectors per thread are in flight together.
-// (Prompts of 32 + 2 x 8 heads of 128, 291 MB: 61 us with four vectors per thread of which the fourth had nothing to do,
-// 53 us, 5470 GB/s, with three and registers for six CTAs per SM; a CTA that walks tokens with the next one's loads in
-// flight needs twice the registers: 93 us.)
-template <typename T, int D, bool FP8, int IL>
-__global__ void __launch_bounds__(kRopeThreads, D * sizeof(T) <= 512 ? (IL == 4 ? 5 : 6) : 2) paged_rope_kernel(const PagedRopeArgs a, int per) {
-  constexpr int kVec = Elem<T>::kVec;
-  constexpr int VPV = D / kVec;            // 16-byte words per vector
-  constexpr int L = VPV < 32 ? VPV : 32;   // lanes per vector
-  constexpr int NV = VPV / L;              // words per lane
-  constexpr int TEAMS = kRopeThreads / L;
-  grid_launch_dependents();
-  grid_dependency_wait();
-  const int64_t n = blockIdx.x;
-  const int kvh = a.c.kv_heads;
-  const int items = a.heads + 2 * kvh;
-  const int i0 = blockIdx.y * per, i1 = min(items, i0 + per);
-  const int lane = threadIdx.x % L, team = threadIdx.x / L;
-  const T* src = reinterpret_cast<const T*>(a.qkv) + n * a.qkv_stride;
-  uint4 u[IL][NV];
-  auto load = [&](int base) {
-#pragma unroll
-    for (int j = 0; j < IL; ++j) {
-      const int it = base + j * TEAMS + team;
-#pragma unroll
-      for (int v = 0; v < NV; ++v)
-        u[j][v] = it < i1 ? __ldg(reinterpret_cast<const uint4*>(src + (int64_t)it * D) + v * L + lane)
-                          : make_uint4(0u, 0u, 0u, 0u);
-    }
-  };
-  load(i0);  // before the position is waited for
-  const int64_t p = a.pos[n];
-  const int64_t slot = a.slots[n];
-  const bool pos_ok = p >= 0 && p < a.cs_positions;
-  const bool slot_ok = slot >= 0 && slot < a.c.pages * a.c.page;
-  if (threadIdx.x == 0 && (!pos_ok || slot >= a.c.pages * a.c.page)) raise_status(a.status, kStatusIndex);
-  const int64_t pg = slot_ok ? slot / a.c.page : 0;
-  const int off = slot_ok ? (int)(slot - pg * a.c.page) : 0;
-
-  float cs[NV][kVec];
-#pragma unroll
-  for (int v = 0; v < NV; ++v)
-#pragma unroll
-    for (int i = 0; i < kVec / 4; ++i) {
-      const float4 f = pos_ok ? __ldg(reinterpret_cast<const float4*>(a.cs + p * D + (v * L + lane) * kVec) + i)
-                              : make_float4(0.f, 0.f, 0.f, 0.f);
-      cs[v][4 * i] = f.x;
-      cs[v][4 * i + 1] = f.y;
-      cs[v][4 * i + 2] = f.z;
-      cs[v][4 * i + 3] = f.w;
-    }
-  // Every team of a warp takes the same number of rounds (the scale's shuffles need the whole warp).
-  for (int base = i0; base < i1; base += TEAMS * IL) {
-    if (base > i0) load(base);
-#pragma unroll
-    for (int j = 0; j < IL; ++j) {
-      const int it = base + j * TEAMS + team;
-      const bool turn = it < a.heads + kvh;
-      const bool live = it < i1;
-      float y[NV][kVec];
-      uint4 r[NV];
-      if (turn) {
-#pragma unroll
-        for (int v = 0; v < NV; ++v) {
-          float x[kVec];
-          Elem<T>::unpack(u[j][v], x);
-#pragma unroll
-          for (int i = 0; i < kVec / 2; ++i) {
-            const float re = x[2 * i], im = x[2 * i + 1], co = cs[v][2 * i], si = cs[v][2 * i + 1];
-            y[v][2 * i] = __fsub_rn(__fmul_rn(re, co), __fmul_rn(im, si));
-            y[v][2 * i + 1] = __fadd_rn(__fmul_rn(re, si), __fmul_rn(im, co));
-          }
-          r[v] = pos_ok ? Pack<T>::pack(y[v]) : make_uint4(0u, 0u, 0u, 0u);
-        }
-      } else {
-#pragma unroll
-        for (int v = 0; v < NV; ++v) r[v] = u[j][v];
-      }
-      if (live && it < a.heads) {
-#pragma unroll
-        for (int v = 0; v < NV; ++v)
-          reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.q_out) + (n * a.heads + it) * D)[v * L + lane] = r[v];
-      }
-      const bool is_k = it < a.heads + kvh;
-      const int h = it - a.heads - (is_k ? 0 : kvh);
-      const bool write = live && it >= a.heads && slot_ok && (pos_ok || !is_k);
-      const int64_t dst = pg * a.c.s_page + (int64_t)h * a.c.s_head + (int64_t)off * a.c.s_pos;
-      if constexpr (FP8) {
-        if (__all_sync(0xffffffffu, it < a.heads)) continue;  // a warp of query heads (the same for all its lanes)
-        uint32_t amax = 0u;
-#pragma unroll
-        for (int v = 0; v < NV; ++v) {
-          Elem<T>::unpack(r[v], y[v]);  // the vector as the model's type holds it
-#pragma unroll
-          for (int i = 0; i < kVec; ++i) {
-            const uint32_t b = __float_as_uint(y[v][i]) & 0x7fffffffu;
-            amax = max(amax, b < 0x7f800000u ? b : 0u);
-          }
-        }
-#pragma unroll
-        for (int o = L / 2; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        if (write) {
-          const int e = scale_exponent(amax);
-          const float inv = pow2(-e);
-          uint8_t* row = reinterpret_cast<uint8_t*>(is_k ? a.c.k : a.c.v) + dst;
-#pragma unroll
-          for (int v = 0; v < NV; ++v) {
-            if constexpr (kVec == 8)
-              reinterpret_cast<uint2*>(row)[v * L + lane] = make_uint2(codes4(y[v], inv), codes4(y[v] + 4, inv));
-            else
-              reinterpret_cast<uint32_t*>(row)[v * L + lane] = codes4(y[v], inv);
-          }
-          if (lane == 0) (is_k ? a.c.k_scale : a.c.v_scale)[(pg * kvh + h) * a.c.page + off] = (uint8_t)(e + 127);
-        }
-      } else if (write) {
-        T* row = reinterpret_cast<T*>(is_k ? a.c.k : a.c.v) + dst;
-#pragma unroll
-        for (int v = 0; v < NV; ++v) reinterpret_cast<uint4*>(row)[v * L + lane] = r[v];
-      }
-    }
-  }
 }
 
 constexpr int kReadThreads = 256;
@@ -191,7 +36,7 @@ constexpr int kReadThreads = 256;
 // 16 bytes of the output per thread and round. Threads find the tokens' places first (the sequence by bisection in the
 // offsets, the page in its table row); then all rounds' loads are in flight together, and every store of a warp covers
 // whole lines: 195 MB of an fp8 context 34 us (5741 GB/s); 44 us with 16-byte loads (two half-line stores each), token-major.
-template <typename T, int D, bool FP8, int R>
+template <typename T, int D, int KIND, int R>
 __global__ void __launch_bounds__(kReadThreads) paged_read_kernel(const PagedReadArgs a) {
   constexpr int kOut = 16 / sizeof(T);       // elements per thread and round
   constexpr int W = D / kOut;                // threads per vector
@@ -227,7 +72,7 @@ __global__ void __launch_bounds__(kReadThreads) paged_read_kernel(const PagedRea
   }
   __syncthreads();
   const int c = threadIdx.x % W;
-  using In = std::conditional_t<!FP8, uint4, std::conditional_t<kOut == 8, uint2, uint32_t>>;
+  using In = std::conditional_t<KIND == kOwnType, uint4, std::conditional_t<KIND == kFp8 && kOut == 8, uint2, uint32_t>>;
   In ku[R], vu[R];
   float ks[R], vs[R];
 #pragma unroll
@@ -238,12 +83,25 @@ __global__ void __launch_bounds__(kReadThreads) paged_read_kernel(const PagedRea
     vu[r] = In{};
     ks[r] = vs[r] = 0.f;
     if (page >= 0) {
-      const int64_t at = page * a.c.s_page + (int64_t)h * a.c.s_head + (int64_t)s_off[i] * a.c.s_pos + c * kOut;
-      constexpr int es = FP8 ? 1 : sizeof(T);
-      ku[r] = __ldcs(reinterpret_cast<const In*>(reinterpret_cast<const char*>(a.c.k) + at * es));
-      vu[r] = __ldcs(reinterpret_cast<const In*>(reinterpret_cast<const char*>(a.c.v) + at * es));
-      if (FP8) {
-        const int64_t si = (page * kvh + h) * a.c.page + s_off[i];
+      const int64_t row = page * a.c.s_page + (int64_t)h * a.c.s_head + (int64_t)s_off[i] * a.c.s_pos, at = row + c * kOut;
+      constexpr int es = KIND == kFp8 ? 1 : sizeof(T);
+      const int64_t si = (page * kvh + h) * a.c.page + s_off[i];
+      if constexpr (KIND == kInt4) {
+        const uint16_t* kr = reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(a.c.k) + row);
+        const uint16_t* vr = reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(a.c.v) + row);
+#pragma unroll
+        for (int q = 0; q < kOut / 4; ++q) {
+          ku[r] |= (uint32_t)__ldcs(kr + quad_at<D, true>(c * (kOut / 4) + q)) << (16 * q);
+          vu[r] |= (uint32_t)__ldcs(vr + quad_at<D, false>(c * (kOut / 4) + q)) << (16 * q);
+        }
+        const int64_t g = si * (D / 32) + c * kOut / 32;
+        ks[r] = bf16_value(__ldg(reinterpret_cast<const uint16_t*>(a.c.k_scale) + g));
+        vs[r] = bf16_value(__ldg(reinterpret_cast<const uint16_t*>(a.c.v_scale) + g));
+      } else {
+        ku[r] = __ldcs(reinterpret_cast<const In*>(reinterpret_cast<const char*>(a.c.k) + at * es));
+        vu[r] = __ldcs(reinterpret_cast<const In*>(reinterpret_cast<const char*>(a.c.v) + at * es));
+      }
+      if constexpr (KIND == kFp8) {
         ks[r] = __uint_as_float((uint32_t)__ldg(a.c.k_scale + si) << 23);
         vs[r] = __uint_as_float((uint32_t)__ldg(a.c.v_scale + si) << 23);
       }
@@ -256,7 +114,16 @@ __global__ void __launch_bounds__(kReadThreads) paged_read_kernel(const PagedRea
     const int64_t dst = (tok * kvh + h) * D + c * kOut;
     uint4* ko = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.k_out) + dst);
     uint4* vo = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.v_out) + dst);
-    if constexpr (FP8) {
+    if constexpr (KIND == kInt4) {
+      float kf[kOut], vf[kOut];
+#pragma unroll
+      for (int q = 0; q < kOut / 4; ++q) {
+        int4_values(ku[r] >> (16 * q), ks[r], kf + 4 * q);
+        int4_values(vu[r] >> (16 * q), vs[r], vf + 4 * q);
+      }
+      __stcs(ko, Pack<T>::pack(kf));
+      __stcs(vo, Pack<T>::pack(vf));
+    } else if constexpr (KIND == kFp8) {
       uint32_t kw[2], vw[2];
       if constexpr (kOut == 8) {
         kw[0] = ku[r].x, kw[1] = ku[r].y, vw[0] = vu[r].x, vw[1] = vu[r].y;
@@ -281,87 +148,42 @@ __global__ void __launch_bounds__(kReadThreads) paged_read_kernel(const PagedRea
   }
 }
 
-template <typename T, int D, bool FP8>
-cudaError_t rope_launch(const PagedRopeArgs& a, cudaStream_t s) {
-  constexpr int VPV = D / Elem<T>::kVec;
-  constexpr int TEAMS = kRopeThreads / (VPV < 32 ? VPV : 32);
-  const int items = a.heads + 2 * a.c.kv_heads;
-  // A token's vectors go to several CTAs while the tokens alone leave SMs idle (a decode step).
-  const int want = 2 * device_sm_count();
-  int parts = (want + a.n - 1) / a.n;
-  const int most = (items + TEAMS - 1) / TEAMS;
-  parts = parts < 1 ? 1 : (parts > most ? most : parts);
-  const int per = (items + parts - 1) / parts;
-  const dim3 grid((unsigned)a.n, (unsigned)((items + per - 1) / per));
-  // Vectors per thread in flight: of 4, 3 and 2, the one that leaves the fewest without work.
-  const int rounds = (per + TEAMS - 1) / TEAMS;
-  int il = 1;
-  if (rounds > 1) {
-    int idle = 1 << 30;
-    for (int k = 4; k >= 2; --k) {
-      const int w = (rounds + k - 1) / k * k - rounds;
-      if (w < idle) {
-        idle = w;
-        il = k;
-      }
-    }
-  }
-  switch (il) {
-    case 1: return launch_dependent(paged_rope_kernel<T, D, FP8, 1>, grid, dim3(kRopeThreads), 0, s, a, per);
-    case 2: return launch_dependent(paged_rope_kernel<T, D, FP8, 2>, grid, dim3(kRopeThreads), 0, s, a, per);
-    case 3: return launch_dependent(paged_rope_kernel<T, D, FP8, 3>, grid, dim3(kRopeThreads), 0, s, a, per);
-    default: return launch_dependent(paged_rope_kernel<T, D, FP8, 4>, grid, dim3(kRopeThreads), 0, s, a, per);
-  }
-}
-
-template <typename T, int D, bool FP8>
+template <typename T, int D, int KIND>
 cudaError_t read_launch(const PagedReadArgs& a, cudaStream_t s) {
   constexpr int TP = kReadThreads / (D / (16 / (int)sizeof(T)));
   // Four rounds per CTA, one where four would leave SMs without work.
   const int64_t four = (a.tokens + 4 * TP - 1) / (4 * TP) * a.c.kv_heads;
   const int64_t one = (a.tokens + TP - 1) / TP * a.c.kv_heads;
   if (four >= 2 * device_sm_count())
-    return launch_dependent(paged_read_kernel<T, D, FP8, 4>, dim3((unsigned)four), dim3(kReadThreads), 0, s, a);
-  return launch_dependent(paged_read_kernel<T, D, FP8, 1>, dim3((unsigned)one), dim3(kReadThreads), 0, s, a);
+    return launch_dependent(paged_read_kernel<T, D, KIND, 4>, dim3((unsigned)four), dim3(kReadThreads), 0, s, a);
+  return launch_dependent(paged_read_kernel<T, D, KIND, 1>, dim3((unsigned)one), dim3(kReadThreads), 0, s, a);
 }
 
-#define OMNI_DIM_SWITCH(DIM, CALL)      \
-  switch (DIM) {                        \
-    case 16: return CALL(16);           \
-    case 32: return CALL(32);           \
-    case 64: return CALL(64);           \
-    case 128: return CALL(128);         \
-    case 256: return CALL(256);         \
-    case 512: return CALL(512);         \
-    default: return cudaErrorInvalidValue; \
-  }
-
-template <typename T, bool FP8>
-cudaError_t rope_dim(const PagedRopeArgs& a, cudaStream_t s) {
-#define CALL(D) rope_launch<T, D, FP8>(a, s)
-  OMNI_DIM_SWITCH(a.c.dim, CALL)
-#undef CALL
-}
-
-template <typename T, bool FP8>
+template <typename T, int KIND>
 cudaError_t read_dim(const PagedReadArgs& a, cudaStream_t s) {
-#define CALL(D) read_launch<T, D, FP8>(a, s)
+#define CALL(D) read_launch<T, D, KIND == kInt4 && D < 32 ? -1 : KIND>(a, s)
+  if (KIND == kInt4 && a.c.dim < 32) return cudaErrorInvalidValue;
   OMNI_DIM_SWITCH(a.c.dim, CALL)
 #undef CALL
+}
+
+template <typename T>
+cudaError_t read_kind(const PagedReadArgs& a, cudaStream_t s) {
+  if (a.c.type == kFp8) return read_dim<T, kFp8>(a, s);
+  if (a.c.type == kInt4) return read_dim<T, kInt4>(a, s);
+  return read_dim<T, kOwnType>(a, s);
 }
 
 }  // namespace
 
 cudaError_t launch_paged_rope_kv(int dtype, const PagedRopeArgs& a, cudaStream_t stream) {
   if (a.n <= 0) return cudaSuccess;
-  if (dtype == kBF16) return a.c.type == kFp8 ? rope_dim<__nv_bfloat16, true>(a, stream) : rope_dim<__nv_bfloat16, false>(a, stream);
-  return a.c.type == kFp8 ? rope_dim<float, true>(a, stream) : rope_dim<float, false>(a, stream);
+  return dtype == kBF16 ? rope_kind<__nv_bfloat16, false>(a, stream) : rope_kind<float, false>(a, stream);
 }
 
 cudaError_t launch_paged_kv_read(int dtype, const PagedReadArgs& a, cudaStream_t stream) {
   if (a.tokens <= 0) return cudaSuccess;
-  if (dtype == kBF16) return a.c.type == kFp8 ? read_dim<__nv_bfloat16, true>(a, stream) : read_dim<__nv_bfloat16, false>(a, stream);
-  return a.c.type == kFp8 ? read_dim<float, true>(a, stream) : read_dim<float, false>(a, stream);
+  return dtype == kBF16 ? read_kind<__nv_bfloat16>(a, stream) : read_kind<float>(a, stream);
 }
 
 }  // namespace omni

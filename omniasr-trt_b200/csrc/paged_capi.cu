@@ -1,5 +1,6 @@
 // extern "C" entry points of the paged-cache operators and the packed-prompt attention: argument checks and launches.
 
+#include <math.h>
 #include <stdarg.h>
 #include <stdio.h>
 
@@ -28,16 +29,18 @@ int done(const char* name, cudaError_t e) {
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-int esize(int type) { return type == OMNIASR_F32 ? 4 : type == OMNIASR_BF16 ? 2 : 1; }
+int esize(int type) { return type == OMNIASR_F32 ? 4 : type == OMNIASR_BF16 ? 2 : 1; }  // (of 4-bit pages: a byte of two codes)
 bool stride_ok(int64_t stride, int type) { return stride >= 0 && stride * esize(type) % 16 == 0; }
 
-// dtype, head_dim and head counts; `type`: the cache's element type (dtype itself, or fp8).
+// dtype, head_dim and head counts; `type`: the cache's element type (dtype itself, fp8 or int4).
 int check(const char* name, int dtype, int type, int dim, int heads, int kv_heads) {
   if (dtype != OMNIASR_BF16 && dtype != OMNIASR_F32) return fail(OMNIASR_ERR_UNSUPPORTED, "%s: dtype %d", name, dtype);
-  if (type != dtype && type != OMNIASR_FP8)
-    return fail(OMNIASR_ERR_UNSUPPORTED, "%s: cache type %d with dtype %d (the same, or fp8)", name, type, dtype);
+  if (type != dtype && type != OMNIASR_FP8 && type != OMNIASR_INT4)
+    return fail(OMNIASR_ERR_UNSUPPORTED, "%s: cache type %d with dtype %d (the same, fp8 or int4)", name, type, dtype);
   if (!omni::dim_supported(dtype, dim))
     return fail(OMNIASR_ERR_UNSUPPORTED, "%s: head_dim %d (supported: 16, 32, 64, 128, 256, 512)", name, dim);
+  if (type == OMNIASR_INT4 && dim < 32)
+    return fail(OMNIASR_ERR_UNSUPPORTED, "%s: head_dim %d with an int4 cache (its groups are 32 dims)", name, dim);
   if (kv_heads <= 0 || heads <= 0 || heads > 65535 || heads % kv_heads)
     return fail(OMNIASR_ERR_ARGUMENT, "%s: heads %d, kv_heads %d (a multiple, at most 65535)", name, heads, kv_heads);
   int dev = 0;
@@ -55,11 +58,12 @@ int check_pages(const char* name, const omni::PageCache& c) {
   if (!stride_ok(c.s_page, c.type) || !stride_ok(c.s_head, c.type) || !stride_ok(c.s_pos, c.type))
     return fail(OMNIASR_ERR_ARGUMENT, "%s: page strides (%lld, %lld, %lld) must keep 16-byte alignment", name,
                 (long long)c.s_page, (long long)c.s_head, (long long)c.s_pos);
-  if (c.page > 1 && c.s_pos < c.dim) return fail(OMNIASR_ERR_ARGUMENT, "%s: positions overlap", name);
-  if (c.type == OMNIASR_FP8 && (!c.k_scale || !c.v_scale))
-    return fail(OMNIASR_ERR_ARGUMENT, "%s: an fp8 cache needs its scale bytes", name);
-  if (c.type == OMNIASR_FP8 && (!aligned16(c.k_scale) || !aligned16(c.v_scale)))
-    return fail(OMNIASR_ERR_ARGUMENT, "%s: scale bytes must be 16-byte aligned", name);
+  const bool coded = c.type == OMNIASR_FP8 || c.type == OMNIASR_INT4;
+  if (c.page > 1 && c.s_pos < (c.type == OMNIASR_INT4 ? c.dim / 2 : c.dim))
+    return fail(OMNIASR_ERR_ARGUMENT, "%s: positions overlap", name);
+  if (coded && (!c.k_scale || !c.v_scale)) return fail(OMNIASR_ERR_ARGUMENT, "%s: an fp8 or int4 cache needs its scales", name);
+  if (coded && (!aligned16(c.k_scale) || !aligned16(c.v_scale)))
+    return fail(OMNIASR_ERR_ARGUMENT, "%s: scales must be 16-byte aligned", name);
   return OMNIASR_OK;
 }
 
@@ -81,15 +85,12 @@ omni::PageCache cache_of(const void* k, const void* v, const void* ks, const voi
   return c;
 }
 
-}  // namespace
-
-extern "C" {
-
-int omniasr_paged_rope_kv(const void* qkv, int64_t qkv_stride, const float* cs, int64_t cs_positions, const int64_t* pos,
-                          const int64_t* slots, void* q_out, void* k_pages, void* v_pages, void* k_scale, void* v_scale,
-                          int64_t pages, int page, int64_t stride_page, int64_t stride_head, int64_t stride_pos, int n,
-                          int heads, int kv_heads, int dim, int dtype, int cache_type, int* status, cudaStream_t stream) {
-  const char* name = "paged_rope_kv";
+// paged_rope_kv and paged_norm_rope_kv (norm).
+int rope(const char* name, bool norm, const void* q_norm, const void* k_norm, float eps, const void* qkv, int64_t qkv_stride,
+         const float* cs, int64_t cs_positions, const int64_t* pos, const int64_t* slots, void* q_out, void* k_pages,
+         void* v_pages, void* k_scale, void* v_scale, int64_t pages, int page, int64_t stride_page, int64_t stride_head,
+         int64_t stride_pos, int n, int heads, int kv_heads, int dim, int dtype, int cache_type, int* status,
+         cudaStream_t stream) {
   if (int e = check(name, dtype, cache_type, dim, heads, kv_heads)) return e;
   if (n < 0 || cs_positions < 0) return fail(OMNIASR_ERR_ARGUMENT, "%s: n %d", name, n);
   omni::PagedRopeArgs a;
@@ -99,6 +100,14 @@ int omniasr_paged_rope_kv(const void* qkv, int64_t qkv_stride, const float* cs, 
   if (!qkv || !cs || !pos || !slots || !q_out) return fail(OMNIASR_ERR_ARGUMENT, "%s: null pointer", name);
   if (!aligned16(qkv) || !aligned16(cs) || !aligned16(q_out) || !stride_ok(qkv_stride, dtype))
     return fail(OMNIASR_ERR_ARGUMENT, "%s: qkv, cs and q must keep 16-byte alignment", name);
+  if (norm) {
+    if (!q_norm || !k_norm || !aligned16(q_norm) || !aligned16(k_norm))
+      return fail(OMNIASR_ERR_ARGUMENT, "%s: the norms' weights must be 16-byte aligned", name);
+    if (!(eps >= 0.f) || isinf(eps)) return fail(OMNIASR_ERR_ARGUMENT, "%s: eps %g", name, (double)eps);
+  }
+  a.q_norm = q_norm;
+  a.k_norm = k_norm;
+  a.eps = eps;
   a.qkv = qkv;
   a.qkv_stride = qkv_stride;
   a.cs = cs;
@@ -109,7 +118,30 @@ int omniasr_paged_rope_kv(const void* qkv, int64_t qkv_stride, const float* cs, 
   a.n = n;
   a.heads = heads;
   a.status = status;
-  return done(name, omni::launch_paged_rope_kv(dtype, a, stream));
+  return done(name, norm ? omni::launch_paged_norm_rope_kv(dtype, a, stream) : omni::launch_paged_rope_kv(dtype, a, stream));
+}
+
+}  // namespace
+
+extern "C" {
+
+int omniasr_paged_rope_kv(const void* qkv, int64_t qkv_stride, const float* cs, int64_t cs_positions, const int64_t* pos,
+                          const int64_t* slots, void* q_out, void* k_pages, void* v_pages, void* k_scale, void* v_scale,
+                          int64_t pages, int page, int64_t stride_page, int64_t stride_head, int64_t stride_pos, int n,
+                          int heads, int kv_heads, int dim, int dtype, int cache_type, int* status, cudaStream_t stream) {
+  return rope("paged_rope_kv", false, nullptr, nullptr, 0.f, qkv, qkv_stride, cs, cs_positions, pos, slots, q_out, k_pages,
+              v_pages, k_scale, v_scale, pages, page, stride_page, stride_head, stride_pos, n, heads, kv_heads, dim, dtype,
+              cache_type, status, stream);
+}
+
+int omniasr_paged_norm_rope_kv(const void* qkv, int64_t qkv_stride, const void* q_norm, const void* k_norm, float eps,
+                               const float* cs, int64_t cs_positions, const int64_t* pos, const int64_t* slots, void* q_out,
+                               void* k_pages, void* v_pages, void* k_scale, void* v_scale, int64_t pages, int page,
+                               int64_t stride_page, int64_t stride_head, int64_t stride_pos, int n, int heads, int kv_heads,
+                               int dim, int dtype, int cache_type, int* status, cudaStream_t stream) {
+  return rope("paged_norm_rope_kv", true, q_norm, k_norm, eps, qkv, qkv_stride, cs, cs_positions, pos, slots, q_out, k_pages,
+              v_pages, k_scale, v_scale, pages, page, stride_page, stride_head, stride_pos, n, heads, kv_heads, dim, dtype,
+              cache_type, status, stream);
 }
 
 int omniasr_paged_kv_read(const void* k_pages, const void* v_pages, const void* k_scale, const void* v_scale, int64_t pages,

@@ -14,7 +14,7 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent.parent / "lib" / "libomniasr_b200.so"
 BINDING_PATH = LIB_PATH.parent / "_omniasr_torch.so"  # csrc/binding.cpp: the calls that take torch tensors themselves
 
-BF16, F32, FP8 = 0, 1, 2
+BF16, F32, FP8, INT4 = 0, 1, 2, 3
 OK, ERR_ARGUMENT, ERR_UNSUPPORTED, ERR_WORKSPACE, ERR_CUDA, ERR_DEVICE = range(6)
 DECODE, DRAFT, BEAM = 0, 1, 2
 
@@ -60,6 +60,8 @@ SIGNATURES = {
     "omniasr_accept": (_i, [_p, _p, _p, _i64, _i64, _p, _p, _p, _p, _p, _p, _i, _i, _i64, _i64, _p, _p]),
     "omniasr_paged_rope_kv": (_i, [_p, _i64, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _i, _i64, _i64, _i64, _i, _i, _i,
                                    _i, _i, _i, _p, _p]),
+    "omniasr_paged_norm_rope_kv": (_i, [_p, _i64, _p, _p, _f, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _i, _i64, _i64, _i64,
+                                        _i, _i, _i, _i, _i, _i, _p, _p]),
     "omniasr_paged_kv_read": (_i, [_p, _p, _p, _p, _i64, _i, _i64, _i64, _i64, _p, _i64, _i, _i, _p, _i64, _p, _p, _i, _i,
                                    _i, _i, _p, _p]),
     "omniasr_paged_attention_workspace": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i, _i]),

@@ -598,9 +598,23 @@ def paged_rope_kv(qkv: torch.Tensor, cs: torch.Tensor, pos: torch.Tensor, k_page
     ``k_pages``/``v_pages`` [pages, kv_heads, page, D]; returns the rotated q [N, heads, D]. Pages hold qkv's dtype, or
     float8_e4m3fn codes with one scale byte per vector in ``k_scale``/``v_scale`` (uint8 [pages, kv_heads, page]): the
     vector x is held as codes of x * 2^-e and the byte e + 127, e the smallest integer with max|x| <= 448 * 2^e (within
-    [-40, 40])."""
+    [-40, 40]); or (head_dim 32 and more) uint8 [pages, kv_heads, page, D / 2] of 4-bit codes, two to a byte, with a scale per
+    32 dims in ``k_scale``/``v_scale`` (bfloat16 [pages, kv_heads, page, D / 32]): s = -m / 8 with m the group's value of largest
+    magnitude, codes x / s rounded to [-8, 7] plus 8, in the order of ``include/omniasr_b200.h`` (:func:`paged_kv_read` gives
+    the values); a group with an infinity or a NaN reads as NaN."""
     native, status, stream, _ = _context(qkv.device)
     return native.paged_rope_kv(qkv, cs, pos, k_pages, v_pages, slots, heads, kv_heads, k_scale, v_scale, status, stream)
+
+
+def paged_norm_rope_kv(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor, cs: torch.Tensor, pos: torch.Tensor,
+                       k_pages: torch.Tensor, v_pages: torch.Tensor, slots: torch.Tensor, heads: int, kv_heads: int,
+                       eps: float = 1e-6, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`paged_rope_kv` of a model that norms its queries and keys: each head's q and k vector x becomes
+    ``x * rsqrt(mean(x ** 2) + eps) * w`` before the rotation, w being ``q_norm`` / ``k_norm`` [D] (qkv's dtype), in fp32 with one
+    rounding, after the rotation. v is not normed."""
+    native, status, stream, _ = _context(qkv.device)
+    return native.paged_norm_rope_kv(qkv, q_norm, k_norm, cs, pos, k_pages, v_pages, slots, heads, kv_heads, eps, k_scale, v_scale,
+                                     status, stream)
 
 
 def paged_kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, offsets: torch.Tensor,
@@ -608,9 +622,9 @@ def paged_kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torc
                   dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Pages read back as packed rows: k and v [tokens, kv_heads, D], rows ``offsets[i]`` .. ``offsets[i + 1] - 1`` holding
     the first positions of ``page_table`` row i (``offsets`` [rows + 1], ascending, ``tokens`` the last; output rows
-    outside them are zeros). 8-bit pages are read as ``dtype`` (default bfloat16), others as what they hold."""
+    outside them are zeros). 8-bit and 4-bit pages are read as ``dtype`` (default bfloat16), others as what they hold."""
     if dtype is None:
-        dtype = torch.bfloat16 if k_pages.dtype == torch.float8_e4m3fn else k_pages.dtype
+        dtype = torch.bfloat16 if k_pages.dtype in (torch.float8_e4m3fn, torch.uint8) else k_pages.dtype
     native, status, stream, _ = _context(k_pages.device)
     return native.paged_kv_read(k_pages, v_pages, page_table, offsets, tokens, k_scale, v_scale, dtype, status, stream)
 
