@@ -217,6 +217,17 @@ int omniasr_decode_gemm(const void* x, int64_t x_stride, int rows, const void* w
                         int mode, const void* residual, int64_t residual_stride, void* y, int64_t y_stride,
                         void* workspace, size_t workspace_bytes, int* status, cudaStream_t stream);
 
+/* omniasr_decode_gemm() over 4-bit weights: W[j, c] = s[j, c / group] * (code[j, c] - 8), group 32, 64 or 128 columns (the last
+ * one of a row may be shorter), k a multiple of 32. Modes as omniasr_decode_gemm(), but every value is rounded once, at the end, and
+ * SwiGLU's halves are not rounded before. `codes` holds 8 weight rows x 128 columns in 512 bytes, [ceil(weight rows / 8)][ceil(k /
+ * 128)][8][4] words of 16 bytes (what lies past the weights: code 8): of a row's 128 columns word t of 4 holds, in its 32-bit word
+ * w, columns 32 w + 8 t + 2 i in bits 4 i .. and 32 w + 8 t + 2 i + 1 in bits 16 + 4 i .., i < 4. `scales` is bf16 [ceil(weight rows /
+ * 8)][ceil(k / group)][8]. x rows, codes and scales 16-byte aligned; no workspace. The weights must not be written by the kernel
+ * launched just before on the same stream. No counterpart in the reference. */
+int omniasr_decode_gemm_int4(const void* x, int64_t x_stride, int rows, const void* codes, const void* scales, int n, int k,
+                             int group, int mode, const void* residual, int64_t residual_stride, void* y, int64_t y_stride,
+                             cudaStream_t stream);
+
 /* The QKV product of the decoder step with RoPE and the KV-cache append in its epilogue (bf16, rows <= 64): the
  * product qkv = x . w^T (w [3 * heads * dim, k]) is formed, each value rounded to bf16 as the GEMM's output would
  * be, and then handled as omniasr_rope_kv() handles a qkv row -- q rotated into q_out [rows, heads, dim], k rotated
@@ -311,6 +322,34 @@ int omniasr_paged_attention(const void* q, const void* k_pages, const void* v_pa
                             const int32_t* table, int64_t table_stride, int table_width, const int64_t* lengths, void* out,
                             int rows, int tokens, int heads, int kv_heads, int dim, float scale, int dtype, int cache_type,
                             void* workspace, size_t workspace_bytes, int* status, cudaStream_t stream);
+
+/* A step's tables on the GPU. The state: length [seqs] (int64, positions of each sequence), table [seqs, table_width] (int32, the
+ * page numbers of a sequence's positions in order; row stride table_stride), and a stack of free page numbers, the first
+ * *free_count (int64) of free [pages] (int32), its top last. Request i < requests (at most 8192) adds fresh[i] tokens to sequence
+ * rows[i]; `taken` [requests] (one byte each) says whether it got the pages that this takes. Requests are taken in order: one that
+ * needs pages if they and those of the requests before it that needed some are free, one that needs none always. Refused, with
+ * status bit 1, are a sequence outside the state, a second request of a sequence, a negative number, tokens past `tokens`; without,
+ * positions past batch_width pages. Pages come from the top of the stack, a request's first page first, into its table row and off
+ * the stack; lengths grow. Outputs: pos, slots [tokens] (int64: each token's position, and page number * page + offset, -1 for
+ * tokens of refused requests; 0 and -1 behind the last token); batch_table [requests, batch_width] (contiguous; the sequences' page
+ * numbers, 0 past them); lengths [requests] = positions before the step + 1 (0: refused), as omniasr_paged_attention() takes them;
+ * q_offsets, k_offsets [requests + 1], sums of the new tokens (refused ones' too, held to `tokens`) and of the positions after the
+ * step. The workspace (OMNIASR_PLAN_WORKSPACE bytes, 16-byte aligned) holds a counter under the rule of
+ * omniasr_attention_workspace(). */
+#define OMNIASR_PLAN_WORKSPACE 16
+int omniasr_paged_plan(const int64_t* rows, const int64_t* fresh, int requests, int64_t tokens, int page, int64_t* length,
+                       int64_t seqs, int32_t* table, int64_t table_stride, int table_width, int32_t* free, int64_t* free_count,
+                       int64_t pages, int64_t* pos, int64_t* slots, int32_t* batch_table, int batch_width, int64_t* lengths,
+                       int64_t* q_offsets, int64_t* k_offsets, uint8_t* taken, void* workspace, size_t workspace_bytes, int* status,
+                       cudaStream_t stream);
+
+/* Sequence rows[i] keeps its first keep[i] positions; the pages past them go back onto the stack, the last request's first and each
+ * request's last page first, so that a trim to the lengths before omniasr_paged_plan() of the same requests leaves the stack as it
+ * was. A request that names no sequence, one that an earlier request names, or more positions than there are changes nothing and
+ * raises status bit 1; so do all where more pages would lie on the stack than `pages`. Workspace as omniasr_paged_plan(). */
+int omniasr_paged_trim(const int64_t* rows, const int64_t* keep, int requests, int page, int64_t* length, int64_t seqs,
+                       int32_t* table, int64_t table_stride, int table_width, int32_t* free, int64_t* free_count, int64_t pages,
+                       void* workspace, size_t workspace_bytes, int* status, cudaStream_t stream);
 
 /* Causal attention of packed sequences with grouped heads: sequence s has queries q_offsets[s] .. q_offsets[s + 1] - 1 of
  * q [q_tokens, heads, dim] and keys k_offsets[s] .. k_offsets[s + 1] - 1 of k / v [k_tokens, kv_heads, dim] (token and

@@ -236,6 +236,95 @@ py::object packed_attention(const at::Tensor& q, const at::Tensor& k, const at::
   return py::cast(out);
 }
 
+at::Tensor decode_gemm_int4(const at::Tensor& x, const at::Tensor& codes, const at::Tensor& scales, int64_t wrows, int64_t k,
+                            int64_t group, int64_t mode, const Opt& residual, const Opt& out, int64_t stream) {
+  const char* name = "decode_gemm_int4";
+  if (x.scalar_type() != at::kBFloat16 || x.dim() != 2 || x.size(1) != k || (k > 1 && x.size(0) && x.stride(1) != 1))
+    refuse(name, "x must be bfloat16 [rows, " + std::to_string(k) + "] with unit inner stride");
+  const int64_t rows = x.size(0), n = mode == OMNIASR_GEMM_SWIGLU ? wrows / 2 : wrows;
+  if (mode == OMNIASR_GEMM_SWIGLU && wrows % 2) refuse(name, "swiglu needs the rows of [gate; inner]");
+  auto bf16_rows = [&](const at::Tensor& t, const char* what) {
+    if (t.scalar_type() != at::kBFloat16 || t.dim() != 2 || t.size(0) != rows || t.size(1) != n || (n > 1 && rows && t.stride(1) != 1))
+      refuse(name, std::string(what) + " must be bfloat16 [rows, n] with unit inner stride");
+  };
+  if ((mode == OMNIASR_GEMM_RESIDUAL) != residual.has_value()) refuse(name, "a residual belongs to the residual mode, and that to it");
+  if (residual) bf16_rows(*residual, "residual");
+  if (out) bf16_rows(*out, "out");
+  if (rows > 64) refuse(name, "at most 64 rows");
+  at::Tensor y = out ? *out : at::empty({rows, n}, x.options());
+  if (rows == 0 || n == 0) return y;
+  same_device(name, x, {&codes, &scales, &y});
+  if (residual) same_device(name, x, {&*residual});
+  done("omniasr_decode_gemm_int4",
+       omniasr_decode_gemm_int4(x.data_ptr(), stride_of(x, 0), (int)rows, codes.data_ptr(), scales.data_ptr(), (int)n, (int)k,
+                                (int)group, (int)mode, residual ? residual->data_ptr() : nullptr,
+                                residual ? stride_of(*residual, 0) : 0, y.data_ptr(), stride_of(y, 0), stream_of(stream)));
+  return y;
+}
+
+struct Tables {
+  int64_t requests;
+  at::Tensor rows, want;
+};
+
+Tables tables_of(const char* name, const at::Tensor& rows, const at::Tensor& want, int64_t page, const at::Tensor& length,
+                 const at::Tensor& table, const at::Tensor& free, const at::Tensor& free_count) {
+  if (rows.dim() != 1 || want.sizes() != rows.sizes()) refuse(name, "rows and their numbers must be [requests]");
+  if (length.scalar_type() != at::kLong || length.dim() != 1 || !length.is_contiguous())
+    refuse(name, "length must be contiguous int64 [sequences]");
+  if (table.scalar_type() != at::kInt || table.dim() != 2 || table.size(0) != length.size(0) || (table.size(1) > 1 && table.stride(1) != 1))
+    refuse(name, "table must be int32 [sequences, width] with unit inner stride");
+  if (free.scalar_type() != at::kInt || free.dim() != 1 || !free.is_contiguous()) refuse(name, "free must be contiguous int32 [pages]");
+  if (free_count.scalar_type() != at::kLong || free_count.numel() != 1) refuse(name, "free_count must be one int64");
+  if (page < 1 || page > 0x7fffffff || table.size(1) > 0x7fffffff) refuse(name, "pages of " + std::to_string(page) + " positions");
+  if (rows.size(0) > 0x7fffffff) refuse(name, "too many requests");
+  same_device(name, length, {&rows, &want, &table, &free, &free_count});
+  return {rows.size(0), index_of(rows), index_of(want)};
+}
+
+// (A table of one row or none may have any stride.)
+int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+py::object paged_plan(const at::Tensor& rows, const at::Tensor& fresh, int64_t tokens, int64_t page, const at::Tensor& length,
+                      const at::Tensor& table, const at::Tensor& free, const at::Tensor& free_count, std::optional<int64_t> width,
+                      int64_t status, int64_t stream, const Opt& ws) {
+  const char* name = "paged_plan";
+  const Tables t = tables_of(name, rows, fresh, page, length, table, free, free_count);
+  const int64_t w = width ? *width : table.size(1);
+  if (tokens < 0 || tokens > 0x7fffffff) refuse(name, std::to_string(tokens) + " tokens");
+  if (w < 0 || w > table.size(1)) refuse(name, "a width of " + std::to_string(w) + " of a table of " + std::to_string(table.size(1)));
+  if (!ws) return py::int_(OMNIASR_PLAN_WORKSPACE);
+  const int64_t b = t.requests;
+  const auto i64 = length.options();
+  // One allocation for the int64 outputs: positions, slots, lengths, offsets.
+  at::Tensor all = at::empty({2 * tokens + 3 * b + 2}, i64);
+  auto part = [&](int64_t from, int64_t n) { return all.narrow(0, from, n); };
+  at::Tensor pos = part(0, tokens), slots = part(tokens, tokens), lengths = part(2 * tokens, b), qo = part(2 * tokens + b, b + 1),
+             ko = part(2 * tokens + 2 * b + 1, b + 1);
+  at::Tensor out = at::empty({b, w}, table.options()), taken = at::empty({b}, i64.dtype(at::kBool));
+  done("omniasr_paged_plan",
+       omniasr_paged_plan(t.rows.data_ptr<int64_t>(), t.want.data_ptr<int64_t>(), (int)b, tokens, (int)page, length.data_ptr<int64_t>(),
+                          length.size(0), table.data_ptr<int32_t>(), row_stride(table), (int)table.size(1), free.data_ptr<int32_t>(),
+                          free_count.data_ptr<int64_t>(), free.size(0), pos.data_ptr<int64_t>(), slots.data_ptr<int64_t>(),
+                          out.data_ptr<int32_t>(), (int)w, lengths.data_ptr<int64_t>(), qo.data_ptr<int64_t>(), ko.data_ptr<int64_t>(),
+                          reinterpret_cast<uint8_t*>(taken.data_ptr()), ws->data_ptr(), ws->numel(), status_of(status),
+                          stream_of(stream)));
+  return py::make_tuple(pos, slots, out, lengths, qo, ko, taken);
+}
+
+py::object paged_trim(const at::Tensor& rows, const at::Tensor& keep, int64_t page, const at::Tensor& length, const at::Tensor& table,
+                      const at::Tensor& free, const at::Tensor& free_count, int64_t status, int64_t stream, const Opt& ws) {
+  const char* name = "paged_trim";
+  const Tables t = tables_of(name, rows, keep, page, length, table, free, free_count);
+  if (!ws) return py::int_(OMNIASR_PLAN_WORKSPACE);
+  done("omniasr_paged_trim",
+       omniasr_paged_trim(t.rows.data_ptr<int64_t>(), t.want.data_ptr<int64_t>(), (int)t.requests, (int)page, length.data_ptr<int64_t>(),
+                          length.size(0), table.data_ptr<int32_t>(), row_stride(table), (int)table.size(1), free.data_ptr<int32_t>(),
+                          free_count.data_ptr<int64_t>(), free.size(0), ws->data_ptr(), ws->numel(), status_of(status),
+                          stream_of(stream)));
+  return py::none();
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_omniasr_torch, m) {
@@ -244,4 +333,7 @@ PYBIND11_MODULE(_omniasr_torch, m) {
   m.def("paged_kv_read", &paged_kv_read);
   m.def("paged_attention", &paged_attention);
   m.def("packed_attention", &packed_attention);
+  m.def("decode_gemm_int4", &decode_gemm_int4);
+  m.def("paged_plan", &paged_plan);
+  m.def("paged_trim", &paged_trim);
 }

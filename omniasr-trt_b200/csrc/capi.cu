@@ -14,6 +14,7 @@
 #include "rope_kv.cuh"
 #include "spec.cuh"
 #include "wgemm.cuh"
+#include "wgemm4.cuh"
 
 static_assert(omni::kCounterBytes == OMNIASR_ATTENTION_COUNTER_BYTES, "counter prefix of the decode / draft workspace");
 
@@ -773,6 +774,45 @@ int omniasr_decode_gemm(const void* x, int64_t x_stride, int rows, const void* w
   a.status = status;
   return cuda_status(omni::launch_decode_gemm(x, x_stride, w, w_stride, a, workspace, workspace_bytes, stream),
                      "decode_gemm launch");
+}
+
+int omniasr_decode_gemm_int4(const void* x, int64_t x_stride, int rows, const void* codes, const void* scales, int n, int k,
+                             int group, int mode, const void* residual, int64_t residual_stride, void* y, int64_t y_stride,
+                             cudaStream_t stream) {
+  if (int e = check_device()) return e;
+  if (rows < 0 || rows > omni::kGemmMaxRows || n < 0 || k < 0 || k % 32 || n > 0x3fffffff)
+    return fail(OMNIASR_ERR_ARGUMENT, "decode_gemm_int4: rows %d (at most %d), n %d, k %d (a multiple of 32)", rows,
+                omni::kGemmMaxRows, n, k);
+  if (group != 32 && group != 64 && group != 128)
+    return fail(OMNIASR_ERR_UNSUPPORTED, "decode_gemm_int4: groups of %d (supported: 32, 64, 128)", group);
+  if (mode != omni::kGemmStore && mode != omni::kGemmResidual && mode != omni::kGemmSwiglu)
+    return fail(OMNIASR_ERR_ARGUMENT, "decode_gemm_int4: mode %d", mode);
+  if (rows == 0 || n == 0) return ok();
+  if (k == 0) return fail(OMNIASR_ERR_ARGUMENT, "decode_gemm_int4: k = 0");
+  if (!x || !codes || !scales || !y) return fail(OMNIASR_ERR_ARGUMENT, "decode_gemm_int4: null pointer");
+  if (mode == omni::kGemmResidual && !residual) return fail(OMNIASR_ERR_ARGUMENT, "decode_gemm_int4: no residual");
+  if (!aligned16(x) || !aligned16(codes) || !aligned16(scales) || (x_stride * 2) % 16 || x_stride < (rows > 1 ? k : 0))
+    return fail(OMNIASR_ERR_ARGUMENT, "decode_gemm_int4: x and the weights must be 16-byte aligned, row strides >= k keeping it");
+  if (rows > 1 && (y_stride < n || (mode == omni::kGemmResidual && residual_stride < n)))
+    return fail(OMNIASR_ERR_ARGUMENT, "decode_gemm_int4: output / residual row stride < n");
+  omni::Gemm4Args a{};
+  a.x = static_cast<const __nv_bfloat16*>(x);
+  a.ldx = x_stride;
+  a.codes = static_cast<const uint4*>(codes);
+  a.scales = static_cast<const uint16_t*>(scales);
+  a.rows = rows;
+  a.n = n;
+  a.k = k;
+  a.wrows = mode == omni::kGemmSwiglu ? 2 * n : n;
+  a.blocks = (k + 127) / 128;
+  a.groups = (k + group - 1) / group;
+  a.group = group;
+  a.mode = mode;
+  a.residual = static_cast<const __nv_bfloat16*>(residual);
+  a.ld_res = residual_stride;
+  a.y = static_cast<__nv_bfloat16*>(y);
+  a.ld_y = y_stride;
+  return cuda_status(omni::launch_decode_gemm_int4(a, stream), "decode_gemm_int4 launch");
 }
 
 }  // extern "C"

@@ -7,6 +7,7 @@
 #include "attention.cuh"
 #include "omniasr_b200.h"
 #include "paged.cuh"
+#include "paged_plan.cuh"
 
 namespace omni {
 int set_last_error(int code, const char* message);
@@ -121,6 +122,42 @@ int rope(const char* name, bool norm, const void* q_norm, const void* k_norm, fl
   return done(name, norm ? omni::launch_paged_norm_rope_kv(dtype, a, stream) : omni::launch_paged_rope_kv(dtype, a, stream));
 }
 
+// The state and requests that plan and trim share.
+int plan_args(const char* name, omni::PlanArgs& a, const int64_t* rows, const int64_t* want, int requests, int page, int64_t* length,
+              int64_t seqs, int32_t* table, int64_t table_stride, int table_width, int32_t* free, int64_t* free_count, int64_t pages,
+              void* workspace, size_t workspace_bytes, int* status) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return fail(OMNIASR_ERR_DEVICE, "no CUDA device");
+  if (!omniasr_device_supported(dev))
+    return fail(OMNIASR_ERR_DEVICE, "device %d is not compute capability 10.0 (sm_100a code)", dev);
+  if (requests < 0 || requests > omni::kPlanMaxRequests)
+    return fail(OMNIASR_ERR_ARGUMENT, "%s: %d requests (at most %d)", name, requests, omni::kPlanMaxRequests);
+  if (page <= 0 || table_width < 0 || ((int64_t)table_width + 1) * page > 0x7fffff00ll || table_stride < table_width)
+    return fail(OMNIASR_ERR_ARGUMENT, "%s: a table of %d pages of %d positions, stride %lld", name, table_width, page,
+                (long long)table_stride);
+  if (seqs < 0 || seqs > 0x7fffffffll || pages < 0 || pages > 0x7fffffffll)
+    return fail(OMNIASR_ERR_ARGUMENT, "%s: %lld sequences, %lld pages", name, (long long)seqs, (long long)pages);
+  if (!free_count || (requests && (!rows || !want || !length || (!table && table_width) || (!free && pages))))
+    return fail(OMNIASR_ERR_ARGUMENT, "%s: null pointer", name);
+  if (!workspace || !aligned16(workspace) || workspace_bytes < OMNIASR_PLAN_WORKSPACE)
+    return fail(OMNIASR_ERR_WORKSPACE, "%s: workspace of %zu bytes, %d needed", name, workspace_bytes, OMNIASR_PLAN_WORKSPACE);
+  a.s.length = length;
+  a.s.seqs = seqs;
+  a.s.table = table;
+  a.s.table_stride = table_stride;
+  a.s.table_width = table_width;
+  a.s.free = free;
+  a.s.count = free_count;
+  a.s.pages = pages;
+  a.s.page = page;
+  a.rows = rows;
+  a.want = want;
+  a.requests = requests;
+  a.arrivals = reinterpret_cast<unsigned*>(workspace);
+  a.status = status;
+  return OMNIASR_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -223,6 +260,45 @@ int omniasr_paged_attention(const void* q, const void* k_pages, const void* v_pa
     return done(name, e);
   }
   return done(name, omni::launch_paged_attention(dtype, a, stream));
+}
+
+int omniasr_paged_plan(const int64_t* rows, const int64_t* fresh, int requests, int64_t tokens, int page, int64_t* length,
+                       int64_t seqs, int32_t* table, int64_t table_stride, int table_width, int32_t* free, int64_t* free_count,
+                       int64_t pages, int64_t* pos, int64_t* slots, int32_t* batch_table, int batch_width, int64_t* lengths,
+                       int64_t* q_offsets, int64_t* k_offsets, uint8_t* taken, void* workspace, size_t workspace_bytes, int* status,
+                       cudaStream_t stream) {
+  const char* name = "paged_plan";
+  omni::PlanArgs a{};
+  if (int e = plan_args(name, a, rows, fresh, requests, page, length, seqs, table, table_stride, table_width, free, free_count, pages,
+                        workspace, workspace_bytes, status))
+    return e;
+  if (tokens < 0 || tokens > 0x3fffffffll) return fail(OMNIASR_ERR_ARGUMENT, "%s: %lld tokens", name, (long long)tokens);
+  if (batch_width < 0 || batch_width > table_width || (int64_t)requests * batch_width > 0x7fffffffll)
+    return fail(OMNIASR_ERR_ARGUMENT, "%s: %d rows of %d pages of a table of %d", name, requests, batch_width, table_width);
+  if (!q_offsets || !k_offsets || (tokens && (!pos || !slots)) || (requests && ((!batch_table && batch_width) || !lengths || !taken)))
+    return fail(OMNIASR_ERR_ARGUMENT, "%s: null pointer", name);
+  a.tokens = (int)tokens;
+  a.pos = pos;
+  a.slots = slots;
+  a.batch_table = batch_table;
+  a.batch_width = batch_width;
+  a.lengths = lengths;
+  a.q_offsets = q_offsets;
+  a.k_offsets = k_offsets;
+  a.taken = taken;
+  return done(name, omni::launch_paged_plan(a, stream));
+}
+
+int omniasr_paged_trim(const int64_t* rows, const int64_t* keep, int requests, int page, int64_t* length, int64_t seqs,
+                       int32_t* table, int64_t table_stride, int table_width, int32_t* free, int64_t* free_count, int64_t pages,
+                       void* workspace, size_t workspace_bytes, int* status, cudaStream_t stream) {
+  const char* name = "paged_trim";
+  omni::PlanArgs a{};
+  if (int e = plan_args(name, a, rows, keep, requests, page, length, seqs, table, table_stride, table_width, free, free_count, pages,
+                        workspace, workspace_bytes, status))
+    return e;
+  if (requests == 0) return done(name, cudaSuccess);
+  return done(name, omni::launch_paged_trim(a, stream));
 }
 
 size_t omniasr_packed_attention_workspace(int64_t q_tokens, int heads, int kv_heads, int dim, int dtype) {

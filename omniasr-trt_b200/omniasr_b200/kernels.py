@@ -32,6 +32,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+from dataclasses import dataclass
 
 import torch
 
@@ -491,6 +492,81 @@ def decode_gemm(x: torch.Tensor, w: torch.Tensor, mode: str = "store", residual:
     return out
 
 
+@dataclass(frozen=True)
+class Int4Weights:
+    """A weight matrix [n, k] in 4 bits as the kernels read it: what :func:`int4_weights` and :func:`int4_quantise` make."""
+
+    codes: torch.Tensor  # uint8 [ceil(n / 8), ceil(k / 128), 512]
+    scales: torch.Tensor  # bfloat16 [ceil(n / 8), ceil(k / group), 8]
+    n: int
+    k: int
+    group: int
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def values(self) -> torch.Tensor:
+        """The matrix that the codes stand for (float32 [n, k], exact)."""
+        w = self.codes.view(-1, self.codes.size(1), 8, 4, 4, 4)  # [rows / 8, blocks, row, lane, word, byte]
+        c = torch.stack([w & 15, w >> 4], -1).flatten(-2)  # 8 codes: the even columns', the odd ones'
+        c = c.view(*c.shape[:-1], 2, 4).transpose(-1, -2)  # [..., lane, word, column / 2, odd]
+        c = c.permute(0, 2, 1, 4, 3, 5, 6).reshape(8 * self.codes.size(0), -1)[: self.n, : self.k]
+        s = self.scales.transpose(1, 2).reshape(-1, self.scales.size(1))[: self.n].float()
+        return (c.float() - 8) * s.repeat_interleave(self.group, 1)[:, : self.k]
+
+
+def int4_weights(codes: torch.Tensor, scales: torch.Tensor, group: int = 128) -> Int4Weights:
+    """Lays a 4-bit weight matrix out for :func:`decode_gemm_int4`, once, when a model is loaded: ``codes`` [n, k] (uint8, 0 to
+    15), ``scales`` [n, ceil(k / group)] (bfloat16; groups of 32, 64 or 128 columns, k a multiple of 32); the weight is
+    ``scales * (codes - 8)``."""
+    if codes.dim() != 2 or codes.dtype != torch.uint8:
+        raise ValueError("int4_weights: codes must be uint8 [n, k]")
+    n, k = codes.shape
+    if group not in (32, 64, 128) or k % 32 or k == 0:
+        raise ValueError(f"int4_weights: groups of {group} columns (32, 64 or 128) of {k} (a multiple of 32)")
+    if scales.dtype != torch.bfloat16 or scales.shape != (n, -(-k // group)) or scales.device != codes.device:
+        raise ValueError(f"int4_weights: scales must be bfloat16 [n, {-(-k // group)}] on the codes' device")
+    tiles, blocks = -(-n // 8), -(-k // 128)
+    c = torch.full((tiles * 8, blocks * 128), 8, dtype=torch.uint8, device=codes.device)
+    c[:n, :k] = codes & 15
+    c = c.view(tiles, 8, blocks, 4, 4, 4, 2)  # [.., row, block, word, lane, column / 2, odd]
+    c = c.permute(0, 2, 1, 4, 3, 6, 5).reshape(tiles, blocks, 512, 2)  # [.., row, lane, word, odd, column / 2]
+    s = torch.zeros(tiles * 8, scales.size(1), dtype=torch.bfloat16, device=codes.device)
+    s[:n] = scales
+    s = s.view(tiles, 8, -1).transpose(1, 2).contiguous()
+    return Int4Weights(c[..., 0] | c[..., 1] << 4, s, n, k, group)
+
+
+def int4_quantise(w: torch.Tensor, group: int = 128) -> Int4Weights:
+    """A weight matrix [n, k] in 4 bits: per group of columns s = -m / 8 rounded to bf16, m the weight of largest magnitude, and
+    codes w / s rounded to [-8, 7], plus 8. The rows of a swiglu product are [gate; inner]."""
+    if w.dim() != 2 or not w.is_floating_point() or group not in (32, 64, 128) or w.size(1) % 32 or w.size(1) == 0:
+        raise ValueError("int4_quantise: w must be floating point [n, k], k a multiple of 32, groups of 32, 64 or 128 columns")
+    n, k = w.shape
+    groups = -(-k // group)
+    f = torch.zeros(n, groups * group, dtype=torch.float32, device=w.device)
+    f[:, :k] = w
+    f = f.view(n, groups, group)
+    lo, hi = f.amin(-1), f.amax(-1)
+    scales = (torch.where(hi > -lo, hi, lo) * -0.125).to(torch.bfloat16)
+    s = scales.float()[..., None]
+    codes = torch.where(s == 0, torch.zeros_like(f), f / s).round().clamp(-8, 7).add(8).to(torch.uint8)
+    return int4_weights(codes.view(n, -1)[:, :k], scales, group)
+
+
+def decode_gemm_int4(x: torch.Tensor, w: Int4Weights, mode: str = "store", residual: torch.Tensor | None = None,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`decode_gemm` over 4-bit weights, at most 64 token rows (bf16): ``x @ W.t()`` ("store"), ``residual + x @ W.t()``
+    ("residual"), or with W's rows [gate; inner] ``inner * silu(gate)`` ("swiglu"); products and sums in fp32, rounded once, at the
+    end (swiglu's halves are not rounded before). ``w`` must not be written by the kernel launched just before on the stream."""
+    native, _, stream, _ = _context(x.device)
+    code = GEMM_MODES.get(mode)
+    if code is None:
+        raise ValueError(f"decode_gemm_int4: mode {mode!r} (supported: {', '.join(GEMM_MODES)})")
+    return native.decode_gemm_int4(x, w.codes, w.scales, w.n, w.k, w.group, code, residual, out, stream)
+
+
 @_on_its_device
 def decode_gemm_rope(x: torch.Tensor, w: torch.Tensor, cs: torch.Tensor, pos: torch.Tensor, k_cache: torch.Tensor,
                      v_cache: torch.Tensor, heads: int, slots: torch.Tensor | None = None,
@@ -643,6 +719,37 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         ws = _attn_workspace(out, device, stream)
         out = native.paged_attention(q, k_pages, v_pages, page_table, lengths, scale, tokens, k_scale, v_scale, status, stream, ws)
     return out
+
+
+def paged_plan(rows: torch.Tensor, new: torch.Tensor, tokens: int, page: int, length: torch.Tensor, table: torch.Tensor,
+               free: torch.Tensor, free_count: torch.Tensor, width: int | None = None) -> tuple[torch.Tensor, ...]:
+    """A step's index tensors from its requests' lengths, all on the GPU: request i adds ``new[i]`` tokens to sequence ``rows[i]``
+    (int64, at most 8192 requests, a sequence once). The state, updated in place: ``length`` [S] int64, ``table`` [S, W] int32
+    (the sequences' page numbers), ``free`` [pages] int32 with ``free_count`` [1] int64, a stack whose first ``free_count``
+    entries are the free pages. Returns ``(pos, slots, batch_table, lengths, q_offsets, k_offsets, taken)``: ``pos`` and ``slots``
+    [tokens] as :func:`paged_rope_kv` takes them (``tokens`` is a number that the host knows, at least the sum of ``new``; behind
+    the last token 0 and -1), ``batch_table`` [B, width] and ``lengths`` [B] as :func:`paged_attention`, the offsets [B + 1] as
+    :func:`packed_attention`. Requests are taken in order: ``taken`` [B] (bool) is False where the pages did not suffice (or
+    ``width`` pages would not, default W): that request's slots are -1, its sequence unchanged and the results of its queries mean
+    nothing. Sequences out of range or named twice, negative numbers and tokens past ``tokens`` are refused the same way and
+    raise status bit 1."""
+    native, status, stream, ws = _context(length.device)
+    out = native.paged_plan(rows, new, tokens, page, length, table, free, free_count, width, status, stream, ws)
+    if out.__class__ is int:
+        ws = _attn_workspace(out, length.device, stream)
+        out = native.paged_plan(rows, new, tokens, page, length, table, free, free_count, width, status, stream, ws)
+    return out
+
+
+def paged_trim(rows: torch.Tensor, keep: torch.Tensor, page: int, length: torch.Tensor, table: torch.Tensor, free: torch.Tensor,
+               free_count: torch.Tensor) -> None:
+    """Sequence ``rows[i]`` keeps its first ``keep[i]`` positions (int64; drafts that were not accepted go, 0 frees it), the pages
+    past them return to the stack. State as :func:`paged_plan`; a trim to the lengths before a plan of the same rows undoes it.
+    A request that names no sequence, one named before, or more positions than it has changes nothing and raises status bit 1."""
+    native, status, stream, ws = _context(length.device)
+    out = native.paged_trim(rows, keep, page, length, table, free, free_count, status, stream, ws)
+    if out is not None:
+        native.paged_trim(rows, keep, page, length, table, free, free_count, status, stream, _attn_workspace(out, length.device, stream))
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor,
