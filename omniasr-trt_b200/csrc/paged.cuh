@@ -77,6 +77,11 @@ bool paged_tc_supported(int dtype, int type, int dim, int page);
 size_t paged_tc_workspace(int dim);
 cudaError_t launch_paged_attention_tc(const PagedAttnArgs& a, cudaStream_t stream);
 
+// The pass over 4-bit pages (paged_attention_int4.cu): bf16 queries, head_dim from 64, every page size.
+bool paged_int4_supported(int dtype, int type, int dim);
+size_t paged_int4_workspace(int dim);
+cudaError_t launch_paged_attention_int4(const PagedAttnArgs& a, cudaStream_t stream);
+
 struct PackedArgs {
   const void* q;
   int64_t q_st, q_sh;  // q[token, head, :] strides (elements)

@@ -215,6 +215,7 @@ size_t omniasr_paged_attention_workspace(int dtype, int cache_type, int rows, in
       table_width < 0)
     return 0;
   if (omni::paged_tc_supported(dtype, cache_type, dim, page)) return omni::paged_tc_workspace(dim);
+  if (omni::paged_int4_supported(dtype, cache_type, dim)) return omni::paged_int4_workspace(dim);
   return omni::paged_attention_workspace(dtype, cache_type, rows ? rows : 1, tokens, heads, kv_heads, dim, page, table_width);
 }
 
@@ -259,6 +260,7 @@ int omniasr_paged_attention(const void* q, const void* k_pages, const void* v_pa
                   (long long)stride_page, (long long)stride_head, (long long)stride_pos);
     return done(name, e);
   }
+  if (omni::paged_int4_supported(dtype, cache_type, dim)) return done(name, omni::launch_paged_attention_int4(a, stream));
   return done(name, omni::launch_paged_attention(dtype, a, stream));
 }
 
