@@ -5,19 +5,22 @@
 // to it the instructions that make operands of the codes: 2 D codes a key, about 0.17 keys a clock and SM at HBM's rate, with 64
 // integer lanes a clock. Hence:
 //
-// * The codes never become a tile in shared memory (for tcgen05 they would be written and read there in four times their bytes,
-//   more than its 128 bytes a clock): each lane dequantises in registers what it feeds to mma.m16n8k16 itself, whose rate
-//   (one per two clocks and SM) is more than twice what is needed. The cache's order of codes (int4.cuh) makes a lane's share of a
-//   vector one run of 16 bytes (K) or 8 (V).
-// * S^T = K Q^T, 16 keys x 8 columns. A code masked out of its word is, read as fp16, the subnormal c 2^-24 (16 c 2^-24 four bits
-//   up), exact, so a word of 8 codes takes four ands and a shift; the queries (fp16, scaled by a power of two per column so that the
-//   largest is 2^14 and more: exact but for values 2^-28 of it) carry the factors. The sums start from -8 sum q, which is the
+// * The codes never become a tile in shared memory (for tcgen05 they would be written and read there in two or four times their
+//   bytes, with 128 bytes a clock): each lane dequantises in registers what it feeds to mma.sync itself, whose rate (a
+//   product of 16 x 8 x 16 in two clocks) is more than twice what is needed. The cache's order of codes
+//   (int4.cuh) makes a lane's share of a vector one run of 16 bytes (K) or 8 (V).
+// * S^T = K Q^T in fp16, 16 keys x 8 columns a step: a code masked out of its word is, read as fp16, the subnormal c 2^-24 (16 c 2^-24
+//   four bits up), exact, so a word of 8 codes takes four ands and a shift. The queries, scaled by a power of two per column
+//   (largest value 2^14 and more; exact but for values 2^-28 of it), carry the factors. The sums start from -8 sum q, which is the
 //   codes' offset, and every group's sum is scaled in fp32.
-// * O^T = V^T P^T: two keys' codes of a dim are the halves of a word after one byte permutation; 128 + c - 8 is exact in
-//   bf16. The scales go onto the probabilities: P^T is turned by movmatrix and multiplied per group, so that no value needs one.
+// * O^T = V^T P^T in fp16: two keys' codes of a dim are the halves of a word after one byte permutation, and a code masked out of it
+//   is the subnormal c 2^-24 (16 c 2^-24 four bits up), exact; the offset is a second product, with constants. The scales go onto
+//   the probabilities in fp32, before these are rounded, once, to fp16 (2^-12) and turned by movmatrix. What keeps them in
+//   fp16's range is the number that is taken off the scores: a column's weights 2^(x - m) may grow until weight x scale is 2^12,
+//   then m is raised so that the largest is about 2^4. Sums of weights and accumulators share m, so nothing else sees it.
 // * Warps are independent: each takes blocks of 16 or 32 keys of the CTA's share with a maximum, a sum and an accumulator of
-//   its own, and copies its next blocks asynchronously into a ring of its own; no barrier in the loop. A column's maximum is raised
-//   only when a score passes it by 2^8. At a unit's end the CTA's warps join through shared memory.
+//   its own, and copies its next blocks asynchronously into a ring of its own; no barrier in the loop. At a unit's end the CTA's
+//   warps join through shared memory.
 // * All blocks of all units are cut evenly between the CTAs. A unit that is cut leaves parts in the workspace; the CTA that
 //   publishes last joins them in the order of the keys, so a call repeats its bits.
 //
@@ -25,6 +28,8 @@
 // NaN) are masked out of the products; keys past the row's last are not read.
 
 #include <math.h>
+
+#include <cuda_fp16.h>
 
 #include <algorithm>
 
@@ -38,7 +43,11 @@ namespace paged4 {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr float kLazy = 8.f;  // log2 of how far a score may pass its column's maximum
+constexpr float kMost = 12.f, kGoal = 4.f;  // log2 of a weight times a scale: the most, and the largest when m is raised
+constexpr float kLeast = -60.f;             // the smallest exponent of a scale that is looked at (weights stay inside fp32)
+constexpr float kNone = -3e38f;  // a maximum before any score: below what a score can be, and a number, so that nothing needs a case for it
+// A unit's start and end (queries, the join of the warps), about 3 us of a CTA, counted as so many blocks in the shares.
+constexpr int kStart = 8;
 
 template <int DIM, int NT>  // NT: tiles of 8 columns
 struct Cfg {
@@ -60,13 +69,15 @@ struct Cfg {
   static constexpr int kLim = kMl + kWarps * kCols * 8;
   static constexpr int kJoin = (kLim + kCols * 8 + 15) / 16 * 16;
   static constexpr int kBytes = kJoin + kWarps * 8 * kPitch * 4;
-  static constexpr int kCtas = DIM == 512 || NT * DIM >= 384 || NT * DIM == 256 && DIM == 64 ? 2 : NT * DIM > 128 ? 3 : 4;  // per SM, for the registers
+  static constexpr int kCtas = DIM == 512 || NT * DIM >= 384 || NT * DIM == 256 && DIM == 64 ? 2 : NT * DIM > 64 ? 3 : 4;  // per SM, for the registers
 };
 
 struct Params {
   PagedAttnArgs a;
   int cols, chunks;  // columns of a (row, kv head); units per (row, kv head)
   int grid;
+  int page_shift;        // pages of 2^page_shift positions, 16 and more, one behind another in a head's part; else -1
+  uint32_t page_scales;  // bytes of a page's scales
   unsigned* counters;  // [grid], zero on entry and left zero
   float* part_o;       // [2 grid][cols of a unit][dim]
   float2* part_ml;     // [2 grid][cols of a unit]
@@ -97,13 +108,15 @@ OMNI_DEV void load_words(uint32_t* w, uint32_t addr) {
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(addr));
 }
 
-OMNI_DEV void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, const uint32_t* b) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]));
+// d = a b + c.
+OMNI_DEV void mma_f16(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, const uint32_t* b, float c0, float c1, float c2, float c3) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
-OMNI_DEV void mma_bf16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+// c += a b.
+OMNI_DEV void mma_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -112,18 +125,19 @@ OMNI_DEV uint32_t turned(uint32_t x) {  // an 8 x 8 tile of 16-bit values across
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-OMNI_DEV uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+OMNI_DEV uint32_t max_abs_bf16x2(uint32_t a, uint32_t b) {  // (of a NaN and a number the number)
   uint32_t r;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a & 0x7fff7fffu), "r"(b & 0x7fff7fffu));
   return r;
 }
-// Nibble n of each half of z as bf16 c - 8.
-OMNI_DEV uint32_t centred(uint32_t z, int n) {
-  const uint32_t v = ((z >> (4 * n)) & 0x000f000fu) | 0x43004300u;  // 128 + c
+// Two fp32 as fp16 (lo, hi).
+OMNI_DEV uint32_t half2_of(float lo, float hi) {
   uint32_t r;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(0x43084308u));
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+// A bf16 magnitude's exponent, of infinities and NaN that of 0.
+OMNI_DEV float exponent_of(uint32_t bits) { return bits < 0x7f80u ? fmaxf((float)((int)(bits >> 7) - 127), kLeast) : kLeast; }
 
 // Where the 16-byte word c of key r's codes lies in a tile: so that a quarter warp's reads (K: 16 bytes of 2 keys x 4 lanes; V, 8
 // bytes: 4 keys x 4 lanes) meet all banks. Keys of V lie in the order of its operand, so that a lane's four are 4 apart.
@@ -131,16 +145,17 @@ template <int DIM>
 OMNI_DEV int k_place(int r, int c) {
   return r * (DIM / 32) + (DIM >= 256 ? c ^ ((r & 1) << 2) : c);
 }
-OMNI_DEV int v_slot(int r) { return (r & 24) | ((r & 1) << 2) | ((r >> 1) & 3); }
+OMNI_DEV int v_slot(int r) { return (r & 8) | ((r & 1) << 2) | ((r >> 1) & 3); }
 template <int DIM>
 OMNI_DEV int v_place(int slot, int c) {
   return slot * (DIM / 32) + (DIM >= 256 ? c ^ ((slot & 3) << 1) : DIM == 128 ? c ^ (slot & 2) : c);
 }
 
-// A walk over the units in order: unit (row, hc) has the blocks [u0, u0 + nb).
+// A walk over the units in order. The shares are cut along a line on which a unit takes kStart places and then one per block: the
+// blocks of unit (row, head, chunk of columns) are the places [u0, u0 + nb).
 struct Walk {
   int64_t u0;
-  int row, hc, nb;
+  int row, head, chunk, nb;
   int len, need;  // keys the row's first query sees (at least 0), and its last
 };
 
@@ -149,23 +164,31 @@ struct Rows {
   const Params& p;
   int64_t cap;
   OMNI_DEV explicit Rows(const Params& q) : p(q), cap((int64_t)q.a.table_width * q.a.c.page) {}
-  OMNI_DEV void look(int row, Walk& w) const {
-    const int64_t len = min(p.a.lengths[row], cap);
+  OMNI_DEV int64_t look(int row, Walk& w) const {
+    const int64_t given = p.a.lengths[row], len = min(given, cap);
     w.need = (int)max((int64_t)0, min(cap, len + p.a.tokens - 1));
     w.len = (int)max(len, (int64_t)-p.a.tokens);
     w.nb = (w.need + KEYS - 1) / KEYS;
+    return given;
   }
+  OMNI_DEV static int places(int nb) { return nb ? nb + kStart : 0; }
   OMNI_DEV void next(Walk& w) const {
-    w.u0 += w.nb;
-    if (++w.hc == p.a.c.kv_heads * p.chunks) {
-      w.hc = 0;
-      while (++w.row < p.a.rows) {
-        look(w.row, w);
-        if (w.nb) break;
-      }
+    w.u0 += w.nb + kStart;
+    if (++w.chunk < p.chunks) return;
+    w.chunk = 0;
+    if (++w.head < p.a.c.kv_heads) return;
+    w.head = 0;
+    while (++w.row < p.a.rows) {
+      look(w.row, w);
+      if (w.nb) break;
     }
   }
 };
+
+// a / b of numbers that are mostly small (a >= 0, b > 0).
+OMNI_DEV int64_t quotient(int64_t a, int64_t b) {
+  return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
 
 OMNI_DEV int64_t block_sum(int64_t v, int64_t* s) {
 #pragma unroll
@@ -189,9 +212,12 @@ struct Kernel {
   uint32_t ring;  // this warp's
   int lane, warp, g, t;
   uint32_t q_at, init_at;
+  int k_lane, v_lane;  // this lane's words in a tile: of key g in K, of slot t in V (block b's: ^ 64 b)
 
   float o[C::kBlocks * C::kGroups][2][NT][4];
-  float m[NT][2], l[NT][2], qs[NT][2];
+  float m[NT][2], l[NT][2], qs[NT][2];  // what is taken off the scores, sums of weights, the scores' factors
+  float es[NT][2];                      // the largest exponent of a scale of V that the column has seen
+  uint32_t run;                         // the largest scale of V (bf16 bits) of blocks that all columns see
 
   OMNI_DEV Kernel(const Params& q, char* s) : p(q), smem(s) {
     lane = threadIdx.x & 31;
@@ -199,52 +225,117 @@ struct Kernel {
     g = lane >> 2;
     t = lane & 3;
     ring = smem_addr(smem) + C::kRing + warp * C::kStages * C::kStage;
-    q_at = smem_addr(smem) + C::kQ + lane * 8;
+    q_at = smem_addr(smem) + C::kQ + lane * 16;
     init_at = smem_addr(smem) + C::kInit + t * 8;
+    k_lane = DIM == 64 ? g * C::kRow + t * 8 : k_place<DIM>(g, t) * 16;
+    v_lane = DIM == 64 ? t * C::kRow + g * 4 : v_place<DIM>(t, g >> 1) * 16 + (g & 1) * 8;
   }
 
   // ---- loads: block n (of the walk's unit) into a stage of the ring
 
-  OMNI_DEV void fetch(const Walk& w, int64_t n, int stage) {
+  // Pages of whole tiles of 16 keys whose positions lie one behind another (p.page_shift >= 0): a tile is one run of bytes of K,
+  // V and their scales each. What a lane needs of a unit to copy its part of any tile, and the pages of the next block:
+  struct Source {
+    const char *k, *v, *scale;  // where the head's part of page 0 starts, this lane's bytes of it (scales: V's in the upper half warp)
+    const int32_t* table;
+    int id[C::kMt];
+  };
+  static constexpr int kCopy = C::kScale < 16 ? C::kScale : 16;  // bytes of scales per copy
+
+  OMNI_DEV void look_up(Source& f, const Walk& w, int block) const {  // (past the row's end: its last page)
+    const int last = (w.need - 1) >> p.page_shift;
+#pragma unroll
+    for (int tile = 0; tile < C::kMt; ++tile) f.id[tile] = __ldg(f.table + min((block * C::kKeys + tile * 16) >> p.page_shift, last));
+  }
+  OMNI_DEV void open(Source& f, const Walk& w, int block) const {
+    if (p.page_shift < 0) return;
     const PagedAttnArgs& a = p.a;
-    const int j0 = (int)(n - w.u0) * C::kKeys;
-    const int h = w.hc / p.chunks;
-    const uint32_t kd = ring + stage * C::kStage, vd = kd + C::kKeys * C::kRow, ksd = vd + C::kKeys * C::kRow,
-                   vsd = ksd + C::kKeys * C::kScale;
-    // The page of each key: lane r's.
-    const int jr = j0 + (lane < C::kKeys ? lane : 0);
-    int id = -1, off = 0;
-    if (jr < w.need) {
-      const int pi = jr / a.c.page;
-      off = jr - pi * a.c.page;
-      id = a.table[w.row * a.table_stride + pi];
-      if (id < 0 || id >= a.c.pages) {
-        if (lane < C::kKeys) raise_status(a.status, kStatusIndex);
-        id = -1;
+    f.k = reinterpret_cast<const char*>(a.c.k) + w.head * a.c.s_head + lane * 16;
+    f.v = reinterpret_cast<const char*>(a.c.v) + w.head * a.c.s_head + lane * 16;
+    const bool upper = C::kScale <= 16 && lane >= 16;
+    f.scale = reinterpret_cast<const char*>(upper ? a.c.v_scale : a.c.k_scale) + ((int64_t)w.head << p.page_shift) * C::kScale +
+              (C::kScale <= 16 ? lane & 15 : lane) * kCopy;
+    f.table = a.table + w.row * a.table_stride;
+    look_up(f, w, block);
+  }
+
+  // A block of whole tiles; false (and nothing done) where a tile is not whole or its page number is none.
+  OMNI_DEV bool fetch_whole(Source& f, const Walk& w, int block, int stage) const {
+    bool ok = (block + 1) * C::kKeys <= w.need;
+#pragma unroll
+    for (int tile = 0; tile < C::kMt; ++tile) ok = ok && (unsigned)f.id[tile] < (unsigned)p.a.c.pages;
+    if (!ok) return false;
+    const uint32_t kd = ring + stage * C::kStage, vd = kd + C::kKeys * C::kRow, ksd = vd + C::kKeys * C::kRow;
+    const PagedAttnArgs& a = p.a;
+    constexpr int N = 16 * C::kRow / 512;  // copies of 16 bytes per lane and tile
+    constexpr int CPR = C::kRow / 16;
+#pragma unroll
+    for (int tile = 0; tile < C::kMt; ++tile) {
+      const uint32_t off = (block * C::kKeys + tile * 16) & ((1 << p.page_shift) - 1);
+      const uint64_t at = (uint64_t)(uint32_t)f.id[tile] * (uint32_t)a.c.s_page + off * C::kRow;
+      const char *k = f.k + at, *v = f.v + at;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int r = (lane + 32 * i) / CPR, c = lane % CPR;
+        copy_async(kd + (tile * 16 * CPR + k_place<DIM>(r, c)) * 16, k + i * 512, true, 16);
+        copy_async(vd + (tile * 16 * CPR + v_place<DIM>(v_slot(r), c)) * 16, v + i * 512, true, 16);
+      }
+      const char* scale = f.scale + ((uint64_t)(uint32_t)f.id[tile] * p.page_scales + off * C::kScale);
+      if constexpr (C::kScale <= 16) {
+        copy_async(ksd + (lane >= 16 ? C::kKeys * C::kScale : 0) + (tile * 16 + (lane & 15)) * C::kScale, scale, true, kCopy);
+      } else {
+        const int64_t apart = reinterpret_cast<const char*>(a.c.v_scale) - reinterpret_cast<const char*>(a.c.k_scale);
+        copy_async(ksd + tile * 16 * C::kScale + lane * 16, scale, true, 16);
+        copy_async(ksd + (C::kKeys + tile * 16) * C::kScale + lane * 16, scale + apart, true, 16);
       }
     }
-    constexpr int CPR = C::kRow / 16;              // 16-byte words per key
-    constexpr int N = C::kKeys * CPR / 32;         // per lane
+    return true;
+  }
+
+  // Any page size: each key's page number by a lane of its own.
+  OMNI_DEV void fetch_keys(const Walk& w, int j0, int stage) {
+    const PagedAttnArgs& a = p.a;
+    const int h = w.head;
+    const uint32_t kd = ring + stage * C::kStage, vd = kd + C::kKeys * C::kRow, ksd = vd + C::kKeys * C::kRow,
+                   vsd = ksd + C::kKeys * C::kScale;
+    const int jr = j0 + (lane < C::kKeys ? lane : 0);
+    bool live = false;
+    int64_t at = 0, sat = 0;
+    if (jr < w.need) {
+      const int pi = (int)((uint32_t)jr / (uint32_t)a.c.page), off = jr - pi * a.c.page;
+      const int id = a.table[w.row * a.table_stride + pi];
+      live = (unsigned)id < (unsigned)a.c.pages;
+      if (live) {
+        at = (int64_t)id * a.c.s_page + h * a.c.s_head + off * a.c.s_pos;
+        sat = (((int64_t)id * a.c.kv_heads + h) * a.c.page + off) * C::kScale;
+      } else if (lane < C::kKeys) {
+        raise_status(a.status, kStatusIndex);
+      }
+    }
+    constexpr int CPR = C::kRow / 16, N = C::kKeys * CPR / 32;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int r = (lane + 32 * i) / CPR, c = lane % CPR;
-      const int rid = __shfl_sync(0xffffffffu, id, r), roff = __shfl_sync(0xffffffffu, off, r);
-      const bool on = rid >= 0;
-      const int64_t at = on ? rid * a.c.s_page + h * a.c.s_head + roff * a.c.s_pos + c * 16 : 0;
-      const int tile = r >> 4, rr = r & 15;
-      copy_async(kd + (tile * 16 * CPR + k_place<DIM>(rr, c)) * 16, reinterpret_cast<const char*>(a.c.k) + at, on, 16);
-      copy_async(vd + (tile * 16 * CPR + v_place<DIM>(v_slot(rr), c)) * 16, reinterpret_cast<const char*>(a.c.v) + at, on, 16);
+      const int r = (lane + 32 * i) / CPR, c = lane % CPR, rr = r & 15;
+      const bool on = __shfl_sync(0xffffffffu, live, r);
+      const int64_t in = __shfl_sync(0xffffffffu, at, r) + (on ? c * 16 : 0);
+      copy_async(kd + ((r & ~15) * CPR + k_place<DIM>(rr, c)) * 16, reinterpret_cast<const char*>(a.c.k) + in, on, 16);
+      copy_async(vd + ((r & ~15) * CPR + v_place<DIM>(v_slot(rr), c)) * 16, reinterpret_cast<const char*>(a.c.v) + in, on, 16);
     }
-    constexpr int CS = C::kScale < 16 ? C::kScale : 16, SPR = C::kScale / CS;  // bytes of a copy, copies per key
+    constexpr int CS = C::kScale < 16 ? C::kScale : 16, SPR = C::kScale / CS;
     static_assert(C::kKeys * SPR <= 32, "a copy per lane");
     const int r = lane / SPR % C::kKeys, c = lane % SPR;
-    const int rid = __shfl_sync(0xffffffffu, id, r), roff = __shfl_sync(0xffffffffu, off, r);
-    if (C::kKeys * SPR == 32 || lane < C::kKeys * SPR) {
-      const bool on = rid >= 0;
-      const int64_t at = on ? (((int64_t)rid * a.c.kv_heads + h) * a.c.page + roff) * C::kScale + c * CS : 0;
-      copy_async(ksd + r * C::kScale + c * CS, reinterpret_cast<const char*>(a.c.k_scale) + at, on, CS);
-      copy_async(vsd + v_slot(r) * C::kScale + c * CS, reinterpret_cast<const char*>(a.c.v_scale) + at, on, CS);
+    const bool on = __shfl_sync(0xffffffffu, live, r);
+    const int64_t in = __shfl_sync(0xffffffffu, sat, r) + (on ? c * CS : 0);
+    if (lane < C::kKeys * SPR) {
+      copy_async(ksd + r * C::kScale + c * CS, reinterpret_cast<const char*>(a.c.k_scale) + in, on, CS);
+      copy_async(vsd + r * C::kScale + c * CS, reinterpret_cast<const char*>(a.c.v_scale) + in, on, CS);
     }
+  }
+
+  // Block `block` of the unit into a stage; `then`: the one that comes next, if it is the unit's.
+  OMNI_DEV void fetch(Source& f, const Walk& w, int block, int then, int stage) {
+    if (p.page_shift < 0 || !fetch_whole(f, w, block, stage)) fetch_keys(w, block * C::kKeys, stage);
+    if (p.page_shift >= 0) look_up(f, w, then);
   }
 
   // ---- a unit's queries
@@ -255,73 +346,81 @@ struct Kernel {
   }
   OMNI_DEV int64_t query_row(const Walk& w, int col) const {
     const int gr = p.a.heads / p.a.c.kv_heads, tok = col / gr;
-    return ((int64_t)w.row * p.a.tokens + tok) * p.a.heads + w.hc / p.chunks * gr + (col - tok * gr);
+    return ((int64_t)w.row * p.a.tokens + tok) * p.a.heads + w.head * gr + (col - tok * gr);
   }
 
-  // Warp by warp a column: fp16 operands in the order of the codes, the sums' start per group, the factor of its scores.
-  OMNI_DEV void load_queries(const Walk& w) {
-    const int c0 = w.hc % p.chunks * C::kCols;
+  // A warp's columns of a unit: their words in flight ...
+  static constexpr int kPer = C::kCols / kWarps, kWords = DIM > 256 ? 2 : 1;  // columns per warp, words of 8 dims per lane
+  OMNI_DEV void read_queries(const Walk& w, uint4 (&u)[kPer][kWords]) const {
+    const int c0 = w.chunk * C::kCols;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int col = c0 + warp + k * kWarps;
+      const bool on = col < p.cols;
+      const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.a.q) + (on ? query_row(w, col) * DIM : 0));
+#pragma unroll
+      for (int v = 0; v < kWords; ++v) {
+        const int word = v * 32 + lane;
+        u[k][v] = on && word * 8 < DIM ? __ldg(src + word) : make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+  }
+
+  // ... and as fp16 operands in the order of the codes, with the sums' start per group and the factor of the scores. (A column with
+  // an infinity or a NaN comes out NaN through its sums' start.)
+  OMNI_DEV void store_queries(const Walk& w, const uint4 (&u)[kPer][kWords]) {
+    const int c0 = w.chunk * C::kCols;
     float* init = reinterpret_cast<float*>(smem + C::kInit);
     float* factor = reinterpret_cast<float*>(smem + C::kLim);
     int* lims = reinterpret_cast<int*>(smem + C::kLim) + C::kCols;
-    constexpr int V = DIM > 256 ? 2 : 1;  // words of 8 dims per lane
-    for (int col = warp; col < C::kCols; col += kWarps) {
-      const int lim = limit(w, c0 + col);
-      float x[V][8];
-      uint32_t top = 0u;
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const int word = v * 32 + lane;
-        uint4 u = make_uint4(0u, 0u, 0u, 0u);
-        if (lim >= 0 && word * 8 < DIM)
-          u = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.a.q) + query_row(w, c0 + col) * DIM) + word);
-        Elem<__nv_bfloat16>::unpack(u, x[v]);
+    for (int k = 0; k < kPer; ++k) {
+      const int col = warp + k * kWarps;
+      uint32_t top2 = 0u;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t b = __float_as_uint(x[v][i]) & 0x7fffffffu;
-          top = max(top, b < 0x7f800000u ? b : 0u);
-        }
-      }
-      top = __reduce_max_sync(0xffffffffu, top);
-      const int e = top == 0u ? 0 : max(-112, (int)(top >> 23) - 127);
+      for (int v = 0; v < kWords; ++v)
+        top2 = max_abs_bf16x2(top2, max_abs_bf16x2(max_abs_bf16x2(u[k][v].x, u[k][v].y), max_abs_bf16x2(u[k][v].z, u[k][v].w)));
+      const uint32_t top = __reduce_max_sync(0xffffffffu, max(top2 & 0xffffu, top2 >> 16));
+      const int e = top == 0u ? 0 : max(-112, (int)(top >> 7) - 127);
       const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
+      for (int v = 0; v < kWords; ++v) {
         const int word = v * 32 + lane;
-        uint32_t b[4];
+        float x[8];
+        Elem<__nv_bfloat16>::unpack(u[k][v], x);
         float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {  // nibbles i and i + 4 of the word; odd ones stand for 16 c
-          const float f = (i & 1) ? up * 0.0625f : up;
-          const __half2 h = __floats2half2_rn(x[v][i] * f, x[v][i + 4] * f);
-          b[i] = *reinterpret_cast<const uint32_t*>(&h);
-          const float2 back = __half22float2(h);
-          sum += (back.x + back.y) * ((i & 1) ? 16.f : 1.f);
+        for (int i = 0; i < 8; ++i) {
+          x[i] *= up;
+          sum += x[i];
         }
+        uint32_t b[4];  // nibbles i and i + 4 of the word; odd ones stand for 16 c
+#pragma unroll
+        for (int i = 0; i < 4; ++i) b[i] = (i & 1) ? half2_of(x[i] * 0.0625f, x[i + 4] * 0.0625f) : half2_of(x[i], x[i + 4]);
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
         if (word * 8 < DIM) {
           const int group = word >> 2;
-          uint2* dst = reinterpret_cast<uint2*>(smem + C::kQ) + ((group * 2) * NT + (col >> 3)) * 32 + (col & 7) * 4 + (word & 3);
-          dst[0] = make_uint2(b[0], b[1]);
-          dst[NT * 32] = make_uint2(b[2], b[3]);
+          reinterpret_cast<uint4*>(smem + C::kQ)[(group * NT + (col >> 3)) * 32 + (col & 7) * 4 + (word & 3)] = make_uint4(b[0], b[1], b[2], b[3]);
           if ((word & 3) == 0) init[group * C::kCols + col] = sum * (-8.f * 0x1p-24f);
         }
       }
       if (lane == 0) {
         factor[col] = p.a.scale * kLog2e * 0x1p10f * __uint_as_float((uint32_t)(e + 127) << 23);
-        lims[col] = lim;
+        lims[col] = limit(w, c0 + col);
       }
     }
   }
 
   OMNI_DEV void start_unit() {
+    run = 0u;
     const float* factor = reinterpret_cast<const float*>(smem + C::kLim);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        m[n][i] = -INFINITY;
+        m[n][i] = kNone;
+        es[n][i] = kLeast;
         l[n][i] = 0.f;
         qs[n][i] = factor[n * 8 + 2 * t + i];
       }
@@ -356,17 +455,16 @@ struct Kernel {
       for (int k = 0; k < C::kMt; ++k)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int r = g + 8 * e;
           if constexpr (C::kGroups == 4)
-            load_words<4>(kw[k][e], kd + k * 16 * C::kRow + k_place<DIM>(r, b * 4 + t) * 16);
+            load_words<4>(kw[k][e], kd + k * 16 * C::kRow + 8 * e * C::kRow + (k_lane ^ (b * 64)));
           else
-            load_words<2>(kw[k][e], kd + k * 16 * C::kRow + r * C::kRow + t * 8);
-          load_words<W2>(ks[k][e], ksd + (k * 16 + r) * C::kScale + b * 8);
+            load_words<2>(kw[k][e], kd + k * 16 * C::kRow + 8 * e * C::kRow + k_lane);
+          load_words<W2>(ks[k][e], ksd + g * C::kScale + (k * 16 + 8 * e) * C::kScale + b * 8);
         }
 #pragma unroll
       for (int gr = 0; gr < C::kGroups; ++gr) {
         const int group = b * C::kGroups + gr;
-        uint32_t lo[C::kMt][4], hi[C::kMt][4];  // the operands of keys g and g + 8: nibbles (0, 4), (1, 5), (2, 6), (3, 7)
+        uint32_t lo[C::kMt][4], hi[C::kMt][4];  // of keys g and g + 8 the nibbles (0, 4), (1, 5), (2, 6), (3, 7)
 #pragma unroll
         for (int k = 0; k < C::kMt; ++k) {
           const uint32_t x = kw[k][0][gr], y = kw[k][1][gr];
@@ -375,15 +473,15 @@ struct Kernel {
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          uint32_t q0[2], q1[2], start[2];
-          load_words<2>(q0, q_at + ((group * 2) * NT + n) * 256);
-          load_words<2>(q1, q_at + ((group * 2 + 1) * NT + n) * 256);
+          uint32_t q[4], start[2];
+          load_words<4>(q, q_at + (group * NT + n) * 512);
           load_words<2>(start, init_at + (group * C::kCols + n * 8) * 4);
+          const float i0 = __uint_as_float(start[0]), i1 = __uint_as_float(start[1]);
 #pragma unroll
           for (int k = 0; k < C::kMt; ++k) {
-            float c[4] = {__uint_as_float(start[0]), __uint_as_float(start[1]), __uint_as_float(start[0]), __uint_as_float(start[1])};
-            mma_f16(c, lo[k][0], hi[k][0], lo[k][1], hi[k][1], q0);
-            mma_f16(c, lo[k][2], hi[k][2], lo[k][3], hi[k][3], q1);
+            float h[4], c[4];
+            mma_f16(h, lo[k][0], hi[k][0], lo[k][1], hi[k][1], q, i0, i1, i0, i1);
+            mma_f16(c, lo[k][2], hi[k][2], lo[k][3], hi[k][3], q + 2, h[0], h[1], h[2], h[3]);
             const uint32_t w0 = ks[k][0][gr >> 1], w1 = ks[k][1][gr >> 1];
             const float s0 = __uint_as_float((gr & 1) ? w0 & 0xffff0000u : w0 << 16), s1 = __uint_as_float((gr & 1) ? w1 & 0xffff0000u : w1 << 16);
             s[k][n][0] = fmaf(s0, c[0], s[k][n][0]);
@@ -394,31 +492,84 @@ struct Kernel {
         }
       }
     }
-    // Scores, masks, the maxima.
+    auto masked = [&](int k, int n, int i) {
+      return TAIL && j0 + k * 16 + g + (i & 2) * 4 >= lims[n * 8 + 2 * t + (i & 1)];
+    };
+    // How large V's scales are: of a block that every column sees one number for all of them, else of each column's own keys.
+    if constexpr (!TAIL) {
+      constexpr int SW = C::kKeys * C::kScale / 128;  // words of scales per lane
+      uint32_t w[SW], top = 0u;
+      load_words<SW>(w, vsd + lane * SW * 4);
+#pragma unroll
+      for (int i = 0; i < SW; ++i) top = max_abs_bf16x2(top, w[i]);
+      top = max(top & 0xffffu, top >> 16);
+      if (__any_sync(0xffffffffu, top > run)) {
+        run = __reduce_max_sync(0xffffffffu, top < 0x7f80u ? top : 0u);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) es[n][i] = fmaxf(es[n][i], exponent_of(run));
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < C::kMt; ++k)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          uint32_t top = 0u;
+#pragma unroll
+          for (int b = 0; b < C::kBlocks; ++b) {
+            uint32_t w[W2];
+            load_words<W2>(w, vsd + (k * 16 + 8 * e + g) * C::kScale + b * 8);
+#pragma unroll
+            for (int i = 0; i < W2; ++i) top = max_abs_bf16x2(top, w[i]);
+          }
+          const float x = fmaxf(exponent_of(top & 0xffffu), exponent_of(top >> 16));
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              if (!masked(k, n, 2 * e + i)) es[n][i] = fmaxf(es[n][i], x);
+        }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int w = 4; w < 32; w <<= 1) es[n][i] = fmaxf(es[n][i], __shfl_xor_sync(0xffffffffu, es[n][i], w));
+    }
+    // Scores less m, masked.
     bool raise = false;
+    float d[C::kMt][NT][4];
 #pragma unroll
     for (int k = 0; k < C::kMt; ++k)
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float& x = s[k][n][i];
-          x *= qs[n][i & 1];
-          if (TAIL && j0 + k * 16 + g + (i & 2) * 4 >= lims[n * 8 + 2 * t + (i & 1)]) x = -INFINITY;
-          raise |= x > m[n][i & 1] + kLazy;
+          d[k][n][i] = masked(k, n, i) ? -INFINITY : fmaf(s[k][n][i], qs[n][i & 1], -m[n][i & 1]);
+          raise |= d[k][n][i] > kMost - es[n][i & 1];
         }
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float top = m[n][i];
+          float top = -INFINITY;
 #pragma unroll
-          for (int k = 0; k < C::kMt; ++k) top = fmaxf(top, fmaxf(s[k][n][i], s[k][n][i + 2]));
+          for (int k = 0; k < C::kMt; ++k)
+#pragma unroll
+            for (int e = i; e < 4; e += 2)
+              if (!masked(k, n, e)) top = fmaxf(top, s[k][n][e] * qs[n][i]);
 #pragma unroll
           for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-          const float f = m[n][i] == top ? 1.f : ex2(m[n][i] - top);
+          top = fmaxf(m[n][i], top + es[n][i] - kGoal);
+          const float f = ex2(m[n][i] - top);
           m[n][i] = top;
+#pragma unroll
+          for (int k = 0; k < C::kMt; ++k)
+#pragma unroll
+            for (int e = i; e < 4; e += 2)
+              if (!masked(k, n, e)) d[k][n][e] = fmaf(s[k][n][e], qs[n][i], -top);
           l[n][i] *= f;
 #pragma unroll
           for (int b = 0; b < C::kBlocks * C::kGroups; ++b)
@@ -431,54 +582,39 @@ struct Kernel {
     }
 #pragma unroll
     for (int k = 0; k < C::kMt; ++k) {
-      uint32_t pt[NT][2], seen[NT][2];  // P^T's operand: column g, keys (2 t, 2 t + 1) and those + 8
+      float e[NT][4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float e[4];
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float base = m[n][i & 1] == -INFINITY ? 0.f : m[n][i & 1];
-          e[i] = ex2(s[k][n][i] - base);
-          l[n][i & 1] += e[i];
+          e[n][i] = ex2(d[k][n][i]);
+          l[n][i & 1] += e[n][i];
         }
-        const __nv_bfloat162 a = __floats2bfloat162_rn(e[0], e[1]), b = __floats2bfloat162_rn(e[2], e[3]);
-        pt[n][0] = turned(*reinterpret_cast<const uint32_t*>(&a));
-        pt[n][1] = turned(*reinterpret_cast<const uint32_t*>(&b));
-        if (TAIL) {
-          const int lim = lims[n * 8 + g], j = j0 + k * 16 + 2 * t;
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            seen[n][i] = (j + 8 * i < lim ? 0xffffu : 0u) | (j + 8 * i + 1 < lim ? 0xffff0000u : 0u);
-        }
-      }
 #pragma unroll
       for (int b = 0; b < C::kBlocks; ++b) {
-        uint32_t vw[4][W2], vs[4][W2];  // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9: the slots t, t + 4, t + 8, t + 12
+        uint32_t vw[4][W2], vs[2][W2];  // codes of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9 (slots t, t + 4, ...); scales of keys g, g + 8
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int slot = t + 4 * i;
-          if constexpr (W2 == 2)
-            load_words<2>(vw[i], vd + k * 16 * C::kRow + v_place<DIM>(slot, b * 4 + (g >> 1)) * 16 + (g & 1) * 8);
-          else
-            load_words<1>(vw[i], vd + k * 16 * C::kRow + slot * C::kRow + g * 4);
-          load_words<W2>(vs[i], vsd + (k * 16 + slot) * C::kScale + b * 8);
-        }
+        for (int i = 0; i < 4; ++i) load_words<W2>(vw[i], vd + k * 16 * C::kRow + 4 * i * C::kRow + (v_lane ^ (b * 64)));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) load_words<W2>(vs[i], vsd + g * C::kScale + (k * 16 + 8 * i) * C::kScale + b * 8);
 #pragma unroll
         for (int gr = 0; gr < C::kGroups; ++gr) {
           const uint32_t sel = (gr & 1) ? 0x7632u : 0x5410u;
           const uint32_t za = __byte_perm(vw[0][gr >> 1], vw[1][gr >> 1], sel), zb = __byte_perm(vw[2][gr >> 1], vw[3][gr >> 1], sel);
-          const uint32_t sa = __byte_perm(vs[0][gr >> 1], vs[1][gr >> 1], sel), sb = __byte_perm(vs[2][gr >> 1], vs[3][gr >> 1], sel);
-          const uint32_t a0[4] = {centred(za, 0), centred(za, 1), centred(zb, 0), centred(zb, 1)};
-          const uint32_t a1[4] = {centred(za, 2), centred(za, 3), centred(zb, 2), centred(zb, 3)};
+          const uint32_t a0[4] = {za & 0x000f000fu, za & 0x00f000f0u, zb & 0x000f000fu, zb & 0x00f000f0u};
+          const uint32_t a1[4] = {(za >> 8) & 0x000f000fu, (za >> 8) & 0x00f000f0u, (zb >> 8) & 0x000f000fu, (zb >> 8) & 0x00f000f0u};
+          const uint32_t eight[4] = {0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u};  // -8 in each place
+          const uint32_t w0 = vs[0][gr >> 1], w1 = vs[1][gr >> 1];
+          const float s0 = __uint_as_float((gr & 1) ? w0 & 0xffff0000u : w0 << 16), s1 = __uint_as_float((gr & 1) ? w1 & 0xffff0000u : w1 << 16);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            uint32_t b0 = mul_bf16x2(pt[n][0], sa), b1 = mul_bf16x2(pt[n][1], sb);
-            if (TAIL) {
-              b0 &= seen[n][0];
-              b1 &= seen[n][1];
-            }
-            mma_bf16(o[b * C::kGroups + gr][0][n], a0, b0, b1);
-            mma_bf16(o[b * C::kGroups + gr][1][n], a1, b0, b1);
+            auto weight = [&](int i) { return masked(k, n, i) ? 0.f : e[n][i] * ((i & 2) ? s1 : s0); };  // (a hidden scale may be NaN)
+            const uint32_t b0 = turned(half2_of(weight(0), weight(1))), b1 = turned(half2_of(weight(2), weight(3)));
+            float(&x)[2][NT][4] = o[b * C::kGroups + gr];
+            mma_f16(x[0][n], a0, b0, b1);
+            mma_f16(x[1][n], a1, b0, b1);
+            mma_f16(x[0][n], eight, b0, b1);
+            mma_f16(x[1][n], eight, b0, b1);
           }
         }
       }
@@ -503,7 +639,7 @@ struct Kernel {
   OMNI_DEV void end_unit(const Walk& w, int part) {
     float2* ml = reinterpret_cast<float2*>(smem + C::kMl);
     float* join = reinterpret_cast<float*>(smem + C::kJoin);
-    const int c0 = w.hc % p.chunks * C::kCols;
+    const int c0 = w.chunk * C::kCols;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -513,23 +649,30 @@ struct Kernel {
         if (g == 0) ml[warp * C::kCols + n * 8 + 2 * t + i] = make_float2(m[n][i], l[n][i]);
       }
     __syncthreads();
-    auto joined = [&](int col, float& top, float& sum) {
-      top = -INFINITY;
-      for (int k = 0; k < kWarps; ++k) top = fmaxf(top, ml[k * C::kCols + col].x);
-      const float base = top == -INFINITY ? 0.f : top;
-      sum = 0.f;
-      for (int k = 0; k < kWarps; ++k) sum = fmaf(ml[k * C::kCols + col].y, ex2(ml[k * C::kCols + col].x - base), sum);
-    };
+    if (threadIdx.x < C::kCols) {  // a column's maximum and sum; ml becomes (the warps' factors, the sum)
+      const int col = threadIdx.x;
+      float2 s[kWarps];
+      float top = kNone, sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) {
+        s[k] = ml[k * C::kCols + col];
+        top = fmaxf(top, s[k].x);
+      }
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) {
+        s[k].x = ex2(s[k].x - top);
+        sum = fmaf(s[k].y, s[k].x, sum);
+      }
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) ml[k * C::kCols + col] = make_float2(s[k].x, sum);
+      if (part >= 0 && c0 + col < p.cols) p.part_ml[(int64_t)part * C::kCols + col] = make_float2(top, sum);
+    }
+    __syncthreads();
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       if (c0 + n * 8 >= p.cols) break;
-      float f[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float top, sum;
-        joined(n * 8 + 2 * t + i, top, sum);
-        f[i] = ex2(m[n][i] - (top == -INFINITY ? 0.f : top));
-      }
+      const float f[2] = {ml[warp * C::kCols + n * 8 + 2 * t].x, ml[warp * C::kCols + n * 8 + 2 * t + 1].x};
+      const float low[2] = {f[0] * 0x1p24f, f[1] * 0x1p24f}, high[2] = {f[0] * 0x1p20f, f[1] * 0x1p20f};  // (by the dim's nibble)
 #pragma unroll
       for (int b = 0; b < C::kBlocks; ++b) {
 #pragma unroll
@@ -538,27 +681,24 @@ struct Kernel {
           for (int i = 0; i < 2; ++i) {
             const float(&x)[2][NT][4] = o[b * C::kGroups + gr];
             *reinterpret_cast<float4*>(join + (warp * 8 + 2 * t + i) * C::kPitch + gr * 32 + g * 4) =
-                make_float4(x[0][n][i] * f[i], x[0][n][i + 2] * f[i], x[1][n][i] * f[i], x[1][n][i + 2] * f[i]);
+                make_float4(x[0][n][i] * low[i], x[0][n][i + 2] * high[i], x[1][n][i] * low[i], x[1][n][i + 2] * high[i]);
           }
         __syncthreads();
         constexpr int Q4 = C::kGroups * 8;  // float4 of a column
+#pragma unroll
         for (int e = threadIdx.x; e < 8 * Q4; e += kThreads) {
           const int col = e / Q4, d = e % Q4 * 4;
           if (c0 + n * 8 + col < p.cols) {
             float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
             for (int k = 0; k < kWarps; ++k) {
               const float4 y = *reinterpret_cast<const float4*>(join + (k * 8 + col) * C::kPitch + d);
               x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
             }
-            float top, sum;
-            joined(n * 8 + col, top, sum);
-            if (part < 0) {
-              write_out(w, c0 + n * 8 + col, b * 128 + d, x, sum);
-            } else {
-              const int64_t at = (int64_t)part * C::kCols + n * 8 + col;
-              *reinterpret_cast<float4*>(p.part_o + at * DIM + b * 128 + d) = x;
-              if (b == 0 && d == 0) p.part_ml[at] = make_float2(top, sum);
-            }
+            if (part < 0)
+              write_out(w, c0 + n * 8 + col, b * 128 + d, x, ml[n * 8 + col].y);
+            else
+              *reinterpret_cast<float4*>(p.part_o + ((int64_t)part * C::kCols + n * 8 + col) * DIM + b * 128 + d) = x;
           }
         }
         __syncthreads();
@@ -569,26 +709,48 @@ struct Kernel {
   // The parts of a unit cut between the CTAs first .. last, in their order. A CTA's part of a unit that starts before its share is
   // its slot 0, of one that starts in it slot 1.
   OMNI_DEV void join_parts(const Walk& w, int first, int last) {
-    const int c0 = w.hc % p.chunks * C::kCols;
-    constexpr int Q4 = DIM / 4;
-    for (int e = threadIdx.x; e < C::kCols * Q4; e += kThreads) {
-      const int col = e / Q4, d = e % Q4 * 4;
-      if (c0 + col >= p.cols) break;
-      auto at = [&](int c) { return (int64_t)(2 * c + (c == first)) * C::kCols + col; };
-      float top = -INFINITY;
-      for (int c = first; c <= last; ++c) top = fmaxf(top, __ldcg(p.part_ml + at(c)).x);
-      const float base = top == -INFINITY ? 0.f : top;
-      float sum = 0.f;
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int c = first; c <= last; ++c) {
-        const float2 s = __ldcg(p.part_ml + at(c));
-        const float4 y = __ldcg(reinterpret_cast<const float4*>(p.part_o + at(c) * DIM + d));
-        const float f = ex2(s.x - base);
-        sum = fmaf(s.y, f, sum);
-        x.x = fmaf(y.x, f, x.x), x.y = fmaf(y.y, f, x.y), x.z = fmaf(y.z, f, x.z), x.w = fmaf(y.w, f, x.w);
+    const int c0 = w.chunk * C::kCols, cols = min(C::kCols, p.cols - c0);
+    float2* ml = reinterpret_cast<float2*>(smem + C::kMl);  // per column the maximum and the sum
+    auto at = [&](int c, int col) { return (int64_t)(2 * c + (c == first)) * C::kCols + col; };
+    for (int col = warp; col < cols; col += kWarps) {
+      float top = kNone, sum = 0.f;
+      for (int c = first + lane; c <= last; c += 32) top = fmaxf(top, __ldcg(p.part_ml + at(c, col)).x);
+#pragma unroll
+      for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+      for (int c = first + lane; c <= last; c += 32) {
+        const float2 s = __ldcg(p.part_ml + at(c, col));
+        sum = fmaf(s.y, ex2(s.x - top), sum);
       }
-      write_out(w, c0 + col, d, x, sum);
+#pragma unroll
+      for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+      if (lane == 0) ml[col] = make_float2(top, sum);
     }
+    __syncthreads();
+    constexpr int Q4 = DIM / 4;
+    for (int e = threadIdx.x; e < cols * Q4; e += kThreads) {
+      const int col = e / Q4, d = e % Q4 * 4;
+      const float2 s = ml[col];
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      constexpr int U = 8;  // parts in flight
+      for (int c = first; c <= last; c += U) {
+        float4 y[U];
+        float f[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+          const int64_t from = at(min(c + k, last), col);
+          y[k] = __ldcg(reinterpret_cast<const float4*>(p.part_o + from * DIM + d));
+          f[k] = __ldcg(p.part_ml + from).x;
+        }
+#pragma unroll
+        for (int k = 0; k < U; ++k)
+          if (c + k <= last) {
+            const float g = ex2(f[k] - s.x);
+            x.x = fmaf(y[k].x, g, x.x), x.y = fmaf(y[k].y, g, x.y), x.z = fmaf(y[k].z, g, x.z), x.w = fmaf(y[k].w, g, x.w);
+          }
+      }
+      write_out(w, c0 + col, d, x, s.y);
+    }
+    __syncthreads();  // (ml is the next unit's)
   }
 };
 
@@ -607,35 +769,34 @@ __global__ void __launch_bounds__(kThreads, Cfg<DIM, NT>::kCtas) int4_kernel(con
 
   // The shares: all units' blocks cut evenly.
   int64_t mine = 0;
+  int first_nb = 0;  // of the thread's first row
   for (int r = threadIdx.x; r < p.a.rows; r += kThreads) {
     Walk w;
-    rows.look(r, w);
-    mine += w.nb;
-    const int64_t given = p.a.lengths[r];
+    const int64_t given = rows.look(r, w);
+    mine += rows.places(w.nb);
+    if (r < kThreads) first_nb = w.nb;
     if (cta == 0 && (given < 0 || given > rows.cap - (p.a.tokens - 1))) raise_status(p.a.status, kStatusIndex);
-  }
-  const int64_t total = block_sum(mine, s_sum) * hcs;
-  const int64_t per = max((total + p.grid - 1) / p.grid, (int64_t)kWarps);
-  const int64_t b0 = min(total, per * cta), b1 = min(total, b0 + per);
-  // Rows without keys: zeros.
-  for (int r = cta; r < p.a.rows; r += p.grid) {
-    Walk w;
-    rows.look(r, w);
-    if (w.nb == 0) {
+    if (w.nb == 0 && r % p.grid == cta) {  // no keys: zeros
       const int64_t n = (int64_t)p.a.tokens * p.a.heads * DIM / 8;
       uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.a.out) + (int64_t)r * p.a.tokens * p.a.heads * DIM);
-      for (int64_t i = threadIdx.x; i < n; i += kThreads) dst[i] = make_uint4(0u, 0u, 0u, 0u);
+      for (int64_t i = 0; i < n; ++i) dst[i] = make_uint4(0u, 0u, 0u, 0u);
     }
   }
+  const int64_t total = block_sum(mine, s_sum) * hcs;
+  const int64_t per = max(quotient(total + p.grid - 1, p.grid), (int64_t)(kStart + kWarps));
+  const int64_t b0 = min(total, per * cta), b1 = min(total, b0 + per);
   if (b0 >= b1) return;
   // The row that b0 lies in: sums of kThreads rows at a time, then one after another within.
   {
     int64_t before = 0;
     for (int r0 = 0;; r0 += kThreads) {
       Walk w;
-      w.nb = 0;
-      if (r0 + (int)threadIdx.x < p.a.rows) rows.look(r0 + threadIdx.x, w);
-      const int64_t n = (int64_t)w.nb * hcs;
+      w.nb = first_nb;
+      if (r0 > 0) {
+        w.nb = 0;
+        if (r0 + (int)threadIdx.x < p.a.rows) rows.look(r0 + threadIdx.x, w);
+      }
+      const int64_t n = (int64_t)rows.places(w.nb) * hcs;
       int64_t x = n;  // the sum up to this thread's row
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -664,46 +825,66 @@ __global__ void __launch_bounds__(kThreads, Cfg<DIM, NT>::kCtas) int4_kernel(con
   Walk use;
   use.row = s_row;
   rows.look(use.row, use);
-  use.hc = (int)((b0 - s_u0) / use.nb);
-  use.u0 = s_u0 + (int64_t)use.hc * use.nb;
+  const int unit = (int)quotient(b0 - s_u0, use.nb + kStart);  // of the row
+  use.head = unit / p.chunks;
+  use.chunk = unit - use.head * p.chunks;
+  use.u0 = s_u0 + (int64_t)unit * (use.nb + kStart) + kStart;
 
-  // This warp's blocks: b0 + warp, and every kWarps-th from there.
+  // This warp's blocks of a unit: every kWarps-th from the CTA's first of it on.
+  auto from = [&](const Walk& w) { return (int)max((int64_t)0, b0 - w.u0) + k.warp; };
+  auto to = [&](const Walk& w) { return (int)min((int64_t)w.nb, b1 - w.u0); };
   Walk get = use;
-  int64_t next = b0 + k.warp;  // the next block to copy
-  int put = 0;                 // its stage
+  int next = from(get), upto = to(get);  // the next block to copy, of `get`'s unit; its end in this share
+  int put = 0;                           // its stage
+  typename Kernel<DIM, NT>::Source source;
+  k.open(source, get, next);
   auto fetch = [&]() {
-    if (next < b1) {
-      while (next >= get.u0 + get.nb) rows.next(get);
-      k.fetch(get, next, put);
+    if (next >= upto && get.u0 + get.nb < b1) {
+      do {
+        rows.next(get);
+        next = k.warp;
+        upto = to(get);
+      } while (next >= upto && get.u0 + get.nb < b1);
+      k.open(source, get, next);
+    }
+    if (next < upto) {
+      k.fetch(source, get, next, next + kWarps, put);
       next += kWarps;
     }
     copy_commit();
     put = put + 1 == C::kStages ? 0 : put + 1;
   };
+  uint4 words[Kernel<DIM, NT>::kPer][Kernel<DIM, NT>::kWords];
+  k.read_queries(use, words);
 #pragma unroll 1
   for (int i = 0; i < C::kStages - 1; ++i) fetch();
 
-  int64_t n = b0 + k.warp;
   int take = 0;
-  while (true) {
-    k.load_queries(use);
+  while (use.u0 < b1) {
+    k.store_queries(use, words);
     __syncthreads();
     k.start_unit();
-    const int64_t end = min(b1, use.u0 + use.nb);
-    const int full = max(0, use.len);  // keys that every column sees
+    const int end = to(use);
 #pragma unroll 1
-    for (; n < end; n += kWarps) {
+    for (int n = from(use); n < end; n += kWarps) {
       fetch();  // into the stage that the block before has left
       copy_wait<C::kStages - 1>();
       __syncwarp();
-      const int j0 = (int)(n - use.u0) * C::kKeys;
-      if (j0 + C::kKeys <= full) k.template block<false>(take, j0);
+      const int j0 = n * C::kKeys;
+      if (j0 + C::kKeys <= use.len) k.template block<false>(take, j0);
       else k.template block<true>(take, j0);
       __syncwarp();
       take = take + 1 == C::kStages ? 0 : take + 1;
     }
-    const int first = (int)(use.u0 / per), last = (int)((use.u0 + use.nb - 1) / per);
+    const int first = (int)quotient(use.u0, per), last = (int)quotient(use.u0 + use.nb - 1, per);
     const bool cut = first != last;
+    Walk then = use;
+    then.u0 = b1;  // (none)
+    if (use.u0 + use.nb < b1) {
+      then.u0 = use.u0;
+      rows.next(then);
+      if (then.u0 < b1) k.read_queries(then, words);  // while this unit ends
+    }
     k.end_unit(use, cut ? 2 * cta + (cta == first) : -1);
     if (cut) {
       __threadfence();
@@ -716,8 +897,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<DIM, NT>::kCtas) int4_kernel(con
       __syncthreads();
       if (s_last) k.join_parts(use, first, last);
     }
-    if (end == b1) break;
-    rows.next(use);
+    use = then;
   }
   copy_wait<0>();
 }
@@ -725,8 +905,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<DIM, NT>::kCtas) int4_kernel(con
 // Tiles of 8 columns of a unit: as many as share the keys while the accumulators stay in registers.
 int most_tiles(int dim) { return dim <= 128 ? 4 : dim == 256 ? 2 : 1; }
 
-int tiles_of(int dim, int cols) {
+// One tile per unit where a block per warp covers all tiles' keys all the same (the keys are then read by several units, out of L2):
+// a unit's start and end take as long as its tiles are many (5 x 32 queries over 700 keys, 8 kv heads: ONETILE us; three tiles a unit: MANYTILES).
+int tiles_of(const PagedAttnArgs& a) {
+  const int cols = a.tokens * (a.heads / a.c.kv_heads), dim = a.c.dim;
   const int tiles = (cols + 7) / 8, most = most_tiles(dim);
+  const int64_t blocks = ((int64_t)a.table_width * a.c.page + 31) / 32 * a.rows * a.c.kv_heads;
+  if (blocks * tiles <= (int64_t)4 * kWarps * device_sm_count()) return 1;
   const int chunks = (tiles + most - 1) / most;
   return (tiles + chunks - 1) / chunks;
 }
@@ -746,6 +931,11 @@ cudaError_t launch(const PagedAttnArgs& a, cudaStream_t s) {
   p.cols = a.tokens * (a.heads / a.c.kv_heads);
   p.chunks = (p.cols + C::kCols - 1) / C::kCols;
   p.grid = grid_of<DIM, NT>();
+  p.page_shift = -1;
+  const int64_t scales = (int64_t)a.c.kv_heads * a.c.page * C::kScale;
+  if (a.c.page >= 16 && (a.c.page & (a.c.page - 1)) == 0 && a.c.s_pos == C::kRow && a.c.s_page < 0x7fffffff && scales < 0x7fffffff)
+    p.page_shift = __builtin_ctz(a.c.page);
+  p.page_scales = (uint32_t)scales;
   p.counters = reinterpret_cast<unsigned*>(a.workspace);
   p.part_o = reinterpret_cast<float*>(reinterpret_cast<char*>(a.workspace) + kCounterBytes);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + (int64_t)2 * p.grid * C::kCols * DIM);
@@ -763,7 +953,7 @@ size_t paged_int4_workspace(int dim) {
 
 cudaError_t launch_paged_attention_int4(const PagedAttnArgs& a, cudaStream_t s) {
   using namespace paged4;
-  const int nt = tiles_of(a.c.dim, a.tokens * (a.heads / a.c.kv_heads));
+  const int nt = tiles_of(a);
   switch (a.c.dim * 8 + nt) {
     case 64 * 8 + 1: return launch<64, 1>(a, s);
     case 64 * 8 + 2: return launch<64, 2>(a, s);

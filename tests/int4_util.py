@@ -57,6 +57,8 @@ def cache(pages, kv, page, dim, gen):
     return k, v, ks, vs, kval, vval
 
 
-def paged_want(q, kval, vval, table, length, scale, tokens):
-    """(o, sum p |v| / sum p) in float64."""
-    return (pu.paged(q, kval, vval, table, length, scale, tokens), pu.paged(q, kval, vval.abs(), table, length, scale, tokens))
+def paged_want(q, kval, vval, vs, table, length, scale, tokens):
+    """(o, (sum p |v| / sum p, sum p |s| / sum p with each group's scale s)) in float64."""
+    groups = vs.float().abs().repeat_interleave(32, -1)
+    return (pu.paged(q, kval, vval, table, length, scale, tokens),
+            (pu.paged(q, kval, vval.abs(), table, length, scale, tokens), pu.paged(q, kval, groups, table, length, scale, tokens)))

@@ -1,9 +1,11 @@
 """The 4-bit paged cache on the GPU: write, read back and attention, and the norms of queries and keys with the append.
 
 Writes and read-backs of paged_rope_kv are exact (the rotation is rounded as the plain form rounds it, the codes are one fp32
-division). Attention, bf16: the output's rounding is at most 2^-8 |o|; a probability is rounded to bf16 (2^-8 of it, in the sum
-of weights too) and its product with a group's scale once more (2^-8): 2^-7 A + 2^-8 |o| with A = sum p |v| / sum p; fp32 sums, the
-exponential and the products stay well under 2^-10 A. fp32: 2e-5 (1 + |o|), the framework's own.
+division). Attention, bf16: the output's rounding is at most 2^-8 |o|; a probability times its group's scale s is rounded once, to
+fp16, by 2^-11 of it: 2^-11 A with A = sum p |v| / sum p; the scores' products and sums, the exponential and the weights' sum stay well
+under 2^-10 A. The sums of products with the codes c and with their offset, each at most 15 B with B = sum p |s| / sum p, are kept in
+fp32: two steps per 16 keys and warp, at least 4 warps, each off by at most 2^-23 of 15 B, for at most 5000 keys 158 x 15 x 2^-23 B <
+2^-11 B. fp32: 2e-5 (1 + |o|), the framework's own.
 Norms: the sum of squares takes at most 21 roundings (16 terms a lane, 5 steps of a shuffle), which the root halves, the root
 itself 4 half steps, the two products, the rotation's and its sum 4: under 32 x 2^-24 = 2^-19 of the terms that a rotation adds,
 and the one rounding to the type."""
@@ -25,7 +27,10 @@ dev = lambda t: None if t is None else t.to(DEV)  # noqa: E731
 def check(got, want, size, dtype):
     got = got.double().cpu()
     assert bool(torch.isfinite(got).all()), "not finite"
-    bound = 2e-5 * (1 + want.abs()) if dtype == torch.float32 else 2.0**-7 * (want.abs() + size) + 2.0**-10 * size + 1e-30
+    if dtype == torch.float32:
+        bound = 2e-5 * (1 + want.abs())
+    else:
+        bound = 2.0**-8 * want.abs() + (2.0**-11 + 2.0**-10) * size[0] + 2.0**-11 * size[1] + 1e-30
     bad = (got - want).abs() > bound
     assert not bool(bad.any()), f"{int(bad.sum())} of {bad.numel()} past the bound; worst " \
                                 f"{float(((got - want).abs() / bound).max()):.3g} times"
@@ -55,7 +60,7 @@ def run_paged(heads, kv, dim, page, lens, tokens, dtype, seed=0, layout="page", 
     _, covered, table, k, v, ks, vs, kval, vval, q = inputs(heads, kv, dim, page, lens, tokens, dtype, seed)
     scale = dim**-0.5 if scale is None else scale
     length = torch.tensor(lens)
-    want, size = iu.paged_want(q, kval, vval, table, length, scale, tokens)
+    want, size = iu.paged_want(q, kval, vval, vs, table, length, scale, tokens)
     spoil(k, v, ks, vs, table, covered, page)
     k, v = dev(k), dev(v)
     if layout == "token":  # [pages, page, kv, D / 2] storage
@@ -113,7 +118,7 @@ def test_attention_of_queries_of_all_sizes():
     for h, e in enumerate([-100, -40, -20, -8, 0, 2, 4, 6]):
         q[:, h] *= 2.0**e
     length = torch.tensor([200, 31])
-    want, size = iu.paged_want(q, kval, vval, table, length, 0.2, 1)
+    want, size = iu.paged_want(q, kval, vval, vs, table, length, 0.2, 1)
     got = kernels.paged_attention(dev(q), dev(k), dev(v), dev(table), dev(length), 0.2, k_scale=dev(ks), v_scale=dev(vs))
     check(got, want, size, torch.bfloat16)
 
@@ -125,7 +130,7 @@ def test_values_that_are_not_finite(dim, dtype):
     heads, kv, page, tokens, lens = 4, 2, 16, 3, [70, 20, 48, 5]
     _, covered, table, k, v, ks, vs, kval, vval, q = inputs(heads, kv, dim, page, lens, tokens, dtype, 9)
     length = torch.tensor(lens)
-    want, size = iu.paged_want(q, kval, vval, table, length, 0.1, tokens)
+    want, size = iu.paged_want(q, kval, vval, vs, table, length, 0.1, tokens)
     spoil(k, v, ks, vs, table, covered, page)
     at = lambda r, j: (int(table[r, j // page]), j % page)  # noqa: E731
     hide = torch.zeros(len(lens) * tokens, heads, dim, dtype=torch.bool)
@@ -157,7 +162,7 @@ def test_bad_pages_are_reported_and_skipped():
     _, covered, table, k, v, ks, vs, kval, vval, q = inputs(8, 2, 128, 16, [60, 60], 1, "bf16", 11)
     table[1, 2] = k.size(0)
     length = torch.tensor([60, 60])
-    want, size = iu.paged_want(q[:1], kval, vval, table[:1], length[:1], 0.1, 1)
+    want, size = iu.paged_want(q[:1], kval, vval, vs, table[:1], length[:1], 0.1, 1)
     got = kernels.paged_attention(dev(q), dev(k), dev(v), dev(table), dev(length), 0.1, k_scale=dev(ks), v_scale=dev(vs))
     assert kernels.read_status() == 1
     check(got[:1], want, size, torch.bfloat16)
