@@ -19,6 +19,7 @@ struct Gemm4Args {
   int wrows;              // weight rows: n, SwiGLU 2n
   int blocks, groups;     // ceil(k / 128), ceil(k / group)
   int group;              // 32, 64 or 128
+  uint32_t mask;          // set by the launcher
   int mode;               // GemmMode: store, residual, SwiGLU
   const __nv_bfloat16* residual;
   int64_t ld_res;
