@@ -114,7 +114,13 @@ __global__ void __launch_bounds__(kReadThreads) paged_read_kernel(const PagedRea
     const int64_t dst = (tok * kvh + h) * D + c * kOut;
     uint4* ko = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.k_out) + dst);
     uint4* vo = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.v_out) + dst);
-    if constexpr (KIND == kInt4) {
+    if constexpr (KIND == kInt4 && kOut == 8) {
+      const uint32_t k2 = __float_as_uint(ks[r]) >> 16, v2 = __float_as_uint(vs[r]) >> 16;
+      const uint2 k0 = int4_values_bf16(ku[r] & 0xffffu, k2 | k2 << 16), k1 = int4_values_bf16(ku[r] >> 16, k2 | k2 << 16);
+      const uint2 v0 = int4_values_bf16(vu[r] & 0xffffu, v2 | v2 << 16), v1 = int4_values_bf16(vu[r] >> 16, v2 | v2 << 16);
+      __stcs(ko, make_uint4(k0.x, k0.y, k1.x, k1.y));
+      __stcs(vo, make_uint4(v0.x, v0.y, v1.x, v1.y));
+    } else if constexpr (KIND == kInt4) {
       float kf[kOut], vf[kOut];
 #pragma unroll
       for (int q = 0; q < kOut / 4; ++q) {

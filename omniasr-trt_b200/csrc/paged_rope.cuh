@@ -52,10 +52,10 @@ constexpr int kRopeThreads = 256;
 // 53 us, 5470 GB/s, with three and registers for six CTAs per SM; a CTA that walks tokens with the next one's loads in
 // flight needs twice the registers: 93 us.)
 // KIND: what the pages hold. NORM: q and k are normed per head first, x * rsqrt(mean x^2 + eps) * w, all in fp32 with the one rounding
-// after the rotation; a thread's dims are the same for all its vectors, so it holds their two weights' words (q's, k's) in
-// registers, and the sum of squares is a shuffle reduction over the vector's lanes of values that are there already.
+// after the rotation; the weights come out of L1 (held in registers they cost a CTA per SM: 71 us for the prompts below with the norm, 65 without), and
+// the sum of squares is a shuffle reduction over the vector's lanes of values that are there already.
 template <typename T, int D, int KIND, bool NORM, int IL>
-__global__ void __launch_bounds__(kRopeThreads, D * sizeof(T) > 512 ? 2 : KIND == kInt4 || NORM ? 4 : IL == 4 ? 5 : 6) paged_rope_kernel(const PagedRopeArgs a, int per) {
+__global__ void __launch_bounds__(kRopeThreads, D * sizeof(T) > 512 ? 2 : KIND == kInt4 ? 5 : IL == 4 ? 5 : 6) paged_rope_kernel(const PagedRopeArgs a, int per) {
   constexpr int kVec = Elem<T>::kVec;
   constexpr int VPV = D / kVec;            // 16-byte words per vector
   constexpr int L = VPV < 32 ? VPV : 32;   // lanes per vector
@@ -101,14 +101,6 @@ __global__ void __launch_bounds__(kRopeThreads, D * sizeof(T) > 512 ? 2 : KIND =
       cs[v][4 * i + 2] = f.z;
       cs[v][4 * i + 3] = f.w;
     }
-  uint4 wq[NORM ? NV : 1], wk[NORM ? NV : 1];
-  if constexpr (NORM) {
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      wq[v] = __ldg(reinterpret_cast<const uint4*>(a.q_norm) + v * L + lane);
-      wk[v] = __ldg(reinterpret_cast<const uint4*>(a.k_norm) + v * L + lane);
-    }
-  }
   // Every team of a warp takes the same number of rounds (the scale's shuffles need the whole warp).
   for (int base = i0; base < i1; base += TEAMS * IL) {
     if (base > i0) load(base);
@@ -142,7 +134,7 @@ __global__ void __launch_bounds__(kRopeThreads, D * sizeof(T) > 512 ? 2 : KIND =
           Elem<T>::unpack(u[j][v], x);
           if constexpr (NORM) {
             float w[kVec];
-            Elem<T>::unpack(it < a.heads ? wq[v] : wk[v], w);
+            Elem<T>::unpack(__ldg(reinterpret_cast<const uint4*>(it < a.heads ? a.q_norm : a.k_norm) + v * L + lane), w);
 #pragma unroll
             for (int i = 0; i < kVec; ++i) x[i] = x[i] * inv_rms * w[i];
           }
@@ -219,13 +211,15 @@ __global__ void __launch_bounds__(kRopeThreads, D * sizeof(T) > 512 ? 2 : KIND =
           const bool finite = amax < 0x7f800000u;
           const uint32_t bits = finite ? (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn((hi > -lo ? hi : lo) * -0.125f)) : 0x7fffu;
           const float s = finite ? bf16_value(bits) : 0.f;
+          const bool fast = sizeof(T) == 2 && (s == 0.f || fabsf(s) >= kInt4Fast);
+          const float inv = fast && s != 0.f ? __fdividef(1.f, s) : 0.f;
           if (write) {
             const int w = v * L + lane;  // the vector's 16-byte word
 #pragma unroll
             for (int q = 0; q < kVec / 4; ++q) {
               const int quad = w * (kVec / 4) + q;
               reinterpret_cast<uint16_t*>(row)[is_k ? quad_at<D, true>(quad) : quad_at<D, false>(quad)] =
-                  (uint16_t)int4_codes(y[v] + 4 * q, s);
+                  (uint16_t)(fast ? int4_codes_bf16(y[v] + 4 * q, inv) : int4_codes(y[v] + 4 * q, s));
             }
             if (lane % GL == 0) scales[w / GL] = (uint16_t)bits;
           }
