@@ -26,21 +26,23 @@ namespace paged {
 
 constexpr int kThreads = 128;
 
+// Eight consecutive elements of a cache row (or a query) as floats. Ordinary loads: one through the read-only path may be moved ahead
+// of the wait for the kernel that writes the queries.
 template <typename T>
-struct Row8;  // eight consecutive elements of a cache row as floats
+struct Row8;
 
 template <>
 struct Row8<__nv_bfloat16> {
   uint4 u;
-  OMNI_DEV void load(const void* base, int64_t at) { u = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(base) + at)); }
+  OMNI_DEV void load(const void* base, int64_t at) { u = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(base) + at); }
   OMNI_DEV void get(float* f) const { Elem<__nv_bfloat16>::unpack(u, f); }
 };
 template <>
 struct Row8<float> {
   float4 a, b;
   OMNI_DEV void load(const void* base, int64_t at) {
-    a = __ldg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(base) + at));
-    b = __ldg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(base) + at) + 1);
+    a = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(base) + at);
+    b = *(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(base) + at) + 1);
   }
   OMNI_DEV void get(float* f) const {
     f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;

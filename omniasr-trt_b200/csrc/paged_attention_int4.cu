@@ -245,7 +245,7 @@ struct Kernel {
   OMNI_DEV void look_up(Source& f, const Walk& w, int block) const {  // (past the row's end: its last page)
     const int last = (w.need - 1) >> p.page_shift;
 #pragma unroll
-    for (int tile = 0; tile < C::kMt; ++tile) f.id[tile] = __ldg(f.table + min((block * C::kKeys + tile * 16) >> p.page_shift, last));
+    for (int tile = 0; tile < C::kMt; ++tile) f.id[tile] = *(f.table + min((block * C::kKeys + tile * 16) >> p.page_shift, last));
   }
   OMNI_DEV void open(Source& f, const Walk& w, int block) const {
     if (p.page_shift < 0) return;
@@ -361,7 +361,7 @@ struct Kernel {
 #pragma unroll
       for (int v = 0; v < kWords; ++v) {
         const int word = v * 32 + lane;
-        u[k][v] = on && word * 8 < DIM ? __ldg(src + word) : make_uint4(0u, 0u, 0u, 0u);
+        u[k][v] = on && word * 8 < DIM ? src[word] : make_uint4(0u, 0u, 0u, 0u);
       }
     }
   }

@@ -76,7 +76,8 @@ __global__ void __launch_bounds__(kRopeThreads, D * sizeof(T) > 512 ? 2 : KIND =
       const int it = base + j * TEAMS + team;
 #pragma unroll
       for (int v = 0; v < NV; ++v)
-        u[j][v] = it < i1 ? __ldg(reinterpret_cast<const uint4*>(src + (int64_t)it * D) + v * L + lane)
+        // (An ordinary load: one through the read-only path may be moved ahead of the wait for the kernel before.)
+        u[j][v] = it < i1 ? reinterpret_cast<const uint4*>(src + (int64_t)it * D)[v * L + lane]
                           : make_uint4(0u, 0u, 0u, 0u);
     }
   };

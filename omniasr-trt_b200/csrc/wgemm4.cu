@@ -41,6 +41,10 @@ OMNI_DEV uint32_t pair_of(uint32_t w, int i, uint32_t mask) {
   return r;
 }
 
+// Tokens come from the kernel before: an ordinary load, which stays behind the wait for it. (A load through the read-only path
+// counts as independent of every write and may be moved ahead of the wait.)
+OMNI_DEV uint4 token_words(const __nv_bfloat16* p) { return *reinterpret_cast<const uint4*>(p); }
+
 // A block of 128 columns of two weight rows (words u0, u1; scales f0, f1 per group) times NT tiles of 8 tokens; x(n, w): a lane's 8
 // columns 32 w + 8 t .. of token n * 8 + g.
 template <int NT, int PER, typename X>
@@ -132,7 +136,7 @@ __global__ void __launch_bounds__(32 * W, W == 4 ? 5 : NT <= 4 ? 2 : 1) gemm4_ke
 #pragma unroll
     for (int p = 0; p < N; ++p)
       block_product<NT, PER>(u0[p], u1[p], f0[p], f1[p], a.mask,
-                             [&](int n, int w) { return __ldg(reinterpret_cast<const uint4*>(x[n] + p * W * 128 + w * 32)); }, acc);
+                             [&](int n, int w) { return token_words(x[n] + p * W * 128 + w * 32); }, acc);
     c0 += N * W * 32;
     c1 += N * W * 32;
     s0 += N * W * PER * 8;
@@ -156,7 +160,7 @@ __global__ void __launch_bounds__(32 * W, W == 4 ? 5 : NT <= 4 ? 2 : 1) gemm4_ke
     waited = true;
     block_product<NT, PER>(u0, u1, f0, f1, a.mask,
                            [&](int n, int w) {
-                             return b * 128 + w * 32 + t * 8 < a.k ? __ldg(reinterpret_cast<const uint4*>(x[n] + w * 32)) : make_uint4(0u, 0u, 0u, 0u);
+                             return b * 128 + w * 32 + t * 8 < a.k ? token_words(x[n] + w * 32) : make_uint4(0u, 0u, 0u, 0u);
                            },
                            acc);
   }

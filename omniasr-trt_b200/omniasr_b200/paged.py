@@ -4,6 +4,8 @@
 A sequence holds whole pages of every layer; its positions lie in them in order. :class:`PagedCache` keeps which pages a
 sequence has and gives the kernels' index tensors for a batch; :meth:`PagedCache.prefill` and :meth:`PagedCache.decode` are
 one layer's attention of a batch of prompts (or chunks of them) and of one new token (or a draft) per sequence.
+:class:`DeviceTables` is the same bookkeeping on the GPU (``paged_plan``, ``paged_trim``), for decode loops that the host does
+not steer step by step, in a CUDA graph for instance.
 """
 
 from __future__ import annotations
@@ -20,7 +22,7 @@ class Batch:
     """A step's index tensors (device): which sequences, where their new tokens go, and what they see."""
 
     tokens: int  # new tokens in all
-    new: list[int]  # new tokens per sequence
+    new: list[int] | None  # new tokens per sequence (None: the GPU alone knows)
     total: int  # keys in all, the new tokens' among them
     pos: torch.Tensor  # [tokens] position of each new token
     slots: torch.Tensor  # [tokens] page number * page + offset
@@ -28,25 +30,32 @@ class Batch:
     lengths: torch.Tensor  # [sequences] keys before the new tokens, plus one
     q_offsets: torch.Tensor  # [sequences + 1]
     k_offsets: torch.Tensor  # [sequences + 1]
-    fresh: bool  # no sequence had keys before this step
+    fresh: bool  # no sequence had keys before this step (False where the GPU alone knows)
+    taken: torch.Tensor | None = None  # DeviceTables: [sequences] which requests got their pages
 
 
 class PagedCache:
     """``layers`` caches of ``pages`` pages of ``page`` positions, ``kv_heads`` heads of ``dim``; ``kind`` is the element type:
-    the model's dtype, or ``torch.float8_e4m3fn`` (codes with one power-of-two scale byte per position and head)."""
+    the model's dtype, ``torch.float8_e4m3fn`` (codes with one power-of-two scale byte per position and head), or ``torch.uint8``
+    (4-bit codes with a bfloat16 scale per 32 dims, ``dim`` 32 and more: 4.5 bits a value)."""
 
     def __init__(self, layers: int, pages: int, page: int, kv_heads: int, dim: int, dtype: torch.dtype = torch.bfloat16,
                  kind: torch.dtype | None = None, device: torch.device | str = "cuda"):
         self.page, self.kv_heads, self.dim, self.dtype = page, kv_heads, dim, dtype
         self.device = torch.device(device)
         kind = dtype if kind is None else kind
-        shape = (layers, pages, kv_heads, page, dim)
+        if kind == torch.uint8 and dim % 32:
+            raise ValueError(f"PagedCache: 4-bit codes of head_dim {dim} (a multiple of 32)")
+        shape = (layers, pages, kv_heads, page, dim // 2 if kind == torch.uint8 else dim)
         self.k = torch.zeros(shape, dtype=kind, device=self.device)
         self.v = torch.zeros(shape, dtype=kind, device=self.device)
         self.k_scale = self.v_scale = None
         if kind == torch.float8_e4m3fn:
             self.k_scale = torch.full(shape[:-1], 127, dtype=torch.uint8, device=self.device)
             self.v_scale = torch.full(shape[:-1], 127, dtype=torch.uint8, device=self.device)
+        if kind == torch.uint8:
+            self.k_scale = torch.zeros(*shape[:-1], dim // 32, dtype=torch.bfloat16, device=self.device)
+            self.v_scale = torch.zeros_like(self.k_scale)
         self._free = list(range(pages - 1, -1, -1))
         self._pages: dict[int, list[int]] = {}
         self._length: dict[int, int] = {}
@@ -105,33 +114,83 @@ class PagedCache:
                      up(torch.tensor([p + 1 for p in past], dtype=torch.int64)), up(offsets(list(new))), up(offsets(both)),
                      not any(past))
 
+    def device_tables(self, seqs: int, width: int, pages: int | None = None) -> DeviceTables:
+        """Tables on the GPU for ``seqs`` sequences of at most ``width`` pages, which take ``pages`` of the free pages (all of them
+        by default) over: this object's own sequences no longer get those."""
+        count = len(self._free) if pages is None else pages
+        if not 0 <= count <= len(self._free):
+            raise ValueError(f"device_tables: {count} pages of {len(self._free)} free")
+        taken = [self._free.pop() for _ in range(count)]
+        return DeviceTables(seqs, width, self.page, taken[::-1], self.device)
+
     def _layer(self, layer: int) -> tuple:
         scales = (None, None) if self.k_scale is None else (self.k_scale[layer], self.v_scale[layer])
         return self.k[layer], self.v[layer], scales
 
-    def write(self, layer: int, qkv: torch.Tensor, cs: torch.Tensor, batch: Batch, heads: int) -> torch.Tensor:
-        """RoPE of the new tokens' q and k, their k and v into the layer's pages; returns q [tokens, heads, D]."""
+    def write(self, layer: int, qkv: torch.Tensor, cs: torch.Tensor, batch: Batch, heads: int,
+              norms: tuple[torch.Tensor, torch.Tensor, float] | None = None) -> torch.Tensor:
+        """RoPE of the new tokens' q and k, their k and v into the layer's pages; returns q [tokens, heads, D]. ``norms`` (q's
+        weights [D], k's, epsilon): q and k are normed per head before."""
         k, v, (ks, vs) = self._layer(layer)
-        return kernels.paged_rope_kv(qkv, cs, batch.pos, k, v, batch.slots, heads, self.kv_heads, k_scale=ks, v_scale=vs)
+        if norms is None:
+            return kernels.paged_rope_kv(qkv, cs, batch.pos, k, v, batch.slots, heads, self.kv_heads, k_scale=ks, v_scale=vs)
+        return kernels.paged_norm_rope_kv(qkv, norms[0], norms[1], cs, batch.pos, k, v, batch.slots, heads, self.kv_heads,
+                                          eps=norms[2], k_scale=ks, v_scale=vs)
 
-    def prefill(self, layer: int, qkv: torch.Tensor, cs: torch.Tensor, batch: Batch, heads: int,
-                scale: float | None = None) -> torch.Tensor:
+    def prefill(self, layer: int, qkv: torch.Tensor, cs: torch.Tensor, batch: Batch, heads: int, scale: float | None = None,
+                norms: tuple[torch.Tensor, torch.Tensor, float] | None = None) -> torch.Tensor:
         """One layer's causal attention of a batch of prompts, or of chunks whose earlier keys the cache holds: writes the new
-        keys and reads all of them back as packed rows (what a later step sees, an 8-bit cache's rounding included)."""
-        q = self.write(layer, qkv, cs, batch, heads)
+        keys and reads all of them back as packed rows (what a later step sees, an 8-bit or 4-bit cache's rounding included)."""
+        q = self.write(layer, qkv, cs, batch, heads, norms)
         k, v, (ks, vs) = self._layer(layer)
         kk, vv = kernels.paged_kv_read(k, v, batch.table, batch.k_offsets, batch.total, k_scale=ks, v_scale=vs, dtype=self.dtype)
         return kernels.packed_attention(q, kk, vv, batch.q_offsets, batch.k_offsets, scale)
 
-    def decode(self, layer: int, qkv: torch.Tensor, cs: torch.Tensor, batch: Batch, heads: int,
-               scale: float | None = None) -> torch.Tensor:
+    def decode(self, layer: int, qkv: torch.Tensor, cs: torch.Tensor, batch: Batch, heads: int, scale: float | None = None,
+               norms: tuple[torch.Tensor, torch.Tensor, float] | None = None) -> torch.Tensor:
         """One layer's attention of the same number of new tokens (one, or a draft) of every sequence, straight over the
         pages."""
-        if len(set(batch.new)) > 1:
+        if batch.new is None or len(set(batch.new)) > 1:
             raise ValueError("decode: the same number of new tokens for every sequence (prefill takes others)")
-        q = self.write(layer, qkv, cs, batch, heads)
+        q = self.write(layer, qkv, cs, batch, heads, norms)
         if not any(batch.new):
             return q  # no queries
         k, v, (ks, vs) = self._layer(layer)
         return kernels.paged_attention(q, k, v, batch.table, batch.lengths, self.dim**-0.5 if scale is None else scale,
                                        tokens=batch.new[0], k_scale=ks, v_scale=vs)
+
+
+class DeviceTables:
+    """Which pages ``seqs`` sequences have, on the GPU: lengths, a table of at most ``width`` page numbers a sequence, and the free
+    pages as a stack (``free``: their numbers, the last is taken first). Sequences are numbered from 0 and begin without keys."""
+
+    def __init__(self, seqs: int, width: int, page: int, free: list[int], device: torch.device | str = "cuda"):
+        device = torch.device(device)
+        self.page, self.width = page, width
+        self.length = torch.zeros(seqs, dtype=torch.int64, device=device)
+        self.table = torch.zeros(seqs, width, dtype=torch.int32, device=device)
+        self.free = torch.tensor(free, dtype=torch.int32).to(device)
+        self.free_count = torch.tensor([len(free)], dtype=torch.int64).to(device)
+
+    def _state(self) -> tuple:
+        return self.length, self.table, self.free, self.free_count
+
+    def plan(self, rows: torch.Tensor, new: int | torch.Tensor, tokens: int | None = None, total: int | None = None,
+             width: int | None = None) -> Batch:
+        """Room for new tokens of the sequences ``rows`` [B] (int64, on the GPU), ``new`` of each or ``new[i]`` of the i-th ([B], then
+        with ``tokens``, a number that the host knows, at least their sum). ``total`` (for :meth:`PagedCache.prefill`): at least the
+        keys of all these sequences after the step. ``width``: pages a sequence that the step's table has room for. Nothing waits
+        for the GPU: whether the pages sufficed is in the batch's ``taken``, as :func:`kernels.paged_plan` describes it."""
+        b = rows.numel()
+        each = None
+        if isinstance(new, int):
+            each, new, tokens = new, torch.full((b,), new, dtype=torch.int64, device=rows.device), b * new
+        if tokens is None:
+            raise ValueError("plan: new tokens per request on the GPU need their number (tokens)")
+        pos, slots, table, lengths, q_offsets, k_offsets, taken = kernels.paged_plan(rows, new, tokens, self.page, *self._state(), width=width)
+        return Batch(tokens, None if each is None else [each] * b, 0 if total is None else total, pos, slots, table, lengths, q_offsets,
+                     k_offsets, False, taken)
+
+    def trim(self, rows: torch.Tensor, keep: torch.Tensor) -> None:
+        """The sequences ``rows`` keep their first ``keep`` positions (both int64 on the GPU; 0 frees a sequence)."""
+        kernels.paged_trim(rows, keep, self.page, *self._state())
