@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(256) split_attention_kernel(const SplitArgs a)
       for (int c = 0; c < S::kCpl; ++c) {
         float f[S::kVec];
         if (i < nqb) {
-          const uint4 u = __ldg(reinterpret_cast<const uint4*>(qb + (int64_t)i * a.heads * D) + lane + c * S::kLanes);
+          const uint4 u = reinterpret_cast<const uint4*>(qb + (int64_t)i * a.heads * D)[lane + c * S::kLanes];
           Elem<T>::unpack(u, f);
         } else {
 #pragma unroll

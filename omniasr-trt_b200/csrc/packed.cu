@@ -74,12 +74,12 @@ template <typename T>
 OMNI_DEV void load4(const T* p, float* f);
 template <>
 OMNI_DEV void load4<float>(const float* p, float* f) {
-  const float4 v = __ldg(reinterpret_cast<const float4*>(p));
+  const float4 v = *reinterpret_cast<const float4*>(p);
   f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
 }
 template <>
 OMNI_DEV void load4<__nv_bfloat16>(const __nv_bfloat16* p, float* f) {
-  const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+  const uint2 v = *reinterpret_cast<const uint2*>(p);
   f[0] = __uint_as_float(v.x << 16), f[1] = __uint_as_float(v.x & 0xffff0000u);
   f[2] = __uint_as_float(v.y << 16), f[3] = __uint_as_float(v.y & 0xffff0000u);
 }
