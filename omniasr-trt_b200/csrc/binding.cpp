@@ -297,10 +297,8 @@ py::object paged_plan(const at::Tensor& rows, const at::Tensor& fresh, int64_t t
   const int64_t b = t.requests;
   const auto i64 = length.options();
   // One allocation for the int64 outputs: positions, slots, lengths, offsets.
-  at::Tensor all = at::empty({2 * tokens + 3 * b + 2}, i64);
-  auto part = [&](int64_t from, int64_t n) { return all.narrow(0, from, n); };
-  at::Tensor pos = part(0, tokens), slots = part(tokens, tokens), lengths = part(2 * tokens, b), qo = part(2 * tokens + b, b + 1),
-             ko = part(2 * tokens + 2 * b + 1, b + 1);
+  const std::vector<at::Tensor> parts = at::empty({2 * tokens + 3 * b + 2}, i64).unsafe_split_with_sizes({tokens, tokens, b, b + 1, b + 1});
+  const at::Tensor &pos = parts[0], &slots = parts[1], &lengths = parts[2], &qo = parts[3], &ko = parts[4];
   at::Tensor out = at::empty({b, w}, table.options()), taken = at::empty({b}, i64.dtype(at::kBool));
   done("omniasr_paged_plan",
        omniasr_paged_plan(t.rows.data_ptr<int64_t>(), t.want.data_ptr<int64_t>(), (int)b, tokens, (int)page, length.data_ptr<int64_t>(),
