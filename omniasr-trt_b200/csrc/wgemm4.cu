@@ -14,7 +14,8 @@
 // order of the tokens' memory.
 //
 // A CTA takes one 16-row tile (SwiGLU: 8 gate and their 8 inner rows), its warps the blocks of 128 columns in turn, a few
-// of a warp's blocks in flight; their sums meet in shared memory in warp order.
+// of a warp's blocks in flight; their sums meet in shared memory in warp order. Measured: 8 tokens, 2 x 11008 x 4096 SwiGLU, 13.4 us (7.1 at HBM's
+// rate). From between 16 and 32 tokens on the tokens' reads out of L2 bound it: 22016 x 4096, 64 tokens 75 us (a bf16 library product 37).
 
 #include <type_traits>
 

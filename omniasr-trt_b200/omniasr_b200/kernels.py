@@ -15,11 +15,14 @@ CUDA-graph capture run on these kernels unchanged:
 * :func:`reorder_gather` -- the beam reorder ``dst[r] = src[parent[r]]``, byte-exact (``llm.py:237-238``,
   ``beam.py:175-176``).
 
-Beside the reference's surface, a cache of pages for serving, with grouped heads and an optional 8-bit form:
+Beside the reference's surface, a cache of pages for serving, with grouped heads and optional 8-bit and 4-bit forms:
 
 * :func:`paged_rope_kv` / :func:`paged_kv_read` -- RoPE and the append into pages, and pages read back as packed rows;
 * :func:`paged_attention` -- each sequence's newest token(s) over its pages;
-* :func:`packed_attention` -- causal attention of packed prompts (or chunks of them) of different lengths.
+* :func:`packed_attention` -- causal attention of packed prompts (or chunks of them) of different lengths;
+* :func:`paged_norm_rope_kv` -- the append with queries and keys normed per head;
+* :func:`paged_plan` / :func:`paged_trim` -- a step's tables, slots and offsets on the GPU, and pages given back;
+* :func:`decode_gemm_int4` (:func:`int4_weights`, :func:`int4_quantise`) -- the decode GEMMs over 4-bit weights.
 
 Each call is a launch (or two) of hand-written CUDA through the C ABI of ``include/omniasr_b200.h`` on the
 current stream; outputs and the beam search's split workspace are allocated with ``torch.empty`` on the caller's
