@@ -251,6 +251,11 @@ at::Tensor decode_gemm_int4(const at::Tensor& x, const at::Tensor& codes, const 
   if (residual) bf16_rows(*residual, "residual");
   if (out) bf16_rows(*out, "out");
   if (rows > 64) refuse(name, "at most 64 rows");
+  if (group != 32 && group != 64 && group != 128) refuse(name, "groups of 32, 64 or 128 columns");
+  const int64_t tiles = (wrows + 7) / 8;
+  if (wrows < 0 || codes.scalar_type() != at::kByte || !codes.is_contiguous() || codes.numel() != tiles * ((k + 127) / 128) * 512 ||
+      scales.scalar_type() != at::kBFloat16 || !scales.is_contiguous() || scales.numel() != tiles * ((k + group - 1) / group) * 8)
+    refuse(name, "codes and scales are not those of " + std::to_string(wrows) + " x " + std::to_string(k) + " weights (int4_weights)");
   at::Tensor y = out ? *out : at::empty({rows, n}, x.options());
   if (rows == 0 || n == 0) return y;
   same_device(name, x, {&codes, &scales, &y});

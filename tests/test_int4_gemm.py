@@ -6,6 +6,8 @@ count as up to 16 roundings of 2^-23), then k / 128 scaled blocks and 8 warps: (
 the bound used is 2^-14 S. The output's rounding is 2^-8 of the value. silu's exponential and division: 2^-20 of it, its slope is at
 most 1.1."""
 
+import dataclasses
+
 import pytest
 import torch
 
@@ -146,3 +148,16 @@ def test_gemm_values_that_are_not_finite():
     keep = [i for i in range(12) if i not in (3, 9)]
     cols = [i for i in range(40) if i != 21]
     check(y[keep][:, cols], want[cols], x[keep], None, "store")
+
+
+def test_weights_of_other_sizes_are_refused():
+    w = kernels.int4_weights(torch.zeros(16, 256, dtype=torch.uint8), torch.ones(16, 4, dtype=torch.bfloat16), 64)
+    x = torch.zeros(2, 256, dtype=torch.bfloat16)
+    for bad in (dict(n=17), dict(n=24), dict(n=8), dict(group=32), dict(codes=w.codes[:1]), dict(scales=w.scales[:1]),
+                dict(codes=w.codes.int()), dict(scales=w.scales.float()), dict(codes=w.codes.transpose(0, 1))):
+        with pytest.raises(ValueError, match="codes and scales"):
+            kernels.decode_gemm_int4(x, dataclasses.replace(w, **bad))
+    with pytest.raises(ValueError, match="groups"):
+        kernels.decode_gemm_int4(x, dataclasses.replace(w, group=0))
+    with pytest.raises(ValueError, match="codes and scales"):
+        kernels.decode_gemm_int4(torch.zeros(2, 512, dtype=torch.bfloat16), dataclasses.replace(w, k=512))
