@@ -236,6 +236,18 @@ py::object packed_attention(const at::Tensor& q, const at::Tensor& k, const at::
   return py::cast(out);
 }
 
+// Whether rows of a and of b (2-D, unit inner stride, one element size) share memory. Columns of one buffer's rows that lie side by side
+// do not.
+bool rows_overlap(const at::Tensor& a, const at::Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  const int64_t es = a.element_size(), la = stride_of(a, 0), lb = stride_of(b, 0);
+  const int64_t pa = reinterpret_cast<int64_t>(a.data_ptr()) / es, pb = reinterpret_cast<int64_t>(b.data_ptr()) / es;
+  if (pa + (a.size(0) - 1) * la + a.size(1) <= pb || pb + (b.size(0) - 1) * lb + b.size(1) <= pa) return false;
+  if (la != lb || la <= 0) return true;
+  const int64_t at = ((pb - pa) % la + la) % la;  // where b's rows begin in a's
+  return at < a.size(1) || at + b.size(1) > la;
+}
+
 at::Tensor decode_gemm_int4(const at::Tensor& x, const at::Tensor& codes, const at::Tensor& scales, int64_t wrows, int64_t k,
                             int64_t group, int64_t mode, const Opt& residual, const Opt& out, int64_t stream) {
   const char* name = "decode_gemm_int4";
@@ -250,6 +262,9 @@ at::Tensor decode_gemm_int4(const at::Tensor& x, const at::Tensor& codes, const 
   if ((mode == OMNIASR_GEMM_RESIDUAL) != residual.has_value()) refuse(name, "a residual belongs to the residual mode, and that to it");
   if (residual) bf16_rows(*residual, "residual");
   if (out) bf16_rows(*out, "out");
+  if (out && (rows_overlap(x, *out) || (residual && (residual->data_ptr() != out->data_ptr() ||
+                                                     stride_of(*residual, 0) != stride_of(*out, 0)) && rows_overlap(*residual, *out))))
+    refuse(name, "out must not share memory with x, nor with the residual unless it is the residual");
   if (rows > 64) refuse(name, "at most 64 rows");
   if (group != 32 && group != 64 && group != 128) refuse(name, "groups of 32, 64 or 128 columns");
   const int64_t tiles = (wrows + 7) / 8;

@@ -562,7 +562,7 @@ def decode_gemm_int4(x: torch.Tensor, w: Int4Weights, mode: str = "store", resid
                      out: torch.Tensor | None = None) -> torch.Tensor:
     """:func:`decode_gemm` over 4-bit weights, at most 64 token rows (bf16): ``x @ W.t()`` ("store"), ``residual + x @ W.t()``
     ("residual"), or with W's rows [gate; inner] ``inner * silu(gate)`` ("swiglu"); products and sums in fp32, rounded once, at the
-    end (swiglu's halves are not rounded before). ``w`` must not be written by the kernel launched just before on the stream."""
+    end (swiglu's halves are not rounded before). ``out`` may be the residual and shares memory with no input else. ``w`` must not be written by the kernel launched just before on the stream."""
     native, _, stream, _ = _context(x.device)
     code = GEMM_MODES.get(mode)
     if code is None:

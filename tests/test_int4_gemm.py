@@ -161,3 +161,31 @@ def test_weights_of_other_sizes_are_refused():
         kernels.decode_gemm_int4(x, dataclasses.replace(w, group=0))
     with pytest.raises(ValueError, match="codes and scales"):
         kernels.decode_gemm_int4(torch.zeros(2, 512, dtype=torch.bfloat16), dataclasses.replace(w, k=512))
+
+
+def test_out_over_an_input_is_refused():
+    w = kernels.int4_weights(torch.zeros(128, 128, dtype=torch.uint8), torch.ones(128, 1, dtype=torch.bfloat16))
+    buf = torch.zeros(4, 256, dtype=torch.bfloat16)
+    flat = torch.zeros(2048, dtype=torch.bfloat16)
+    x, y = buf[:, :128], buf[:, 128:]
+    for tokens, bad in ((x, x), (x, buf[:, 64:192]), (flat[128:640].view(4, 128), flat[:512].view(4, 128))):
+        with pytest.raises(ValueError, match="share memory"):
+            kernels.decode_gemm_int4(tokens, w, out=bad)
+    with pytest.raises(ValueError, match="share memory"):
+        kernels.decode_gemm_int4(x, w, "residual", residual=flat[128:640].view(4, 128), out=flat[:512].view(4, 128))
+    for mode, res in (("store", None), ("residual", y)):  # side by side, and the residual itself: the CPU is what is refused
+        with pytest.raises(ValueError, match="CUDA"):
+            kernels.decode_gemm_int4(x, w, mode, residual=res, out=y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 5, 64])
+def test_residual_in_place_and_out_beside_x(rows):
+    gen = torch.Generator().manual_seed(rows)
+    w = kernels.int4_quantise(torch.randn(128, 128, generator=gen).to(DEV), 32)
+    buf = torch.randn(rows, 256, generator=gen).bfloat16().to(DEV)
+    x, y = buf[:, :128], buf[:, 128:]
+    want = kernels.decode_gemm_int4(x.clone(), w, "residual", residual=y.clone())
+    before = x.clone()
+    got = kernels.decode_gemm_int4(x, w, "residual", residual=y, out=y)
+    assert got.data_ptr() == y.data_ptr() and torch.equal(got, want) and torch.equal(x, before)
