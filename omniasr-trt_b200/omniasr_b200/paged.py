@@ -23,7 +23,7 @@ class Batch:
 
     tokens: int  # new tokens in all
     new: list[int] | None  # new tokens per sequence (None: the GPU alone knows)
-    total: int  # keys in all, the new tokens' among them
+    total: int | None  # keys in all, the new tokens' among them (None: the GPU alone knows)
     pos: torch.Tensor  # [tokens] position of each new token
     slots: torch.Tensor  # [tokens] page number * page + offset
     table: torch.Tensor  # [sequences, width] int32
@@ -141,6 +141,8 @@ class PagedCache:
                 norms: tuple[torch.Tensor, torch.Tensor, float] | None = None) -> torch.Tensor:
         """One layer's causal attention of a batch of prompts, or of chunks whose earlier keys the cache holds: writes the new
         keys and reads all of them back as packed rows (what a later step sees, an 8-bit or 4-bit cache's rounding included)."""
+        if batch.total is None:
+            raise ValueError("prefill: a batch of tables on the GPU needs its number of keys (DeviceTables.plan's total)")
         q = self.write(layer, qkv, cs, batch, heads, norms)
         k, v, (ks, vs) = self._layer(layer)
         kk, vv = kernels.paged_kv_read(k, v, batch.table, batch.k_offsets, batch.total, k_scale=ks, v_scale=vs, dtype=self.dtype)
@@ -188,7 +190,7 @@ class DeviceTables:
         if tokens is None:
             raise ValueError("plan: new tokens per request on the GPU need their number (tokens)")
         pos, slots, table, lengths, q_offsets, k_offsets, taken = kernels.paged_plan(rows, new, tokens, self.page, *self._state(), width=width)
-        return Batch(tokens, None if each is None else [each] * b, 0 if total is None else total, pos, slots, table, lengths, q_offsets,
+        return Batch(tokens, None if each is None else [each] * b, total, pos, slots, table, lengths, q_offsets,
                      k_offsets, False, taken)
 
     def trim(self, rows: torch.Tensor, keep: torch.Tensor) -> None:

@@ -10,7 +10,7 @@ import torch
 import int4_util as iu
 from conftest import ROOT
 from omniasr_b200 import kernels
-from omniasr_b200.paged import DeviceTables, PagedCache
+from omniasr_b200.paged import Batch, DeviceTables, PagedCache
 
 DEV = "cuda"
 
@@ -130,3 +130,11 @@ def test_two_streams_at_once():
         assert torch.equal(a.slots, b.slots) and torch.equal(a.table, b.table) and bool(a.taken.all())
     assert tables[0].length.tolist() == [140] * 3
     assert kernels.read_status() == 0
+
+
+def test_prefill_needs_the_number_of_keys():
+    cache = PagedCache(1, 4, 8, 1, 32, kind=torch.uint8, device="cpu")
+    none = torch.zeros(0)
+    batch = Batch(2, [2], None, none, none, none, none, none, none, False, none)
+    with pytest.raises(ValueError, match="total"):
+        cache.prefill(0, none, none, batch, 1)
