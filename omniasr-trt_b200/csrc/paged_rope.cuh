@@ -135,7 +135,8 @@ __global__ void __launch_bounds__(kRopeThreads, D * sizeof(T) > 512 ? 2 : KIND =
           Elem<T>::unpack(u[j][v], x);
           if constexpr (NORM) {
             float w[kVec];
-            Elem<T>::unpack(__ldg(reinterpret_cast<const uint4*>(it < a.heads ? a.q_norm : a.k_norm) + v * L + lane), w);
+            // (Ordinary loads, as the vectors': the weights may come from the kernel before.)
+            Elem<T>::unpack(reinterpret_cast<const uint4*>(it < a.heads ? a.q_norm : a.k_norm)[v * L + lane], w);
 #pragma unroll
             for (int i = 0; i < kVec; ++i) x[i] = x[i] * inv_rms * w[i];
           }

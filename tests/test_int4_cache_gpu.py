@@ -312,3 +312,34 @@ def test_refusals():
         with pytest.raises(ValueError, match="eps"):
             kernels.paged_norm_rope_kv(qkv, z(64), z(64), cs, pos, k, k.clone(), pos, 4, 2, eps=eps, k_scale=s, v_scale=s.clone())
     assert kernels.read_status() == 0
+
+
+def test_norm_weights_of_the_kernel_before():
+    heads, kv, dim, n = 4, 2, 128, 40
+    g, pages, x, pos, slots, cs = append_inputs(n, heads, kv, dim, 16, "bf16", 5)
+    w = kernels.int4_quantise(torch.randn(dim, 64, generator=g).to(DEV), 32)
+    qkv, pos, slots, cs = dev(x.reshape(n, -1)), dev(pos), dev(slots), dev(cs)
+    rows = torch.zeros(2, 64, dtype=torch.bfloat16, device=DEV)
+    k, v = (torch.zeros(pages, kv, 16, dim, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+
+    def step():
+        norms = kernels.decode_gemm_int4(rows, w)
+        return kernels.paged_norm_rope_kv(qkv, norms[0], norms[1], cs, pos, k, v, slots, heads, kv)
+
+    step()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        q = step()
+    for i in range(20):
+        rows.copy_(torch.randn(2, 64, generator=g))
+        graph.replay()
+        norms = kernels.decode_gemm_int4(rows, w)
+        torch.cuda.synchronize()
+        got, gk = q.clone(), k.clone()
+        want = kernels.paged_norm_rope_kv(qkv, norms[0], norms[1], cs, pos, k, v, slots, heads, kv)
+        assert torch.equal(got, want) and torch.equal(gk, k), i
