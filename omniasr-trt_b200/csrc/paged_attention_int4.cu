@@ -11,13 +11,16 @@
 //   (int4.cuh) makes a lane's share of a vector one run of 16 bytes (K) or 8 (V).
 // * S^T = K Q^T in fp16, 16 keys x 8 columns a step: a code masked out of its word is, read as fp16, the subnormal c 2^-24 (16 c 2^-24
 //   four bits up), exact, so a word of 8 codes takes four ands and a shift. The queries, scaled by a power of two per column
-//   (largest value 2^14 and more; exact but for values 2^-28 of it), carry the factors. The sums start from -8 sum q, which is the
+//   (largest value 2^14 and more; exact but for values under 2^-27 of it), carry the factors. The sums start from -8 sum q, which is the
 //   codes' offset, and every group's sum is scaled in fp32.
 // * O^T = V^T P^T in fp16: two keys' codes of a dim are the halves of a word after one byte permutation, and a code masked out of it
 //   is the subnormal c 2^-24 (16 c 2^-24 four bits up), exact; the offset is a second product, with constants. The scales go onto
-//   the probabilities in fp32, before these are rounded, once, to fp16 (2^-12) and turned by movmatrix. What keeps them in
-//   fp16's range is the number that is taken off the scores: a column's weights 2^(x - m) may grow until weight x scale is 2^12,
-//   then m is raised so that the largest is about 2^4. Sums of weights and accumulators share m, so nothing else sees it.
+//   the probabilities in fp32, before these are rounded, once, to fp16 and turned by movmatrix. Two things keep them in fp16's range.
+//   A column's weights 2^(x - m) may grow to 2^13, then m is raised so that the largest is 2^8. And every group of 32 dims has a unit, a
+//   power of two that a warp's accumulators of the group count in, which the scales of a block lie between 2^-7 and 2^2 of; a block
+//   whose scales do not moves the unit (and the accumulators with it), and one with scales too far apart for any unit is summed in
+//   fp32 on the CUDA cores. So a weight is rounded by 2^-11 of itself or, if that is more, by 2^-26 of the row's largest (half of fp16's
+//   smallest step, 2^-25, is 2^-33 of the largest weight in units of at most 2^7 times the key's own scale), whatever the scales are.
 // * Warps are independent: each takes blocks of 16 or 32 keys of the CTA's share with a maximum, a sum and an accumulator of
 //   its own, and copies its next blocks asynchronously into a ring of its own; no barrier in the loop. At a unit's end the CTA's
 //   warps join through shared memory.
@@ -46,8 +49,11 @@ namespace paged4 {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr float kMost = 12.f, kGoal = 4.f;  // log2 of a weight times a scale: the most, and the largest when m is raised
-constexpr float kLeast = -60.f;             // the smallest exponent of a scale that is looked at (weights stay inside fp32)
+constexpr float kMost = 13.f, kGoal = 8.f;  // log2 of a weight: the most, and the largest when m is raised
+// Units: a block's scales have exponents from unit - kBelow to unit + kAbove, so that a product stays under 2^(kMost + kAbove + 1) = 2^15.
+// Units stay from kUnitLeast to kUnitMost (2^-unit and what the join multiplies by are fp32 numbers), and at most kFall below the highest
+// that the warp's unit had (an accumulator, under 2^50 with 2^31 keys, is scaled up by no more).
+constexpr int kAbove = 1, kBelow = 7, kUnitLeast = -100, kUnitMost = 110, kFall = 64;
 constexpr float kNone = -3e38f;  // a maximum before any score: below what a score can be, and a number, so that nothing needs a case for it
 // A unit's start and end (queries, the join of the warps), about 3 us of a CTA, counted as so many blocks in the shares.
 constexpr int kStart = 8;
@@ -139,8 +145,18 @@ OMNI_DEV uint32_t half2_of(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// A bf16 magnitude's exponent, of infinities and NaN that of 0.
-OMNI_DEV float exponent_of(uint32_t bits) { return bits < 0x7f80u ? fmaxf((float)((int)(bits >> 7) - 127), kLeast) : kLeast; }
+OMNI_DEV uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// Whether one of two scales (bf16, relative to their units) is not 0 and outside [2^-kBelow, 2^(kAbove + 1)); of a NaN no.
+OMNI_DEV bool outside(uint32_t scales) {
+  const uint32_t x = scales & 0x7fff7fffu;
+  constexpr uint32_t lo = (127u - kBelow) << 7, hi = (127u + kAbove + 1) << 7;
+  auto pair = [](uint32_t u) { return *reinterpret_cast<const __nv_bfloat162*>(&u); };
+  return (__hge2_mask(pair(x), pair(hi | hi << 16)) | (__hlt2_mask(pair(x), pair(lo | lo << 16)) & __hgt2_mask(pair(x), pair(0u)))) != 0u;
+}
 
 // Where the 16-byte word c of key r's codes lies in a tile: so that a quarter warp's reads (K: 16 bytes of 2 keys x 4 lanes; V, 8
 // bytes: 4 keys x 4 lanes) meet all banks. Keys of V lie in the order of its operand, so that a lane's four are 4 apart.
@@ -219,8 +235,9 @@ struct Kernel {
 
   float o[C::kBlocks * C::kGroups][2][NT][4];
   float m[NT][2], l[NT][2], qs[NT][2];  // what is taken off the scores, sums of weights, the scores' factors
-  float es[NT][2];                      // the largest exponent of a scale of V that the column has seen
-  uint32_t run;                         // the largest scale of V (bf16 bits) of blocks that all columns see
+  static constexpr int kWordsS = DIM / 64;  // 32-bit words of a vector's scales
+  uint32_t down[kWordsS];                   // 2^-unit of each group (bf16, as the scales lie)
+  int highest;                              // of the units so far
 
   OMNI_DEV Kernel(const Params& q, char* s) : p(q), smem(s) {
     lane = threadIdx.x & 31;
@@ -416,14 +433,15 @@ struct Kernel {
   }
 
   OMNI_DEV void start_unit() {
-    run = 0u;
+    highest = 0;
+#pragma unroll
+    for (int i = 0; i < kWordsS; ++i) down[i] = 0x3f803f80u;  // (2^0: values of 2^-4 to 2^5, or whatever set_units() makes it)
     const float* factor = reinterpret_cast<const float*>(smem + C::kLim);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         m[n][i] = kNone;
-        es[n][i] = kLeast;
         l[n][i] = 0.f;
         qs[n][i] = factor[n * 8 + 2 * t + i];
       }
@@ -437,7 +455,125 @@ struct Kernel {
           for (int i = 0; i < 4; ++i) o[b][j][n][i] = 0.f;
   }
 
-  // ---- one block. TAIL: some column does not see all of it.
+  // ---- the groups' units, and blocks that have none
+
+  static constexpr int kLook = C::kKeys * C::kScale / 128;  // words of a block's scales per lane: a key's, half a key's from 256 dims on
+
+  // Whether a block's scales (a lane's words of them) lie within reach of the units.
+  OMNI_DEV bool in_units(const uint32_t (&w)[kLook]) const {
+    bool off = false;
+#pragma unroll
+    for (int i = 0; i < kLook; ++i) off |= outside(mul_bf16x2(w[i], DIM >= 256 && (lane & 1) ? down[(kWordsS - kLook) + i] : down[i]));
+    return !__any_sync(0xffffffffu, off);
+  }
+  OMNI_DEV bool in_units(int stage) const {
+    uint32_t w[kLook];
+    load_words<kLook>(w, ring + stage * C::kStage + 2 * C::kKeys * C::kRow + C::kKeys * C::kScale + lane * kLook * 4);
+    return in_units(w);
+  }
+
+  // Units that a block with the scales w (a lane's words of them) can be counted in, the nearest to those so far; the accumulators go
+  // along. True: there are none, some group's scales are too far apart.
+  OMNI_DEV bool set_units(const uint32_t (&w)[kLook]) {
+    uint32_t top[kLook], least[kLook];  // bits of the largest and of the least number that is not 0; halves are groups
+#pragma unroll
+    for (int i = 0; i < kLook; ++i) {
+      top[i] = 0u;
+      least[i] = 0u;
+#pragma unroll
+      for (int sh = 0; sh < 32; sh += 16) {
+        const uint32_t x = (w[i] >> sh) & 0x7fffu;
+        const bool number = x != 0u && x < 0x7f80u;
+        top[i] |= (number ? x : 0u) << sh;
+        least[i] |= (number ? x : 0x7f80u) << sh;
+      }
+#pragma unroll
+      for (int o = DIM >= 256 ? 2 : 1; o < 32; o <<= 1) {
+        top[i] = __vmaxu2(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+        least[i] = __vminu2(least[i], __shfl_xor_sync(0xffffffffu, least[i], o));
+      }
+    }
+    bool wild = false;
+    int up = highest;
+#pragma unroll
+    for (int j = 0; j < kWordsS; ++j) {
+      const uint32_t tw = __shfl_sync(0xffffffffu, top[j % kLook], j / kLook), lw = __shfl_sync(0xffffffffu, least[j % kLook], j / kLook);
+      uint32_t next = 0u;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int t = (int)((tw >> (16 * half)) & 0xffffu) >> 7, s = (int)((lw >> (16 * half)) & 0xffffu) >> 7;  // exponents + 127
+        const int now = 127 - (int)(((down[j] >> (16 * half)) & 0xffffu) >> 7);
+        int unit = now;
+        if (t != 0) {  // (else no scale but zeros and numbers too small for one)
+          const int lo = t - 127 - kAbove, hi = s - 127 + kBelow;  // units that the block can be counted in
+          if (unit < lo) unit = max(lo, min(lo + 1, hi));  // (with room for scales twice as large)
+          else if (unit > hi && hi >= lo) unit = hi;
+          unit = min(max(max(unit, highest - kFall), kUnitLeast), kUnitMost);
+          wild |= unit < lo || unit > hi;
+          up = max(up, unit);
+        } else if ((tw >> (16 * half)) & 0xffffu) {
+          wild = true;
+        }
+        next |= (uint32_t)(127 - unit) << (7 + 16 * half);
+        const float f = ex2((float)(now - unit));
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[2 * j + half][i][n][c] *= f;
+      }
+      down[j] = next;
+    }
+    highest = up;
+    return wild;
+  }
+
+  // What the 16 keys from `key` of a block on add, in fp32: e[n][2 h + i] is the weight of key g + 8 h for column 2 t + i of tile n.
+  OMNI_DEV void add_values(const float (&e)[NT][4], int key, int j0, uint32_t vd, uint32_t vsd) {
+    const int* lims = reinterpret_cast<const int*>(smem + C::kLim) + C::kCols;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll 1
+      for (int r = 0; r < 8; ++r) {
+        const int at = key + 8 * h + r, slot = v_slot(8 * h + r);
+        float p[NT][2];
+        bool hidden[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            p[n][i] = __shfl_sync(0xffffffffu, e[n][2 * h + i], r * 4 + t);
+            hidden[n][i] = j0 + at >= lims[n * 8 + 2 * t + i];
+          }
+#pragma unroll
+        for (int b = 0; b < C::kBlocks; ++b) {
+          uint32_t vw[W2], vs[W2];  // dims 4 g .. of each group, and the groups' scales
+          load_words<W2>(vw, vd + key * C::kRow + (DIM == 64 ? slot * C::kRow + g * 4 : v_place<DIM>(slot, b * 4 + (g >> 1)) * 16 + (g & 1) * 8));
+          load_words<W2>(vs, vsd + at * C::kScale + b * 8);
+#pragma unroll
+          for (int gr = 0; gr < C::kGroups; ++gr) {
+            const int sh = 16 * (gr & 1);
+            const float s = bf16_value((vs[gr >> 1] >> sh) & 0xffffu) * bf16_value((down[b * W2 + (gr >> 1)] >> sh) & 0xffffu);
+            float c[4];
+            int4_values(vw[gr >> 1] >> sh, 1.f, c);
+            float(&x)[2][NT][4] = o[b * C::kGroups + gr];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const float y = hidden[n][i] ? 0.f : p[n][i] * s;
+                x[0][n][i] = fmaf(y, c[0] * 0x1p-24f, x[0][n][i]);
+                x[0][n][i + 2] = fmaf(y, c[1] * 0x1p-20f, x[0][n][i + 2]);
+                x[1][n][i] = fmaf(y, c[2] * 0x1p-24f, x[1][n][i]);
+                x[1][n][i + 2] = fmaf(y, c[3] * 0x1p-20f, x[1][n][i + 2]);
+              }
+          }
+        }
+      }
+  }
+
+  // ---- one block. TAIL: some column does not see all of it, or its scales do not fit the units.
 
   template <bool TAIL>
   OMNI_DEV void block(int stage, int j0) {
@@ -498,47 +634,11 @@ struct Kernel {
     auto masked = [&](int k, int n, int i) {
       return TAIL && j0 + k * 16 + g + (i & 2) * 4 >= lims[n * 8 + 2 * t + (i & 1)];
     };
-    // How large V's scales are: of a block that every column sees one number for all of them, else of each column's own keys.
-    if constexpr (!TAIL) {
-      constexpr int SW = C::kKeys * C::kScale / 128;  // words of scales per lane
-      uint32_t w[SW], top = 0u;
-      load_words<SW>(w, vsd + lane * SW * 4);
-#pragma unroll
-      for (int i = 0; i < SW; ++i) top = max_abs_bf16x2(top, w[i]);
-      top = max(top & 0xffffu, top >> 16);
-      if (__any_sync(0xffffffffu, top > run)) {
-        run = __reduce_max_sync(0xffffffffu, top < 0x7f80u ? top : 0u);
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) es[n][i] = fmaxf(es[n][i], exponent_of(run));
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < C::kMt; ++k)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          uint32_t top = 0u;
-#pragma unroll
-          for (int b = 0; b < C::kBlocks; ++b) {
-            uint32_t w[W2];
-            load_words<W2>(w, vsd + (k * 16 + 8 * e + g) * C::kScale + b * 8);
-#pragma unroll
-            for (int i = 0; i < W2; ++i) top = max_abs_bf16x2(top, w[i]);
-          }
-          const float x = fmaxf(exponent_of(top & 0xffffu), exponent_of(top >> 16));
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-              if (!masked(k, n, 2 * e + i)) es[n][i] = fmaxf(es[n][i], x);
-        }
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int w = 4; w < 32; w <<= 1) es[n][i] = fmaxf(es[n][i], __shfl_xor_sync(0xffffffffu, es[n][i], w));
+    bool wild = false;
+    if constexpr (TAIL) {
+      uint32_t w[kLook];
+      load_words<kLook>(w, vsd + lane * kLook * 4);
+      if (!in_units(w)) wild = set_units(w);
     }
     // Scores less m, masked.
     bool raise = false;
@@ -550,7 +650,7 @@ struct Kernel {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           d[k][n][i] = masked(k, n, i) ? -INFINITY : fmaf(s[k][n][i], qs[n][i & 1], -m[n][i & 1]);
-          raise |= d[k][n][i] > kMost - es[n][i & 1];
+          raise |= d[k][n][i] > kMost;
         }
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
@@ -565,7 +665,7 @@ struct Kernel {
               if (!masked(k, n, e)) top = fmaxf(top, s[k][n][e] * qs[n][i]);
 #pragma unroll
           for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-          top = fmaxf(m[n][i], top + es[n][i] - kGoal);
+          top = fmaxf(m[n][i], top - kGoal);
           const float f = ex2(m[n][i] - top);
           m[n][i] = top;
 #pragma unroll
@@ -593,13 +693,21 @@ struct Kernel {
           e[n][i] = ex2(d[k][n][i]);
           l[n][i & 1] += e[n][i];
         }
+      if (TAIL && wild) {
+        add_values(e, k * 16, j0, vd, vsd);
+        continue;
+      }
 #pragma unroll
       for (int b = 0; b < C::kBlocks; ++b) {
         uint32_t vw[4][W2], vs[2][W2];  // codes of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9 (slots t, t + 4, ...); scales of keys g, g + 8
 #pragma unroll
         for (int i = 0; i < 4; ++i) load_words<W2>(vw[i], vd + k * 16 * C::kRow + 4 * i * C::kRow + (v_lane ^ (b * 64)));
 #pragma unroll
-        for (int i = 0; i < 2; ++i) load_words<W2>(vs[i], vsd + g * C::kScale + (k * 16 + 8 * i) * C::kScale + b * 8);
+        for (int i = 0; i < 2; ++i) {
+          load_words<W2>(vs[i], vsd + g * C::kScale + (k * 16 + 8 * i) * C::kScale + b * 8);
+#pragma unroll
+          for (int j = 0; j < W2; ++j) vs[i][j] = mul_bf16x2(vs[i][j], down[b * W2 + j]);  // (exact)
+        }
 #pragma unroll
         for (int gr = 0; gr < C::kGroups; ++gr) {
           const uint32_t sel = (gr & 1) ? 0x7632u : 0x5410u;
@@ -661,6 +769,7 @@ struct Kernel {
         s[k] = ml[k * C::kCols + col];
         top = fmaxf(top, s[k].x);
       }
+      top += kMost;  // (weights of at most 1, so that values up to the type's largest do not pass fp32's)
 #pragma unroll
       for (int k = 0; k < kWarps; ++k) {
         s[k].x = ex2(s[k].x - top);
@@ -674,18 +783,23 @@ struct Kernel {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       if (c0 + n * 8 >= p.cols) break;
-      const float f[2] = {ml[warp * C::kCols + n * 8 + 2 * t].x, ml[warp * C::kCols + n * 8 + 2 * t + 1].x};
+      constexpr float kHigh = 0x1p-13f;  // 2^-kMost; more only in a column whose scores are all -inf, where a unit's 2^110 would make it infinite
+      const float f[2] = {fminf(ml[warp * C::kCols + n * 8 + 2 * t].x, kHigh), fminf(ml[warp * C::kCols + n * 8 + 2 * t + 1].x, kHigh)};
       const float low[2] = {f[0] * 0x1p24f, f[1] * 0x1p24f}, high[2] = {f[0] * 0x1p20f, f[1] * 0x1p20f};  // (by the dim's nibble)
 #pragma unroll
       for (int b = 0; b < C::kBlocks; ++b) {
 #pragma unroll
-        for (int gr = 0; gr < C::kGroups; ++gr)
+        for (int gr = 0; gr < C::kGroups; ++gr) {
+          const uint32_t exp = ((down[b * W2 + (gr >> 1)] >> (16 * (gr & 1))) & 0xffffu) >> 7;  // 127 - unit
+          const float unit = __uint_as_float((254u - exp) << 23);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const float(&x)[2][NT][4] = o[b * C::kGroups + gr];
+            const float lo = low[i] * unit, hi = high[i] * unit;
             *reinterpret_cast<float4*>(join + (warp * 8 + 2 * t + i) * C::kPitch + gr * 32 + g * 4) =
-                make_float4(x[0][n][i] * low[i], x[0][n][i + 2] * high[i], x[1][n][i] * low[i], x[1][n][i + 2] * high[i]);
+                make_float4(x[0][n][i] * lo, x[0][n][i + 2] * hi, x[1][n][i] * lo, x[1][n][i + 2] * hi);
           }
+        }
         __syncthreads();
         constexpr int Q4 = C::kGroups * 8;  // float4 of a column
 #pragma unroll
@@ -874,7 +988,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<DIM, NT>::kCtas) int4_kernel(con
       copy_wait<C::kStages - 1>();
       __syncwarp();
       const int j0 = n * C::kKeys;
-      if (j0 + C::kKeys <= use.len) k.template block<false>(take, j0);
+      if (j0 + C::kKeys <= use.len && k.in_units(take)) k.template block<false>(take, j0);
       else k.template block<true>(take, j0);
       __syncwarp();
       take = take + 1 == C::kStages ? 0 : take + 1;
