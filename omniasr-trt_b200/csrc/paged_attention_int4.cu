@@ -85,7 +85,7 @@ struct Params {
   PagedAttnArgs a;
   int cols, chunks;  // columns of a (row, kv head); units per (row, kv head)
   int grid;
-  int page_shift;        // pages of 2^page_shift positions, 16 and more, one behind another in a head's part; else -1
+  int page_shift;        // pages of 2^page_shift positions, 16 and more, one behind another in a head's part of under 2^31 bytes; else -1
   uint32_t page_scales;  // bytes of a page's scales
   unsigned* counters;  // [grid], zero on entry and left zero
   float* part_o;       // [2 grid][cols of a unit][dim]
@@ -1051,7 +1051,9 @@ cudaError_t launch(const PagedAttnArgs& a, cudaStream_t s) {
   p.grid = grid_of<DIM, NT>();
   p.page_shift = -1;
   const int64_t scales = (int64_t)a.c.kv_heads * a.c.page * C::kScale;
-  if (a.c.page >= 16 && (a.c.page & (a.c.page - 1)) == 0 && a.c.s_pos == C::kRow && a.c.s_page < 0x7fffffff && scales < 0x7fffffff)
+  const int64_t codes = (int64_t)a.c.page * C::kRow;  // (one page alone has no stride that would bound it)
+  if (a.c.page >= 16 && (a.c.page & (a.c.page - 1)) == 0 && a.c.s_pos == C::kRow && a.c.s_page < 0x7fffffff && codes < 0x7fffffff &&
+      scales < 0x7fffffff)
     p.page_shift = __builtin_ctz(a.c.page);
   p.page_scales = (uint32_t)scales;
   p.counters = reinterpret_cast<unsigned*>(a.workspace);
