@@ -213,6 +213,9 @@ inline cudaError_t launch_dependent(Kern kern, dim3 grid, dim3 block, size_t sme
   return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
+// What earlier kernels write is read by ordinary loads. One through the read-only path (__ldg) promises memory that nobody writes while
+// the kernel lives, but this kernel lives while they still write; the compiler may also move it ahead of the wait. (Weights
+// that the wait is not for may be loaded either way.)
 OMNI_DEV void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 OMNI_DEV void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

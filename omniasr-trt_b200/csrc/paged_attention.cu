@@ -26,8 +26,7 @@ namespace paged {
 
 constexpr int kThreads = 128;
 
-// Eight consecutive elements of a cache row (or a query) as floats. Ordinary loads: one through the read-only path may be moved ahead
-// of the wait for the kernel that writes the queries.
+// Eight consecutive elements of a cache row (or a query) as floats. Ordinary loads (grid_dependency_wait() in common.cuh says why).
 template <typename T>
 struct Row8;
 
@@ -51,7 +50,7 @@ struct Row8<float> {
 template <>
 struct Row8<__nv_fp8_e4m3> {
   uint2 u;
-  OMNI_DEV void load(const void* base, int64_t at) { u = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(base) + at)); }
+  OMNI_DEV void load(const void* base, int64_t at) { u = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(base) + at); }
   OMNI_DEV void get(float* f) const {
     const uint32_t w[2] = {u.x, u.y};
 #pragma unroll
@@ -77,7 +76,7 @@ struct CacheRow8<Int4, D, KEYS> {
   uint32_t u;
   OMNI_DEV void load(const void* base, int64_t row, int w) {
     const uint16_t* q = reinterpret_cast<const uint16_t*>(reinterpret_cast<const uint8_t*>(base) + row);
-    u = (uint32_t)__ldg(q + quad_at<D, KEYS>(2 * w)) | (uint32_t)__ldg(q + quad_at<D, KEYS>(2 * w + 1)) << 16;
+    u = (uint32_t)q[quad_at<D, KEYS>(2 * w)] | (uint32_t)q[quad_at<D, KEYS>(2 * w + 1)] << 16;
   }
   OMNI_DEV void get(float* f) const {
     int4_values(u, 1.f, f);
@@ -197,8 +196,8 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const PagedAttnArgs a, 
         kr[v].get(kf);
         if constexpr (INT4) {
           const int64_t g = si * (D / 32) + (v * L + lane) / 4;
-          kg[v] = bf16_value(__ldg(reinterpret_cast<const uint16_t*>(a.c.k_scale) + g));
-          vg[v] = bf16_value(__ldg(reinterpret_cast<const uint16_t*>(a.c.v_scale) + g));
+          kg[v] = bf16_value(reinterpret_cast<const uint16_t*>(a.c.k_scale)[g]);
+          vg[v] = bf16_value(reinterpret_cast<const uint16_t*>(a.c.v_scale)[g]);
 #pragma unroll
           for (int i = 0; i < 8; ++i) kf[i] *= kg[v];
         }

@@ -310,7 +310,7 @@ __device__ __noinline__ BadValues bad_page_values(const PageCache& c, const int3
     uint32_t any = FP8 && c.v_scale[(id * c.kv_heads + h) * c.page + off] == 255 ? 1u : 0u;
 #pragma unroll 8
     for (int i = 0; i < DIM * (FP8 ? 1 : 2) / 16; ++i) {
-      const uint4 u = __ldg(row + i);
+      const uint4 u = row[i];
       const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {  // a code that is NaN; a half whose exponent bits are all ones
@@ -578,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       x.live = small ? min(boxes, (left + rows_box - 1) >> p.page_shift) : 1;
       x.row = small ? 0 : (t * BN) % p.c.page;
       const int pi = small ? ((t * BN) >> p.page_shift) + lane : (t * BN) / p.c.page;
-      x.id = lane < x.live ? __ldg(p.table + (int64_t)s.b * p.table_stride + pi) : 0;
+      x.id = lane < x.live ? p.table[(int64_t)s.b * p.table_stride + pi] : 0;
     };
     auto step = [&]() {  // to the next tile; false past the last
       if (++ntile >= tiles) return false;
@@ -989,7 +989,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           int tt;
           const uint2* src = reinterpret_cast<const uint2*>(p.q + query_row(p, sq.b, sq.h, sq.col0 + j, &tt) * DIM) + lane;
 #pragma unroll
-          for (int c = 0; c < DC; ++c) qr[k][c] = CD == 128 || lane < 16 ? __ldg(src + c * 32) : make_uint2(0u, 0u);
+          for (int c = 0; c < DC; ++c) qr[k][c] = CD == 128 || lane < 16 ? src[c * 32] : make_uint2(0u, 0u);
         }
       }
     };

@@ -95,15 +95,15 @@ __global__ void __launch_bounds__(kReadThreads) paged_read_kernel(const PagedRea
           vu[r] |= (uint32_t)__ldcs(vr + quad_at<D, false>(c * (kOut / 4) + q)) << (16 * q);
         }
         const int64_t g = si * (D / 32) + c * kOut / 32;
-        ks[r] = bf16_value(__ldg(reinterpret_cast<const uint16_t*>(a.c.k_scale) + g));
-        vs[r] = bf16_value(__ldg(reinterpret_cast<const uint16_t*>(a.c.v_scale) + g));
+        ks[r] = bf16_value(reinterpret_cast<const uint16_t*>(a.c.k_scale)[g]);
+        vs[r] = bf16_value(reinterpret_cast<const uint16_t*>(a.c.v_scale)[g]);
       } else {
         ku[r] = __ldcs(reinterpret_cast<const In*>(reinterpret_cast<const char*>(a.c.k) + at * es));
         vu[r] = __ldcs(reinterpret_cast<const In*>(reinterpret_cast<const char*>(a.c.v) + at * es));
       }
       if constexpr (KIND == kFp8) {
-        ks[r] = __uint_as_float((uint32_t)__ldg(a.c.k_scale + si) << 23);
-        vs[r] = __uint_as_float((uint32_t)__ldg(a.c.v_scale + si) << 23);
+        ks[r] = __uint_as_float((uint32_t)a.c.k_scale[si] << 23);
+        vs[r] = __uint_as_float((uint32_t)a.c.v_scale[si] << 23);
       }
     }
   }

@@ -76,7 +76,6 @@ __global__ void __launch_bounds__(kRopeThreads, D * sizeof(T) > 512 ? 2 : KIND =
       const int it = base + j * TEAMS + team;
 #pragma unroll
       for (int v = 0; v < NV; ++v)
-        // (An ordinary load: one through the read-only path may be moved ahead of the wait for the kernel before.)
         u[j][v] = it < i1 ? reinterpret_cast<const uint4*>(src + (int64_t)it * D)[v * L + lane]
                           : make_uint4(0u, 0u, 0u, 0u);
     }
@@ -95,7 +94,7 @@ __global__ void __launch_bounds__(kRopeThreads, D * sizeof(T) > 512 ? 2 : KIND =
   for (int v = 0; v < NV; ++v)
 #pragma unroll
     for (int i = 0; i < kVec / 4; ++i) {
-      const float4 f = pos_ok ? __ldg(reinterpret_cast<const float4*>(a.cs + p * D + (v * L + lane) * kVec) + i)
+      const float4 f = pos_ok ? reinterpret_cast<const float4*>(a.cs + p * D + (v * L + lane) * kVec)[i]
                               : make_float4(0.f, 0.f, 0.f, 0.f);
       cs[v][4 * i] = f.x;
       cs[v][4 * i + 1] = f.y;
@@ -135,7 +134,6 @@ __global__ void __launch_bounds__(kRopeThreads, D * sizeof(T) > 512 ? 2 : KIND =
           Elem<T>::unpack(u[j][v], x);
           if constexpr (NORM) {
             float w[kVec];
-            // (Ordinary loads, as the vectors': the weights may come from the kernel before.)
             Elem<T>::unpack(reinterpret_cast<const uint4*>(it < a.heads ? a.q_norm : a.k_norm)[v * L + lane], w);
 #pragma unroll
             for (int i = 0; i < kVec; ++i) x[i] = x[i] * inv_rms * w[i];

@@ -396,7 +396,7 @@ __device__ __noinline__ BadValues bad_values(const __nv_bfloat16* v, int64_t v_s
     uint32_t any = 0u;
 #pragma unroll 8
     for (int i = 0; i < ND / 8; ++i) {
-      const uint4 u = __ldg(row + i);
+      const uint4 u = row[i];
       const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
       for (int c = 0; c < 4; ++c) {  // a half whose exponent bits are all ones

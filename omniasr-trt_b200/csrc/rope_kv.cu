@@ -39,7 +39,7 @@ __global__ void __launch_bounds__(256) rope_kv_kernel(const RopeArgs a) {
   for (int w = threadIdx.x; w < nvec; w += blockDim.x) {
     const int h = w / kPerHead;
     const int c = w - h * kPerHead;
-    const uint4 u = *reinterpret_cast<const uint4*>(src + (int64_t)w * kVec);  // (an ordinary load: see token_words in wgemm4.cu)
+    const uint4 u = *reinterpret_cast<const uint4*>(src + (int64_t)w * kVec);  // (an ordinary load: see grid_dependency_wait())
     const int64_t cache_off = row * a.s_kb + (int64_t)h * a.s_kh + cp * a.s_ks + c * kVec;
     if (part == 2) {
       if (dst_ok) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.v_cache) + cache_off) = u;
@@ -52,7 +52,7 @@ __global__ void __launch_bounds__(256) rope_kv_kernel(const RopeArgs a) {
       const float4* cr = reinterpret_cast<const float4*>(a.cs + p * D + c * kVec);
 #pragma unroll
       for (int i = 0; i < kVec / 4; ++i) {
-        const float4 f = __ldg(cr + i);
+        const float4 f = cr[i];
         cs[4 * i] = f.x;
         cs[4 * i + 1] = f.y;
         cs[4 * i + 2] = f.z;

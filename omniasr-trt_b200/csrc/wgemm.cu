@@ -221,7 +221,7 @@ OMNI_DEV void finish_tile(const GemmArgs& a, int tile, int row, const float (&ac
         const int m = m0 + j;
         const int64_t so = m < a.rows && part < 2 ? place[m].cs_off : -1;
         rot[j] = so >= 0;
-        cs[j] = rot[j] ? __ldg(reinterpret_cast<const float2*>(cs_base + so)) : make_float2(0.f, 0.f);
+        cs[j] = rot[j] ? *reinterpret_cast<const float2*>(cs_base + so) : make_float2(0.f, 0.f);
       }
 #pragma unroll
       for (int j = 0; j < HALF; ++j) {

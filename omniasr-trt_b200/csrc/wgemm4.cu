@@ -42,8 +42,7 @@ OMNI_DEV uint32_t pair_of(uint32_t w, int i, uint32_t mask) {
   return r;
 }
 
-// Tokens come from the kernel before: an ordinary load, which stays behind the wait for it. (A load through the read-only path
-// counts as independent of every write and may be moved ahead of the wait.)
+// Tokens come from the kernel before: an ordinary load, which stays behind the wait for it.
 OMNI_DEV uint4 token_words(const __nv_bfloat16* p) { return *reinterpret_cast<const uint4*>(p); }
 
 // A block of 128 columns of two weight rows (words u0, u1; scales f0, f1 per group) times NT tiles of 8 tokens; x(n, w): a lane's 8
