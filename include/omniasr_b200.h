@@ -222,8 +222,9 @@ int omniasr_decode_gemm(const void* x, int64_t x_stride, int rows, const void* w
  * SwiGLU's halves are not rounded before. `codes` holds 8 weight rows x 128 columns in 512 bytes, [ceil(weight rows / 8)][ceil(k /
  * 128)][8][4] words of 16 bytes (what lies past the weights: code 8): of a row's 128 columns word t of 4 holds, in its 32-bit word
  * w, columns 32 w + 8 t + 2 i in bits 4 i .. and 32 w + 8 t + 2 i + 1 in bits 16 + 4 i .., i < 4. `scales` is bf16 [ceil(weight rows /
- * 8)][ceil(k / group)][8]. x rows, codes and scales 16-byte aligned; no workspace. The weights must not be written by the kernel
- * launched just before on the same stream. No counterpart in the reference. */
+ * 8)][ceil(k / group)][8]. x rows, codes and scales 16-byte aligned; no workspace. The weights are read before the kernel
+ * waits for those before it on the stream: between what writes them and the call must come an operation of the stream that does not
+ * and is launched without programmatic serialization (no call of this library). No counterpart in the reference. */
 int omniasr_decode_gemm_int4(const void* x, int64_t x_stride, int rows, const void* codes, const void* scales, int n, int k,
                              int group, int mode, const void* residual, int64_t residual_stride, void* y, int64_t y_stride,
                              cudaStream_t stream);

@@ -522,7 +522,7 @@ class Int4Weights:
 def int4_weights(codes: torch.Tensor, scales: torch.Tensor, group: int = 128) -> Int4Weights:
     """Lays a 4-bit weight matrix out for :func:`decode_gemm_int4`, once, when a model is loaded: ``codes`` [n, k] (uint8, 0 to
     15), ``scales`` [n, ceil(k / group)] (bfloat16; groups of 32, 64 or 128 columns, k a multiple of 32); the weight is
-    ``scales * (codes - 8)``."""
+    ``scales * (codes - 8)``. The result may be used by the next call on the stream."""
     if codes.dim() != 2 or codes.dtype != torch.uint8:
         raise ValueError("int4_weights: codes must be uint8 [n, k]")
     n, k = codes.shape
@@ -537,8 +537,11 @@ def int4_weights(codes: torch.Tensor, scales: torch.Tensor, group: int = 128) ->
     c = c.permute(0, 2, 1, 4, 3, 6, 5).reshape(tiles, blocks, 512, 2)  # [.., row, lane, word, odd, column / 2]
     s = torch.zeros(tiles * 8, scales.size(1), dtype=torch.bfloat16, device=codes.device)
     s[:n] = scales
-    s = s.view(tiles, 8, -1).transpose(1, 2).contiguous()
-    return Int4Weights(c[..., 0] | c[..., 1] << 4, s, n, k, group)
+    w = Int4Weights(c[..., 0] | c[..., 1] << 4, s.view(tiles, 8, -1).transpose(1, 2).contiguous(), n, k, group)
+    # The products read weights before they wait for the launch before them. It is this one, which writes none and itself starts
+    # after those that do have ended.
+    torch.empty(1, dtype=torch.uint8, device=codes.device).fill_(0)
+    return w
 
 
 def int4_quantise(w: torch.Tensor, group: int = 128) -> Int4Weights:
@@ -562,7 +565,9 @@ def decode_gemm_int4(x: torch.Tensor, w: Int4Weights, mode: str = "store", resid
                      out: torch.Tensor | None = None) -> torch.Tensor:
     """:func:`decode_gemm` over 4-bit weights, at most 64 token rows (bf16): ``x @ W.t()`` ("store"), ``residual + x @ W.t()``
     ("residual"), or with W's rows [gate; inner] ``inner * silu(gate)`` ("swiglu"); products and sums in fp32, rounded once, at the
-    end (swiglu's halves are not rounded before). ``out`` may be the residual and shares memory with no input else. ``w`` must not be written by the kernel launched just before on the stream."""
+    end (swiglu's halves are not rounded before). ``out`` may be the residual and shares memory with no input else. ``w`` is read
+    before the kernel waits for those before it on the stream: whoever writes into ``w.codes`` or ``w.scales`` puts a launch or a copy
+    that does not, and is no call of this library, between that and the product (:func:`int4_weights` has)."""
     native, _, stream, _ = _context(x.device)
     code = GEMM_MODES.get(mode)
     if code is None:

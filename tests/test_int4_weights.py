@@ -1,0 +1,58 @@
+"""4-bit weights as they are made: what a product that reads them at once finds, and values that no code stands for."""
+
+import pytest
+import torch
+from torch.utils._python_dispatch import TorchDispatchMode
+
+from omniasr_b200 import kernels
+
+DEV = "cuda"
+
+
+class Launches(TorchDispatchMode):
+    """The memory that each operation's results lie in (views launch nothing)."""
+
+    def __init__(self):
+        super().__init__()
+        self.written = []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        out = func(*args, **(kwargs or {}))
+        if isinstance(out, torch.Tensor) and not func.is_view and "empty" not in str(func) and "_unsafe_view" not in str(func):
+            self.written.append(out.untyped_storage().data_ptr())
+        return out
+
+
+@pytest.mark.parametrize("n,k,group", [(8, 128, 128), (13, 160, 32), (64, 256, 64)])
+def test_the_last_launch_writes_no_weights(n, k, group):
+    """The products read weights before they wait for the launch before them, so that must not be one that writes them."""
+    codes = torch.randint(0, 16, (n, k), dtype=torch.uint8)
+    with Launches() as seen:
+        w = kernels.int4_weights(codes, torch.ones(n, -(-k // group), dtype=torch.bfloat16), group)
+    held = {w.codes.untyped_storage().data_ptr(), w.scales.untyped_storage().data_ptr()}
+    assert len(held & set(seen.written)) == 2 and seen.written[-1] not in held
+    with Launches() as seen:
+        w = kernels.int4_quantise(torch.randn(n, k), group)
+    assert seen.written[-1] not in {w.codes.untyped_storage().data_ptr(), w.scales.untyped_storage().data_ptr()}
+
+
+@pytest.mark.gpu
+def test_weights_made_just_before_in_a_graph():
+    """Weights laid out and used in one graph, replayed over other codes: every product is that of the codes of its replay."""
+    g = torch.Generator().manual_seed(0)
+    codes, scales = torch.zeros(512, 1024, dtype=torch.uint8, device=DEV), torch.ones(512, 8, dtype=torch.bfloat16, device=DEV)
+    x = torch.randint(-4, 5, (8, 1024), generator=g).bfloat16().to(DEV)
+    step = lambda: kernels.decode_gemm_int4(x, kernels.int4_weights(codes, scales))  # noqa: E731
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            y = step()
+    torch.cuda.current_stream().wait_stream(stream)
+    for _ in range(20):
+        codes.copy_(torch.randint(0, 16, codes.shape, generator=g, dtype=torch.uint8))
+        graph.replay()
+        want = (x.double() @ (codes.double() - 8).t()).bfloat16()  # (whole numbers: exact but for the one rounding)
+        assert torch.equal(y, want)
