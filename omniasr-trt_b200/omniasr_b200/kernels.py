@@ -522,7 +522,8 @@ class Int4Weights:
 def int4_weights(codes: torch.Tensor, scales: torch.Tensor, group: int = 128) -> Int4Weights:
     """Lays a 4-bit weight matrix out for :func:`decode_gemm_int4`, once, when a model is loaded: ``codes`` [n, k] (uint8, 0 to
     15), ``scales`` [n, ceil(k / group)] (bfloat16; groups of 32, 64 or 128 columns, k a multiple of 32); the weight is
-    ``scales * (codes - 8)``. The result may be used by the next call on the stream."""
+    ``scales * (codes - 8)``. The result may be used by the next call on the stream. Codes above 15 are refused (which waits for them;
+    during a graph capture, where that cannot be, their low four bits count)."""
     if codes.dim() != 2 or codes.dtype != torch.uint8:
         raise ValueError("int4_weights: codes must be uint8 [n, k]")
     n, k = codes.shape
@@ -530,6 +531,13 @@ def int4_weights(codes: torch.Tensor, scales: torch.Tensor, group: int = 128) ->
         raise ValueError(f"int4_weights: groups of {group} columns (32, 64 or 128) of {k} (a multiple of 32)")
     if scales.dtype != torch.bfloat16 or scales.shape != (n, -(-k // group)) or scales.device != codes.device:
         raise ValueError(f"int4_weights: scales must be bfloat16 [n, {-(-k // group)}] on the codes' device")
+    if n and not (codes.is_cuda and torch.cuda.is_current_stream_capturing()) and int(codes.max()) > 15:
+        raise ValueError(f"int4_weights: a code of {int(codes.max())} (0 to 15)")
+    return _int4_layout(codes, scales, group)
+
+
+def _int4_layout(codes: torch.Tensor, scales: torch.Tensor, group: int) -> Int4Weights:
+    n, k = codes.shape
     tiles, blocks = -(-n // 8), -(-k // 128)
     c = torch.full((tiles * 8, blocks * 128), 8, dtype=torch.uint8, device=codes.device)
     c[:n, :k] = codes & 15
@@ -546,7 +554,7 @@ def int4_weights(codes: torch.Tensor, scales: torch.Tensor, group: int = 128) ->
 
 def int4_quantise(w: torch.Tensor, group: int = 128) -> Int4Weights:
     """A weight matrix [n, k] in 4 bits: per group of columns s = -m / 8 rounded to bf16, m the weight of largest magnitude, and
-    codes w / s rounded to [-8, 7], plus 8. The rows of a swiglu product are [gate; inner]."""
+    codes w / s rounded to [-8, 7], plus 8. A group with an infinity or a NaN is NaN. The rows of a swiglu product are [gate; inner]."""
     if w.dim() != 2 or not w.is_floating_point() or group not in (32, 64, 128) or w.size(1) % 32 or w.size(1) == 0:
         raise ValueError("int4_quantise: w must be floating point [n, k], k a multiple of 32, groups of 32, 64 or 128 columns")
     n, k = w.shape
@@ -556,9 +564,10 @@ def int4_quantise(w: torch.Tensor, group: int = 128) -> Int4Weights:
     f = f.view(n, groups, group)
     lo, hi = f.amin(-1), f.amax(-1)
     scales = (torch.where(hi > -lo, hi, lo) * -0.125).to(torch.bfloat16)
+    scales = torch.where(torch.isfinite(lo) & torch.isfinite(hi), scales, torch.full_like(scales, float("nan")))
     s = scales.float()[..., None]
-    codes = torch.where(s == 0, torch.zeros_like(f), f / s).round().clamp(-8, 7).add(8).to(torch.uint8)
-    return int4_weights(codes.view(n, -1)[:, :k], scales, group)
+    codes = torch.where((s == 0) | s.isnan(), torch.zeros_like(f), f / s).round().clamp(-8, 7).add(8).to(torch.uint8)
+    return _int4_layout(codes.view(n, -1)[:, :k], scales, group)
 
 
 def decode_gemm_int4(x: torch.Tensor, w: Int4Weights, mode: str = "store", residual: torch.Tensor | None = None,

@@ -36,6 +36,32 @@ def test_the_last_launch_writes_no_weights(n, k, group):
     assert seen.written[-1] not in {w.codes.untyped_storage().data_ptr(), w.scales.untyped_storage().data_ptr()}
 
 
+def test_codes_that_are_none_are_refused():
+    codes, scales = torch.full((9, 64), 15, dtype=torch.uint8), torch.ones(9, 1, dtype=torch.bfloat16)
+    assert bool((kernels.int4_weights(codes, scales).values() == 7).all())
+    codes[8, 63] = 16
+    with pytest.raises(ValueError, match="code of 16"):
+        kernels.int4_weights(codes, scales)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param(DEV, marks=pytest.mark.gpu)])
+def test_groups_that_are_not_finite_are_nan(device):
+    """A group with an infinity, a NaN or a number past float32's is NaN, its codes those of zeros; the others are as without it."""
+    x = torch.randn(5, 128, generator=torch.Generator().manual_seed(0), dtype=torch.float64)
+    want = kernels.int4_quantise(x.to(device), 32)
+    bad = ((0, 3, float("nan")), (1, 40, float("inf")), (2, 70, float("-inf")), (3, 100, 1e300), (4, 127, float("inf")), (4, 126, float("-inf")))
+    hide = torch.zeros(5, 4, dtype=torch.bool)
+    for r, c, v in bad:
+        x[r, c] = v
+        hide[r, c // 32] = True
+    w = kernels.int4_quantise(x.to(device), 32)
+    wide = hide.repeat_interleave(32, 1)
+    got = w.values().cpu()
+    assert bool(got[wide].isnan().all()) and torch.equal(got[~wide], want.values().cpu()[~wide])
+    unit = kernels.Int4Weights(w.codes, torch.ones_like(w.scales), w.n, w.k, w.group).values().cpu()
+    assert bool((unit[wide] == 0).all())
+
+
 @pytest.mark.gpu
 def test_weights_made_just_before_in_a_graph():
     """Weights laid out and used in one graph, replayed over other codes: every product is that of the codes of its replay."""
