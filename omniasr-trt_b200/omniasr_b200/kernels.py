@@ -511,11 +511,11 @@ class Int4Weights:
 
     def values(self) -> torch.Tensor:
         """The matrix that the codes stand for (float32 [n, k], exact)."""
-        w = self.codes.view(-1, self.codes.size(1), 8, 4, 4, 4)  # [rows / 8, blocks, row, lane, word, byte]
+        w = self.codes.view(*self.codes.shape[:2], 8, 4, 4, 4)  # [rows / 8, blocks, row, lane, word, byte]
         c = torch.stack([w & 15, w >> 4], -1).flatten(-2)  # 8 codes: the even columns', the odd ones'
         c = c.view(*c.shape[:-1], 2, 4).transpose(-1, -2)  # [..., lane, word, column / 2, odd]
-        c = c.permute(0, 2, 1, 4, 3, 5, 6).reshape(8 * self.codes.size(0), -1)[: self.n, : self.k]
-        s = self.scales.transpose(1, 2).reshape(-1, self.scales.size(1))[: self.n].float()
+        c = c.permute(0, 2, 1, 4, 3, 5, 6).reshape(8 * self.codes.size(0), 128 * self.codes.size(1))[: self.n, : self.k]
+        s = self.scales.transpose(1, 2).reshape(8 * self.scales.size(0), self.scales.size(1))[: self.n].float()
         return (c.float() - 8) * s.repeat_interleave(self.group, 1)[:, : self.k]
 
 
@@ -545,7 +545,7 @@ def _int4_layout(codes: torch.Tensor, scales: torch.Tensor, group: int) -> Int4W
     c = c.permute(0, 2, 1, 4, 3, 6, 5).reshape(tiles, blocks, 512, 2)  # [.., row, lane, word, odd, column / 2]
     s = torch.zeros(tiles * 8, scales.size(1), dtype=torch.bfloat16, device=codes.device)
     s[:n] = scales
-    w = Int4Weights(c[..., 0] | c[..., 1] << 4, s.view(tiles, 8, -1).transpose(1, 2).contiguous(), n, k, group)
+    w = Int4Weights(c[..., 0] | c[..., 1] << 4, s.view(tiles, 8, scales.size(1)).transpose(1, 2).contiguous(), n, k, group)
     # The products read weights before they wait for the launch before them. It is this one, which writes none and itself starts
     # after those that do have ended.
     torch.empty(1, dtype=torch.uint8, device=codes.device).fill_(0)
@@ -567,7 +567,7 @@ def int4_quantise(w: torch.Tensor, group: int = 128) -> Int4Weights:
     scales = torch.where(torch.isfinite(lo) & torch.isfinite(hi), scales, torch.full_like(scales, float("nan")))
     s = scales.float()[..., None]
     codes = torch.where((s == 0) | s.isnan(), torch.zeros_like(f), f / s).round().clamp(-8, 7).add(8).to(torch.uint8)
-    return _int4_layout(codes.view(n, -1)[:, :k], scales, group)
+    return _int4_layout(codes.view(n, groups * group)[:, :k], scales, group)
 
 
 def decode_gemm_int4(x: torch.Tensor, w: Int4Weights, mode: str = "store", residual: torch.Tensor | None = None,

@@ -44,6 +44,13 @@ def test_codes_that_are_none_are_refused():
         kernels.int4_weights(codes, scales)
 
 
+def test_weights_without_rows():
+    w = kernels.int4_weights(torch.zeros(0, 64, dtype=torch.uint8), torch.ones(0, 2, dtype=torch.bfloat16), 32)
+    assert w.values().shape == (0, 64)
+    w = kernels.int4_quantise(torch.zeros(0, 160), 64)
+    assert w.values().shape == (0, 160) and w.codes.shape == (0, 2, 512) and w.scales.shape == (0, 3, 8)
+
+
 @pytest.mark.parametrize("device", ["cpu", pytest.param(DEV, marks=pytest.mark.gpu)])
 def test_groups_that_are_not_finite_are_nan(device):
     """A group with an infinity, a NaN or a number past float32's is NaN, its codes those of zeros; the others are as without it."""
