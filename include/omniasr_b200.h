@@ -343,6 +343,13 @@ int omniasr_paged_plan(const int64_t* rows, const int64_t* fresh, int requests, 
                        int64_t pages, int64_t* pos, int64_t* slots, int32_t* batch_table, int batch_width, int64_t* lengths,
                        int64_t* q_offsets, int64_t* k_offsets, uint8_t* taken, void* workspace, size_t workspace_bytes, int* status,
                        cudaStream_t stream);
+/* omniasr_paged_plan() with the positions of refused requests' tokens held below `positions` (at least 1): with a rope table of that many,
+ * the append of the step, which looks at a token's position whatever its slot, raises no status for a sequence that has run out of room. */
+int omniasr_paged_plan_within(const int64_t* rows, const int64_t* fresh, int requests, int64_t tokens, int page, int64_t* length,
+                              int64_t seqs, int32_t* table, int64_t table_stride, int table_width, int32_t* free, int64_t* free_count,
+                              int64_t pages, int64_t positions, int64_t* pos, int64_t* slots, int32_t* batch_table, int batch_width,
+                              int64_t* lengths, int64_t* q_offsets, int64_t* k_offsets, uint8_t* taken, void* workspace,
+                              size_t workspace_bytes, int* status, cudaStream_t stream);
 
 /* Sequence rows[i] keeps its first keep[i] positions; the pages past them go back onto the stack, the last request's first and each
  * request's last page first, so that a trim to the lengths before omniasr_paged_plan() of the same requests leaves the stack as it

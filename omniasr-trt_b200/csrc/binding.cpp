@@ -307,12 +307,13 @@ int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t
 
 py::object paged_plan(const at::Tensor& rows, const at::Tensor& fresh, int64_t tokens, int64_t page, const at::Tensor& length,
                       const at::Tensor& table, const at::Tensor& free, const at::Tensor& free_count, std::optional<int64_t> width,
-                      int64_t status, int64_t stream, const Opt& ws) {
+                      std::optional<int64_t> positions, int64_t status, int64_t stream, const Opt& ws) {
   const char* name = "paged_plan";
   const Tables t = tables_of(name, rows, fresh, page, length, table, free, free_count);
   const int64_t w = width ? *width : table.size(1);
   if (tokens < 0 || tokens > 0x7fffffff) refuse(name, std::to_string(tokens) + " tokens");
   if (w < 0 || w > table.size(1)) refuse(name, "a width of " + std::to_string(w) + " of a table of " + std::to_string(table.size(1)));
+  if (positions && *positions < 1) refuse(name, std::to_string(*positions) + " positions");
   if (!ws) return py::int_(OMNIASR_PLAN_WORKSPACE);
   const int64_t b = t.requests;
   const auto i64 = length.options();
@@ -321,12 +322,13 @@ py::object paged_plan(const at::Tensor& rows, const at::Tensor& fresh, int64_t t
   const at::Tensor &pos = parts[0], &slots = parts[1], &lengths = parts[2], &qo = parts[3], &ko = parts[4];
   at::Tensor out = at::empty({b, w}, table.options()), taken = at::empty({b}, i64.dtype(at::kBool));
   done("omniasr_paged_plan",
-       omniasr_paged_plan(t.rows.data_ptr<int64_t>(), t.want.data_ptr<int64_t>(), (int)b, tokens, (int)page, length.data_ptr<int64_t>(),
-                          length.size(0), table.data_ptr<int32_t>(), row_stride(table), (int)table.size(1), free.data_ptr<int32_t>(),
-                          free_count.data_ptr<int64_t>(), free.size(0), pos.data_ptr<int64_t>(), slots.data_ptr<int64_t>(),
-                          out.data_ptr<int32_t>(), (int)w, lengths.data_ptr<int64_t>(), qo.data_ptr<int64_t>(), ko.data_ptr<int64_t>(),
-                          reinterpret_cast<uint8_t*>(taken.data_ptr()), ws->data_ptr(), ws->numel(), status_of(status),
-                          stream_of(stream)));
+       omniasr_paged_plan_within(t.rows.data_ptr<int64_t>(), t.want.data_ptr<int64_t>(), (int)b, tokens, (int)page,
+                                 length.data_ptr<int64_t>(), length.size(0), table.data_ptr<int32_t>(), row_stride(table),
+                                 (int)table.size(1), free.data_ptr<int32_t>(), free_count.data_ptr<int64_t>(), free.size(0),
+                                 positions.value_or(INT64_MAX), pos.data_ptr<int64_t>(), slots.data_ptr<int64_t>(),
+                                 out.data_ptr<int32_t>(), (int)w, lengths.data_ptr<int64_t>(), qo.data_ptr<int64_t>(),
+                                 ko.data_ptr<int64_t>(), reinterpret_cast<uint8_t*>(taken.data_ptr()), ws->data_ptr(), ws->numel(),
+                                 status_of(status), stream_of(stream)));
   return py::make_tuple(pos, slots, out, lengths, qo, ko, taken);
 }
 

@@ -269,6 +269,16 @@ int omniasr_paged_plan(const int64_t* rows, const int64_t* fresh, int requests, 
                        int64_t pages, int64_t* pos, int64_t* slots, int32_t* batch_table, int batch_width, int64_t* lengths,
                        int64_t* q_offsets, int64_t* k_offsets, uint8_t* taken, void* workspace, size_t workspace_bytes, int* status,
                        cudaStream_t stream) {
+  return omniasr_paged_plan_within(rows, fresh, requests, tokens, page, length, seqs, table, table_stride, table_width, free, free_count,
+                                   pages, INT64_MAX, pos, slots, batch_table, batch_width, lengths, q_offsets, k_offsets, taken, workspace,
+                                   workspace_bytes, status, stream);
+}
+
+int omniasr_paged_plan_within(const int64_t* rows, const int64_t* fresh, int requests, int64_t tokens, int page, int64_t* length,
+                              int64_t seqs, int32_t* table, int64_t table_stride, int table_width, int32_t* free, int64_t* free_count,
+                              int64_t pages, int64_t positions, int64_t* pos, int64_t* slots, int32_t* batch_table, int batch_width,
+                              int64_t* lengths, int64_t* q_offsets, int64_t* k_offsets, uint8_t* taken, void* workspace,
+                              size_t workspace_bytes, int* status, cudaStream_t stream) {
   const char* name = "paged_plan";
   omni::PlanArgs a{};
   if (int e = plan_args(name, a, rows, fresh, requests, page, length, seqs, table, table_stride, table_width, free, free_count, pages,
@@ -279,7 +289,9 @@ int omniasr_paged_plan(const int64_t* rows, const int64_t* fresh, int requests, 
     return fail(OMNIASR_ERR_ARGUMENT, "%s: %d rows of %d pages of a table of %d", name, requests, batch_width, table_width);
   if (!q_offsets || !k_offsets || (tokens && (!pos || !slots)) || (requests && ((!batch_table && batch_width) || !lengths || !taken)))
     return fail(OMNIASR_ERR_ARGUMENT, "%s: null pointer", name);
+  if (positions < 1) return fail(OMNIASR_ERR_ARGUMENT, "%s: %lld positions", name, (long long)positions);
   a.tokens = (int)tokens;
+  a.last = (int)(positions - 1 < 0x7fffffff ? positions - 1 : 0x7fffffff);
   a.pos = pos;
   a.slots = slots;
   a.batch_table = batch_table;

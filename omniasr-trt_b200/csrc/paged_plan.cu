@@ -217,6 +217,8 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const PlanArgs a) {
         const int pi = p / page, held = pages(r.past);
         const int64_t id = pi < held ? a.s.table[r.row * a.s.table_stride + pi] : stack(r, pi - held);
         slot = id * page + (p - pi * page);
+      } else {
+        pos = min(p, a.last);
       }
     }
     a.pos[t] = pos;

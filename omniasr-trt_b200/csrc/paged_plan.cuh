@@ -29,6 +29,7 @@ struct PlanArgs {
   const int64_t* want;  // [requests] new tokens (plan), positions kept (trim)
   int requests;
   int tokens;             // entries of pos and slots
+  int last;               // refused requests' tokens get positions up to this
   int64_t* pos;           // [tokens]
   int64_t* slots;         // [tokens]
   int32_t* batch_table;   // [requests, batch_width]

@@ -69,6 +69,8 @@ SIGNATURES = {
                                      _i, _f, _i, _i, _p, _sz, _p, _p]),
     "omniasr_paged_plan": (_i, [_p, _p, _i, _i64, _i, _p, _i64, _p, _i64, _i, _p, _p, _i64, _p, _p, _p, _i, _p, _p, _p, _p, _p, _sz,
                                 _p, _p]),
+    "omniasr_paged_plan_within": (_i, [_p, _p, _i, _i64, _i, _p, _i64, _p, _i64, _i, _p, _p, _i64, _i64, _p, _p, _p, _i, _p, _p, _p, _p,
+                                       _p, _sz, _p, _p]),
     "omniasr_paged_trim": (_i, [_p, _p, _i, _i, _p, _i64, _p, _i64, _i, _p, _p, _i64, _p, _sz, _p, _p]),
     "omniasr_packed_attention_workspace": (_sz, [_i64, _i, _i, _i, _i]),
     "omniasr_packed_attention": (_i, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _i64, _i, _i, _i,

@@ -739,7 +739,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
 
 def paged_plan(rows: torch.Tensor, new: torch.Tensor, tokens: int, page: int, length: torch.Tensor, table: torch.Tensor,
-               free: torch.Tensor, free_count: torch.Tensor, width: int | None = None) -> tuple[torch.Tensor, ...]:
+               free: torch.Tensor, free_count: torch.Tensor, width: int | None = None,
+               positions: int | None = None) -> tuple[torch.Tensor, ...]:
     """A step's index tensors from its requests' lengths, all on the GPU: request i adds ``new[i]`` tokens to sequence ``rows[i]``
     (int64, at most 8192 requests, a sequence once). The state, updated in place: ``length`` [S] int64, ``table`` [S, W] int32
     (the sequences' page numbers), ``free`` [pages] int32 with ``free_count`` [1] int64, a stack whose first ``free_count``
@@ -748,13 +749,14 @@ def paged_plan(rows: torch.Tensor, new: torch.Tensor, tokens: int, page: int, le
     the last token 0 and -1), ``batch_table`` [B, width] and ``lengths`` [B] as :func:`paged_attention`, the offsets [B + 1] as
     :func:`packed_attention`. Requests are taken in order: ``taken`` [B] (bool) is False where the pages did not suffice (or
     ``width`` pages would not, default W): that request's slots are -1, its sequence unchanged and the results of its queries mean
-    nothing. Sequences out of range or named twice, negative numbers and tokens past ``tokens`` are refused the same way and
+    nothing. ``positions``: refused requests' tokens get positions below it (a rope table's size: the append looks at a token's
+    position whatever its slot). Sequences out of range or named twice, negative numbers and tokens past ``tokens`` are refused the same way and
     raise status bit 1."""
     native, status, stream, ws = _context(length.device)
-    out = native.paged_plan(rows, new, tokens, page, length, table, free, free_count, width, status, stream, ws)
+    out = native.paged_plan(rows, new, tokens, page, length, table, free, free_count, width, positions, status, stream, ws)
     if out.__class__ is int:
         ws = _attn_workspace(out, length.device, stream)
-        out = native.paged_plan(rows, new, tokens, page, length, table, free, free_count, width, status, stream, ws)
+        out = native.paged_plan(rows, new, tokens, page, length, table, free, free_count, width, positions, status, stream, ws)
     return out
 
 

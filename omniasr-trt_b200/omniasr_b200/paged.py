@@ -189,7 +189,9 @@ class DeviceTables:
             each, new, tokens = new, torch.full((b,), new, dtype=torch.int64, device=rows.device), b * new
         if tokens is None:
             raise ValueError("plan: new tokens per request on the GPU need their number (tokens)")
-        pos, slots, table, lengths, q_offsets, k_offsets, taken = kernels.paged_plan(rows, new, tokens, self.page, *self._state(), width=width)
+        # (A refused request may ask for positions past the tables; a rope table need not reach there.)
+        pos, slots, table, lengths, q_offsets, k_offsets, taken = kernels.paged_plan(rows, new, tokens, self.page, *self._state(), width=width,
+                                                                                     positions=max(1, self.width * self.page))
         return Batch(tokens, None if each is None else [each] * b, total, pos, slots, table, lengths, q_offsets,
                      k_offsets, False, taken)
 
