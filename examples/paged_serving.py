@@ -125,14 +125,16 @@ def serve_graph(model: Decoder, prompts: list[list[int]], steps: int, kind: torc
     stream = torch.cuda.Stream()
     stream.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(stream):
-        step()  # (eager once: what is set up at first use is)
-        out.append(current.tolist())
-        captured = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(captured, stream=stream):
-            step()
-        for _ in range(steps - 1):
-            captured.replay()
+        if steps > 0:
+            step()  # (eager once: what is set up at first use is)
             out.append(current.tolist())
+        if steps > 1:
+            captured = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(captured, stream=stream):
+                step()
+            for _ in range(steps - 1):
+                captured.replay()
+                out.append(current.tolist())
         tables.trim(rows, torch.zeros_like(rows))
     torch.cuda.current_stream().wait_stream(stream)
     assert int(tables.free_count) == tables.free.numel()
