@@ -137,7 +137,9 @@ def serve_graph(model: Decoder, prompts: list[list[int]], steps: int, kind: torc
                 out.append(current.tolist())
         tables.trim(rows, torch.zeros_like(rows))
     torch.cuda.current_stream().wait_stream(stream)
-    assert int(tables.free_count) == tables.free.numel()
+    free = cache.free_pages
+    cache.take_back(tables)
+    assert free == 0 and cache.free_pages == tables.free.numel()
     return [list(o) for o in zip(*out)]
 
 

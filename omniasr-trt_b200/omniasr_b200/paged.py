@@ -116,12 +116,24 @@ class PagedCache:
 
     def device_tables(self, seqs: int, width: int, pages: int | None = None) -> DeviceTables:
         """Tables on the GPU for ``seqs`` sequences of at most ``width`` pages, which take ``pages`` of the free pages (all of them
-        by default) over: this object's own sequences no longer get those."""
+        by default) over: this object's own sequences no longer get those until :meth:`take_back`."""
         count = len(self._free) if pages is None else pages
         if not 0 <= count <= len(self._free):
             raise ValueError(f"device_tables: {count} pages of {len(self._free)} free")
         taken = [self._free.pop() for _ in range(count)]
         return DeviceTables(seqs, width, self.page, taken[::-1], self.device)
+
+    def take_back(self, tables: DeviceTables) -> None:
+        """Takes the pages of :meth:`device_tables` back, once all of the tables' sequences are freed (``trim`` to 0). Waits for the
+        GPU. The tables have no pages from then on, in graphs that captured their steps too."""
+        pages = tables.free.tolist()
+        if int(tables.free_count) != len(pages):
+            raise ValueError(f"take_back: {len(pages) - int(tables.free_count)} of {len(pages)} pages are still in use")
+        mine = set(self._free).union(*self._pages.values())
+        if tables.page != self.page or len(set(pages)) != len(pages) or any(p in mine or not 0 <= p < self.k.size(1) for p in pages):
+            raise ValueError("take_back: tables of another cache, or taken back before")
+        tables.free_count.zero_()
+        self._free.extend(pages)
 
     def _layer(self, layer: int) -> tuple:
         scales = (None, None) if self.k_scale is None else (self.k_scale[layer], self.v_scale[layer])
