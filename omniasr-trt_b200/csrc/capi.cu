@@ -803,7 +803,6 @@ int omniasr_decode_gemm_int4(const void* x, int64_t x_stride, int rows, const vo
   a.rows = rows;
   a.n = n;
   a.k = k;
-  a.wrows = mode == omni::kGemmSwiglu ? 2 * n : n;
   a.blocks = (k + 127) / 128;
   a.groups = (k + group - 1) / group;
   a.group = group;

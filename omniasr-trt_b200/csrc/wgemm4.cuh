@@ -16,7 +16,6 @@ struct Gemm4Args {
   const uint4* codes;     // [ceil(weight rows / 8), blocks, 8, 4] 16-byte words
   const uint16_t* scales; // bf16 [ceil(weight rows / 8), groups, 8]
   int rows, n, k;         // token rows, outputs, reduction length
-  int wrows;              // weight rows: n, SwiGLU 2n
   int blocks, groups;     // ceil(k / 128), ceil(k / group)
   int group;              // 32, 64 or 128
   uint32_t mask;          // set by the launcher
