@@ -39,8 +39,9 @@ OMNI_DEV uint32_t int4_codes(const float* x, float s) {
 
 // The same codes of bf16 values, with inv = 1 / s (0 for s = 0; |s| at least kInt4Fast, so that it is a number). Quotients of two numbers
 // of 8 bits near n + 1/2 (n < 8) are n + 1/2 or at least 2^-10 away from it: the numerator 2 X 2^d - (2 n + 1) S of the difference is
-// a multiple of 1/2 and the denominator 2 S at most 510. So the product, 2^-20 off at most, is rounded to multiples of 2^-14 first (by
-// adding 768), which gives the ties back exactly and moves nothing across one.
+// a multiple of 1/2 and the denominator 2 S at most 510. So the product, 2^-18 off at most (the reciprocal by 2 units in the last
+// place, the product by half of one, of up to 8), is rounded to multiples of 2^-14 first (by adding 768), which gives the ties back exactly
+// and moves nothing across one.
 constexpr float kInt4Fast = 0x1p-100f;
 OMNI_DEV uint32_t int4_codes_bf16(const float* x, float inv) {
   uint32_t r = 0u;
