@@ -51,9 +51,10 @@ def want_of(q, kval, vval, vs, table, lens, scale, tokens, page):
     return out, bound
 
 
-def run(heads, kv, dim, page, lens, tokens, sizes, seed, low=(), rising=0.0, scale=None):
+def run(heads, kv, dim, page, lens, tokens, sizes, seed, low=(), rising=0.0, scale=None, wide=False):
     """`sizes(exponent [keys, groups], g)` sets the power of two of each position's groups of V in row order; the keys `low` get scores
-    far below the others'; `rising`: how much the scores grow over a row."""
+    far below the others'; `rising`: how much the scores grow over a row; `wide`: tables with room for so many keys that a unit takes
+    all the columns it can."""
     g = torch.Generator().manual_seed(seed)
     covered = [max(0, n + tokens - 1) for n in lens]
     table, pool = pu.table_for(covered, page, g, 2)
@@ -77,6 +78,8 @@ def run(heads, kv, dim, page, lens, tokens, sizes, seed, low=(), rising=0.0, sca
     q = (base.repeat_interleave(heads // kv, 0) + 0.3 * torch.randn(len(lens) * tokens, heads, dim, generator=g)).bfloat16()
     scale = dim**-0.5 if scale is None else scale
     want, bound = want_of(q, kval, vval, vs, table, lens, scale, tokens, page)
+    if wide:
+        table = torch.cat([table, torch.zeros(len(lens), 100_000 // page, dtype=torch.int32)], 1)
     got = kernels.paged_attention(dev(q), dev(k), dev(v), dev(table), torch.tensor(lens, device=DEV), scale, tokens=tokens,
                                   k_scale=dev(ks), v_scale=dev(vs)).double().cpu()
     assert bool(torch.isfinite(got).all()), "not finite"
@@ -160,3 +163,26 @@ def test_drafts_do_not_spoil_the_queries_before_them(dim):
         e[-2:] += 40
 
     run(8, 2, dim, 16, [5, 30, 64, 200], 4, sizes, dim)
+
+
+# heads, kv heads, tokens whose columns make 2, 3, 4 and 2 x 3 tiles of 8 (256 dims: 2 and 2 x 2)
+COLUMNS = [(32, 8, 4), (32, 8, 5), (16, 1, 2), (40, 1, 1), (7, 1, 2)]
+
+
+@pytest.mark.parametrize("page", [16, 12])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("heads,kv,tokens", COLUMNS)
+def test_units_of_several_tiles(heads, kv, tokens, dim, page):
+    """Tame values, groups and keys of every size, and scores that grow, with all of a unit's columns at once."""
+    lens = [0, 3, 33, 64, 300]
+    args = (heads, kv, dim, page, lens, tokens)
+    run(*args, lambda e, g: None, dim, wide=True)
+    run(*args, lambda e, g: e.add_(torch.randint(-12, 13, e.shape, generator=g)), dim + 1, wide=True)
+    run(*args, lambda e, g: e[5::50].add_(24), dim + 2, wide=True, rising=2.0)
+
+
+@pytest.mark.parametrize("heads,kv,dim,page,n,tokens", [(32, 8, 128, 64, 4000, 5), (16, 2, 64, 16, 4500, 3), (16, 1, 256, 32, 3000, 2), (40, 1, 128, 16, 4900, 2)])
+def test_long_rows_in_several_tiles(heads, kv, dim, page, n, tokens):
+    """Units that are cut between many CTAs, of several tiles of columns, with keys and groups of different sizes."""
+    run(heads, kv, dim, page, [n, n // 3], tokens, lambda e, g: e.add_(torch.randint(-6, 7, (len(e) // 64 + 1, e.size(1)), generator=g)
+                                                                      .repeat_interleave(64, 0)[: len(e)]), n, wide=True)
