@@ -296,7 +296,8 @@ int omniasr_paged_rope_kv(const void* qkv, int64_t qkv_stride, const float* cs, 
 
 /* omniasr_paged_rope_kv() of a model that norms its queries and keys: each q and k vector x (one head of one token) becomes
  * x * rsqrt(mean(x^2) + eps) * w before it is rotated, w being q_norm or k_norm [dim] of dtype (16-byte aligned), in fp32 with one
- * rounding, after the rotation. v is not normed. No counterpart in the reference. */
+ * rounding, after the rotation. v is not normed. Pairs (2 i, 2 i + 1) turn, as in omniasr_rope_kv(); a model that turns (i, i + dim / 2)
+ * permutes the rows of its q and k weights and its norms' weights alike. No counterpart in the reference. */
 int omniasr_paged_norm_rope_kv(const void* qkv, int64_t qkv_stride, const void* q_norm, const void* k_norm, float eps,
                                const float* cs, int64_t cs_positions, const int64_t* pos, const int64_t* slots, void* q_out,
                                void* k_pages, void* v_pages, void* k_scale, void* v_scale, int64_t pages, int page,

@@ -27,8 +27,8 @@
 // * All blocks of all units are cut evenly between the CTAs. A unit that is cut leaves parts in the workspace; the CTA that
 //   publishes last joins them in the order of the keys, so a call repeats its bits.
 //
-// Measured (graph of five calls, L2 flushed before): 48 rows of 61 to 4093 keys, 32 heads on 8 of 128, 48 us (e4m3 pages 64); 48 rows of
-// 4096 keys 74 us (e4m3 79); 32 rows of 1400 to 1600 keys, 8 heads of 512, 86 us (e4m3 79: eight warps an SM are too few there).
+// Measured (graph of five calls, L2 flushed before): 48 rows of 61 to 4093 keys, 32 heads on 8 of 128, 50 us (e4m3 pages 65); 48 rows of
+// 4096 keys 75 us (e4m3 79); 32 rows of 1400 to 1600 keys, 8 heads of 512, 88 us (e4m3 79: eight warps an SM are too few there).
 //
 // What a column does not see has weight zero: its score is masked before the exponential, and its group scales (which may be
 // NaN) are masked out of the products; keys past the row's last are not read.
@@ -1019,7 +1019,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<DIM, NT>::kCtas) int4_kernel(con
   copy_wait<0>();
 }
 
-// Tiles of 8 columns of a unit: as many as share the keys while the accumulators stay in registers.
+// Tiles of 8 columns of a unit, which share its reads of the keys and their operands. Two and more at head_dim 128, three and more at 64 and
+// two at 256 do not fit the registers and spill (40 to 900 bytes a thread): 16 rows of 5 drafts, 200 to 2000 keys, 32 heads on 8 of
+// 128, three tiles a unit, 51 us.
 int most_tiles(int dim) { return dim <= 128 ? 4 : dim == 256 ? 2 : 1; }
 
 // One tile per unit where a block per warp covers all tiles' keys all the same (the keys are then read by several units, out of L2):

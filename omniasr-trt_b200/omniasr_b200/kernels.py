@@ -704,7 +704,8 @@ def paged_norm_rope_kv(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Te
                        eps: float = 1e-6, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None) -> torch.Tensor:
     """:func:`paged_rope_kv` of a model that norms its queries and keys: each head's q and k vector x becomes
     ``x * rsqrt(mean(x ** 2) + eps) * w`` before the rotation, w being ``q_norm`` / ``k_norm`` [D] (qkv's dtype), in fp32 with one
-    rounding, after the rotation. v is not normed."""
+    rounding, after the rotation. v is not normed. Pairs (2 i, 2 i + 1) turn, as in :func:`rope_kv`; a model that turns
+    (i, i + D / 2) permutes the rows of its q and k weights and its norms' weights alike."""
     native, status, stream, _ = _context(qkv.device)
     return native.paged_norm_rope_kv(qkv, q_norm, k_norm, cs, pos, k_pages, v_pages, slots, heads, kv_heads, eps, k_scale, v_scale,
                                      status, stream)
