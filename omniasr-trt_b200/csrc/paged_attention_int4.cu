@@ -16,11 +16,12 @@
 // * O^T = V^T P^T in fp16: two keys' codes of a dim are the halves of a word after one byte permutation, and a code masked out of it
 //   is the subnormal c 2^-24 (16 c 2^-24 four bits up), exact; the offset is a second product, with constants. The scales go onto
 //   the probabilities in fp32, before these are rounded, once, to fp16 and turned by movmatrix. Two things keep them in fp16's range.
-//   A column's weights 2^(x - m) may grow to 2^13, then m is raised so that the largest is 2^8. And every group of 32 dims has a unit, a
-//   power of two that a warp's accumulators of the group count in, which the scales of a block lie between 2^-7 and 2^2 of; a block
+//   A column's weights 2^(x - m) may grow to 2^14, then m is raised so that the largest is 2^12. And every group of 32 dims has a unit, a
+//   power of two that a warp's accumulators of the group count in, which the scales of a block lie between 2^-11 and 2^2 of; a block
 //   whose scales do not moves the unit (and the accumulators with it), and one with scales too far apart for any unit is summed in
-//   fp32 on the CUDA cores. So a weight is rounded by 2^-11 of itself or, if that is more, by 2^-26 of the row's largest (half of fp16's
-//   smallest step, 2^-25, is 2^-33 of the largest weight in units of at most 2^7 times the key's own scale), whatever the scales are.
+//   fp32 on the CUDA cores (four to six times as long). So a weight is rounded by 2^-11 of itself or, if that is more, by 2^-26 of the
+//   row's largest (half of fp16's smallest step, 2^-25, is 2^-37 of the largest weight in units of at most 2^11 times the key's own
+//   scale), whatever the scales are.
 // * Warps are independent: each takes blocks of 16 or 32 keys of the CTA's share with a maximum, a sum and an accumulator of
 //   its own, and copies its next blocks asynchronously into a ring of its own; no barrier in the loop. At a unit's end the CTA's
 //   warps join through shared memory.
@@ -49,11 +50,13 @@ namespace paged4 {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr float kMost = 13.f, kGoal = 8.f;  // log2 of a weight: the most, and the largest when m is raised
-// Units: a block's scales have exponents from unit - kBelow to unit + kAbove, so that a product stays under 2^(kMost + kAbove + 1) = 2^15.
+constexpr float kMost = 14.f, kGoal = 12.f;  // log2 of a weight: the most, and the largest when m is raised
+// Units: a block's scales have exponents from unit - kBelow to unit + kAbove, so that a product is at most 2^kMost (4 - 2^-6) = 65,280
+// (a bf16 number under 4), which fp16 holds.
 // Units stay from kUnitLeast to kUnitMost (2^-unit and what the join multiplies by are fp32 numbers), and at most kFall below the highest
-// that the warp's unit had (an accumulator, under 2^50 with 2^31 keys, is scaled up by no more).
-constexpr int kAbove = 1, kBelow = 7, kUnitLeast = -100, kUnitMost = 110, kFall = 64;
+// that the warp's unit had (an accumulator, under 2^50 with 2^31 keys, is scaled up by no more). They start where groups whose largest
+// values are 2^-6 to 2^7 need no other (32 rows of 1400 to 1600 keys, 8 heads of 512, keys' sizes spread by a factor of 2: from 2^0 97 us, from 2^2 82).
+constexpr int kAbove = 1, kBelow = 11, kUnitFirst = 2, kUnitLeast = -100, kUnitMost = 110, kFall = 64;
 constexpr float kNone = -3e38f;  // a maximum before any score: below what a score can be, and a number, so that nothing needs a case for it
 // A unit's start and end (queries, the join of the warps), about 3 us of a CTA, counted as so many blocks in the shares.
 constexpr int kStart = 8;
@@ -433,9 +436,9 @@ struct Kernel {
   }
 
   OMNI_DEV void start_unit() {
-    highest = 0;
+    highest = kUnitFirst;
 #pragma unroll
-    for (int i = 0; i < kWordsS; ++i) down[i] = 0x3f803f80u;  // (2^0: values of 2^-4 to 2^5, or whatever set_units() makes it)
+    for (int i = 0; i < kWordsS; ++i) down[i] = (uint32_t)(127 - kUnitFirst) << 7 | (uint32_t)(127 - kUnitFirst) << 23;
     const float* factor = reinterpret_cast<const float*>(smem + C::kLim);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -783,7 +786,7 @@ struct Kernel {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       if (c0 + n * 8 >= p.cols) break;
-      constexpr float kHigh = 0x1p-13f;  // 2^-kMost; more only in a column whose scores are all -inf, where a unit's 2^110 would make it infinite
+      constexpr float kHigh = 0x1p-14f;  // 2^-kMost; more only in a column whose scores are all -inf, where a unit's 2^110 would make it infinite
       const float f[2] = {fminf(ml[warp * C::kCols + n * 8 + 2 * t].x, kHigh), fminf(ml[warp * C::kCols + n * 8 + 2 * t + 1].x, kHigh)};
       const float low[2] = {f[0] * 0x1p24f, f[1] * 0x1p24f}, high[2] = {f[0] * 0x1p20f, f[1] * 0x1p20f};  // (by the dim's nibble)
 #pragma unroll
@@ -1021,7 +1024,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<DIM, NT>::kCtas) int4_kernel(con
 
 // Tiles of 8 columns of a unit, which share its reads of the keys and their operands. Two and more at head_dim 128, three and more at 64 and
 // two at 256 do not fit the registers and spill (40 to 900 bytes a thread): 16 rows of 5 drafts, 200 to 2000 keys, 32 heads on 8 of
-// 128, three tiles a unit, 51 us.
+// 128, three tiles a unit, 52 us.
 int most_tiles(int dim) { return dim <= 128 ? 4 : dim == 256 ? 2 : 1; }
 
 // One tile per unit where a block per warp covers all tiles' keys all the same (the keys are then read by several units, out of L2):

@@ -2,11 +2,11 @@
 of keys, and as a whole; against float64.
 
 The bound of test_int4_cache_gpu.py, 2^-8 |o| + (2^-11 + 2^-10) A + 2^-11 B with A = sum p |v| / sum p and B = sum p |s| / sum p, and what
-fp16 loses below its normal numbers. A weight is 2^8 or more where it is a warp's largest, and a scale that fp16 sees is taken relative to a
-power of two that is at most 2^7 times it; so half a step of fp16's smallest numbers, 2^-25, is at most 2^-25 2^-8 2^7 = 2^-26 of the
-largest weight times the key's scale, and times a code of at most 8 2^-23 of it. Keys whose scales lie further apart than 2^9 within
-their 16 are summed in fp32, so a scale counts for at most 2^9 times the least (of those that are not 0) among its key's 16:
-2^-23 C with C = max p * sum min(|s|, 2^9 least) / sum p."""
+fp16 loses below its normal numbers. A weight is 2^12 or more where it is a warp's largest, and a scale that fp16 sees is taken relative to a
+power of two that is at most 2^11 times it; so half a step of fp16's smallest numbers, 2^-25, is at most 2^-25 2^-12 2^11 = 2^-26 of the
+largest weight times the key's scale, and times a code of at most 8 2^-23 of it. Keys whose scales lie further apart than 2^13 within
+their 16 are summed in fp32, so a scale counts for at most 2^13 times the least (of those that are not 0) among its key's 16:
+2^-23 C with C = max p * sum min(|s|, 2^13 least) / sum p."""
 
 import pytest
 import torch
@@ -35,7 +35,7 @@ def want_of(q, kval, vval, vs, table, lens, scale, tokens, page):
         pad = torch.full((-most % 16, kv, s.size(2)), float("inf"), dtype=torch.float64)
         least = torch.cat([torch.where(s == 0, float("inf"), s), pad]).unflatten(0, (-1, 16)).amin(1)
         least = torch.where(least.isinf(), 0.0, least).repeat_interleave(16, 0)[:most]
-        held = torch.minimum(s, 2.0**9 * least)
+        held = torch.minimum(s, 2.0**13 * least)
         for t in range(tokens):
             m = n + t
             if m <= 0:
@@ -93,7 +93,7 @@ SHAPES = [(4, 4, 64, 16, 1), (12, 2, 64, 32, 3), (16, 1, 64, 128, 2), (4, 4, 128
 LENS = [1, 15, 40, 130, 700]
 
 
-@pytest.mark.parametrize("by", [10, 20, 26, 30, 40])
+@pytest.mark.parametrize("by", [10, 14, 20, 26, 30, 40])
 @pytest.mark.parametrize("heads,kv,dim,page,tokens", SHAPES)
 def test_a_key_of_little_weight_with_large_values(heads, kv, dim, page, tokens, by):
     """Keys of every warp's first blocks whose values are 2^by times the others' and whose weights are next to nothing."""
