@@ -296,7 +296,7 @@ int omniasr_paged_rope_kv(const void* qkv, int64_t qkv_stride, const float* cs, 
 
 /* omniasr_paged_rope_kv() of a model that norms its queries and keys: each q and k vector x (one head of one token) becomes
  * x * rsqrt(mean(x^2) + eps) * w before it is rotated, w being q_norm or k_norm [dim] of dtype (16-byte aligned), in fp32 with one
- * rounding, after the rotation. v is not normed. Pairs (2 i, 2 i + 1) turn, as in omniasr_rope_kv(); a model that turns (i, i + dim / 2)
+ * rounding, after the rotation (|x| up to 2^59: squares past fp32 make the vector zeros). v is not normed. Pairs (2 i, 2 i + 1) turn, as in omniasr_rope_kv(); a model that turns (i, i + dim / 2)
  * permutes the rows of its q and k weights and its norms' weights alike. No counterpart in the reference. */
 int omniasr_paged_norm_rope_kv(const void* qkv, int64_t qkv_stride, const void* q_norm, const void* k_norm, float eps,
                                const float* cs, int64_t cs_positions, const int64_t* pos, const int64_t* slots, void* q_out,
